@@ -14,10 +14,12 @@ CSRC = os.path.join("neural_scaling_weather_b200", "ops", "csrc")
 
 SOURCES = [
     os.path.join(CSRC, "bindings.cpp"),
+    os.path.join(CSRC, "bindings_block.cpp"),
     os.path.join(CSRC, "elementwise.cu"),
     os.path.join(CSRC, "attention.cu"),
     os.path.join(CSRC, "attention_tc.cu"),
     os.path.join(CSRC, "gemm_tcgen05.cu"),
+    os.path.join(CSRC, "gated_mlp.cu"),
     os.path.join(CSRC, "noalloc_rmsnorm.cu"),
     os.path.join(CSRC, "rmsnorm_tma.cu"),
     os.path.join(CSRC, "sht.cu"),
@@ -45,6 +47,9 @@ setup(
             name="neural_scaling_weather_b200._C",
             sources=SOURCES,
             include_dirs=[os.path.join(HERE, CSRC)],
+            # the shared C++ runtime, also where the compiler would link its static one: message formatting
+            # goes through streams that libtorch shares, and two runtimes in one process crash there
+            extra_link_args=["-l:libstdc++.so.6"],
             extra_compile_args={"cxx": ["-O3", "-std=c++17"], "nvcc": NVCC_FLAGS},
         )
     ],
