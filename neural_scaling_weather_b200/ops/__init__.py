@@ -141,6 +141,35 @@ def mlp(x: torch.Tensor, w1: torch.Tensor, b1: torch.Tensor, w2: torch.Tensor, b
     return mlp_cuda(x, w1, b1, w2, b2, residual)
 
 
+GATED_ACTIVATIONS = ("silu", "gelu")
+
+
+def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down: torch.Tensor,
+              b_gate: Optional[torch.Tensor] = None, b_up: Optional[torch.Tensor] = None,
+              b_down: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+              activation: str = "silu") -> torch.Tensor:
+    """Gated feed-forward network ``(act(x Wg^T + bg) * (x Wu^T + bu)) Wd^T + bd + residual``.
+
+    ``x`` (..., K); ``w_gate`` and ``w_up`` (H, K), ``w_down`` (N, H); biases (H,), (H,), (N,) or None;
+    ``residual`` (..., N).  ``activation``: ``"silu"`` or ``"gelu"`` (exact).  Any sizes and strides; rows whose
+    strides are not multiples of 16 bytes cost one copy of the operand.  On CUDA both projections, the
+    activation and the product are one kernel; the backward's data gradients read the weights as they are
+    stored.  Calls without gradients of at most 64 rows take kernels that stream the weights once."""
+    if activation not in GATED_ACTIVATIONS:
+        raise ValueError(f"gated_mlp: activation {activation!r} is not one of {GATED_ACTIVATIONS}")
+    H, K = w_gate.shape
+    if x.shape[-1] != K or w_up.shape != w_gate.shape or w_down.shape[1:] != (H,):
+        raise ValueError(f"gated_mlp: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)} "
+                         f"and w_down {tuple(w_down.shape)} do not fit together")
+    if residual is not None and residual.shape != x.shape[:-1] + w_down.shape[:1]:
+        raise ValueError(f"gated_mlp: residual {tuple(residual.shape)} is not the output's shape")
+    if not _use_cuda(x):
+        return reference.gated_mlp(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, activation)
+    from .fused import gated_mlp_cuda
+
+    return gated_mlp_cuda(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, activation)
+
+
 def window_attention(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torch.Tensor,
                      num_heads: int, head_dim: int, geom: WindowGeometry, scale: float):
     """Shifted-window attention over (B, T, H, W, 3*nh*hd) -> (B, T, H, W, nh*hd)."""
@@ -204,6 +233,7 @@ __all__ = [
     "WindowGeometry",
     "compute_dtype",
     "extension_available",
+    "gated_mlp",
     "head_unpatchify",
     "linear",
     "mlp",

@@ -763,8 +763,11 @@ std::vector<Tensor> window_attn_bwd(Tensor qkv, Tensor qw, Tensor kw, Tensor out
 
 }  // namespace
 
+void bind_block(py::module& m);  // bindings_block.cpp
+
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "sm_100a kernels of neural_scaling_weather_b200";
+  bind_block(m);
   m.def("read_error_flag", &read_error_flag, py::arg("clear") = true);
   m.def("wgrad_supported", &wgrad_supported, py::arg("dy"), py::arg("x"));
   m.def("legendre_table", &legendre_table);

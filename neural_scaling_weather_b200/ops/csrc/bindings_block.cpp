@@ -1,0 +1,334 @@
+// PyTorch bindings of the transformer-block operators: the gated feed-forward network, the norms with gate
+// and skip connection, and gradient clipping.  Argument checks, outputs and workspaces (from PyTorch's
+// allocator, on the current stream) and the launches.
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/extension.h>
+
+#include "kernels.h"
+
+namespace {
+
+using torch::Tensor;
+using OptTensor = c10::optional<Tensor>;
+
+cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
+
+void check(cudaError_t e, const char* what) {
+  TORCH_CHECK(e == cudaSuccess, what, " failed: ", cudaGetErrorString(e));
+}
+
+int dt_code(const Tensor& t, const char* what) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return nsw::kBF16;
+    case at::kHalf: return nsw::kF16;
+    case at::kFloat: return nsw::kF32;
+    default: TORCH_CHECK(false, what, ": unsupported dtype ", t.scalar_type());
+  }
+  return -1;
+}
+
+int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
+
+// A [rows, cols] operand the TMA kernels can read: unit column stride, 16-byte aligned rows.
+struct Rows {
+  Tensor t;
+  int64_t ld;
+  void* ptr() const { return t.data_ptr(); }
+};
+bool rows_aligned(const Tensor& t) {
+  return t.stride(1) == 1 && (t.size(0) == 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1))) &&
+         (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
+}
+// t itself, or a copy with padded rows where t's strides or address do not allow 16-byte accesses
+Rows aligned_rows(const Tensor& t) {
+  if (rows_aligned(t)) return {t, t.size(0) == 1 ? round8(t.size(1)) : t.stride(0)};
+  const int64_t ld = round8(t.size(1));
+  auto c = torch::empty({t.size(0), ld}, t.options());
+  check(nsw::pad_copy(t.data_ptr(), t.stride(0), t.stride(1), c.data_ptr(), ld, t.size(0), t.size(1), stream()),
+        "pad_copy");
+  return {c.narrow(1, 0, t.size(1)), ld};
+}
+// contiguous [rows, cols] view or copy of a padded buffer
+Tensor packed(const Tensor& buf, int64_t cols) {
+  if (buf.size(1) == cols) return buf;
+  auto out = torch::empty({buf.size(0), cols}, buf.options());
+  check(nsw::pad_copy(buf.data_ptr(), buf.stride(0), 1, out.data_ptr(), cols, buf.size(0), cols, stream()),
+        "pad_copy");
+  return out;
+}
+
+const void* opt_ptr(const OptTensor& t) { return t && t->defined() ? t->data_ptr() : nullptr; }
+
+void check_matrix(const Tensor& t, int64_t rows, int64_t cols, const Tensor& like, const char* name) {
+  TORCH_CHECK(t.is_cuda() && t.device() == like.device(), "gated_mlp: ", name, " must be on the input's device");
+  TORCH_CHECK(t.scalar_type() == like.scalar_type(), "gated_mlp: ", name, " must have the compute dtype ",
+              like.scalar_type(), ", got ", t.scalar_type());
+  TORCH_CHECK(t.dim() == 2 && t.size(0) == rows && t.size(1) == cols, "gated_mlp: ", name, " must be [", rows, ", ",
+              cols, "], got ", t.sizes());
+}
+void check_bias(const OptTensor& b, int64_t n, const Tensor& like, int* dtype, const char* name) {
+  if (!b || !b->defined()) return;
+  TORCH_CHECK(b->is_cuda() && b->device() == like.device() && b->dim() == 1 && b->numel() == n && b->is_contiguous(),
+              "gated_mlp: ", name, " must be a contiguous CUDA vector of ", n, " elements");
+  const int d = dt_code(*b, name);
+  TORCH_CHECK(*dtype < 0 || *dtype == d, "gated_mlp: the gate's and the up projection's biases must share a dtype");
+  *dtype = d;
+}
+
+struct GatedShape {
+  int64_t M, K, H, N, Hp;
+};
+GatedShape gated_shape(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd) {
+  TORCH_CHECK(x.is_cuda() && x.dim() == 2, "gated_mlp: x must be a CUDA matrix");
+  TORCH_CHECK(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, "gated_mlp: bf16 or fp16, got ",
+              x.scalar_type());
+  GatedShape d{x.size(0), x.size(1), wg.size(0), wd.size(0), 0};
+  d.Hp = round8(d.H);
+  check_matrix(wg, d.H, d.K, x, "w_gate");
+  check_matrix(wu, d.H, d.K, x, "w_up");
+  check_matrix(wd, d.N, d.H, x, "w_down");
+  TORCH_CHECK(d.K > 0 && d.H > 0 && d.N > 0, "gated_mlp: empty weights");
+  TORCH_CHECK(d.M < (int64_t(1) << 31) - 256 && d.K < (int64_t(1) << 30) && d.H < (int64_t(1) << 30) &&
+                  d.N < (int64_t(1) << 30),
+              "gated_mlp: too many rows or features");
+  return d;
+}
+
+// y = (act(x wg^T + bg) * (x wu^T + bu)) wd^T + bd + residual.  With save, also what the backward reads:
+// returns {y} or {y, x (as read), g, u, h} (rows of g, u and h padded to a multiple of 8 elements).
+std::vector<Tensor> gated_mlp_fwd(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd,
+                                  const OptTensor& bg, const OptTensor& bu, const OptTensor& bd,
+                                  const OptTensor& residual, int64_t act, bool save) {
+  const GatedShape d = gated_shape(x, wg, wu, wd);
+  int bdt = -1, ddt = -1;
+  check_bias(bg, d.H, x, &bdt, "b_gate");
+  check_bias(bu, d.H, x, &bdt, "b_up");
+  check_bias(bd, d.N, x, &ddt, "b_down");
+  const bool has_res = residual && residual->defined();
+  if (has_res) check_matrix(*residual, d.M, d.N, x, "residual");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const auto opt = x.options();
+  if (d.M == 0) {
+    auto y = torch::empty({0, d.N}, opt), e = torch::empty({0, d.Hp}, opt);
+    if (!save) return {y};
+    return {y, x, e, e, e};
+  }
+  auto h = torch::empty({d.M, d.Hp}, opt);
+  nsw::GatedArgs up{}, down{};
+  up.mode = nsw::kGatedUp;
+  down.mode = nsw::kGatedDown;
+  up.dtype = down.dtype = dt_code(x, "x");
+  up.act = (int)act;
+  up.M = down.M = d.M;
+  up.N = d.H;
+  up.K = d.K;
+  up.bias0 = opt_ptr(bg);
+  up.bias1 = opt_ptr(bu);
+  up.bias_dtype = bdt;
+  up.out0 = h.data_ptr();
+  up.ldout = d.Hp;
+  down.N = d.N;
+  down.K = d.H;
+  down.a0 = h.data_ptr();
+  down.lda = d.Hp;
+  down.bias0 = opt_ptr(bd);
+  down.bias_dtype = ddt;
+  const auto unit = [](const Tensor& t) { return t.stride(1) == 1 || t.size(1) == 1; };
+  if (!save && d.M <= nsw::kGatedSkinnyTokens && unit(x) && unit(wg) && unit(wu) && unit(wd) &&
+      (!has_res || unit(*residual))) {
+    auto y = torch::empty({d.M, d.N}, opt);
+    up.a0 = x.data_ptr();
+    up.lda = x.stride(0);
+    up.b0 = wg.data_ptr();
+    up.ldb0 = wg.stride(0);
+    up.b1 = wu.data_ptr();
+    up.ldb1 = wu.stride(0);
+    check(nsw::gated_skinny(up, false, stream()), "gated_mlp up");
+    down.b0 = wd.data_ptr();
+    down.ldb0 = wd.stride(0);
+    down.in0 = has_res ? residual->data_ptr() : nullptr;
+    down.ldin = has_res ? residual->stride(0) : 0;
+    down.out0 = y.data_ptr();
+    down.ldout = d.N;
+    check(nsw::gated_skinny(down, true, stream()), "gated_mlp down");
+    return {y};
+  }
+  const Rows xa = aligned_rows(x), ga = aligned_rows(wg), ua = aligned_rows(wu), da = aligned_rows(wd);
+  Tensor g, u;
+  if (save) {
+    g = torch::empty({d.M, d.Hp}, opt);
+    u = torch::empty({d.M, d.Hp}, opt);
+    up.out1 = g.data_ptr();
+    up.out2 = u.data_ptr();
+    up.ldaux = d.Hp;
+  }
+  up.a0 = xa.ptr();
+  up.lda = xa.ld;
+  up.b0 = ga.ptr();
+  up.ldb0 = ga.ld;
+  up.b1 = ua.ptr();
+  up.ldb1 = ua.ld;
+  check(nsw::gated_product(up, stream()), "gated_mlp up");
+  auto y = torch::empty({d.M, round8(d.N)}, opt);
+  down.b0 = da.ptr();
+  down.ldb0 = da.ld;
+  Rows ra;
+  if (has_res) {
+    ra = aligned_rows(*residual);
+    down.in0 = ra.ptr();
+    down.ldin = ra.ld;
+  }
+  down.out0 = y.data_ptr();
+  down.ldout = round8(d.N);
+  check(nsw::gated_product(down, stream()), "gated_mlp down");
+  y = packed(y, d.N);
+  if (!save) return {y};
+  return {y, xa.t, g, u, h};
+}
+
+// Weight gradient of `segs` equal row segments (and the sums of dy's columns): fp32 into the given buffers
+// (added), or fresh tensors of `dtype`.  dy [T, segs * rows_pad], x [T, n].
+void weight_grad(const Rows& dy, const Rows& x, int segs, int64_t rows, int64_t rows_pad,
+                 std::vector<OptTensor> into, std::vector<OptTensor> bias_into, bool want_bias, at::ScalarType dtype,
+                 at::ScalarType bias_dtype, std::vector<Tensor>& dw, std::vector<Tensor>& db) {
+  const int64_t T = x.t.size(0), n = x.t.size(1);
+  const auto f32 = x.t.options().dtype(at::kFloat);
+  nsw::WgradArgs a{};
+  bool inplace = rows == rows_pad, bias_inplace = rows == rows_pad && want_bias;
+  for (int i = 0; i < segs; ++i) {
+    inplace = inplace && into[i].has_value();
+    bias_inplace = bias_inplace && bias_into[i].has_value();
+  }
+  std::vector<Tensor> w(segs), b(segs);
+  for (int i = 0; i < segs; ++i) {
+    w[i] = inplace ? *into[i] : torch::empty({rows_pad, n}, f32);
+    a.D[i] = w[i].data_ptr<float>();
+    if (want_bias) {
+      b[i] = bias_inplace ? *bias_into[i] : torch::empty({rows_pad}, f32);
+      a.db[i] = b[i].data_ptr<float>();
+    }
+  }
+  a.dy = dy.ptr();
+  a.ldy = dy.ld;
+  a.x = x.ptr();
+  a.ldx = x.ld;
+  a.T = T;
+  a.M = segs * rows_pad;
+  a.N = n;
+  a.ldd = n;
+  a.seg_rows = rows_pad;
+  a.accumulate = inplace;
+  a.db_accumulate = bias_inplace;
+  a.dtype = dt_code(x.t, "x");
+  const auto plan = nsw::wgrad_plan(a.M, a.N, a.T);
+  const int64_t wsn = nsw::wgrad_workspace_floats(a.M, a.N, plan);
+  Tensor ws;
+  if (wsn > 0) {
+    ws = torch::empty({wsn}, f32);
+    a.ws = ws.data_ptr<float>();
+  }
+  check(nsw::wgrad_tcgen05(a, plan, stream()), "gated_mlp weight gradient");
+  const auto finish = [&](bool done, const Tensor& t, const OptTensor& dst, at::ScalarType dt) {
+    if (done) return Tensor();
+    const Tensor v = t.narrow(0, 0, rows);
+    if (dst) {
+      dst->view_as(v).add_(v);
+      return Tensor();
+    }
+    return v.to(dt);
+  };
+  for (int i = 0; i < segs; ++i) {
+    dw.push_back(finish(inplace, w[i], into[i], dtype));
+    db.push_back(want_bias ? finish(bias_inplace, b[i], bias_into[i], bias_dtype) : Tensor());
+  }
+}
+
+// Gradients from dy and what the forward saved: {dx, dwg, dwu, dwd, dbg, dbu, dbd}.  An entry is undefined
+// where it was not asked for (need_dx, need_w, need_b) or was added into the given fp32 buffer.
+std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tensor& wg, const Tensor& wu,
+                                  const Tensor& wd, const Tensor& g, const Tensor& u, const Tensor& h, int64_t act,
+                                  bool need_dx, bool need_w, bool need_b, std::vector<OptTensor> dw_into,
+                                  std::vector<OptTensor> db_into, at::ScalarType wdt, at::ScalarType bdt) {
+  const GatedShape d = gated_shape(x, wg, wu, wd);
+  check_matrix(dy, d.M, d.N, x, "dy");
+  check_matrix(g, d.M, d.Hp, x, "g");
+  check_matrix(u, d.M, d.Hp, x, "u");
+  check_matrix(h, d.M, d.Hp, x, "h");
+  TORCH_CHECK(g.is_contiguous() && u.is_contiguous() && h.is_contiguous() && (d.M == 0 || rows_aligned(x)),
+              "gated_mlp backward: saved tensors must be as the forward returned them");
+  TORCH_CHECK(dw_into.size() == 3 && db_into.size() == 3, "gated_mlp backward: three weights and biases");
+  const c10::cuda::CUDAGuard guard(x.device());
+  const auto opt = x.options();
+  std::vector<Tensor> out(7);
+  if (d.M == 0) {
+    if (need_dx) out[0] = torch::empty({0, d.K}, opt);
+    const Tensor w[3] = {wg, wu, wd};
+    for (int i = 0; i < 3; ++i) {
+      if (need_w && !dw_into[i]) out[1 + i] = torch::zeros(w[i].sizes(), opt.dtype(wdt));
+      if (need_b && !db_into[i]) out[4 + i] = torch::zeros({w[i].size(0)}, opt.dtype(bdt));
+    }
+    return out;
+  }
+  const Rows dya = aligned_rows(dy);
+  const Rows xa{x, d.M == 1 ? round8(d.K) : x.stride(0)};
+  const Rows ga = aligned_rows(wg), ua = aligned_rows(wu), da = aligned_rows(wd);
+  auto dgu = torch::empty({d.M, 2 * d.Hp}, opt);
+  char* du = reinterpret_cast<char*>(dgu.data_ptr()) + 2 * d.Hp;
+  nsw::GatedArgs a{};
+  a.mode = nsw::kGatedDh;
+  a.dtype = dt_code(x, "x");
+  a.act = (int)act;
+  a.M = d.M;
+  a.N = d.H;
+  a.K = d.N;
+  a.a0 = dya.ptr();
+  a.lda = dya.ld;
+  a.b0 = da.ptr();
+  a.ldb0 = da.ld;
+  a.in0 = g.data_ptr();
+  a.in1 = u.data_ptr();
+  a.ldin = d.Hp;
+  a.out0 = dgu.data_ptr();
+  a.out1 = du;
+  a.ldout = a.ldaux = 2 * d.Hp;
+  check(nsw::gated_product(a, stream()), "gated_mlp dh");
+  if (need_dx) {
+    auto dx = torch::empty({d.M, round8(d.K)}, opt);
+    nsw::GatedArgs b{};
+    b.mode = nsw::kGatedDx;
+    b.dtype = a.dtype;
+    b.M = d.M;
+    b.N = d.K;
+    b.K = d.H;
+    b.a0 = dgu.data_ptr();
+    b.a1 = du;
+    b.lda = 2 * d.Hp;
+    b.b0 = ga.ptr();
+    b.ldb0 = ga.ld;
+    b.b1 = ua.ptr();
+    b.ldb1 = ua.ld;
+    b.out0 = dx.data_ptr();
+    b.ldout = round8(d.K);
+    check(nsw::gated_product(b, stream()), "gated_mlp dx");
+    out[0] = packed(dx, d.K);
+  }
+  if (need_w || need_b) {
+    std::vector<Tensor> dw, db;
+    weight_grad({dgu, 2 * d.Hp}, xa, 2, d.H, d.Hp, {dw_into[0], dw_into[1]}, {db_into[0], db_into[1]}, need_b, wdt,
+                bdt, dw, db);
+    weight_grad(dya, {h.narrow(1, 0, d.H), d.Hp}, 1, d.N, d.N, {dw_into[2]}, {db_into[2]}, need_b, wdt, bdt, dw, db);
+    for (int i = 0; i < 3; ++i) {
+      out[1 + i] = dw[i];
+      out[4 + i] = db[i];
+    }
+  }
+  return out;
+}
+
+}  // namespace
+
+void bind_block(py::module& m) {
+  m.def("gated_mlp_fwd", &gated_mlp_fwd);
+  m.def("gated_mlp_bwd", &gated_mlp_bwd);
+}

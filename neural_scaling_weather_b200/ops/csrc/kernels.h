@@ -167,6 +167,39 @@ int64_t wgrad_workspace_floats(int64_t M, int64_t N, const WgradPlan& plan);
 int wgrad_tcgen05_supported(const WgradArgs& a);
 cudaError_t wgrad_tcgen05(const WgradArgs& a, const WgradPlan& plan, cudaStream_t s);
 
+// ---- gated feed-forward network (gated_mlp.cu) -------------------------------------------------------
+// One product of the network with its epilogue.  A operands are [M, K] rows, 16-byte aligned; weights are
+// read as stored.  mode:
+//   kGatedUp    out0 = act(a0 b0^T + bias0) * (a0 b1^T + bias1); out1 / out2 (both or neither, ldaux): the
+//               two pre-activations; b0 / b1 [N, K]
+//   kGatedDown  out0 = a0 b0^T + bias0 + in0 (optional, ldin); b0 [N, K]
+//   kGatedDh    d = a0 b0 with b0 [K, N]; out0 = d * in1 * act'(in0), out1 = d * act(in0) (in: g, u, ldin;
+//               out0 in rows of ldout, out1 in rows of ldaux)
+//   kGatedDx    out0 = a0 b0 + a1 b1 with b0, b1 [K, N]
+enum GatedMode : int { kGatedUp = 0, kGatedDown = 1, kGatedDh = 2, kGatedDx = 3 };
+struct GatedArgs {
+  int mode, dtype, act;  // act: 0 SiLU, 1 GELU
+  int64_t M, N, K;
+  const void *a0, *a1;
+  int64_t lda;
+  const void *b0, *b1;
+  int64_t ldb0, ldb1;
+  const void *bias0, *bias1;  // [N] in bias_dtype, or null
+  int bias_dtype;
+  const void *in0, *in1;
+  int64_t ldin;
+  void *out0, *out1, *out2;
+  int64_t ldout, ldaux;
+};
+cudaError_t gated_product(const GatedArgs& a, cudaStream_t s);
+// kGatedUp (no out1 / out2) and kGatedDown for at most kGatedSkinnyTokens rows, any strides; dependent:
+// launched as a programmatic dependent of the kernel before it on the stream, which writes a0
+constexpr int kGatedSkinnyTokens = 64;
+cudaError_t gated_skinny(const GatedArgs& a, bool dependent, cudaStream_t s);
+// 16-bit strided copy into rows of ld elements (cols of them written)
+cudaError_t pad_copy(const void* src, int64_t s0, int64_t s1, void* dst, int64_t ld, int64_t rows, int64_t cols,
+                     cudaStream_t s);
+
 // Data-parallel reduction / sharded AdamW over peer memory (dp_fused.cu).  Every rank's buffers:
 // grad / data fp32 flat buffers, shadow 16-bit (or null), flags uint32 [kDpFlagBase + world * slots]
 // (flag word of (rank r, slot) at kDpFlagBase + r * slots + slot in every rank's array).

@@ -357,6 +357,71 @@ def mlp_cuda(x, w1, b1, w2, b2, residual=None):
     return _MLP.apply(x, residual, w1, b1, w2, b2)
 
 
+# ---------------------------------------------------------------------------- gated MLP
+_GATED_ACT = {"silu": 0, "gelu": 1}
+
+
+def _rows(t: torch.Tensor, n: int) -> torch.Tensor:
+    return t if t.dim() == 2 else t.reshape(-1, n)
+
+
+class _GatedMLP(torch.autograd.Function):
+    """The gated feed-forward network.  The forward keeps the input, both pre-activations and their
+    gated product h (16 bits); the backward is dg and du from one product with a fused epilogue, the input
+    gradient from one product of depth 2 H, and the weight gradients (with the biases' from the same
+    passes) in place into the optimizer's buffers where possible (``gradsink``)."""
+
+    @staticmethod
+    def forward(ctx, x, residual, act, wg, wu, wd, bg, bu, bd):
+        ext = require()
+        dt = _cdtype(x)
+        K, N = wg.shape[1], wd.shape[0]
+        W = [wcache.get(w, dt) for w in (wg, wu, wd)]
+        res = None if residual is None else _rows(residual, N).to(dt)
+        y, *saved = ext.gated_mlp_fwd(_rows(x, K).to(dt), *W, bg, bu, bd, res, act, True)
+        ctx.save_for_backward(*saved)
+        ctx.params, ctx.biases, ctx.W, ctx.act = (wg, wu, wd), (bg, bu, bd), W, act
+        ctx.x_shape, ctx.x_dtype = x.shape, x.dtype
+        ctx.res_dtype = None if residual is None else residual.dtype
+        if any(ctx.needs_input_grad[3:]):
+            gradsink.use([t for t in ctx.params + ctx.biases if t is not None])
+        return y.view(*x.shape[:-1], N)
+
+    @staticmethod
+    def backward(ctx, dy):
+        ext = require()
+        x2, g, u, h = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        need_w = any(need[3:])
+        has_b = [b is not None for b in ctx.biases]
+        tw = [gradsink.target(w) for w in ctx.params] if need_w else [None] * 3
+        tb = [gradsink.target(b) for b in ctx.biases] if need_w else [None] * 3
+        bdt = next((b.dtype for b in ctx.biases if b is not None), torch.float32)
+        dx, *grads = ext.gated_mlp_bwd(_rows(dy, dy.shape[-1]).to(x2.dtype), x2, *ctx.W, g, u, h, ctx.act, need[0],
+                                       need_w, need_w and any(has_b), tw, tb, ctx.params[0].dtype, bdt)
+        if need_w:
+            for p, t in zip(ctx.params + ctx.biases, tw + tb):
+                if p is not None:
+                    gradsink.done(p, t is not None)
+        out = [gr if p is not None and n else None
+               for p, n, gr in zip(ctx.params + ctx.biases, need[3:], grads)]
+        dx = dx.view(ctx.x_shape).to(ctx.x_dtype) if need[0] else None
+        return (dx, dy.to(ctx.res_dtype) if need[1] else None, None, *out)
+
+
+def gated_mlp_cuda(x, wg, wu, wd, bg, bu, bd, residual, activation):
+    act = _GATED_ACT[activation]
+    args = (x, wg, wu, wd, bg, bu, bd, residual)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+        return _GatedMLP.apply(x, residual, act, wg, wu, wd, bg, bu, bd)
+    dt = _cdtype(x)
+    N = wd.shape[0]
+    res = None if residual is None else _rows(residual, N).to(dt)
+    (y,) = require().gated_mlp_fwd(_rows(x, x.shape[-1]).to(dt), wcache.get(wg, dt), wcache.get(wu, dt),
+                                   wcache.get(wd, dt), bg, bu, bd, res, act, False)
+    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+
+
 # ---------------------------------------------------------------------------- attention
 def _geom_ints(B, T, H, W, nh, hd, g: WindowGeometry):
     return [B, T, H, W, nh, hd, g.window[0], g.window[1], g.shift[0], g.shift[1], int(g.mask),

@@ -41,6 +41,12 @@ def linear(x, weight, bias=None, residual=None, activation=None):
     return y
 
 
+def gated_mlp(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, residual=None, activation="silu"):
+    g = linear(x, w_gate, b_gate)
+    a = F.silu(g) if activation == "silu" else F.gelu(g)
+    return linear(a * linear(x, w_up, b_up), w_down, b_down, residual)
+
+
 def wrap_labels(geom: WindowGeometry, n_rows: int, device) -> torch.Tensor:
     """Region label (0/1) of each local (rolled) token row for the shift mask."""
     rows = torch.arange(n_rows, device=device) + geom.row_offset
