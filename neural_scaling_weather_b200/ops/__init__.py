@@ -170,6 +170,50 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     return gated_mlp_cuda(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, activation)
 
 
+def norm_gate_residual(y: torch.Tensor, skip: torch.Tensor, w_post: torch.Tensor,
+                       gate: Optional[torch.Tensor] = None, w_next: Optional[torch.Tensor] = None,
+                       skip_scale: float = 1.0, eps: Optional[float] = None):
+    """The norms around a residual connection in one pass: ``(s, n)`` with
+    ``s = skip_scale skip + gate * rms_norm(y, w_post)`` and ``n = rms_norm(s, w_next)``.
+
+    ``y`` (a branch's output) and ``skip`` (..., D); ``w_post``, ``w_next`` (D,); ``gate`` (D,), or one row for
+    each index of the first dimension (samples, D), or None for ones.  ``n`` is None without ``w_next`` (the
+    last branch of a network)."""
+    D = y.shape[-1]
+    if y.dim() < 2 or skip.shape != y.shape:
+        raise ValueError(f"norm_gate_residual: y {tuple(y.shape)} and skip {tuple(skip.shape)} must be of one shape "
+                         "(..., D)")
+    if w_post.shape != (D,) or (w_next is not None and w_next.shape != (D,)):
+        raise ValueError(f"norm_gate_residual: w_post and w_next must be ({D},)")
+    if gate is not None and gate.shape not in ((D,), (y.shape[0], D)):
+        raise ValueError(f"norm_gate_residual: gate {tuple(gate.shape)} is neither ({D},) nor ({y.shape[0]}, {D})")
+    if not _use_cuda(y):
+        return reference.norm_gate_residual(y, skip, w_post, gate, w_next, skip_scale, eps)
+    from .fused import norm_gate_residual_cuda
+
+    return norm_gate_residual_cuda(y, skip, w_post, gate, w_next, skip_scale, eps)
+
+
+def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float,
+                   out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
+    """Scale ``grads`` (separate tensors, fp32 / bf16 / fp16 mixed freely) to a global L2 norm of at most
+    ``max_norm``, in place or into ``out``; returns the norm before clipping (an fp32 scalar tensor; nothing
+    waits for the device).  The factor is the trainer's: ``max_norm / (norm + 1e-6)`` where the norm exceeds
+    ``max_norm``, else 1 (also for a NaN norm: non-finite gradients stay visible)."""
+    if isinstance(grads, torch.Tensor):
+        grads = [grads]
+    if len(grads) == 0:
+        raise ValueError("clip_grad_norm: no tensors")
+    if not max_norm > 0:
+        raise ValueError(f"clip_grad_norm: max_norm must be positive, got {max_norm}")
+    if out is not None and len(out) != len(grads):
+        raise ValueError(f"clip_grad_norm: {len(out)} outputs for {len(grads)} tensors")
+    if not _use_cuda(grads[0]):
+        with torch.no_grad():
+            return reference.clip_grad_norm(grads, max_norm, out)
+    return require_extension().clip_grads(grads, max_norm, [] if out is None else out)
+
+
 def window_attention(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torch.Tensor,
                      num_heads: int, head_dim: int, geom: WindowGeometry, scale: float):
     """Shifted-window attention over (B, T, H, W, 3*nh*hd) -> (B, T, H, W, nh*hd)."""
@@ -231,12 +275,14 @@ def weighted_se_per_channel(x: torch.Tensor, y: torch.Tensor, area_w: torch.Tens
 
 __all__ = [
     "WindowGeometry",
+    "clip_grad_norm",
     "compute_dtype",
     "extension_available",
     "gated_mlp",
     "head_unpatchify",
     "linear",
     "mlp",
+    "norm_gate_residual",
     "patch_embed",
     "reference",
     "rms_norm",

@@ -326,9 +326,139 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
   return out;
 }
 
+// ------------------------------------------------------------------------------ norms, gate, skip
+int sm_count(const Tensor& t) { return at::cuda::getDeviceProperties(t.get_device())->multiProcessorCount; }
+
+void check_vec(const OptTensor& v, int64_t rows, int64_t n, const Tensor& like, const char* name) {
+  if (!v || !v->defined()) return;
+  TORCH_CHECK(v->is_cuda() && v->device() == like.device() && v->scalar_type() == at::kFloat && v->is_contiguous() &&
+                  v->numel() == rows * n,
+              "norm_gate_residual: ", name, " must be a contiguous fp32 CUDA tensor of ", rows * n, " elements");
+}
+void check_like(const OptTensor& t, const Tensor& y, const char* name) {
+  if (!t || !t->defined()) return;
+  TORCH_CHECK(t->device() == y.device() && t->scalar_type() == y.scalar_type() && t->is_contiguous() &&
+                  t->sizes() == y.sizes(),
+              "norm_gate_residual: ", name, " must be a contiguous tensor like y");
+}
+nsw::NormGateArgs norm_args(const Tensor& y, const Tensor& skip, const Tensor& wp, const OptTensor& gate,
+                            const OptTensor& wn, double skip_scale, double eps) {
+  TORCH_CHECK(y.is_cuda() && y.dim() == 3 && y.is_contiguous(),
+              "norm_gate_residual: y must be a contiguous CUDA tensor [samples, rows, n]");
+  TORCH_CHECK(y.scalar_type() == at::kBFloat16 || y.scalar_type() == at::kHalf, "norm_gate_residual: bf16 or fp16");
+  const int64_t n = y.size(2);
+  TORCH_CHECK(n >= 1 && n <= nsw::kNormGateMaxWidth, "norm_gate_residual: width ", n, " is not in 1 .. ",
+              nsw::kNormGateMaxWidth);
+  TORCH_CHECK(y.size(0) <= 65535, "norm_gate_residual: at most 65535 samples");
+  check_like(skip, y, "skip");
+  check_vec(wp, 1, n, y, "w_post");
+  check_vec(gate, y.size(0), n, y, "gate");
+  check_vec(wn, 1, n, y, "w_next");
+  nsw::NormGateArgs a{};
+  a.y = y.data_ptr();
+  a.skip = skip.data_ptr();
+  a.wp = wp.data_ptr<float>();
+  a.gate = static_cast<const float*>(opt_ptr(gate));
+  a.wn = static_cast<const float*>(opt_ptr(wn));
+  a.gate_stride = n;
+  a.samples = y.size(0);
+  a.rows = y.size(1);
+  a.n = (int)n;
+  a.dtype = dt_code(y, "y");
+  a.skip_scale = (float)skip_scale;
+  a.eps = (float)eps;
+  return a;
+}
+
+// {stream, normed} (normed undefined without wn)
+std::vector<Tensor> norm_gate_fwd(const Tensor& y, const Tensor& skip, const Tensor& wp, const OptTensor& gate,
+                                  const OptTensor& wn, double skip_scale, double eps) {
+  auto a = norm_args(y, skip, wp, gate, wn, skip_scale, eps);
+  const c10::cuda::CUDAGuard guard(y.device());
+  auto stream_out = torch::empty_like(y);
+  Tensor normed;
+  a.stream = stream_out.data_ptr();
+  if (a.wn) {
+    normed = torch::empty_like(y);
+    a.normed = normed.data_ptr();
+  }
+  if (y.numel() > 0) check(nsw::norm_gate_fwd(a, sm_count(y), stream()), "norm_gate_fwd");
+  return {stream_out, normed};
+}
+
+// {dy, dskip, dwp, dgate, dwn}: gradients of the vectors in fp32
+std::vector<Tensor> norm_gate_bwd(const OptTensor& ds, const OptTensor& dn, const Tensor& y, const Tensor& skip,
+                                  const Tensor& wp, const OptTensor& gate, const OptTensor& wn, double skip_scale,
+                                  double eps) {
+  auto a = norm_args(y, skip, wp, gate, wn, skip_scale, eps);
+  check_like(ds, y, "ds");
+  check_like(dn, y, "dn");
+  const c10::cuda::CUDAGuard guard(y.device());
+  const auto f32 = y.options().dtype(at::kFloat);
+  auto dy = torch::empty_like(y), dskip = torch::empty_like(y);
+  const int64_t n = a.n;
+  if (y.numel() == 0)
+    return {dy, dskip, torch::zeros({n}, f32), a.gate ? torch::zeros({a.samples, n}, f32) : Tensor(),
+            a.wn ? torch::zeros({n}, f32) : Tensor()};
+  const int blocks = nsw::norm_gate_blocks(a.samples, a.rows, a.n, sm_count(y));
+  auto part = torch::empty({a.samples * blocks * 2 * n}, f32);
+  auto dwp = torch::empty({n}, f32);
+  Tensor dgate, dwn;
+  if (a.gate) dgate = torch::empty({a.samples, n}, f32);
+  if (a.wn) dwn = torch::empty({n}, f32);
+  a.ds = opt_ptr(ds);
+  a.dn = a.wn ? opt_ptr(dn) : nullptr;
+  a.dy = dy.data_ptr();
+  a.dskip = dskip.data_ptr();
+  a.part = part.data_ptr<float>();
+  a.dwp = dwp.data_ptr<float>();
+  a.dgate = a.gate ? dgate.data_ptr<float>() : nullptr;
+  a.dwn = a.wn ? dwn.data_ptr<float>() : nullptr;
+  check(nsw::norm_gate_bwd(a, blocks, stream()), "norm_gate_bwd");
+  return {dy, dskip, dwp, dgate, dwn};
+}
+
+// ------------------------------------------------------------------------------ clipping
+// out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)) (out empty: in place); returns the norm (fp32 scalar)
+Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, const std::vector<Tensor>& out) {
+  TORCH_CHECK(!grads.empty(), "clip_grad_norm: no tensors");
+  TORCH_CHECK(out.empty() || out.size() == grads.size(), "clip_grad_norm: ", out.size(), " outputs for ",
+              grads.size(), " tensors");
+  const auto dev = grads[0].device();
+  std::vector<nsw::ClipTensor> v;
+  v.reserve(grads.size());
+  int64_t total = 0;
+  for (size_t i = 0; i < grads.size(); ++i) {
+    const Tensor& g = grads[i];
+    const Tensor& o = out.empty() ? g : out[i];
+    TORCH_CHECK(g.is_cuda() && g.device() == dev && o.device() == dev, "clip_grad_norm: tensor ", i,
+                " is not on the first one's CUDA device");
+    TORCH_CHECK(g.is_contiguous() && o.is_contiguous() && o.numel() == g.numel() &&
+                    o.scalar_type() == g.scalar_type(),
+                "clip_grad_norm: tensor ", i, " and its output must be contiguous, of one size and dtype");
+    if (g.numel() == 0) continue;
+    v.push_back({g.data_ptr(), o.data_ptr(), g.numel(), dt_code(g, "clip_grad_norm")});
+    total += g.numel();
+  }
+  const c10::cuda::CUDAGuard guard(dev);
+  const auto f32 = grads[0].options().dtype(at::kFloat);
+  if (v.empty()) return torch::zeros({}, f32);
+  const int64_t tables = ((int64_t)v.size() + nsw::kClipTensors - 1) / nsw::kClipTensors;
+  const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>(8 * sm_count(grads[0]), total / 2048 + (int64_t)v.size()));
+  auto partial = torch::empty({tables * blocks + 1}, f32);
+  auto norm = torch::empty({}, f32);
+  check(nsw::clip_tensors(v.data(), (int)v.size(), (float)max_norm, partial.data_ptr<float>(), blocks,
+                          norm.data_ptr<float>(), stream()),
+        "clip_grad_norm");
+  return norm;
+}
+
 }  // namespace
 
 void bind_block(py::module& m) {
   m.def("gated_mlp_fwd", &gated_mlp_fwd);
   m.def("gated_mlp_bwd", &gated_mlp_bwd);
+  m.def("norm_gate_fwd", &norm_gate_fwd);
+  m.def("norm_gate_bwd", &norm_gate_bwd);
+  m.def("clip_grads", &clip_grads);
 }

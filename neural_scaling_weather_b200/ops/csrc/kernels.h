@@ -200,6 +200,37 @@ cudaError_t gated_skinny(const GatedArgs& a, bool dependent, cudaStream_t s);
 cudaError_t pad_copy(const void* src, int64_t s0, int64_t s1, void* dst, int64_t ld, int64_t rows, int64_t cols,
                      cudaStream_t s);
 
+// ---- norms with gate and skip connection (norm_gate.cu) ------------------------------------------------
+// Forward: stream = skip_scale skip + gate * rms(y) * wp; normed = rms(stream) * wn (normed and wn null: only
+// the stream).  Backward: dy, dskip from ds and / or dn (null: zero), and dwp, dgate (null: not wanted), dwn
+// (null with wn).  Tensors are contiguous [samples, rows, n]; gate of sample i at gate + i gate_stride (null:
+// ones).  part: samples * blocks * 2 * n floats.
+struct NormGateArgs {
+  const void *y, *skip, *ds, *dn;
+  void *stream, *normed, *dy, *dskip;
+  const float *wp, *gate, *wn;
+  int64_t gate_stride, samples, rows;
+  int n, dtype;
+  float skip_scale, eps;
+  float *part, *dwp, *dgate, *dwn;
+};
+constexpr int kNormGateMaxWidth = 16384;
+int norm_gate_blocks(int64_t samples, int64_t rows, int n, int sms);  // of the backward, per sample
+cudaError_t norm_gate_fwd(const NormGateArgs& a, int sms, cudaStream_t s);
+cudaError_t norm_gate_bwd(const NormGateArgs& a, int blocks, cudaStream_t s);
+
+// ---- gradient clipping over separate tensors (grad_clip.cu) --------------------------------------------
+struct ClipTensor {
+  const void* in;
+  void* out;
+  int64_t n;
+  int dtype;
+};
+constexpr int kClipTensors = 512;  // tensors in one launch's parameter table
+// partial: blocks floats per table of kClipTensors tensors; norm: one float
+cudaError_t clip_tensors(const ClipTensor* v, int count, float max_norm, float* partial, int blocks, float* norm,
+                         cudaStream_t s);
+
 // Data-parallel reduction / sharded AdamW over peer memory (dp_fused.cu).  Every rank's buffers:
 // grad / data fp32 flat buffers, shadow 16-bit (or null), flags uint32 [kDpFlagBase + world * slots]
 // (flag word of (rank r, slot) at kDpFlagBase + r * slots + slot in every rank's array).

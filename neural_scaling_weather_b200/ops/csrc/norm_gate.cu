@@ -1,0 +1,412 @@
+// The norms before and after a residual connection, fused with its gate and scale:
+//
+//   s = c skip + gate * (y / rms(y)) * wp,    n = (s / rms(s)) * wn,    rms(v) = sqrt(mean(v^2) + eps)
+//
+// and its gradient, in one pass over the rows: with yh = y / rms(y), sh = s / rms(s), a = dn * wn,
+//   d     = ds + (a - sh mean(a sh)) / rms(s)                    (gradient of s)
+//   dskip = c d,   b = d gate wp,   dy = (b - yh mean(b yh)) / rms(y)
+//   dwn = sum dn sh,   Q = sum over a sample's rows of d yh,   dgate = wp Q,   dwp = sum over samples gate Q
+//
+// Bound by memory: the forward reads two rows and writes two, the backward reads four (it recomputes s from
+// y and skip in fp32 instead of reading the rounded stream) and writes two; everything in between stays in
+// registers.  A row belongs to WPR warps, a lane holds NV groups of eight elements of it; the row sums go
+// through shuffles and, for WPR > 1, one shared-memory exchange behind a barrier of the row's warps.  The
+// sums over rows (Q, dwn) stay in the lanes' registers over all rows of a block, then are added over the
+// block's rows in a fixed order and written as one partial per block; a second kernel adds the partials in
+// block order, so results repeat bit for bit.  All arithmetic is fp32; only the outputs are rounded.
+#include <algorithm>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace nsw {
+namespace ng {
+
+struct Params {
+  const void *y, *skip, *ds, *dn;
+  void *stream, *normed, *dy, *dskip;
+  const float *wp, *gate, *wn;  // gate, wn: null for none
+  int64_t gate_stride;          // elements from one sample's gate to the next
+  float* part;                  // backward: [samples][blocks][2][n] partials (Q, dwn)
+  int64_t rows;                 // of one sample
+  int n;
+  float c, eps, inv_n;
+};
+
+// the elements a lane holds: contiguous groups of eight (16-byte accesses), or strided single elements
+// where the rows are not 16-byte aligned (coalesced 2-byte accesses)
+template <bool VEC, int GL>
+__device__ __forceinline__ int elem(int v, int j, int gl) {
+  return VEC ? (v * GL + gl) * 8 + j : (v * 8 + j) * GL + gl;
+}
+
+template <typename T, bool VEC, int GL>
+__device__ __forceinline__ uint4 load_row(const T* row, int v, int gl, int n) {
+  uint4 r = make_uint4(0, 0, 0, 0);
+  if (VEC) {
+    const int e = elem<VEC, GL>(v, 0, gl);
+    if (e < n) r = __ldcs(reinterpret_cast<const uint4*>(row + e));
+  } else {
+    uint32_t w[4] = {0, 0, 0, 0};
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(row);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int e = elem<VEC, GL>(v, j, gl);
+      if (e < n) w[j >> 1] |= (uint32_t)p[e] << (16 * (j & 1));
+    }
+    r = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  return r;
+}
+template <typename T, bool VEC, int GL>
+__device__ __forceinline__ void store_row(T* row, int v, int gl, int n, const float* f) {
+  if (VEC) {
+    const int e = elem<VEC, GL>(v, 0, gl);
+    if (e < n) __stcs(reinterpret_cast<uint4*>(row + e), pack8<T>(f));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int e = elem<VEC, GL>(v, j, gl);
+      if (e < n) row[e] = from_f<T>(f[j]);
+    }
+  }
+}
+// a parameter vector's elements of this lane (`none` past the end and for a null pointer)
+template <bool VEC, int GL>
+__device__ __forceinline__ void load_vec(const float* p, int v, int gl, int n, float none, float* f) {
+  if constexpr (VEC) {
+    const int e = elem<VEC, GL>(v, 0, gl);
+    float4 a = make_float4(none, none, none, none), b = a;
+    if (p && e < n) {
+      a = __ldg(reinterpret_cast<const float4*>(p + e));
+      b = __ldg(reinterpret_cast<const float4*>(p + e) + 1);
+    }
+    f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int e = elem<VEC, GL>(v, j, gl);
+      f[j] = p && e < n ? __ldg(p + e) : none;
+    }
+  }
+}
+
+// sums of K values over the row's warps (every lane gets them); `slot` names the exchange buffer: two
+// consecutive exchanges use different slots, so one barrier each is enough
+template <int WPR, int K>
+__device__ __forceinline__ void row_sum(float (&v)[K], float (*red)[WPR][2], int slot, int bar) {
+#pragma unroll
+  for (int k = 0; k < K; ++k) v[k] = warp_sum(v[k]);
+  if (WPR > 1) {
+    const int w = (threadIdx.x >> 5) % WPR;
+    if ((threadIdx.x & 31) == 0) {
+#pragma unroll
+      for (int k = 0; k < K; ++k) red[slot][w][k] = v[k];
+    }
+    asm volatile("bar.sync %0, %1;" ::"r"(bar), "r"(32 * WPR) : "memory");
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+      v[k] = red[slot][0][k];
+#pragma unroll
+      for (int i = 1; i < WPR; ++i) v[k] += red[slot][i][k];
+    }
+  }
+}
+
+template <typename T, bool VEC, int WPR, int NV>
+__global__ void __launch_bounds__(WPR > 8 ? 32 * WPR : 256) fwd_kernel(const Params p) {
+  constexpr int GL = 32 * WPR;
+  constexpr int RPB = WPR > 8 ? 1 : 8 / WPR;  // rows a block works on at a time
+  __shared__ float red[RPB][2][WPR][2];
+  const int rg = threadIdx.x / GL, gl = threadIdx.x % GL;
+  const int64_t sample = blockIdx.y;
+  const float* gate = p.gate ? p.gate + sample * p.gate_stride : nullptr;
+  for (int64_t r = (int64_t)blockIdx.x * RPB + rg; r < p.rows; r += (int64_t)gridDim.x * RPB) {
+    const int64_t at = (sample * p.rows + r) * p.n;
+    const T* y = reinterpret_cast<const T*>(p.y) + at;
+    const T* k = reinterpret_cast<const T*>(p.skip) + at;
+    uint4 yr[NV], kr[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) yr[v] = load_row<T, VEC, GL>(y, v, gl, p.n);
+#pragma unroll
+    for (int v = 0; v < NV; ++v) kr[v] = load_row<T, VEC, GL>(k, v, gl, p.n);
+    float q[1] = {0.f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float f[8];
+      unpack8<T>(yr[v], f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q[0] = fmaf(f[j], f[j], q[0]);
+    }
+    row_sum<WPR>(q, red[rg], 0, 1 + rg);
+    const float ry = rsqrtf(q[0] * p.inv_n + p.eps);
+    float s[NV][8];
+    q[0] = 0.f;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float f[8], w[8], g[8];
+      unpack8<T>(yr[v], f);
+      unpack8<T>(kr[v], s[v]);
+      load_vec<VEC, GL>(p.wp, v, gl, p.n, 0.f, w);
+      load_vec<VEC, GL>(gate, v, gl, p.n, 1.f, g);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        s[v][j] = fmaf(p.c, s[v][j], f[j] * ry * (w[j] * g[j]));
+        q[0] = fmaf(s[v][j], s[v][j], q[0]);
+      }
+      store_row<T, VEC, GL>(reinterpret_cast<T*>(p.stream) + at, v, gl, p.n, s[v]);
+    }
+    row_sum<WPR>(q, red[rg], 1, 1 + rg);  // also without a second norm: it separates two uses of slot 0
+    if (p.normed) {
+      const float rs = rsqrtf(q[0] * p.inv_n + p.eps);
+#pragma unroll
+      for (int v = 0; v < NV; ++v) {
+        float w[8];
+        load_vec<VEC, GL>(p.wn, v, gl, p.n, 0.f, w);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) s[v][j] *= rs * w[j];
+        store_row<T, VEC, GL>(reinterpret_cast<T*>(p.normed) + at, v, gl, p.n, s[v]);
+      }
+    }
+  }
+}
+
+template <typename T, bool VEC, int WPR, int NV>
+__global__ void __launch_bounds__(WPR > 8 ? 32 * WPR : 256) bwd_kernel(const Params p) {
+  constexpr int GL = 32 * WPR;
+  constexpr int RPB = WPR > 8 ? 1 : 8 / WPR;
+  extern __shared__ float sums[];  // [2][n]
+  __shared__ float red[RPB][3][WPR][2];
+  const int rg = threadIdx.x / GL, gl = threadIdx.x % GL;
+  const int64_t sample = blockIdx.y;
+  const float* gate = p.gate ? p.gate + sample * p.gate_stride : nullptr;
+  float gw[NV][8], wn[NV][8], aq[NV][8], aw[NV][8];
+#pragma unroll
+  for (int v = 0; v < NV; ++v) {
+    float g[8];
+    load_vec<VEC, GL>(p.wp, v, gl, p.n, 0.f, gw[v]);
+    load_vec<VEC, GL>(gate, v, gl, p.n, 1.f, g);
+    load_vec<VEC, GL>(p.wn, v, gl, p.n, 0.f, wn[v]);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      gw[v][j] *= g[j];
+      aq[v][j] = aw[v][j] = 0.f;
+    }
+  }
+  for (int64_t r = (int64_t)blockIdx.x * RPB + rg; r < p.rows; r += (int64_t)gridDim.x * RPB) {
+    const int64_t at = (sample * p.rows + r) * p.n;
+    uint4 yr[NV], kr[NV], dsr[NV], dnr[NV];
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      yr[v] = load_row<T, VEC, GL>(reinterpret_cast<const T*>(p.y) + at, v, gl, p.n);
+      kr[v] = load_row<T, VEC, GL>(reinterpret_cast<const T*>(p.skip) + at, v, gl, p.n);
+      dnr[v] = dsr[v] = make_uint4(0, 0, 0, 0);
+      if (p.dn) dnr[v] = load_row<T, VEC, GL>(reinterpret_cast<const T*>(p.dn) + at, v, gl, p.n);
+      if (p.ds) dsr[v] = load_row<T, VEC, GL>(reinterpret_cast<const T*>(p.ds) + at, v, gl, p.n);
+    }
+    float q1[1] = {0.f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float f[8];
+      unpack8<T>(yr[v], f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) q1[0] = fmaf(f[j], f[j], q1[0]);
+    }
+    row_sum<WPR>(q1, red[rg], 0, 1 + rg);
+    const float ry = rsqrtf(q1[0] * p.inv_n + p.eps);
+    float s[NV][8];
+    float q2[2] = {0.f, 0.f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float f[8], a[8];
+      unpack8<T>(yr[v], f);
+      unpack8<T>(kr[v], s[v]);
+      unpack8<T>(dnr[v], a);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        s[v][j] = fmaf(p.c, s[v][j], f[j] * ry * gw[v][j]);
+        q2[0] = fmaf(s[v][j], s[v][j], q2[0]);
+        q2[1] = fmaf(a[j] * wn[v][j], s[v][j], q2[1]);
+      }
+    }
+    row_sum<WPR>(q2, red[rg], 1, 1 + rg);
+    const float rs = rsqrtf(q2[0] * p.inv_n + p.eps);
+    const float m = q2[1] * rs * p.inv_n;  // mean(a sh)
+    float q3[1] = {0.f};
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float f[8], a[8], d[8], o[8];
+      unpack8<T>(yr[v], f);
+      unpack8<T>(dnr[v], a);
+      unpack8<T>(dsr[v], d);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float sh = s[v][j] * rs;
+        aw[v][j] = fmaf(a[j], sh, aw[v][j]);
+        d[j] = fmaf(rs, fmaf(-sh, m, a[j] * wn[v][j]), d[j]);
+        const float dq = d[j] * (f[j] * ry);
+        aq[v][j] += dq;
+        q3[0] = fmaf(gw[v][j], dq, q3[0]);
+        s[v][j] = d[j];
+        o[j] = p.c * d[j];
+      }
+      store_row<T, VEC, GL>(reinterpret_cast<T*>(p.dskip) + at, v, gl, p.n, o);
+    }
+    row_sum<WPR>(q3, red[rg], 2, 1 + rg);
+    const float my = q3[0] * p.inv_n;  // mean(b yh)
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      float f[8];
+      unpack8<T>(yr[v], f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f[j] = ry * fmaf(-f[j] * ry, my, s[v][j] * gw[v][j]);
+      store_row<T, VEC, GL>(reinterpret_cast<T*>(p.dy) + at, v, gl, p.n, f);
+    }
+  }
+  // the block's sums: its row groups in order
+  for (int g = 0; g < RPB; ++g) {
+    if (rg == g) {
+#pragma unroll
+      for (int v = 0; v < NV; ++v)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const int e = elem<VEC, GL>(v, j, gl);
+          if (e < p.n) {
+            sums[e] = g ? sums[e] + aq[v][j] : aq[v][j];
+            sums[p.n + e] = g ? sums[p.n + e] + aw[v][j] : aw[v][j];
+          }
+        }
+    }
+    __syncthreads();
+  }
+  float* part = p.part + (sample * gridDim.x + blockIdx.x) * 2 * p.n;
+  for (int e = threadIdx.x; e < 2 * p.n; e += blockDim.x) part[e] = sums[e];
+}
+
+// dwn[e] = sum of all partials; per sample Q[e]; dgate = wp Q (gate_stride > 0: of each sample, else summed
+// over the one "sample"), dwp = sum gate Q.  32 columns by 32 rows of threads a block; rows in a fixed order.
+__global__ void __launch_bounds__(1024) finish_kernel(const float* __restrict__ part, int64_t samples, int64_t blocks, int n,
+                              const float* __restrict__ wp, const float* __restrict__ gate, int64_t gate_stride,
+                              float* dwp, float* dgate, float* dwn) {
+  __shared__ float acc[2][32][33];
+  const int c = threadIdx.x & 31, t = threadIdx.x >> 5;
+  const int e = blockIdx.x * 32 + c;
+  float wn_sum = 0.f, wp_sum = 0.f;
+  for (int64_t s = 0; s < samples; ++s) {
+    float q = 0.f, w = 0.f;
+    if (e < n)
+      for (int64_t b = t; b < blocks; b += 32) {
+        const float* p = part + (s * blocks + b) * 2 * n;
+        q += p[e];
+        w += p[n + e];
+      }
+    acc[0][t][c] = q;
+    acc[1][t][c] = w;
+    __syncthreads();
+    if (t == 0 && e < n) {
+      q = acc[0][0][c];
+      w = acc[1][0][c];
+      for (int i = 1; i < 32; ++i) {
+        q += acc[0][i][c];
+        w += acc[1][i][c];
+      }
+      wn_sum += w;
+      wp_sum += q * (gate ? gate[s * gate_stride + e] : 1.f);
+      if (dgate) dgate[s * gate_stride + e] = q * wp[e];
+    }
+    __syncthreads();
+  }
+  if (t == 0 && e < n) {
+    dwp[e] = wp_sum;
+    if (dwn) dwn[e] = wn_sum;
+  }
+}
+
+template <typename T, bool VEC, int WPR, int NV>
+static cudaError_t launch(const Params& p, bool backward, dim3 grid, cudaStream_t s) {
+  const int threads = WPR > 8 ? 32 * WPR : 256;
+  if (!backward) {
+    fwd_kernel<T, VEC, WPR, NV><<<grid, threads, 0, s>>>(p);
+    return cudaGetLastError();
+  }
+  auto k = bwd_kernel<T, VEC, WPR, NV>;
+  const size_t smem = 2 * sizeof(float) * p.n;
+  if (smem > 48 * 1024) NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  k<<<grid, threads, smem, s>>>(p);
+  return cudaGetLastError();
+}
+
+// a lane holds at most 16 elements of a row (the backward's registers: two accumulators, two parameters and
+// four operands per element); rows longer than 512 take 2, 4, ... 32 warps
+template <typename T, bool VEC>
+static cudaError_t launch_width(const Params& p, bool backward, dim3 grid, cudaStream_t s) {
+  if (p.n <= 256) return launch<T, VEC, 1, 1>(p, backward, grid, s);
+  if (p.n <= 512) return launch<T, VEC, 1, 2>(p, backward, grid, s);
+  if (p.n <= 1024) return launch<T, VEC, 2, 2>(p, backward, grid, s);
+  if (p.n <= 2048) return launch<T, VEC, 4, 2>(p, backward, grid, s);
+  if (p.n <= 4096) return launch<T, VEC, 8, 2>(p, backward, grid, s);
+  if (p.n <= 8192) return launch<T, VEC, 16, 2>(p, backward, grid, s);
+  return launch<T, VEC, 32, 2>(p, backward, grid, s);
+}
+
+}  // namespace ng
+
+static int norm_gate_rows_per_block(int n) { return n <= 512 ? 8 : (n <= 1024 ? 4 : (n <= 2048 ? 2 : 1)); }
+
+int norm_gate_blocks(int64_t samples, int64_t rows, int n, int sms) {
+  // two blocks an SM over all samples, at least one a sample and none without rows
+  const int64_t rpb = norm_gate_rows_per_block(n);
+  const int64_t want = std::max<int64_t>(1, 2 * (int64_t)sms / samples);
+  return (int)std::max<int64_t>(1, std::min<int64_t>(want, (rows + rpb - 1) / rpb));
+}
+
+static cudaError_t norm_gate_launch(const NormGateArgs& a, bool backward, int blocks, cudaStream_t s) {
+  if (a.n < 1 || a.n > kNormGateMaxWidth || a.samples < 1 || a.samples > 65535 || a.rows < 1 ||
+      (a.dtype != kBF16 && a.dtype != kF16))
+    return cudaErrorInvalidValue;
+  ng::Params p;
+  p.y = a.y;
+  p.skip = a.skip;
+  p.ds = a.ds;
+  p.dn = a.dn;
+  p.stream = a.stream;
+  p.normed = a.normed;
+  p.dy = a.dy;
+  p.dskip = a.dskip;
+  p.wp = a.wp;
+  p.gate = a.gate;
+  p.wn = a.wn;
+  p.gate_stride = a.gate_stride;
+  p.part = a.part;
+  p.rows = a.rows;
+  p.n = a.n;
+  p.c = a.skip_scale;
+  p.eps = a.eps;
+  p.inv_n = 1.f / (float)a.n;
+  uintptr_t bits = 0;
+  for (const void* q : {a.y, a.skip, a.ds, a.dn, (const void*)a.stream, (const void*)a.normed, (const void*)a.dy,
+                        (const void*)a.dskip, (const void*)a.wp, (const void*)a.gate, (const void*)a.wn})
+    bits |= reinterpret_cast<uintptr_t>(q);
+  const bool vec = a.n % 8 == 0 && (bits & 15) == 0;
+  const dim3 grid((unsigned)blocks, (unsigned)a.samples, 1);
+  if (a.dtype == kBF16)
+    return vec ? ng::launch_width<__nv_bfloat16, true>(p, backward, grid, s)
+               : ng::launch_width<__nv_bfloat16, false>(p, backward, grid, s);
+  return vec ? ng::launch_width<__half, true>(p, backward, grid, s)
+             : ng::launch_width<__half, false>(p, backward, grid, s);
+}
+
+cudaError_t norm_gate_fwd(const NormGateArgs& a, int sms, cudaStream_t s) {
+  const int64_t rpb = norm_gate_rows_per_block(a.n);
+  const int64_t blocks = std::min<int64_t>((a.rows + rpb - 1) / rpb, std::max<int64_t>(1, 16 * (int64_t)sms / a.samples));
+  return norm_gate_launch(a, false, (int)blocks, s);
+}
+
+cudaError_t norm_gate_bwd(const NormGateArgs& a, int blocks, cudaStream_t s) {
+  NSW_CUDA_CHECK(norm_gate_launch(a, true, blocks, s));
+  ng::finish_kernel<<<(a.n + 31) / 32, 1024, 0, s>>>(a.part, a.samples, blocks, a.n, a.wp, a.gate, a.gate_stride,
+                                                     a.dwp, a.dgate, a.dwn);
+  return cudaGetLastError();
+}
+
+}  // namespace nsw

@@ -47,6 +47,26 @@ def gated_mlp(x, w_gate, w_up, w_down, b_gate=None, b_up=None, b_down=None, resi
     return linear(a * linear(x, w_up, b_up), w_down, b_down, residual)
 
 
+def norm_gate_residual(y, skip, w_post, gate=None, w_next=None, skip_scale=1.0, eps=None):
+    """``(s, rms_norm(s, w_next))`` with ``s = skip_scale skip + gate rms_norm(y, w_post)``, in fp32 until the
+    outputs are rounded; ``gate`` (D,) or (samples, D) over the leading dimension."""
+    branch = rms_norm(y.float(), w_post, eps)
+    if gate is not None:
+        g = gate.float()
+        branch = branch * (g if g.dim() == 1 else g.view(g.shape[0], *[1] * (y.dim() - 2), g.shape[1]))
+    s = skip_scale * skip.float() + branch
+    n = None if w_next is None else rms_norm(s, w_next, eps).to(y.dtype)
+    return s.to(y.dtype), n
+
+
+def clip_grad_norm(grads, max_norm, out=None):
+    norm = torch.stack([g.float().square().sum() for g in grads]).sum().sqrt()
+    coef = torch.where(norm > max_norm, max_norm / (norm + 1e-6), torch.ones_like(norm))
+    for g, o in zip(grads, grads if out is None else out):
+        o.copy_(g.float() * coef)
+    return norm
+
+
 def wrap_labels(geom: WindowGeometry, n_rows: int, device) -> torch.Tensor:
     """Region label (0/1) of each local (rolled) token row for the shift mask."""
     rows = torch.arange(n_rows, device=device) + geom.row_offset

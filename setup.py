@@ -20,6 +20,8 @@ SOURCES = [
     os.path.join(CSRC, "attention_tc.cu"),
     os.path.join(CSRC, "gemm_tcgen05.cu"),
     os.path.join(CSRC, "gated_mlp.cu"),
+    os.path.join(CSRC, "norm_gate.cu"),
+    os.path.join(CSRC, "grad_clip.cu"),
     os.path.join(CSRC, "noalloc_rmsnorm.cu"),
     os.path.join(CSRC, "rmsnorm_tma.cu"),
     os.path.join(CSRC, "sht.cu"),

@@ -1,8 +1,8 @@
 """The transformer-block operators (gated feed-forward network, norms with gate and skip connection, gradient
 clipping) against their definitions in 64 bits, on inputs that are exact in the tested type.
 
-Tolerances are relative 2-norms, counted in unit roundoffs u of the 16-bit type (2^-9 for bf16, 2^-11 for fp16:
-round to nearest): each value that a kernel rounds to 16 bits on the way to a result adds at most u to that
+Tolerances are relative 2-norms, counted in u, 2^-9 for bf16 and 2^-11 for fp16 (the largest relative rounding
+error is 2^-8 in bf16; over the spread of a tensor's significands its 2-norm is below 2^-9): each value that a kernel rounds to 16 bits on the way to a result adds at most u to that
 result's relative error (the operators are products and sums of such values; act' has relative condition at most
 about one).  fp32 sums of up to 2^16 terms stay far below u."""
 
@@ -221,3 +221,201 @@ def test_gated_refusals():
         ops.gated_mlp(x, *w, b[0], b[1].float())
     with pytest.raises(RuntimeError, match="device"):
         ops.gated_mlp(x, w[0].cpu(), w[1], w[2])
+
+
+# --------------------------------------------------------------------------- norms, gate, skip
+def norm_inputs(S, R, D, dtype, gate, nxt, seed=0):
+    g = torch.Generator(device=DEV).manual_seed(seed)
+
+    def randn(*s, std=1.0, mean=0.0, dt=dtype):
+        return (torch.randn(*s, generator=g, device=DEV) * std + mean).to(dt)
+
+    f = torch.float32
+    gt = {"none": None, "channel": randn(D, std=0.5, dt=f), "sample": randn(S, D, std=0.5, dt=f)}[gate]
+    return (randn(S, R, D), randn(S, R, D, std=2.0), randn(D, std=0.2, mean=1.0, dt=f), gt,
+            randn(D, std=0.2, mean=1.0, dt=f) if nxt else None, randn(S, R, D), randn(S, R, D))
+
+
+def norm_exact(y, skip, wp, gate, wn, c, ds=None, dn=None):
+    """Outputs, and with gradients their values and the sums of the absolute terms of the vectors' gradients."""
+    eps = torch.finfo(torch.float32).eps
+    y, skip, wp = (t.detach().double().requires_grad_() for t in (y, skip, wp))
+    S, D = y.shape[0], y.shape[-1]
+    shape = (S,) + (1,) * (y.dim() - 2) + (D,)
+    full = torch.ones(y.shape, dtype=torch.float64, device=DEV)
+    gf = full if gate is None else full * (gate.double() if gate.dim() == 1 else gate.double().view(shape))
+    gf = gf.requires_grad_()  # gradients of every row's gate; summed below
+    wf = wp.expand(y.shape).detach().requires_grad_()
+    rms = lambda v: v * torch.rsqrt(v.pow(2).mean(-1, keepdim=True) + eps)  # noqa: E731
+    s = c * skip + gf * rms(y) * wf
+    outs, grads, leaves = [s], [ds], [y, skip, wf, gf]
+    if wn is not None:
+        nf = wn.double().expand(y.shape).detach().requires_grad_()
+        outs.append(rms(s) * nf)
+        grads.append(dn)
+        leaves.append(nf)
+    res = [o.detach() for o in outs]
+    if ds is None and dn is None:
+        return res
+    use = [(o, g.double()) for o, g in zip(outs, grads) if g is not None]
+    got = torch.autograd.grad([o for o, _ in use], leaves, [g for _, g in use], allow_unused=True)
+    got = [torch.zeros_like(t) if g is None else g for g, t in zip(got, leaves)]
+    rows = tuple(range(y.dim() - 1))
+    per = rows if gate is None or gate.dim() == 1 else rows[1:]
+    vec = [(got[2].sum(rows), got[2].abs().sum(rows)), (got[3].sum(per), got[3].abs().sum(per))]
+    if wn is not None:
+        vec.append((got[4].sum(rows), got[4].abs().sum(rows)))
+    return res, got[:2], vec
+
+
+NORM_SIZES = [(1, 1, 1024), (1, 1, 1), (3, 5, 8), (2, 33, 96), (4, 257, 520), (3, 77, 1001), (2, 300, 1024),
+              (1, 64, 1544), (2, 21, 4096), (1, 9, 6001), (1, 3, 16384), (300, 2, 64)]
+
+
+@pytest.mark.parametrize("S,R,D", NORM_SIZES)
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("gate,nxt", [("sample", True), ("channel", True), ("none", False)])
+def test_norm_gate_residual(S, R, D, dtype, gate, nxt):
+    """Tensors: one rounding at the end (u) of fp32 arithmetic.  Vectors (fp32): sums over the rows, each row's
+    term a few fp32 roundings, relative to the sum of the terms' absolute values."""
+    y, skip, wp, gt, wn, ds, dn = norm_inputs(S, R, D, dtype, gate, nxt)
+    leaves = [t.requires_grad_() for t in (y, skip, wp, gt, wn) if t is not None]
+    s, n = ops.norm_gate_residual(y, skip, wp, gt, wn, skip_scale=0.7)
+    assert s.dtype == dtype and s.shape == y.shape and (n is None) == (not nxt)
+    outs = [s] if n is None else [s, n]
+    got = torch.autograd.grad(outs, leaves, [ds, dn][:len(outs)])
+    exact, tens, vec = norm_exact(y, skip, wp, gt, wn, 0.7, ds, dn if nxt else None)
+    with torch.no_grad():
+        s2, n2 = ops.norm_gate_residual(y, skip, wp, gt, wn, skip_scale=0.7)
+    assert torch.equal(s, s2) and (n is None or torch.equal(n, n2))
+    for i, (a, e) in enumerate(zip(outs + list(got[:2]), exact + list(tens))):
+        if y.numel() == 1 and i < len(outs):  # one number: the exact one, rounded
+            assert torch.equal(a, e.to(dtype))
+            continue
+        # rows of one element: the gradient through a norm is 0 up to eps, a difference of equal numbers
+        tol = (U[dtype] + 1e-5) * e.norm() + 1e-6 * ds.double().norm() * (D == 1)
+        assert (a.double() - e).norm() <= tol
+    if gt is None:
+        vec.pop(1)
+    for a, (e, terms) in zip(got[2:], vec):
+        assert a.dtype == torch.float32 and a.shape == e.shape
+        assert (a.double() - e).norm() <= 1e-5 * terms.norm()
+
+
+@pytest.mark.parametrize("only", ["stream", "normed"])
+def test_norm_gate_residual_with_one_output_used(only):
+    y, skip, wp, gt, wn, ds, dn = norm_inputs(2, 19, 200, torch.bfloat16, "sample", True)
+    leaves = [t.requires_grad_() for t in (y, skip, wp, gt, wn)]
+    s, n = ops.norm_gate_residual(y, skip, wp, gt, wn)
+    out, g = (s, ds) if only == "stream" else (n, dn)
+    got = torch.autograd.grad(out, leaves, g, allow_unused=True)
+    _, tens, vec = norm_exact(y, skip, wp, gt, wn, 1.0, ds if only == "stream" else None,
+                              dn if only == "normed" else None)
+    for a, e in zip(got[:2], tens):
+        assert rel(a, e) < U[torch.bfloat16] + 1e-5
+    for a, (e, terms) in zip(got[2:], vec):
+        assert (a.double() - e).norm() <= 1e-5 * terms.norm()
+
+
+def test_norm_gate_residual_strides_zeros_and_infinities():
+    """Non-contiguous inputs; a zero row and a zero branch stay finite; an infinite row spoils itself only."""
+    y, skip, wp, gt, wn, _, _ = norm_inputs(2, 12, 136, torch.bfloat16, "sample", True)
+    s, n = ops.norm_gate_residual(y, skip, wp, gt, wn)
+    wide = torch.zeros(2, 12, 300, device=DEV, dtype=y.dtype)
+    wide[..., 7:143] = y
+    s2, n2 = ops.norm_gate_residual(wide[..., 7:143], skip.transpose(0, 1).contiguous().transpose(0, 1),
+                                    wp.repeat_interleave(2)[::2], gt.t().contiguous().t(), wn)
+    assert torch.equal(s, s2) and torch.equal(n, n2)
+    y5 = y.view(2, 1, 3, 4, 136)
+    s5, n5 = ops.norm_gate_residual(y5, skip.view_as(y5), wp, gt, wn)
+    assert torch.equal(s5.view_as(s), s) and torch.equal(n5.view_as(n), n)
+    y[0, 3], skip[0, 3] = 0, 0
+    y[1, 4, 7] = float("inf")
+    s3, n3 = ops.norm_gate_residual(y, skip, wp, gt, wn)
+    assert not s3[0, 3].any() and not n3[0, 3].any()
+    keep = torch.ones(2, 12, dtype=torch.bool, device=DEV)
+    keep[0, 3] = keep[1, 4] = False
+    assert torch.equal(s3[keep], s[keep]) and torch.equal(n3[keep], n[keep])
+    assert torch.isnan(s3[1, 4]).any()
+
+
+def test_norm_gate_residual_empty_and_refusals():
+    y, skip, wp, gt, wn, _, _ = norm_inputs(2, 3, 64, torch.bfloat16, "sample", True)
+    e = y[:, :0].clone().requires_grad_()
+    w = wp.clone().requires_grad_()
+    s, n = ops.norm_gate_residual(e, skip[:, :0], w, gt, wn)
+    assert s.shape == (2, 0, 64) and n.shape == s.shape
+    de, dw = torch.autograd.grad([s, n], [e, w], [s.detach(), n.detach()])
+    assert de.shape == e.shape and not dw.any()
+    with pytest.raises(ValueError, match="skip"):
+        ops.norm_gate_residual(y, skip[:1], wp, gt, wn)
+    with pytest.raises(ValueError, match="w_post"):
+        ops.norm_gate_residual(y, skip, wp[:8], gt, wn)
+    with pytest.raises(ValueError, match="gate"):
+        ops.norm_gate_residual(y, skip, wp, gt[:1], wn)
+    with pytest.raises(RuntimeError, match="width"):
+        z = torch.zeros(1, 1, 16385, device=DEV, dtype=y.dtype)
+        ops.norm_gate_residual(z, z, torch.ones(16385, device=DEV))
+
+
+# --------------------------------------------------------------------------- gradient clipping
+def clip_inputs(shapes, dtypes, std=0.1):
+    g = torch.Generator(device=DEV).manual_seed(3)
+    return [(torch.randn(s, generator=g, device=DEV) * std).to(dtypes[i % len(dtypes)]) for i, s in enumerate(shapes)]
+
+
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
+
+
+@pytest.mark.parametrize("shapes,dtypes", [
+    ([(1,)], [F32]), ([(7,), (0,), (1, 1)], [BF16]), ([(64, 64), (64,), (8193,), (3, 5, 7)], [F32, BF16, F16]),
+    ([(8192,), (8191,), (16385,)], [F16]), ([(1000, 1001), (17,)], [F32]), ([(i % 13 + 1, 9) for i in range(1300)], [F32, BF16]),
+])
+@pytest.mark.parametrize("max_norm", [0.05, 1e9])
+def test_clip_grad_norm(shapes, dtypes, max_norm):
+    """The norm: fp32 sums of positive terms.  Scaled tensors: bit for bit the fp32 factor of that norm times
+    the element, rounded once."""
+    grads = clip_inputs(shapes, dtypes)
+    before = [g.clone() for g in grads]
+    exact = torch.cat([g.double().reshape(-1) for g in grads]).norm()
+    out = [torch.full_like(g, 9.0) for g in grads]
+    norm = ops.clip_grad_norm(grads, max_norm, out=out)
+    assert norm.dtype == torch.float32 and norm.shape == () and abs(norm.item() / exact.item() - 1) < 1e-5
+    assert all(torch.equal(g, b) for g, b in zip(grads, before))
+    norm2 = ops.clip_grad_norm(grads, max_norm)
+    assert torch.equal(norm, norm2)
+    limit = torch.full_like(norm, max_norm)  # tensor / tensor: one rounding (scalar / tensor has two)
+    coef = torch.where(norm > limit, limit / (norm + 1e-6), torch.ones_like(norm))
+    for g, b, o in zip(grads, before, out):
+        assert torch.equal(g, o) and torch.equal(o, (b.float() * coef).to(b.dtype))
+
+
+def test_clip_grad_norm_unaligned_and_non_finite():
+    flat = clip_inputs([(5000,)], [BF16])[0]
+    views = [flat[1:100], flat[101:4000], flat[4001:]]
+    exact = torch.cat([v.double() for v in views]).norm()
+    out = torch.zeros_like(flat)
+    norm = ops.clip_grad_norm(views, 0.5, out=[out[1:100], out[101:4000], out[4001:]])
+    assert abs(norm.item() / exact.item() - 1) < 1e-5
+    assert not out[0] and not out[100] and not out[4000]
+    assert rel(out[101:4000], views[1].double() * (0.5 / (exact + 1e-6))) < U[BF16] + 1e-5
+    g = [torch.ones(10, device=DEV), torch.tensor([float("nan")], device=DEV)]
+    assert torch.isnan(ops.clip_grad_norm(g, 1.0)) and torch.equal(g[0], torch.ones(10, device=DEV))
+    g = [torch.ones(10, device=DEV), torch.tensor([float("inf")], device=DEV)]
+    assert torch.isinf(ops.clip_grad_norm(g, 1.0)) and not g[0].any() and torch.isnan(g[1]).all()
+
+
+def test_clip_grad_norm_refusals():
+    g = [torch.ones(4, 4, device=DEV)]
+    with pytest.raises(ValueError, match="no tensors"):
+        ops.clip_grad_norm([], 1.0)
+    with pytest.raises(ValueError, match="positive"):
+        ops.clip_grad_norm(g, 0.0)
+    with pytest.raises(ValueError, match="outputs"):
+        ops.clip_grad_norm(g, 1.0, out=[])
+    with pytest.raises(RuntimeError, match="contiguous"):
+        ops.clip_grad_norm([torch.ones(4, 6, device=DEV).t()], 1.0)
+    with pytest.raises(RuntimeError, match="device"):
+        ops.clip_grad_norm([g[0], torch.ones(3)], 1.0)
+    with pytest.raises(RuntimeError, match="dtype"):
+        ops.clip_grad_norm([torch.ones(3, device=DEV, dtype=torch.float64)], 1.0)
