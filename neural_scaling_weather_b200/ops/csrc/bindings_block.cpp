@@ -200,15 +200,20 @@ void weight_grad(const Rows& dy, const Rows& x, int segs, int64_t rows, int64_t 
     inplace = inplace && into[i].has_value();
     bias_inplace = bias_inplace && bias_into[i].has_value();
   }
+  // 16-bit parameters: the kernel rounds the fp32 totals itself
+  bool out16 = dtype == x.t.scalar_type() && (!want_bias || bias_dtype == dtype);
+  for (int i = 0; i < segs; ++i) out16 = out16 && !into[i].has_value() && !(want_bias && bias_into[i].has_value());
+  const auto wopt = out16 ? x.t.options() : f32;
   std::vector<Tensor> w(segs), b(segs);
   for (int i = 0; i < segs; ++i) {
-    w[i] = inplace ? *into[i] : torch::empty({rows_pad, n}, f32);
-    a.D[i] = w[i].data_ptr<float>();
+    w[i] = inplace ? *into[i] : torch::empty({rows_pad, n}, wopt);
+    a.D[i] = static_cast<float*>(w[i].data_ptr());
     if (want_bias) {
-      b[i] = bias_inplace ? *bias_into[i] : torch::empty({rows_pad}, f32);
-      a.db[i] = b[i].data_ptr<float>();
+      b[i] = bias_inplace ? *bias_into[i] : torch::empty({rows_pad}, wopt);
+      a.db[i] = static_cast<float*>(b[i].data_ptr());
     }
   }
+  a.out16 = a.db16 = out16;
   a.dy = dy.ptr();
   a.ldy = dy.ld;
   a.x = x.ptr();
@@ -222,7 +227,7 @@ void weight_grad(const Rows& dy, const Rows& x, int segs, int64_t rows, int64_t 
   a.db_accumulate = bias_inplace;
   a.dtype = dt_code(x.t, "x");
   const auto plan = nsw::wgrad_plan(a.M, a.N, a.T);
-  const int64_t wsn = nsw::wgrad_workspace_floats(a.M, a.N, plan);
+  const int64_t wsn = nsw::wgrad_workspace_floats(a.M, a.N, plan, out16);
   Tensor ws;
   if (wsn > 0) {
     ws = torch::empty({wsn}, f32);
@@ -231,12 +236,12 @@ void weight_grad(const Rows& dy, const Rows& x, int segs, int64_t rows, int64_t 
   check(nsw::wgrad_tcgen05(a, plan, stream()), "gated_mlp weight gradient");
   const auto finish = [&](bool done, const Tensor& t, const OptTensor& dst, at::ScalarType dt) {
     if (done) return Tensor();
-    const Tensor v = t.narrow(0, 0, rows);
+    const Tensor v = rows == rows_pad ? t : t.narrow(0, 0, rows);
     if (dst) {
       dst->view_as(v).add_(v);
       return Tensor();
     }
-    return v.to(dt);
+    return v.scalar_type() == dt ? v : v.to(dt);
   };
   for (int i = 0; i < segs; ++i) {
     dw.push_back(finish(inplace, w[i], into[i], dtype));
@@ -326,6 +331,73 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
   return out;
 }
 
+// (..., n) as a matrix; a matrix y with x's leading dimensions
+Tensor flat(const Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
+OptTensor flat(const OptTensor& t) { return t ? OptTensor(flat(*t)) : OptTensor(); }
+Tensor unflat(const Tensor& y, const Tensor& x) {
+  if (x.dim() == 2) return y;
+  auto sizes = x.sizes().vec();
+  sizes.back() = y.size(1);
+  return y.view(sizes);
+}
+
+// The network of 16-bit parameters as one autograd node (fp32 master parameters, whose gradients may go
+// straight into the optimizer's buffers, go through the Python node on the same two functions).
+struct GatedNode : public torch::autograd::Function<GatedNode> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& wg, const Tensor& wu,
+                        const Tensor& wd, const OptTensor& bg, const OptTensor& bu, const OptTensor& bd,
+                        const OptTensor& residual, int64_t act) {
+    auto out = gated_mlp_fwd(flat(x), wg, wu, wd, bg, bu, bd, flat(residual), act, true);
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->save_for_backward({out[1], wg, wu, wd, out[2], out[3], out[4]});
+    ctx->saved_data["act"] = act;
+    int64_t given = 0, type = -1;  // which optional inputs there are, and the biases' type
+    int bit = 0;
+    for (const OptTensor* t : {&bg, &bu, &bd, &residual}) {
+      if (*t) {
+        given |= 1 << bit;
+        if (bit < 3 && type < 0) type = (int64_t)(*t)->scalar_type();
+      }
+      ++bit;
+    }
+    ctx->saved_data["given"] = given;
+    ctx->saved_data["bias"] = type;
+    return unflat(out[0], x);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grad) {
+    const auto v = ctx->get_saved_variables();
+    const int64_t bias = ctx->saved_data["bias"].toInt(), given = ctx->saved_data["given"].toInt();
+    bool need[8];
+    size_t edge = 4;  // graph edges exist for the inputs that were given, in order
+    for (int i = 0; i < 8; ++i)
+      need[i] = i < 4 ? ctx->needs_input_grad(i) : (((given >> (i - 4)) & 1) != 0 && ctx->needs_input_grad(edge++));
+    const bool need_w = need[1] || need[2] || need[3], need_b = need[4] || need[5] || need[6];
+    auto g = gated_mlp_bwd(flat(grad[0]), v[0], v[1], v[2], v[3], v[4], v[5], v[6], ctx->saved_data["act"].toInt(),
+                           need[0], need_w, need_b, std::vector<OptTensor>(3),
+                           std::vector<OptTensor>(3), v[1].scalar_type(),
+                           bias < 0 ? at::kFloat : (at::ScalarType)bias);
+    if (need[0]) g[0] = g[0].view(ctx->saved_data["shape"].toIntVector());
+    for (int i = 1; i < 7; ++i)
+      if (!need[i]) g[i] = Tensor();
+    g.push_back(need[7] ? grad[0] : Tensor());  // residual
+    g.push_back(Tensor());                      // act
+    return g;
+  }
+};
+
+// x (..., K) and residual (..., N) in the weights' 16-bit type
+Tensor gated_mlp(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, const OptTensor& bg,
+                 const OptTensor& bu, const OptTensor& bd, const OptTensor& residual, int64_t act) {
+  bool grad = false;
+  if (at::GradMode::is_enabled()) {
+    for (const Tensor* t : {&x, &wg, &wu, &wd}) grad = grad || t->requires_grad();
+    for (const OptTensor* t : {&bg, &bu, &bd, &residual}) grad = grad || (*t && (*t)->requires_grad());
+  }
+  if (grad) return GatedNode::apply(x, wg, wu, wd, bg, bu, bd, residual, act);
+  return unflat(gated_mlp_fwd(flat(x), wg, wu, wd, bg, bu, bd, flat(residual), act, false)[0], x);
+}
+
 // ------------------------------------------------------------------------------ norms, gate, skip
 int sm_count(const Tensor& t) { return at::cuda::getDeviceProperties(t.get_device())->multiProcessorCount; }
 
@@ -341,18 +413,20 @@ void check_like(const OptTensor& t, const Tensor& y, const char* name) {
                   t->sizes() == y.sizes(),
               "norm_gate_residual: ", name, " must be a contiguous tensor like y");
 }
+// y (..., n); gate (n,), or (samples, n) with y's rows in as many equal groups
 nsw::NormGateArgs norm_args(const Tensor& y, const Tensor& skip, const Tensor& wp, const OptTensor& gate,
                             const OptTensor& wn, double skip_scale, double eps) {
-  TORCH_CHECK(y.is_cuda() && y.dim() == 3 && y.is_contiguous(),
-              "norm_gate_residual: y must be a contiguous CUDA tensor [samples, rows, n]");
+  TORCH_CHECK(y.is_cuda() && y.dim() >= 1 && y.is_contiguous(), "norm_gate_residual: y must be a contiguous CUDA tensor");
   TORCH_CHECK(y.scalar_type() == at::kBFloat16 || y.scalar_type() == at::kHalf, "norm_gate_residual: bf16 or fp16");
-  const int64_t n = y.size(2);
+  const int64_t n = y.size(-1), samples = gate && gate->dim() == 2 ? gate->size(0) : 1;
   TORCH_CHECK(n >= 1 && n <= nsw::kNormGateMaxWidth, "norm_gate_residual: width ", n, " is not in 1 .. ",
               nsw::kNormGateMaxWidth);
-  TORCH_CHECK(y.size(0) <= 65535, "norm_gate_residual: at most 65535 samples");
+  TORCH_CHECK(samples <= 65535, "norm_gate_residual: at most 65535 samples");
+  TORCH_CHECK(y.numel() == 0 || (y.numel() / n) % samples == 0, "norm_gate_residual: ", y.numel() / n,
+              " rows are not whole groups of ", samples, " samples");
   check_like(skip, y, "skip");
   check_vec(wp, 1, n, y, "w_post");
-  check_vec(gate, y.size(0), n, y, "gate");
+  check_vec(gate, samples, n, y, "gate");
   check_vec(wn, 1, n, y, "w_next");
   nsw::NormGateArgs a{};
   a.y = y.data_ptr();
@@ -361,8 +435,8 @@ nsw::NormGateArgs norm_args(const Tensor& y, const Tensor& skip, const Tensor& w
   a.gate = static_cast<const float*>(opt_ptr(gate));
   a.wn = static_cast<const float*>(opt_ptr(wn));
   a.gate_stride = n;
-  a.samples = y.size(0);
-  a.rows = y.size(1);
+  a.samples = samples;
+  a.rows = y.numel() == 0 ? 0 : y.numel() / n / samples;
   a.n = (int)n;
   a.dtype = dt_code(y, "y");
   a.skip_scale = (float)skip_scale;
@@ -418,6 +492,60 @@ std::vector<Tensor> norm_gate_bwd(const OptTensor& ds, const OptTensor& dn, cons
   return {dy, dskip, dwp, dgate, dwn};
 }
 
+OptTensor packed_vec(const OptTensor& t) { return t ? OptTensor(t->contiguous()) : OptTensor(); }
+
+struct NormGateNode : public torch::autograd::Function<NormGateNode> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& y_in,
+                                                const Tensor& skip_in, const Tensor& wp, const OptTensor& gate,
+                                                const OptTensor& wn, double skip_scale, double eps) {
+    const Tensor y = y_in.contiguous(), skip = skip_in.contiguous(), wpc = wp.contiguous();
+    const OptTensor gc = packed_vec(gate), wnc = packed_vec(wn);
+    auto out = norm_gate_fwd(y, skip, wpc, gc, wnc, skip_scale, eps);
+    if (!out[1].defined()) out.pop_back();
+    ctx->save_for_backward({y, skip, wpc, gc ? *gc : Tensor(), wnc ? *wnc : Tensor()});
+    ctx->saved_data["c"] = skip_scale;
+    ctx->saved_data["eps"] = eps;
+    ctx->saved_data["gate"] = gate ? gate->dim() : (int64_t)0;
+    ctx->saved_data["next"] = wn.has_value();
+    ctx->set_materialize_grads(false);
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grad) {
+    const auto v = ctx->get_saved_variables();
+    const auto o = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    const auto c = [&](size_t i) {
+      return i < grad.size() && grad[i].defined() ? OptTensor(grad[i].contiguous()) : OptTensor();
+    };
+    auto g = norm_gate_bwd(c(0), c(1), v[0], v[1], v[2], o(v[3]), o(v[4]), ctx->saved_data["c"].toDouble(),
+                           ctx->saved_data["eps"].toDouble());
+    const int64_t gate = ctx->saved_data["gate"].toInt();
+    if (gate == 1) g[3] = g[3].view({-1});
+    size_t edge = 0;  // graph edges exist for the inputs that were given, in order
+    for (int i = 0; i < 5; ++i) {
+      const bool given = i < 3 || (i == 3 ? gate > 0 : ctx->saved_data["next"].toBool());
+      if (!given || !ctx->needs_input_grad(edge++)) g[i] = Tensor();
+    }
+    g.resize(7);
+    return g;
+  }
+};
+
+// y, skip (..., D) of one 16-bit type; fp32 vectors
+std::vector<Tensor> norm_gate(const Tensor& y, const Tensor& skip, const Tensor& wp, const OptTensor& gate,
+                              const OptTensor& wn, double skip_scale, double eps) {
+  bool grad = false;
+  if (at::GradMode::is_enabled()) {
+    for (const Tensor* t : {&y, &skip, &wp}) grad = grad || t->requires_grad();
+    for (const OptTensor* t : {&gate, &wn}) grad = grad || (*t && (*t)->requires_grad());
+  }
+  auto out = grad ? NormGateNode::apply(y, skip, wp, gate, wn, skip_scale, eps)
+                  : norm_gate_fwd(y.contiguous(), skip.contiguous(), wp.contiguous(), packed_vec(gate),
+                                  packed_vec(wn), skip_scale, eps);
+  out.resize(2);
+  return out;
+}
+
 // ------------------------------------------------------------------------------ clipping
 // out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)) (out empty: in place); returns the norm (fp32 scalar)
 Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, const std::vector<Tensor>& out) {
@@ -458,7 +586,7 @@ Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, const std::
 void bind_block(py::module& m) {
   m.def("gated_mlp_fwd", &gated_mlp_fwd);
   m.def("gated_mlp_bwd", &gated_mlp_bwd);
-  m.def("norm_gate_fwd", &norm_gate_fwd);
-  m.def("norm_gate_bwd", &norm_gate_bwd);
+  m.def("gated_mlp", &gated_mlp);
+  m.def("norm_gate", &norm_gate);
   m.def("clip_grads", &clip_grads);
 }

@@ -428,8 +428,8 @@ template <typename T, int MODE>
 static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
   const size_t smem = sizeof(SmemG<T>) + 1024;
   auto k = gated_kernel<T, MODE>;
-  // before the tensor maps: a runtime call that makes the device's context current on this thread (an
-  // autograd thread may not have one yet, and the encoder needs it)
+  // on each call: the attribute belongs to the current device, and a runtime call has to make that device's
+  // context current on this thread (an autograd thread may not have one yet) before the maps are encoded
   NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   GatedParams p;
   memset(&p, 0, sizeof(p));

@@ -152,7 +152,8 @@ struct WgradArgs {
   float* db[4];  // db[0] null: no bias gradient
   int db_accumulate;
   int dtype;
-  float* ws;   // wgrad_workspace_floats(M, N, plan) floats (none needed when that is 0)
+  int out16, db16;  // D / db point to the operands' 16-bit type instead of fp32 (both or neither; no accumulate)
+  float* ws;   // wgrad_workspace_floats(M, N, plan, out16) floats (none needed when that is 0)
   int splits;  // set from the plan
   int k1;      // set from the plan
 };
@@ -163,7 +164,7 @@ struct WgradPlan {
   int splits, k1, pairs;
 };
 WgradPlan wgrad_plan(int64_t M, int64_t N, int64_t T);
-int64_t wgrad_workspace_floats(int64_t M, int64_t N, const WgradPlan& plan);
+int64_t wgrad_workspace_floats(int64_t M, int64_t N, const WgradPlan& plan, bool out16 = false);
 int wgrad_tcgen05_supported(const WgradArgs& a);
 cudaError_t wgrad_tcgen05(const WgradArgs& a, const WgradPlan& plan, cudaStream_t s);
 

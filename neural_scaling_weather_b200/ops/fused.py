@@ -24,6 +24,7 @@ from ._ext import require
 from .geometry import WindowGeometry
 
 DT = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+EPS32 = float(torch.finfo(torch.float32).eps)
 
 
 def _cdtype(x: torch.Tensor) -> torch.dtype:
@@ -411,59 +412,26 @@ class _GatedMLP(torch.autograd.Function):
 
 def gated_mlp_cuda(x, wg, wu, wd, bg, bu, bd, residual, activation):
     act = _GATED_ACT[activation]
-    args = (x, wg, wu, wd, bg, bu, bd, residual)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
-        return _GatedMLP.apply(x, residual, act, wg, wu, wd, bg, bu, bd)
     dt = _cdtype(x)
-    N = wd.shape[0]
-    res = None if residual is None else _rows(residual, N).to(dt)
-    (y,) = require().gated_mlp_fwd(_rows(x, x.shape[-1]).to(dt), wcache.get(wg, dt), wcache.get(wu, dt),
-                                   wcache.get(wd, dt), bg, bu, bd, res, act, False)
-    return y if x.dim() == 2 else y.view(*x.shape[:-1], N)
+    if residual is not None and residual.dtype != dt:
+        residual = residual.to(dt)
+    if wg.dtype == wu.dtype == wd.dtype == dt:  # parameters already in the compute type: one native node
+        return require().gated_mlp(x if x.dtype == dt else x.to(dt), wg, wu, wd, bg, bu, bd, residual, act)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, wg, wu, wd, bg, bu, bd, residual)):
+        return _GatedMLP.apply(x, residual, act, wg, wu, wd, bg, bu, bd)
+    return require().gated_mlp(x.to(dt), wcache.get(wg, dt), wcache.get(wu, dt), wcache.get(wd, dt), bg, bu, bd,
+                               residual, act)
 
 
 # ---------------------------------------------------------------------------- norms, gate, skip
-def _f32(t):
-    return None if t is None else t.detach().float().contiguous()
-
-
-class _NormGateResidual(torch.autograd.Function):
-    """Keeps the branch's output and the skip connection; the backward recomputes the stream from them in
-    fp32 (the same bytes as reading the stream back, without its rounding)."""
-
-    @staticmethod
-    def forward(ctx, y, skip, w_post, gate, w_next, skip_scale, eps):
-        s, n = require().norm_gate_fwd(y, skip, _f32(w_post), _f32(gate), _f32(w_next), skip_scale, eps)
-        ctx.save_for_backward(y, skip, w_post, gate, w_next)
-        ctx.scale, ctx.eps = skip_scale, eps
-        return s, n
-
-    @staticmethod
-    def backward(ctx, ds, dn):
-        y, skip, w_post, gate, w_next = ctx.saved_tensors
-        cont = lambda t: None if t is None else t.to(y.dtype).contiguous()  # noqa: E731
-        dy, dskip, dwp, dgate, dwn = require().norm_gate_bwd(cont(ds), cont(dn), y, skip, _f32(w_post), _f32(gate),
-                                                             _f32(w_next), ctx.scale, ctx.eps)
-        need = ctx.needs_input_grad
-        out = lambda g, p, n: g.view(p.shape).to(p.dtype) if n and g is not None else None  # noqa: E731
-        return (dy, dskip, out(dwp, w_post, need[2]), out(dgate, gate, need[3]), out(dwn, w_next, need[4]), None, None)
-
-
 def norm_gate_residual_cuda(y, skip, w_post, gate, w_next, skip_scale, eps):
-    eps = float(torch.finfo(torch.float32).eps) if eps is None else float(eps)
+    """One native autograd node.  It keeps the branch's output and the skip connection; the backward recomputes
+    the stream from them in fp32 (the same bytes as reading the stream back, without its rounding)."""
     dt = _cdtype(y)
-    D = y.shape[-1]
-    # one "sample" unless the gate differs between them
-    shape = (y.shape[0], -1, D) if gate is not None and gate.dim() == 2 else (1, -1, D)
-    if y.numel() == 0:
-        shape = (shape[0], 0, D)
-    y3, k3 = (t.to(dt).reshape(shape).contiguous() for t in (y, skip))
-    args = (y3, k3, w_post, gate, w_next)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
-        s, n = _NormGateResidual.apply(*args, float(skip_scale), eps)
-    else:
-        s, n = require().norm_gate_fwd(y3, k3, _f32(w_post), _f32(gate), _f32(w_next), float(skip_scale), eps)
-    return s.view(y.shape), None if n is None else n.view(y.shape)
+    f32 = torch.float32
+    y, skip = (t if t.dtype == dt else t.to(dt) for t in (y, skip))
+    w_post, gate, w_next = (t if t is None or t.dtype == f32 else t.float() for t in (w_post, gate, w_next))
+    return tuple(require().norm_gate(y, skip, w_post, gate, w_next, skip_scale, EPS32 if eps is None else eps))
 
 
 # ---------------------------------------------------------------------------- attention
