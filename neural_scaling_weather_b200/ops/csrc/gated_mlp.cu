@@ -502,13 +502,15 @@ static cudaError_t launch_gated_mode(const GatedArgs& a, cudaStream_t s) {
 }  // namespace tc
 
 // ============================================================================ few tokens
-// Up to 64 tokens: the products are bound by reading the weights once, so a block takes 8 output rows
-// and its warps split the depth.  A warp's step is one mma.sync m16n8k16 pair over 32 values of k: lane
-// (r, t) reads 16 contiguous bytes, k = k0 + 8 t .. 8 t + 7, of weight row r, and of token row r for the
-// other operand.  Which four of those values meet in which MMA is a permutation of k that both operands
-// share, so the sum is unchanged and every load is a full 16-byte vector.  In the DUAL form the upper
-// eight MMA rows are the same hidden units' rows of Wu, so g and u of a unit end in one thread.
-// Partials of the warps are added in warp order through shared memory (deterministic).
+// Up to 64 tokens: the products are bound by moving the weights into the SMs once, and the tokens as often
+// as there are blocks.  A tile is the 16 rows of one mma.sync m16n8k16: 16 output rows, or, in the DUAL form,
+// the rows of Wg and of Wu of 8 hidden units, so that g and u of a unit end in one thread.  A block takes G
+// tiles (they share each token load) of a K slice, its warps split the slice in steps of 32: lane (r, t) reads
+// 16 contiguous bytes, k = k0 + 8 t .. 8 t + 7, of weight row r, and of token row r for the other operand.
+// Which four of those values meet in which MMA is a permutation of k that both operands share, so the sum is
+// unchanged and every load is a full 16-byte vector.  The K slices are the CTAs of a cluster.  Partials are
+// added in warp order through shared memory, then in slice order through the cluster's shared memory
+// (deterministic).  plan_skinny picks G and the number of slices.
 namespace gated {
 
 constexpr int SK_WARPS = 8;
@@ -522,7 +524,7 @@ struct SkinnyParams {
   const void* res;
   void* out;
   int64_t ldx, ldw0, ldw1, ldres, ldout;
-  int M, N, K;
+  int M, N, K, k_slice;
   int bias_dtype, act;
   int dependent;  // launched as a programmatic dependent of the kernel that writes x
 };
@@ -562,32 +564,49 @@ __device__ __forceinline__ uint4 load8(const uint16_t* p, int left) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <typename T, int NT, bool DUAL, bool VEC>
+template <typename T, int NT, int G, bool DUAL, bool VEC>
 __global__ void __launch_bounds__(32 * SK_WARPS) skinny_kernel(const SkinnyParams p) {
-  constexpr int U = 4;  // steps whose weight loads are in flight together
+  constexpr int U = 4 / G;  // steps whose weight loads are in flight together
+  constexpr int R = DUAL ? 8 : 16;  // output rows of a tile
   __shared__ float red[SK_WARPS][NT][32][4];
+  __shared__ float part[G][NT][32][4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, t = lane & 3;
-  const int64_t row = (int64_t)blockIdx.x * 8 + r;
-  const bool row_ok = row < p.N;
-  const uint16_t* w0 = reinterpret_cast<const uint16_t*>(p.w0) + row * p.ldw0;
-  const uint16_t* w1 = reinterpret_cast<const uint16_t*>(p.w1) + row * p.ldw1;
+  const int slice = blockIdx.y, slices = gridDim.y;
+  const int k_begin = slice * p.k_slice;
+  const int k_end = min(p.K, k_begin + p.k_slice);
   const uint16_t* x = reinterpret_cast<const uint16_t*>(p.x);
-  float acc[NT][4];
+  const uint16_t *w0[G], *w1[G];
+  bool ok0[G], ok1[G];
 #pragma unroll
-  for (int i = 0; i < NT; ++i)
+  for (int g = 0; g < G; ++g) {
+    const int64_t row = ((int64_t)blockIdx.x * G + g) * R + r;
+    const int64_t row1 = DUAL ? row : row + 8;
+    ok0[g] = row < p.N;
+    ok1[g] = row1 < p.N;
+    w0[g] = reinterpret_cast<const uint16_t*>(p.w0) + row * p.ldw0;
+    w1[g] = DUAL ? reinterpret_cast<const uint16_t*>(p.w1) + row * p.ldw1
+                 : reinterpret_cast<const uint16_t*>(p.w0) + row1 * p.ldw0;
+  }
+  float acc[G][NT][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
+  for (int g = 0; g < G; ++g)
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) acc[g][i][j] = 0.f;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   bool waited = !p.dependent;
-  for (int k0 = warp * 32; k0 < p.K; k0 += SK_WARPS * 32 * U) {
-    uint4 wa[U], wb[U];
+  for (int k0 = k_begin + warp * 32; k0 < k_end; k0 += SK_WARPS * 32 * U) {
+    uint4 wa[U][G], wb[U][G];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int kk = k0 + i * SK_WARPS * 32 + 8 * t;
-      const int left = row_ok ? p.K - kk : 0;
-      wa[i] = load8<VEC, true>(w0 + kk, left);
-      wb[i] = DUAL ? load8<VEC, true>(w1 + kk, left) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int g = 0; g < G; ++g) {
+        wa[i][g] = load8<VEC, true>(w0[g] + kk, ok0[g] ? k_end - kk : 0);
+        wb[i][g] = load8<VEC, true>(w1[g] + kk, ok1[g] ? k_end - kk : 0);
+      }
     }
     if (!waited) {  // the weights do not depend on the kernel before; x does
       asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -600,62 +619,147 @@ __global__ void __launch_bounds__(32 * SK_WARPS) skinny_kernel(const SkinnyParam
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
         const int tok = 8 * n + r;
-        xv[n] = load8<VEC, false>(x + tok * p.ldx + kk, tok < p.M ? p.K - kk : 0);
+        xv[n] = load8<VEC, false>(x + tok * p.ldx + kk, tok < p.M ? k_end - kk : 0);
       }
 #pragma unroll
-      for (int n = 0; n < NT; ++n) {
-        mma16816<T>(acc[n], wa[i].x, wb[i].x, wa[i].y, wb[i].y, xv[n].x, xv[n].y);
-        mma16816<T>(acc[n], wa[i].z, wb[i].z, wa[i].w, wb[i].w, xv[n].z, xv[n].w);
-      }
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int g = 0; g < G; ++g) {
+          mma16816<T>(acc[g][n], wa[i][g].x, wb[i][g].x, wa[i][g].y, wb[i][g].y, xv[n].x, xv[n].y);
+          mma16816<T>(acc[g][n], wa[i][g].z, wb[i][g].z, wa[i][g].w, wb[i][g].w, xv[n].z, xv[n].w);
+        }
     }
   }
+  if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
 #pragma unroll
-  for (int n = 0; n < NT; ++n)
-    *reinterpret_cast<float4*>(red[warp][n][lane]) = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
-  __syncthreads();
-  for (int i = threadIdx.x; i < NT * 32; i += 32 * SK_WARPS) {
-    const int n = i >> 5, l = i & 31;
-    float4 v = *reinterpret_cast<const float4*>(red[0][n][l]);
+  for (int g = 0; g < G; ++g) {
+    if (g) __syncthreads();
 #pragma unroll
-    for (int w = 1; w < SK_WARPS; ++w) {
-      const float4 o = *reinterpret_cast<const float4*>(red[w][n][l]);
-      v.x += o.x;
-      v.y += o.y;
-      v.z += o.z;
-      v.w += o.w;
+    for (int n = 0; n < NT; ++n)
+      *reinterpret_cast<float4*>(red[warp][n][lane]) =
+          make_float4(acc[g][n][0], acc[g][n][1], acc[g][n][2], acc[g][n][3]);
+    __syncthreads();
+    for (int i = threadIdx.x; i < NT * 32; i += 32 * SK_WARPS) {
+      const int n = i >> 5, l = i & 31;
+      float4 v = *reinterpret_cast<const float4*>(red[0][n][l]);
+#pragma unroll
+      for (int w = 1; w < SK_WARPS; ++w) {
+        const float4 o = *reinterpret_cast<const float4*>(red[w][n][l]);
+        v.x += o.x;
+        v.y += o.y;
+        v.z += o.z;
+        v.w += o.w;
+      }
+      *reinterpret_cast<float4*>(part[g][n][l]) = v;
     }
-    const int64_t col = (int64_t)blockIdx.x * 8 + (l >> 2);
-    if (col >= p.N) continue;
+  }
+  if (slices > 1)
+    tc::cluster_sync_all();
+  else
+    __syncthreads();
+  // this CTA's share of the (tile, token group, lane) entries: the slices' partials in order, then the epilogue
+  const int entries = G * NT * 32;
+  for (int i = slice * (32 * SK_WARPS) + threadIdx.x; i < entries; i += slices * (32 * SK_WARPS)) {
+    const int g = i / (NT * 32), n = (i >> 5) % NT, l = i & 31;
+    float4 v;
+    if (slices == 1) {
+      v = *reinterpret_cast<const float4*>(part[g][n][l]);
+    } else {
+      v = make_float4(0.f, 0.f, 0.f, 0.f);
+      for (int c = 0; c < slices; ++c) {
+        float4 o;
+        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w)
+                     : "r"(tc::map_rank(part[g][n][l], (uint32_t)c))
+                     : "memory");
+        v.x += o.x;
+        v.y += o.y;
+        v.z += o.z;
+        v.w += o.w;
+      }
+    }
+    const int64_t col = ((int64_t)blockIdx.x * G + g) * R + (l >> 2);
     const int tok = 8 * n + 2 * (l & 3);
-    const float b0 = p.bias0 ? tc::ld_bias(p.bias0, p.bias_dtype, col) : 0.f;
-    float f[2] = {v.x + b0, v.y + b0};
-    if (DUAL) {
-      const float b1 = p.bias1 ? tc::ld_bias(p.bias1, p.bias_dtype, col) : 0.f;
-      f[0] = tc::act_parts(f[0], p.act).val * (v.z + b1);
-      f[1] = tc::act_parts(f[1], p.act).val * (v.w + b1);
-    }
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      if (tok + j >= p.M) break;
-      if (!DUAL && p.res) f[j] += to_f(reinterpret_cast<const T*>(p.res)[(tok + j) * p.ldres + col]);
-      reinterpret_cast<T*>(p.out)[(tok + j) * p.ldout + col] = from_f<T>(f[j]);
+    for (int half = 0; half < (DUAL ? 1 : 2); ++half) {
+      const int64_t c = col + 8 * half;
+      if (c >= p.N) break;
+      const float b0 = p.bias0 ? tc::ld_bias(p.bias0, p.bias_dtype, c) : 0.f;
+      float f[2] = {(half ? v.z : v.x) + b0, (half ? v.w : v.y) + b0};
+      if (DUAL) {
+        const float b1 = p.bias1 ? tc::ld_bias(p.bias1, p.bias_dtype, c) : 0.f;
+        f[0] = tc::act_parts(f[0], p.act).val * (v.z + b1);
+        f[1] = tc::act_parts(f[1], p.act).val * (v.w + b1);
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        if (tok + j >= p.M) break;
+        if (!DUAL && p.res) f[j] += to_f(reinterpret_cast<const T*>(p.res)[(tok + j) * p.ldres + c]);
+        reinterpret_cast<T*>(p.out)[(tok + j) * p.ldout + c] = from_f<T>(f[j]);
+      }
     }
   }
+  if (slices > 1) tc::cluster_sync_all();  // the peers have read this CTA's partials
+}
+
+// G tiles a block and `slices` K slices that move the fewest bytes through the busiest SM: blocks per SM times
+// (tokens' slice + weights' slice).  A slice's exchange through the cluster's shared memory costs about as
+// much as 16 KB more (a cluster launch and two barriers; fitted at 1 and 37 tokens).
+struct SkinnyPlan {
+  int g, slices;
+};
+static SkinnyPlan plan_skinny(int64_t M, int64_t N, int64_t K, bool dual) {
+  const int64_t sms = tc::sm_count(), tiles = (N + (dual ? 7 : 15)) / (dual ? 8 : 16);
+  SkinnyPlan best = {1, 1};
+  int64_t best_cost = INT64_MAX;
+  for (int slices = 1; slices <= 8; slices *= 2) {
+    if (slices > 1 && K / slices < 32 * SK_WARPS) break;  // a step for every warp
+    for (int g = 1; g <= 4; g *= 2) {
+      if (g > 1 && (tiles + g - 1) / g * slices < sms / 2) break;
+      const int64_t blocks = (tiles + g - 1) / g * slices;
+      const int64_t bytes = 2 * (K / slices) * (M + 16 * g) + (slices > 1 ? 16384 : 0);
+      const int64_t cost = (blocks + sms - 1) / sms * bytes;
+      if (cost < best_cost) {
+        best_cost = cost;
+        best = {g, slices};
+      }
+    }
+  }
+  return best;
+}
+
+template <typename T, int NT, int G, bool DUAL>
+static cudaError_t launch_skinny_g(SkinnyParams p, int slices, bool vec, cudaStream_t s) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  int n = 0;
+  if (p.dependent) {
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (slices > 1) {
+    attr[n].id = cudaLaunchAttributeClusterDimension;
+    attr[n].val.clusterDim.x = 1;
+    attr[n].val.clusterDim.y = (unsigned)slices;
+    attr[n++].val.clusterDim.z = 1;
+  }
+  constexpr int rows = (DUAL ? 8 : 16) * G;
+  p.k_slice = (p.K + 32 * slices - 1) / (32 * slices) * 32;
+  cfg.gridDim = dim3((unsigned)((p.N + rows - 1) / rows), (unsigned)slices, 1);
+  cfg.blockDim = dim3(32 * SK_WARPS, 1, 1);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = n;
+  if (vec) return cudaLaunchKernelEx(&cfg, skinny_kernel<T, NT, G, DUAL, true>, p);
+  return cudaLaunchKernelEx(&cfg, skinny_kernel<T, NT, G, DUAL, false>, p);
 }
 
 template <typename T, int NT, bool DUAL>
 static cudaError_t launch_skinny_nt(const SkinnyParams& p, bool vec, cudaStream_t s) {
-  cudaLaunchConfig_t cfg = {};
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.gridDim = dim3((unsigned)((p.N + 7) / 8), 1, 1);
-  cfg.blockDim = dim3(32 * SK_WARPS, 1, 1);
-  cfg.stream = s;
-  cfg.attrs = attr;
-  cfg.numAttrs = p.dependent ? 1 : 0;
-  if (vec) return cudaLaunchKernelEx(&cfg, skinny_kernel<T, NT, DUAL, true>, p);
-  return cudaLaunchKernelEx(&cfg, skinny_kernel<T, NT, DUAL, false>, p);
+  const SkinnyPlan plan = plan_skinny(p.M, p.N, p.K, DUAL);
+  if (plan.g == 1) return launch_skinny_g<T, NT, 1, DUAL>(p, plan.slices, vec, s);
+  if (plan.g == 2) return launch_skinny_g<T, NT, 2, DUAL>(p, plan.slices, vec, s);
+  return launch_skinny_g<T, NT, 4, DUAL>(p, plan.slices, vec, s);
 }
 
 template <typename T, bool DUAL>

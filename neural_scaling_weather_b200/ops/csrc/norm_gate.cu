@@ -171,8 +171,11 @@ __global__ void __launch_bounds__(WPR > 8 ? 32 * WPR : 256) fwd_kernel(const Par
   }
 }
 
+// two blocks of eight warps an SM: the next row's four operands are loaded while a row is worked on, so that
+// about 64 KB an SM are in flight (one block with 16 elements a lane and no prefetch: 245 us at
+// 64800 x 1024 instead of MEASURED)
 template <typename T, bool VEC, int WPR, int NV>
-__global__ void __launch_bounds__(WPR > 8 ? 32 * WPR : 256) bwd_kernel(const Params p) {
+__global__ void __launch_bounds__(WPR > 8 ? 32 * WPR : 256, WPR > 8 ? 1 : 2) bwd_kernel(const Params p) {
   constexpr int GL = 32 * WPR;
   constexpr int RPB = WPR > 8 ? 1 : 8 / WPR;
   extern __shared__ float sums[];  // [2][n]
@@ -193,17 +196,32 @@ __global__ void __launch_bounds__(WPR > 8 ? 32 * WPR : 256) bwd_kernel(const Par
       aq[v][j] = aw[v][j] = 0.f;
     }
   }
-  for (int64_t r = (int64_t)blockIdx.x * RPB + rg; r < p.rows; r += (int64_t)gridDim.x * RPB) {
+  uint4 nxt[4][NV];  // the next row's y, skip, ds, dn
+  auto fetch = [&](int64_t r) {
+    const int64_t at = (sample * p.rows + r) * p.n;
+#pragma unroll
+    for (int v = 0; v < NV; ++v) {
+      nxt[0][v] = load_row<T, VEC, GL>(reinterpret_cast<const T*>(p.y) + at, v, gl, p.n);
+      nxt[1][v] = load_row<T, VEC, GL>(reinterpret_cast<const T*>(p.skip) + at, v, gl, p.n);
+      nxt[2][v] = nxt[3][v] = make_uint4(0, 0, 0, 0);
+      if (p.ds) nxt[2][v] = load_row<T, VEC, GL>(reinterpret_cast<const T*>(p.ds) + at, v, gl, p.n);
+      if (p.dn) nxt[3][v] = load_row<T, VEC, GL>(reinterpret_cast<const T*>(p.dn) + at, v, gl, p.n);
+    }
+  };
+  const int64_t step = (int64_t)gridDim.x * RPB;
+  int64_t r = (int64_t)blockIdx.x * RPB + rg;
+  if (r < p.rows) fetch(r);
+  for (; r < p.rows; r += step) {
     const int64_t at = (sample * p.rows + r) * p.n;
     uint4 yr[NV], kr[NV], dsr[NV], dnr[NV];
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
-      yr[v] = load_row<T, VEC, GL>(reinterpret_cast<const T*>(p.y) + at, v, gl, p.n);
-      kr[v] = load_row<T, VEC, GL>(reinterpret_cast<const T*>(p.skip) + at, v, gl, p.n);
-      dnr[v] = dsr[v] = make_uint4(0, 0, 0, 0);
-      if (p.dn) dnr[v] = load_row<T, VEC, GL>(reinterpret_cast<const T*>(p.dn) + at, v, gl, p.n);
-      if (p.ds) dsr[v] = load_row<T, VEC, GL>(reinterpret_cast<const T*>(p.ds) + at, v, gl, p.n);
+      yr[v] = nxt[0][v];
+      kr[v] = nxt[1][v];
+      dsr[v] = nxt[2][v];
+      dnr[v] = nxt[3][v];
     }
+    if (r + step < p.rows) fetch(r + step);
     float q1[1] = {0.f};
 #pragma unroll
     for (int v = 0; v < NV; ++v) {
@@ -323,39 +341,54 @@ __global__ void __launch_bounds__(1024) finish_kernel(const float* __restrict__ 
 }
 
 template <typename T, bool VEC, int WPR, int NV>
-static cudaError_t launch(const Params& p, bool backward, dim3 grid, cudaStream_t s) {
-  const int threads = WPR > 8 ? 32 * WPR : 256;
-  if (!backward) {
-    fwd_kernel<T, VEC, WPR, NV><<<grid, threads, 0, s>>>(p);
-    return cudaGetLastError();
-  }
+static cudaError_t launch_fwd(const Params& p, dim3 grid, cudaStream_t s) {
+  fwd_kernel<T, VEC, WPR, NV><<<grid, WPR > 8 ? 32 * WPR : 256, 0, s>>>(p);
+  return cudaGetLastError();
+}
+template <typename T, bool VEC, int WPR, int NV>
+static cudaError_t launch_bwd(const Params& p, dim3 grid, cudaStream_t s) {
   auto k = bwd_kernel<T, VEC, WPR, NV>;
   const size_t smem = 2 * sizeof(float) * p.n;
   if (smem > 48 * 1024) NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  k<<<grid, threads, smem, s>>>(p);
+  k<<<grid, WPR > 8 ? 32 * WPR : 256, smem, s>>>(p);
   return cudaGetLastError();
 }
 
-// a lane holds at most 16 elements of a row (the backward's registers: two accumulators, two parameters and
-// four operands per element); rows longer than 512 take 2, 4, ... 32 warps
+// Warps a row.  Forward: a lane holds at most 16 elements (two rows of registers).  Backward: at most 8, since
+// a lane keeps two sums, two parameters and eight operand values of each of its elements in registers; 16
+// only for rows longer than a block of 512 threads covers with 8.
+constexpr int fwd_warps(int n) { return n <= 512 ? 1 : n <= 1024 ? 2 : n <= 2048 ? 4 : n <= 4096 ? 8 : n <= 8192 ? 16 : 32; }
+constexpr int bwd_warps(int n) { return n <= 256 ? 1 : n <= 512 ? 2 : n <= 1024 ? 4 : n <= 2048 ? 8 : n <= 8192 ? 16 : 32; }
+constexpr int rows_per_block(int warps) { return warps > 8 ? 1 : 8 / warps; }
+
 template <typename T, bool VEC>
 static cudaError_t launch_width(const Params& p, bool backward, dim3 grid, cudaStream_t s) {
-  if (p.n <= 256) return launch<T, VEC, 1, 1>(p, backward, grid, s);
-  if (p.n <= 512) return launch<T, VEC, 1, 2>(p, backward, grid, s);
-  if (p.n <= 1024) return launch<T, VEC, 2, 2>(p, backward, grid, s);
-  if (p.n <= 2048) return launch<T, VEC, 4, 2>(p, backward, grid, s);
-  if (p.n <= 4096) return launch<T, VEC, 8, 2>(p, backward, grid, s);
-  if (p.n <= 8192) return launch<T, VEC, 16, 2>(p, backward, grid, s);
-  return launch<T, VEC, 32, 2>(p, backward, grid, s);
+  if (!backward) {
+    if (p.n <= 256) return launch_fwd<T, VEC, 1, 1>(p, grid, s);
+    switch (fwd_warps(p.n)) {
+      case 1: return launch_fwd<T, VEC, 1, 2>(p, grid, s);
+      case 2: return launch_fwd<T, VEC, 2, 2>(p, grid, s);
+      case 4: return launch_fwd<T, VEC, 4, 2>(p, grid, s);
+      case 8: return launch_fwd<T, VEC, 8, 2>(p, grid, s);
+      case 16: return launch_fwd<T, VEC, 16, 2>(p, grid, s);
+      default: return launch_fwd<T, VEC, 32, 2>(p, grid, s);
+    }
+  }
+  switch (bwd_warps(p.n)) {
+    case 1: return launch_bwd<T, VEC, 1, 1>(p, grid, s);
+    case 2: return launch_bwd<T, VEC, 2, 1>(p, grid, s);
+    case 4: return launch_bwd<T, VEC, 4, 1>(p, grid, s);
+    case 8: return launch_bwd<T, VEC, 8, 1>(p, grid, s);
+    case 16: return p.n <= 4096 ? launch_bwd<T, VEC, 16, 1>(p, grid, s) : launch_bwd<T, VEC, 16, 2>(p, grid, s);
+    default: return launch_bwd<T, VEC, 32, 2>(p, grid, s);
+  }
 }
 
 }  // namespace ng
 
-static int norm_gate_rows_per_block(int n) { return n <= 512 ? 8 : (n <= 1024 ? 4 : (n <= 2048 ? 2 : 1)); }
-
 int norm_gate_blocks(int64_t samples, int64_t rows, int n, int sms) {
   // two blocks an SM over all samples, at least one a sample and none without rows
-  const int64_t rpb = norm_gate_rows_per_block(n);
+  const int64_t rpb = ng::rows_per_block(ng::bwd_warps(n));
   const int64_t want = std::max<int64_t>(1, 2 * (int64_t)sms / samples);
   return (int)std::max<int64_t>(1, std::min<int64_t>(want, (rows + rpb - 1) / rpb));
 }
@@ -397,7 +430,7 @@ static cudaError_t norm_gate_launch(const NormGateArgs& a, bool backward, int bl
 }
 
 cudaError_t norm_gate_fwd(const NormGateArgs& a, int sms, cudaStream_t s) {
-  const int64_t rpb = norm_gate_rows_per_block(a.n);
+  const int64_t rpb = ng::rows_per_block(ng::fwd_warps(a.n));
   const int64_t blocks = std::min<int64_t>((a.rows + rpb - 1) / rpb, std::max<int64_t>(1, 16 * (int64_t)sms / a.samples));
   return norm_gate_launch(a, false, (int)blocks, s);
 }
