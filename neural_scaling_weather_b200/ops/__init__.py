@@ -154,7 +154,7 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     ``residual`` (..., N).  ``activation``: ``"silu"`` or ``"gelu"`` (exact).  Any sizes and strides; rows whose
     strides are not multiples of 16 bytes cost one copy of the operand.  On CUDA both projections, the
     activation and the product are one kernel; the backward's data gradients read the weights as they are
-    stored.  Calls without gradients of at most 64 rows take kernels that stream the weights once."""
+    stored.  Calls without gradients of at most 16 rows take kernels that stream the weights once."""
     if activation not in GATED_ACTIVATIONS:
         raise ValueError(f"gated_mlp: activation {activation!r} is not one of {GATED_ACTIVATIONS}")
     H, K = w_gate.shape

@@ -154,7 +154,14 @@ std::vector<Tensor> gated_mlp_fwd(const Tensor& x, const Tensor& wg, const Tenso
     check(nsw::gated_skinny(down, true, stream()), "gated_mlp down");
     return {y};
   }
+  // all copies come before the first product: the second may start under it
   const Rows xa = aligned_rows(x), ga = aligned_rows(wg), ua = aligned_rows(wu), da = aligned_rows(wd);
+  Rows ra;
+  if (has_res) {
+    ra = aligned_rows(*residual);
+    down.in0 = ra.ptr();
+    down.ldin = ra.ld;
+  }
   Tensor g, u;
   if (save) {
     g = torch::empty({d.M, d.Hp}, opt);
@@ -169,19 +176,13 @@ std::vector<Tensor> gated_mlp_fwd(const Tensor& x, const Tensor& wg, const Tenso
   up.ldb0 = ga.ld;
   up.b1 = ua.ptr();
   up.ldb1 = ua.ld;
-  check(nsw::gated_product(up, stream()), "gated_mlp up");
+  check(nsw::gated_product(up, false, stream()), "gated_mlp up");
   auto y = torch::empty({d.M, round8(d.N)}, opt);
   down.b0 = da.ptr();
   down.ldb0 = da.ld;
-  Rows ra;
-  if (has_res) {
-    ra = aligned_rows(*residual);
-    down.in0 = ra.ptr();
-    down.ldin = ra.ld;
-  }
   down.out0 = y.data_ptr();
   down.ldout = round8(d.N);
-  check(nsw::gated_product(down, stream()), "gated_mlp down");
+  check(nsw::gated_product(down, true, stream()), "gated_mlp down");
   y = packed(y, d.N);
   if (!save) return {y};
   return {y, xa.t, g, u, h};
@@ -297,7 +298,7 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
   a.out0 = dgu.data_ptr();
   a.out1 = du;
   a.ldout = a.ldaux = 2 * d.Hp;
-  check(nsw::gated_product(a, stream()), "gated_mlp dh");
+  check(nsw::gated_product(a, false, stream()), "gated_mlp dh");
   if (need_dx) {
     auto dx = torch::empty({d.M, round8(d.K)}, opt);
     nsw::GatedArgs b{};
@@ -315,7 +316,7 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
     b.ldb1 = ua.ld;
     b.out0 = dx.data_ptr();
     b.ldout = round8(d.K);
-    check(nsw::gated_product(b, stream()), "gated_mlp dx");
+    check(nsw::gated_product(b, true, stream()), "gated_mlp dx");
     out[0] = packed(dx, d.K);
   }
   if (need_w || need_b) {

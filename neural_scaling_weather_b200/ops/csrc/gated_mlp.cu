@@ -16,7 +16,7 @@
 //            copy exists); the epilogue loads g and u tiles by TMA and writes dg and du.
 //     kDx    dg Wg + du Wu as ONE product of depth 2 H: the k-loop runs through (dg, Wg), then
 //            (du, Wu), into the same accumulator; the weights are again read MN-major as stored.
-// * skinny_kernel: up to 64 tokens, where the time is that of streaming the weights once.  See there.
+// * skinny_kernel: up to 16 tokens, where the time is that of streaming the weights once.  See there.
 //
 // Sums are fp32 in TMEM / registers.  Rounded to 16 bits: g, u (kept for the backward), h, dg, du,
 // because the following products take 16-bit operands; the forward's h is computed from the unrounded
@@ -488,13 +488,439 @@ static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
+// ============================================================================ split-depth form
+// The same four products where gated_kernel would have too few tiles to fill the device (a few hundred rows,
+// or few output columns with a long depth).  The weights are the MMA's M operand (128 of their rows, in kUp 64
+// rows of Wg and the same 64 of Wu) and NTOK tokens its N operand, one CTA per tile and depth slice; the
+// slices of a tile are the CTAs of a cluster.  Each CTA leaves its fp32 partial in its shared memory (over
+// the drained pipeline stages), and after a cluster barrier every CTA adds its share of the tile over the
+// slices in order (deterministic) and does the epilogue with plain, row-contiguous accesses.
+//   warp 0: TMA producer; warp 1: MMA issuer; warps 2-9: TMEM to shared memory; all: the final sums.
+// In a dependent launch the weight tiles of the first stages are on their way before the wait for the kernel
+// that writes the tokens.
+constexpr int kSplitThreads = 320;  // a multiple of a tile's quads: a thread's columns stay the same
+constexpr int kMaxSlices = 8;  // the largest portable cluster
+
+__device__ __forceinline__ float4 ld_cluster4(uint32_t at) {
+  float4 o;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w)
+               : "r"(at)
+               : "memory");
+  return o;
+}
+
+struct SplitParams {
+  CUtensorMap w0, w1, x0, x1;
+  int64_t M, N;
+  int kb0, kb;
+  const void *bias0, *bias1, *in0, *in1;
+  void *out0, *out1, *out2;
+  int64_t ldin, ldout, ldaux;
+  int bias_dtype, act, dependent;
+};
+
+template <typename T, int NTOK, int STAGES>
+struct SmemS {
+  union {
+    struct {
+      alignas(1024) T w[STAGES][BM * BK];
+      alignas(1024) T x[STAGES][NTOK * BK];
+    };
+    float part[NTOK][BM];  // [token][weight row]
+  };
+  uint64_t full[STAGES], empty[STAGES];
+  uint64_t tmem_full;
+  uint32_t tmem_base;
+  int abort_flag;
+};
+
+// four consecutive columns of a row, those below N
 template <typename T>
-static cudaError_t launch_gated_mode(const GatedArgs& a, cudaStream_t s) {
+__device__ __forceinline__ void load4(const T* p, int64_t left, bool vec, float* f) {
+  if (vec && left >= 4) {
+    uint2 w = *reinterpret_cast<const uint2*>(p);
+    unpack2(w.x, f, T());
+    unpack2(w.y, f + 2, T());
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) f[j] = j < left ? to_f(p[j]) : 0.f;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* p, int64_t left, bool vec, const float* f) {
+  if (vec && left >= 4) {
+    T h[4] = {from_f<T>(f[0]), from_f<T>(f[1]), from_f<T>(f[2]), from_f<T>(f[3])};
+    uint2 w;
+    memcpy(&w, h, 8);
+    *reinterpret_cast<uint2*>(p) = w;
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (j < left) p[j] = from_f<T>(f[j]);
+  }
+}
+
+template <typename T, int MODE, int NTOK, int STAGES>
+__global__ void __launch_bounds__(kSplitThreads, NTOK <= 64 ? 2 : 1) split_kernel(const __grid_constant__ SplitParams p, uint32_t idesc,
+                                                              int* err) {
+  constexpr bool kMn = MODE == kDh || MODE == kDx;
+  constexpr int kUnits = MODE == kUp ? 64 : 128;  // output columns of a tile
+  extern __shared__ __align__(1024) unsigned char smem_raw[];
+  unsigned char* base = reinterpret_cast<unsigned char*>(
+      (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  using Smem = SmemS<T, NTOK, STAGES>;
+  auto& S = *reinterpret_cast<Smem*>(base);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int slice = blockIdx.y, slices = gridDim.y;
+  const int64_t n0 = (int64_t)blockIdx.x * kUnits, m0 = (int64_t)blockIdx.z * NTOK;
+  const int kb_begin = (int)((int64_t)slice * p.kb / slices), kb_end = (int)((int64_t)(slice + 1) * p.kb / slices);
+  const int nkb = kb_end - kb_begin;
+  volatile int* abort_flag = &S.abort_flag;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(&S.full[s], 1);
+      mbar_init(&S.empty[s], 1);
+    }
+    mbar_init(&S.tmem_full, 1);
+    S.abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&S.tmem_base)),
+                 "r"(NTOK));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = S.tmem_base;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      auto load_w = [&](int i) {
+        const int kb = kb_begin + i, st = i % STAGES;
+        const bool second = MODE == kDx && kb >= p.kb0;
+        const int k0 = (second ? kb - p.kb0 : kb) * BK;
+        const CUtensorMap* m = second ? &p.w1 : &p.w0;
+        if (kMn) {
+          tma_load_2d(&S.w[st][0], m, &S.full[st], (int)n0, k0);
+          tma_load_2d(&S.w[st][64 * BK], m, &S.full[st], (int)n0 + 64, k0);
+        } else if (MODE == kUp) {
+          tma_load_2d(&S.w[st][0], &p.w0, &S.full[st], k0, (int)n0);
+          tma_load_2d(&S.w[st][64 * BK], &p.w1, &S.full[st], k0, (int)n0);
+        } else {
+          tma_load_2d(&S.w[st][0], m, &S.full[st], k0, (int)n0);
+        }
+      };
+      auto load_x = [&](int i) {
+        const int kb = kb_begin + i, st = i % STAGES;
+        const bool second = MODE == kDx && kb >= p.kb0;
+        tma_load_2d(&S.x[st][0], second ? &p.x1 : &p.x0, &S.full[st], (second ? kb - p.kb0 : kb) * BK, (int)m0);
+      };
+      constexpr uint32_t kBytes = (BM + NTOK) * BK * sizeof(T);
+      const int first = nkb < STAGES ? nkb : STAGES;
+      for (int i = 0; i < first; ++i) {
+        mbar_expect_tx(&S.full[i], kBytes);
+        load_w(i);
+      }
+      if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
+      for (int i = 0; i < first; ++i) load_x(i);
+      int issued = first;
+      for (; issued < nkb; ++issued) {
+        const int st = issued % STAGES;
+        if (!mbar_wait(&S.empty[st], (uint32_t)((issued / STAGES - 1) & 1), abort_flag, err)) break;
+        mbar_expect_tx(&S.full[st], kBytes);
+        load_w(issued);
+        load_x(issued);
+      }
+      // every load has landed before the stages are reused (bounded; at once unless something gave up)
+      for (int i = issued > STAGES ? issued - STAGES : 0; i < issued; ++i) {
+        const unsigned long long t0 = globaltimer();
+        while (!mbar_try_wait(&S.full[i % STAGES], (uint32_t)((i / STAGES) & 1)) && globaltimer() - t0 < kWaitBudgetNs) {
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      bool ok = true;
+      for (int i = 0; i < nkb; ++i) {
+        const int st = i % STAGES;
+        if (!mbar_wait(&S.full[st], (uint32_t)((i / STAGES) & 1), abort_flag, err)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+#pragma unroll
+        for (int k = 0; k < BK / 16; ++k) {
+          const uint64_t da = kMn ? smem_desc_mn(&S.w[st][k * 16 * 64], 64 * BK * (uint32_t)sizeof(T))
+                                  : smem_desc_sw128(&S.w[st][k * 16]);
+          umma_f16(tmem_base, da, smem_desc_sw128(&S.x[st][k * 16]), idesc, (i > 0 || k > 0) ? 1u : 0u);
+        }
+        umma_commit(&S.empty[st]);
+      }
+      if (ok) umma_commit(&S.tmem_full);
+    }
+  }
+  __syncwarp();
+  // the accumulator is complete (and every stage read): all warps wait for it before the stages become `part`
+  if (warp >= 1) mbar_wait(&S.tmem_full, 0, abort_flag, err);
+  tc_fence_after();
+  __syncthreads();
+  if (warp >= 2) {
+    const int q = warp & 3;
+#pragma unroll 1
+    for (int c = 32 * ((warp - 2) >> 2); c < NTOK; c += 64) {
+      uint32_t r[32];
+      tmem_ld32(tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)c, r);
+#pragma unroll
+      for (int j = 0; j < 32; ++j) S.part[c + j][q * 32 + lane] = __uint_as_float(r[j]);
+    }
+    tc_fence_before();
+  }
+  cluster_sync_all();
+  tc_fence_after();
+  if (warp == 1)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(NTOK));
+  if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
+
+  constexpr int kQuads = kUnits / 4;
+  constexpr int kBatch = MODE == kUp ? 2 : 4;  // items whose loads are in flight together
+  static_assert(kSplitThreads % kQuads == 0, "a thread's columns");
+  const int tokens = (int)(p.M - m0 < NTOK ? p.M - m0 : NTOK);
+  const int64_t col = n0 + 4 * (threadIdx.x % kQuads), left = p.N - col;
+  const bool vec = ((p.ldout | p.ldaux | p.ldin) & 3) == 0 &&
+                   ((reinterpret_cast<uintptr_t>(p.out0) | reinterpret_cast<uintptr_t>(p.out1) |
+                     reinterpret_cast<uintptr_t>(p.out2) | reinterpret_cast<uintptr_t>(p.in0) |
+                     reinterpret_cast<uintptr_t>(p.in1)) & 7) == 0;
+  float b0[4] = {0.f, 0.f, 0.f, 0.f}, b1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (p.bias0 && j < left) b0[j] = ld_bias(p.bias0, p.bias_dtype, col + j);
+    if (MODE == kUp && p.bias1 && j < left) b1[j] = ld_bias(p.bias1, p.bias_dtype, col + j);
+  }
+  const int step = slices * (kSplitThreads / kQuads);
+  const float* mine = &S.part[0][4 * (threadIdx.x % kQuads)];
+  for (int t0 = (slice * kSplitThreads + threadIdx.x) / kQuads; t0 < tokens && left > 0; t0 += step * kBatch) {
+    float f[kBatch][4], u[kBatch][4];
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int tok = t0 + b * step;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) f[b][j] = b0[j], u[b][j] = b1[j];
+      if (tok >= tokens) continue;
+      const int64_t row = m0 + tok;
+      if (MODE == kDown && p.in0)
+        load4<T>(reinterpret_cast<const T*>(p.in0) + row * p.ldin + col, left, vec, u[b]);
+      if (MODE == kDh) {
+        load4<T>(reinterpret_cast<const T*>(p.in0) + row * p.ldin + col, left, vec, b0);  // (no bias: g)
+        load4<T>(reinterpret_cast<const T*>(p.in1) + row * p.ldin + col, left, vec, u[b]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const ActParts a = act_parts(b0[j], p.act);
+          f[b][j] = u[b][j] * a.slope;
+          u[b][j] = a.val;
+        }
+      }
+    }
+    // every slice's partials, in slice order
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int tok = t0 + b * step;
+      if (tok >= tokens) continue;
+      float4 o[kMaxSlices], o2[MODE == kUp ? kMaxSlices : 1];
+#pragma unroll
+      for (int c = 0; c < kMaxSlices; ++c) {
+        o[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (MODE == kUp) o2[c] = o[c];
+        if (c < slices) {
+          const uint32_t at = map_rank(mine + tok * BM, (uint32_t)c);
+          o[c] = ld_cluster4(at);
+          if (MODE == kUp) o2[c] = ld_cluster4(at + 256u);
+        }
+      }
+      float a[4] = {o[0].x, o[0].y, o[0].z, o[0].w};
+#pragma unroll
+      for (int c = 1; c < kMaxSlices; ++c) a[0] += o[c].x, a[1] += o[c].y, a[2] += o[c].z, a[3] += o[c].w;
+      if (MODE == kUp) {
+        float w[4] = {o2[0].x, o2[0].y, o2[0].z, o2[0].w};
+#pragma unroll
+        for (int c = 1; c < kMaxSlices; ++c) w[0] += o2[c].x, w[1] += o2[c].y, w[2] += o2[c].z, w[3] += o2[c].w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) u[b][j] += w[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (MODE == kDh) {
+          f[b][j] *= a[j];
+          u[b][j] *= a[j];
+        } else {
+          f[b][j] += a[j];
+        }
+      }
+    }
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int tok = t0 + b * step;
+      if (tok >= tokens) continue;
+      const int64_t row = m0 + tok;
+      if (MODE == kUp && p.out1) {
+        store4<T>(reinterpret_cast<T*>(p.out1) + row * p.ldaux + col, left, vec, f[b]);
+        store4<T>(reinterpret_cast<T*>(p.out2) + row * p.ldaux + col, left, vec, u[b]);
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (MODE == kUp) f[b][j] = act_parts(f[b][j], p.act).val * u[b][j];
+        if (MODE == kDown) f[b][j] += p.in0 ? u[b][j] : 0.f;
+      }
+      if (MODE == kDh) store4<T>(reinterpret_cast<T*>(p.out1) + row * p.ldaux + col, left, vec, u[b]);
+      store4<T>(reinterpret_cast<T*>(p.out0) + row * p.ldout + col, left, vec, f[b]);
+    }
+  }
+  cluster_sync_all();  // the peers have read this CTA's partials
+}
+
+template <typename T, int MODE, int NTOK, int STAGES>
+static cudaError_t launch_split(const GatedArgs& a, int slices, bool dependent, cudaStream_t s) {
+  constexpr bool mn = MODE == kDh || MODE == kDx;
+  auto k = split_kernel<T, MODE, NTOK, STAGES>;
+  const size_t smem = sizeof(SmemS<T, NTOK, STAGES>) + 1024;
+  NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  SplitParams p;
+  memset(&p, 0, sizeof(p));
+  const int rows = MODE == kUp ? 64 : 128;
+  bool ok = make_map(&p.x0, a.a0, a.M, a.K, a.lda, NTOK, a.dtype);
+  if (MODE == kDx) ok = ok && make_map(&p.x1, a.a1, a.M, a.K, a.lda, NTOK, a.dtype);
+  ok = ok && (mn ? make_map_mn(&p.w0, a.b0, a.K, a.N, a.ldb0, a.dtype)
+                 : make_map(&p.w0, a.b0, a.N, a.K, a.ldb0, rows, a.dtype));
+  if (MODE == kUp) ok = ok && make_map(&p.w1, a.b1, a.N, a.K, a.ldb1, rows, a.dtype);
+  if (MODE == kDx) ok = ok && make_map_mn(&p.w1, a.b1, a.K, a.N, a.ldb1, a.dtype);
+  if (!ok) return cudaErrorInvalidValue;
+  p.M = a.M;
+  p.N = a.N;
+  p.kb0 = (int)((a.K + BK - 1) / BK);
+  p.kb = MODE == kDx ? 2 * p.kb0 : p.kb0;
+  p.bias0 = a.bias0;
+  p.bias1 = a.bias1;
+  p.bias_dtype = a.bias_dtype;
+  p.in0 = a.in0;
+  p.in1 = a.in1;
+  p.out0 = a.out0;
+  p.out1 = a.out1;
+  p.out2 = a.out2;
+  p.ldin = a.ldin;
+  p.ldout = a.ldout;
+  p.ldaux = a.ldaux;
+  p.act = a.act;
+  p.dependent = dependent;
+  const uint32_t fmt = a.dtype == kBF16 ? 1u : 0u;
+  const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (mn ? 1u << 15 : 0u) |
+                         ((uint32_t)(NTOK >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 1;
+  attr[0].val.clusterDim.y = (unsigned)slices;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)((a.N + rows - 1) / rows), (unsigned)slices, (unsigned)((a.M + NTOK - 1) / NTOK));
+  cfg.blockDim = dim3(kSplitThreads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, k, p, idesc, device_error_flag());
+}
+
+// CTAs of clusters of `slices` that the device holds at once, one a SM (clusters do not cross the groups of
+// SMs they are placed in, so the larger ones leave some SMs idle)
+static int64_t split_room(int slices) {
+  static int64_t room[kMaxSlices + 1] = {};
+  if (!room[slices]) {
+    auto k = split_kernel<__nv_bfloat16, kDown, 256, 4>;
+    const size_t smem = sizeof(SmemS<__nv_bfloat16, 256, 4>) + 1024;
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = 1;
+    attr[0].val.clusterDim.y = (unsigned)slices;
+    attr[0].val.clusterDim.z = 1;
+    cfg.gridDim = dim3(1, (unsigned)slices, 64);
+    cfg.blockDim = dim3(kSplitThreads, 1, 1);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess ||
+        cudaOccupancyMaxActiveClusters(&n, k, &cfg) != cudaSuccess || n < 1)
+      n = 1;
+    room[slices] = (int64_t)n * slices;
+  }
+  return room[slices];
+}
+
+// Tokens a tile and depth slices of the split form, and whether it beats gated_kernel.  Both forms' times are
+// modelled in microseconds, launch to launch: waves of CTAs times (k-blocks, final sums, fixed part).  The
+// constants were fitted to 1500 timings of both forms over the four products at 17 to 2048 rows and widths
+// 128 x 344 to 2048 x 5464; the plan's choice is on average 3.5% (at most 28%) above the best of them, the
+// general form alone 54%.  For example, 256 rows of h [.., 2736] times Wd [1024, ..]: 18.9 us in gated_kernel
+// (4 tiles), 9.5 us as 64 x 4.
+struct SplitPlan {
+  int ntok, slices;
+  bool use;
+};
+static SplitPlan plan_split(const GatedArgs& a) {
+  const int64_t units = a.mode == kGatedUp ? 64 : 128, cols = a.mode == kGatedUp ? 128 : 256;
+  const int64_t kb = (a.K + BK - 1) / BK * (a.mode == kGatedDx ? 2 : 1);
+  const double tail = a.mode == kGatedUp || a.mode == kGatedDh ? 0.052 : 0.035;  // final sums of a token
+  SplitPlan best = {0, 1, false};
+  double best_cost = 1e30;
+  for (int ntok = 32; ntok <= 256; ntok *= 2) {
+    const double step = ntok == 32 ? 0.28 : ntok == 64 ? 0.31 : ntok == 128 ? 0.32 : 0.48;
+    const int64_t tiles = (a.M + ntok - 1) / ntok * ((a.N + units - 1) / units);
+    for (int slices = 1; slices <= kMaxSlices && slices <= kb; slices *= 2) {
+      const int64_t one = split_room(slices), room = one * (ntok <= 64 ? 2 : 1);  // 64 tokens: two CTAs a SM
+      const int64_t ctas = tiles * slices, waves = (ctas + room - 1) / room;
+      const double crowd = 1.0 + 0.15 * std::max<int64_t>(0, std::min(ctas, room) - one) / (double)one;
+      const double cost = waves * ((double)((kb + slices - 1) / slices) * step * crowd +
+                                   tail * std::min<int64_t>(a.M, ntok) / slices + 3.75) +
+                          0.5 + 0.55 * (slices > 4 ? 3 : slices > 2 ? 2 : slices > 1 ? 1 : 0);
+      if (cost < best_cost) {
+        best_cost = cost;
+        best.ntok = ntok;
+        best.slices = slices;
+      }
+    }
+  }
+  const int64_t tiles = ((a.M + BM2 - 1) / BM2) * ((a.N + cols - 1) / cols), pairs = sm_count() / 2;
+  const double fixed = a.mode == kGatedUp ? 0.75 : a.mode == kGatedDown ? 1.1 : a.mode == kGatedDh ? 5.4 : 0.0;
+  const double general = 5.0 + (double)((tiles + pairs - 1) / pairs) * (0.31 * kb + fixed);
+  best.use = best_cost < general && (a.M + best.ntok - 1) / best.ntok <= 65535;
+  return best;
+}
+
+template <typename T, int MODE>
+static cudaError_t launch_any(const GatedArgs& a, bool dependent, cudaStream_t s) {
+  const SplitPlan plan = plan_split(a);
+  if (!plan.use) return launch_gated<T, MODE>(a, s);
+  switch (plan.ntok) {
+    case 32: return launch_split<T, MODE, 32, 5>(a, plan.slices, dependent, s);
+    case 64: return launch_split<T, MODE, 64, 4>(a, plan.slices, dependent, s);
+    case 128: return launch_split<T, MODE, 128, 6>(a, plan.slices, dependent, s);
+    default: return launch_split<T, MODE, 256, 4>(a, plan.slices, dependent, s);
+  }
+}
+
+template <typename T>
+static cudaError_t launch_gated_mode(const GatedArgs& a, bool dependent, cudaStream_t s) {
   switch (a.mode) {
-    case kGatedUp: return launch_gated<T, kUp>(a, s);
-    case kGatedDown: return launch_gated<T, kDown>(a, s);
-    case kGatedDh: return launch_gated<T, kDh>(a, s);
-    case kGatedDx: return launch_gated<T, kDx>(a, s);
+    case kGatedUp: return launch_any<T, kUp>(a, dependent, s);
+    case kGatedDown: return launch_any<T, kDown>(a, dependent, s);
+    case kGatedDh: return launch_any<T, kDh>(a, dependent, s);
+    case kGatedDx: return launch_any<T, kDx>(a, dependent, s);
   }
   return cudaErrorInvalidValue;
 }
@@ -502,7 +928,7 @@ static cudaError_t launch_gated_mode(const GatedArgs& a, cudaStream_t s) {
 }  // namespace tc
 
 // ============================================================================ few tokens
-// Up to 64 tokens: the products are bound by moving the weights into the SMs once, and the tokens as often
+// Up to 16 tokens: the products are bound by moving the weights into the SMs once, and the tokens as often
 // as there are blocks.  A tile is the 16 rows of one mma.sync m16n8k16: 16 output rows, or, in the DUAL form,
 // the rows of Wg and of Wu of 8 hidden units, so that g and u of a unit end in one thread.  A block takes G
 // tiles (they share each token load) of a K slice, its warps split the slice in steps of 32: lane (r, t) reads
@@ -667,11 +1093,7 @@ __global__ void __launch_bounds__(32 * SK_WARPS) skinny_kernel(const SkinnyParam
     } else {
       v = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int c = 0; c < slices; ++c) {
-        float4 o;
-        asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-                     : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w)
-                     : "r"(tc::map_rank(part[g][n][l], (uint32_t)c))
-                     : "memory");
+        const float4 o = tc::ld_cluster4(tc::map_rank(part[g][n][l], (uint32_t)c));
         v.x += o.x;
         v.y += o.y;
         v.z += o.z;
@@ -764,10 +1186,7 @@ static cudaError_t launch_skinny_nt(const SkinnyParams& p, bool vec, cudaStream_
 
 template <typename T, bool DUAL>
 static cudaError_t launch_skinny(const SkinnyParams& p, bool vec, cudaStream_t s) {
-  if (p.M <= 8) return launch_skinny_nt<T, 1, DUAL>(p, vec, s);
-  if (p.M <= 16) return launch_skinny_nt<T, 2, DUAL>(p, vec, s);
-  if (p.M <= 32) return launch_skinny_nt<T, 4, DUAL>(p, vec, s);
-  return launch_skinny_nt<T, 8, DUAL>(p, vec, s);
+  return p.M <= 8 ? launch_skinny_nt<T, 1, DUAL>(p, vec, s) : launch_skinny_nt<T, 2, DUAL>(p, vec, s);
 }
 
 // dst[i, j] = src[i s0 + j s1] (16-bit), rows of ld elements: operands whose rows are not 16-byte aligned
@@ -782,10 +1201,10 @@ __global__ void pad_copy_kernel(const uint16_t* __restrict__ src, int64_t s0, in
 
 }  // namespace gated
 
-cudaError_t gated_product(const GatedArgs& a, cudaStream_t s) {
+cudaError_t gated_product(const GatedArgs& a, bool dependent, cudaStream_t s) {
   if ((a.dtype != kBF16 && a.dtype != kF16) || a.M <= 0 || a.N <= 0 || a.K <= 0) return cudaErrorInvalidValue;
-  if (a.dtype == kBF16) return tc::launch_gated_mode<__nv_bfloat16>(a, s);
-  return tc::launch_gated_mode<__half>(a, s);
+  if (a.dtype == kBF16) return tc::launch_gated_mode<__nv_bfloat16>(a, dependent, s);
+  return tc::launch_gated_mode<__half>(a, dependent, s);
 }
 
 cudaError_t gated_skinny(const GatedArgs& a, bool dependent, cudaStream_t s) {

@@ -192,10 +192,11 @@ struct GatedArgs {
   void *out0, *out1, *out2;
   int64_t ldout, ldaux;
 };
-cudaError_t gated_product(const GatedArgs& a, cudaStream_t s);
-// kGatedUp (no out1 / out2) and kGatedDown for at most kGatedSkinnyTokens rows, any strides; dependent:
-// launched as a programmatic dependent of the kernel before it on the stream, which writes a0
-constexpr int kGatedSkinnyTokens = 64;
+// dependent: the A operand is written by the kernel before it on the stream, which this one may overlap (a
+// programmatic dependent launch: it waits for that kernel before it touches anything but the weights)
+cudaError_t gated_product(const GatedArgs& a, bool dependent, cudaStream_t s);
+// kGatedUp (no out1 / out2) and kGatedDown for at most kGatedSkinnyTokens rows, any strides
+constexpr int kGatedSkinnyTokens = 16;
 cudaError_t gated_skinny(const GatedArgs& a, bool dependent, cudaStream_t s);
 // 16-bit strided copy into rows of ld elements (cols of them written)
 cudaError_t pad_copy(const void* src, int64_t s0, int64_t s1, void* dst, int64_t ld, int64_t rows, int64_t cols,
