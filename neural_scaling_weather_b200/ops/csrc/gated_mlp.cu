@@ -32,8 +32,12 @@ namespace nsw {
 namespace tc {
 
 constexpr int GS = 5;        // pipeline stages (32 KB a CTA)
-constexpr int GBUFS = 4;     // 2 KB tile buffers per epilogue warp
 enum : int { kUp = 0, kDown = 1, kDh = 2, kDx = 3 };
+// Epilogue warps and 2 KB tile buffers of each.  kDh loads two tiles and stores two for each 32 columns, more
+// latency than arithmetic: sixteen warps with one pair of buffers each (413 us with eight warps and two pairs
+// at 64800 x 2736 x 1024, KDH16 us with sixteen).
+constexpr int epi_warps(int mode) { return mode == kDh ? 16 : 8; }
+constexpr int epi_bufs(int mode) { return mode == kDh ? 2 : 4; }
 
 struct GatedParams {
   CUtensorMap a0, a1, b0, b1;    // operands (a1 / b1: Wu in kUp, the second half of the depth in kDx)
@@ -49,14 +53,15 @@ struct GatedParams {
   int has_res;  // kDown
 };
 
-template <typename T>
+template <typename T, int MODE>
 struct SmemG {
+  static constexpr int EW = epi_warps(MODE);
   alignas(1024) T a[GS][BM * BK];
   alignas(1024) T b[GS][128 * BK];
-  alignas(1024) T buf[kEpiWarps][GBUFS][32 * kStageRow];
+  alignas(1024) T buf[EW][epi_bufs(MODE)][32 * kStageRow];
   uint64_t full[GS], empty[GS];
   uint64_t tmem_full[2], tmem_empty[2];
-  uint64_t in_full[kEpiWarps][2];
+  uint64_t in_full[EW];
   uint64_t done;
   uint32_t tmem_base;
   int abort_flag;
@@ -122,11 +127,11 @@ __device__ __forceinline__ void add_bias32(const void* p, int dtype, int64_t nb,
 
 __device__ __forceinline__ void bulk_wait_read_3() { asm volatile("cp.async.bulk.wait_group.read 3;" ::: "memory"); }
 
-// this lane's row of a 32 x 32 tile into the warp's next buffer (ring of GBUFS), then one TMA store
+// this lane's row of a 32 x 32 tile into the warp's next buffer (ring of four), then one TMA store
 template <typename T>
 __device__ __forceinline__ void ring_store(const CUtensorMap* map, const float* f, T (*buf)[32 * kStageRow], int lane,
                                            int64_t nb, int64_t row_base, uint32_t& ring) {
-  T* b = buf[ring & (GBUFS - 1)];
+  T* b = buf[ring & 3];
   if (lane == 0) bulk_wait_read_3();  // at most three later stores pending: this buffer's has been read
   __syncwarp();
 #pragma unroll
@@ -138,14 +143,15 @@ __device__ __forceinline__ void ring_store(const CUtensorMap* map, const float* 
 }
 
 template <typename T, int MODE>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(MODE), 1)
     gated_kernel(const __grid_constant__ GatedParams p, uint32_t idesc, int* err) {
   constexpr bool kMnB = MODE == kDh || MODE == kDx;  // B read as stored, N contiguous
   constexpr int kCols = MODE == kUp ? 128 : 256;     // result columns of a pair tile
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  auto& S = *reinterpret_cast<SmemG<T>*>(base);
+  constexpr int EW = epi_warps(MODE);
+  auto& S = *reinterpret_cast<SmemG<T, MODE>*>(base);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int64_t pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
@@ -161,9 +167,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     }
     for (int a = 0; a < 2; ++a) {
       mbar_init(&S.tmem_full[a], 1);
-      mbar_init(&S.tmem_empty[a], 2 * kEpiWarps);
-      for (int w = 0; w < kEpiWarps; ++w) mbar_init(&S.in_full[w][a], 1);
+      mbar_init(&S.tmem_empty[a], 2 * EW);
     }
+    for (int w = 0; w < EW; ++w) mbar_init(&S.in_full[w], 1);
     mbar_init(&S.done, 1);
     S.abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -250,56 +256,57 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     // ------------------------------------------------------------------ epilogue (both CTAs)
     const int ew = warp - 2;
     const int q = warp & 3;
-    const int half = ew >> 2;
+    const int part = ew >> 2;            // which share of the result's columns this warp drains
+    constexpr int kShare = kCols / (EW / 4);
+    constexpr int kChunks = kShare / 32;
     T(*buf)[32 * kStageRow] = S.buf[ew];
-    uint64_t* in_full = S.in_full[ew];
+    uint64_t* in_full = &S.in_full[ew];
     const uint32_t empty_leader = map_rank(&S.tmem_empty[0], 0);
     uint32_t ring = 0;
-    uint32_t in_phase = 0;  // parity of each in_full barrier, one bit each
+    uint32_t in_phase = 0;
     int acc = 0;
     uint32_t acc_phase = 0;
-    uint32_t pending = 0;  // input loads issued and not waited for, one bit per in_full barrier
+    bool pending = false;  // input tiles issued and not waited for
     bool ok = true;
     for (int64_t tile = pair; tile < num_tiles && ok; tile += npairs) {
       const int64_t row_base = (tile / n_tiles) * BM2 + (int64_t)rank * BM + q * 32;
-      const int64_t n0 = (tile % n_tiles) * kCols + half * (kCols / 2);
+      const int64_t n0 = (tile % n_tiles) * kCols + part * kShare;
       const bool rows = row_base < p.M;  // warp-uniform; a tile's lower rows may be past the end
-      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN2);
-      // kDh: g and u of chunk c into buffers 2 (c & 1), 2 (c & 1) + 1
+      const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN2 + part * kShare);
+      // kDh: g and u of chunk c into the warp's two buffers
       auto issue_gu = [&](int c) {
         const int64_t nb = n0 + 32 * c;
-        if (!rows || nb >= p.N) return;
+        if (c >= kChunks || !rows || nb >= p.N) return;
         if (lane == 0) {
           bulk_wait_read_0();  // the stores that last used these buffers have read them
-          uint64_t* bar = &in_full[c & 1];
-          mbar_expect_tx(bar, 2 * 32 * kStageRow * sizeof(T));
-          tma_load_2d(buf[2 * (c & 1)], &p.in0, bar, (int)nb, (int)row_base);
-          tma_load_2d(buf[2 * (c & 1) + 1], &p.in1, bar, (int)nb, (int)row_base);
+          mbar_expect_tx(in_full, 2 * 32 * kStageRow * sizeof(T));
+          tma_load_2d(buf[0], &p.in0, in_full, (int)nb, (int)row_base);
+          tma_load_2d(buf[1], &p.in1, in_full, (int)nb, (int)row_base);
         }
-        pending |= 1u << (c & 1);
+        pending = true;
       };
       if (MODE == kDh) issue_gu(0);
       if (MODE == kDown && p.has_res && rows && n0 < p.N) {
         if (lane == 0) {
           bulk_wait_read_0();
           uint32_t chunks = 0;
-          for (int c = 0; c < 4; ++c) chunks += n0 + 32 * c < p.N;
-          mbar_expect_tx(&in_full[0], chunks * 32 * kStageRow * (uint32_t)sizeof(T));
-          for (int c = 0; c < 4; ++c)
-            if (n0 + 32 * c < p.N) tma_load_2d(buf[c], &p.in0, &in_full[0], (int)(n0 + 32 * c), (int)row_base);
+          for (int c = 0; c < kChunks; ++c) chunks += n0 + 32 * c < p.N;
+          mbar_expect_tx(in_full, chunks * 32 * kStageRow * (uint32_t)sizeof(T));
+          for (int c = 0; c < kChunks; ++c)
+            if (n0 + 32 * c < p.N) tma_load_2d(buf[c], &p.in0, in_full, (int)(n0 + 32 * c), (int)row_base);
         }
-        pending |= 1u;
+        pending = true;
       }
       if (!mbar_wait(&S.tmem_full[acc], acc_phase, abort_flag, err)) break;
       tc_fence_after();
       if (MODE == kUp) {
 #pragma unroll 1
-        for (int c = 0; c < 2; ++c) {
+        for (int c = 0; c < kChunks; ++c) {
           const int64_t nb = n0 + 32 * c;
           if (!rows || nb >= p.N) break;
           uint32_t rg[32], ru[32];
-          tmem_ld32_async(t_row + (uint32_t)(64 * half + 32 * c), rg);
-          tmem_ld32_async(t_row + (uint32_t)(128 + 64 * half + 32 * c), ru);
+          tmem_ld32_async(t_row + (uint32_t)(32 * c), rg);
+          tmem_ld32_async(t_row + (uint32_t)(128 + 32 * c), ru);
           tmem_wait_ld(rg);
           tmem_wait_ld(ru);
           float* g = reinterpret_cast<float*>(rg);
@@ -321,22 +328,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         }
       } else if (MODE == kDh) {
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < kChunks; ++c) {
           const int64_t nb = n0 + 32 * c;
           if (!rows || nb >= p.N) break;
           uint32_t r[32];
-          tmem_ld32_async(t_row + (uint32_t)(128 * half + 32 * c), r);
-          if (c + 1 < 4) issue_gu(c + 1);
-          if (!mbar_wait(&in_full[c & 1], (in_phase >> (c & 1)) & 1u, abort_flag, err)) {
+          tmem_ld32_async(t_row + (uint32_t)(32 * c), r);
+          if (!mbar_wait(in_full, in_phase, abort_flag, err)) {
             ok = false;
             tmem_wait_ld(r);
             break;
           }
-          in_phase ^= 1u << (c & 1);
-          pending &= ~(1u << (c & 1));
+          in_phase ^= 1u;
+          pending = false;
           tmem_wait_ld(r);
-          T* bg = buf[2 * (c & 1)];
-          T* bu = buf[2 * (c & 1) + 1];
+          T* bg = buf[0];
+          T* bu = buf[1];
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
             float g[8], u[8];
@@ -358,19 +364,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
             tma_store_2d(&p.out0, bg, (int)nb, (int)row_base);
             tma_store_2d(&p.out1, bu, (int)nb, (int)row_base);
           }
+          issue_gu(c + 1);
         }
       } else {
-        if (MODE == kDown && (pending & 1u)) {
-          if (!mbar_wait(&in_full[0], in_phase & 1u, abort_flag, err)) break;
+        if (MODE == kDown && pending) {
+          if (!mbar_wait(in_full, in_phase, abort_flag, err)) break;
           in_phase ^= 1u;
-          pending = 0;
+          pending = false;
         }
 #pragma unroll 1
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < kChunks; ++c) {
           const int64_t nb = n0 + 32 * c;
           if (!rows || nb >= p.N) break;
           uint32_t r[32];
-          tmem_ld32(t_row + (uint32_t)(128 * half + 32 * c), r);
+          tmem_ld32(t_row + (uint32_t)(32 * c), r);
           float* f = reinterpret_cast<float*>(r);
           if (MODE == kDown && p.bias0) add_bias32(p.bias0, p.bias_dtype, nb, p.N, f);
           if (MODE == kDown && p.has_res) {
@@ -402,10 +409,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
     if (lane == 0) {
       bulk_wait_all();
       // after an abort, input loads still in flight land before the shared memory is released
-      for (int b = 0; b < 2; ++b) {
-        if (!(pending & (1u << b))) continue;
+      if (pending) {
         const unsigned long long t0 = globaltimer();
-        while (!mbar_try_wait(&in_full[b], (in_phase >> b) & 1u) && globaltimer() - t0 < kWaitBudgetNs) {
+        while (!mbar_try_wait(in_full, in_phase) && globaltimer() - t0 < kWaitBudgetNs) {
         }
       }
     }
@@ -426,7 +432,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 template <typename T, int MODE>
 static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
-  const size_t smem = sizeof(SmemG<T>) + 1024;
+  const size_t smem = sizeof(SmemG<T, MODE>) + 1024;
   auto k = gated_kernel<T, MODE>;
   // on each call: the attribute belongs to the current device, and a runtime call has to make that device's
   // context current on this thread (an autograd thread may not have one yet) before the maps are encoded
@@ -470,7 +476,7 @@ static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
   attr[0].val.clusterDim.x = 2;
   attr[0].val.clusterDim.y = 1;
   attr[0].val.clusterDim.z = 1;
-  cfg.blockDim = dim3(kThreads, 1, 1);
+  cfg.blockDim = dim3(64 + 32 * epi_warps(MODE), 1, 1);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = s;
   cfg.attrs = attr;
@@ -930,13 +936,15 @@ static cudaError_t launch_gated_mode(const GatedArgs& a, bool dependent, cudaStr
 // ============================================================================ few tokens
 // Up to 16 tokens: the products are bound by moving the weights into the SMs once, and the tokens as often
 // as there are blocks.  A tile is the 16 rows of one mma.sync m16n8k16: 16 output rows, or, in the DUAL form,
-// the rows of Wg and of Wu of 8 hidden units, so that g and u of a unit end in one thread.  A block takes G
-// tiles (they share each token load) of a K slice, its warps split the slice in steps of 32: lane (r, t) reads
+// the rows of Wg and of Wu of 8 hidden units, so that g and u of a unit end in one thread.  A block takes one
+// tile of a K slice, its warps split the slice in steps of 32: lane (r, t) reads
 // 16 contiguous bytes, k = k0 + 8 t .. 8 t + 7, of weight row r, and of token row r for the other operand.
 // Which four of those values meet in which MMA is a permutation of k that both operands share, so the sum is
 // unchanged and every load is a full 16-byte vector.  The K slices are the CTAs of a cluster.  Partials are
 // added in warp order through shared memory, then in slice order through the cluster's shared memory
-// (deterministic).  plan_skinny picks G and the number of slices.
+// (deterministic).  Larger blocks, whose tiles share the token loads, measured slower at up to 16 tokens: what
+// counts is how many loads are in flight (1 token, 1024 x 2736, up: 3.5 us with one tile a block, 5.2 with four;
+// 11.2 MB of weights from L2, 3.2 TB/s).
 namespace gated {
 
 constexpr int SK_WARPS = 8;
@@ -990,49 +998,37 @@ __device__ __forceinline__ uint4 load8(const uint16_t* p, int left) {
   return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-template <typename T, int NT, int G, bool DUAL, bool VEC>
+template <typename T, int NT, bool DUAL, bool VEC>
 __global__ void __launch_bounds__(32 * SK_WARPS) skinny_kernel(const SkinnyParams p) {
-  constexpr int U = 4 / G;  // steps whose weight loads are in flight together
+  constexpr int U = 4;  // steps whose weight loads are in flight together
   constexpr int R = DUAL ? 8 : 16;  // output rows of a tile
   __shared__ float red[SK_WARPS][NT][32][4];
-  __shared__ float part[G][NT][32][4];
+  __shared__ float part[NT][32][4];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, t = lane & 3;
   const int slice = blockIdx.y, slices = gridDim.y;
   const int k_begin = slice * p.k_slice;
   const int k_end = min(p.K, k_begin + p.k_slice);
   const uint16_t* x = reinterpret_cast<const uint16_t*>(p.x);
-  const uint16_t *w0[G], *w1[G];
-  bool ok0[G], ok1[G];
+  const int64_t row = (int64_t)blockIdx.x * R + r, row1 = DUAL ? row : row + 8;
+  const bool ok0 = row < p.N, ok1 = row1 < p.N;
+  const uint16_t* w0 = reinterpret_cast<const uint16_t*>(p.w0) + row * p.ldw0;
+  const uint16_t* w1 = DUAL ? reinterpret_cast<const uint16_t*>(p.w1) + row * p.ldw1
+                            : reinterpret_cast<const uint16_t*>(p.w0) + row1 * p.ldw0;
+  float acc[NT][4];
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    const int64_t row = ((int64_t)blockIdx.x * G + g) * R + r;
-    const int64_t row1 = DUAL ? row : row + 8;
-    ok0[g] = row < p.N;
-    ok1[g] = row1 < p.N;
-    w0[g] = reinterpret_cast<const uint16_t*>(p.w0) + row * p.ldw0;
-    w1[g] = DUAL ? reinterpret_cast<const uint16_t*>(p.w1) + row * p.ldw1
-                 : reinterpret_cast<const uint16_t*>(p.w0) + row1 * p.ldw0;
-  }
-  float acc[G][NT][4];
+  for (int i = 0; i < NT; ++i)
 #pragma unroll
-  for (int g = 0; g < G; ++g)
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) acc[g][i][j] = 0.f;
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.f;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   bool waited = !p.dependent;
   for (int k0 = k_begin + warp * 32; k0 < k_end; k0 += SK_WARPS * 32 * U) {
-    uint4 wa[U][G], wb[U][G];
+    uint4 wa[U], wb[U];
 #pragma unroll
     for (int i = 0; i < U; ++i) {
       const int kk = k0 + i * SK_WARPS * 32 + 8 * t;
-#pragma unroll
-      for (int g = 0; g < G; ++g) {
-        wa[i][g] = load8<VEC, true>(w0[g] + kk, ok0[g] ? k_end - kk : 0);
-        wb[i][g] = load8<VEC, true>(w1[g] + kk, ok1[g] ? k_end - kk : 0);
-      }
+      wa[i] = load8<VEC, true>(w0 + kk, ok0 ? k_end - kk : 0);
+      wb[i] = load8<VEC, true>(w1 + kk, ok1 ? k_end - kk : 0);
     }
     if (!waited) {  // the weights do not depend on the kernel before; x does
       asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -1048,59 +1044,53 @@ __global__ void __launch_bounds__(32 * SK_WARPS) skinny_kernel(const SkinnyParam
         xv[n] = load8<VEC, false>(x + tok * p.ldx + kk, tok < p.M ? k_end - kk : 0);
       }
 #pragma unroll
-      for (int n = 0; n < NT; ++n)
-#pragma unroll
-        for (int g = 0; g < G; ++g) {
-          mma16816<T>(acc[g][n], wa[i][g].x, wb[i][g].x, wa[i][g].y, wb[i][g].y, xv[n].x, xv[n].y);
-          mma16816<T>(acc[g][n], wa[i][g].z, wb[i][g].z, wa[i][g].w, wb[i][g].w, xv[n].z, xv[n].w);
-        }
+      for (int n = 0; n < NT; ++n) {
+        mma16816<T>(acc[n], wa[i].x, wb[i].x, wa[i].y, wb[i].y, xv[n].x, xv[n].y);
+        mma16816<T>(acc[n], wa[i].z, wb[i].z, wa[i].w, wb[i].w, xv[n].z, xv[n].w);
+      }
     }
   }
   if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
 #pragma unroll
-  for (int g = 0; g < G; ++g) {
-    if (g) __syncthreads();
+  for (int n = 0; n < NT; ++n)
+    *reinterpret_cast<float4*>(red[warp][n][lane]) = make_float4(acc[n][0], acc[n][1], acc[n][2], acc[n][3]);
+  __syncthreads();
+  for (int i = threadIdx.x; i < NT * 32; i += 32 * SK_WARPS) {
+    const int n = i >> 5, l = i & 31;
+    float4 v = *reinterpret_cast<const float4*>(red[0][n][l]);
 #pragma unroll
-    for (int n = 0; n < NT; ++n)
-      *reinterpret_cast<float4*>(red[warp][n][lane]) =
-          make_float4(acc[g][n][0], acc[g][n][1], acc[g][n][2], acc[g][n][3]);
-    __syncthreads();
-    for (int i = threadIdx.x; i < NT * 32; i += 32 * SK_WARPS) {
-      const int n = i >> 5, l = i & 31;
-      float4 v = *reinterpret_cast<const float4*>(red[0][n][l]);
-#pragma unroll
-      for (int w = 1; w < SK_WARPS; ++w) {
-        const float4 o = *reinterpret_cast<const float4*>(red[w][n][l]);
-        v.x += o.x;
-        v.y += o.y;
-        v.z += o.z;
-        v.w += o.w;
-      }
-      *reinterpret_cast<float4*>(part[g][n][l]) = v;
+    for (int w = 1; w < SK_WARPS; ++w) {
+      const float4 o = *reinterpret_cast<const float4*>(red[w][n][l]);
+      v.x += o.x;
+      v.y += o.y;
+      v.z += o.z;
+      v.w += o.w;
     }
+    *reinterpret_cast<float4*>(part[n][l]) = v;
   }
   if (slices > 1)
     tc::cluster_sync_all();
   else
     __syncthreads();
-  // this CTA's share of the (tile, token group, lane) entries: the slices' partials in order, then the epilogue
-  const int entries = G * NT * 32;
-  for (int i = slice * (32 * SK_WARPS) + threadIdx.x; i < entries; i += slices * (32 * SK_WARPS)) {
-    const int g = i / (NT * 32), n = (i >> 5) % NT, l = i & 31;
+  // this CTA's share of the (token group, lane) entries: the slices' partials in order, then the epilogue
+  constexpr int entries = NT * 32;
+  const int share = (entries + slices - 1) / slices;
+  for (int i = slice * share + threadIdx.x; i < min(entries, (slice + 1) * share); i += 32 * SK_WARPS) {
+    const int n = i >> 5, l = i & 31;
     float4 v;
     if (slices == 1) {
-      v = *reinterpret_cast<const float4*>(part[g][n][l]);
+      v = *reinterpret_cast<const float4*>(part[n][l]);
     } else {
       v = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int c = 0; c < slices; ++c) {
-        const float4 o = tc::ld_cluster4(tc::map_rank(part[g][n][l], (uint32_t)c));
+        const float4 o = tc::ld_cluster4(tc::map_rank(part[n][l], (uint32_t)c));
         v.x += o.x;
         v.y += o.y;
         v.z += o.z;
         v.w += o.w;
       }
     }
-    const int64_t col = ((int64_t)blockIdx.x * G + g) * R + (l >> 2);
+    const int64_t col = (int64_t)blockIdx.x * R + (l >> 2);
     const int tok = 8 * n + 2 * (l & 3);
 #pragma unroll
     for (int half = 0; half < (DUAL ? 1 : 2); ++half) {
@@ -1124,34 +1114,14 @@ __global__ void __launch_bounds__(32 * SK_WARPS) skinny_kernel(const SkinnyParam
   if (slices > 1) tc::cluster_sync_all();  // the peers have read this CTA's partials
 }
 
-// G tiles a block and `slices` K slices that move the fewest bytes through the busiest SM: blocks per SM times
-// (tokens' slice + weights' slice).  A slice's exchange through the cluster's shared memory costs about as
-// much as 16 KB more (a cluster launch and two barriers; fitted at 1 and 37 tokens).
-struct SkinnyPlan {
-  int g, slices;
-};
-static SkinnyPlan plan_skinny(int64_t M, int64_t N, int64_t K, bool dual) {
-  const int64_t sms = tc::sm_count(), tiles = (N + (dual ? 7 : 15)) / (dual ? 8 : 16);
-  SkinnyPlan best = {1, 1};
-  int64_t best_cost = INT64_MAX;
-  for (int slices = 1; slices <= 8; slices *= 2) {
-    if (slices > 1 && K / slices < 32 * SK_WARPS) break;  // a step for every warp
-    for (int g = 1; g <= 4; g *= 2) {
-      if (g > 1 && (tiles + g - 1) / g * slices < sms / 2) break;
-      const int64_t blocks = (tiles + g - 1) / g * slices;
-      const int64_t bytes = 2 * (K / slices) * (M + 16 * g) + (slices > 1 ? 16384 : 0);
-      const int64_t cost = (blocks + sms - 1) / sms * bytes;
-      if (cost < best_cost) {
-        best_cost = cost;
-        best = {g, slices};
-      }
-    }
-  }
-  return best;
-}
-
-template <typename T, int NT, int G, bool DUAL>
-static cudaError_t launch_skinny_g(SkinnyParams p, int slices, bool vec, cudaStream_t s) {
+template <typename T, int NT, bool DUAL>
+static cudaError_t launch_skinny_nt(SkinnyParams p, bool vec, cudaStream_t s) {
+  constexpr int rows = DUAL ? 8 : 16;
+  // depth slices while there are fewer tiles than two an SM and every warp keeps a step
+  // (1 token, h [2736] times Wd [1024, 2736]: 5.4 us in one slice, 3.7 in four)
+  const int tiles = (p.N + rows - 1) / rows;
+  int slices = 1;
+  while (slices < 4 && 2 * slices * tiles <= 2 * tc::sm_count() && p.K / (2 * slices) >= 32 * SK_WARPS) slices *= 2;
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[2];
   int n = 0;
@@ -1165,23 +1135,14 @@ static cudaError_t launch_skinny_g(SkinnyParams p, int slices, bool vec, cudaStr
     attr[n].val.clusterDim.y = (unsigned)slices;
     attr[n++].val.clusterDim.z = 1;
   }
-  constexpr int rows = (DUAL ? 8 : 16) * G;
   p.k_slice = (p.K + 32 * slices - 1) / (32 * slices) * 32;
-  cfg.gridDim = dim3((unsigned)((p.N + rows - 1) / rows), (unsigned)slices, 1);
+  cfg.gridDim = dim3((unsigned)tiles, (unsigned)slices, 1);
   cfg.blockDim = dim3(32 * SK_WARPS, 1, 1);
   cfg.stream = s;
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  if (vec) return cudaLaunchKernelEx(&cfg, skinny_kernel<T, NT, G, DUAL, true>, p);
-  return cudaLaunchKernelEx(&cfg, skinny_kernel<T, NT, G, DUAL, false>, p);
-}
-
-template <typename T, int NT, bool DUAL>
-static cudaError_t launch_skinny_nt(const SkinnyParams& p, bool vec, cudaStream_t s) {
-  const SkinnyPlan plan = plan_skinny(p.M, p.N, p.K, DUAL);
-  if (plan.g == 1) return launch_skinny_g<T, NT, 1, DUAL>(p, plan.slices, vec, s);
-  if (plan.g == 2) return launch_skinny_g<T, NT, 2, DUAL>(p, plan.slices, vec, s);
-  return launch_skinny_g<T, NT, 4, DUAL>(p, plan.slices, vec, s);
+  if (vec) return cudaLaunchKernelEx(&cfg, skinny_kernel<T, NT, DUAL, true>, p);
+  return cudaLaunchKernelEx(&cfg, skinny_kernel<T, NT, DUAL, false>, p);
 }
 
 template <typename T, bool DUAL>
