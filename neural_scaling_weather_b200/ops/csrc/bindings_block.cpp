@@ -188,65 +188,71 @@ std::vector<Tensor> gated_mlp_fwd(const Tensor& x, const Tensor& wg, const Tenso
   return {y, xa.t, g, u, h};
 }
 
-// Weight gradient of `segs` equal row segments (and the sums of dy's columns): fp32 into the given buffers
-// (added), or fresh tensors of `dtype`.  dy [T, segs * rows_pad], x [T, n].
-void weight_grad(const Rows& dy, const Rows& x, int segs, int64_t rows, int64_t rows_pad,
-                 std::vector<OptTensor> into, std::vector<OptTensor> bias_into, bool want_bias, at::ScalarType dtype,
-                 at::ScalarType bias_dtype, std::vector<Tensor>& dw, std::vector<Tensor>& db) {
+// Gradient of one weight, or of two from the same x: a0^T x (and a1^T x), a0 / a1 [T, rows] in rows of lda.
+// fp32 into the given buffers (added), or fresh tensors of `dtype`.
+void weight_grad(const void* a0, const void* a1, int64_t lda, int64_t rows, const Rows& x, const OptTensor* into,
+                 at::ScalarType dtype, Tensor* dw) {
   const int64_t T = x.t.size(0), n = x.t.size(1);
+  const int segs = a1 ? 2 : 1;
   const auto f32 = x.t.options().dtype(at::kFloat);
-  nsw::WgradArgs a{};
-  bool inplace = rows == rows_pad, bias_inplace = rows == rows_pad && want_bias;
-  for (int i = 0; i < segs; ++i) {
-    inplace = inplace && into[i].has_value();
-    bias_inplace = bias_inplace && bias_into[i].has_value();
-  }
-  // 16-bit parameters: the kernel rounds the fp32 totals itself
-  bool out16 = dtype == x.t.scalar_type() && (!want_bias || bias_dtype == dtype);
-  for (int i = 0; i < segs; ++i) out16 = out16 && !into[i].has_value() && !(want_bias && bias_into[i].has_value());
-  const auto wopt = out16 ? x.t.options() : f32;
-  std::vector<Tensor> w(segs), b(segs);
-  for (int i = 0; i < segs; ++i) {
-    w[i] = inplace ? *into[i] : torch::empty({rows_pad, n}, wopt);
-    a.D[i] = static_cast<float*>(w[i].data_ptr());
-    if (want_bias) {
-      b[i] = bias_inplace ? *bias_into[i] : torch::empty({rows_pad}, wopt);
-      a.db[i] = static_cast<float*>(b[i].data_ptr());
-    }
-  }
-  a.out16 = a.db16 = out16;
-  a.dy = dy.ptr();
-  a.ldy = dy.ld;
-  a.x = x.ptr();
-  a.ldx = x.ld;
-  a.T = T;
-  a.M = segs * rows_pad;
-  a.N = n;
-  a.ldd = n;
-  a.seg_rows = rows_pad;
-  a.accumulate = inplace;
-  a.db_accumulate = bias_inplace;
+  bool inplace = true;
+  for (int i = 0; i < segs; ++i) inplace = inplace && into[i].has_value();
+  nsw::GatedArgs a{};
+  a.mode = nsw::kGatedDw;
   a.dtype = dt_code(x.t, "x");
-  const auto plan = nsw::wgrad_plan(a.M, a.N, a.T);
-  const int64_t wsn = nsw::wgrad_workspace_floats(a.M, a.N, plan, out16);
+  a.out_f32 = inplace || dtype != x.t.scalar_type();
+  a.accumulate = inplace;
+  Tensor w[2];
+  for (int i = 0; i < segs; ++i)
+    w[i] = inplace ? *into[i] : torch::empty({rows, n}, a.out_f32 ? f32 : x.t.options());
+  a.M = rows;
+  a.N = n;
+  a.K = T;
+  a.a0 = a0;
+  a.a1 = a1;
+  a.lda = lda;
+  a.b0 = x.ptr();
+  a.ldb0 = x.ld;
+  a.out0 = w[0].data_ptr();
+  a.out1 = a1 ? w[1].data_ptr() : nullptr;
+  a.ldout = a.ldaux = n;
+  const int64_t wsn = nsw::gated_dw_workspace(rows, n, T, segs);
   Tensor ws;
   if (wsn > 0) {
     ws = torch::empty({wsn}, f32);
     a.ws = ws.data_ptr<float>();
   }
-  check(nsw::wgrad_tcgen05(a, plan, stream()), "gated_mlp weight gradient");
-  const auto finish = [&](bool done, const Tensor& t, const OptTensor& dst, at::ScalarType dt) {
-    if (done) return Tensor();
-    const Tensor v = rows == rows_pad ? t : t.narrow(0, 0, rows);
-    if (dst) {
-      dst->view_as(v).add_(v);
-      return Tensor();
-    }
-    return v.scalar_type() == dt ? v : v.to(dt);
-  };
+  check(nsw::gated_product(a, false, stream()), "gated_mlp weight gradient");
   for (int i = 0; i < segs; ++i) {
-    dw.push_back(finish(inplace, w[i], into[i], dtype));
-    db.push_back(want_bias ? finish(bias_inplace, b[i], bias_into[i], bias_dtype) : Tensor());
+    if (inplace) continue;
+    if (into[i])
+      into[i]->add_(w[i]);
+    else
+      dw[i] = w[i].scalar_type() == dtype ? w[i] : w[i].to(dtype);
+  }
+}
+
+// Column sums of x [rows, n] as bias gradients: columns [0, seg), and with two, [off, off + seg)
+void bias_grad(const void* x, int64_t ld, int64_t rows, int64_t n, int64_t seg, int64_t off, int segs,
+               const Tensor& like, const OptTensor* into, at::ScalarType dtype, Tensor* db) {
+  const auto f32 = like.options().dtype(at::kFloat);
+  bool inplace = true;
+  for (int i = 0; i < segs; ++i) inplace = inplace && into[i].has_value();
+  const bool out_f32 = inplace || dtype != like.scalar_type();
+  Tensor b[2];
+  for (int i = 0; i < segs; ++i) b[i] = inplace ? *into[i] : torch::empty({seg}, out_f32 ? f32 : like.options());
+  const int parts = nsw::col_sum_parts(rows, n), code = dt_code(like, "x");
+  auto partial = torch::empty({parts, n}, f32);
+  check(nsw::col_partial(x, ld, rows, n, parts, partial.data_ptr<float>(), code, stream()), "gated_mlp bias gradient");
+  check(nsw::col_finish(partial.data_ptr<float>(), parts, n, seg, off, b[0].data_ptr(),
+                        segs > 1 ? b[1].data_ptr() : nullptr, code, out_f32, inplace, stream()),
+        "gated_mlp bias gradient");
+  for (int i = 0; i < segs; ++i) {
+    if (inplace) continue;
+    if (into[i])
+      into[i]->add_(b[i]);
+    else
+      db[i] = b[i].scalar_type() == dtype ? b[i] : b[i].to(dtype);
   }
 }
 
@@ -319,15 +325,13 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
     check(nsw::gated_product(b, true, stream()), "gated_mlp dx");
     out[0] = packed(dx, d.K);
   }
-  if (need_w || need_b) {
-    std::vector<Tensor> dw, db;
-    weight_grad({dgu, 2 * d.Hp}, xa, 2, d.H, d.Hp, {dw_into[0], dw_into[1]}, {db_into[0], db_into[1]}, need_b, wdt,
-                bdt, dw, db);
-    weight_grad(dya, {h.narrow(1, 0, d.H), d.Hp}, 1, d.N, d.N, {dw_into[2]}, {db_into[2]}, need_b, wdt, bdt, dw, db);
-    for (int i = 0; i < 3; ++i) {
-      out[1 + i] = dw[i];
-      out[4 + i] = db[i];
-    }
+  if (need_w) {
+    weight_grad(dgu.data_ptr(), du, 2 * d.Hp, d.H, xa, &dw_into[0], wdt, &out[1]);
+    weight_grad(dya.ptr(), nullptr, dya.ld, d.N, {h.narrow(1, 0, d.H), d.Hp}, &dw_into[2], wdt, &out[3]);
+  }
+  if (need_b) {
+    bias_grad(dgu.data_ptr(), 2 * d.Hp, d.M, 2 * d.Hp, d.H, d.Hp, 2, x, &db_into[0], bdt, &out[4]);
+    bias_grad(dya.ptr(), dya.ld, d.M, d.N, d.N, 0, 1, x, &db_into[2], bdt, &out[6]);
   }
   return out;
 }

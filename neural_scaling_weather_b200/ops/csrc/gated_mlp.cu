@@ -16,6 +16,8 @@
 //            copy exists); the epilogue loads g and u tiles by TMA and writes dg and du.
 //     kDx    dg Wg + du Wu as ONE product of depth 2 H: the k-loop runs through (dg, Wg), then
 //            (du, Wu), into the same accumulator; the weights are again read MN-major as stored.
+//     kDw    the weight gradients dg^T x, du^T x and dy^T h: both operands token-major as they are, MN-major
+//            for the MMA, the depth is the tokens.  See dw_unit for the schedule.
 // * skinny_kernel: up to 16 tokens, where the time is that of streaming the weights once.  See there.
 //
 // Sums are fp32 in TMEM / registers.  Rounded to 16 bits: g, u (kept for the backward), h, dg, du,
@@ -32,7 +34,7 @@ namespace nsw {
 namespace tc {
 
 constexpr int GS = 5;        // pipeline stages (32 KB a CTA)
-enum : int { kUp = 0, kDown = 1, kDh = 2, kDx = 3 };
+enum : int { kUp = 0, kDown = 1, kDh = 2, kDx = 3, kDw = 4 };
 // Epilogue warps and 2 KB tile buffers of each.  kDh loads two tiles and stores two for each 32 columns, more
 // latency than arithmetic: sixteen warps with one pair of buffers each (413 us with eight warps and two pairs
 // at 64800 x 2736 x 1024, KDH16 us with sixteen).
@@ -51,6 +53,52 @@ struct GatedParams {
   int act;      // 0 SiLU, 1 GELU
   int save;     // kUp: store g and u
   int has_res;  // kDown
+  // kDw: tiles of both segments (a0 -> D0, a1 -> D1), in order; see dw_unit
+  int64_t direct;
+  int rem, splits;
+  void *D0, *D1;  // out_f32: fp32 results, else 16-bit ones that the output maps cannot address (tma_out 0)
+  int64_t ldd;
+  int out_f32, accumulate, tma_out;
+  float* ws;      // [splits][rem][256][256]
+};
+
+// A pair's i-th unit of work: a tile and its range of k-blocks.  Every form but kDw: tiles pair, pair + npairs,
+// ...  kDw has few tiles and a long depth, so whole waves of tiles (`direct` of them, a multiple of the
+// pairs) are worked in full, and the depth of the `rem` tiles that are left is cut into `splits` pieces, in
+// piece-major order, whose fp32 partials go to the workspace and are added in piece order by dw_sum_kernel.
+// Pairs that run at one time read the same tokens' slab of both operands from L2.
+struct GUnit {
+  int64_t tile;
+  int kb0, kb1;
+  int64_t slot;  // partial's index, or -1
+};
+template <int MODE>
+__device__ __forceinline__ bool gated_unit(const GatedParams& p, int64_t num_tiles, int64_t pair, int64_t npairs,
+                                           int64_t i, GUnit& u) {
+  const int64_t v = pair + i * npairs;
+  u.slot = -1;
+  u.kb0 = 0;
+  u.kb1 = p.kb;
+  u.tile = v;
+  if (MODE != kDw || v < p.direct) return v < num_tiles;
+  const int64_t w = v - p.direct;
+  if (w >= (int64_t)p.rem * p.splits) return false;
+  const int64_t piece = w / p.rem;
+  u.tile = p.direct + (w - piece * p.rem);
+  u.kb0 = (int)(piece * p.kb / p.splits);
+  u.kb1 = (int)((piece + 1) * p.kb / p.splits);
+  u.slot = w;
+  return true;
+}
+
+struct DwPlan {
+  int64_t direct;
+  int rem, splits;
+};
+struct DwSum {
+  void *D0, *D1;
+  int64_t first, seg_tiles, n_tiles, M, N, ldd;
+  int rem, splits, out_f32, accumulate;
 };
 
 template <typename T, int MODE>
@@ -142,11 +190,69 @@ __device__ __forceinline__ void ring_store(const CUtensorMap* map, const float* 
   ++ring;
 }
 
+// 32 columns of one row of a weight gradient by plain stores: fp32 (added to what is there), or 16-bit rows
+// that are not 16-byte aligned
+template <typename T>
+__device__ __forceinline__ void dw_row_store(const GatedParams& p, bool seg1, int64_t row, int64_t nb, const float* f) {
+  void* D = seg1 ? p.D1 : p.D0;
+  if (p.out_f32) {
+    float* d = reinterpret_cast<float*>(D) + row * p.ldd + nb;
+    if (nb + 32 <= p.N && (p.ldd & 3) == 0) {
+#pragma unroll
+      for (int v = 0; v < 8; ++v) {
+        float4 o = make_float4(f[4 * v], f[4 * v + 1], f[4 * v + 2], f[4 * v + 3]);
+        if (p.accumulate) {
+          const float4 old = reinterpret_cast<const float4*>(d)[v];
+          o.x += old.x, o.y += old.y, o.z += old.z, o.w += old.w;
+        }
+        reinterpret_cast<float4*>(d)[v] = o;
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 32; ++j)
+        if (nb + j < p.N) d[j] = p.accumulate ? d[j] + f[j] : f[j];
+    }
+  } else {
+    T* d = reinterpret_cast<T*>(D) + row * p.ldd + nb;
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (nb + j < p.N) d[j] = from_f<T>(f[j]);
+  }
+}
+
+// The cut tiles' partials added in piece order: one block a tile row, one thread four columns.
+template <typename T>
+__global__ void dw_sum_kernel(const float* __restrict__ ws, const __grid_constant__ DwSum p) {
+  const int r = blockIdx.x >> 8, row_in = blockIdx.x & 255;
+  const int64_t tile = p.first + r;
+  const bool seg1 = tile >= p.seg_tiles;
+  const int64_t t = seg1 ? tile - p.seg_tiles : tile;
+  const int64_t row = (t / p.n_tiles) * BM2 + row_in, col = (t % p.n_tiles) * BN2 + 4 * threadIdx.x;
+  if (row >= p.M || col >= p.N) return;
+  const float* src = ws + ((int64_t)r * BM2 + row_in) * BN2 + 4 * threadIdx.x;
+  float4 a = __ldcs(reinterpret_cast<const float4*>(src));
+  for (int k = 1; k < p.splits; ++k) {
+    const float4 b = __ldcs(reinterpret_cast<const float4*>(src + (int64_t)k * p.rem * BM2 * BN2));
+    a.x += b.x, a.y += b.y, a.z += b.z, a.w += b.w;
+  }
+  const float f[4] = {a.x, a.y, a.z, a.w};
+  void* D = seg1 ? p.D1 : p.D0;
+  for (int j = 0; j < 4 && col + j < p.N; ++j) {
+    if (p.out_f32) {
+      float* d = reinterpret_cast<float*>(D) + row * p.ldd + col + j;
+      *d = p.accumulate ? *d + f[j] : f[j];
+    } else {
+      reinterpret_cast<T*>(D)[row * p.ldd + col + j] = from_f<T>(f[j]);
+    }
+  }
+}
+
 template <typename T, int MODE>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(MODE), 1)
     gated_kernel(const __grid_constant__ GatedParams p, uint32_t idesc, int* err) {
-  constexpr bool kMnB = MODE == kDh || MODE == kDx;  // B read as stored, N contiguous
-  constexpr int kCols = MODE == kUp ? 128 : 256;     // result columns of a pair tile
+  constexpr bool kMnA = MODE == kDw;                                // A read as stored, M contiguous
+  constexpr bool kMnB = MODE == kDh || MODE == kDx || MODE == kDw;  // B read as stored, N contiguous
+  constexpr int kCols = MODE == kUp ? 128 : 256;                    // result columns of a pair tile
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -157,7 +263,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
   const int64_t pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   const int64_t m_tiles = (p.M + BM2 - 1) / BM2;
   const int64_t n_tiles = (p.N + kCols - 1) / kCols;
-  const int64_t num_tiles = m_tiles * n_tiles;
+  const int64_t seg_tiles = m_tiles * n_tiles;
+  const int64_t num_tiles = MODE == kDw ? p.direct : seg_tiles;
   volatile int* abort_flag = &S.abort_flag;
 
   if (threadIdx.x == 0) {
@@ -190,16 +297,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
       const uint32_t full_leader = map_rank(&S.full[0], 0);
       int stage = 0;
       uint32_t phase = 0;
-      for (int64_t tile = pair; tile < num_tiles && !*abort_flag; tile += npairs) {
+      GUnit un;
+      for (int64_t i = 0; gated_unit<MODE>(p, num_tiles, pair, npairs, i, un) && !*abort_flag; ++i) {
+        const bool seg1 = MODE == kDw && un.tile >= seg_tiles;
+        const int64_t tile = seg1 ? un.tile - seg_tiles : un.tile;
         const int m0 = (int)((tile / n_tiles) * BM2) + (int)rank * BM;
         const int nb0 = (int)((tile % n_tiles) * kCols) + (MODE == kUp ? 0 : (int)rank * 128);
-        for (int kb = 0; kb < p.kb; ++kb) {
+        for (int kb = un.kb0; kb < un.kb1; ++kb) {
           if (!mbar_wait(&S.empty[stage], phase ^ 1, abort_flag, err)) break;
           if (rank == 0) mbar_expect_tx(&S.full[stage], (uint32_t)(2 * (BM + 128) * BK * sizeof(T)));
           const uint32_t fb = full_leader + 8u * stage;
           const bool second = MODE == kDx && kb >= p.kb0;
           const int k0 = (second ? kb - p.kb0 : kb) * BK;
-          tma_load_2d_pair(S.a[stage], second ? &p.a1 : &p.a0, fb, k0, m0);
+          if (kMnA) {
+            const CUtensorMap* ma = seg1 ? &p.a1 : &p.a0;
+            tma_load_2d_pair(&S.a[stage][0], ma, fb, m0, k0);
+            tma_load_2d_pair(&S.a[stage][64 * BK], ma, fb, m0 + 64, k0);
+          } else {
+            tma_load_2d_pair(S.a[stage], second ? &p.a1 : &p.a0, fb, k0, m0);
+          }
           if (kMnB) {
             const CUtensorMap* mb = second ? &p.b1 : &p.b0;
             tma_load_2d_pair(&S.b[stage][0], mb, fb, nb0, k0);
@@ -221,12 +337,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
       uint32_t phase = 0;
       int acc = 0;
       uint32_t acc_phase = 0;
-      for (int64_t tile = pair; tile < num_tiles && !*abort_flag; tile += npairs) {
+      GUnit un;
+      for (int64_t i = 0; gated_unit<MODE>(p, num_tiles, pair, npairs, i, un) && !*abort_flag; ++i) {
         if (!mbar_wait(&S.tmem_empty[acc], acc_phase ^ 1, abort_flag, err)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN2);
         bool ok = true;
-        for (int kb = 0; kb < p.kb; ++kb) {
+        for (int kb = un.kb0; kb < un.kb1; ++kb) {
           if (!mbar_wait(&S.full[stage], phase, abort_flag, err)) {
             ok = false;
             break;
@@ -236,7 +353,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
           for (int k = 0; k < BK / 16; ++k) {
             const uint64_t db = kMnB ? smem_desc_mn(&S.b[stage][k * 16 * 64], 64 * BK * (uint32_t)sizeof(T))
                                      : smem_desc_sw128(&S.b[stage][k * 16]);
-            umma2_f16(d_tmem, smem_desc_sw128(&S.a[stage][k * 16]), db, idesc, (kb > 0 || k > 0) ? 1u : 0u);
+            const uint64_t da = kMnA ? smem_desc_mn(&S.a[stage][k * 16 * 64], 64 * BK * (uint32_t)sizeof(T))
+                                     : smem_desc_sw128(&S.a[stage][k * 16]);
+            umma2_f16(d_tmem, da, db, idesc, (kb > un.kb0 || k > 0) ? 1u : 0u);
           }
           umma2_commit_both(&S.empty[stage]);
           if (++stage == GS) {
@@ -268,7 +387,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
     uint32_t acc_phase = 0;
     bool pending = false;  // input tiles issued and not waited for
     bool ok = true;
-    for (int64_t tile = pair; tile < num_tiles && ok; tile += npairs) {
+    GUnit un;
+    for (int64_t i = 0; ok && gated_unit<MODE>(p, num_tiles, pair, npairs, i, un); ++i) {
+      const bool seg1 = MODE == kDw && un.tile >= seg_tiles;
+      const int64_t tile = seg1 ? un.tile - seg_tiles : un.tile;
       const int64_t row_base = (tile / n_tiles) * BM2 + (int64_t)rank * BM + q * 32;
       const int64_t n0 = (tile % n_tiles) * kCols + part * kShare;
       const bool rows = row_base < p.M;  // warp-uniform; a tile's lower rows may be past the end
@@ -379,6 +501,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
           uint32_t r[32];
           tmem_ld32(t_row + (uint32_t)(32 * c), r);
           float* f = reinterpret_cast<float*>(r);
+          if (MODE == kDw && un.slot >= 0) {  // a piece's partial: this lane's row, 32 columns
+            float* w = p.ws + ((un.slot * BM2 + (int64_t)rank * BM + q * 32 + lane) * BN2 + part * kShare + 32 * c);
+#pragma unroll
+            for (int v = 0; v < 8; ++v)
+              __stcg(reinterpret_cast<float4*>(w) + v, make_float4(f[4 * v], f[4 * v + 1], f[4 * v + 2], f[4 * v + 3]));
+            continue;
+          }
+          if (MODE == kDw && !p.tma_out) {
+            const int64_t row = row_base + lane;
+            if (row < p.M) dw_row_store<T>(p, seg1, row, nb, f);
+            continue;
+          }
           if (MODE == kDown && p.bias0) add_bias32(p.bias0, p.bias_dtype, nb, p.N, f);
           if (MODE == kDown && p.has_res) {
             T* b = buf[c];
@@ -394,7 +528,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
             __syncwarp();
             if (lane == 0) tma_store_2d(&p.out0, b, (int)nb, (int)row_base);
           } else {
-            ring_store<T>(&p.out0, f, buf, lane, nb, row_base, ring);
+            ring_store<T>(MODE == kDw && seg1 ? &p.out1 : &p.out0, f, buf, lane, nb, row_base, ring);
           }
         }
       }
@@ -430,6 +564,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
     asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(2 * BN2));
 }
 
+// Whole waves of tiles, and how to cut the tiles that are left (none if they fill a wave well).  In k-block
+// steps (0.31 us a pair): a cut costs its longest pair, plus 0.26 steps a partial (256 KB written and read
+// over the device) and about 15 for the second kernel and the shorter units.
+static DwPlan dw_plan(int64_t M, int64_t N, int64_t K, int segs) {
+  const int64_t pairs = sm_count() / 2, tiles = segs * ((M + BM2 - 1) / BM2) * ((N + BN2 - 1) / BN2);
+  const int64_t kb = (K + BK - 1) / BK, left = tiles % pairs;
+  DwPlan best = {tiles, 0, 1};
+  double best_cost = (double)kb;  // one more wave
+  if (left == 0) return best;
+  for (int s = 2; s <= 16 && kb / s >= 4; ++s) {
+    const double cost = (double)((left * s + pairs - 1) / pairs * ((kb + s - 1) / s)) + 0.26 * left * s + 15.0;
+    if (cost < best_cost) {
+      best_cost = cost;
+      best = {tiles - left, (int)left, s};
+    }
+  }
+  return best;
+}
+
 template <typename T, int MODE>
 static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
   const size_t smem = sizeof(SmemG<T, MODE>) + 1024;
@@ -439,8 +592,10 @@ static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
   NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   GatedParams p;
   memset(&p, 0, sizeof(p));
-  const bool mn = MODE == kDh || MODE == kDx;
-  bool ok = make_map(&p.a0, a.a0, a.M, a.K, a.lda, BM, a.dtype);
+  const bool mn = MODE == kDh || MODE == kDx || MODE == kDw;
+  bool ok = MODE == kDw ? make_map_mn(&p.a0, a.a0, a.K, a.M, a.lda, a.dtype)
+                        : make_map(&p.a0, a.a0, a.M, a.K, a.lda, BM, a.dtype);
+  if (MODE == kDw && a.a1) ok = ok && make_map_mn(&p.a1, a.a1, a.K, a.M, a.lda, a.dtype);
   if (MODE == kDx) ok = ok && make_map(&p.a1, a.a1, a.M, a.K, a.lda, BM, a.dtype);
   if (mn) {
     ok = ok && make_map_mn(&p.b0, a.b0, a.K, a.N, a.ldb0, a.dtype);
@@ -451,8 +606,10 @@ static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
   }
   if (a.in0) ok = ok && make_store_map(&p.in0, const_cast<void*>(a.in0), a.M, a.N, a.ldin, a.dtype);
   if (a.in1) ok = ok && make_store_map(&p.in1, const_cast<void*>(a.in1), a.M, a.N, a.ldin, a.dtype);
-  ok = ok && make_store_map(&p.out0, a.out0, a.M, a.N, a.ldout, a.dtype);
-  if (a.out1) ok = ok && make_store_map(&p.out1, a.out1, a.M, a.N, a.ldaux, a.dtype);
+  p.tma_out = MODE != kDw || (!a.out_f32 && a.ldout % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out0) & 15) == 0 &&
+                              (reinterpret_cast<uintptr_t>(a.out1) & 15) == 0);
+  if (p.tma_out) ok = ok && make_store_map(&p.out0, a.out0, a.M, a.N, a.ldout, a.dtype);
+  if (a.out1 && p.tma_out) ok = ok && make_store_map(&p.out1, a.out1, a.M, a.N, a.ldaux, a.dtype);
   if (a.out2) ok = ok && make_store_map(&p.out2, a.out2, a.M, a.N, a.ldaux, a.dtype);
   if (!ok) return cudaErrorInvalidValue;
   p.M = a.M;
@@ -466,10 +623,25 @@ static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
   p.save = MODE == kUp && a.out1 != nullptr;
   p.has_res = MODE == kDown && a.in0 != nullptr;
   const uint32_t fmt = a.dtype == kBF16 ? 1u : 0u;
-  const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (mn ? 1u << 16 : 0u) | ((uint32_t)(BN2 >> 3) << 17) |
+  const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (MODE == kDw ? 1u << 15 : 0u) | (mn ? 1u << 16 : 0u) | ((uint32_t)(BN2 >> 3) << 17) |
                          ((uint32_t)(BM2 >> 4) << 24);
   const int cols = MODE == kUp ? 128 : 256;
-  const int64_t tiles = ((a.M + BM2 - 1) / BM2) * ((a.N + cols - 1) / cols);
+  const int64_t seg_tiles = ((a.M + BM2 - 1) / BM2) * ((a.N + cols - 1) / cols);
+  int64_t tiles = seg_tiles;
+  if (MODE == kDw) {
+    const DwPlan plan = dw_plan(a.M, a.N, a.K, a.a1 ? 2 : 1);
+    p.direct = plan.direct;
+    p.rem = plan.rem;
+    p.splits = plan.splits;
+    p.D0 = a.out0;
+    p.D1 = a.out1;
+    p.ldd = a.ldout;
+    p.out_f32 = a.out_f32;
+    p.accumulate = a.accumulate;
+    p.ws = a.ws;
+    if (plan.rem > 0 && !a.ws) return cudaErrorInvalidValue;
+    tiles = std::max<int64_t>(plan.direct, (int64_t)plan.rem * plan.splits);
+  }
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -491,6 +663,11 @@ static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
   const int pairs = tiles < max_pairs ? (int)tiles : max_pairs;
   cfg.gridDim = dim3(2 * pairs, 1, 1);
   NSW_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, p, idesc, device_error_flag()));
+  if (MODE == kDw && p.rem > 0) {
+    const DwSum d = {a.out0, a.out1, p.direct, seg_tiles, (a.N + cols - 1) / cols, a.M, a.N, a.ldout,
+                     p.rem,  p.splits, a.out_f32, a.accumulate};
+    dw_sum_kernel<T><<<p.rem * 256, 64, 0, s>>>(a.ws, d);
+  }
   return cudaGetLastError();
 }
 
@@ -927,6 +1104,7 @@ static cudaError_t launch_gated_mode(const GatedArgs& a, bool dependent, cudaStr
     case kGatedDown: return launch_any<T, kDown>(a, dependent, s);
     case kGatedDh: return launch_any<T, kDh>(a, dependent, s);
     case kGatedDx: return launch_any<T, kDx>(a, dependent, s);
+    case kGatedDw: return launch_gated<T, kDw>(a, s);
   }
   return cudaErrorInvalidValue;
 }
@@ -1160,7 +1338,97 @@ __global__ void pad_copy_kernel(const uint16_t* __restrict__ src, int64_t s0, in
   }
 }
 
+// Column sums of a 16-bit [rows, n] matrix (rows 16-byte aligned, ld >= round8(n)): partial[y][c] over the
+// y-th slice of the rows; a warp takes 256 columns of a row, 16 bytes a lane.
+template <typename T>
+__global__ void __launch_bounds__(256) col_partial_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t n,
+                                                          float* __restrict__ partial) {
+  __shared__ float red[8][256];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t c = (int64_t)blockIdx.x * 256 + lane * 8;
+  float a[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) a[j] = 0.f;
+  if (c < n) {
+#pragma unroll 4
+    for (int64_t r = (int64_t)blockIdx.y * 8 + warp; r < rows; r += (int64_t)gridDim.y * 8) {
+      float f[8];
+      unpack8<T>(__ldg(reinterpret_cast<const uint4*>(x + r * ld + c)), f);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) a[j] += f[j];
+    }
+  }
+#pragma unroll
+  for (int j = 0; j < 8; ++j) red[warp][lane * 8 + j] = a[j];
+  __syncthreads();
+  float v = red[0][threadIdx.x];
+#pragma unroll
+  for (int w = 1; w < 8; ++w) v += red[w][threadIdx.x];
+  const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (col < n) partial[(int64_t)blockIdx.y * n + col] = v;
+}
+
+// out[c] (+)= sum of partial[0 .. parts)[c], in order; columns [0, seg) go to out0, [off, off + seg) to out1
+struct ColFinish {
+  const float* partial;
+  int64_t parts, n, seg, off;
+  void *out0, *out1;
+  int f32, accumulate;
+};
+template <typename T>
+__global__ void __launch_bounds__(256) col_finish_kernel(const __grid_constant__ ColFinish p) {
+  __shared__ float red[8][33];
+  const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+  const int64_t c = (int64_t)blockIdx.x * 32 + lane;
+  float a = 0.f;
+  if (c < p.n)
+    for (int64_t r = w; r < p.parts; r += 8) a += p.partial[r * p.n + c];
+  red[w][lane] = a;
+  __syncthreads();
+  if (w || c >= p.n) return;
+  for (int i = 1; i < 8; ++i) a += red[i][lane];
+  const bool second = p.out1 && c >= p.off;
+  const int64_t at = second ? c - p.off : c;
+  void* out = second ? p.out1 : p.out0;
+  if (at >= p.seg || !out) return;
+  if (p.f32) {
+    float* o = reinterpret_cast<float*>(out) + at;
+    *o = p.accumulate ? *o + a : a;
+  } else {
+    reinterpret_cast<T*>(out)[at] = from_f<T>(a);
+  }
+}
+
 }  // namespace gated
+
+int col_sum_parts(int64_t rows, int64_t n) {
+  const int64_t cols = (n + 255) / 256;
+  return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 31) / 32, 4 * (int64_t)tc::sm_count() / cols));
+}
+cudaError_t col_partial(const void* x, int64_t ld, int64_t rows, int64_t n, int parts, float* partial, int dtype,
+                        cudaStream_t s) {
+  const dim3 grid((unsigned)((n + 255) / 256), (unsigned)parts, 1);
+  if (dtype == kBF16)
+    gated::col_partial_kernel<<<grid, 256, 0, s>>>(reinterpret_cast<const __nv_bfloat16*>(x), ld, rows, n, partial);
+  else
+    gated::col_partial_kernel<<<grid, 256, 0, s>>>(reinterpret_cast<const __half*>(x), ld, rows, n, partial);
+  return cudaGetLastError();
+}
+cudaError_t col_finish(const float* partial, int64_t parts, int64_t n, int64_t seg, int64_t off, void* out0, void* out1,
+                       int dtype, bool f32, bool accumulate, cudaStream_t s) {
+  const gated::ColFinish p = {partial, parts, n, seg, off, out0, out1, f32, accumulate};
+  const int blocks = (int)((n + 31) / 32);
+  if (dtype == kBF16)
+    gated::col_finish_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(p);
+  else
+    gated::col_finish_kernel<__half><<<blocks, 256, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+int64_t gated_dw_workspace(int64_t M, int64_t N, int64_t K, int segs) {
+  const tc::DwPlan p = tc::dw_plan(M, N, K, segs);
+  return (int64_t)p.rem * p.splits * tc::BM2 * tc::BN2;
+}
 
 cudaError_t gated_product(const GatedArgs& a, bool dependent, cudaStream_t s) {
   if ((a.dtype != kBF16 && a.dtype != kF16) || a.M <= 0 || a.N <= 0 || a.K <= 0) return cudaErrorInvalidValue;

@@ -1134,10 +1134,7 @@ struct WgradParams {
   int64_t ldd;
   int accumulate;     // D += result
   int db_accumulate;  // db += sums
-  int splits;         // S of the uniform split, or the remainder pieces of the balanced one
-  int slots;          // partial slots: splits, and one more where direct_slot is used
-  int out16, db16;    // D / db in the operands' 16-bit type (each element rounded once, from the fp32 total)
-  int direct_slot;    // >= 0: the balanced schedule's first part also goes to a slot (16-bit D cannot be added to)
+  int splits;         // partial slots: S of the uniform split, or the remainder pieces of the balanced one
   int k1;             // 0: uniform split; > 0: balanced (see wg_unit)
   float* ws;          // partials [splits][M_pad][N_pad], then feature sums [splits][M_pad]
   int64_t m_pad;      // M rounded up to the pair tile
@@ -1175,7 +1172,7 @@ __device__ __forceinline__ bool wg_unit(const WgradParams& wp, int64_t tiles, in
     u.tile = pair;
     u.kb0 = 0;
     u.kb1 = wp.k1;
-    u.slot = wp.direct_slot;
+    u.slot = -1;
     return true;
   }
   const int64_t ps = npairs - tiles;
@@ -1356,20 +1353,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           uint32_t r[32];
           tmem_ld32(trow + (uint32_t)(128 * half + 32 * c), r);
           const int64_t col = n0 + 32 * c;
-          if (wp.out16) {
-            if (row_ok && col < N) {
-              T* dp = reinterpret_cast<T*>(wp.D[seg]) + lrow * wp.ldd + col;
-              if (col + 32 <= N && (wp.ldd & 7) == 0) {
-#pragma unroll
-                for (int v = 0; v < 4; ++v)
-                  reinterpret_cast<uint4*>(dp)[v] = pack8<T>(reinterpret_cast<const float*>(&r[8 * v]));
-              } else {
-#pragma unroll
-                for (int j = 0; j < 32; ++j)
-                  if (col + j < N) dp[j] = from_f<T>(__uint_as_float(r[j]));
-              }
-            }
-          } else if (row_ok && col < N) {
+          if (row_ok && col < N) {
             float* dp = wp.D[seg] + lrow * wp.ldd + col;
             if (col + 32 <= N && (wp.ldd & 3) == 0) {
 #pragma unroll
@@ -1396,9 +1380,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
           uint32_t r[32];
           tmem_ld32(trow + 256u, r);
           sum_v = __uint_as_float(r[0]);
-          if (row_ok && wp.db16) {
-            reinterpret_cast<T*>(wp.db[seg])[lrow] = from_f<T>(sum_v);
-          } else if (row_ok) {
+          if (row_ok) {
             float* bp = wp.db[seg] + lrow;
             *bp = wp.db_accumulate ? *bp + sum_v : sum_v;
           }
@@ -1423,7 +1405,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
         if (sums && half == 0) {
           uint32_t r[32];
           tmem_ld32(trow + 256u, r);
-          __stcg(wp.ws + (int64_t)wp.slots * wp.m_pad * wp.n_pad + (int64_t)un.slot * wp.m_pad + prow_i,
+          __stcg(wp.ws + (int64_t)wp.splits * wp.m_pad * wp.n_pad + (int64_t)un.slot * wp.m_pad + prow_i,
                  __uint_as_float(r[0]));
         }
         tc_fence_before();
@@ -1449,10 +1431,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kThreads, 1)
 
 // D[m, n] (+)= sum_s ws[s][m][n] in split order; db[m] (+)= sum_s sums[s][m].  One thread per four
 // consecutive columns of a row (scalar at a ragged edge).
-template <typename T>
 __global__ void wgrad_reduce_kernel(const float* __restrict__ ws, int64_t M, int64_t N,
                                     const __grid_constant__ WgradParams wp, int accumulate, int db_accumulate) {
-  const int splits = wp.slots;
+  const int splits = wp.splits;
   const int64_t m_pad = wp.m_pad, n_pad = wp.n_pad, ldd = wp.ldd;
   const int64_t n4 = (N + 3) / 4;
   const int64_t total = M * n4;
@@ -1461,27 +1442,8 @@ __global__ void wgrad_reduce_kernel(const float* __restrict__ ws, int64_t M, int
     const int64_t m = i / n4, c = (i - m * n4) * 4;
     const int seg = (int)(m / wp.seg_rows);
     const float* p = ws + m * n_pad + c;
-    const int64_t at = (m - (int64_t)seg * wp.seg_rows) * ldd + c;
-    float* dp = wp.D[seg] + at;
-    if (wp.out16) {
-      T* hp = reinterpret_cast<T*>(wp.D[seg]) + at;
-      float f[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int sp = 0; sp < splits; ++sp) {
-        const float4 x = __ldcs(reinterpret_cast<const float4*>(p + sp * plane));
-        f[0] += x.x;
-        f[1] += x.y;
-        f[2] += x.z;
-        f[3] += x.w;
-      }
-      if (c + 4 <= N && (ldd & 3) == 0) {
-        T h[4] = {from_f<T>(f[0]), from_f<T>(f[1]), from_f<T>(f[2]), from_f<T>(f[3])};
-        uint2 w;
-        memcpy(&w, h, 8);
-        *reinterpret_cast<uint2*>(hp) = w;
-      } else {
-        for (int j = 0; j < 4 && c + j < N; ++j) hp[j] = from_f<T>(f[j]);
-      }
-    } else if (c + 4 <= N && (ldd & 3) == 0) {
+    float* dp = wp.D[seg] + (m - (int64_t)seg * wp.seg_rows) * ldd + c;
+    if (c + 4 <= N && (ldd & 3) == 0) {
       float4 acc = __ldcs(reinterpret_cast<const float4*>(p));
       for (int sp = 1; sp < splits; ++sp) {
         const float4 x = __ldcs(reinterpret_cast<const float4*>(p + sp * plane));
@@ -1512,11 +1474,8 @@ __global__ void wgrad_reduce_kernel(const float* __restrict__ ws, int64_t M, int
       float acc = sums[m];
       for (int sp = 1; sp < splits; ++sp) acc += sums[sp * m_pad + m];
       const int seg = (int)(m / wp.seg_rows);
-      const int64_t at = m - (int64_t)seg * wp.seg_rows;
-      if (wp.db16)
-        reinterpret_cast<T*>(wp.db[seg])[at] = from_f<T>(acc);
-      else
-        wp.db[seg][at] = db_accumulate ? wp.db[seg][at] + acc : acc;
+      float* bp = wp.db[seg] + (m - (int64_t)seg * wp.seg_rows);
+      *bp = db_accumulate ? *bp + acc : acc;
     }
   }
 }
@@ -1578,11 +1537,6 @@ static cudaError_t launch_wgrad(const WgradArgs& a, int pairs_plan, cudaStream_t
   wp.db_accumulate = a.db_accumulate;
   wp.splits = a.splits;
   wp.k1 = a.k1;
-  wp.out16 = a.out16;
-  wp.db16 = a.db16;
-  // a 16-bit result is rounded once, from the total: the balanced schedule's first part joins the pieces
-  wp.direct_slot = a.k1 > 0 && (a.out16 || a.db16) ? a.splits : -1;
-  wp.slots = a.splits + (wp.direct_slot >= 0 ? 1 : 0);
   wp.ws = a.ws;
   wp.m_pad = (a.M + BM2 - 1) / BM2 * BM2;
   wp.n_pad = (a.N + BN2 - 1) / BN2 * BN2;
@@ -1616,9 +1570,8 @@ static cudaError_t launch_wgrad(const WgradArgs& a, int pairs_plan, cudaStream_t
     const int64_t work = a.M * ((a.N + 3) / 4);
     const int blocks = (int)std::min<int64_t>((work + 255) / 256, 8 * sm_count());
     // balanced: the direct part already holds D (with the caller's accumulate), the pieces add to it
-    const bool add = a.k1 > 0 && wp.direct_slot < 0;
-    wgrad_reduce_kernel<T><<<blocks, 256, 0, s>>>(a.ws, a.M, a.N, wp, add ? 1 : a.accumulate,
-                                                  add ? 1 : a.db_accumulate);
+    wgrad_reduce_kernel<<<blocks, 256, 0, s>>>(a.ws, a.M, a.N, wp, a.k1 > 0 ? 1 : a.accumulate,
+                                               a.k1 > 0 ? 1 : a.db_accumulate);
   }
   return cudaGetLastError();
 }
@@ -1696,7 +1649,6 @@ int wgrad_tcgen05_supported(const WgradArgs& a) {
   if (a.T <= 0 || a.M <= 0 || a.N <= 0 || !a.D[0] || a.ldd < a.N) return 0;
   const int64_t seg = a.seg_rows > 0 ? a.seg_rows : a.M;
   if ((a.M + seg - 1) / seg > 4) return 0;
-  if ((a.out16 && a.accumulate) || (a.db16 && a.db_accumulate) || (a.db[0] && !a.out16 != !a.db16)) return 0;
   for (int i = 0; i < (int)((a.M + seg - 1) / seg); ++i)
     if (!a.D[i] || ((a.db[0] != nullptr) != (a.db[i] != nullptr))) return 0;
   if (a.ldy % 8 || a.ldx % 8 || a.ldy < a.M || a.ldx < a.N) return 0;  // 16-byte TMA strides
@@ -1753,9 +1705,9 @@ WgradPlan wgrad_plan(int64_t M, int64_t N, int64_t T) {
   return plan;
 }
 
-int64_t wgrad_workspace_floats(int64_t M, int64_t N, const WgradPlan& plan, bool out16) {
-  const int splits = plan.splits + (out16 && plan.k1 > 0 ? 1 : 0);
-  if (plan.splits <= 1 && plan.k1 == 0) return 0;
+int64_t wgrad_workspace_floats(int64_t M, int64_t N, const WgradPlan& plan) {
+  const int splits = plan.splits;
+  if (splits <= 1 && plan.k1 == 0) return 0;
   const int64_t m_pad = (M + tc::BM2 - 1) / tc::BM2 * tc::BM2, n_pad = (N + tc::BN2 - 1) / tc::BN2 * tc::BN2;
   return (int64_t)splits * m_pad * (n_pad + 1);
 }

@@ -152,8 +152,7 @@ struct WgradArgs {
   float* db[4];  // db[0] null: no bias gradient
   int db_accumulate;
   int dtype;
-  int out16, db16;  // D / db point to the operands' 16-bit type instead of fp32 (both or neither; no accumulate)
-  float* ws;   // wgrad_workspace_floats(M, N, plan, out16) floats (none needed when that is 0)
+  float* ws;   // wgrad_workspace_floats(M, N, plan) floats (none needed when that is 0)
   int splits;  // set from the plan
   int k1;      // set from the plan
 };
@@ -164,7 +163,7 @@ struct WgradPlan {
   int splits, k1, pairs;
 };
 WgradPlan wgrad_plan(int64_t M, int64_t N, int64_t T);
-int64_t wgrad_workspace_floats(int64_t M, int64_t N, const WgradPlan& plan, bool out16 = false);
+int64_t wgrad_workspace_floats(int64_t M, int64_t N, const WgradPlan& plan);
 int wgrad_tcgen05_supported(const WgradArgs& a);
 cudaError_t wgrad_tcgen05(const WgradArgs& a, const WgradPlan& plan, cudaStream_t s);
 
@@ -177,7 +176,9 @@ cudaError_t wgrad_tcgen05(const WgradArgs& a, const WgradPlan& plan, cudaStream_
 //   kGatedDh    d = a0 b0 with b0 [K, N]; out0 = d * in1 * act'(in0), out1 = d * act(in0) (in: g, u, ldin;
 //               out0 in rows of ldout, out1 in rows of ldaux)
 //   kGatedDx    out0 = a0 b0 + a1 b1 with b0, b1 [K, N]
-enum GatedMode : int { kGatedUp = 0, kGatedDown = 1, kGatedDh = 2, kGatedDx = 3 };
+//   kGatedDw    out0 (+)= a0^T b0, and with a1: out1 (+)= a1^T b0 (depth K = tokens; a0, a1 [K, M] rows of lda,
+//               b0 [K, N]); 16-bit or (out_f32) fp32 results in rows of ldout; ws: gated_dw_workspace floats
+enum GatedMode : int { kGatedUp = 0, kGatedDown = 1, kGatedDh = 2, kGatedDx = 3, kGatedDw = 4 };
 struct GatedArgs {
   int mode, dtype, act;  // act: 0 SiLU, 1 GELU
   int64_t M, N, K;
@@ -191,7 +192,18 @@ struct GatedArgs {
   int64_t ldin;
   void *out0, *out1, *out2;
   int64_t ldout, ldaux;
+  int out_f32, accumulate;  // kGatedDw (accumulate: fp32 only)
+  float* ws;
 };
+int64_t gated_dw_workspace(int64_t M, int64_t N, int64_t K, int segs);
+// Column sums: partial [parts][n] of a 16-bit matrix whose rows are 16-byte aligned (ld >= n rounded up to 8),
+// and their sums; columns [0, seg) to out0 and [off, off + seg) to out1 (may be null), fp32 (f32; added with
+// accumulate) or in dtype
+int col_sum_parts(int64_t rows, int64_t n);
+cudaError_t col_partial(const void* x, int64_t ld, int64_t rows, int64_t n, int parts, float* partial, int dtype,
+                        cudaStream_t s);
+cudaError_t col_finish(const float* partial, int64_t parts, int64_t n, int64_t seg, int64_t off, void* out0, void* out1,
+                       int dtype, bool f32, bool accumulate, cudaStream_t s);
 // dependent: the A operand is written by the kernel before it on the stream, which this one may overlap (a
 // programmatic dependent launch: it waits for that kernel before it touches anything but the weights)
 cudaError_t gated_product(const GatedArgs& a, bool dependent, cudaStream_t s);
