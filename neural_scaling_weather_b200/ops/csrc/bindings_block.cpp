@@ -232,18 +232,24 @@ void weight_grad(const void* a0, const void* a1, int64_t lda, int64_t rows, cons
   }
 }
 
-// Column sums of x [rows, n] as bias gradients: columns [0, seg), and with two, [off, off + seg)
+// Column sums of x [rows, n] as bias gradients: columns [0, seg), and with two, [off, off + seg); `sums`: the
+// sums of groups of rows where a kernel already has them
 void bias_grad(const void* x, int64_t ld, int64_t rows, int64_t n, int64_t seg, int64_t off, int segs,
-               const Tensor& like, const OptTensor* into, at::ScalarType dtype, Tensor* db) {
+               const Tensor& sums, const Tensor& like, const OptTensor* into, at::ScalarType dtype, Tensor* db) {
   const auto f32 = like.options().dtype(at::kFloat);
   bool inplace = true;
   for (int i = 0; i < segs; ++i) inplace = inplace && into[i].has_value();
   const bool out_f32 = inplace || dtype != like.scalar_type();
   Tensor b[2];
   for (int i = 0; i < segs; ++i) b[i] = inplace ? *into[i] : torch::empty({seg}, out_f32 ? f32 : like.options());
-  const int parts = nsw::col_sum_parts(rows, n), code = dt_code(like, "x");
-  auto partial = torch::empty({parts, n}, f32);
-  check(nsw::col_partial(x, ld, rows, n, parts, partial.data_ptr<float>(), code, stream()), "gated_mlp bias gradient");
+  const int code = dt_code(like, "x");
+  int64_t parts = sums.defined() ? sums.size(0) : nsw::col_sum_parts(rows, n);
+  Tensor partial = sums;
+  if (!sums.defined()) {
+    partial = torch::empty({parts, n}, f32);
+    check(nsw::col_partial(x, ld, rows, n, (int)parts, partial.data_ptr<float>(), code, stream()),
+          "gated_mlp bias gradient");
+  }
   check(nsw::col_finish(partial.data_ptr<float>(), parts, n, seg, off, b[0].data_ptr(),
                         segs > 1 ? b[1].data_ptr() : nullptr, code, out_f32, inplace, stream()),
         "gated_mlp bias gradient");
@@ -304,6 +310,15 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
   a.out0 = dgu.data_ptr();
   a.out1 = du;
   a.ldout = a.ldaux = 2 * d.Hp;
+  Tensor sums;
+  if (need_b) {
+    const int64_t rows = nsw::gated_sum_rows(a);
+    if (rows > 0) {
+      sums = torch::empty({rows, 2 * d.Hp}, opt.dtype(at::kFloat));
+      a.sums = sums.data_ptr<float>();
+      a.sums_half = d.Hp;
+    }
+  }
   check(nsw::gated_product(a, false, stream()), "gated_mlp dh");
   if (need_dx) {
     auto dx = torch::empty({d.M, round8(d.K)}, opt);
@@ -330,8 +345,8 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
     weight_grad(dya.ptr(), nullptr, dya.ld, d.N, {h.narrow(1, 0, d.H), d.Hp}, &dw_into[2], wdt, &out[3]);
   }
   if (need_b) {
-    bias_grad(dgu.data_ptr(), 2 * d.Hp, d.M, 2 * d.Hp, d.H, d.Hp, 2, x, &db_into[0], bdt, &out[4]);
-    bias_grad(dya.ptr(), dya.ld, d.M, d.N, d.N, 0, 1, x, &db_into[2], bdt, &out[6]);
+    bias_grad(dgu.data_ptr(), 2 * d.Hp, d.M, 2 * d.Hp, d.H, d.Hp, 2, sums, x, &db_into[0], bdt, &out[4]);
+    bias_grad(dya.ptr(), dya.ld, d.M, d.N, d.N, 0, 1, Tensor(), x, &db_into[2], bdt, &out[6]);
   }
   return out;
 }

@@ -33,13 +33,13 @@
 namespace nsw {
 namespace tc {
 
-constexpr int GS = 5;        // pipeline stages (32 KB a CTA)
 enum : int { kUp = 0, kDown = 1, kDh = 2, kDx = 3, kDw = 4 };
 // Epilogue warps and 2 KB tile buffers of each.  kDh loads two tiles and stores two for each 32 columns, more
 // latency than arithmetic: sixteen warps with one pair of buffers each (413 us with eight warps and two pairs
 // at 64800 x 2736 x 1024, KDH16 us with sixteen).
 constexpr int epi_warps(int mode) { return mode == kDh ? 16 : 8; }
 constexpr int epi_bufs(int mode) { return mode == kDh ? 2 : 4; }
+constexpr int stages(int mode) { return mode == kDh ? 4 : 5; }  // 32 KB a CTA; kDh's column sums take one
 
 struct GatedParams {
   CUtensorMap a0, a1, b0, b1;    // operands (a1 / b1: Wu in kUp, the second half of the depth in kDx)
@@ -60,6 +60,9 @@ struct GatedParams {
   int64_t ldd;
   int out_f32, accumulate, tma_out;
   float* ws;      // [splits][rem][256][256]
+  // kDh: column sums of the rounded dg and du over each CTA's 128 rows, [2 m_tiles][2 sums_half] (null: none)
+  float* sums;
+  int64_t sums_half;
 };
 
 // A pair's i-th unit of work: a tile and its range of k-blocks.  Every form but kDw: tiles pair, pair + npairs,
@@ -103,10 +106,11 @@ struct DwSum {
 
 template <typename T, int MODE>
 struct SmemG {
-  static constexpr int EW = epi_warps(MODE);
+  static constexpr int EW = epi_warps(MODE), GS = stages(MODE);
   alignas(1024) T a[GS][BM * BK];
   alignas(1024) T b[GS][128 * BK];
   alignas(1024) T buf[EW][epi_bufs(MODE)][32 * kStageRow];
+  float sums[MODE == kDh ? 2 : 1][MODE == kDh ? 4 : 1][MODE == kDh ? 512 : 1];  // [tile parity][32 rows][column]
   uint64_t full[GS], empty[GS];
   uint64_t tmem_full[2], tmem_empty[2];
   uint64_t in_full[EW];
@@ -174,6 +178,17 @@ __device__ __forceinline__ void add_bias32(const void* p, int dtype, int64_t nb,
 }
 
 __device__ __forceinline__ void bulk_wait_read_3() { asm volatile("cp.async.bulk.wait_group.read 3;" ::: "memory"); }
+
+// named barrier that also ANDs a predicate over its threads
+__device__ __forceinline__ bool bar_and(int id, int threads, bool v) {
+  uint32_t out;
+  asm volatile(
+      "{\n .reg .pred p, q;\n setp.ne.u32 p, %1, 0;\n bar.red.and.pred q, %3, %2, p;\n selp.u32 %0, 1, 0, q;\n}\n"
+      : "=r"(out)
+      : "r"(v ? 1u : 0u), "r"(threads), "r"(id)
+      : "memory");
+  return out != 0;
+}
 
 // this lane's row of a 32 x 32 tile into the warp's next buffer (ring of four), then one TMA store
 template <typename T>
@@ -256,7 +271,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
   extern __shared__ __align__(1024) unsigned char smem_raw[];
   unsigned char* base = reinterpret_cast<unsigned char*>(
       (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  constexpr int EW = epi_warps(MODE);
+  constexpr int EW = epi_warps(MODE), GS = stages(MODE);
   auto& S = *reinterpret_cast<SmemG<T, MODE>*>(base);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -419,7 +434,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
         }
         pending = true;
       }
-      if (!mbar_wait(&S.tmem_full[acc], acc_phase, abort_flag, err)) break;
+      if (!mbar_wait(&S.tmem_full[acc], acc_phase, abort_flag, err)) {
+        if (MODE != kDh) break;
+        ok = false;  // kDh: the warps leave together, below
+      }
       tc_fence_after();
       if (MODE == kUp) {
 #pragma unroll 1
@@ -450,9 +468,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
         }
       } else if (MODE == kDh) {
 #pragma unroll 1
-        for (int c = 0; c < kChunks; ++c) {
+        for (int c = 0; c < kChunks && ok; ++c) {
           const int64_t nb = n0 + 32 * c;
-          if (!rows || nb >= p.N) break;
+          float* sums = &S.sums[i & 1][q][part * kShare + 32 * c];
+          if (!rows || nb >= p.N) {
+            if (p.sums) sums[lane] = sums[lane + 256] = 0.f;
+            continue;
+          }
           uint32_t r[32];
           tmem_ld32_async(t_row + (uint32_t)(32 * c), r);
           if (!mbar_wait(in_full, in_phase, abort_flag, err)) {
@@ -485,6 +507,28 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
           if (lane == 0) {
             tma_store_2d(&p.out0, bg, (int)nb, (int)row_base);
             tma_store_2d(&p.out1, bu, (int)nb, (int)row_base);
+          }
+          if (p.sums) {
+            // the tiles' column sums: lane l adds columns 2 (l % 16), 2 (l % 16) + 1 of the rows of l / 16's parity
+            float a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+              const int at = stg_off(2 * k + (lane >> 4), (lane & 15) >> 2) + 2 * (lane & 3);
+              float x[2];
+              unpack2(*reinterpret_cast<const uint32_t*>(bg + at), x, T());
+              a[0] += x[0];
+              a[1] += x[1];
+              unpack2(*reinterpret_cast<const uint32_t*>(bu + at), x, T());
+              a[2] += x[0];
+              a[3] += x[1];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) a[k] += __shfl_xor_sync(0xffffffffu, a[k], 16);
+            if (lane < 16) {
+              *reinterpret_cast<float2*>(sums + 2 * lane) = make_float2(a[0], a[1]);
+              *reinterpret_cast<float2*>(sums + 256 + 2 * lane) = make_float2(a[2], a[3]);
+            }
+            __syncwarp();  // the buffers have been read: the next tiles may land in them
           }
           issue_gu(c + 1);
         }
@@ -534,10 +578,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(empty_leader + 8u * acc);
+      if (lane == 0 && ok) mbar_arrive_cluster(empty_leader + 8u * acc);
       if (++acc == 2) {
         acc = 0;
         acc_phase ^= 1;
+      }
+      if constexpr (MODE == kDh) {
+        if (!p.sums) continue;
+        // the four 32-row groups of these columns; the other parity's sums are untouched until every warp has
+        // been through the next tile's barrier.  A warp that gave up makes all of them leave.
+        ok = bar_and(1 + part, 128, ok);
+        const int t = q * 32 + lane;  // 64 columns of dg, then of du
+        const int col = part * kShare + (t & 63);
+        const int64_t at = (tile % n_tiles) * kCols + col;
+        if (ok && at < p.N) {
+          const float(*v)[512] = S.sums[i & 1];
+          const int k = col + 256 * (t >> 6);
+          const int64_t m = (tile / n_tiles) * 2 + rank;
+          p.sums[m * 2 * p.sums_half + (t >> 6) * p.sums_half + at] = ((v[0][k] + v[1][k]) + v[2][k]) + v[3][k];
+        }
       }
     }
     if (lane == 0) {
@@ -620,6 +679,8 @@ static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
   p.bias1 = a.bias1;
   p.bias_dtype = a.bias_dtype;
   p.act = a.act;
+  p.sums = MODE == kDh ? a.sums : nullptr;
+  p.sums_half = a.sums_half;
   p.save = MODE == kUp && a.out1 != nullptr;
   p.has_res = MODE == kDown && a.in0 != nullptr;
   const uint32_t fmt = a.dtype == kBF16 ? 1u : 0u;
@@ -1428,6 +1489,10 @@ cudaError_t col_finish(const float* partial, int64_t parts, int64_t n, int64_t s
 int64_t gated_dw_workspace(int64_t M, int64_t N, int64_t K, int segs) {
   const tc::DwPlan p = tc::dw_plan(M, N, K, segs);
   return (int64_t)p.rem * p.splits * tc::BM2 * tc::BN2;
+}
+
+int64_t gated_sum_rows(const GatedArgs& a) {
+  return a.mode == kGatedDh && !tc::plan_split(a).use ? 2 * ((a.M + tc::BM2 - 1) / tc::BM2) : 0;
 }
 
 cudaError_t gated_product(const GatedArgs& a, bool dependent, cudaStream_t s) {

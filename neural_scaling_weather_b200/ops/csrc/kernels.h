@@ -194,7 +194,12 @@ struct GatedArgs {
   int64_t ldout, ldaux;
   int out_f32, accumulate;  // kGatedDw (accumulate: fp32 only)
   float* ws;
+  // kGatedDh, where gated_sum_rows(args) > 0: that many rows of 2 sums_half column sums, of out0 at [0, N), of
+  // out1 at [sums_half, sums_half + N) (null: none)
+  float* sums;
+  int64_t sums_half;
 };
+int64_t gated_sum_rows(const GatedArgs& a);
 int64_t gated_dw_workspace(int64_t M, int64_t N, int64_t K, int segs);
 // Column sums: partial [parts][n] of a 16-bit matrix whose rows are 16-byte aligned (ld >= n rounded up to 8),
 // and their sums; columns [0, seg) to out0 and [off, off + seg) to out1 (may be null), fp32 (f32; added with
