@@ -12,6 +12,12 @@ Architecture and parameter layout follow the reference (``models/swin.py:36-323`
   latitude wrap (longitude is periodic and unmasked);
 * a linear head and unpatchify; only the last time step is returned.
 
+Two options that the reference does not have (defaults keep its blocks and parameter names):
+``mlp_type`` "swiglu" or "geglu" replaces the GELU MLP with a gated feed-forward network of hidden width
+``int(dim * mlp_ratio)`` (``mlp_ratio`` 8/3 has about the parameters of the GELU MLP's 4), and
+``block_norm`` "sandwich" also normalises each branch's output and adds it through a learned gate per
+channel: ``x + gate * rms_norm(branch(rms_norm(x)))``.
+
 The B200 design departs from the reference's data flow, not its math:
 
 * q/k/v are one fused GEMM (the three weights keep their own parameters and names);
@@ -119,11 +125,54 @@ class MLP(nn.Module):
         return y if residual is None else y + residual
 
 
+class GatedMLP(nn.Module):
+    """Gated feed-forward network ``down(act(gate(x)) * up(x))`` with biases; gate and up column-parallel, down
+    row-parallel over tp."""
+
+    ACTIVATIONS = {"swiglu": "silu", "geglu": "gelu"}
+
+    def __init__(self, in_features, hidden_features, mlp_type: str = "swiglu", drop: float = 0.0):
+        super().__init__()
+        tp = comm.get_size("tp")
+        if hidden_features % tp:
+            raise AssertionError(f"cannot shard MLP hidden {hidden_features} into {tp} shards")
+        hl = hidden_features // tp
+        col = lambda: _meta(["tp", None], ["sp1-sp2"], ["sp1-sp2"])  # noqa: E731
+        colb = lambda: _meta(["tp"], ["sp1-sp2"], ["sp1-sp2"])  # noqa: E731
+        self.gate = LinearLayer(in_features, hl, comm_metadata=col())
+        self.biasgate = BiasLayer(hl, comm_metadata=colb())
+        self.up = LinearLayer(in_features, hl, comm_metadata=col())
+        self.biasup = BiasLayer(hl, comm_metadata=colb())
+        self.down = LinearLayer(hl, in_features, comm_metadata=_meta([None, "tp"], ["sp1-sp2"], ["sp1-sp2"]))
+        self.biasdown = BiasLayer(in_features, comm_metadata=_meta([], ["tp-sp1-sp2"], ["sp1-sp2"]))
+        self.activation = self.ACTIVATIONS[mlp_type]
+        self.drop = drop
+
+    @profile("mlp")
+    def forward(self, x, residual: Optional[torch.Tensor] = None):
+        drop = self.drop > 0 and self.training
+        if comm.get_size("tp") == 1 and not drop:
+            return ops.gated_mlp(x, self.gate.weight, self.up.weight, self.down.weight, self.biasgate.bias,
+                                 self.biasup.bias, self.biasdown.bias, residual=residual, activation=self.activation)
+        g = ops.linear_colparallel(x, self.gate.weight, self.biasgate.bias, group="tp")
+        u = ops.linear_colparallel(x, self.up.weight, self.biasup.bias, group="tp")
+        h = (F.silu(g) if self.activation == "silu" else F.gelu(g)) * u
+        if not drop:
+            return ops.linear_allreduce(h, self.down.weight, self.biasdown.bias, residual=residual, group="tp")
+        y = ops.linear_allreduce(F.dropout(h, self.drop, True), self.down.weight, self.biasdown.bias, group="tp")
+        y = F.dropout(y, self.drop, True)
+        return y if residual is None else y + residual
+
+
 class Block(nn.Module):
     def __init__(self, dim, num_heads, feat_size, window_size, temporal_context_window_size,
                  shift_size=(0, 0), mlp_ratio=4.0, drop=0.0, act_layer=nn.GELU,
-                 sp1_shapes=None, sp2_shapes=None):
+                 sp1_shapes=None, sp2_shapes=None, mlp_type: str = "gelu", block_norm: str = "pre"):
         super().__init__()
+        if mlp_type != "gelu" and mlp_type not in GatedMLP.ACTIVATIONS:
+            raise ValueError(f"mlp_type {mlp_type!r} is not 'gelu' or one of {sorted(GatedMLP.ACTIVATIONS)}")
+        if block_norm not in ("pre", "sandwich"):
+            raise ValueError(f"block_norm {block_norm!r} is neither 'pre' nor 'sandwich'")
         self.dim = dim
         self.feat_size = tuple(feat_size)
         self.window_size = tuple(window_size)
@@ -141,7 +190,15 @@ class Block(nn.Module):
         self.norm1 = NormLayer(dim, norm_type="rms_norm", comm_metadata=norm_meta())
         self.attn = WindowMultiHeadAttention(dim, num_heads=num_heads, window_size=window_size)
         self.norm2 = NormLayer(dim, norm_type="rms_norm", comm_metadata=norm_meta())
-        self.mlp = MLP(dim, hidden_features=int(dim * mlp_ratio), act_layer=act_layer, drop=drop)
+        hidden = int(dim * mlp_ratio)
+        self.mlp = (MLP(dim, hidden_features=hidden, act_layer=act_layer, drop=drop) if mlp_type == "gelu"
+                    else GatedMLP(dim, hidden, mlp_type, drop))
+        if block_norm == "sandwich":
+            for i in (1, 2):
+                setattr(self, f"post_norm{i}", NormLayer(dim, norm_type="rms_norm", comm_metadata=norm_meta()))
+                gate = nn.Parameter(torch.ones(dim))
+                gate.comm_metadata = norm_meta()
+                self.register_parameter(f"branch_gate{i}", gate)
         # global row offset of this rank's shard (patch units), for the wrap mask
         self.row_offset = offsets(self.sp1_shapes)[comm.get_rank("sp1")]
         self.h_global = sum(self.sp1_shapes)
@@ -197,6 +254,13 @@ class Block(nn.Module):
         h, skip = self._norm_skip(self.norm2, x)
         return self.mlp(h, residual=skip)
 
+    def forward_sandwich(self, x: torch.Tensor, normed: torch.Tensor, next_weight: Optional[torch.Tensor]):
+        """The stream ``x`` and its norm for this block -> the stream after the block and its norm for the next
+        one (None without ``next_weight``).  Everything between two branches is one operator."""
+        a = self._shifted_window_attn(normed, None)
+        x, normed = ops.norm_gate_residual(a, x, self.post_norm1.weight, self.branch_gate1, self.norm2.weight)
+        return ops.norm_gate_residual(self.mlp(normed), x, self.post_norm2.weight, self.branch_gate2, next_weight)
+
     @staticmethod
     def _norm_skip(norm, x):
         if norm.norm_type == "rms_norm":
@@ -224,6 +288,8 @@ class SwinTransformer(nn.Module):
             mlp_ratio=cfg.model.mlp_ratio,
             drop_rate=cfg.model.dropout,
             coord_pos_embed=getattr(cfg.model, "coord_pos_embed", True),
+            mlp_type=getattr(cfg.model, "mlp_type", "gelu"),
+            block_norm=getattr(cfg.model, "block_norm", "pre"),
             use_transformer_engine=getattr(cfg.parallelism, "use_transformer_engine", True),
             domain_metadata=domain_metadata,
         )
@@ -231,7 +297,8 @@ class SwinTransformer(nn.Module):
     def __init__(self, temporal_context_window_size=1, window_size=(9, 9), patch_size=16,
                  in_chans=3, out_chans=3, embed_dim=768, depth=12, num_heads=12, mlp_ratio=4.0,
                  drop_rate=0.0, coord_pos_embed=True, domain_metadata=None,
-                 use_transformer_engine=True, use_big_skip_conv=False, **kwargs):
+                 use_transformer_engine=True, use_big_skip_conv=False, mlp_type="gelu", block_norm="pre",
+                 **kwargs):
         super().__init__()
         if domain_metadata is None:
             raise AssertionError("the data loader must provide domain metadata")
@@ -244,6 +311,7 @@ class SwinTransformer(nn.Module):
         self.coord_pos_embed = coord_pos_embed
         self.domain_metadata = domain_metadata
         self.use_big_skip_conv = use_big_skip_conv
+        self.block_norm = block_norm
         sp1_shapes, sp2_shapes = domain_metadata["sp_shapes"]
         shared = lambda: _meta([], ["tp-sp1-sp2"], ["sp1-sp2"])  # noqa: E731
 
@@ -267,7 +335,7 @@ class SwinTransformer(nn.Module):
                   shift_size=tuple(0 if i % 2 == 0 else w // 2 for w in self.window_size),
                   mlp_ratio=mlp_ratio, drop=drop_rate,
                   sp1_shapes=self.patch_embed.sp1_patch_shapes,
-                  sp2_shapes=self.patch_embed.sp2_patch_shapes)
+                  sp2_shapes=self.patch_embed.sp2_patch_shapes, mlp_type=mlp_type, block_norm=block_norm)
             for i in range(depth)
         ])
         self.out_size = out_chans * patch_size * patch_size
@@ -321,8 +389,13 @@ class SwinTransformer(nn.Module):
         b, t, c, h, w = x.shape
         skip = x if self.use_big_skip_conv else None
         x = self.prepare_tokens(x)
-        for blk in self.blocks:
-            x = blk(x)
+        if self.block_norm == "sandwich":
+            normed = ops.rms_norm(x, self.blocks[0].norm1.weight)
+            for blk, following in zip(self.blocks, [*self.blocks[1:], None]):
+                x, normed = blk.forward_sandwich(x, normed, None if following is None else following.norm1.weight)
+        else:
+            for blk in self.blocks:
+                x = blk(x)
         x = self.forward_head(x)
         if self.use_big_skip_conv:
             s = self.skip_conv(skip.reshape(b * t, c, h, w)).view(b, t, self.out_chans, h, w)

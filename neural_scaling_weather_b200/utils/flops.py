@@ -30,6 +30,13 @@ def mlp_flops(batchseq, embed, hidden):
     return (fc1 + act + fc2) * TFLOPS
 
 
+def gated_mlp_flops(batchseq, embed, hidden):
+    """Three products with biases, the activation (8 an element, as above) and the gate's product."""
+    up = 2 * (2 * batchseq * embed * hidden + batchseq * hidden)
+    down = 2 * batchseq * hidden * embed + batchseq * embed
+    return (up + 9 * batchseq * hidden + down) * TFLOPS
+
+
 def patch_embed_flops(batch, h, w, c, patch_size, embed):
     seq = h // patch_size * w // patch_size
     return (2 * batch * h * w * c * embed + batch * seq * embed) * TFLOPS
@@ -58,6 +65,10 @@ class FlopsCalculator:
         self.num_windows = self.h_patch // self.wh * self.w_patch // self.ww
         self.c_in, self.c_out = c_in, c_out
         self.params_backbone = 0.0
+        # the options beside the reference's block: a gated network of hidden width int(embed * ratio), and two
+        # more norms (the gate and skip are counted with them, 3 an element)
+        self.gated_hidden = (0 if getattr(m, "mlp_type", "gelu") == "gelu" else int(m.embed_dim * m.mlp_ratio))
+        self.extra_norms = 4 if getattr(m, "block_norm", "pre") == "sandwich" else 0
 
     def flops(self, verbose: bool = False) -> float:
         """Forward TFLOPs of one micro-batch."""
@@ -66,9 +77,10 @@ class FlopsCalculator:
         pos = patch_embed_flops(bt, self.h, self.w, 4, self.patch_size, self.embed)
         attn = attention_flops(self.batch * self.num_windows, self.seq, self.embed, self.heads)
         ntok = bt * self.h_patch * self.w_patch
-        mlp = mlp_flops(ntok, self.embed, 4 * self.embed)
+        mlp = (gated_mlp_flops(ntok, self.embed, self.gated_hidden) if self.gated_hidden
+               else mlp_flops(ntok, self.embed, 4 * self.embed))
         norm = rms_norm_flops(ntok * self.embed)
-        block = attn + mlp + 4 * norm
+        block = attn + mlp + (4 + self.extra_norms) * norm
         head = head_flops(self.batch, self.h, self.w, self.embed, self.patch_size, self.c_out)
         if verbose:
             print(f"patch {patch} pos {pos} attn {attn} mlp {mlp} norm {norm} block {block} head {head} TFLOP")
@@ -78,7 +90,8 @@ class FlopsCalculator:
         e, p = self.embed, self.patch_size
         patch = e * self.c_in * p * p + e
         pos = e * 4 * p * p + e
-        block = e * e * 3 + e * e + e * 4 * e * 2 + e * 4
+        ffn = 3 * e * self.gated_hidden if self.gated_hidden else e * 4 * e * 2
+        block = e * e * 3 + e * e + ffn + e * (4 + self.extra_norms)
         head = self.c_out * e * p * p
         self.params_backbone = block * self.depth * 1e-6
         return (patch + pos + block * self.depth + head) * 1e-6

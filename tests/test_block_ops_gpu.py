@@ -419,3 +419,70 @@ def test_clip_grad_norm_refusals():
         ops.clip_grad_norm([g[0], torch.ones(3)], 1.0)
     with pytest.raises(RuntimeError, match="dtype"):
         ops.clip_grad_norm([torch.ones(3, device=DEV, dtype=torch.float64)], 1.0)
+
+
+# --------------------------------------------------------------------------- in the model
+def test_model_with_gated_networks_and_sandwich_norms_matches_cpu():
+    """The tolerances of the plain model's comparison (tests/test_model_gpu.py): bf16 activations through two
+    blocks against fp32."""
+    from neural_scaling_weather_b200 import config as C
+    from neural_scaling_weather_b200.models import get_model
+    from neural_scaling_weather_b200.utils.misc import create_dummy_metadata
+
+    torch.manual_seed(0)
+    cfg = C.create(dict(
+        model=dict(arch="swin", embed_dim=64, patch_size=2, depth=2, window_size=[4, 8], num_heads=4, dropout=0.0,
+                   mlp_ratio=8 / 3, coord_pos_embed=True, mlp_type="swiglu", block_norm="sandwich"),
+        data=dict(invariants=["a"]), train=dict(temporal_context_window=1, num_rollout_steps=2),
+        parallelism=dict(use_transformer_engine=False)))
+    md = create_dummy_metadata(32, 64, 5)
+    cpu = get_model(cfg, md)
+    gpu = get_model(cfg, md).cuda()
+    gpu.load_state_dict(cpu.state_dict())
+    x, y = torch.randn(2, 1, 6, 32, 64), torch.randn(2, 2, 5, 32, 64)
+    out_c = cpu(x)
+    ((out_c - y) ** 2).mean().backward()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        out_g = gpu(x.cuda())
+    ((out_g.float() - y.cuda()) ** 2).mean().backward()
+    assert rel(out_g.cpu(), out_c) < 3e-2
+    grads = dict(cpu.named_parameters())
+    for name, p in gpu.named_parameters():
+        assert p.grad is not None and rel(p.grad.cpu(), grads[name].grad) < 8e-2, name
+
+
+def test_trainer_with_gated_blocks_and_cuda_graphs(tmp_path):
+    """Four training steps of the options through the trainer, from captured micro-batches."""
+    import os
+
+    from neural_scaling_weather_b200 import config as C
+    from neural_scaling_weather_b200.training.trainer import Trainer
+
+    os.environ["MASTER_PORT"] = "29541"
+    t = Trainer(C.compose("default", [
+        f"hydra.run.dir={tmp_path}", "parallelism.backend=nccl", "model.embed_dim=64", "model.depth=2",
+        "model.num_heads=4", "model.window_size=[4,8]", "model.patch_size=2", "data.synthetic.nlat=32",
+        "data.synthetic.nlon=64", "data.synthetic.n_samples=40", "data.levels=[500]", "data.batch_size=2",
+        "optimizer=adamw", "optimizer.max_iterations=4", "train.log_every=2", "train.amp_dtype=bf16",
+        "train.clip_grad_norm=1.0", "logging.log_to_wandb=false", "train.seed=1", "train.cuda_graphs=true",
+        "model.mlp_type=swiglu", "model.block_norm=sandwich", "model.mlp_ratio=2.6667"]))
+    t.launch()
+    assert t.iters == 4 and all(torch.isfinite(p).all() for p in t.model.parameters())
+    import torch.distributed as dist
+
+    dist.destroy_process_group()
+
+
+def test_example_training_step_on_gpu():
+    import os
+    import sys
+
+    sys.path.insert(0, os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples"))
+    import train_gated_block as ex
+
+    torch.manual_seed(0)
+    model = ex.build(128, 2, (36, 72), 4, DEV, torch.bfloat16)
+    losses, norms = ex.train(model, 8, (36, 72), 4)
+    assert torch.isfinite(losses).all() and torch.isfinite(norms).all() and losses[-1] < losses[0]
+    out = ex.rollout(model, torch.randn(1, 1, 4, 36, 72, device=DEV).bfloat16(), 2)
+    assert torch.isfinite(out).all()
