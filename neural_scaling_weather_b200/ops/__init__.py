@@ -22,7 +22,7 @@ from typing import Optional, Sequence, Union
 
 import torch
 
-from . import reference
+from . import fused, reference
 from ._ext import available as extension_available
 from ._ext import require as require_extension
 from .geometry import WindowGeometry
@@ -157,17 +157,10 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     stored.  Calls without gradients of at most 16 rows take kernels that stream the weights once."""
     if activation not in GATED_ACTIVATIONS:
         raise ValueError(f"gated_mlp: activation {activation!r} is not one of {GATED_ACTIVATIONS}")
-    H, K = w_gate.shape
-    if x.shape[-1] != K or w_up.shape != w_gate.shape or w_down.shape[1:] != (H,):
-        raise ValueError(f"gated_mlp: x {tuple(x.shape)}, w_gate {tuple(w_gate.shape)}, w_up {tuple(w_up.shape)} "
-                         f"and w_down {tuple(w_down.shape)} do not fit together")
-    if residual is not None and residual.shape != x.shape[:-1] + w_down.shape[:1]:
-        raise ValueError(f"gated_mlp: residual {tuple(residual.shape)} is not the output's shape")
-    if not _use_cuda(x):
-        return reference.gated_mlp(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, activation)
-    from .fused import gated_mlp_cuda
-
-    return gated_mlp_cuda(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, activation)
+    if _use_cuda(x):  # checks the shapes itself
+        return fused.gated_mlp_cuda(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, activation)
+    fused.check_gated_shapes(x, w_gate, w_up, w_down, residual)
+    return reference.gated_mlp(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, activation)
 
 
 def norm_gate_residual(y: torch.Tensor, skip: torch.Tensor, w_post: torch.Tensor,
@@ -179,6 +172,8 @@ def norm_gate_residual(y: torch.Tensor, skip: torch.Tensor, w_post: torch.Tensor
     ``y`` (a branch's output) and ``skip`` (..., D); ``w_post``, ``w_next`` (D,); ``gate`` (D,), or one row for
     each index of the first dimension (samples, D), or None for ones.  ``n`` is None without ``w_next`` (the
     last branch of a network)."""
+    if _use_cuda(y):  # checks the shapes itself
+        return fused.norm_gate_residual_cuda(y, skip, w_post, gate, w_next, skip_scale, eps)
     D = y.shape[-1]
     if y.dim() < 2 or skip.shape != y.shape:
         raise ValueError(f"norm_gate_residual: y {tuple(y.shape)} and skip {tuple(skip.shape)} must be of one shape "
@@ -187,11 +182,7 @@ def norm_gate_residual(y: torch.Tensor, skip: torch.Tensor, w_post: torch.Tensor
         raise ValueError(f"norm_gate_residual: w_post and w_next must be ({D},)")
     if gate is not None and gate.shape not in ((D,), (y.shape[0], D)):
         raise ValueError(f"norm_gate_residual: gate {tuple(gate.shape)} is neither ({D},) nor ({y.shape[0]}, {D})")
-    if not _use_cuda(y):
-        return reference.norm_gate_residual(y, skip, w_post, gate, w_next, skip_scale, eps)
-    from .fused import norm_gate_residual_cuda
-
-    return norm_gate_residual_cuda(y, skip, w_post, gate, w_next, skip_scale, eps)
+    return reference.norm_gate_residual(y, skip, w_post, gate, w_next, skip_scale, eps)
 
 
 def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float,

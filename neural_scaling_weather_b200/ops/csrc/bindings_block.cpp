@@ -188,79 +188,20 @@ std::vector<Tensor> gated_mlp_fwd(const Tensor& x, const Tensor& wg, const Tenso
   return {y, xa.t, g, u, h};
 }
 
-// Gradient of one weight, or of two from the same x: a0^T x (and a1^T x), a0 / a1 [T, rows] in rows of lda.
-// fp32 into the given buffers (added), or fresh tensors of `dtype`.
-void weight_grad(const void* a0, const void* a1, int64_t lda, int64_t rows, const Rows& x, const OptTensor* into,
-                 at::ScalarType dtype, Tensor* dw) {
-  const int64_t T = x.t.size(0), n = x.t.size(1);
-  const int segs = a1 ? 2 : 1;
-  const auto f32 = x.t.options().dtype(at::kFloat);
-  bool inplace = true;
-  for (int i = 0; i < segs; ++i) inplace = inplace && into[i].has_value();
-  nsw::GatedArgs a{};
-  a.mode = nsw::kGatedDw;
-  a.dtype = dt_code(x.t, "x");
-  a.out_f32 = inplace || dtype != x.t.scalar_type();
-  a.accumulate = inplace;
-  Tensor w[2];
-  for (int i = 0; i < segs; ++i)
-    w[i] = inplace ? *into[i] : torch::empty({rows, n}, a.out_f32 ? f32 : x.t.options());
-  a.M = rows;
-  a.N = n;
-  a.K = T;
-  a.a0 = a0;
-  a.a1 = a1;
-  a.lda = lda;
-  a.b0 = x.ptr();
-  a.ldb0 = x.ld;
-  a.out0 = w[0].data_ptr();
-  a.out1 = a1 ? w[1].data_ptr() : nullptr;
-  a.ldout = a.ldaux = n;
-  const int64_t wsn = nsw::gated_dw_workspace(rows, n, T, segs);
-  Tensor ws;
-  if (wsn > 0) {
-    ws = torch::empty({wsn}, f32);
-    a.ws = ws.data_ptr<float>();
+// Where a parameter's gradient goes: added into the given fp32 buffer, or a fresh tensor (16-bit where that is
+// the parameter's type, else fp32 and cast at the end)
+struct GradOut {
+  Tensor t;
+  bool f32, into;
+  GradOut(const OptTensor& dst, at::IntArrayRef sizes, const Tensor& like, at::ScalarType dtype)
+      : f32(dst.has_value() || dtype != like.scalar_type()), into(dst.has_value()) {
+    t = into ? *dst : torch::empty(sizes, f32 ? like.options().dtype(at::kFloat) : like.options());
   }
-  check(nsw::gated_product(a, false, stream()), "gated_mlp weight gradient");
-  for (int i = 0; i < segs; ++i) {
-    if (inplace) continue;
-    if (into[i])
-      into[i]->add_(w[i]);
-    else
-      dw[i] = w[i].scalar_type() == dtype ? w[i] : w[i].to(dtype);
+  Tensor result(at::ScalarType dtype) const {
+    if (into) return Tensor();
+    return t.scalar_type() == dtype ? t : t.to(dtype);
   }
-}
-
-// Column sums of x [rows, n] as bias gradients: columns [0, seg), and with two, [off, off + seg); `sums`: the
-// sums of groups of rows where a kernel already has them
-void bias_grad(const void* x, int64_t ld, int64_t rows, int64_t n, int64_t seg, int64_t off, int segs,
-               const Tensor& sums, const Tensor& like, const OptTensor* into, at::ScalarType dtype, Tensor* db) {
-  const auto f32 = like.options().dtype(at::kFloat);
-  bool inplace = true;
-  for (int i = 0; i < segs; ++i) inplace = inplace && into[i].has_value();
-  const bool out_f32 = inplace || dtype != like.scalar_type();
-  Tensor b[2];
-  for (int i = 0; i < segs; ++i) b[i] = inplace ? *into[i] : torch::empty({seg}, out_f32 ? f32 : like.options());
-  const int code = dt_code(like, "x");
-  int64_t parts = sums.defined() ? sums.size(0) : nsw::col_sum_parts(rows, n);
-  Tensor partial = sums;
-  if (!sums.defined()) {
-    partial = torch::empty({parts, n}, f32);
-    check(nsw::col_partial(x, ld, rows, n, (int)parts, partial.data_ptr<float>(), code, stream()),
-          "gated_mlp bias gradient");
-  }
-  check(nsw::col_finish(partial.data_ptr<float>(), parts, n, seg, off, b[0].data_ptr(),
-                        segs > 1 ? b[1].data_ptr() : nullptr, code, out_f32, inplace, stream()),
-        "gated_mlp bias gradient");
-  for (int i = 0; i < segs; ++i) {
-    if (inplace) continue;
-    if (into[i])
-      into[i]->add_(b[i]);
-    else
-      db[i] = b[i].scalar_type() == dtype ? b[i] : b[i].to(dtype);
-  }
-}
+};
 
 // Gradients from dy and what the forward saved: {dx, dwg, dwu, dwd, dbg, dbu, dbd}.  An entry is undefined
 // where it was not asked for (need_dx, need_w, need_b) or was added into the given fp32 buffer.
@@ -341,12 +282,42 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
     out[0] = packed(dx, d.K);
   }
   if (need_w) {
-    weight_grad(dgu.data_ptr(), du, 2 * d.Hp, d.H, xa, &dw_into[0], wdt, &out[1]);
-    weight_grad(dya.ptr(), nullptr, dya.ld, d.N, {h.narrow(1, 0, d.H), d.Hp}, &dw_into[2], wdt, &out[3]);
+    const GradOut g0(dw_into[0], {d.H, d.K}, x, wdt), g1(dw_into[1], {d.H, d.K}, x, wdt),
+        g2(dw_into[2], {d.N, d.H}, x, wdt);
+    nsw::GatedDwArgs w{};
+    w.dtype = a.dtype;
+    w.T = d.M;
+    w.w[0] = {dgu.data_ptr(), xa.ptr(), 2 * d.Hp, xa.ld, d.H, d.K, g0.t.data_ptr(), g0.f32, g0.into};
+    w.w[1] = {du, xa.ptr(), 2 * d.Hp, xa.ld, d.H, d.K, g1.t.data_ptr(), g1.f32, g1.into};
+    w.w[2] = {dya.ptr(), h.data_ptr(), dya.ld, d.Hp, d.N, d.H, g2.t.data_ptr(), g2.f32, g2.into};
+    Tensor ws;
+    const int64_t wsn = nsw::gated_dw_workspace(w);
+    if (wsn > 0) {
+      ws = torch::empty({wsn}, opt.dtype(at::kFloat));
+      w.ws = ws.data_ptr<float>();
+    }
+    check(nsw::gated_dw(w, stream()), "gated_mlp weight gradients");
+    out[1] = g0.result(wdt);
+    out[2] = g1.result(wdt);
+    out[3] = g2.result(wdt);
   }
   if (need_b) {
-    bias_grad(dgu.data_ptr(), 2 * d.Hp, d.M, 2 * d.Hp, d.H, d.Hp, 2, sums, x, &db_into[0], bdt, &out[4]);
-    bias_grad(dya.ptr(), dya.ld, d.M, d.N, d.N, 0, 1, Tensor(), x, &db_into[2], bdt, &out[6]);
+    const GradOut g0(db_into[0], {d.H}, x, bdt), g1(db_into[1], {d.H}, x, bdt), g2(db_into[2], {d.N}, x, bdt);
+    const int64_t n = 2 * d.Hp, pd = nsw::col_sum_parts(d.M, d.N), pg = sums.defined() ? 0 : nsw::col_sum_parts(d.M, n);
+    auto partial = torch::empty({pd * d.N + pg * n}, opt.dtype(at::kFloat));
+    float* pp = partial.data_ptr<float>();
+    const nsw::ColSource src[2] = {{dya.ptr(), dya.ld, d.M, d.N, pd, pp},
+                                   {dgu.data_ptr(), n, d.M, n, pg, pp + pd * d.N}};
+    check(nsw::col_partial(src, pg > 0 ? 2 : 1, a.dtype, stream()), "gated_mlp bias gradients");
+    const float* ps = pg > 0 ? src[1].partial : sums.data_ptr<float>();
+    const int64_t rows = pg > 0 ? pg : sums.size(0);
+    const nsw::ColSum fin[3] = {{ps, rows, n, 0, d.H, g0.t.data_ptr(), g0.f32, g0.into},
+                                {ps, rows, n, d.Hp, d.H, g1.t.data_ptr(), g1.f32, g1.into},
+                                {pp, pd, d.N, 0, d.N, g2.t.data_ptr(), g2.f32, g2.into}};
+    check(nsw::col_finish(fin, a.dtype, stream()), "gated_mlp bias gradients");
+    out[4] = g0.result(bdt);
+    out[5] = g1.result(bdt);
+    out[6] = g2.result(bdt);
   }
   return out;
 }
@@ -406,9 +377,17 @@ struct GatedNode : public torch::autograd::Function<GatedNode> {
   }
 };
 
-// x (..., K) and residual (..., N) in the weights' 16-bit type
+// x (..., K) and residual (..., N) in the weights' 16-bit type (the public entry point on CUDA, which leaves the
+// checks of the shapes to this function)
 Tensor gated_mlp(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd, const OptTensor& bg,
                  const OptTensor& bu, const OptTensor& bd, const OptTensor& residual, int64_t act) {
+  TORCH_CHECK_VALUE(x.dim() >= 1 && wg.dim() == 2 && wd.dim() == 2 && wu.sizes() == wg.sizes() &&
+                        x.size(-1) == wg.size(1) && wd.size(1) == wg.size(0),
+                    "gated_mlp: x ", x.sizes(), ", w_gate ", wg.sizes(), ", w_up ", wu.sizes(), " and w_down ",
+                    wd.sizes(), " do not fit together");
+  TORCH_CHECK_VALUE(!residual || (residual->dim() == x.dim() && residual->size(-1) == wd.size(0) &&
+                                  residual->sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1)),
+                    "gated_mlp: residual ", residual->sizes(), " is not the output's shape");
   bool grad = false;
   if (at::GradMode::is_enabled()) {
     for (const Tensor* t : {&x, &wg, &wu, &wd}) grad = grad || t->requires_grad();
@@ -551,9 +530,17 @@ struct NormGateNode : public torch::autograd::Function<NormGateNode> {
   }
 };
 
-// y, skip (..., D) of one 16-bit type; fp32 vectors
+// y, skip (..., D) of one 16-bit type; fp32 vectors (as above: the shapes are checked here)
 std::vector<Tensor> norm_gate(const Tensor& y, const Tensor& skip, const Tensor& wp, const OptTensor& gate,
                               const OptTensor& wn, double skip_scale, double eps) {
+  const int64_t n = y.dim() ? y.size(-1) : 0;
+  TORCH_CHECK_VALUE(y.dim() >= 2 && skip.sizes() == y.sizes(), "norm_gate_residual: y ", y.sizes(), " and skip ",
+                    skip.sizes(), " must be of one shape (..., D)");
+  TORCH_CHECK_VALUE(wp.dim() == 1 && wp.size(0) == n && (!wn || (wn->dim() == 1 && wn->size(0) == n)),
+                    "norm_gate_residual: w_post and w_next must be (", n, ",)");
+  TORCH_CHECK_VALUE(!gate || ((gate->dim() == 1 || (gate->dim() == 2 && gate->size(0) == y.size(0))) &&
+                              gate->size(-1) == n),
+                    "norm_gate_residual: gate ", gate->sizes(), " is neither (", n, ",) nor (", y.size(0), ", ", n, ")");
   bool grad = false;
   if (at::GradMode::is_enabled()) {
     for (const Tensor* t : {&y, &skip, &wp}) grad = grad || t->requires_grad();

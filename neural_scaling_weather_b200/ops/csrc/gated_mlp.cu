@@ -38,11 +38,21 @@ enum : int { kUp = 0, kDown = 1, kDh = 2, kDx = 3, kDw = 4 };
 // latency than arithmetic: sixteen warps with one pair of buffers each (413 us with eight warps and two pairs
 // at 64800 x 2736 x 1024, KDH16 us with sixteen).
 constexpr int epi_warps(int mode) { return mode == kDh ? 16 : 8; }
-constexpr int epi_bufs(int mode) { return mode == kDh ? 2 : 4; }
+constexpr int epi_bufs(int mode) { return 32 / epi_warps(mode); }
 constexpr int stages(int mode) { return mode == kDh ? 4 : 5; }  // 32 KB a CTA; kDh's column sums take one
 
+// One weight's gradient in kDw
+struct DwSeg {
+  int64_t end;      // tiles of this weight and those before it
+  int64_t n_tiles;  // of a tile row
+  int64_t M, N, ldd;
+  void* D;
+  int out_f32, accumulate, tma_out;  // tma_out: 16-bit rows that an output map can address
+};
+constexpr int kDwWeights = 3;
+
 struct GatedParams {
-  CUtensorMap a0, a1, b0, b1;    // operands (a1 / b1: Wu in kUp, the second half of the depth in kDx)
+  CUtensorMap a0, a1, a2, b0, b1;  // operands (a1 / b1: Wu in kUp, the second half of the depth in kDx)
   CUtensorMap in0, in1;          // kDh: g, u; kDown: residual
   CUtensorMap out0, out1, out2;  // kUp: h, g, u; kDh: dg, du; kDown / kDx: the result
   int64_t M, N;                  // rows; columns of the result (hidden units in kUp / kDh)
@@ -53,13 +63,11 @@ struct GatedParams {
   int act;      // 0 SiLU, 1 GELU
   int save;     // kUp: store g and u
   int has_res;  // kDown
-  // kDw: tiles of both segments (a0 -> D0, a1 -> D1), in order; see dw_unit
+  // kDw: the weights' tiles in order; see gated_unit
+  DwSeg seg[kDwWeights];  // (weight i: out_i, a_i and b_(i / 2))
   int64_t direct;
   int rem, splits;
-  void *D0, *D1;  // out_f32: fp32 results, else 16-bit ones that the output maps cannot address (tma_out 0)
-  int64_t ldd;
-  int out_f32, accumulate, tma_out;
-  float* ws;      // [splits][rem][256][256]
+  float* ws;  // [splits][rem][256][256]
   // kDh: column sums of the rounded dg and du over each CTA's 128 rows, [2 m_tiles][2 sums_half] (null: none)
   float* sums;
   int64_t sums_half;
@@ -97,11 +105,6 @@ __device__ __forceinline__ bool gated_unit(const GatedParams& p, int64_t num_til
 struct DwPlan {
   int64_t direct;
   int rem, splits;
-};
-struct DwSum {
-  void *D0, *D1;
-  int64_t first, seg_tiles, n_tiles, M, N, ldd;
-  int rem, splits, out_f32, accumulate;
 };
 
 template <typename T, int MODE>
@@ -190,12 +193,17 @@ __device__ __forceinline__ bool bar_and(int id, int threads, bool v) {
   return out != 0;
 }
 
-// this lane's row of a 32 x 32 tile into the warp's next buffer (ring of four), then one TMA store
-template <typename T>
+// this lane's row of a 32 x 32 tile into the warp's next buffer (ring of BUFS), then one TMA store
+template <typename T, int BUFS>
 __device__ __forceinline__ void ring_store(const CUtensorMap* map, const float* f, T (*buf)[32 * kStageRow], int lane,
                                            int64_t nb, int64_t row_base, uint32_t& ring) {
-  T* b = buf[ring & 3];
-  if (lane == 0) bulk_wait_read_3();  // at most three later stores pending: this buffer's has been read
+  T* b = buf[ring & (BUFS - 1)];
+  if (lane == 0) {  // at most BUFS - 1 later stores pending: this buffer's has been read
+    if (BUFS == 4)
+      bulk_wait_read_3();
+    else
+      bulk_wait_read_1();
+  }
   __syncwarp();
 #pragma unroll
   for (int v = 0; v < 4; ++v) *reinterpret_cast<uint4*>(b + stg_off(lane, v)) = pack8<T>(&f[8 * v]);
@@ -208,10 +216,9 @@ __device__ __forceinline__ void ring_store(const CUtensorMap* map, const float* 
 // 32 columns of one row of a weight gradient by plain stores: fp32 (added to what is there), or 16-bit rows
 // that are not 16-byte aligned
 template <typename T>
-__device__ __forceinline__ void dw_row_store(const GatedParams& p, bool seg1, int64_t row, int64_t nb, const float* f) {
-  void* D = seg1 ? p.D1 : p.D0;
+__device__ __forceinline__ void dw_row_store(const DwSeg& p, int64_t row, int64_t nb, const float* f) {
   if (p.out_f32) {
-    float* d = reinterpret_cast<float*>(D) + row * p.ldd + nb;
+    float* d = reinterpret_cast<float*>(p.D) + row * p.ldd + nb;
     if (nb + 32 <= p.N && (p.ldd & 3) == 0) {
 #pragma unroll
       for (int v = 0; v < 8; ++v) {
@@ -228,36 +235,48 @@ __device__ __forceinline__ void dw_row_store(const GatedParams& p, bool seg1, in
         if (nb + j < p.N) d[j] = p.accumulate ? d[j] + f[j] : f[j];
     }
   } else {
-    T* d = reinterpret_cast<T*>(D) + row * p.ldd + nb;
+    T* d = reinterpret_cast<T*>(p.D) + row * p.ldd + nb;
 #pragma unroll
     for (int j = 0; j < 32; ++j)
       if (nb + j < p.N) d[j] = from_f<T>(f[j]);
   }
 }
 
+// a tile of all weights' -> its weight, and the tile within it
+struct DwList {
+  DwSeg seg[kDwWeights];
+};
+template <typename P>
+__device__ __forceinline__ void dw_place(const P& p, int64_t v, int& seg, int64_t& tile, int64_t& n_tiles) {
+  seg = v < p.seg[0].end ? 0 : v < p.seg[1].end ? 1 : 2;
+  tile = v - (seg ? p.seg[seg - 1].end : 0);
+  n_tiles = p.seg[seg].n_tiles;
+}
+
 // The cut tiles' partials added in piece order: one block a tile row, one thread four columns.
 template <typename T>
-__global__ void dw_sum_kernel(const float* __restrict__ ws, const __grid_constant__ DwSum p) {
+__global__ void dw_sum_kernel(const float* __restrict__ ws, const __grid_constant__ DwList l, int64_t first, int rem,
+                              int splits) {
   const int r = blockIdx.x >> 8, row_in = blockIdx.x & 255;
-  const int64_t tile = p.first + r;
-  const bool seg1 = tile >= p.seg_tiles;
-  const int64_t t = seg1 ? tile - p.seg_tiles : tile;
-  const int64_t row = (t / p.n_tiles) * BM2 + row_in, col = (t % p.n_tiles) * BN2 + 4 * threadIdx.x;
+  int seg;
+  int64_t t, nt;
+  dw_place(l, first + r, seg, t, nt);
+  const DwSeg& p = l.seg[seg];
+  const int64_t row = (t / nt) * BM2 + row_in, col = (t % nt) * BN2 + 4 * threadIdx.x;
   if (row >= p.M || col >= p.N) return;
   const float* src = ws + ((int64_t)r * BM2 + row_in) * BN2 + 4 * threadIdx.x;
   float4 a = __ldcs(reinterpret_cast<const float4*>(src));
-  for (int k = 1; k < p.splits; ++k) {
-    const float4 b = __ldcs(reinterpret_cast<const float4*>(src + (int64_t)k * p.rem * BM2 * BN2));
+  for (int k = 1; k < splits; ++k) {
+    const float4 b = __ldcs(reinterpret_cast<const float4*>(src + (int64_t)k * rem * BM2 * BN2));
     a.x += b.x, a.y += b.y, a.z += b.z, a.w += b.w;
   }
   const float f[4] = {a.x, a.y, a.z, a.w};
-  void* D = seg1 ? p.D1 : p.D0;
   for (int j = 0; j < 4 && col + j < p.N; ++j) {
     if (p.out_f32) {
-      float* d = reinterpret_cast<float*>(D) + row * p.ldd + col + j;
+      float* d = reinterpret_cast<float*>(p.D) + row * p.ldd + col + j;
       *d = p.accumulate ? *d + f[j] : f[j];
     } else {
-      reinterpret_cast<T*>(D)[row * p.ldd + col + j] = from_f<T>(f[j]);
+      reinterpret_cast<T*>(p.D)[row * p.ldd + col + j] = from_f<T>(f[j]);
     }
   }
 }
@@ -278,8 +297,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
   const int64_t pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
   const int64_t m_tiles = (p.M + BM2 - 1) / BM2;
   const int64_t n_tiles = (p.N + kCols - 1) / kCols;
-  const int64_t seg_tiles = m_tiles * n_tiles;
-  const int64_t num_tiles = MODE == kDw ? p.direct : seg_tiles;
+  const int64_t num_tiles = MODE == kDw ? p.direct : m_tiles * n_tiles;
   volatile int* abort_flag = &S.abort_flag;
 
   if (threadIdx.x == 0) {
@@ -314,10 +332,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
       uint32_t phase = 0;
       GUnit un;
       for (int64_t i = 0; gated_unit<MODE>(p, num_tiles, pair, npairs, i, un) && !*abort_flag; ++i) {
-        const bool seg1 = MODE == kDw && un.tile >= seg_tiles;
-        const int64_t tile = seg1 ? un.tile - seg_tiles : un.tile;
-        const int m0 = (int)((tile / n_tiles) * BM2) + (int)rank * BM;
-        const int nb0 = (int)((tile % n_tiles) * kCols) + (MODE == kUp ? 0 : (int)rank * 128);
+        int seg = 0;
+        int64_t tile = un.tile, nt = n_tiles;
+        if (MODE == kDw) dw_place(p, un.tile, seg, tile, nt);
+        const int m0 = (int)((tile / nt) * BM2) + (int)rank * BM;
+        const int nb0 = (int)((tile % nt) * kCols) + (MODE == kUp ? 0 : (int)rank * 128);
         for (int kb = un.kb0; kb < un.kb1; ++kb) {
           if (!mbar_wait(&S.empty[stage], phase ^ 1, abort_flag, err)) break;
           if (rank == 0) mbar_expect_tx(&S.full[stage], (uint32_t)(2 * (BM + 128) * BK * sizeof(T)));
@@ -325,14 +344,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
           const bool second = MODE == kDx && kb >= p.kb0;
           const int k0 = (second ? kb - p.kb0 : kb) * BK;
           if (kMnA) {
-            const CUtensorMap* ma = seg1 ? &p.a1 : &p.a0;
+            const CUtensorMap* ma = seg == 0 ? &p.a0 : seg == 1 ? &p.a1 : &p.a2;
             tma_load_2d_pair(&S.a[stage][0], ma, fb, m0, k0);
             tma_load_2d_pair(&S.a[stage][64 * BK], ma, fb, m0 + 64, k0);
           } else {
             tma_load_2d_pair(S.a[stage], second ? &p.a1 : &p.a0, fb, k0, m0);
           }
           if (kMnB) {
-            const CUtensorMap* mb = second ? &p.b1 : &p.b0;
+            const CUtensorMap* mb = second || seg == 2 ? &p.b1 : &p.b0;
             tma_load_2d_pair(&S.b[stage][0], mb, fb, nb0, k0);
             tma_load_2d_pair(&S.b[stage][64 * BK], mb, fb, nb0 + 64, k0);
           } else {
@@ -404,11 +423,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
     bool ok = true;
     GUnit un;
     for (int64_t i = 0; ok && gated_unit<MODE>(p, num_tiles, pair, npairs, i, un); ++i) {
-      const bool seg1 = MODE == kDw && un.tile >= seg_tiles;
-      const int64_t tile = seg1 ? un.tile - seg_tiles : un.tile;
-      const int64_t row_base = (tile / n_tiles) * BM2 + (int64_t)rank * BM + q * 32;
-      const int64_t n0 = (tile % n_tiles) * kCols + part * kShare;
-      const bool rows = row_base < p.M;  // warp-uniform; a tile's lower rows may be past the end
+      int seg = 0;
+      int64_t tile = un.tile, nt = n_tiles;
+      if (MODE == kDw) dw_place(p, un.tile, seg, tile, nt);
+      const int64_t M = MODE == kDw ? p.seg[seg].M : p.M, N = MODE == kDw ? p.seg[seg].N : p.N;
+      const int64_t row_base = (tile / nt) * BM2 + (int64_t)rank * BM + q * 32;
+      const int64_t n0 = (tile % nt) * kCols + part * kShare;
+      const bool rows = row_base < M;  // warp-uniform; a tile's lower rows may be past the end
       const uint32_t t_row = tmem_base + ((uint32_t)(q * 32) << 16) + (uint32_t)(acc * BN2 + part * kShare);
       // kDh: g and u of chunk c into the warp's two buffers
       auto issue_gu = [&](int c) {
@@ -454,8 +475,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
           if (p.bias0) add_bias32(p.bias0, p.bias_dtype, nb, p.N, g);
           if (p.bias1) add_bias32(p.bias1, p.bias_dtype, nb, p.N, u);
           if (p.save) {
-            ring_store<T>(&p.out1, g, buf, lane, nb, row_base, ring);
-            ring_store<T>(&p.out2, u, buf, lane, nb, row_base, ring);
+            ring_store<T, epi_bufs(MODE)>(&p.out1, g, buf, lane, nb, row_base, ring);
+            ring_store<T, epi_bufs(MODE)>(&p.out2, u, buf, lane, nb, row_base, ring);
           }
           if (p.act == 0) {
 #pragma unroll
@@ -464,7 +485,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
 #pragma unroll
             for (int j = 0; j < 32; ++j) u[j] *= act_parts(g[j], 1).val;
           }
-          ring_store<T>(&p.out0, u, buf, lane, nb, row_base, ring);
+          ring_store<T, epi_bufs(MODE)>(&p.out0, u, buf, lane, nb, row_base, ring);
         }
       } else if (MODE == kDh) {
 #pragma unroll 1
@@ -541,7 +562,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
 #pragma unroll 1
         for (int c = 0; c < kChunks; ++c) {
           const int64_t nb = n0 + 32 * c;
-          if (!rows || nb >= p.N) break;
+          if (!rows || nb >= N) break;
           uint32_t r[32];
           tmem_ld32(t_row + (uint32_t)(32 * c), r);
           float* f = reinterpret_cast<float*>(r);
@@ -552,9 +573,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
               __stcg(reinterpret_cast<float4*>(w) + v, make_float4(f[4 * v], f[4 * v + 1], f[4 * v + 2], f[4 * v + 3]));
             continue;
           }
-          if (MODE == kDw && !p.tma_out) {
+          if (MODE == kDw && !p.seg[seg].tma_out) {
             const int64_t row = row_base + lane;
-            if (row < p.M) dw_row_store<T>(p, seg1, row, nb, f);
+            if (row < M) dw_row_store<T>(p.seg[seg], row, nb, f);
             continue;
           }
           if (MODE == kDown && p.bias0) add_bias32(p.bias0, p.bias_dtype, nb, p.N, f);
@@ -572,7 +593,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
             __syncwarp();
             if (lane == 0) tma_store_2d(&p.out0, b, (int)nb, (int)row_base);
           } else {
-            ring_store<T>(MODE == kDw && seg1 ? &p.out1 : &p.out0, f, buf, lane, nb, row_base, ring);
+            ring_store<T, epi_bufs(MODE)>(seg == 0 ? &p.out0 : seg == 1 ? &p.out1 : &p.out2, f, buf, lane, nb, row_base, ring);
           }
         }
       }
@@ -626,9 +647,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
 // Whole waves of tiles, and how to cut the tiles that are left (none if they fill a wave well).  In k-block
 // steps (0.31 us a pair): a cut costs its longest pair, plus 0.26 steps a partial (256 KB written and read
 // over the device) and about 15 for the second kernel and the shorter units.
-static DwPlan dw_plan(int64_t M, int64_t N, int64_t K, int segs) {
-  const int64_t pairs = sm_count() / 2, tiles = segs * ((M + BM2 - 1) / BM2) * ((N + BN2 - 1) / BN2);
-  const int64_t kb = (K + BK - 1) / BK, left = tiles % pairs;
+static DwPlan dw_plan(int64_t tiles, int64_t K) {
+  const int64_t pairs = sm_count() / 2, kb = (K + BK - 1) / BK, left = tiles % pairs;
   DwPlan best = {tiles, 0, 1};
   double best_cost = (double)kb;  // one more wave
   if (left == 0) return best;
@@ -641,68 +661,22 @@ static DwPlan dw_plan(int64_t M, int64_t N, int64_t K, int segs) {
   }
   return best;
 }
+static int64_t dw_tiles(int64_t M, int64_t N) { return ((M + BM2 - 1) / BM2) * ((N + BN2 - 1) / BN2); }
 
-template <typename T, int MODE>
-static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
+// launches gated_kernel for `units` tiles of work; `fill` encodes the operands (false: refused)
+template <typename T, int MODE, typename Fill>
+static cudaError_t launch_pairs(int64_t units, int dtype, cudaStream_t s, GatedParams& p, Fill fill) {
   const size_t smem = sizeof(SmemG<T, MODE>) + 1024;
   auto k = gated_kernel<T, MODE>;
   // on each call: the attribute belongs to the current device, and a runtime call has to make that device's
   // context current on this thread (an autograd thread may not have one yet) before the maps are encoded
   NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  GatedParams p;
   memset(&p, 0, sizeof(p));
-  const bool mn = MODE == kDh || MODE == kDx || MODE == kDw;
-  bool ok = MODE == kDw ? make_map_mn(&p.a0, a.a0, a.K, a.M, a.lda, a.dtype)
-                        : make_map(&p.a0, a.a0, a.M, a.K, a.lda, BM, a.dtype);
-  if (MODE == kDw && a.a1) ok = ok && make_map_mn(&p.a1, a.a1, a.K, a.M, a.lda, a.dtype);
-  if (MODE == kDx) ok = ok && make_map(&p.a1, a.a1, a.M, a.K, a.lda, BM, a.dtype);
-  if (mn) {
-    ok = ok && make_map_mn(&p.b0, a.b0, a.K, a.N, a.ldb0, a.dtype);
-    if (MODE == kDx) ok = ok && make_map_mn(&p.b1, a.b1, a.K, a.N, a.ldb1, a.dtype);
-  } else {
-    ok = ok && make_map(&p.b0, a.b0, a.N, a.K, a.ldb0, 128, a.dtype);
-    if (MODE == kUp) ok = ok && make_map(&p.b1, a.b1, a.N, a.K, a.ldb1, 128, a.dtype);
-  }
-  if (a.in0) ok = ok && make_store_map(&p.in0, const_cast<void*>(a.in0), a.M, a.N, a.ldin, a.dtype);
-  if (a.in1) ok = ok && make_store_map(&p.in1, const_cast<void*>(a.in1), a.M, a.N, a.ldin, a.dtype);
-  p.tma_out = MODE != kDw || (!a.out_f32 && a.ldout % 8 == 0 && (reinterpret_cast<uintptr_t>(a.out0) & 15) == 0 &&
-                              (reinterpret_cast<uintptr_t>(a.out1) & 15) == 0);
-  if (p.tma_out) ok = ok && make_store_map(&p.out0, a.out0, a.M, a.N, a.ldout, a.dtype);
-  if (a.out1 && p.tma_out) ok = ok && make_store_map(&p.out1, a.out1, a.M, a.N, a.ldaux, a.dtype);
-  if (a.out2) ok = ok && make_store_map(&p.out2, a.out2, a.M, a.N, a.ldaux, a.dtype);
-  if (!ok) return cudaErrorInvalidValue;
-  p.M = a.M;
-  p.N = a.N;
-  p.kb0 = (int)((a.K + BK - 1) / BK);
-  p.kb = MODE == kDx ? 2 * p.kb0 : p.kb0;
-  p.bias0 = a.bias0;
-  p.bias1 = a.bias1;
-  p.bias_dtype = a.bias_dtype;
-  p.act = a.act;
-  p.sums = MODE == kDh ? a.sums : nullptr;
-  p.sums_half = a.sums_half;
-  p.save = MODE == kUp && a.out1 != nullptr;
-  p.has_res = MODE == kDown && a.in0 != nullptr;
-  const uint32_t fmt = a.dtype == kBF16 ? 1u : 0u;
-  const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (MODE == kDw ? 1u << 15 : 0u) | (mn ? 1u << 16 : 0u) | ((uint32_t)(BN2 >> 3) << 17) |
-                         ((uint32_t)(BM2 >> 4) << 24);
-  const int cols = MODE == kUp ? 128 : 256;
-  const int64_t seg_tiles = ((a.M + BM2 - 1) / BM2) * ((a.N + cols - 1) / cols);
-  int64_t tiles = seg_tiles;
-  if (MODE == kDw) {
-    const DwPlan plan = dw_plan(a.M, a.N, a.K, a.a1 ? 2 : 1);
-    p.direct = plan.direct;
-    p.rem = plan.rem;
-    p.splits = plan.splits;
-    p.D0 = a.out0;
-    p.D1 = a.out1;
-    p.ldd = a.ldout;
-    p.out_f32 = a.out_f32;
-    p.accumulate = a.accumulate;
-    p.ws = a.ws;
-    if (plan.rem > 0 && !a.ws) return cudaErrorInvalidValue;
-    tiles = std::max<int64_t>(plan.direct, (int64_t)plan.rem * plan.splits);
-  }
+  if (!fill()) return cudaErrorInvalidValue;
+  constexpr bool mn = MODE == kDh || MODE == kDx || MODE == kDw;
+  const uint32_t fmt = dtype == kBF16 ? 1u : 0u;
+  const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (MODE == kDw ? 1u << 15 : 0u) | (mn ? 1u << 16 : 0u) |
+                         ((uint32_t)(BN2 >> 3) << 17) | ((uint32_t)(BM2 >> 4) << 24);
   cudaLaunchConfig_t cfg = {};
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -721,13 +695,83 @@ static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
     NSW_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, k, &cfg));
     max_pairs = n > 0 ? n : 1;
   }
-  const int pairs = tiles < max_pairs ? (int)tiles : max_pairs;
-  cfg.gridDim = dim3(2 * pairs, 1, 1);
+  const int64_t pairs = std::min<int64_t>(units, max_pairs);
+  cfg.gridDim = dim3((unsigned)(2 * pairs), 1, 1);
   NSW_CUDA_CHECK(cudaLaunchKernelEx(&cfg, k, p, idesc, device_error_flag()));
-  if (MODE == kDw && p.rem > 0) {
-    const DwSum d = {a.out0, a.out1, p.direct, seg_tiles, (a.N + cols - 1) / cols, a.M, a.N, a.ldout,
-                     p.rem,  p.splits, a.out_f32, a.accumulate};
-    dw_sum_kernel<T><<<p.rem * 256, 64, 0, s>>>(a.ws, d);
+  return cudaGetLastError();
+}
+
+template <typename T, int MODE>
+static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
+  constexpr int cols = MODE == kUp ? 128 : 256;
+  const int64_t tiles = ((a.M + BM2 - 1) / BM2) * ((a.N + cols - 1) / cols);
+  GatedParams p;
+  return launch_pairs<T, MODE>(tiles, a.dtype, s, p, [&]() {
+    constexpr bool mn = MODE == kDh || MODE == kDx;
+    bool ok = make_map(&p.a0, a.a0, a.M, a.K, a.lda, BM, a.dtype);
+    if (MODE == kDx) ok = ok && make_map(&p.a1, a.a1, a.M, a.K, a.lda, BM, a.dtype);
+    if (mn) {
+      ok = ok && make_map_mn(&p.b0, a.b0, a.K, a.N, a.ldb0, a.dtype);
+      if (MODE == kDx) ok = ok && make_map_mn(&p.b1, a.b1, a.K, a.N, a.ldb1, a.dtype);
+    } else {
+      ok = ok && make_map(&p.b0, a.b0, a.N, a.K, a.ldb0, 128, a.dtype);
+      if (MODE == kUp) ok = ok && make_map(&p.b1, a.b1, a.N, a.K, a.ldb1, 128, a.dtype);
+    }
+    if (a.in0) ok = ok && make_store_map(&p.in0, const_cast<void*>(a.in0), a.M, a.N, a.ldin, a.dtype);
+    if (a.in1) ok = ok && make_store_map(&p.in1, const_cast<void*>(a.in1), a.M, a.N, a.ldin, a.dtype);
+    ok = ok && make_store_map(&p.out0, a.out0, a.M, a.N, a.ldout, a.dtype);
+    if (a.out1) ok = ok && make_store_map(&p.out1, a.out1, a.M, a.N, a.ldaux, a.dtype);
+    if (a.out2) ok = ok && make_store_map(&p.out2, a.out2, a.M, a.N, a.ldaux, a.dtype);
+    p.M = a.M;
+    p.N = a.N;
+    p.kb0 = (int)((a.K + BK - 1) / BK);
+    p.kb = MODE == kDx ? 2 * p.kb0 : p.kb0;
+    p.bias0 = a.bias0;
+    p.bias1 = a.bias1;
+    p.bias_dtype = a.bias_dtype;
+    p.act = a.act;
+    p.sums = MODE == kDh ? a.sums : nullptr;
+    p.sums_half = a.sums_half;
+    p.save = MODE == kUp && a.out1 != nullptr;
+    p.has_res = MODE == kDown && a.in0 != nullptr;
+    return ok;
+  });
+}
+
+template <typename T>
+static cudaError_t launch_dw(const GatedDwArgs& a, cudaStream_t s) {
+  int64_t tiles = 0;
+  for (const auto& w : a.w) tiles += dw_tiles(w.M, w.N);
+  const DwPlan plan = dw_plan(tiles, a.T);
+  if (plan.rem > 0 && !a.ws) return cudaErrorInvalidValue;
+  GatedParams p;
+  NSW_CUDA_CHECK((launch_pairs<T, kDw>(
+      std::max<int64_t>(plan.direct, (int64_t)plan.rem * plan.splits), a.dtype, s, p, [&]() {
+        const auto& w = a.w;
+        bool ok = make_map_mn(&p.a0, w[0].a, a.T, w[0].M, w[0].lda, a.dtype) &&
+                  make_map_mn(&p.a1, w[1].a, a.T, w[1].M, w[1].lda, a.dtype) &&
+                  make_map_mn(&p.a2, w[2].a, a.T, w[2].M, w[2].lda, a.dtype) &&
+                  make_map_mn(&p.b0, w[0].b, a.T, w[0].N, w[0].ldb, a.dtype) &&
+                  make_map_mn(&p.b1, w[2].b, a.T, w[2].N, w[2].ldb, a.dtype);
+        CUtensorMap* out[kDwWeights] = {&p.out0, &p.out1, &p.out2};
+        int64_t end = 0;
+        for (int i = 0; i < kDwWeights; ++i) {
+          end += dw_tiles(w[i].M, w[i].N);
+          const bool tma = !w[i].out_f32 && w[i].N % 8 == 0 && (reinterpret_cast<uintptr_t>(w[i].D) & 15) == 0;
+          p.seg[i] = {end, (w[i].N + BN2 - 1) / BN2, w[i].M, w[i].N, w[i].N, w[i].D, w[i].out_f32, w[i].accumulate, tma};
+          if (tma) ok = ok && make_store_map(out[i], w[i].D, w[i].M, w[i].N, w[i].N, a.dtype);
+        }
+        p.kb = (int)((a.T + BK - 1) / BK);
+        p.direct = plan.direct;
+        p.rem = plan.rem;
+        p.splits = plan.splits;
+        p.ws = a.ws;
+        return ok;
+      })));
+  if (plan.rem > 0) {
+    DwList l;
+    for (int i = 0; i < kDwWeights; ++i) l.seg[i] = p.seg[i];
+    dw_sum_kernel<T><<<plan.rem * 256, 64, 0, s>>>(a.ws, l, plan.direct, plan.rem, plan.splits);
   }
   return cudaGetLastError();
 }
@@ -1165,7 +1209,6 @@ static cudaError_t launch_gated_mode(const GatedArgs& a, bool dependent, cudaStr
     case kGatedDown: return launch_any<T, kDown>(a, dependent, s);
     case kGatedDh: return launch_any<T, kDh>(a, dependent, s);
     case kGatedDx: return launch_any<T, kDx>(a, dependent, s);
-    case kGatedDw: return launch_gated<T, kDw>(a, s);
   }
   return cudaErrorInvalidValue;
 }
@@ -1389,32 +1432,54 @@ static cudaError_t launch_skinny(const SkinnyParams& p, bool vec, cudaStream_t s
   return p.M <= 8 ? launch_skinny_nt<T, 1, DUAL>(p, vec, s) : launch_skinny_nt<T, 2, DUAL>(p, vec, s);
 }
 
-// dst[i, j] = src[i s0 + j s1] (16-bit), rows of ld elements: operands whose rows are not 16-byte aligned
-__global__ void pad_copy_kernel(const uint16_t* __restrict__ src, int64_t s0, int64_t s1, uint16_t* __restrict__ dst,
-                                int64_t ld, int64_t rows, int64_t cols) {
-  const int64_t total = rows * ld;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t m = i / ld, c = i - m * ld;
-    if (c < cols) dst[i] = src[m * s0 + c * s1];
+// dst[i, j] = src[i s0 + j s1] (16-bit), rows of ld elements: operands whose rows are not 16-byte aligned.  A
+// thread copies eight elements, one 16-byte store where dst's rows allow it (5.6 MB: PADUS us).
+__global__ void __launch_bounds__(256) pad_copy_kernel(const uint16_t* __restrict__ src, int64_t s0, int64_t s1,
+                                                       uint16_t* __restrict__ dst, int64_t ld, int64_t rows,
+                                                       int64_t cols, int vec) {
+  const int64_t groups = (cols + 7) / 8;
+  for (int64_t m = blockIdx.y; m < rows; m += gridDim.y) {
+    const uint16_t* p = src + m * s0;
+    uint16_t* d = dst + m * ld;
+    for (int64_t g = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; g < groups; g += (int64_t)gridDim.x * blockDim.x) {
+      const int64_t c = 8 * g;
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int j = 0; j < 8; ++j)
+        if (c + j < cols) w[j >> 1] |= (uint32_t)p[(c + j) * s1] << (16 * (j & 1));
+      if (vec && c + 8 <= ld) {
+        *reinterpret_cast<uint4*>(d + c) = make_uint4(w[0], w[1], w[2], w[3]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c + j < cols) d[c + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
+      }
+    }
   }
 }
 
-// Column sums of a 16-bit [rows, n] matrix (rows 16-byte aligned, ld >= round8(n)): partial[y][c] over the
-// y-th slice of the rows; a warp takes 256 columns of a row, 16 bytes a lane.
+// Column sums of up to two 16-bit [rows, n] matrices (rows 16-byte aligned, ld >= n rounded up to 8; blockIdx.z):
+// partial[y][c] over the y-th slice of the rows; a warp takes 256 columns of a row, 16 bytes a lane.
+struct ColSources {
+  ColSource v[2];
+};
 template <typename T>
-__global__ void __launch_bounds__(256) col_partial_kernel(const T* __restrict__ x, int64_t ld, int64_t rows, int64_t n,
-                                                          float* __restrict__ partial) {
+__global__ void __launch_bounds__(256) col_partial_kernel(const __grid_constant__ ColSources p) {
+  const ColSource& s = p.v[blockIdx.z];
+  const int64_t rows = s.rows, n = s.n, ld = s.ld, step = 8 * s.parts;
+  if ((int64_t)blockIdx.x * 256 >= n || (int64_t)blockIdx.y >= s.parts) return;
   __shared__ float red[8][256];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t c = (int64_t)blockIdx.x * 256 + lane * 8;
+  const T* x = reinterpret_cast<const T*>(s.x) + c;
   float a[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) a[j] = 0.f;
   if (c < n) {
 #pragma unroll 4
-    for (int64_t r = (int64_t)blockIdx.y * 8 + warp; r < rows; r += (int64_t)gridDim.y * 8) {
+    for (int64_t r = (int64_t)blockIdx.y * 8 + warp; r < rows; r += step) {
       float f[8];
-      unpack8<T>(__ldg(reinterpret_cast<const uint4*>(x + r * ld + c)), f);
+      unpack8<T>(__ldg(reinterpret_cast<const uint4*>(x + r * ld)), f);
 #pragma unroll
       for (int j = 0; j < 8; ++j) a[j] += f[j];
     }
@@ -1426,37 +1491,32 @@ __global__ void __launch_bounds__(256) col_partial_kernel(const T* __restrict__ 
 #pragma unroll
   for (int w = 1; w < 8; ++w) v += red[w][threadIdx.x];
   const int64_t col = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (col < n) partial[(int64_t)blockIdx.y * n + col] = v;
+  if (col < n) s.partial[(int64_t)blockIdx.y * n + col] = v;
 }
 
-// out[c] (+)= sum of partial[0 .. parts)[c], in order; columns [0, seg) go to out0, [off, off + seg) to out1
-struct ColFinish {
-  const float* partial;
-  int64_t parts, n, seg, off;
-  void *out0, *out1;
-  int f32, accumulate;
+// out[c] (+)= sum over the parts of partial[.][first + c], in a fixed order; blockIdx.y: which sum
+struct ColSums {
+  ColSum v[kColSums];
 };
 template <typename T>
-__global__ void __launch_bounds__(256) col_finish_kernel(const __grid_constant__ ColFinish p) {
-  __shared__ float red[8][33];
+__global__ void __launch_bounds__(1024) col_finish_kernel(const __grid_constant__ ColSums p) {
+  __shared__ float red[32][33];
+  const ColSum& s = p.v[blockIdx.y];
+  if (!s.out || (int64_t)blockIdx.x * 32 >= s.n) return;
   const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane;
   float a = 0.f;
-  if (c < p.n)
-    for (int64_t r = w; r < p.parts; r += 8) a += p.partial[r * p.n + c];
+  if (c < s.n)
+    for (int64_t r = w; r < s.parts; r += 32) a += s.partial[r * s.stride + s.first + c];
   red[w][lane] = a;
   __syncthreads();
-  if (w || c >= p.n) return;
-  for (int i = 1; i < 8; ++i) a += red[i][lane];
-  const bool second = p.out1 && c >= p.off;
-  const int64_t at = second ? c - p.off : c;
-  void* out = second ? p.out1 : p.out0;
-  if (at >= p.seg || !out) return;
-  if (p.f32) {
-    float* o = reinterpret_cast<float*>(out) + at;
-    *o = p.accumulate ? *o + a : a;
+  if (w || c >= s.n) return;
+  for (int i = 1; i < 32; ++i) a += red[i][lane];
+  if (s.f32) {
+    float* o = reinterpret_cast<float*>(s.out) + c;
+    *o = s.accumulate ? *o + a : a;
   } else {
-    reinterpret_cast<T*>(out)[at] = from_f<T>(a);
+    reinterpret_cast<T*>(s.out)[c] = from_f<T>(a);
   }
 }
 
@@ -1466,29 +1526,44 @@ int col_sum_parts(int64_t rows, int64_t n) {
   const int64_t cols = (n + 255) / 256;
   return (int)std::max<int64_t>(1, std::min<int64_t>((rows + 31) / 32, 4 * (int64_t)tc::sm_count() / cols));
 }
-cudaError_t col_partial(const void* x, int64_t ld, int64_t rows, int64_t n, int parts, float* partial, int dtype,
-                        cudaStream_t s) {
-  const dim3 grid((unsigned)((n + 255) / 256), (unsigned)parts, 1);
+cudaError_t col_partial(const ColSource* src, int count, int dtype, cudaStream_t s) {
+  if (count < 1 || count > 2) return cudaErrorInvalidValue;
+  const ColSource &a = src[0], &b = src[count - 1];
+  const gated::ColSources p = {{a, b}};
+  const dim3 grid((unsigned)((std::max(a.n, b.n) + 255) / 256), (unsigned)std::max(a.parts, b.parts), (unsigned)count);
   if (dtype == kBF16)
-    gated::col_partial_kernel<<<grid, 256, 0, s>>>(reinterpret_cast<const __nv_bfloat16*>(x), ld, rows, n, partial);
+    gated::col_partial_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(p);
   else
-    gated::col_partial_kernel<<<grid, 256, 0, s>>>(reinterpret_cast<const __half*>(x), ld, rows, n, partial);
+    gated::col_partial_kernel<__half><<<grid, 256, 0, s>>>(p);
   return cudaGetLastError();
 }
-cudaError_t col_finish(const float* partial, int64_t parts, int64_t n, int64_t seg, int64_t off, void* out0, void* out1,
-                       int dtype, bool f32, bool accumulate, cudaStream_t s) {
-  const gated::ColFinish p = {partial, parts, n, seg, off, out0, out1, f32, accumulate};
-  const int blocks = (int)((n + 31) / 32);
+cudaError_t col_finish(const ColSum* v, int dtype, cudaStream_t s) {
+  gated::ColSums p;
+  int64_t n = 1;
+  for (int i = 0; i < kColSums; ++i) {
+    p.v[i] = v[i];
+    if (v[i].out) n = std::max(n, v[i].n);
+  }
+  const dim3 grid((unsigned)((n + 31) / 32), kColSums, 1);
   if (dtype == kBF16)
-    gated::col_finish_kernel<__nv_bfloat16><<<blocks, 256, 0, s>>>(p);
+    gated::col_finish_kernel<__nv_bfloat16><<<grid, 1024, 0, s>>>(p);
   else
-    gated::col_finish_kernel<__half><<<blocks, 256, 0, s>>>(p);
+    gated::col_finish_kernel<__half><<<grid, 1024, 0, s>>>(p);
   return cudaGetLastError();
 }
 
-int64_t gated_dw_workspace(int64_t M, int64_t N, int64_t K, int segs) {
-  const tc::DwPlan p = tc::dw_plan(M, N, K, segs);
+int64_t gated_dw_workspace(const GatedDwArgs& a) {
+  int64_t tiles = 0;
+  for (const auto& w : a.w) tiles += tc::dw_tiles(w.M, w.N);
+  const tc::DwPlan p = tc::dw_plan(tiles, a.T);
   return (int64_t)p.rem * p.splits * tc::BM2 * tc::BN2;
+}
+
+cudaError_t gated_dw(const GatedDwArgs& a, cudaStream_t s) {
+  if ((a.dtype != kBF16 && a.dtype != kF16) || a.T <= 0) return cudaErrorInvalidValue;
+  for (const auto& w : a.w)
+    if (w.M <= 0 || w.N <= 0 || !w.D || (w.accumulate && !w.out_f32)) return cudaErrorInvalidValue;
+  return a.dtype == kBF16 ? tc::launch_dw<__nv_bfloat16>(a, s) : tc::launch_dw<__half>(a, s);
 }
 
 int64_t gated_sum_rows(const GatedArgs& a) {
@@ -1536,11 +1611,12 @@ cudaError_t gated_skinny(const GatedArgs& a, bool dependent, cudaStream_t s) {
 
 cudaError_t pad_copy(const void* src, int64_t s0, int64_t s1, void* dst, int64_t ld, int64_t rows, int64_t cols,
                      cudaStream_t s) {
-  const int64_t total = rows * ld;
-  if (total <= 0) return cudaSuccess;
-  const int blocks = (int)std::min<int64_t>((total + 255) / 256, 16 * tc::sm_count());
-  gated::pad_copy_kernel<<<blocks, 256, 0, s>>>(reinterpret_cast<const uint16_t*>(src), s0, s1,
-                                                reinterpret_cast<uint16_t*>(dst), ld, rows, cols);
+  if (rows <= 0 || cols <= 0) return cudaSuccess;
+  const int64_t groups = (cols + 7) / 8;
+  const dim3 grid((unsigned)std::min<int64_t>((groups + 255) / 256, 1024), (unsigned)std::min<int64_t>(rows, 65535), 1);
+  const int vec = ld % 8 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
+  gated::pad_copy_kernel<<<grid, 256, 0, s>>>(reinterpret_cast<const uint16_t*>(src), s0, s1,
+                                              reinterpret_cast<uint16_t*>(dst), ld, rows, cols, vec);
   return cudaGetLastError();
 }
 

@@ -176,9 +176,7 @@ cudaError_t wgrad_tcgen05(const WgradArgs& a, const WgradPlan& plan, cudaStream_
 //   kGatedDh    d = a0 b0 with b0 [K, N]; out0 = d * in1 * act'(in0), out1 = d * act(in0) (in: g, u, ldin;
 //               out0 in rows of ldout, out1 in rows of ldaux)
 //   kGatedDx    out0 = a0 b0 + a1 b1 with b0, b1 [K, N]
-//   kGatedDw    out0 (+)= a0^T b0, and with a1: out1 (+)= a1^T b0 (depth K = tokens; a0, a1 [K, M] rows of lda,
-//               b0 [K, N]); 16-bit or (out_f32) fp32 results in rows of ldout; ws: gated_dw_workspace floats
-enum GatedMode : int { kGatedUp = 0, kGatedDown = 1, kGatedDh = 2, kGatedDx = 3, kGatedDw = 4 };
+enum GatedMode : int { kGatedUp = 0, kGatedDown = 1, kGatedDh = 2, kGatedDx = 3 };
 struct GatedArgs {
   int mode, dtype, act;  // act: 0 SiLU, 1 GELU
   int64_t M, N, K;
@@ -192,30 +190,54 @@ struct GatedArgs {
   int64_t ldin;
   void *out0, *out1, *out2;
   int64_t ldout, ldaux;
-  int out_f32, accumulate;  // kGatedDw (accumulate: fp32 only)
-  float* ws;
   // kGatedDh, where gated_sum_rows(args) > 0: that many rows of 2 sums_half column sums, of out0 at [0, N), of
   // out1 at [sums_half, sums_half + N) (null: none)
   float* sums;
   int64_t sums_half;
 };
 int64_t gated_sum_rows(const GatedArgs& a);
-int64_t gated_dw_workspace(int64_t M, int64_t N, int64_t K, int segs);
-// Column sums: partial [parts][n] of a 16-bit matrix whose rows are 16-byte aligned (ld >= n rounded up to 8),
-// and their sums; columns [0, seg) to out0 and [off, off + seg) to out1 (may be null), fp32 (f32; added with
-// accumulate) or in dtype
+// The three weight gradients in one launch: w[i].D (+)= w[i].a^T w[i].b over T tokens; a [T, M] in rows of lda,
+// b [T, N] in rows of ldb (16-byte aligned rows; w[1].b is w[0].b), D contiguous [M, N], 16-bit or (out_f32) fp32,
+// added to with accumulate; ws: gated_dw_workspace floats.
+struct GatedDwArgs {
+  int dtype;
+  int64_t T;
+  struct Weight {
+    const void *a, *b;
+    int64_t lda, ldb, M, N;
+    void* D;
+    int out_f32, accumulate;
+  } w[3];
+  float* ws;
+};
+int64_t gated_dw_workspace(const GatedDwArgs& a);
+cudaError_t gated_dw(const GatedDwArgs& a, cudaStream_t s);
+// Column sums.  col_partial: `parts` partial rows of n sums of one or two 16-bit matrices (rows 16-byte aligned,
+// ld >= n rounded up to 8).  col_finish: sums of partial rows of `stride` floats, columns [first, first + n), into
+// out (null: none): fp32 (f32; added to with accumulate) or dtype.
+struct ColSource {
+  const void* x;
+  int64_t ld, rows, n;
+  int64_t parts;
+  float* partial;
+};
+struct ColSum {
+  const float* partial;
+  int64_t parts, stride, first, n;
+  void* out;
+  int f32, accumulate;
+};
+constexpr int kColSums = 3;
 int col_sum_parts(int64_t rows, int64_t n);
-cudaError_t col_partial(const void* x, int64_t ld, int64_t rows, int64_t n, int parts, float* partial, int dtype,
-                        cudaStream_t s);
-cudaError_t col_finish(const float* partial, int64_t parts, int64_t n, int64_t seg, int64_t off, void* out0, void* out1,
-                       int dtype, bool f32, bool accumulate, cudaStream_t s);
+cudaError_t col_partial(const ColSource* src, int count, int dtype, cudaStream_t s);
+cudaError_t col_finish(const ColSum* v, int dtype, cudaStream_t s);
 // dependent: the A operand is written by the kernel before it on the stream, which this one may overlap (a
 // programmatic dependent launch: it waits for that kernel before it touches anything but the weights)
 cudaError_t gated_product(const GatedArgs& a, bool dependent, cudaStream_t s);
 // kGatedUp (no out1 / out2) and kGatedDown for at most kGatedSkinnyTokens rows, any strides
 constexpr int kGatedSkinnyTokens = 16;
 cudaError_t gated_skinny(const GatedArgs& a, bool dependent, cudaStream_t s);
-// 16-bit strided copy into rows of ld elements (cols of them written)
+// 16-bit strided copy into rows of ld elements (cols of them written, and zeros up to a multiple of eight)
 cudaError_t pad_copy(const void* src, int64_t s0, int64_t s1, void* dst, int64_t ld, int64_t rows, int64_t cols,
                      cudaStream_t s);
 

@@ -366,6 +366,15 @@ def _rows(t: torch.Tensor, n: int) -> torch.Tensor:
     return t if t.dim() == 2 else t.reshape(-1, n)
 
 
+def check_gated_shapes(x, wg, wu, wd, residual):
+    if (wg.dim() != 2 or wu.shape != wg.shape or wd.dim() != 2 or wd.shape[1] != wg.shape[0]
+            or x.shape[-1:] != wg.shape[1:]):
+        raise ValueError(f"gated_mlp: x {tuple(x.shape)}, w_gate {tuple(wg.shape)}, w_up {tuple(wu.shape)} "
+                         f"and w_down {tuple(wd.shape)} do not fit together")
+    if residual is not None and residual.shape != x.shape[:-1] + wd.shape[:1]:
+        raise ValueError(f"gated_mlp: residual {tuple(residual.shape)} is not the output's shape")
+
+
 class _GatedMLP(torch.autograd.Function):
     """The gated feed-forward network.  The forward keeps the input, both pre-activations and their
     gated product h (16 bits); the backward is dg and du from one product with a fused epilogue, the input
@@ -418,6 +427,7 @@ def gated_mlp_cuda(x, wg, wu, wd, bg, bu, bd, residual, activation):
     if wg.dtype == wu.dtype == wd.dtype == dt:  # parameters already in the compute type: one native node
         return require().gated_mlp(x if x.dtype == dt else x.to(dt), wg, wu, wd, bg, bu, bd, residual, act)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, wg, wu, wd, bg, bu, bd, residual)):
+        check_gated_shapes(x, wg, wu, wd, residual)
         return _GatedMLP.apply(x, residual, act, wg, wu, wd, bg, bu, bd)
     return require().gated_mlp(x.to(dt), wcache.get(wg, dt), wcache.get(wu, dt), wcache.get(wd, dt), bg, bu, bd,
                                residual, act)

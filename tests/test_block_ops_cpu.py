@@ -96,7 +96,7 @@ def test_extension_refuses_with_numbers_in_the_message():
     with FakeTensorMode():
         x = torch.empty(4, 32, device="cuda", dtype=torch.bfloat16)
         w = torch.empty(64, 64, device="cuda", dtype=torch.bfloat16)
-        with pytest.raises(RuntimeError, match=r"w_gate must be \[64, 32\], got \[64, 64\]"):
+        with pytest.raises(ValueError, match=r"x \[4, 32\], w_gate \[64, 64\].* do not fit together"):
             ext.gated_mlp(x, w, w, w, None, None, None, None, 0)
 
 
