@@ -579,7 +579,7 @@ Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, const std::
   const auto f32 = grads[0].options().dtype(at::kFloat);
   if (v.empty()) return torch::zeros({}, f32);
   const int64_t tables = ((int64_t)v.size() + nsw::kClipTensors - 1) / nsw::kClipTensors;
-  const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>(8 * sm_count(grads[0]), total / 2048 + (int64_t)v.size()));
+  const int blocks = (int)std::max<int64_t>(1, std::min<int64_t>(16 * sm_count(grads[0]), total / 2048 + (int64_t)v.size()));
   auto partial = torch::empty({tables * blocks + 1}, f32);
   auto norm = torch::empty({}, f32);
   check(nsw::clip_tensors(v.data(), (int)v.size(), (float)max_norm, partial.data_ptr<float>(), blocks,

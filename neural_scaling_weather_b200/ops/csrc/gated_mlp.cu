@@ -182,6 +182,10 @@ __device__ __forceinline__ void add_bias32(const void* p, int dtype, int64_t nb,
 
 __device__ __forceinline__ void bulk_wait_read_3() { asm volatile("cp.async.bulk.wait_group.read 3;" ::: "memory"); }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+}
+
 // named barrier that also ANDs a predicate over its threads
 __device__ __forceinline__ bool bar_and(int id, int threads, bool v) {
   uint32_t out;
@@ -300,6 +304,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
   const int64_t num_tiles = MODE == kDw ? p.direct : m_tiles * n_tiles;
   volatile int* abort_flag = &S.abort_flag;
 
+  if (threadIdx.x == 64) {
+    prefetch_map(&p.a0);
+    prefetch_map(&p.b0);
+    if (MODE != kDown && MODE != kDh) prefetch_map(&p.b1);
+  }
   if (threadIdx.x == 0) {
     for (int s = 0; s < GS; ++s) {
       mbar_init(&S.full[s], 1);
@@ -866,6 +875,12 @@ __global__ void __launch_bounds__(kSplitThreads, NTOK <= 64 ? 2 : 1) split_kerne
   const int nkb = kb_end - kb_begin;
   volatile int* abort_flag = &S.abort_flag;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  if (threadIdx.x == 64) {
+    prefetch_map(&p.w0);
+    prefetch_map(&p.x0);
+    if (MODE == kUp || MODE == kDx) prefetch_map(&p.w1);
+    if (MODE == kDx) prefetch_map(&p.x1);
+  }
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < STAGES; ++s) {

@@ -19,16 +19,19 @@ namespace gc {
 constexpr int kThreads = 256;
 constexpr int kChunk = 8192;  // elements
 
+// N tensors: the few of a small model travel in a small table (a launch copies its parameters)
+template <int N>
 struct Table {
-  const void* in[kClipTensors];
-  void* out[kClipTensors];
-  int64_t n[kClipTensors];
-  int first[kClipTensors + 1];  // a tensor's first chunk
-  uint8_t dtype[kClipTensors];
+  const void* in[N];
+  void* out[N];
+  int64_t n[N];
+  int first[N + 1];  // a tensor's first chunk
+  uint8_t dtype[N];
   int count;
 };
 
-__device__ __forceinline__ int find(const Table& t, int chunk) {
+template <int N>
+__device__ __forceinline__ int find(const Table<N>& t, int chunk) {
   int lo = 0, hi = t.count;  // the last tensor whose first chunk is <= chunk
   while (hi - lo > 1) {
     const int mid = (lo + hi) >> 1;
@@ -110,7 +113,8 @@ __device__ __forceinline__ void chunk_scale(const T* p, T* o, int len, float c) 
   for (int i = i0 + threadIdx.x; i < len; i += kThreads) o[i] = from_f<T>(to_f(p[i]) * c);
 }
 
-__global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ Table t, float* partial) {
+template <int N>
+__global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__ Table<N> t, float* partial) {
   float a = 0.f;
   const int chunks = t.first[t.count];
   for (int c = blockIdx.x; c < chunks; c += gridDim.x) {
@@ -128,7 +132,8 @@ __global__ void __launch_bounds__(kThreads) sumsq_kernel(const __grid_constant__
   if (threadIdx.x == 0) partial[blockIdx.x] = a;
 }
 
-__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table t, const float* partial,
+template <int N>
+__global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__ Table<N> t, const float* partial,
                                                          int partials, float max_norm, float* norm_out) {
   float a = 0.f;
   for (int i = threadIdx.x; i < partials; i += kThreads) a += partial[i];
@@ -154,8 +159,9 @@ __global__ void __launch_bounds__(kThreads) scale_kernel(const __grid_constant__
 
 }  // namespace gc
 
-// Tables of at most kClipTensors tensors and 2^31 - 1 chunks; each launch over `blocks` blocks
-static bool fill(gc::Table& t, const ClipTensor* v, int count) {
+// false: more than 2^31 - 1 chunks
+template <int N>
+static bool fill(gc::Table<N>& t, const ClipTensor* v, int count) {
   t.count = count;
   int64_t chunks = 0;
   for (int i = 0; i < count; ++i) {
@@ -171,23 +177,30 @@ static bool fill(gc::Table& t, const ClipTensor* v, int count) {
   return true;
 }
 
-cudaError_t clip_tensors(const ClipTensor* v, int count, float max_norm, float* partial, int blocks, float* norm,
-                         cudaStream_t s) {
+template <int N>
+static cudaError_t clip_tables(const ClipTensor* v, int count, float max_norm, float* partial, int blocks, float* norm,
+                               cudaStream_t s) {
   // every table's blocks write their own partials; every scaling launch adds all of them
-  const int tables = std::max(1, (count + kClipTensors - 1) / kClipTensors);
-  gc::Table t;
+  const int tables = (count + N - 1) / N;
+  gc::Table<N> t;
   for (int pass = 0; pass < 2; ++pass)
     for (int k = 0; k < tables; ++k) {
       const int i = pass ? tables - 1 - k : k;
-      const int first = i * kClipTensors;
-      if (!fill(t, v + first, std::min(kClipTensors, count - first))) return cudaErrorInvalidValue;
+      if ((pass == 0 || tables > 1) && !fill(t, v + i * N, std::min(N, count - i * N))) return cudaErrorInvalidValue;
       if (pass == 0)
-        gc::sumsq_kernel<<<blocks, gc::kThreads, 0, s>>>(t, partial + i * blocks);
+        gc::sumsq_kernel<N><<<blocks, gc::kThreads, 0, s>>>(t, partial + i * blocks);
       else
-        gc::scale_kernel<<<blocks, gc::kThreads, 0, s>>>(t, partial, tables * blocks, max_norm, k == 0 ? norm : nullptr);
+        gc::scale_kernel<N>
+            <<<blocks, gc::kThreads, 0, s>>>(t, partial, tables * blocks, max_norm, k == 0 ? norm : nullptr);
       NSW_CUDA_CHECK(cudaGetLastError());
     }
   return cudaSuccess;
+}
+
+cudaError_t clip_tensors(const ClipTensor* v, int count, float max_norm, float* partial, int blocks, float* norm,
+                         cudaStream_t s) {
+  if (count <= 32) return clip_tables<32>(v, count, max_norm, partial, blocks, norm, s);
+  return clip_tables<kClipTensors>(v, count, max_norm, partial, blocks, norm, s);
 }
 
 }  // namespace nsw
