@@ -832,17 +832,19 @@ struct SmemS {
   int abort_flag;
 };
 
-// four consecutive columns of a row, those below N
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, int64_t left, bool vec, float* f) {
-  if (vec && left >= 4) {
-    uint2 w = *reinterpret_cast<const uint2*>(p);
-    unpack2(w.x, f, T());
-    unpack2(w.y, f + 2, T());
-  } else {
+// four consecutive 16-bit columns of a row, those of the first `left` (zeros after)
+__device__ __forceinline__ uint2 load4(const uint16_t* p, int64_t left, bool vec) {
+  if (vec && left >= 4) return *reinterpret_cast<const uint2*>(p);
+  uint32_t w[2] = {0, 0};
 #pragma unroll
-    for (int j = 0; j < 4; ++j) f[j] = j < left ? to_f(p[j]) : 0.f;
-  }
+  for (int j = 0; j < 4; ++j)
+    if (j < left) w[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
+  return make_uint2(w[0], w[1]);
+}
+template <typename T>
+__device__ __forceinline__ void unpack4(uint2 w, float* f) {
+  unpack2(w.x, f, T());
+  unpack2(w.y, f + 2, T());
 }
 template <typename T>
 __device__ __forceinline__ void store4(T* p, int64_t left, bool vec, const float* f) {
@@ -968,11 +970,42 @@ __global__ void __launch_bounds__(kSplitThreads, NTOK <= 64 ? 2 : 1) split_kerne
     }
   }
   __syncwarp();
-  // the accumulator is complete (and every stage read): all warps wait for it before the stages become `part`
-  if (warp >= 1) mbar_wait(&S.tmem_full, 0, abort_flag, err);
-  tc_fence_after();
-  __syncthreads();
+  // what the epilogue reads from global memory is on its way while the products run
+  constexpr int kQuads = kUnits / 4;
+  constexpr int kBatch = MODE == kUp ? 2 : 4;  // items whose loads are in flight together
+  static_assert(kSplitThreads % kQuads == 0, "a thread's columns");
+  const int tokens = (int)(p.M - m0 < NTOK ? p.M - m0 : NTOK);
+  const int64_t col = n0 + 4 * (threadIdx.x % kQuads), left = p.N - col;
+  const bool vec = ((p.ldout | p.ldaux | p.ldin) & 3) == 0 &&
+                   ((reinterpret_cast<uintptr_t>(p.out0) | reinterpret_cast<uintptr_t>(p.out1) |
+                     reinterpret_cast<uintptr_t>(p.out2) | reinterpret_cast<uintptr_t>(p.in0) |
+                     reinterpret_cast<uintptr_t>(p.in1)) & 7) == 0;
+  const int step = slices * (kSplitThreads / kQuads);
+  int t0 = (slice * kSplitThreads + threadIdx.x) / kQuads;
+  if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
+  float b0[4] = {0.f, 0.f, 0.f, 0.f}, b1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    if (p.bias0 && j < left) b0[j] = ld_bias(p.bias0, p.bias_dtype, col + j);
+    if (MODE == kUp && p.bias1 && j < left) b1[j] = ld_bias(p.bias1, p.bias_dtype, col + j);
+  }
+  uint2 in0[kBatch], in1[kBatch];
+  auto fetch = [&](int first) {
+#pragma unroll
+    for (int b = 0; b < kBatch; ++b) {
+      const int tok = first + b * step;
+      in0[b] = in1[b] = make_uint2(0, 0);
+      if (tok >= tokens || left <= 0 || !p.in0) continue;
+      const int64_t at = (m0 + tok) * p.ldin + col;
+      in0[b] = load4(reinterpret_cast<const uint16_t*>(p.in0) + at, left, vec);
+      if (MODE == kDh) in1[b] = load4(reinterpret_cast<const uint16_t*>(p.in1) + at, left, vec);
+    }
+  };
+  fetch(t0);
   if (warp >= 2) {
+    // the accumulator is complete, so every stage has landed and been read: they become `part`
+    mbar_wait(&S.tmem_full, 0, abort_flag, err);
+    tc_fence_after();
     const int q = warp & 3;
 #pragma unroll 1
     for (int c = 32 * ((warp - 2) >> 2); c < NTOK; c += 64) {
@@ -987,51 +1020,37 @@ __global__ void __launch_bounds__(kSplitThreads, NTOK <= 64 ? 2 : 1) split_kerne
   tc_fence_after();
   if (warp == 1)
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(NTOK));
-  if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
 
-  constexpr int kQuads = kUnits / 4;
-  constexpr int kBatch = MODE == kUp ? 2 : 4;  // items whose loads are in flight together
-  static_assert(kSplitThreads % kQuads == 0, "a thread's columns");
-  const int tokens = (int)(p.M - m0 < NTOK ? p.M - m0 : NTOK);
-  const int64_t col = n0 + 4 * (threadIdx.x % kQuads), left = p.N - col;
-  const bool vec = ((p.ldout | p.ldaux | p.ldin) & 3) == 0 &&
-                   ((reinterpret_cast<uintptr_t>(p.out0) | reinterpret_cast<uintptr_t>(p.out1) |
-                     reinterpret_cast<uintptr_t>(p.out2) | reinterpret_cast<uintptr_t>(p.in0) |
-                     reinterpret_cast<uintptr_t>(p.in1)) & 7) == 0;
-  float b0[4] = {0.f, 0.f, 0.f, 0.f}, b1[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    if (p.bias0 && j < left) b0[j] = ld_bias(p.bias0, p.bias_dtype, col + j);
-    if (MODE == kUp && p.bias1 && j < left) b1[j] = ld_bias(p.bias1, p.bias_dtype, col + j);
-  }
-  const int step = slices * (kSplitThreads / kQuads);
   const float* mine = &S.part[0][4 * (threadIdx.x % kQuads)];
-  for (int t0 = (slice * kSplitThreads + threadIdx.x) / kQuads; t0 < tokens && left > 0; t0 += step * kBatch) {
+  for (; t0 < tokens && left > 0; t0 += step * kBatch) {
     float f[kBatch][4], u[kBatch][4];
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int tok = t0 + b * step;
 #pragma unroll
       for (int j = 0; j < 4; ++j) f[b][j] = b0[j], u[b][j] = b1[j];
-      if (tok >= tokens) continue;
-      const int64_t row = m0 + tok;
-      if (MODE == kDown && p.in0)
-        load4<T>(reinterpret_cast<const T*>(p.in0) + row * p.ldin + col, left, vec, u[b]);
+      if (MODE == kDown) {
+        unpack4<T>(in0[b], u[b]);  // the residual (zeros without one)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) f[b][j] += u[b][j];
+      }
       if (MODE == kDh) {
-        load4<T>(reinterpret_cast<const T*>(p.in0) + row * p.ldin + col, left, vec, b0);  // (no bias: g)
-        load4<T>(reinterpret_cast<const T*>(p.in1) + row * p.ldin + col, left, vec, u[b]);
+        float g[4];
+        unpack4<T>(in0[b], g);
+        unpack4<T>(in1[b], u[b]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          const ActParts a = act_parts(b0[j], p.act);
+          const ActParts a = act_parts(g[j], p.act);
           f[b][j] = u[b][j] * a.slope;
           u[b][j] = a.val;
         }
       }
     }
+    const int now = t0;
+    if (p.in0) fetch(t0 + step * kBatch);
     // every slice's partials, in slice order
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int tok = t0 + b * step;
+      const int tok = now + b * step;
       if (tok >= tokens) continue;
       float4 o[kMaxSlices], o2[MODE == kUp ? kMaxSlices : 1];
 #pragma unroll
@@ -1066,7 +1085,7 @@ __global__ void __launch_bounds__(kSplitThreads, NTOK <= 64 ? 2 : 1) split_kerne
     }
 #pragma unroll
     for (int b = 0; b < kBatch; ++b) {
-      const int tok = t0 + b * step;
+      const int tok = now + b * step;
       if (tok >= tokens) continue;
       const int64_t row = m0 + tok;
       if (MODE == kUp && p.out1) {
@@ -1076,13 +1095,14 @@ __global__ void __launch_bounds__(kSplitThreads, NTOK <= 64 ? 2 : 1) split_kerne
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
         if (MODE == kUp) f[b][j] = act_parts(f[b][j], p.act).val * u[b][j];
-        if (MODE == kDown) f[b][j] += p.in0 ? u[b][j] : 0.f;
       }
       if (MODE == kDh) store4<T>(reinterpret_cast<T*>(p.out1) + row * p.ldaux + col, left, vec, u[b]);
       store4<T>(reinterpret_cast<T*>(p.out0) + row * p.ldout + col, left, vec, f[b]);
     }
   }
-  cluster_sync_all();  // the peers have read this CTA's partials
+  // the peers have read this CTA's partials (their loads have returned: nothing needs to be released)
+  __syncwarp();
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::: "memory");
 }
 
 template <typename T, int MODE, int NTOK, int STAGES>
@@ -1166,11 +1186,11 @@ static int64_t split_room(int slices) {
 }
 
 // Tokens a tile and depth slices of the split form, and whether it beats gated_kernel.  Both forms' times are
-// modelled in microseconds, launch to launch: waves of CTAs times (k-blocks, final sums, fixed part).  The
-// constants were fitted to 1500 timings of both forms over the four products at 17 to 2048 rows and widths
-// 128 x 344 to 2048 x 5464; the plan's choice is on average 3.5% (at most 28%) above the best of them, the
-// general form alone 54%.  For example, 256 rows of h [.., 2736] times Wd [1024, ..]: 18.9 us in gated_kernel
-// (4 tiles), 9.5 us as 64 x 4.
+// modelled in microseconds, launch to launch: waves of CTAs times (k-blocks, final sums, fixed part), and for
+// the split form the operands' way from L2.  The constants were fitted to 1500 timings of both forms over the
+// four products at 17 to 2048 rows and widths 128 x 344 to 2048 x 5464; the plan's choice is on average 2% (at
+// most 25%) above the best of them, the general form alone 66%.  For example, 256 rows of h [.., 2736] times Wd
+// [1024, ..]: 18.9 us in gated_kernel (4 tiles), 8.8 us as 64 x 4.
 struct SplitPlan {
   int ntok, slices;
   bool use;
@@ -1178,19 +1198,19 @@ struct SplitPlan {
 static SplitPlan plan_split(const GatedArgs& a) {
   const int64_t units = a.mode == kGatedUp ? 64 : 128, cols = a.mode == kGatedUp ? 128 : 256;
   const int64_t kb = (a.K + BK - 1) / BK * (a.mode == kGatedDx ? 2 : 1);
-  const double tail = a.mode == kGatedUp || a.mode == kGatedDh ? 0.052 : 0.035;  // final sums of a token
+  const double tail = a.mode == kGatedUp || a.mode == kGatedDh ? 0.042 : 0.028;  // final sums of a token
   SplitPlan best = {0, 1, false};
   double best_cost = 1e30;
   for (int ntok = 32; ntok <= 256; ntok *= 2) {
-    const double step = ntok == 32 ? 0.28 : ntok == 64 ? 0.31 : ntok == 128 ? 0.32 : 0.48;
+    const double step = ntok == 32 ? 0.22 : ntok == 64 ? 0.25 : ntok == 128 ? 0.28 : 0.40;
     const int64_t tiles = (a.M + ntok - 1) / ntok * ((a.N + units - 1) / units);
-    for (int slices = 1; slices <= kMaxSlices && slices <= kb; slices *= 2) {
+    const double l2 = 0.019 * 1e-6 * (double)(tiles * kb * (BM + ntok) * BK * 2);  // 0.019 us a megabyte
+    for (int slices = 1, log2 = 0; slices <= kMaxSlices && slices <= kb; slices *= 2, ++log2) {
       const int64_t one = split_room(slices), room = one * (ntok <= 64 ? 2 : 1);  // 64 tokens: two CTAs a SM
       const int64_t ctas = tiles * slices, waves = (ctas + room - 1) / room;
-      const double crowd = 1.0 + 0.15 * std::max<int64_t>(0, std::min(ctas, room) - one) / (double)one;
-      const double cost = waves * ((double)((kb + slices - 1) / slices) * step * crowd +
-                                   tail * std::min<int64_t>(a.M, ntok) / slices + 3.75) +
-                          0.5 + 0.55 * (slices > 4 ? 3 : slices > 2 ? 2 : slices > 1 ? 1 : 0);
+      const double cost = 1.0 + l2 + (room > one && ctas > one ? 1.3 : 0.0) + 0.45 * log2 +
+                          waves * ((double)((kb + slices - 1) / slices) * step +
+                                   tail * std::min<int64_t>(a.M, ntok) / slices + 2.85);
       if (cost < best_cost) {
         best_cost = cost;
         best.ntok = ntok;
@@ -1199,8 +1219,8 @@ static SplitPlan plan_split(const GatedArgs& a) {
     }
   }
   const int64_t tiles = ((a.M + BM2 - 1) / BM2) * ((a.N + cols - 1) / cols), pairs = sm_count() / 2;
-  const double fixed = a.mode == kGatedUp ? 0.75 : a.mode == kGatedDown ? 1.1 : a.mode == kGatedDh ? 5.4 : 0.0;
-  const double general = 5.0 + (double)((tiles + pairs - 1) / pairs) * (0.31 * kb + fixed);
+  const double fixed = a.mode == kGatedUp ? 0.85 : a.mode == kGatedDown ? 1.65 : a.mode == kGatedDh ? 6.0 : 0.0;
+  const double general = 4.9 + (double)((tiles + pairs - 1) / pairs) * (0.314 * kb + fixed);
   best.use = best_cost < general && (a.M + best.ntok - 1) / best.ntok <= 65535;
   return best;
 }
