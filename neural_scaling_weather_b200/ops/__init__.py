@@ -170,7 +170,7 @@ def norm_gate_residual(y: torch.Tensor, skip: torch.Tensor, w_post: torch.Tensor
     ``s = skip_scale skip + gate * rms_norm(y, w_post)`` and ``n = rms_norm(s, w_next)``.
 
     ``y`` (a branch's output) and ``skip`` (..., D); ``w_post``, ``w_next`` (D,); ``gate`` (D,), or one row for
-    each index of the first dimension (samples, D), or None for ones.  ``n`` is None without ``w_next`` (the
+    each index of the first dimension (samples, D; at most 65535), or None for ones.  D is at most 16384 on CUDA.  ``n`` is None without ``w_next`` (the
     last branch of a network)."""
     if _use_cuda(y):  # checks the shapes itself
         return fused.norm_gate_residual_cuda(y, skip, w_post, gate, w_next, skip_scale, eps)

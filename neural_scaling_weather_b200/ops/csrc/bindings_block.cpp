@@ -28,6 +28,11 @@ int dt_code(const Tensor& t, const char* what) {
   return -1;
 }
 
+// in a node's backward: gradients of gradients would silently be missing
+void once_differentiable(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, ": second derivatives are not implemented (create_graph=True)");
+}
+
 int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // A [rows, cols] operand the TMA kernels can read: unit column stride, 16-byte aligned rows.
@@ -96,7 +101,8 @@ GatedShape gated_shape(const Tensor& x, const Tensor& wg, const Tensor& wu, cons
 }
 
 // y = (act(x wg^T + bg) * (x wu^T + bu)) wd^T + bd + residual.  With save, also what the backward reads:
-// returns {y} or {y, x (as read), g, u, h} (rows of g, u and h padded to a multiple of 8 elements).
+// returns {y} or {y, x, g, u, h, wg, wu, wd} with x and the weights as read (copies with padded rows where theirs are
+// not aligned) and the rows of g, u and h padded to a multiple of 8 elements.
 std::vector<Tensor> gated_mlp_fwd(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd,
                                   const OptTensor& bg, const OptTensor& bu, const OptTensor& bd,
                                   const OptTensor& residual, int64_t act, bool save) {
@@ -112,7 +118,7 @@ std::vector<Tensor> gated_mlp_fwd(const Tensor& x, const Tensor& wg, const Tenso
   if (d.M == 0) {
     auto y = torch::empty({0, d.N}, opt), e = torch::empty({0, d.Hp}, opt);
     if (!save) return {y};
-    return {y, x, e, e, e};
+    return {y, x, e, e, e, wg, wu, wd};
   }
   auto h = torch::empty({d.M, d.Hp}, opt);
   nsw::GatedArgs up{}, down{};
@@ -185,7 +191,7 @@ std::vector<Tensor> gated_mlp_fwd(const Tensor& x, const Tensor& wg, const Tenso
   check(nsw::gated_product(down, true, stream()), "gated_mlp down");
   y = packed(y, d.N);
   if (!save) return {y};
-  return {y, xa.t, g, u, h};
+  return {y, xa.t, g, u, h, ga.t, ua.t, da.t};
 }
 
 // Where a parameter's gradient goes: added into the given fp32 buffer, or a fresh tensor (16-bit where that is
@@ -340,7 +346,7 @@ struct GatedNode : public torch::autograd::Function<GatedNode> {
                         const OptTensor& residual, int64_t act) {
     auto out = gated_mlp_fwd(flat(x), wg, wu, wd, bg, bu, bd, flat(residual), act, true);
     ctx->saved_data["shape"] = x.sizes().vec();
-    ctx->save_for_backward({out[1], wg, wu, wd, out[2], out[3], out[4]});
+    ctx->save_for_backward({out[1], out[5], out[6], out[7], out[2], out[3], out[4]});
     ctx->saved_data["act"] = act;
     int64_t given = 0, type = -1;  // which optional inputs there are, and the biases' type
     int bit = 0;
@@ -357,6 +363,7 @@ struct GatedNode : public torch::autograd::Function<GatedNode> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grad) {
+    once_differentiable("gated_mlp");
     const auto v = ctx->get_saved_variables();
     const int64_t bias = ctx->saved_data["bias"].toInt(), given = ctx->saved_data["given"].toInt();
     bool need[8];
@@ -511,6 +518,7 @@ struct NormGateNode : public torch::autograd::Function<NormGateNode> {
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grad) {
+    once_differentiable("norm_gate_residual");
     const auto v = ctx->get_saved_variables();
     const auto o = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     const auto c = [&](size_t i) {

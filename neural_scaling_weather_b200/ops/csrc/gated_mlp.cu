@@ -36,7 +36,7 @@ namespace tc {
 enum : int { kUp = 0, kDown = 1, kDh = 2, kDx = 3, kDw = 4 };
 // Epilogue warps and 2 KB tile buffers of each.  kDh loads two tiles and stores two for each 32 columns, more
 // latency than arithmetic: sixteen warps with one pair of buffers each (413 us with eight warps and two pairs
-// at 64800 x 2736 x 1024, KDH16 us with sixteen).
+// at 64800 x 2736 x 1024, 365 us with sixteen and the column sums, uniform operands).
 constexpr int epi_warps(int mode) { return mode == kDh ? 16 : 8; }
 constexpr int epi_bufs(int mode) { return 32 / epi_warps(mode); }
 constexpr int stages(int mode) { return mode == kDh ? 4 : 5; }  // 32 KB a CTA; kDh's column sums take one
@@ -1471,28 +1471,27 @@ static cudaError_t launch_skinny(const SkinnyParams& p, bool vec, cudaStream_t s
 }
 
 // dst[i, j] = src[i s0 + j s1] (16-bit), rows of ld elements: operands whose rows are not 16-byte aligned.  A
-// thread copies eight elements, one 16-byte store where dst's rows allow it (5.6 MB: PADUS us).
+// thread copies eight elements of one row, one 16-byte store where dst's rows allow it, and nothing else: with
+// threads that loop over groups too few loads are in flight (5.6 MB: 10.5 us; as it is, 4.7 us).
 __global__ void __launch_bounds__(256) pad_copy_kernel(const uint16_t* __restrict__ src, int64_t s0, int64_t s1,
-                                                       uint16_t* __restrict__ dst, int64_t ld, int64_t rows,
-                                                       int64_t cols, int vec) {
-  const int64_t groups = (cols + 7) / 8;
-  for (int64_t m = blockIdx.y; m < rows; m += gridDim.y) {
-    const uint16_t* p = src + m * s0;
-    uint16_t* d = dst + m * ld;
-    for (int64_t g = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; g < groups; g += (int64_t)gridDim.x * blockDim.x) {
-      const int64_t c = 8 * g;
-      uint32_t w[4] = {0, 0, 0, 0};
+                                                       uint16_t* __restrict__ dst, int64_t ld, int64_t total,
+                                                       uint32_t groups, int64_t cols, int vec) {
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= total) return;
+  const int64_t m = i < ((int64_t)1 << 32) ? (int64_t)((uint32_t)i / groups) : i / groups;
+  const int64_t c = 8 * (i - m * groups);
+  const uint16_t* p = src + m * s0 + c * s1;
+  uint16_t* d = dst + m * ld + c;
+  uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (c + j < cols) w[j >> 1] |= (uint32_t)p[(c + j) * s1] << (16 * (j & 1));
-      if (vec && c + 8 <= ld) {
-        *reinterpret_cast<uint4*>(d + c) = make_uint4(w[0], w[1], w[2], w[3]);
-      } else {
+  for (int j = 0; j < 8; ++j)
+    if (c + j < cols) w[j >> 1] |= (uint32_t)p[j * s1] << (16 * (j & 1));
+  if (vec && c + 8 <= ld) {
+    *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-          if (c + j < cols) d[c + j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
-      }
-    }
+    for (int j = 0; j < 8; ++j)
+      if (c + j < cols) d[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
   }
 }
 
@@ -1650,11 +1649,12 @@ cudaError_t gated_skinny(const GatedArgs& a, bool dependent, cudaStream_t s) {
 cudaError_t pad_copy(const void* src, int64_t s0, int64_t s1, void* dst, int64_t ld, int64_t rows, int64_t cols,
                      cudaStream_t s) {
   if (rows <= 0 || cols <= 0) return cudaSuccess;
-  const int64_t groups = (cols + 7) / 8;
-  const dim3 grid((unsigned)std::min<int64_t>((groups + 255) / 256, 1024), (unsigned)std::min<int64_t>(rows, 65535), 1);
+  const int64_t groups = (cols + 7) / 8, total = rows * groups;
+  if ((total + 255) / 256 > INT32_MAX) return cudaErrorInvalidValue;
   const int vec = ld % 8 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
-  gated::pad_copy_kernel<<<grid, 256, 0, s>>>(reinterpret_cast<const uint16_t*>(src), s0, s1,
-                                              reinterpret_cast<uint16_t*>(dst), ld, rows, cols, vec);
+  gated::pad_copy_kernel<<<(unsigned)((total + 255) / 256), 256, 0, s>>>(reinterpret_cast<const uint16_t*>(src), s0, s1,
+                                                                         reinterpret_cast<uint16_t*>(dst), ld, total,
+                                                                         (uint32_t)groups, cols, vec);
   return cudaGetLastError();
 }
 

@@ -17,6 +17,7 @@ import weakref
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd.function import once_differentiable
 
 from . import gradsink
 from . import weights as wcache
@@ -388,8 +389,8 @@ class _GatedMLP(torch.autograd.Function):
         K, N = wg.shape[1], wd.shape[0]
         W = [wcache.get(w, dt) for w in (wg, wu, wd)]
         res = None if residual is None else _rows(residual, N).to(dt)
-        y, *saved = ext.gated_mlp_fwd(_rows(x, K).to(dt), *W, bg, bu, bd, res, act, True)
-        ctx.save_for_backward(*saved)
+        y, x2, g, u, h, *W = ext.gated_mlp_fwd(_rows(x, K).to(dt), *W, bg, bu, bd, res, act, True)
+        ctx.save_for_backward(x2, g, u, h)
         ctx.params, ctx.biases, ctx.W, ctx.act = (wg, wu, wd), (bg, bu, bd), W, act
         ctx.x_shape, ctx.x_dtype = x.shape, x.dtype
         ctx.res_dtype = None if residual is None else residual.dtype
@@ -398,6 +399,7 @@ class _GatedMLP(torch.autograd.Function):
         return y.view(*x.shape[:-1], N)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dy):
         ext = require()
         x2, g, u, h = ctx.saved_tensors

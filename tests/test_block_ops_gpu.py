@@ -207,6 +207,24 @@ def test_gated_is_deterministic_and_runs_on_the_current_stream(M):
     assert torch.equal(plain, again_plain)
 
 
+@pytest.mark.parametrize("M", [33, 600])
+def test_gated_some_gradients_only(M):
+    """Frozen weights, a frozen input, a single bias, and a residual alone: the asked gradients are the full
+    call's, the others are not computed."""
+    x, w, b, res, dy = gated_inputs(M, 64, 136, 64, torch.bfloat16, True, True)
+    full = [t.clone().requires_grad_() for t in [x] + w + b + [res]]
+    ref = torch.autograd.grad(ops.gated_mlp(*full[:7], residual=full[7]), full, dy)
+    for pick in ([0], [2], [3, 6], [7], [0, 4]):
+        args = [t.clone().requires_grad_(i in pick) for i, t in enumerate([x] + w + b + [res])]
+        got = torch.autograd.grad(ops.gated_mlp(*args[:7], residual=args[7]), [args[i] for i in pick], dy)
+        assert all(torch.equal(g, ref[i]) for g, i in zip(got, pick))
+    one = [x, *w, None, b[1].clone().requires_grad_(), None]
+    y = ops.gated_mlp(*one)
+    (db,) = torch.autograd.grad(y, [one[5]], dy)
+    _, exact = gated_exact(x, w, [None, b[1], None], None, "silu", dy)
+    assert rel(db, exact[-1]) < 4 * U[torch.bfloat16]
+
+
 def test_gated_refusals():
     x, w, b, res, _ = gated_inputs(4, 64, 72, 64, torch.bfloat16, True, True)
     with pytest.raises(ValueError, match="activation"):
@@ -419,6 +437,16 @@ def test_clip_grad_norm_refusals():
         ops.clip_grad_norm([g[0], torch.ones(3)], 1.0)
     with pytest.raises(RuntimeError, match="dtype"):
         ops.clip_grad_norm([torch.ones(3, device=DEV, dtype=torch.float64)], 1.0)
+
+
+def test_second_derivatives_are_refused():
+    x, w, _, _, dy = gated_inputs(4, 64, 72, 64, BF16, False, False)
+    x.requires_grad_()
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(ops.gated_mlp(x, *w), x, dy, create_graph=True)
+    s, _ = ops.norm_gate_residual(x, x.detach(), torch.ones(64, device=DEV))
+    with pytest.raises(RuntimeError, match="second derivatives"):
+        torch.autograd.grad(s, x, dy, create_graph=True)
 
 
 # --------------------------------------------------------------------------- in the model
