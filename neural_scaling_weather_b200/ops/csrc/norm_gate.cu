@@ -214,14 +214,27 @@ __global__ void __launch_bounds__(WPR > 8 ? 32 * WPR : 256) fwd_kernel(const Par
   }
 }
 
-// two blocks of eight warps an SM: the next row's four operands are loaded while a row is worked on, so that
-// about 64 KB an SM are in flight (one block with 16 elements a lane and no prefetch: 245 us at
-// 64800 x 1024 instead of 167)
+// 16 bytes into shared memory behind the thread's back (zeros where !ok)
+__device__ __forceinline__ void copy_async(void* dst, const void* src, bool ok) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(dst)), "l"(src), "r"(ok ? 16 : 0) : "memory");
+}
+
+// Rows ahead that the backward's operands are copied (kRing - 1) where a ring of kRing rows fits; each thread reads
+// back only what it copied itself, so there is no barrier.
+constexpr int kRing = 4;
+template <bool VEC, int WPR, int NV>
+constexpr bool use_ring() {
+  return VEC && WPR <= 8 && NV == 1;
+}
+
+// Two blocks of eight warps an SM; what bounds it is the bytes in flight.  64800 x 1024: 245 us with 16 elements a
+// lane and no prefetch, 167 with 8 and the next row's operands in registers, 142 with packed arithmetic, 132 with
+// the operands of three rows ahead in shared memory.
 template <typename T, bool VEC, int WPR, int NV>
 __global__ void __launch_bounds__(WPR > 8 ? 32 * WPR : 256, WPR > 8 ? 1 : 2) bwd_kernel(const Params p) {
   constexpr int GL = 32 * WPR;
   constexpr int RPB = WPR > 8 ? 1 : 8 / WPR;
-  extern __shared__ float sums[];  // [2][n]
+  extern __shared__ __align__(16) float sums[];  // [2][n], then the ring [kRing][4][threads] of 16 bytes
   __shared__ float red[RPB][3][WPR][2];
   const int rg = threadIdx.x / GL, gl = threadIdx.x % GL;
   const int64_t sample = blockIdx.y;
@@ -255,18 +268,45 @@ __global__ void __launch_bounds__(WPR > 8 ? 32 * WPR : 256, WPR > 8 ? 1 : 2) bwd
   };
   const int64_t step = (int64_t)gridDim.x * RPB;
   int64_t r = (int64_t)blockIdx.x * RPB + rg;
-  if (r < p.rows) fetch(r);
+  constexpr bool kUseRing = use_ring<VEC, WPR, NV>();
+  uint4* ring = reinterpret_cast<uint4*>(sums + ((2 * p.n + 3) & ~3)) + threadIdx.x;
+  auto copy = [&](int64_t row, int slot) {
+    const bool ok = row < p.rows && 8 * gl < p.n;
+    const int64_t at = ok ? (sample * p.rows + row) * p.n + 8 * gl : 0;
+    const void* src[4] = {p.y, p.skip, p.ds, p.dn};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+      copy_async(ring + (slot * 4 + k) * 256, reinterpret_cast<const T*>(src[k] ? src[k] : p.y) + at, ok && src[k]);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  int slot = 0;
+  if (kUseRing) {
+#pragma unroll
+    for (int k = 0; k < kRing - 1; ++k) copy(r + k * step, k);
+  } else if (r < p.rows) {
+    fetch(r);
+  }
   for (; r < p.rows; r += step) {
     const int64_t at = (sample * p.rows + r) * p.n;
     uint4 yr[NV], kr[NV], dsr[NV], dnr[NV];
+    if (kUseRing) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+      yr[0] = ring[(slot * 4 + 0) * 256];
+      kr[0] = ring[(slot * 4 + 1) * 256];
+      dsr[0] = ring[(slot * 4 + 2) * 256];
+      dnr[0] = ring[(slot * 4 + 3) * 256];
+      copy(r + (kRing - 1) * step, (slot + kRing - 1) % kRing);
+      slot = (slot + 1) % kRing;
+    } else {
 #pragma unroll
-    for (int v = 0; v < NV; ++v) {
-      yr[v] = nxt[0][v];
-      kr[v] = nxt[1][v];
-      dsr[v] = nxt[2][v];
-      dnr[v] = nxt[3][v];
+      for (int v = 0; v < NV; ++v) {
+        yr[v] = nxt[0][v];
+        kr[v] = nxt[1][v];
+        dsr[v] = nxt[2][v];
+        dnr[v] = nxt[3][v];
+      }
+      if (r + step < p.rows) fetch(r + step);
     }
-    if (r + step < p.rows) fetch(r + step);
     const F2 zero = pack2(0.f, 0.f), c2 = pack2(p.c, p.c);
     F2 y[NV][4], t = zero;
 #pragma unroll
@@ -402,7 +442,7 @@ static cudaError_t launch_fwd(const Params& p, dim3 grid, cudaStream_t s) {
 template <typename T, bool VEC, int WPR, int NV>
 static cudaError_t launch_bwd(const Params& p, dim3 grid, cudaStream_t s) {
   auto k = bwd_kernel<T, VEC, WPR, NV>;
-  const size_t smem = 2 * sizeof(float) * p.n;
+  const size_t smem = sizeof(float) * ((2 * p.n + 3) & ~3) + (use_ring<VEC, WPR, NV>() ? kRing * 4 * 256 * 16 : 0);
   if (smem > 48 * 1024) NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   k<<<grid, WPR > 8 ? 32 * WPR : 256, smem, s>>>(p);
   return cudaGetLastError();
