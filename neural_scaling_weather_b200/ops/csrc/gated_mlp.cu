@@ -217,33 +217,33 @@ __device__ __forceinline__ void ring_store(const CUtensorMap* map, const float* 
   ++ring;
 }
 
-// 32 columns of one row of a weight gradient by plain stores: fp32 (added to what is there), or 16-bit rows
-// that are not 16-byte aligned
+// A 32 x 32 tile of a weight gradient by plain stores: fp32 (added to what is there), or 16-bit rows that are not
+// 16-byte aligned.  The lanes' rows are turned through `t` (4 KB, element (r, c) at 32 r + (c ^ r): conflict-free
+// both ways), so that each store is a row segment.
 template <typename T>
-__device__ __forceinline__ void dw_row_store(const DwSeg& p, int64_t row, int64_t nb, const float* f) {
-  if (p.out_f32) {
-    float* d = reinterpret_cast<float*>(p.D) + row * p.ldd + nb;
-    if (nb + 32 <= p.N && (p.ldd & 3) == 0) {
+__device__ __forceinline__ void dw_tile_store(const DwSeg& p, float* t, int64_t row_base, int64_t nb, const float* f,
+                                              int lane) {
+  if (lane == 0) bulk_wait_read_0();  // an earlier tile may still leave from these buffers
+  __syncwarp();
 #pragma unroll
-      for (int v = 0; v < 8; ++v) {
-        float4 o = make_float4(f[4 * v], f[4 * v + 1], f[4 * v + 2], f[4 * v + 3]);
-        if (p.accumulate) {
-          const float4 old = reinterpret_cast<const float4*>(d)[v];
-          o.x += old.x, o.y += old.y, o.z += old.z, o.w += old.w;
-        }
-        reinterpret_cast<float4*>(d)[v] = o;
+  for (int j = 0; j < 32; ++j) t[32 * lane + (j ^ lane)] = f[j];
+  __syncwarp();
+  const int64_t col = nb + lane;
+  const int rows = (int)(p.M - row_base < 32 ? p.M - row_base : 32);
+  if (col < p.N) {
+#pragma unroll 8
+    for (int r = 0; r < rows; ++r) {
+      const float v = t[32 * r + (lane ^ r)];
+      const int64_t at = (row_base + r) * p.ldd + col;
+      if (p.out_f32) {
+        float* d = reinterpret_cast<float*>(p.D) + at;
+        *d = p.accumulate ? *d + v : v;
+      } else {
+        reinterpret_cast<T*>(p.D)[at] = from_f<T>(v);
       }
-    } else {
-#pragma unroll
-      for (int j = 0; j < 32; ++j)
-        if (nb + j < p.N) d[j] = p.accumulate ? d[j] + f[j] : f[j];
     }
-  } else {
-    T* d = reinterpret_cast<T*>(p.D) + row * p.ldd + nb;
-#pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (nb + j < p.N) d[j] = from_f<T>(f[j]);
   }
+  __syncwarp();
 }
 
 // a tile of all weights' -> its weight, and the tile within it
@@ -583,8 +583,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
             continue;
           }
           if (MODE == kDw && !p.seg[seg].tma_out) {
-            const int64_t row = row_base + lane;
-            if (row < M) dw_row_store<T>(p.seg[seg], row, nb, f);
+            dw_tile_store<T>(p.seg[seg], reinterpret_cast<float*>(buf[0]), row_base, nb, f, lane);
             continue;
           }
           if (MODE == kDown && p.bias0) add_bias32(p.bias0, p.bias_dtype, nb, p.N, f);
