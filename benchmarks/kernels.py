@@ -239,10 +239,41 @@ def bench_patch(a):
     report("patchify bf16 70x720x1440 p4", ms, None, y2.numel() * 4)
 
 
+def bench_block_ops(a):
+    """The gated feed-forward network, the norms around a residual connection and gradient clipping, through their
+    public entry points (--M tokens at width 1024, hidden 2736)."""
+    from neural_scaling_weather_b200 import ops
+
+    dt, M, K, H = torch.bfloat16, a.M, 1024, 2736
+    rand = lambda *s, std=1.0: (torch.randn(*s, device="cuda") * std).to(dt)  # noqa: E731
+    x, res, dy = rand(M, K), rand(M, K), rand(M, K)
+    w = [rand(H, K, std=K ** -0.5), rand(H, K, std=K ** -0.5), rand(K, H, std=H ** -0.5)]
+    b = [rand(H), rand(H), rand(K)]
+    flops = 6 * M * K * H
+    with torch.no_grad():
+        ms = timeit(lambda: ops.gated_mlp(x, *w, *b, residual=res), a.iters)
+    report(f"gated_mlp forward {M}x{K}x{H}", ms, flops)
+    leaves = [t.requires_grad_() for t in [x] + w + b]
+    ms = timeit(lambda: torch.autograd.grad(ops.gated_mlp(x, *w, *b, residual=res), leaves, dy), a.iters)
+    report(f"gated_mlp forward + backward {M}x{K}x{H}", ms, 3 * flops)
+    y, skip = (rand(1, M, K).requires_grad_() for _ in range(2))
+    vec = [torch.ones(K, device="cuda", requires_grad=True) for _ in range(3)]
+    ds, dn = rand(1, M, K), rand(1, M, K)
+    with torch.no_grad():
+        ms = timeit(lambda: ops.norm_gate_residual(y, skip, *vec), a.iters)
+    report(f"norm_gate_residual forward {M}x{K}", ms, None, 4 * 2 * M * K)
+    ms = timeit(lambda: torch.autograd.grad(ops.norm_gate_residual(y, skip, *vec), [y, skip, *vec], [ds, dn]), a.iters)
+    report(f"norm_gate_residual forward + backward {M}x{K}", ms, None, 10 * 2 * M * K)
+    grads = [torch.randn(H, K, device="cuda") for _ in range(60)]
+    out = [torch.empty_like(g) for g in grads]
+    ms = timeit(lambda: ops.clip_grad_norm(grads, 1.0, out=out), a.iters)
+    report("clip_grad_norm 60 x 2736 x 1024 fp32 (two reads, one write)", ms, None, 3 * 4 * 60 * H * K)
+
+
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("kernel", choices=["gemm", "block", "attention", "wgrad", "amse", "rmsnorm", "adamw", "sse",
-                                       "patch", "colsum", "all"])
+                                       "patch", "colsum", "blockops", "all"])
     ap.add_argument("--M", type=int, default=64800)
     ap.add_argument("--N", type=int, default=3072)
     ap.add_argument("--K", type=int, default=1024)
@@ -274,6 +305,8 @@ def main():
         bench_amse(a)
     if a.kernel in ("patch", "all"):
         bench_patch(a)
+    if a.kernel in ("blockops", "all"):
+        bench_block_ops(a)
     if a.kernel in ("rmsnorm", "all"):
         a2 = argparse.Namespace(**vars(a))
         if a.kernel == "all":

@@ -3,10 +3,18 @@
 //   g = x Wg^T + bg,  u = x Wu^T + bu,  h = act(g) * u,  y = h Wd^T + bd + residual
 //   dh = dy Wd,  dg = dh * u * act'(g),  du = dh * act(g),  dx = dg Wg + du Wu
 //
-// act is SiLU, g / (1 + exp(-g)), or the exact GELU, g Phi(g).  Two kernel families:
+// act is SiLU, g / (1 + exp(-g)), or the exact GELU, g Phi(g).  Three kernel families:
 //
-// * gated_kernel: one persistent CTA-pair kernel (tcgen05.mma.cta_group::2, 256-row pair tiles) in four
-//   forms that differ in where their operands come from and in the epilogue:
+// * gated_kernel: one persistent CTA-pair kernel (tcgen05.mma.cta_group::2, 256-row pair tiles) in five
+//   forms that differ in where their operands come from and in the epilogue.  64800 x 1024 x 2736, bf16, in
+//   microseconds: short runs with uniform operands (no power limit), with random ones, and in a steady state at
+//   the power limit, beside the library's plain product there:
+//                                   uniform          random   steady   library, steady
+//     kUp, with g and u             481 (1510 TF)    584      678      610 (two projections, nothing else)
+//     kDown                         224 (1623 TF)    279      328      295
+//     kDh, with the column sums     364  (997 TF)    442      495      323
+//     kDx                           383 (1897 TF)    509      595      562
+//     kDw, three weights            597 (1825 TF)    822      941      936
 //     kUp    both projections at once: the pair's B tile is 128 rows of Wg (CTA 0) and the same 128
 //            rows of Wu (CTA 1), so g and u of one hidden unit land in the same TMEM lane 128 columns
 //            apart and the activation and the product happen in registers; h (and, for training, g and
@@ -17,7 +25,10 @@
 //     kDx    dg Wg + du Wu as ONE product of depth 2 H: the k-loop runs through (dg, Wg), then
 //            (du, Wu), into the same accumulator; the weights are again read MN-major as stored.
 //     kDw    the weight gradients dg^T x, du^T x and dy^T h: both operands token-major as they are, MN-major
-//            for the MMA, the depth is the tokens.  See dw_unit for the schedule.
+//            for the MMA, the depth is the tokens.  See gated_unit for the schedule.
+//   The wide forms are bound by the tensor cores at the clock that the power limit leaves; kDh, which moves 22
+//   bytes per hidden unit and token for 2 K operations, by memory and its epilogue.
+// * split_kernel: the four products of a few hundred rows, depth split over a cluster.  See there.
 // * skinny_kernel: up to 16 tokens, where the time is that of streaming the weights once.  See there.
 //
 // Sums are fp32 in TMEM / registers.  Rounded to 16 bits: g, u (kept for the backward), h, dg, du,
@@ -35,8 +46,8 @@ namespace tc {
 
 enum : int { kUp = 0, kDown = 1, kDh = 2, kDx = 3, kDw = 4 };
 // Epilogue warps and 2 KB tile buffers of each.  kDh loads two tiles and stores two for each 32 columns, more
-// latency than arithmetic: sixteen warps with one pair of buffers each (413 us with eight warps and two pairs
-// at 64800 x 2736 x 1024, 365 us with sixteen and the column sums, uniform operands).
+// latency than arithmetic: sixteen warps with one pair of buffers each, where the eight of the other forms took the
+// same time without the column sums that sixteen do beside (kUp with sixteen: no gain).
 constexpr int epi_warps(int mode) { return mode == kDh ? 16 : 8; }
 constexpr int epi_bufs(int mode) { return 32 / epi_warps(mode); }
 constexpr int stages(int mode) { return mode == kDh ? 4 : 5; }  // 32 KB a CTA; kDh's column sums take one
