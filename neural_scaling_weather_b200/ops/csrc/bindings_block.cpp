@@ -45,23 +45,23 @@ bool rows_aligned(const Tensor& t) {
   return t.stride(1) == 1 && (t.size(0) == 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1))) &&
          (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
 }
-// t itself, or a copy with padded rows where t's strides or address do not allow 16-byte accesses
-Rows aligned_rows(const Tensor& t) {
-  if (rows_aligned(t)) return {t, t.size(0) == 1 ? round8(t.size(1)) : t.stride(0)};
-  const int64_t ld = round8(t.size(1));
-  auto c = torch::empty({t.size(0), ld}, t.options());
-  check(nsw::pad_copy(t.data_ptr(), t.stride(0), t.stride(1), c.data_ptr(), ld, t.size(0), t.size(1), stream()),
-        "pad_copy");
-  return {c.narrow(1, 0, t.size(1)), ld};
-}
-// contiguous [rows, cols] view or copy of a padded buffer
-Tensor packed(const Tensor& buf, int64_t cols) {
-  if (buf.size(1) == cols) return buf;
-  auto out = torch::empty({buf.size(0), cols}, buf.options());
-  check(nsw::pad_copy(buf.data_ptr(), buf.stride(0), 1, out.data_ptr(), cols, buf.size(0), cols, stream()),
-        "pad_copy");
-  return out;
-}
+// Operands as the kernels read them: each itself, or a copy with padded rows where its strides or address do not
+// allow 16-byte accesses.  One launch makes all copies of a call.
+struct Aligner {
+  nsw::PadCopy v[nsw::kPadCopies];
+  int count = 0;
+  Rows add(const Tensor& t) {
+    if (rows_aligned(t)) return {t, t.size(0) == 1 ? round8(t.size(1)) : t.stride(0)};
+    TORCH_CHECK(count < nsw::kPadCopies, "too many operands to copy");
+    const int64_t ld = round8(t.size(1));
+    auto c = torch::empty({t.size(0), ld}, t.options());
+    v[count++] = {t.data_ptr(), c.data_ptr(), t.stride(0), t.stride(1), ld, t.size(0), t.size(1)};
+    return {c.narrow(1, 0, t.size(1)), ld};
+  }
+  void run() {
+    if (count) check(nsw::pad_copy(v, count, stream()), "pad_copy");
+  }
+};
 
 const void* opt_ptr(const OptTensor& t) { return t && t->defined() ? t->data_ptr() : nullptr; }
 
@@ -161,13 +161,16 @@ std::vector<Tensor> gated_mlp_fwd(const Tensor& x, const Tensor& wg, const Tenso
     return {y};
   }
   // all copies come before the first product: the second may start under it
-  const Rows xa = aligned_rows(x), ga = aligned_rows(wg), ua = aligned_rows(wu), da = aligned_rows(wd);
+  Aligner al;
+  const Rows xa = al.add(x), ga = al.add(wg), ua = al.add(wu), da = al.add(wd);
   Rows ra;
-  if (has_res) {
-    ra = aligned_rows(*residual);
+  if (has_res) {  // rows of any alignment are read in place
+    const bool rows = unit(*residual) && (d.M == 1 || residual->stride(0) >= d.N);
+    ra = rows ? Rows{*residual, d.M == 1 ? d.N : residual->stride(0)} : al.add(*residual);
     down.in0 = ra.ptr();
     down.ldin = ra.ld;
   }
+  al.run();
   Tensor g, u;
   if (save) {
     g = torch::empty({d.M, d.Hp}, opt);
@@ -183,13 +186,12 @@ std::vector<Tensor> gated_mlp_fwd(const Tensor& x, const Tensor& wg, const Tenso
   up.b1 = ua.ptr();
   up.ldb1 = ua.ld;
   check(nsw::gated_product(up, false, stream()), "gated_mlp up");
-  auto y = torch::empty({d.M, round8(d.N)}, opt);
+  auto y = torch::empty({d.M, d.N}, opt);
   down.b0 = da.ptr();
   down.ldb0 = da.ld;
   down.out0 = y.data_ptr();
-  down.ldout = round8(d.N);
+  down.ldout = d.N;
   check(nsw::gated_product(down, true, stream()), "gated_mlp down");
-  y = packed(y, d.N);
   if (!save) return {y};
   return {y, xa.t, g, u, h, ga.t, ua.t, da.t};
 }
@@ -235,9 +237,10 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
     }
     return out;
   }
-  const Rows dya = aligned_rows(dy);
+  Aligner al;  // (the weights are the forward's aligned ones already)
+  const Rows dya = al.add(dy), ga = al.add(wg), ua = al.add(wu), da = al.add(wd);
+  al.run();
   const Rows xa{x, d.M == 1 ? round8(d.K) : x.stride(0)};
-  const Rows ga = aligned_rows(wg), ua = aligned_rows(wu), da = aligned_rows(wd);
   auto dgu = torch::empty({d.M, 2 * d.Hp}, opt);
   char* du = reinterpret_cast<char*>(dgu.data_ptr()) + 2 * d.Hp;
   nsw::GatedArgs a{};
@@ -268,7 +271,7 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
   }
   check(nsw::gated_product(a, false, stream()), "gated_mlp dh");
   if (need_dx) {
-    auto dx = torch::empty({d.M, round8(d.K)}, opt);
+    auto dx = torch::empty({d.M, d.K}, opt);
     nsw::GatedArgs b{};
     b.mode = nsw::kGatedDx;
     b.dtype = a.dtype;
@@ -283,9 +286,9 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
     b.b1 = ua.ptr();
     b.ldb1 = ua.ld;
     b.out0 = dx.data_ptr();
-    b.ldout = round8(d.K);
+    b.ldout = d.K;
     check(nsw::gated_product(b, true, stream()), "gated_mlp dx");
-    out[0] = packed(dx, d.K);
+    out[0] = dx;
   }
   if (need_w) {
     const GradOut g0(dw_into[0], {d.H, d.K}, x, wdt), g1(dw_into[1], {d.H, d.K}, x, wdt),

@@ -73,7 +73,11 @@ struct GatedParams {
   int bias_dtype;
   int act;      // 0 SiLU, 1 GELU
   int save;     // kUp: store g and u
-  int has_res;  // kDown
+  int has_res;  // kDown: residual tiles by TMA
+  int plain;    // kDown / kDx: rows that no tensor map can address; result and residual by plain accesses
+  void* D;
+  const void* res;
+  int64_t ldd, ldres;
   // kDw: the weights' tiles in order; see gated_unit
   DwSeg seg[kDwWeights];  // (weight i: out_i, a_i and b_(i / 2))
   int64_t direct;
@@ -255,6 +259,33 @@ __device__ __forceinline__ void dw_tile_store(const DwSeg& p, float* t, int64_t 
     }
   }
   __syncwarp();
+}
+
+// The same turn for a 16-bit result [M, N] whose rows are not 16-byte aligned, with its residual: its 32 loads leave
+// before the turn, since a load behind a store that might alias it waits (20003 x 1001 x 2669: 115 us; 249 us
+// with load and store row by row)
+template <typename T>
+__device__ __forceinline__ void plain_tile_store(const GatedParams& p, float* t, int64_t row_base, int64_t nb,
+                                                 const float* f, int lane) {
+  const int64_t col = nb + lane;
+  const int rows = col < p.N ? (int)(p.M - row_base < 32 ? p.M - row_base : 32) : 0;
+  T res[32];
+  if (p.res) {
+    const T* q = reinterpret_cast<const T*>(p.res) + row_base * p.ldres + col;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) res[r] = r < rows ? q[r * p.ldres] : from_f<T>(0.f);
+  }
+  __syncwarp();
+#pragma unroll
+  for (int j = 0; j < 32; ++j) t[32 * lane + (j ^ lane)] = f[j];
+  __syncwarp();
+  T* d = reinterpret_cast<T*>(p.D) + row_base * p.ldd + col;
+#pragma unroll
+  for (int r = 0; r < 32; ++r) {
+    float v = t[32 * r + (lane ^ r)];
+    if (p.res) v += to_f(res[r]);
+    if (r < rows) d[r * p.ldd] = from_f<T>(v);
+  }
 }
 
 // a tile of all weights' -> its weight, and the tile within it
@@ -598,6 +629,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
             continue;
           }
           if (MODE == kDown && p.bias0) add_bias32(p.bias0, p.bias_dtype, nb, p.N, f);
+          if ((MODE == kDown || MODE == kDx) && p.plain) {
+            plain_tile_store<T>(p, reinterpret_cast<float*>(buf[0]), row_base, nb, f, lane);
+            continue;
+          }
           if (MODE == kDown && p.has_res) {
             T* b = buf[c];
 #pragma unroll
@@ -736,9 +771,17 @@ static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
       ok = ok && make_map(&p.b0, a.b0, a.N, a.K, a.ldb0, 128, a.dtype);
       if (MODE == kUp) ok = ok && make_map(&p.b1, a.b1, a.N, a.K, a.ldb1, 128, a.dtype);
     }
-    if (a.in0) ok = ok && make_store_map(&p.in0, const_cast<void*>(a.in0), a.M, a.N, a.ldin, a.dtype);
+    const auto odd = [](const void* q, int64_t ld) { return ld % 8 != 0 || (reinterpret_cast<uintptr_t>(q) & 15) != 0; };
+    p.plain = (MODE == kDown || MODE == kDx) && (odd(a.out0, a.ldout) || (a.in0 && odd(a.in0, a.ldin)));
+    if (p.plain) {
+      p.D = a.out0;
+      p.ldd = a.ldout;
+      p.res = a.in0;
+      p.ldres = a.ldin;
+    }
+    if (a.in0 && !p.plain) ok = ok && make_store_map(&p.in0, const_cast<void*>(a.in0), a.M, a.N, a.ldin, a.dtype);
     if (a.in1) ok = ok && make_store_map(&p.in1, const_cast<void*>(a.in1), a.M, a.N, a.ldin, a.dtype);
-    ok = ok && make_store_map(&p.out0, a.out0, a.M, a.N, a.ldout, a.dtype);
+    if (!p.plain) ok = ok && make_store_map(&p.out0, a.out0, a.M, a.N, a.ldout, a.dtype);
     if (a.out1) ok = ok && make_store_map(&p.out1, a.out1, a.M, a.N, a.ldaux, a.dtype);
     if (a.out2) ok = ok && make_store_map(&p.out2, a.out2, a.M, a.N, a.ldaux, a.dtype);
     p.M = a.M;
@@ -752,7 +795,7 @@ static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
     p.sums = MODE == kDh ? a.sums : nullptr;
     p.sums_half = a.sums_half;
     p.save = MODE == kUp && a.out1 != nullptr;
-    p.has_res = MODE == kDown && a.in0 != nullptr;
+    p.has_res = MODE == kDown && a.in0 != nullptr && !p.plain;
     return ok;
   });
 }
@@ -1480,29 +1523,24 @@ static cudaError_t launch_skinny(const SkinnyParams& p, bool vec, cudaStream_t s
   return p.M <= 8 ? launch_skinny_nt<T, 1, DUAL>(p, vec, s) : launch_skinny_nt<T, 2, DUAL>(p, vec, s);
 }
 
-// dst[i, j] = src[i s0 + j s1] (16-bit), rows of ld elements: operands whose rows are not 16-byte aligned.  A
-// thread copies eight elements of one row, one 16-byte store where dst's rows allow it, and nothing else: with
-// threads that loop over groups too few loads are in flight (5.6 MB: 10.5 us; as it is, 4.7 us).
-__global__ void __launch_bounds__(256) pad_copy_kernel(const uint16_t* __restrict__ src, int64_t s0, int64_t s1,
-                                                       uint16_t* __restrict__ dst, int64_t ld, int64_t total,
-                                                       uint32_t groups, int64_t cols, int vec) {
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= total) return;
-  const int64_t m = i < ((int64_t)1 << 32) ? (int64_t)((uint32_t)i / groups) : i / groups;
-  const int64_t c = 8 * (i - m * groups);
-  const uint16_t* p = src + m * s0 + c * s1;
-  uint16_t* d = dst + m * ld + c;
+// dst[i, j] = src[i s0 + j s1] (16-bit) for several matrices (blockIdx.y): operands whose rows are not 16-byte aligned,
+// into rows that are.  A thread copies eight elements of one row, one 16-byte store, and nothing else: with threads
+// that loop over groups too few loads are in flight (5.6 MB: 10.5 us; as it is, 4.7 us).
+struct PadCopies {
+  PadCopy v[kPadCopies];
+};
+__global__ void __launch_bounds__(256) pad_copy_kernel(const __grid_constant__ PadCopies l) {
+  const PadCopy& a = l.v[blockIdx.y];
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, groups = a.ld / 8;
+  if (i >= a.rows * groups) return;
+  const int64_t m = i < ((int64_t)1 << 32) ? (int64_t)((uint32_t)i / (uint32_t)groups) : i / groups;
+  const int64_t c = 8 * (i - m * groups), s1 = a.s1;
+  const uint16_t* p = reinterpret_cast<const uint16_t*>(a.src) + m * a.s0 + c * s1;
   uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
   for (int j = 0; j < 8; ++j)
-    if (c + j < cols) w[j >> 1] |= (uint32_t)p[j * s1] << (16 * (j & 1));
-  if (vec && c + 8 <= ld) {
-    *reinterpret_cast<uint4*>(d) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (c + j < cols) d[j] = (uint16_t)(w[j >> 1] >> (16 * (j & 1)));
-  }
+    if (c + j < a.cols) w[j >> 1] |= (uint32_t)p[j * s1] << (16 * (j & 1));
+  *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.dst) + m * a.ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
 }
 
 // Column sums of up to two 16-bit [rows, n] matrices (rows 16-byte aligned, ld >= n rounded up to 8; blockIdx.z):
@@ -1656,15 +1694,18 @@ cudaError_t gated_skinny(const GatedArgs& a, bool dependent, cudaStream_t s) {
   return dual ? gated::launch_skinny<__half, true>(p, vec, s) : gated::launch_skinny<__half, false>(p, vec, s);
 }
 
-cudaError_t pad_copy(const void* src, int64_t s0, int64_t s1, void* dst, int64_t ld, int64_t rows, int64_t cols,
-                     cudaStream_t s) {
-  if (rows <= 0 || cols <= 0) return cudaSuccess;
-  const int64_t groups = (cols + 7) / 8, total = rows * groups;
-  if ((total + 255) / 256 > INT32_MAX) return cudaErrorInvalidValue;
-  const int vec = ld % 8 == 0 && (reinterpret_cast<uintptr_t>(dst) & 15) == 0;
-  gated::pad_copy_kernel<<<(unsigned)((total + 255) / 256), 256, 0, s>>>(reinterpret_cast<const uint16_t*>(src), s0, s1,
-                                                                         reinterpret_cast<uint16_t*>(dst), ld, total,
-                                                                         (uint32_t)groups, cols, vec);
+cudaError_t pad_copy(const PadCopy* v, int count, cudaStream_t s) {
+  gated::PadCopies l;
+  int64_t most = 0;
+  if (count > kPadCopies) return cudaErrorInvalidValue;
+  for (int i = 0; i < count; ++i) {
+    if (v[i].ld % 8 || (reinterpret_cast<uintptr_t>(v[i].dst) & 15)) return cudaErrorInvalidValue;
+    l.v[i] = v[i];
+    most = std::max(most, v[i].rows * (v[i].ld / 8));
+  }
+  if (most == 0) return cudaSuccess;
+  if ((most + 255) / 256 > INT32_MAX) return cudaErrorInvalidValue;
+  gated::pad_copy_kernel<<<dim3((unsigned)((most + 255) / 256), (unsigned)count), 256, 0, s>>>(l);
   return cudaGetLastError();
 }
 

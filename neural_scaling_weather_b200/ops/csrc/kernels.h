@@ -172,10 +172,10 @@ cudaError_t wgrad_tcgen05(const WgradArgs& a, const WgradPlan& plan, cudaStream_
 // read as stored.  mode:
 //   kGatedUp    out0 = act(a0 b0^T + bias0) * (a0 b1^T + bias1); out1 / out2 (both or neither, ldaux): the
 //               two pre-activations; b0 / b1 [N, K]
-//   kGatedDown  out0 = a0 b0^T + bias0 + in0 (optional, ldin); b0 [N, K]
+//   kGatedDown  out0 = a0 b0^T + bias0 + in0 (optional, ldin); b0 [N, K]; rows of out0 and in0 of any alignment
 //   kGatedDh    d = a0 b0 with b0 [K, N]; out0 = d * in1 * act'(in0), out1 = d * act(in0) (in: g, u, ldin;
 //               out0 in rows of ldout, out1 in rows of ldaux)
-//   kGatedDx    out0 = a0 b0 + a1 b1 with b0, b1 [K, N]
+//   kGatedDx    out0 = a0 b0 + a1 b1 with b0, b1 [K, N]; rows of out0 of any alignment
 enum GatedMode : int { kGatedUp = 0, kGatedDown = 1, kGatedDh = 2, kGatedDx = 3 };
 struct GatedArgs {
   int mode, dtype, act;  // act: 0 SiLU, 1 GELU
@@ -237,9 +237,15 @@ cudaError_t gated_product(const GatedArgs& a, bool dependent, cudaStream_t s);
 // kGatedUp (no out1 / out2) and kGatedDown for at most kGatedSkinnyTokens rows, any strides
 constexpr int kGatedSkinnyTokens = 16;
 cudaError_t gated_skinny(const GatedArgs& a, bool dependent, cudaStream_t s);
-// 16-bit strided copy into rows of ld elements (cols of them written, and zeros up to a multiple of eight)
-cudaError_t pad_copy(const void* src, int64_t s0, int64_t s1, void* dst, int64_t ld, int64_t rows, int64_t cols,
-                     cudaStream_t s);
+// 16-bit strided copies, one launch: dst[i, j] = src[i s0 + j s1] into 16-byte aligned rows of ld elements (a
+// multiple of eight, the ones past cols zero)
+struct PadCopy {
+  const void* src;
+  void* dst;
+  int64_t s0, s1, ld, rows, cols;
+};
+constexpr int kPadCopies = 5;
+cudaError_t pad_copy(const PadCopy* v, int count, cudaStream_t s);
 
 // ---- norms with gate and skip connection (norm_gate.cu) ------------------------------------------------
 // Forward: stream = skip_scale skip + gate * rms(y) * wp; normed = rms(stream) * wn (normed and wn null: only

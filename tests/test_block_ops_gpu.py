@@ -123,6 +123,29 @@ def test_gated_strides_and_batches(M):
     assert y3.shape == (M, 1, 1, 64) and torch.equal(y3.view(M, 64), y)
 
 
+@pytest.mark.parametrize("rows", ["packed", "offset", "broadcast", "transposed"])
+def test_gated_many_tokens_of_odd_widths(rows):
+    """Results and residuals whose rows are not 16-byte aligned, with enough tokens for the tiled kernels."""
+    M, K, H, N = 9003, 517, 1371, 519
+    x, w, b, res, dy = gated_inputs(M, K, H, N, torch.bfloat16, True, True)
+    if rows == "offset":
+        res = torch.nn.functional.pad(res, (1, 2))[:, 1:-2]
+    elif rows == "broadcast":
+        res = res[:1].expand(M, N)
+    elif rows == "transposed":
+        res = res.t().contiguous().t()
+    leaves = [t.requires_grad_() for t in [x] + w + b]
+    y = ops.gated_mlp(x, *w, *b, residual=res)
+    assert y.shape == (M, N) and y.is_contiguous()
+    got = torch.autograd.grad(y, leaves, dy)
+    ey, exact = gated_exact(x, w, b, res, "silu", dy)
+    assert rel(y, ey) < 2 * U[torch.bfloat16]
+    for i, (a, e) in enumerate(zip(got, exact)):
+        assert rel(a, e) < 4 * U[torch.bfloat16], i
+    with torch.no_grad():
+        assert torch.equal(ops.gated_mlp(x, *w, *b, residual=res), y)
+
+
 def test_gated_empty():
     x, w, b, res, _ = gated_inputs(3, 64, 128, 64, torch.bfloat16, True, False)
     for grad in (False, True):
