@@ -234,29 +234,32 @@ __device__ __forceinline__ void ring_store(const CUtensorMap* map, const float* 
 
 // A 32 x 32 tile of a weight gradient by plain stores: fp32 (added to what is there), or 16-bit rows that are not
 // 16-byte aligned.  The lanes' rows are turned through `t` (4 KB, element (r, c) at 32 r + (c ^ r): conflict-free
-// both ways), so that each store is a row segment.
+// both ways), so that each store is a row segment.  What is added to is loaded first, 32 rows at once: a load behind a
+// store that might alias it waits.
 template <typename T>
 __device__ __forceinline__ void dw_tile_store(const DwSeg& p, float* t, int64_t row_base, int64_t nb, const float* f,
                                               int lane) {
+  const int64_t col = nb + lane, at = row_base * p.ldd + col;
+  const int rows = col < p.N ? (int)(p.M - row_base < 32 ? p.M - row_base : 32) : 0;
   if (lane == 0) bulk_wait_read_0();  // an earlier tile may still leave from these buffers
   __syncwarp();
 #pragma unroll
   for (int j = 0; j < 32; ++j) t[32 * lane + (j ^ lane)] = f[j];
-  __syncwarp();
-  const int64_t col = nb + lane;
-  const int rows = (int)(p.M - row_base < 32 ? p.M - row_base : 32);
-  if (col < p.N) {
-#pragma unroll 8
-    for (int r = 0; r < rows; ++r) {
-      const float v = t[32 * r + (lane ^ r)];
-      const int64_t at = (row_base + r) * p.ldd + col;
-      if (p.out_f32) {
-        float* d = reinterpret_cast<float*>(p.D) + at;
-        *d = p.accumulate ? *d + v : v;
-      } else {
-        reinterpret_cast<T*>(p.D)[at] = from_f<T>(v);
-      }
-    }
+  float old[32];
+  if (p.out_f32) {
+    float* d = reinterpret_cast<float*>(p.D) + at;
+#pragma unroll
+    for (int r = 0; r < 32; ++r) old[r] = p.accumulate && r < rows ? d[r * p.ldd] : 0.f;
+    __syncwarp();
+#pragma unroll
+    for (int r = 0; r < 32; ++r)
+      if (r < rows) d[r * p.ldd] = old[r] + t[32 * r + (lane ^ r)];
+  } else {
+    T* d = reinterpret_cast<T*>(p.D) + at;
+    __syncwarp();
+#pragma unroll
+    for (int r = 0; r < 32; ++r)
+      if (r < rows) d[r * p.ldd] = from_f<T>(t[32 * r + (lane ^ r)]);
   }
   __syncwarp();
 }
