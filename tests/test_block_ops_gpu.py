@@ -343,6 +343,34 @@ def test_norm_gate_residual(S, R, D, dtype, gate, nxt):
         assert (a.double() - e).norm() <= 1e-5 * terms.norm()
 
 
+@pytest.mark.parametrize("S,R,D", [(3, 1001, 131), (1, 2500, 2033), (37, 90, 515), (2, 1500, 250), (1, 1100, 1290),
+                                   (2, 700, 1028), (5, 300, 3), (1, 70, 2045), (2, 2500, 768), (1, 900, 1536)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("start", [0, 1])
+def test_norm_gate_residual_rows_anywhere(S, R, D, dtype, start):
+    """Rows that begin anywhere in a 16-byte group, many for each block, also in tensors that begin off one.  Each
+    element: its own rounding (2^-8 or 2^-11) and fp32 arithmetic, 1e-5 of the tensor's largest value.  An infinite
+    row leaves its neighbours, which share its first and last groups, as they are."""
+    y, skip, wp, gt, wn, ds, dn = norm_inputs(S, R, D, dtype, "sample", True)
+    exact, tens, vec = norm_exact(y, skip, wp, gt, wn, 0.7, ds, dn)
+    if start:
+        y = torch.cat([y.new_zeros(1), y.reshape(-1)])[1:].view(S, R, D)
+    leaves = [t.requires_grad_() for t in (y, skip, wp, gt, wn)]
+    outs = ops.norm_gate_residual(y, skip, wp, gt, wn, skip_scale=0.7)
+    got = torch.autograd.grad(outs, leaves, [ds, dn])
+    for a, e in zip(list(outs) + list(got[:2]), exact + list(tens)):
+        assert ((a.double() - e).abs() <= {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype] * e.abs()
+                + 1e-5 * e.abs().max()).all()
+    for a, (e, terms) in zip(got[2:], vec):
+        assert (a.double() - e).norm() <= 1e-5 * terms.norm()
+    with torch.no_grad():
+        keep = torch.ones(S, R, dtype=torch.bool, device=DEV)
+        keep[0, 1::3] = keep[-1, R - 1] = False
+        y[~keep] = float("inf")
+        again = ops.norm_gate_residual(y, skip, wp, gt, wn, skip_scale=0.7)
+        assert all(torch.equal(a[keep], b[keep]) for a, b in zip(again, outs))
+
+
 @pytest.mark.parametrize("only", ["stream", "normed"])
 def test_norm_gate_residual_with_one_output_used(only):
     y, skip, wp, gt, wn, ds, dn = norm_inputs(2, 19, 200, torch.bfloat16, "sample", True)
