@@ -1526,24 +1526,54 @@ static cudaError_t launch_skinny(const SkinnyParams& p, bool vec, cudaStream_t s
   return p.M <= 8 ? launch_skinny_nt<T, 1, DUAL>(p, vec, s) : launch_skinny_nt<T, 2, DUAL>(p, vec, s);
 }
 
-// dst[i, j] = src[i s0 + j s1] (16-bit) for several matrices (blockIdx.y): operands whose rows are not 16-byte aligned,
-// into rows that are.  A thread copies eight elements of one row, one 16-byte store, and nothing else: with threads
-// that loop over groups too few loads are in flight (5.6 MB: 10.5 us; as it is, 4.7 us).
+// dst[i, j] = src[i s0 + j s1] (16-bit) for several matrices: operands whose rows are not 16-byte aligned, into rows
+// that are.  A group is eight elements of a row, one 16-byte store; a thread copies kPadGroups of them, all loads
+// before the stores, and a matrix has blocks of its own (20003 x 1001 and three weights: 30 us; 41 with a group a
+// thread and as many blocks for each matrix as for the longest).  Where the elements are adjacent, the two aligned
+// groups that hold them are read and shifted; at a tensor's ends, past which nothing is read, single elements.
+constexpr int kPadGroups = 4;
 struct PadCopies {
   PadCopy v[kPadCopies];
+  int64_t first[kPadCopies + 1];  // a matrix's first block
 };
-__global__ void __launch_bounds__(256) pad_copy_kernel(const __grid_constant__ PadCopies l) {
-  const PadCopy& a = l.v[blockIdx.y];
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x, groups = a.ld / 8;
-  if (i >= a.rows * groups) return;
+__device__ __forceinline__ uint4 pad_group(const PadCopy& a, int64_t i, int64_t groups) {
   const int64_t m = i < ((int64_t)1 << 32) ? (int64_t)((uint32_t)i / (uint32_t)groups) : i / groups;
   const int64_t c = 8 * (i - m * groups), s1 = a.s1;
   const uint16_t* p = reinterpret_cast<const uint16_t*>(a.src) + m * a.s0 + c * s1;
-  uint32_t w[4] = {0, 0, 0, 0};
+  uint32_t w[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+  const uintptr_t at = reinterpret_cast<uintptr_t>(p), lo = at & ~(uintptr_t)15;
+  const uintptr_t first = reinterpret_cast<uintptr_t>(a.src), end = first + 2 * ((a.rows - 1) * a.s0 + a.cols);
+  if (s1 == 1 && c + 8 <= a.cols && lo >= first && lo + 32 <= end) {
+    const uint4 u = *reinterpret_cast<const uint4*>(lo), v = *reinterpret_cast<const uint4*>(lo + 16);
+    w[0] = u.x, w[1] = u.y, w[2] = u.z, w[3] = u.w, w[4] = v.x, w[5] = v.y, w[6] = v.z, w[7] = v.w;
 #pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (c + j < a.cols) w[j >> 1] |= (uint32_t)p[j * s1] << (16 * (j & 1));
-  *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.dst) + m * a.ld + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    for (int j = 0; j < 6; ++j) w[j] = at & 8 ? w[j + 2] : w[j];
+#pragma unroll
+    for (int j = 0; j < 5; ++j) w[j] = at & 4 ? w[j + 1] : w[j];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) w[j] = __funnelshift_r(w[j], w[j + 1], 8 * (int)(at & 2));
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (c + j < a.cols) w[j >> 1] |= (uint32_t)p[j * s1] << (16 * (j & 1));
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__global__ void __launch_bounds__(256) pad_copy_kernel(const __grid_constant__ PadCopies l) {
+  int k = 0;
+#pragma unroll
+  for (int i = 1; i < kPadCopies; ++i)
+    if (blockIdx.x >= l.first[i]) k = i;
+  const PadCopy& a = l.v[k];
+  const int64_t groups = a.ld / 8, total = a.rows * groups;
+  const int64_t i0 = (blockIdx.x - l.first[k]) * (256 * kPadGroups) + threadIdx.x;
+  uint4 u[kPadGroups];
+#pragma unroll
+  for (int g = 0; g < kPadGroups; ++g)
+    if (i0 + 256 * g < total) u[g] = pad_group(a, i0 + 256 * g, groups);
+#pragma unroll
+  for (int g = 0; g < kPadGroups; ++g)
+    if (i0 + 256 * g < total) reinterpret_cast<uint4*>(a.dst)[i0 + 256 * g] = u[g];
 }
 
 // Column sums of up to two 16-bit [rows, n] matrices (rows 16-byte aligned, ld >= n rounded up to 8; blockIdx.z):
@@ -1699,16 +1729,18 @@ cudaError_t gated_skinny(const GatedArgs& a, bool dependent, cudaStream_t s) {
 
 cudaError_t pad_copy(const PadCopy* v, int count, cudaStream_t s) {
   gated::PadCopies l;
-  int64_t most = 0;
+  int64_t blocks = 0;
   if (count > kPadCopies) return cudaErrorInvalidValue;
-  for (int i = 0; i < count; ++i) {
+  for (int i = 0; i <= kPadCopies; ++i) {
+    l.first[i] = i <= count ? blocks : INT64_MAX;
+    if (i >= count) continue;
     if (v[i].ld % 8 || (reinterpret_cast<uintptr_t>(v[i].dst) & 15)) return cudaErrorInvalidValue;
     l.v[i] = v[i];
-    most = std::max(most, v[i].rows * (v[i].ld / 8));
+    blocks += (v[i].rows * (v[i].ld / 8) + 256 * gated::kPadGroups - 1) / (256 * gated::kPadGroups);
   }
-  if (most == 0) return cudaSuccess;
-  if ((most + 255) / 256 > INT32_MAX) return cudaErrorInvalidValue;
-  gated::pad_copy_kernel<<<dim3((unsigned)((most + 255) / 256), (unsigned)count), 256, 0, s>>>(l);
+  if (blocks == 0) return cudaSuccess;
+  if (blocks > INT32_MAX) return cudaErrorInvalidValue;
+  gated::pad_copy_kernel<<<(unsigned)blocks, 256, 0, s>>>(l);
   return cudaGetLastError();
 }
 
