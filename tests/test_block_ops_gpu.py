@@ -146,6 +146,36 @@ def test_gated_many_tokens_of_odd_widths(rows):
         assert torch.equal(ops.gated_mlp(x, *w, *b, residual=res), y)
 
 
+@pytest.mark.parametrize("M", [8, 40, 700, 12000])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["gelu", "silu"])
+def test_gated_tail_of_the_gate(M, dtype, act):
+    """Every element of h, dg and du at gates of -6 to 6, with weights of ones that pick single features, so that
+    the gates, the up projections and dh are exact.  An element's own rounding (2^-8 or 2^-11; half the spacing of
+    fp16's subnormals) and 2e-5: the activation's approximations are below 1e-5 each, the slope's two terms cancel
+    to no less than half of them except around its zero (an absolute 1e-6 of terms of at most one)."""
+    H = 256
+    eye, none = torch.eye(H, device=DEV, dtype=dtype), torch.zeros(H, H, device=DEV, dtype=dtype)
+    w = [torch.cat([eye, none], 1), torch.cat([none, eye], 1), eye.clone()]
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    gates = (torch.rand(M, H, generator=gen, device=DEV) * 12 - 6).to(dtype)
+    g = gates.double().requires_grad_()
+    a = torch.nn.functional.silu(g) if act == "silu" else g * torch.special.ndtr(g)
+    (slope,) = torch.autograd.grad(a.sum(), g)
+    a = a.detach()
+    u, tiny = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11}[dtype], 2.0 ** -25 * (dtype == torch.float16)
+    for up, d in [(2.0 ** 13, 1.0), (1.0, 2.0 ** 13)]:  # large enough that fp16 holds the tail in normal numbers
+        x = torch.cat([gates, torch.full_like(gates, up)], 1).requires_grad_()
+        y = ops.gated_mlp(x, *w, activation=act)
+        (dx,) = torch.autograd.grad(y, x, torch.full_like(y, d))
+        with torch.no_grad():
+            y2 = ops.gated_mlp(x, *w, activation=act)
+        for got, exact in [(y, up * a), (y2, up * a), (dx[:, H:], d * a)]:
+            assert ((got.double() - exact).abs() <= (u + 2e-5) * exact.abs() + tiny).all()
+        exact = d * up * slope
+        assert ((dx[:, :H].double() - exact).abs() <= (u + 2e-5) * exact.abs() + 1e-6 * d * up).all()
+
+
 def test_gated_empty():
     x, w, b, res, _ = gated_inputs(3, 64, 128, 64, torch.bfloat16, True, False)
     for grad in (False, True):
