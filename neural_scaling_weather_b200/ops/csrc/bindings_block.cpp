@@ -5,6 +5,10 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <algorithm>
+#include <utility>
+#include <vector>
+
 #include "kernels.h"
 
 namespace {
@@ -211,6 +215,20 @@ struct GradOut {
   }
 };
 
+// The kernels read, add and write their targets without regard to one another
+void check_apart(const std::vector<OptTensor>& a, const std::vector<OptTensor>& b) {
+  std::vector<std::pair<const char*, const char*>> at;
+  for (const auto* v : {&a, &b})
+    for (const OptTensor& t : *v)
+      if (t && t->numel() > 0) {
+        const char* p = static_cast<const char*>(t->data_ptr());
+        at.emplace_back(p, p + t->nbytes());
+      }
+  std::sort(at.begin(), at.end());
+  for (size_t i = 1; i < at.size(); ++i)
+    TORCH_CHECK(at[i].first >= at[i - 1].second, "gated_mlp backward: gradient buffers overlap");
+}
+
 // Gradients from dy and what the forward saved: {dx, dwg, dwu, dwd, dbg, dbu, dbd}.  An entry is undefined
 // where it was not asked for (need_dx, need_w, need_b) or was added into the given fp32 buffer.
 std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tensor& wg, const Tensor& wu,
@@ -225,6 +243,7 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
   TORCH_CHECK(g.is_contiguous() && u.is_contiguous() && h.is_contiguous() && (d.M == 0 || rows_aligned(x)),
               "gated_mlp backward: saved tensors must be as the forward returned them");
   TORCH_CHECK(dw_into.size() == 3 && db_into.size() == 3, "gated_mlp backward: three weights and biases");
+  check_apart(dw_into, db_into);
   const c10::cuda::CUDAGuard guard(x.device());
   const auto opt = x.options();
   std::vector<Tensor> out(7);

@@ -406,8 +406,11 @@ class _GatedMLP(torch.autograd.Function):
         need = ctx.needs_input_grad
         need_w = any(need[3:])
         has_b = [b is not None for b in ctx.biases]
-        tw = [gradsink.target(w) for w in ctx.params] if need_w else [None] * 3
-        tb = [gradsink.target(b) for b in ctx.biases] if need_w else [None] * 3
+        # the kernels add to all targets at once: a parameter that is here more than once gets its shares through
+        # autograd, which adds them one after the other
+        given = [id(p) for p in ctx.params + ctx.biases]
+        into = lambda p: gradsink.target(p) if need_w and given.count(id(p)) == 1 else None  # noqa: E731
+        tw, tb = [into(w) for w in ctx.params], [into(b) for b in ctx.biases]
         bdt = next((b.dtype for b in ctx.biases if b is not None), torch.float32)
         dx, *grads = ext.gated_mlp_bwd(_rows(dy, dy.shape[-1]).to(x2.dtype), x2, *ctx.W, g, u, h, ctx.act, need[0],
                                        need_w, need_w and any(has_b), tw, tb, ctx.params[0].dtype, bdt)

@@ -100,6 +100,55 @@ def test_extension_refuses_with_numbers_in_the_message():
             ext.gated_mlp(x, w, w, w, None, None, None, None, 0)
 
 
+@pytest.mark.parametrize("tied", [(0, 1), (1, 2), (3, 4), (0, 1, 2, 3, 4, 5), ()])
+def test_in_place_gradients_of_tied_parameters(tied, monkeypatch):
+    """The extension adds to all the buffers of a call at once, so no two of a call may be one parameter's: a
+    parameter that is passed twice gets its gradients through autograd.  With a stand-in for the extension, whose
+    forward and gradients are ones."""
+    from neural_scaling_weather_b200.ops import fused, gradsink
+
+    n, seen = 8, []
+
+    class Ext:
+        @staticmethod
+        def gated_mlp_fwd(x, wg, wu, wd, *rest):
+            return [torch.ones_like(x), x, x, x, x, wg, wu, wd]
+
+        @staticmethod
+        def gated_mlp_bwd(dy, x, wg, wu, wd, g, u, h, act, need_dx, need_w, need_b, dw, db, *dtypes):
+            seen.append([t for t in list(dw) + list(db) if t is not None])
+            for t in seen[-1]:
+                t.add_(1)
+            return [None] + [None if t is not None else torch.ones(n, n) for t in dw] + [
+                None if t is not None else torch.ones(n) for t in db]
+
+    monkeypatch.setattr(fused, "require", lambda: Ext)
+    notices = []
+
+    class Reducer:
+        def notice(self, p):
+            notices.append(p)
+
+    reducer = Reducer()
+    gradsink.register(reducer.notice)
+    # one leaf for each place, or the same one in the tied places (a matrix cannot be a vector: ties across them none)
+    ps = [torch.nn.Parameter(torch.ones(n, n)) for _ in range(3)] + [torch.nn.Parameter(torch.ones(n)) for _ in range(3)]
+    for i in tied:
+        ps[i] = ps[tied[0]] if (i < 3) == (tied[0] < 3) else ps[[j for j in tied if (j < 3) == (i < 3)][0]]
+    for p in ps:
+        p.grad = torch.zeros_like(p)
+    y = fused._GatedMLP.apply(torch.ones(4, n), None, 0, *ps)
+    y.sum().backward()
+    gradsink.unregister(reducer.notice)
+    assert len({t.data_ptr() for t in seen[0]}) == len(seen[0])
+    for p in ps:
+        uses = sum(q is p for q in ps)
+        assert (p.grad == uses).all()
+        # what autograd still has to add is not reported as written
+        assert sum(q is p for q in notices) == (uses == 1)
+        assert p._nsw_pending == 0
+
+
 # --------------------------------------------------------------------------- model options
 def _cfg(**model):
     return C.create(dict(

@@ -222,6 +222,31 @@ def test_gated_fp32_parameters_and_in_place_gradients(dtype):
         assert rel(p.grad, 1 + 2 * a.double()) < 1e-5
 
 
+def test_gated_tied_parameters_and_shared_gradient_buffers():
+    """One parameter as both projections and one bias for both: their gradients add up in an existing fp32 ``.grad``
+    as in separate ones (two fp32 sums in another order).  Buffers that overlap are refused."""
+    x, w, b, _, dy = gated_inputs(1500, 256, 512, 256, torch.bfloat16, True, False)
+    sep = [torch.nn.Parameter(t.float()) for t in (w[0], w[0], w[2], b[0], b[0], b[2])]
+    got = torch.autograd.grad(ops.gated_mlp(x, *sep), sep, dy)
+    tied = [torch.nn.Parameter(t.float()) for t in (w[0], w[2], b[0], b[2])]
+    for p in tied:
+        p.grad = torch.zeros_like(p)
+    for _ in range(2):
+        ops.gated_mlp(x, tied[0], tied[0], tied[1], tied[2], tied[2], tied[3]).backward(dy)
+    for p, e in zip(tied, (got[0] + got[1], got[2], got[3] + got[4], got[5])):
+        assert rel(p.grad, 2 * e) < 1e-6
+    ext = _ext.require()
+    _, *saved = ext.gated_mlp_fwd(x, *w, None, None, None, None, 0, True)
+    x2, g, u, h, *ws = saved
+    flat = torch.zeros(2 * 512 * 256, device=DEV)
+    for at in (0, 512 * 256 - 4):
+        into = [flat[:512 * 256].view(512, 256), flat[at:at + 512 * 256].view(512, 256), None]
+        with pytest.raises(RuntimeError, match="overlap"):
+            ext.gated_mlp_bwd(dy, x2, *ws, g, u, h, 0, False, True, False, into, [None] * 3, torch.float32,
+                              torch.float32)
+    assert not flat.any()
+
+
 def test_gated_gradient_against_differences():
     """Directional derivative of sum(y dy) in 64 bits against the kernels' gradients."""
     x, w, b, _, dy = gated_inputs(130, 64, 136, 64, torch.float16, True, False)
