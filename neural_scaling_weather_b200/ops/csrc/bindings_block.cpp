@@ -37,6 +37,15 @@ void once_differentiable(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": second derivatives are not implemented (create_graph=True)");
 }
 
+// The kernels read the values alone, and a missing tangent counts as zero
+void no_tangent(const Tensor& t, const char* what) {
+  TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what,
+              ": forward-mode derivatives are not implemented");
+}
+void no_tangent(const OptTensor& t, const char* what) {
+  if (t) no_tangent(*t, what);
+}
+
 int64_t round8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // A [rows, cols] operand the TMA kernels can read: unit column stride, 16-byte aligned rows.
@@ -417,6 +426,8 @@ Tensor gated_mlp(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tens
   TORCH_CHECK_VALUE(!residual || (residual->dim() == x.dim() && residual->size(-1) == wd.size(0) &&
                                   residual->sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1)),
                     "gated_mlp: residual ", residual->sizes(), " is not the output's shape");
+  for (const Tensor* t : {&x, &wg, &wu, &wd}) no_tangent(*t, "gated_mlp");
+  for (const OptTensor* t : {&bg, &bu, &bd, &residual}) no_tangent(*t, "gated_mlp");
   bool grad = false;
   if (at::GradMode::is_enabled()) {
     for (const Tensor* t : {&x, &wg, &wu, &wd}) grad = grad || t->requires_grad();
@@ -571,6 +582,8 @@ std::vector<Tensor> norm_gate(const Tensor& y, const Tensor& skip, const Tensor&
   TORCH_CHECK_VALUE(!gate || ((gate->dim() == 1 || (gate->dim() == 2 && gate->size(0) == y.size(0))) &&
                               gate->size(-1) == n),
                     "norm_gate_residual: gate ", gate->sizes(), " is neither (", n, ",) nor (", y.size(0), ", ", n, ")");
+  for (const Tensor* t : {&y, &skip, &wp}) no_tangent(*t, "norm_gate_residual");
+  for (const OptTensor* t : {&gate, &wn}) no_tangent(*t, "norm_gate_residual");
   bool grad = false;
   if (at::GradMode::is_enabled()) {
     for (const Tensor* t : {&y, &skip, &wp}) grad = grad || t->requires_grad();
@@ -596,6 +609,8 @@ Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, const std::
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor& g = grads[i];
     const Tensor& o = out.empty() ? g : out[i];
+    no_tangent(g, "clip_grad_norm");
+    no_tangent(o, "clip_grad_norm");
     TORCH_CHECK(g.is_cuda() && g.device() == dev && o.device() == dev, "clip_grad_norm: tensor ", i,
                 " is not on the first one's CUDA device");
     TORCH_CHECK(g.is_contiguous() && o.is_contiguous() && o.numel() == g.numel() &&

@@ -17,6 +17,7 @@ import weakref
 from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from . import gradsink
@@ -424,6 +425,12 @@ class _GatedMLP(torch.autograd.Function):
         return (dx, dy.to(ctx.res_dtype) if need[1] else None, None, *out)
 
 
+def _no_tangents(what: str, *tensors) -> None:
+    """The extension refuses forward-mode derivatives of what it is given; here of what is cast without autograd."""
+    if any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise RuntimeError(f"{what}: forward-mode derivatives are not implemented")
+
+
 def gated_mlp_cuda(x, wg, wu, wd, bg, bu, bd, residual, activation):
     act = _GATED_ACT[activation]
     dt = _cdtype(x)
@@ -431,6 +438,7 @@ def gated_mlp_cuda(x, wg, wu, wd, bg, bu, bd, residual, activation):
         residual = residual.to(dt)
     if wg.dtype == wu.dtype == wd.dtype == dt:  # parameters already in the compute type: one native node
         return require().gated_mlp(x if x.dtype == dt else x.to(dt), wg, wu, wd, bg, bu, bd, residual, act)
+    _no_tangents("gated_mlp", x, wg, wu, wd, bg, bu, bd, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, wg, wu, wd, bg, bu, bd, residual)):
         check_gated_shapes(x, wg, wu, wd, residual)
         return _GatedMLP.apply(x, residual, act, wg, wu, wd, bg, bu, bd)

@@ -100,6 +100,33 @@ def test_extension_refuses_with_numbers_in_the_message():
             ext.gated_mlp(x, w, w, w, None, None, None, None, 0)
 
 
+@pytest.mark.parametrize("grad_mode", [False, True])
+def test_extension_refuses_forward_mode_derivatives(grad_mode):
+    """The kernels would return an output without a tangent, which counts as a zero derivative (on tensors that hold
+    no memory, as above)."""
+    ext = _ext.load()
+    if ext is None:
+        pytest.skip("extension not built")
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.autograd import forward_ad as fw
+
+    def dual(args, i):
+        return [fw.make_dual(a, torch.zeros_like(a)) if j == i else a for j, a in enumerate(args)]
+
+    with FakeTensorMode(), fw.dual_level(), torch.set_grad_enabled(grad_mode):
+        half = lambda *s: torch.empty(*s, device="cuda", dtype=torch.bfloat16)  # noqa: E731
+        gated = [half(4, 32), half(64, 32), half(64, 32), half(16, 64), half(64), half(64), half(16), half(4, 16)]
+        for i in range(len(gated)):
+            with pytest.raises(RuntimeError, match="gated_mlp: forward-mode"):
+                ext.gated_mlp(*dual(gated, i), 0)
+        norm = [half(2, 3, 16), half(2, 3, 16), *(torch.empty(16, device="cuda") for _ in range(3))]
+        for i in range(len(norm)):
+            with pytest.raises(RuntimeError, match="norm_gate_residual: forward-mode"):
+                ext.norm_gate(*dual(norm, i), 1.0, 1e-6)
+        with pytest.raises(RuntimeError, match="clip_grad_norm: forward-mode"):
+            ext.clip_grads(dual(norm[2:], 1), 1.0, [])
+
+
 @pytest.mark.parametrize("tied", [(0, 1), (1, 2), (3, 4), (0, 1, 2, 3, 4, 5), ()])
 def test_in_place_gradients_of_tied_parameters(tied, monkeypatch):
     """The extension adds to all the buffers of a call at once, so no two of a call may be one parameter's: a

@@ -555,6 +555,28 @@ def test_second_derivatives_are_refused():
         torch.autograd.grad(s, x, dy, create_graph=True)
 
 
+@pytest.mark.parametrize("frozen", [True, False])
+def test_forward_mode_derivatives_are_refused(frozen):
+    """Under no_grad or with frozen parameters the output would have no tangent, which counts as zero."""
+    from torch.autograd import forward_ad as fw
+
+    x, w, b, _, _ = gated_inputs(4, 64, 72, 64, BF16, True, False)
+    y, skip, wp, gt, wn, _, _ = norm_inputs(2, 3, 64, BF16, "sample", True)
+    with fw.dual_level(), torch.set_grad_enabled(not frozen):
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.gated_mlp(fw.make_dual(x, x), *w, *b)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.gated_mlp(x, *w, b[0], fw.make_dual(b[1], b[1]))
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.gated_mlp(x, fw.make_dual(w[0].float(), w[0].float()), w[1].float(), w[2].float())
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.norm_gate_residual(y, fw.make_dual(skip, skip), wp, gt, wn)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.norm_gate_residual(y, skip, wp, fw.make_dual(gt, gt), wn)
+        with pytest.raises(RuntimeError, match="forward-mode"):
+            ops.clip_grad_norm([fw.make_dual(wp, wp)], 1.0)
+
+
 # --------------------------------------------------------------------------- in the model
 def test_model_with_gated_networks_and_sandwich_norms_matches_cpu():
     """The tolerances of the plain model's comparison (tests/test_model_gpu.py): bf16 activations through two
