@@ -630,6 +630,9 @@ Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, const std::
   check(nsw::clip_tensors(v.data(), (int)v.size(), (float)max_norm, partial.data_ptr<float>(), blocks,
                           norm.data_ptr<float>(), stream()),
         "clip_grad_norm");
+  // written behind autograd's back: nodes that saved such a tensor and copies made from one have to notice
+  for (const Tensor& t : out.empty() ? grads : out)
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
   return norm;
 }
 

@@ -16,6 +16,7 @@ if not torch.cuda.is_available():  # pragma: no cover
 
 from neural_scaling_weather_b200 import ops  # noqa: E402
 from neural_scaling_weather_b200.ops import _ext  # noqa: E402
+from neural_scaling_weather_b200.ops import weights as wcache  # noqa: E402
 
 DEV = torch.device("cuda")
 U = {torch.bfloat16: 2.0 ** -9, torch.float16: 2.0 ** -11}
@@ -527,6 +528,32 @@ def test_clip_grad_norm_unaligned_and_non_finite():
     assert torch.isnan(ops.clip_grad_norm(g, 1.0)) and torch.equal(g[0], torch.ones(10, device=DEV))
     g = [torch.ones(10, device=DEV), torch.tensor([float("inf")], device=DEV)]
     assert torch.isinf(ops.clip_grad_norm(g, 1.0)) and not g[0].any() and torch.isnan(g[1]).all()
+
+
+def test_clip_grad_norm_counts_as_an_in_place_write():
+    """What is written has a new version, so that a node that saved it refuses to use it, and cached copies of it are
+    made anew."""
+    g = clip_inputs([(64,), (0,), (5, 7)], [F32, BF16, F16])
+    before = [t._version for t in g]
+    ops.clip_grad_norm(g, 0.01)
+    assert all(t._version > v for t, v in zip(g, before))
+    before = [t._version for t in g]
+    out = [torch.empty_like(t) for t in g]
+    seen = [t._version for t in out]
+    ops.clip_grad_norm(g, 0.01, out=out)
+    assert all(t._version > v for t, v in zip(out, seen)) and [t._version for t in g] == before
+    x = torch.randn(64, device=DEV, requires_grad=True)
+    z = x.exp()  # saves its result
+    ops.clip_grad_norm([z.detach()], 0.01)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        z.sum().backward()
+    p = torch.nn.Parameter(torch.randn(8, 8, device=DEV))
+    stale = wcache.get(p, BF16).clone()
+    ops.clip_grad_norm([torch.ones(8, 8, device=DEV)], 1.0, out=[p.detach()])
+    assert torch.equal(wcache.get(p, BF16), p.detach().bfloat16()) and not torch.equal(stale, wcache.get(p, BF16))
+    with torch.inference_mode():
+        t = torch.ones(8, device=DEV)
+        assert ops.clip_grad_norm([t], 1.0) > 2 and t.norm() < 1.001
 
 
 def test_clip_grad_norm_refusals():
