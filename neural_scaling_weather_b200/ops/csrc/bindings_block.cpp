@@ -239,11 +239,12 @@ void check_apart(const std::vector<OptTensor>& a, const std::vector<OptTensor>& 
 }
 
 // Gradients from dy and what the forward saved: {dx, dwg, dwu, dwd, dbg, dbu, dbd}.  An entry is undefined
-// where it was not asked for (need_dx, need_w, need_b) or was added into the given fp32 buffer.
+// where it was not asked for (need_dx, need_w, need_b) or was added into the given fp32 buffer.  types: of the three
+// weights' and the three biases' gradients, their parameters'.
 std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tensor& wg, const Tensor& wu,
                                   const Tensor& wd, const Tensor& g, const Tensor& u, const Tensor& h, int64_t act,
                                   bool need_dx, bool need_w, bool need_b, std::vector<OptTensor> dw_into,
-                                  std::vector<OptTensor> db_into, at::ScalarType wdt, at::ScalarType bdt) {
+                                  std::vector<OptTensor> db_into, std::vector<at::ScalarType> types) {
   const GatedShape d = gated_shape(x, wg, wu, wd);
   check_matrix(dy, d.M, d.N, x, "dy");
   check_matrix(g, d.M, d.Hp, x, "g");
@@ -251,7 +252,8 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
   check_matrix(h, d.M, d.Hp, x, "h");
   TORCH_CHECK(g.is_contiguous() && u.is_contiguous() && h.is_contiguous() && (d.M == 0 || rows_aligned(x)),
               "gated_mlp backward: saved tensors must be as the forward returned them");
-  TORCH_CHECK(dw_into.size() == 3 && db_into.size() == 3, "gated_mlp backward: three weights and biases");
+  TORCH_CHECK(dw_into.size() == 3 && db_into.size() == 3 && types.size() == 6,
+              "gated_mlp backward: three weights and biases");
   check_apart(dw_into, db_into);
   const c10::cuda::CUDAGuard guard(x.device());
   const auto opt = x.options();
@@ -260,8 +262,8 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
     if (need_dx) out[0] = torch::empty({0, d.K}, opt);
     const Tensor w[3] = {wg, wu, wd};
     for (int i = 0; i < 3; ++i) {
-      if (need_w && !dw_into[i]) out[1 + i] = torch::zeros(w[i].sizes(), opt.dtype(wdt));
-      if (need_b && !db_into[i]) out[4 + i] = torch::zeros({w[i].size(0)}, opt.dtype(bdt));
+      if (need_w && !dw_into[i]) out[1 + i] = torch::zeros(w[i].sizes(), opt.dtype(types[i]));
+      if (need_b && !db_into[i]) out[4 + i] = torch::zeros({w[i].size(0)}, opt.dtype(types[3 + i]));
     }
     return out;
   }
@@ -319,8 +321,8 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
     out[0] = dx;
   }
   if (need_w) {
-    const GradOut g0(dw_into[0], {d.H, d.K}, x, wdt), g1(dw_into[1], {d.H, d.K}, x, wdt),
-        g2(dw_into[2], {d.N, d.H}, x, wdt);
+    const GradOut g0(dw_into[0], {d.H, d.K}, x, types[0]), g1(dw_into[1], {d.H, d.K}, x, types[1]),
+        g2(dw_into[2], {d.N, d.H}, x, types[2]);
     nsw::GatedDwArgs w{};
     w.dtype = a.dtype;
     w.T = d.M;
@@ -334,12 +336,13 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
       w.ws = ws.data_ptr<float>();
     }
     check(nsw::gated_dw(w, stream()), "gated_mlp weight gradients");
-    out[1] = g0.result(wdt);
-    out[2] = g1.result(wdt);
-    out[3] = g2.result(wdt);
+    out[1] = g0.result(types[0]);
+    out[2] = g1.result(types[1]);
+    out[3] = g2.result(types[2]);
   }
   if (need_b) {
-    const GradOut g0(db_into[0], {d.H}, x, bdt), g1(db_into[1], {d.H}, x, bdt), g2(db_into[2], {d.N}, x, bdt);
+    const GradOut g0(db_into[0], {d.H}, x, types[3]), g1(db_into[1], {d.H}, x, types[4]),
+        g2(db_into[2], {d.N}, x, types[5]);
     const int64_t n = 2 * d.Hp, pd = nsw::col_sum_parts(d.M, d.N), pg = sums.defined() ? 0 : nsw::col_sum_parts(d.M, n);
     auto partial = torch::empty({pd * d.N + pg * n}, opt.dtype(at::kFloat));
     float* pp = partial.data_ptr<float>();
@@ -352,9 +355,9 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
                                 {ps, rows, n, d.Hp, d.H, g1.t.data_ptr(), g1.f32, g1.into},
                                 {pp, pd, d.N, 0, d.N, g2.t.data_ptr(), g2.f32, g2.into}};
     check(nsw::col_finish(fin, a.dtype, stream()), "gated_mlp bias gradients");
-    out[4] = g0.result(bdt);
-    out[5] = g1.result(bdt);
-    out[6] = g2.result(bdt);
+    out[4] = g0.result(types[3]);
+    out[5] = g1.result(types[4]);
+    out[6] = g2.result(types[5]);
   }
   return out;
 }
@@ -379,33 +382,33 @@ struct GatedNode : public torch::autograd::Function<GatedNode> {
     ctx->saved_data["shape"] = x.sizes().vec();
     ctx->save_for_backward({out[1], out[5], out[6], out[7], out[2], out[3], out[4]});
     ctx->saved_data["act"] = act;
-    int64_t given = 0, type = -1;  // which optional inputs there are, and the biases' type
+    int64_t given = 0;  // which optional inputs there are
+    std::vector<int64_t> types(3, (int64_t)wg.scalar_type());
     int bit = 0;
     for (const OptTensor* t : {&bg, &bu, &bd, &residual}) {
-      if (*t) {
-        given |= 1 << bit;
-        if (bit < 3 && type < 0) type = (int64_t)(*t)->scalar_type();
-      }
+      if (*t) given |= 1 << bit;
+      if (bit < 3) types.push_back((int64_t)(*t ? (*t)->scalar_type() : at::kFloat));
       ++bit;
     }
     ctx->saved_data["given"] = given;
-    ctx->saved_data["bias"] = type;
+    ctx->saved_data["types"] = types;
     return unflat(out[0], x);
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grad) {
     once_differentiable("gated_mlp");
     const auto v = ctx->get_saved_variables();
-    const int64_t bias = ctx->saved_data["bias"].toInt(), given = ctx->saved_data["given"].toInt();
+    const int64_t given = ctx->saved_data["given"].toInt();
+    std::vector<at::ScalarType> types;
+    for (int64_t t : ctx->saved_data["types"].toIntVector()) types.push_back((at::ScalarType)t);
     bool need[8];
     size_t edge = 4;  // graph edges exist for the inputs that were given, in order
     for (int i = 0; i < 8; ++i)
       need[i] = i < 4 ? ctx->needs_input_grad(i) : (((given >> (i - 4)) & 1) != 0 && ctx->needs_input_grad(edge++));
     const bool need_w = need[1] || need[2] || need[3], need_b = need[4] || need[5] || need[6];
     auto g = gated_mlp_bwd(flat(grad[0]), v[0], v[1], v[2], v[3], v[4], v[5], v[6], ctx->saved_data["act"].toInt(),
-                           need[0], need_w, need_b, std::vector<OptTensor>(3),
-                           std::vector<OptTensor>(3), v[1].scalar_type(),
-                           bias < 0 ? at::kFloat : (at::ScalarType)bias);
+                           need[0], need_w, need_b, std::vector<OptTensor>(3), std::vector<OptTensor>(3),
+                           std::move(types));
     if (need[0]) g[0] = g[0].view(ctx->saved_data["shape"].toIntVector());
     for (int i = 1; i < 7; ++i)
       if (!need[i]) g[i] = Tensor();

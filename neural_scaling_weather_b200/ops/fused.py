@@ -412,9 +412,9 @@ class _GatedMLP(torch.autograd.Function):
         given = [id(p) for p in ctx.params + ctx.biases]
         into = lambda p: gradsink.target(p) if need_w and given.count(id(p)) == 1 else None  # noqa: E731
         tw, tb = [into(w) for w in ctx.params], [into(b) for b in ctx.biases]
-        bdt = next((b.dtype for b in ctx.biases if b is not None), torch.float32)
+        types = [torch.float32 if p is None else p.dtype for p in ctx.params + ctx.biases]
         dx, *grads = ext.gated_mlp_bwd(_rows(dy, dy.shape[-1]).to(x2.dtype), x2, *ctx.W, g, u, h, ctx.act, need[0],
-                                       need_w, need_w and any(has_b), tw, tb, ctx.params[0].dtype, bdt)
+                                       need_w, need_w and any(has_b), tw, tb, types)
         if need_w:
             for p, t in zip(ctx.params + ctx.biases, tw + tb):
                 if p is not None:

@@ -223,6 +223,24 @@ def test_gated_fp32_parameters_and_in_place_gradients(dtype):
         assert rel(p.grad, 1 + 2 * a.double()) < 1e-5
 
 
+def test_gated_gradients_keep_their_own_types():
+    """A bias in fp32 beside 16-bit ones gets its fp32 sums (of 300 terms: 1e-6 of their absolute values), and a weight
+    in fp32 beside 16-bit ones the gradient that it has among fp32 ones."""
+    x, w, b, _, dy = gated_inputs(300, 64, 96, 64, BF16, True, False)
+    b = [b[0].requires_grad_(), b[1].requires_grad_(), b[2].float().requires_grad_()]
+    got = torch.autograd.grad(ops.gated_mlp(x, *w, *b), b, dy)
+    assert [t.dtype for t in got] == [BF16, BF16, F32]
+    assert (got[2].double() - dy.double().sum(0)).norm() <= 1e-6 * dy.double().abs().sum(0).norm()
+    for mixed in (0, 1, 2):  # one parameter in fp32 among 16-bit ones
+        ps = [p.clone().float() if i == mixed else p.clone() for i, p in enumerate(w)]
+        all32 = [p.float().requires_grad_() for p in w]
+        ps = [p.requires_grad_() for p in ps]
+        got = torch.autograd.grad(ops.gated_mlp(x, *ps), ps, dy)
+        ref = torch.autograd.grad(ops.gated_mlp(x, *all32), all32, dy)
+        for i, (a, e) in enumerate(zip(got, ref)):
+            assert torch.equal(a, e if i == mixed else e.to(BF16))
+
+
 def test_gated_tied_parameters_and_shared_gradient_buffers():
     """One parameter as both projections and one bias for both: their gradients add up in an existing fp32 ``.grad``
     as in separate ones (two fp32 sums in another order).  Buffers that overlap are refused."""
@@ -243,8 +261,8 @@ def test_gated_tied_parameters_and_shared_gradient_buffers():
     for at in (0, 512 * 256 - 4):
         into = [flat[:512 * 256].view(512, 256), flat[at:at + 512 * 256].view(512, 256), None]
         with pytest.raises(RuntimeError, match="overlap"):
-            ext.gated_mlp_bwd(dy, x2, *ws, g, u, h, 0, False, True, False, into, [None] * 3, torch.float32,
-                              torch.float32)
+            ext.gated_mlp_bwd(dy, x2, *ws, g, u, h, 0, False, True, False, into, [None] * 3,
+                              [torch.float32] * 6)
     assert not flat.any()
 
 
