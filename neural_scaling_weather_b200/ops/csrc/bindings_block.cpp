@@ -76,6 +76,7 @@ struct Aligner {
   }
 };
 
+OptTensor packed_vec(const OptTensor& t) { return t ? OptTensor(t->contiguous()) : OptTensor(); }
 const void* opt_ptr(const OptTensor& t) { return t && t->defined() ? t->data_ptr() : nullptr; }
 
 void check_matrix(const Tensor& t, int64_t rows, int64_t cols, const Tensor& like, const char* name) {
@@ -87,8 +88,8 @@ void check_matrix(const Tensor& t, int64_t rows, int64_t cols, const Tensor& lik
 }
 void check_bias(const OptTensor& b, int64_t n, const Tensor& like, int* dtype, const char* name) {
   if (!b || !b->defined()) return;
-  TORCH_CHECK(b->is_cuda() && b->device() == like.device() && b->dim() == 1 && b->numel() == n && b->is_contiguous(),
-              "gated_mlp: ", name, " must be a contiguous CUDA vector of ", n, " elements");
+  TORCH_CHECK(b->is_cuda() && b->device() == like.device() && b->dim() == 1 && b->numel() == n, "gated_mlp: ", name,
+              " must be a CUDA vector of ", n, " elements");
   const int d = dt_code(*b, name);
   TORCH_CHECK(*dtype < 0 || *dtype == d, "gated_mlp: the gate's and the up projection's biases must share a dtype");
   *dtype = d;
@@ -117,13 +118,13 @@ GatedShape gated_shape(const Tensor& x, const Tensor& wg, const Tensor& wu, cons
 // returns {y} or {y, x, g, u, h, wg, wu, wd} with x and the weights as read (copies with padded rows where theirs are
 // not aligned) and the rows of g, u and h padded to a multiple of 8 elements.
 std::vector<Tensor> gated_mlp_fwd(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tensor& wd,
-                                  const OptTensor& bg, const OptTensor& bu, const OptTensor& bd,
+                                  const OptTensor& b_gate, const OptTensor& b_up, const OptTensor& b_down,
                                   const OptTensor& residual, int64_t act, bool save) {
   const GatedShape d = gated_shape(x, wg, wu, wd);
   int bdt = -1, ddt = -1;
-  check_bias(bg, d.H, x, &bdt, "b_gate");
-  check_bias(bu, d.H, x, &bdt, "b_up");
-  check_bias(bd, d.N, x, &ddt, "b_down");
+  check_bias(b_gate, d.H, x, &bdt, "b_gate");
+  check_bias(b_up, d.H, x, &bdt, "b_up");
+  check_bias(b_down, d.N, x, &ddt, "b_down");
   const bool has_res = residual && residual->defined();
   if (has_res) check_matrix(*residual, d.M, d.N, x, "residual");
   const c10::cuda::CUDAGuard guard(x.device());
@@ -133,6 +134,7 @@ std::vector<Tensor> gated_mlp_fwd(const Tensor& x, const Tensor& wg, const Tenso
     if (!save) return {y};
     return {y, x, e, e, e, wg, wu, wd};
   }
+  const OptTensor bg = packed_vec(b_gate), bu = packed_vec(b_up), bd = packed_vec(b_down);
   auto h = torch::empty({d.M, d.Hp}, opt);
   nsw::GatedArgs up{}, down{};
   up.mode = nsw::kGatedUp;
@@ -533,8 +535,6 @@ std::vector<Tensor> norm_gate_bwd(const OptTensor& ds, const OptTensor& dn, cons
   check(nsw::norm_gate_bwd(a, blocks, stream()), "norm_gate_bwd");
   return {dy, dskip, dwp, dgate, dwn};
 }
-
-OptTensor packed_vec(const OptTensor& t) { return t ? OptTensor(t->contiguous()) : OptTensor(); }
 
 struct NormGateNode : public torch::autograd::Function<NormGateNode> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& y_in,

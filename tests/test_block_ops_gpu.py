@@ -223,6 +223,20 @@ def test_gated_fp32_parameters_and_in_place_gradients(dtype):
         assert rel(p.grad, 1 + 2 * a.double()) < 1e-5
 
 
+@pytest.mark.parametrize("M", [3, 300])
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_gated_strided_biases(M, dt):
+    x, w, b, _, dy = gated_inputs(M, 64, 96, 64, BF16, True, False)
+    b = [t.to(dt) for t in b]
+    strided = [torch.stack([t, 0 * t], 1)[:, 0] for t in b]
+    assert not any(t.is_contiguous() for t in strided)
+    with torch.no_grad():
+        assert torch.equal(ops.gated_mlp(x, *w, *strided), ops.gated_mlp(x, *w, *b))
+    leaves = [[t.requires_grad_() for t in v] for v in (strided, b)]
+    got, ref = (torch.autograd.grad(ops.gated_mlp(x, *w, *v), v, dy) for v in leaves)
+    assert all(torch.equal(a, e) for a, e in zip(got, ref))
+
+
 def test_gated_gradients_keep_their_own_types():
     """A bias in fp32 beside 16-bit ones gets its fp32 sums (of 300 terms: 1e-6 of their absolute values), and a weight
     in fp32 beside 16-bit ones the gradient that it has among fp32 ones."""
