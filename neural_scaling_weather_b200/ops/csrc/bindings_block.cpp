@@ -516,7 +516,8 @@ std::vector<Tensor> norm_gate_bwd(const OptTensor& ds, const OptTensor& dn, cons
   auto dy = torch::empty_like(y), dskip = torch::empty_like(y);
   const int64_t n = a.n;
   if (y.numel() == 0)
-    return {dy, dskip, torch::zeros({n}, f32), a.gate ? torch::zeros({a.samples, n}, f32) : Tensor(),
+    return {dy, dskip, torch::zeros({n}, f32),  // (a gate of no samples has no address)
+            gate && gate->defined() ? torch::zeros({a.samples, n}, f32) : Tensor(),
             a.wn ? torch::zeros({n}, f32) : Tensor()};
   const int blocks = nsw::norm_gate_blocks(a.samples, a.rows, a.n, sm_count(y));
   auto part = torch::empty({a.samples * blocks * 2 * n}, f32);

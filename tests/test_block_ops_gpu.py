@@ -515,6 +515,14 @@ def test_norm_gate_residual_empty_and_refusals():
         ops.norm_gate_residual(z, z, torch.ones(16385, device=DEV))
 
 
+def test_norm_gate_residual_empty_batch():
+    y, skip, wp, gt, wn, _, _ = norm_inputs(2, 3, 64, BF16, "sample", True)
+    leaves = [t.clone().requires_grad_() for t in (y[:0], skip[:0], wp, gt[:0], wn)]
+    s, n = ops.norm_gate_residual(*leaves)
+    got = torch.autograd.grad([s, n], leaves, [torch.zeros_like(s), torch.zeros_like(n)])
+    assert all(g.shape == t.shape and not g.any() for g, t in zip(got, leaves))
+
+
 # --------------------------------------------------------------------------- gradient clipping
 def clip_inputs(shapes, dtypes, std=0.1):
     g = torch.Generator(device=DEV).manual_seed(3)
