@@ -174,6 +174,7 @@ class Block(nn.Module):
         if block_norm not in ("pre", "sandwich"):
             raise ValueError(f"block_norm {block_norm!r} is neither 'pre' nor 'sandwich'")
         self.dim = dim
+        self.block_norm = block_norm
         self.feat_size = tuple(feat_size)
         self.window_size = tuple(window_size)
         self.window_area = window_size[0] * window_size[1]
@@ -245,8 +246,14 @@ class Block(nn.Module):
             shapes=(self.sp1_shapes, self.sp2_shapes))
         return y if skip is None else y + skip
 
-    def forward(self, x: torch.Tensor, condition: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """x: (B, T, H, W, C) -> same shape."""
+    def forward(self, x: torch.Tensor, condition: Optional[torch.Tensor] = None,
+                normed: Optional[torch.Tensor] = None, next_weight: Optional[torch.Tensor] = None):
+        """x: (B, T, H, W, C) -> same shape.  A sandwich block that is given ``normed``, the norm of ``x`` by its
+        first weight, returns the pair of :meth:`forward_sandwich`."""
+        if self.block_norm == "sandwich":
+            if normed is not None:
+                return self.forward_sandwich(x, normed, next_weight)
+            return self.forward_sandwich(x, ops.rms_norm(x, self.norm1.weight), None)[0]
         # each pre-norm and its skip connection come from one node, so the two gradients of
         # the residual stream are summed inside the RMSNorm backward
         h, skip = self._norm_skip(self.norm1, x)
@@ -392,7 +399,8 @@ class SwinTransformer(nn.Module):
         if self.block_norm == "sandwich":
             normed = ops.rms_norm(x, self.blocks[0].norm1.weight)
             for blk, following in zip(self.blocks, [*self.blocks[1:], None]):
-                x, normed = blk.forward_sandwich(x, normed, None if following is None else following.norm1.weight)
+                x, normed = blk(x, normed=normed,
+                                next_weight=None if following is None else following.norm1.weight)
         else:
             for blk in self.blocks:
                 x = blk(x)

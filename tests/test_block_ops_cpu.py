@@ -207,6 +207,26 @@ def test_sandwich_block_is_its_formula(mlp_type):
     assert torch.allclose(model.forward_head(s)[:, -1:], model(x), atol=1e-5)
 
 
+def test_sandwich_blocks_are_called_as_modules():
+    """Hooks on the blocks run, and a block by itself, given the stream alone, is the sandwich block."""
+    torch.manual_seed(0)
+    model = get_model(_cfg(mlp_type="swiglu", block_norm="sandwich"), create_dummy_metadata(16, 32, 4)).model
+    with torch.no_grad():
+        for p in model.parameters():
+            p.add_(0.05 * torch.randn_like(p))
+    streams = []
+    for blk in model.blocks:
+        blk.register_forward_pre_hook(lambda _, args: streams.append(args[0]))
+        blk.register_forward_hook(lambda *a: streams.append(a[-1][0]))
+    model(torch.randn(2, 1, 5, 16, 32))
+    assert len(streams) == 2 * len(model.blocks)
+    for i, blk in enumerate(model.blocks):
+        before, after = streams[2 * i], streams[2 * i + 1]
+        for hooks in (blk._forward_pre_hooks, blk._forward_hooks):
+            hooks.clear()
+        assert torch.allclose(blk(before), after, atol=1e-6)
+
+
 def test_options_validate_and_default_to_the_plain_block():
     md = create_dummy_metadata(16, 32, 4)
     names = lambda **k: set(dict(get_model(_cfg(**k), md).named_parameters()))  # noqa: E731
