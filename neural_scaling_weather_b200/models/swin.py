@@ -154,8 +154,9 @@ class GatedMLP(nn.Module):
         if comm.get_size("tp") == 1 and not drop:
             return ops.gated_mlp(x, self.gate.weight, self.up.weight, self.down.weight, self.biasgate.bias,
                                  self.biasup.bias, self.biasdown.bias, residual=residual, activation=self.activation)
-        g = ops.linear_colparallel(x, self.gate.weight, self.biasgate.bias, group="tp")
-        u = ops.linear_colparallel(x, self.up.weight, self.biasup.bias, group="tp")
+        # as one linear: one product, and one all-reduce of the input's gradient over tp
+        g, u = ops.linear_colparallel(x, [self.gate.weight, self.up.weight], [self.biasgate.bias, self.biasup.bias],
+                                      group="tp").chunk(2, dim=-1)
         h = (F.silu(g) if self.activation == "silu" else F.gelu(g)) * u
         if not drop:
             return ops.linear_allreduce(h, self.down.weight, self.biasdown.bias, residual=residual, group="tp")

@@ -273,6 +273,38 @@ def test_gated_sandwich_model_sharded_matches_single_rank(tp, sp1, sp2):
     run(_sharded_worker, tp * sp1 * sp2, tp, sp1, sp2)
 
 
+def _all_reduces_worker(rank, world, drop):
+    import torch.distributed as dist
+
+    from neural_scaling_weather_b200.models.swin import GatedMLP
+    from neural_scaling_weather_b200.parallel import comm
+
+    comm.init_model_parallel_info(tp=world, sp1=1, sp2=1, dp=1)
+    torch.manual_seed(0)
+    mlp = GatedMLP(16, 48, "swiglu", drop)
+    for p in mlp.parameters():
+        torch.nn.init.normal_(p, std=0.2)
+    x = torch.randn(2, 3, 16, requires_grad=True)
+    y = mlp(x)
+    plain, sizes = dist.all_reduce, []
+
+    def counted(t, *a, **k):
+        sizes.append(t.numel())
+        return plain(t, *a, **k)
+
+    dist.all_reduce = counted
+    try:
+        y.sum().backward()
+    finally:
+        dist.all_reduce = plain
+    assert sizes == [x.numel()], sizes
+
+
+@pytest.mark.parametrize("drop", [0.0, 0.5])
+def test_gated_mlp_sums_its_input_gradient_once_over_tp(drop):
+    run(_all_reduces_worker, 2, drop)
+
+
 def test_example_trains_on_cpu():
     out = subprocess.run([sys.executable, os.path.join(ROOT, "examples", "train_gated_block.py"), "--steps", "4",
                           "--dim", "64", "--depth", "1", "--grid", "36x72", "--channels", "2"], cwd=ROOT,
