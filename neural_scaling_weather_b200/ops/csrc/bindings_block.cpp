@@ -215,7 +215,8 @@ std::vector<Tensor> gated_mlp_fwd(const Tensor& x, const Tensor& wg, const Tenso
 // the parameter's type, else fp32 and cast at the end)
 struct GradOut {
   Tensor t;
-  bool f32, into;
+  bool f32 = false, into = false;
+  GradOut() = default;
   GradOut(const OptTensor& dst, at::IntArrayRef sizes, const Tensor& like, at::ScalarType dtype)
       : f32(dst.has_value() || dtype != like.scalar_type()), into(dst.has_value()) {
     t = into ? *dst : torch::empty(sizes, f32 ? like.options().dtype(at::kFloat) : like.options());
@@ -227,26 +228,25 @@ struct GradOut {
 };
 
 // The kernels read, add and write their targets without regard to one another
-void check_apart(const std::vector<OptTensor>& a, const std::vector<OptTensor>& b) {
+void check_apart(const std::vector<OptTensor>& into) {
   std::vector<std::pair<const char*, const char*>> at;
-  for (const auto* v : {&a, &b})
-    for (const OptTensor& t : *v)
-      if (t && t->numel() > 0) {
-        const char* p = static_cast<const char*>(t->data_ptr());
-        at.emplace_back(p, p + t->nbytes());
-      }
+  for (const OptTensor& t : into)
+    if (t && t->numel() > 0) {
+      const char* p = static_cast<const char*>(t->data_ptr());
+      at.emplace_back(p, p + t->nbytes());
+    }
   std::sort(at.begin(), at.end());
   for (size_t i = 1; i < at.size(); ++i)
     TORCH_CHECK(at[i].first >= at[i - 1].second, "gated_mlp backward: gradient buffers overlap");
 }
 
-// Gradients from dy and what the forward saved: {dx, dwg, dwu, dwd, dbg, dbu, dbd}.  An entry is undefined
-// where it was not asked for (need_dx, need_w, need_b) or was added into the given fp32 buffer.  types: of the three
-// weights' and the three biases' gradients, their parameters'.
+// Gradients from dy and what the forward saved: {dx, dwg, dwu, dwd, dbg, dbu, dbd}, of which only those with need
+// set are computed.  An entry is undefined where it is not needed or was added into its fp32 buffer in `into` (three
+// weights, three biases).  types: of the same six, their parameters'.
 std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tensor& wg, const Tensor& wu,
                                   const Tensor& wd, const Tensor& g, const Tensor& u, const Tensor& h, int64_t act,
-                                  bool need_dx, bool need_w, bool need_b, std::vector<OptTensor> dw_into,
-                                  std::vector<OptTensor> db_into, std::vector<at::ScalarType> types) {
+                                  const std::vector<bool>& need, const std::vector<OptTensor>& into,
+                                  const std::vector<at::ScalarType>& types) {
   const GatedShape d = gated_shape(x, wg, wu, wd);
   check_matrix(dy, d.M, d.N, x, "dy");
   check_matrix(g, d.M, d.Hp, x, "g");
@@ -254,59 +254,63 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
   check_matrix(h, d.M, d.Hp, x, "h");
   TORCH_CHECK(g.is_contiguous() && u.is_contiguous() && h.is_contiguous() && (d.M == 0 || rows_aligned(x)),
               "gated_mlp backward: saved tensors must be as the forward returned them");
-  TORCH_CHECK(dw_into.size() == 3 && db_into.size() == 3 && types.size() == 6,
-              "gated_mlp backward: three weights and biases");
-  check_apart(dw_into, db_into);
+  TORCH_CHECK(need.size() == 7 && into.size() == 6 && types.size() == 6,
+              "gated_mlp backward: x, three weights and three biases");
+  check_apart(into);
   const c10::cuda::CUDAGuard guard(x.device());
   const auto opt = x.options();
   std::vector<Tensor> out(7);
+  const std::vector<int64_t> sizes[6] = {{d.H, d.K}, {d.H, d.K}, {d.N, d.H}, {d.H}, {d.H}, {d.N}};
   if (d.M == 0) {
-    if (need_dx) out[0] = torch::empty({0, d.K}, opt);
-    const Tensor w[3] = {wg, wu, wd};
-    for (int i = 0; i < 3; ++i) {
-      if (need_w && !dw_into[i]) out[1 + i] = torch::zeros(w[i].sizes(), opt.dtype(types[i]));
-      if (need_b && !db_into[i]) out[4 + i] = torch::zeros({w[i].size(0)}, opt.dtype(types[3 + i]));
-    }
+    if (need[0]) out[0] = torch::empty({0, d.K}, opt);
+    for (int i = 0; i < 6; ++i)
+      if (need[1 + i] && !into[i]) out[1 + i] = torch::zeros(sizes[i], opt.dtype(types[i]));
     return out;
   }
+  GradOut grad[6];
+  for (int i = 0; i < 6; ++i)
+    if (need[1 + i]) grad[i] = GradOut(into[i], sizes[i], x, types[i]);
+  const bool need_hidden = need[0] || need[1] || need[2] || need[4] || need[5];  // what follows from dg and du
   Aligner al;  // (the weights are the forward's aligned ones already)
   const Rows dya = al.add(dy), ga = al.add(wg), ua = al.add(wu), da = al.add(wd);
   al.run();
   const Rows xa{x, d.M == 1 ? round8(d.K) : x.stride(0)};
-  auto dgu = torch::empty({d.M, 2 * d.Hp}, opt);
-  char* du = reinterpret_cast<char*>(dgu.data_ptr()) + 2 * d.Hp;
-  nsw::GatedArgs a{};
-  a.mode = nsw::kGatedDh;
-  a.dtype = dt_code(x, "x");
-  a.act = (int)act;
-  a.M = d.M;
-  a.N = d.H;
-  a.K = d.N;
-  a.a0 = dya.ptr();
-  a.lda = dya.ld;
-  a.b0 = da.ptr();
-  a.ldb0 = da.ld;
-  a.in0 = g.data_ptr();
-  a.in1 = u.data_ptr();
-  a.ldin = d.Hp;
-  a.out0 = dgu.data_ptr();
-  a.out1 = du;
-  a.ldout = a.ldaux = 2 * d.Hp;
-  Tensor sums;
-  if (need_b) {
-    const int64_t rows = nsw::gated_sum_rows(a);
+  Tensor dgu, sums;
+  char* du = nullptr;
+  const int dtype = dt_code(x, "x");
+  if (need_hidden) {
+    dgu = torch::empty({d.M, 2 * d.Hp}, opt);
+    du = reinterpret_cast<char*>(dgu.data_ptr()) + 2 * d.Hp;
+    nsw::GatedArgs a{};
+    a.mode = nsw::kGatedDh;
+    a.dtype = dtype;
+    a.act = (int)act;
+    a.M = d.M;
+    a.N = d.H;
+    a.K = d.N;
+    a.a0 = dya.ptr();
+    a.lda = dya.ld;
+    a.b0 = da.ptr();
+    a.ldb0 = da.ld;
+    a.in0 = g.data_ptr();
+    a.in1 = u.data_ptr();
+    a.ldin = d.Hp;
+    a.out0 = dgu.data_ptr();
+    a.out1 = du;
+    a.ldout = a.ldaux = 2 * d.Hp;
+    const int64_t rows = need[4] || need[5] ? nsw::gated_sum_rows(a) : 0;
     if (rows > 0) {
       sums = torch::empty({rows, 2 * d.Hp}, opt.dtype(at::kFloat));
       a.sums = sums.data_ptr<float>();
       a.sums_half = d.Hp;
     }
+    check(nsw::gated_product(a, false, stream()), "gated_mlp dh");
   }
-  check(nsw::gated_product(a, false, stream()), "gated_mlp dh");
-  if (need_dx) {
+  if (need[0]) {
     auto dx = torch::empty({d.M, d.K}, opt);
     nsw::GatedArgs b{};
     b.mode = nsw::kGatedDx;
-    b.dtype = a.dtype;
+    b.dtype = dtype;
     b.M = d.M;
     b.N = d.K;
     b.K = d.H;
@@ -322,15 +326,15 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
     check(nsw::gated_product(b, true, stream()), "gated_mlp dx");
     out[0] = dx;
   }
-  if (need_w) {
-    const GradOut g0(dw_into[0], {d.H, d.K}, x, types[0]), g1(dw_into[1], {d.H, d.K}, x, types[1]),
-        g2(dw_into[2], {d.N, d.H}, x, types[2]);
+  if (need[1] || need[2] || need[3]) {
     nsw::GatedDwArgs w{};
-    w.dtype = a.dtype;
+    w.dtype = dtype;
     w.T = d.M;
-    w.w[0] = {dgu.data_ptr(), xa.ptr(), 2 * d.Hp, xa.ld, d.H, d.K, g0.t.data_ptr(), g0.f32, g0.into};
-    w.w[1] = {du, xa.ptr(), 2 * d.Hp, xa.ld, d.H, d.K, g1.t.data_ptr(), g1.f32, g1.into};
-    w.w[2] = {dya.ptr(), h.data_ptr(), dya.ld, d.Hp, d.N, d.H, g2.t.data_ptr(), g2.f32, g2.into};
+    const auto dst = [&](int i) { return need[1 + i] ? grad[i].t.data_ptr() : nullptr; };
+    w.w[0] = {need_hidden ? dgu.data_ptr() : nullptr, xa.ptr(), 2 * d.Hp, xa.ld, d.H, d.K, dst(0), grad[0].f32,
+              grad[0].into};
+    w.w[1] = {du, xa.ptr(), 2 * d.Hp, xa.ld, d.H, d.K, dst(1), grad[1].f32, grad[1].into};
+    w.w[2] = {dya.ptr(), h.data_ptr(), dya.ld, d.Hp, d.N, d.H, dst(2), grad[2].f32, grad[2].into};
     Tensor ws;
     const int64_t wsn = nsw::gated_dw_workspace(w);
     if (wsn > 0) {
@@ -338,29 +342,32 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
       w.ws = ws.data_ptr<float>();
     }
     check(nsw::gated_dw(w, stream()), "gated_mlp weight gradients");
-    out[1] = g0.result(types[0]);
-    out[2] = g1.result(types[1]);
-    out[3] = g2.result(types[2]);
   }
-  if (need_b) {
-    const GradOut g0(db_into[0], {d.H}, x, types[3]), g1(db_into[1], {d.H}, x, types[4]),
-        g2(db_into[2], {d.N}, x, types[5]);
-    const int64_t n = 2 * d.Hp, pd = nsw::col_sum_parts(d.M, d.N), pg = sums.defined() ? 0 : nsw::col_sum_parts(d.M, n);
-    auto partial = torch::empty({pd * d.N + pg * n}, opt.dtype(at::kFloat));
-    float* pp = partial.data_ptr<float>();
-    const nsw::ColSource src[2] = {{dya.ptr(), dya.ld, d.M, d.N, pd, pp},
-                                   {dgu.data_ptr(), n, d.M, n, pg, pp + pd * d.N}};
-    check(nsw::col_partial(src, pg > 0 ? 2 : 1, a.dtype, stream()), "gated_mlp bias gradients");
-    const float* ps = pg > 0 ? src[1].partial : sums.data_ptr<float>();
-    const int64_t rows = pg > 0 ? pg : sums.size(0);
-    const nsw::ColSum fin[3] = {{ps, rows, n, 0, d.H, g0.t.data_ptr(), g0.f32, g0.into},
-                                {ps, rows, n, d.Hp, d.H, g1.t.data_ptr(), g1.f32, g1.into},
-                                {pp, pd, d.N, 0, d.N, g2.t.data_ptr(), g2.f32, g2.into}};
-    check(nsw::col_finish(fin, a.dtype, stream()), "gated_mlp bias gradients");
-    out[4] = g0.result(types[3]);
-    out[5] = g1.result(types[4]);
-    out[6] = g2.result(types[5]);
+  if (need[4] || need[5] || need[6]) {
+    // dy's columns, and those of dg and du where the product before has not summed them
+    const int64_t n = 2 * d.Hp, pd = need[6] ? nsw::col_sum_parts(d.M, d.N) : 0,
+                  pg = (need[4] || need[5]) && !sums.defined() ? nsw::col_sum_parts(d.M, n) : 0;
+    Tensor partial;
+    float* pp = nullptr;
+    if (pd + pg > 0) {
+      partial = torch::empty({pd * d.N + pg * n}, opt.dtype(at::kFloat));
+      pp = partial.data_ptr<float>();
+      nsw::ColSource src[2];
+      int count = 0;
+      if (pd > 0) src[count++] = {dya.ptr(), dya.ld, d.M, d.N, pd, pp};
+      if (pg > 0) src[count++] = {dgu.data_ptr(), n, d.M, n, pg, pp + pd * d.N};
+      check(nsw::col_partial(src, count, dtype, stream()), "gated_mlp bias gradients");
+    }
+    const float* ps = pg > 0 ? pp + pd * d.N : sums.defined() ? sums.data_ptr<float>() : nullptr;
+    const int64_t rows = pg > 0 ? pg : sums.defined() ? sums.size(0) : 0;
+    const auto dst = [&](int i) { return need[1 + i] ? grad[i].t.data_ptr() : nullptr; };
+    const nsw::ColSum fin[3] = {{ps, rows, n, 0, d.H, dst(3), grad[3].f32, grad[3].into},
+                                {ps, rows, n, d.Hp, d.H, dst(4), grad[4].f32, grad[4].into},
+                                {pp, pd, d.N, 0, d.N, dst(5), grad[5].f32, grad[5].into}};
+    check(nsw::col_finish(fin, dtype, stream()), "gated_mlp bias gradients");
   }
+  for (int i = 0; i < 6; ++i)
+    if (need[1 + i]) out[1 + i] = grad[i].result(types[i]);
   return out;
 }
 
@@ -403,18 +410,15 @@ struct GatedNode : public torch::autograd::Function<GatedNode> {
     const int64_t given = ctx->saved_data["given"].toInt();
     std::vector<at::ScalarType> types;
     for (int64_t t : ctx->saved_data["types"].toIntVector()) types.push_back((at::ScalarType)t);
-    bool need[8];
+    std::vector<bool> need(7);
     size_t edge = 4;  // graph edges exist for the inputs that were given, in order
-    for (int i = 0; i < 8; ++i)
-      need[i] = i < 4 ? ctx->needs_input_grad(i) : (((given >> (i - 4)) & 1) != 0 && ctx->needs_input_grad(edge++));
-    const bool need_w = need[1] || need[2] || need[3], need_b = need[4] || need[5] || need[6];
+    const auto opt_needed = [&](int i) { return ((given >> i) & 1) != 0 && ctx->needs_input_grad(edge++); };
+    for (int i = 0; i < 7; ++i) need[i] = i < 4 ? ctx->needs_input_grad(i) : opt_needed(i - 4);
+    const bool need_res = opt_needed(3);
     auto g = gated_mlp_bwd(flat(grad[0]), v[0], v[1], v[2], v[3], v[4], v[5], v[6], ctx->saved_data["act"].toInt(),
-                           need[0], need_w, need_b, std::vector<OptTensor>(3), std::vector<OptTensor>(3),
-                           std::move(types));
+                           need, std::vector<OptTensor>(6), types);
     if (need[0]) g[0] = g[0].view(ctx->saved_data["shape"].toIntVector());
-    for (int i = 1; i < 7; ++i)
-      if (!need[i]) g[i] = Tensor();
-    g.push_back(need[7] ? grad[0] : Tensor());  // residual
+    g.push_back(need_res ? grad[0] : Tensor());  // residual
     g.push_back(Tensor());                      // act
     return g;
   }

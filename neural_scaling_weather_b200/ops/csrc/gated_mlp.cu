@@ -733,7 +733,9 @@ static DwPlan dw_plan(int64_t tiles, int64_t K) {
   }
   return best;
 }
-static int64_t dw_tiles(int64_t M, int64_t N) { return ((M + BM2 - 1) / BM2) * ((N + BN2 - 1) / BN2); }
+static int64_t dw_tiles(const GatedDwArgs::Weight& w) {
+  return w.D ? ((w.M + BM2 - 1) / BM2) * ((w.N + BN2 - 1) / BN2) : 0;
+}
 
 // launches gated_kernel for `units` tiles of work; `fill` encodes the operands (false: refused)
 template <typename T, int MODE, typename Fill>
@@ -821,13 +823,17 @@ static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
 template <typename T>
 static cudaError_t launch_dw(const GatedDwArgs& a, cudaStream_t s) {
   int64_t tiles = 0;
-  for (const auto& w : a.w) tiles += dw_tiles(w.M, w.N);
+  for (const auto& w : a.w) tiles += dw_tiles(w);
   const DwPlan plan = dw_plan(tiles, a.T);
   if (plan.rem > 0 && !a.ws) return cudaErrorInvalidValue;
   GatedParams p;
   NSW_CUDA_CHECK((launch_pairs<T, kDw>(
       std::max<int64_t>(plan.direct, (int64_t)plan.rem * plan.splits), a.dtype, s, p, [&]() {
-        const auto& w = a.w;
+        // a weight without tiles has the maps of one with them: valid, and not read through
+        const auto with = [&](int i, int j) -> const GatedDwArgs::Weight& {
+          return a.w[i].D ? a.w[i] : a.w[j].D ? a.w[j] : a.w[3 - i - j];
+        };
+        const GatedDwArgs::Weight w[kDwWeights] = {with(0, 1), with(1, 0), with(2, 0)};
         bool ok = make_map_mn(&p.a0, w[0].a, a.T, w[0].M, w[0].lda, a.dtype) &&
                   make_map_mn(&p.a1, w[1].a, a.T, w[1].M, w[1].lda, a.dtype) &&
                   make_map_mn(&p.a2, w[2].a, a.T, w[2].M, w[2].lda, a.dtype) &&
@@ -836,8 +842,8 @@ static cudaError_t launch_dw(const GatedDwArgs& a, cudaStream_t s) {
         CUtensorMap* out[kDwWeights] = {&p.out0, &p.out1, &p.out2};
         int64_t end = 0;
         for (int i = 0; i < kDwWeights; ++i) {
-          end += dw_tiles(w[i].M, w[i].N);
-          const bool tma = !w[i].out_f32 && w[i].N % 8 == 0 && (reinterpret_cast<uintptr_t>(w[i].D) & 15) == 0;
+          end += dw_tiles(a.w[i]);
+          const bool tma = a.w[i].D && !w[i].out_f32 && w[i].N % 8 == 0 && (reinterpret_cast<uintptr_t>(w[i].D) & 15) == 0;
           p.seg[i] = {end, (w[i].N + BN2 - 1) / BN2, w[i].M, w[i].N, w[i].N, w[i].D, w[i].out_f32, w[i].accumulate, tma};
           if (tma) ok = ok && make_store_map(out[i], w[i].D, w[i].M, w[i].N, w[i].N, a.dtype);
         }
@@ -1687,15 +1693,16 @@ cudaError_t col_finish(const ColSum* v, int dtype, cudaStream_t s) {
 
 int64_t gated_dw_workspace(const GatedDwArgs& a) {
   int64_t tiles = 0;
-  for (const auto& w : a.w) tiles += tc::dw_tiles(w.M, w.N);
+  for (const auto& w : a.w) tiles += tc::dw_tiles(w);
   const tc::DwPlan p = tc::dw_plan(tiles, a.T);
   return (int64_t)p.rem * p.splits * tc::BM2 * tc::BN2;
 }
 
 cudaError_t gated_dw(const GatedDwArgs& a, cudaStream_t s) {
   if ((a.dtype != kBF16 && a.dtype != kF16) || a.T <= 0) return cudaErrorInvalidValue;
+  if (!a.w[0].D && !a.w[1].D && !a.w[2].D) return cudaErrorInvalidValue;
   for (const auto& w : a.w)
-    if (w.M <= 0 || w.N <= 0 || !w.D || (w.accumulate && !w.out_f32)) return cudaErrorInvalidValue;
+    if (w.D && (!w.a || !w.b || w.M <= 0 || w.N <= 0 || (w.accumulate && !w.out_f32))) return cudaErrorInvalidValue;
   return a.dtype == kBF16 ? tc::launch_dw<__nv_bfloat16>(a, s) : tc::launch_dw<__half>(a, s);
 }
 

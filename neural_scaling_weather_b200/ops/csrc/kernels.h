@@ -196,7 +196,7 @@ struct GatedArgs {
   int64_t sums_half;
 };
 int64_t gated_sum_rows(const GatedArgs& a);
-// The three weight gradients in one launch: w[i].D (+)= w[i].a^T w[i].b over T tokens; a [T, M] in rows of lda,
+// The three weight gradients, or those of them with a D, in one launch: w[i].D (+)= w[i].a^T w[i].b over T tokens; a [T, M] in rows of lda,
 // b [T, N] in rows of ldb (16-byte aligned rows; w[1].b is w[0].b), D contiguous [M, N], 16-bit or (out_f32) fp32,
 // added to with accumulate; ws: gated_dw_workspace floats.
 struct GatedDwArgs {

@@ -405,22 +405,18 @@ class _GatedMLP(torch.autograd.Function):
         ext = require()
         x2, g, u, h = ctx.saved_tensors
         need = ctx.needs_input_grad
-        need_w = any(need[3:])
-        has_b = [b is not None for b in ctx.biases]
+        params = ctx.params + ctx.biases
         # the kernels add to all targets at once: a parameter that is here more than once gets its shares through
         # autograd, which adds them one after the other
-        given = [id(p) for p in ctx.params + ctx.biases]
-        into = lambda p: gradsink.target(p) if need_w and given.count(id(p)) == 1 else None  # noqa: E731
-        tw, tb = [into(w) for w in ctx.params], [into(b) for b in ctx.biases]
-        types = [torch.float32 if p is None else p.dtype for p in ctx.params + ctx.biases]
-        dx, *grads = ext.gated_mlp_bwd(_rows(dy, dy.shape[-1]).to(x2.dtype), x2, *ctx.W, g, u, h, ctx.act, need[0],
-                                       need_w, need_w and any(has_b), tw, tb, types)
-        if need_w:
-            for p, t in zip(ctx.params + ctx.biases, tw + tb):
+        given = [id(p) for p in params]
+        into = [gradsink.target(p) if n and given.count(id(p)) == 1 else None for p, n in zip(params, need[3:])]
+        types = [torch.float32 if p is None else p.dtype for p in params]
+        dx, *out = ext.gated_mlp_bwd(_rows(dy, dy.shape[-1]).to(x2.dtype), x2, *ctx.W, g, u, h, ctx.act,
+                                     [need[0], *need[3:]], into, types)
+        if any(need[3:]):
+            for p, t in zip(params, into):
                 if p is not None:
                     gradsink.done(p, t is not None)
-        out = [gr if p is not None and n else None
-               for p, n, gr in zip(ctx.params + ctx.biases, need[3:], grads)]
         dx = dx.view(ctx.x_shape).to(ctx.x_dtype) if need[0] else None
         return (dx, dy.to(ctx.res_dtype) if need[1] else None, None, *out)
 

@@ -142,12 +142,12 @@ def test_in_place_gradients_of_tied_parameters(tied, monkeypatch):
             return [torch.ones_like(x), x, x, x, x, wg, wu, wd]
 
         @staticmethod
-        def gated_mlp_bwd(dy, x, wg, wu, wd, g, u, h, act, need_dx, need_w, need_b, dw, db, *dtypes):
-            seen.append([t for t in list(dw) + list(db) if t is not None])
+        def gated_mlp_bwd(dy, x, wg, wu, wd, g, u, h, act, need, into, types):
+            seen.append([t for t in into if t is not None])
             for t in seen[-1]:
                 t.add_(1)
-            return [None] + [None if t is not None else torch.ones(n, n) for t in dw] + [
-                None if t is not None else torch.ones(n) for t in db]
+            return [None] + [None if t is not None else torch.ones(n, n) if i < 3 else torch.ones(n)
+                             for i, t in enumerate(into)]
 
     monkeypatch.setattr(fused, "require", lambda: Ext)
     notices = []

@@ -273,10 +273,9 @@ def test_gated_tied_parameters_and_shared_gradient_buffers():
     x2, g, u, h, *ws = saved
     flat = torch.zeros(2 * 512 * 256, device=DEV)
     for at in (0, 512 * 256 - 4):
-        into = [flat[:512 * 256].view(512, 256), flat[at:at + 512 * 256].view(512, 256), None]
+        into = [flat[:512 * 256].view(512, 256), flat[at:at + 512 * 256].view(512, 256)] + [None] * 4
         with pytest.raises(RuntimeError, match="overlap"):
-            ext.gated_mlp_bwd(dy, x2, *ws, g, u, h, 0, False, True, False, into, [None] * 3,
-                              [torch.float32] * 6)
+            ext.gated_mlp_bwd(dy, x2, *ws, g, u, h, 0, [False] + [True] * 3 + [False] * 3, into, [torch.float32] * 6)
     assert not flat.any()
 
 
@@ -334,6 +333,50 @@ def test_gated_some_gradients_only(M):
     (db,) = torch.autograd.grad(y, [one[5]], dy)
     _, exact = gated_exact(x, w, [None, b[1], None], None, "silu", dy)
     assert rel(db, exact[-1]) < 4 * U[torch.bfloat16]
+
+
+@pytest.mark.parametrize("native", [True, False])
+def test_gated_frozen_parameters_cost_no_gradient_memory(native):
+    x, w, b, _, dy = gated_inputs(64, 1024, 2048, 1024, BF16, True, False)
+    size = w[0].numel()
+    ps = [torch.nn.Parameter(t if native else t.float(), requires_grad=False) for t in w + b]
+
+    def peak(pick):
+        for i, p in enumerate(ps):
+            p.requires_grad_(i in pick)
+        got = torch.autograd.grad(ops.gated_mlp(x, *ps), [ps[i] for i in pick], dy)
+        del got
+        y = ops.gated_mlp(x, *ps)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        at = torch.cuda.memory_allocated()
+        got = torch.autograd.grad(y, [ps[i] for i in pick], dy)
+        torch.cuda.synchronize()
+        return torch.cuda.max_memory_allocated() - at
+
+    each = size * (2 if native else 4)
+    all3 = peak([0, 1, 2])
+    for i in range(3):
+        assert peak([i]) <= all3 - 1.9 * each, i
+
+
+@pytest.mark.parametrize("M,K,H,N", [(40, 100, 72, 64), (3000, 256, 520, 264), (9001, 1024, 1600, 1024)])
+@pytest.mark.parametrize("native", [True, False])
+def test_gated_any_subset_of_gradients(M, K, H, N, native):
+    """Each parameter's gradient by itself and several of them.  Another number of tiles may cut a weight's tokens into
+    other pieces: fp32 sums in another order (1e-5), then the same rounding (half of u where some round apart)."""
+    x, w, b, _, dy = gated_inputs(M, K, H, N, torch.bfloat16, True, False)
+    make = lambda t: t.clone() if native else torch.nn.Parameter(t.float())  # noqa: E731
+    full = [x.clone().requires_grad_()] + [make(t).requires_grad_() for t in w + b]
+    ref = torch.autograd.grad(ops.gated_mlp(*full), full, dy)
+    for pick in [[i] for i in range(7)] + [[1, 3], [2, 3], [0, 5], [3, 6], [1, 2, 4], [0, 2, 3, 6]]:
+        args = [x.clone()] + [make(t) for t in w + b]
+        for i, t in enumerate(args):
+            t.requires_grad_(i in pick)
+        got = torch.autograd.grad(ops.gated_mlp(*args), [args[i] for i in pick], dy)
+        for a, i in zip(got, pick):
+            assert a.dtype == ref[i].dtype
+            assert rel(a, ref[i]) < (0.5 * U[torch.bfloat16] if a.dtype == torch.bfloat16 else 1e-5), (pick, i)
 
 
 def test_gated_refusals():
