@@ -616,7 +616,8 @@ template <typename T, int MODE, int WPR, int NV>
 static cudaError_t launch_bwd(const Params& p, dim3 grid, cudaStream_t s) {
   auto k = bwd_kernel<T, MODE, WPR, NV>;
   const size_t smem = sizeof(float) * ((2 * p.n + 3) & ~3) + (use_ring<MODE, WPR, NV>() ? kRing * 4 * block_threads(WPR) * 16 : 0);
-  if (smem > 48 * 1024) NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (smem + 1024 > 48 * 1024)  // (with the kernel's own at most 768 bytes)
+    NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   k<<<grid, block_threads(WPR), smem, s>>>(p);
   return cudaGetLastError();
 }

@@ -502,6 +502,21 @@ def test_norm_gate_residual_rows_anywhere(S, R, D, dtype, start):
         assert all(torch.equal(a[keep], b[keep]) for a, b in zip(again, outs))
 
 
+@pytest.mark.parametrize("D", [255, 256, 257, 513, 769, 1025, 1537, 2041, 2042, 2048, 2056, 4097, 6096, 6097, 6104, 6144,
+                               6152, 8192, 8193, 12000, 12289, 16383])
+def test_norm_gate_residual_widths_where_the_kernel_changes(D):
+    """At each form's widest and narrowest rows, and where its shared memory passes the default limit."""
+    y, skip, wp, gt, wn, ds, dn = norm_inputs(2, 11, D, torch.bfloat16, "sample", True)
+    leaves = [t.requires_grad_() for t in (y, skip, wp, gt, wn)]
+    outs = ops.norm_gate_residual(*leaves)
+    got = torch.autograd.grad(outs, leaves, [ds, dn])
+    exact, tens, vec = norm_exact(y, skip, wp, gt, wn, 1.0, ds, dn)
+    for a, e in zip(list(outs) + list(got[:2]), exact + list(tens)):
+        assert rel(a, e) < U[torch.bfloat16] + 1e-5
+    for a, (e, terms) in zip(got[2:], vec):
+        assert (a.double() - e).norm() <= 1e-5 * terms.norm()
+
+
 @pytest.mark.parametrize("only", ["stream", "normed"])
 def test_norm_gate_residual_with_one_output_used(only):
     y, skip, wp, gt, wn, ds, dn = norm_inputs(2, 19, 200, torch.bfloat16, "sample", True)
