@@ -508,16 +508,19 @@ std::vector<Tensor> norm_gate_fwd(const Tensor& y, const Tensor& skip, const Ten
   return {stream_out, normed};
 }
 
-// {dy, dskip, dwp, dgate, dwn}: gradients of the vectors in fp32
+// {dy, dskip, dwp, dgate, dwn}: the first two where they are needed, gradients of the vectors in fp32
 std::vector<Tensor> norm_gate_bwd(const OptTensor& ds, const OptTensor& dn, const Tensor& y, const Tensor& skip,
                                   const Tensor& wp, const OptTensor& gate, const OptTensor& wn, double skip_scale,
-                                  double eps) {
+                                  double eps, bool need_dy, bool need_dskip) {
   auto a = norm_args(y, skip, wp, gate, wn, skip_scale, eps);
   check_like(ds, y, "ds");
   check_like(dn, y, "dn");
   const c10::cuda::CUDAGuard guard(y.device());
   const auto f32 = y.options().dtype(at::kFloat);
-  auto dy = torch::empty_like(y), dskip = torch::empty_like(y);
+  if (a.n > nsw::kNormGateSkipWidth) need_dy = need_dskip = true;
+  Tensor dy, dskip;
+  if (need_dy) dy = torch::empty_like(y);
+  if (need_dskip) dskip = torch::empty_like(y);
   const int64_t n = a.n;
   if (y.numel() == 0)
     return {dy, dskip, torch::zeros({n}, f32),  // (a gate of no samples has no address)
@@ -531,8 +534,8 @@ std::vector<Tensor> norm_gate_bwd(const OptTensor& ds, const OptTensor& dn, cons
   if (a.wn) dwn = torch::empty({n}, f32);
   a.ds = opt_ptr(ds);
   a.dn = a.wn ? opt_ptr(dn) : nullptr;
-  a.dy = dy.data_ptr();
-  a.dskip = dskip.data_ptr();
+  a.dy = need_dy ? dy.data_ptr() : nullptr;
+  a.dskip = need_dskip ? dskip.data_ptr() : nullptr;
   a.part = part.data_ptr<float>();
   a.dwp = dwp.data_ptr<float>();
   a.dgate = a.gate ? dgate.data_ptr<float>() : nullptr;
@@ -566,7 +569,7 @@ struct NormGateNode : public torch::autograd::Function<NormGateNode> {
       return i < grad.size() && grad[i].defined() ? OptTensor(grad[i].contiguous()) : OptTensor();
     };
     auto g = norm_gate_bwd(c(0), c(1), v[0], v[1], v[2], o(v[3]), o(v[4]), ctx->saved_data["c"].toDouble(),
-                           ctx->saved_data["eps"].toDouble());
+                           ctx->saved_data["eps"].toDouble(), ctx->needs_input_grad(0), ctx->needs_input_grad(1));
     const int64_t gate = ctx->saved_data["gate"].toInt();
     if (gate == 1) g[3] = g[3].view({-1});
     size_t edge = 0;  // graph edges exist for the inputs that were given, in order

@@ -249,7 +249,7 @@ cudaError_t pad_copy(const PadCopy* v, int count, cudaStream_t s);
 
 // ---- norms with gate and skip connection (norm_gate.cu) ------------------------------------------------
 // Forward: stream = skip_scale skip + gate * rms(y) * wp; normed = rms(stream) * wn (normed and wn null: only
-// the stream).  Backward: dy, dskip from ds and / or dn (null: zero), and dwp, dgate (null: not wanted), dwn
+// the stream).  Backward: dy, dskip (null: not wanted) from ds and / or dn (null: zero), and dwp, dgate (null: not wanted), dwn
 // (null with wn).  Tensors are contiguous [samples, rows, n]; gate of sample i at gate + i gate_stride (null:
 // ones).  part: samples * blocks * 2 * n floats.
 struct NormGateArgs {
@@ -262,6 +262,7 @@ struct NormGateArgs {
   float *part, *dwp, *dgate, *dwn;
 };
 constexpr int kNormGateMaxWidth = 16384;
+constexpr int kNormGateSkipWidth = 8192;  // wider rows: dy and dskip are always written
 int norm_gate_blocks(int64_t samples, int64_t rows, int n, int sms);  // of the backward, per sample
 cudaError_t norm_gate_fwd(const NormGateArgs& a, int sms, cudaStream_t s);
 cudaError_t norm_gate_bwd(const NormGateArgs& a, int blocks, cudaStream_t s);

@@ -403,11 +403,16 @@ __global__ void __launch_bounds__(block_threads(WPR), bwd_blocks(MODE, WPR)) bwd
     else
       load_vec<VEC, GL>(q, v, gl, p.n, none, f);
   };
+  // q null: not wanted.  The predicated form has no branch (20000 x 3000: 215 us; 233 with one); 32 warps a row have no
+  // registers left for a test (3000 x 16384: 519 us; 587 with either).
   const auto store = [&](void* q, int64_t at, int v, const float* f) {
-    if constexpr (kUseRing)
-      grp.store(reinterpret_cast<T*>(q) + at, f);
-    else
-      store_row<T, VEC, GL>(reinterpret_cast<T*>(q) + at, v, gl, p.n, f);
+    if constexpr (kUseRing) {
+      if (q) grp.store(reinterpret_cast<T*>(q) + at, f);
+    } else if constexpr (VEC) {
+      store_row<T, VEC, GL>(reinterpret_cast<T*>(q) + at, v, gl, WPR == 32 || q ? p.n : 0, f);
+    } else {
+      if (WPR == 32 || q) store_row<T, VEC, GL>(reinterpret_cast<T*>(q) + at, v, gl, p.n, f);
+    }
   };
   F2 gw[NV][4], wn[NV][4], aq[NV][4], aw[NV][4];  // gate * wp, wn, and the sums of d yh and dn sh
 #pragma unroll
@@ -736,6 +741,7 @@ static cudaError_t norm_gate_launch(const NormGateArgs& a, bool backward, int bl
                           : a.n % 8 == 0 && (vectors & 15) == 0        ? ng::kVec
                           : a.n >= 8 && ng::span(a.n) <= ng::kRingWidth ? ng::kShift
                                                                        : ng::kScalar;
+  if (backward && a.n > kNormGateSkipWidth && (!a.dy || !a.dskip)) return cudaErrorInvalidValue;
   const bool bf = a.dtype == kBF16;
   if (!backward)
     return bf ? ng::launch_forward<__nv_bfloat16>(p, mode, a.samples, sms, s)

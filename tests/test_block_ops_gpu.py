@@ -532,6 +532,31 @@ def test_norm_gate_residual_with_one_output_used(only):
         assert (a.double() - e).norm() <= 1e-5 * terms.norm()
 
 
+@pytest.mark.parametrize("D", [512, 1001, 3000, 2301, 7001, 9000])
+def test_norm_gate_residual_some_gradients_only(D):
+    """Each input's gradient by itself and several of them are the full call's; what is not asked for takes no
+    memory (in rows of up to 8192)."""
+    y, skip, wp, gt, wn, ds, dn = norm_inputs(2, 500, D, torch.bfloat16, "sample", True)
+
+    def step(pick):
+        args = [t.clone().requires_grad_(i in pick) for i, t in enumerate((y, skip, wp, gt, wn))]
+        outs = ops.norm_gate_residual(*args)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        at = torch.cuda.memory_allocated()
+        got = torch.autograd.grad(outs, [args[i] for i in pick], [ds, dn])
+        return got, torch.cuda.max_memory_allocated() - at
+
+    ref, peak = step(range(5))
+    ref, peak = step(range(5))
+    size = y.numel() * y.element_size()
+    for pick in ([0], [1], [2], [3], [4], [0, 3], [1, 4], [2, 3, 4]):
+        got, used = step(pick)
+        assert all(torch.equal(a, ref[i]) for a, i in zip(got, pick))
+        if D <= 8192:
+            assert used <= peak - 0.99 * size * sum(i not in pick for i in (0, 1)), pick
+
+
 def test_norm_gate_residual_strides_zeros_and_infinities():
     """Non-contiguous inputs; a zero row and a zero branch stay finite; an infinite row spoils itself only."""
     y, skip, wp, gt, wn, _, _ = norm_inputs(2, 12, 136, torch.bfloat16, "sample", True)
