@@ -177,6 +177,51 @@ def test_gated_tail_of_the_gate(M, dtype, act):
         assert ((dx[:, :H].double() - exact).abs() <= (u + 2e-5) * exact.abs() + 1e-6 * d * up).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+def test_gated_many_tokens_of_aligned_widths(dtype, act):
+    """The forms of a full grid: the pair kernel with residual and results by TMA, a wave of whole tiles of the weight
+    gradients and the tiles that are left cut along the tokens (84 tiles for 74 pairs)."""
+    M, K, H, N = 9001, 1024, 1600, 1024
+    x, w, b, res, dy = gated_inputs(M, K, H, N, dtype, True, True)
+    leaves = [t.requires_grad_() for t in [x] + w + b]
+    y = ops.gated_mlp(x, *w, *b, residual=res, activation=act)
+    got = torch.autograd.grad(y, leaves, dy)
+    ey, exact = gated_exact(x, w, b, res, act, dy)
+    assert rel(y, ey) < 2 * U[dtype]
+    for i, (a, e) in enumerate(zip(got, exact)):
+        assert rel(a, e) < 4 * U[dtype], i
+    with torch.no_grad():
+        assert torch.equal(ops.gated_mlp(x, *w, *b, residual=res, activation=act), y)
+
+
+@pytest.mark.parametrize("M", [1, 2, 8, 9, 15, 16, 17])
+@pytest.mark.parametrize("K,H,N", [(64, 72, 64), (1024, 2736, 1024), (1031, 2051, 517), (128, 4096, 24)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gated_few_tokens(M, K, H, N, dtype):
+    """Up to 16 tokens without gradients: one and two groups of eight, whole and partly filled, one and several depth
+    slices; 17 tokens, and any number with gradients: the tiled kernels.  Each token by itself (its 2-norm over the N
+    outputs, of which there may be few: 4 u) and all of them."""
+    x, w, b, res, _ = gated_inputs(M, K, H, N, dtype, True, True)
+    exact = gated_exact(x, w, b, res, "silu")
+    with torch.no_grad():
+        y = ops.gated_mlp(x, *w, *b, residual=res)
+    t = ops.gated_mlp(x.requires_grad_(), *w, *b, residual=res)
+    for out in (y, t):
+        assert rel(out, exact) < 2 * U[dtype]
+        assert ((out.double() - exact).norm(dim=-1) < 4 * U[dtype] * exact.norm(dim=-1)).all()
+
+
+@pytest.mark.parametrize("M", [3, 400])
+def test_gated_large_gates(M):
+    """Gates of 2^60: the sigmoid is 0 or 1, and the values are those of finite arithmetic."""
+    x, w, b, _, _ = gated_inputs(M, 64, 72, 64, BF16, False, False)
+    big = x * 2.0 ** 60
+    y = ops.gated_mlp(big, *w)
+    e = gated_exact(big, w, b, None, "silu")
+    assert torch.isfinite(y).all() and rel(y, e) < 2 * U[BF16]
+
+
 def test_gated_empty():
     x, w, b, res, _ = gated_inputs(3, 64, 128, 64, torch.bfloat16, True, False)
     for grad in (False, True):
