@@ -3,6 +3,7 @@
 // allocator, on the current stream) and the launches.
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -37,7 +38,9 @@ void once_differentiable(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": second derivatives are not implemented (create_graph=True)");
 }
 
-// The kernels read the values alone, and a missing tangent counts as zero
+// The kernels read the values alone, and a missing tangent counts as zero.  (Without a level there are no tangents;
+// the test of each tensor costs 50 ns where it is a view.)
+bool tangents() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
 void no_tangent(const Tensor& t, const char* what) {
   TORCH_CHECK(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what,
               ": forward-mode derivatives are not implemented");
@@ -435,8 +438,10 @@ Tensor gated_mlp(const Tensor& x, const Tensor& wg, const Tensor& wu, const Tens
   TORCH_CHECK_VALUE(!residual || (residual->dim() == x.dim() && residual->size(-1) == wd.size(0) &&
                                   residual->sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1)),
                     "gated_mlp: residual ", residual->sizes(), " is not the output's shape");
-  for (const Tensor* t : {&x, &wg, &wu, &wd}) no_tangent(*t, "gated_mlp");
-  for (const OptTensor* t : {&bg, &bu, &bd, &residual}) no_tangent(*t, "gated_mlp");
+  if (tangents()) {
+    for (const Tensor* t : {&x, &wg, &wu, &wd}) no_tangent(*t, "gated_mlp");
+    for (const OptTensor* t : {&bg, &bu, &bd, &residual}) no_tangent(*t, "gated_mlp");
+  }
   bool grad = false;
   if (at::GradMode::is_enabled()) {
     for (const Tensor* t : {&x, &wg, &wu, &wd}) grad = grad || t->requires_grad();
@@ -593,8 +598,10 @@ std::vector<Tensor> norm_gate(const Tensor& y, const Tensor& skip, const Tensor&
   TORCH_CHECK_VALUE(!gate || ((gate->dim() == 1 || (gate->dim() == 2 && gate->size(0) == y.size(0))) &&
                               gate->size(-1) == n),
                     "norm_gate_residual: gate ", gate->sizes(), " is neither (", n, ",) nor (", y.size(0), ", ", n, ")");
-  for (const Tensor* t : {&y, &skip, &wp}) no_tangent(*t, "norm_gate_residual");
-  for (const OptTensor* t : {&gate, &wn}) no_tangent(*t, "norm_gate_residual");
+  if (tangents()) {
+    for (const Tensor* t : {&y, &skip, &wp}) no_tangent(*t, "norm_gate_residual");
+    for (const OptTensor* t : {&gate, &wn}) no_tangent(*t, "norm_gate_residual");
+  }
   bool grad = false;
   if (at::GradMode::is_enabled()) {
     for (const Tensor* t : {&y, &skip, &wp}) grad = grad || t->requires_grad();
@@ -614,14 +621,17 @@ Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, const std::
   TORCH_CHECK(out.empty() || out.size() == grads.size(), "clip_grad_norm: ", out.size(), " outputs for ",
               grads.size(), " tensors");
   const auto dev = grads[0].device();
+  const bool dual = tangents();
   std::vector<nsw::ClipTensor> v;
   v.reserve(grads.size());
   int64_t total = 0;
   for (size_t i = 0; i < grads.size(); ++i) {
     const Tensor& g = grads[i];
     const Tensor& o = out.empty() ? g : out[i];
-    no_tangent(g, "clip_grad_norm");
-    no_tangent(o, "clip_grad_norm");
+    if (dual) {
+      no_tangent(g, "clip_grad_norm");
+      no_tangent(o, "clip_grad_norm");
+    }
     TORCH_CHECK(g.is_cuda() && g.device() == dev && o.device() == dev, "clip_grad_norm: tensor ", i,
                 " is not on the first one's CUDA device");
     TORCH_CHECK(g.is_contiguous() && o.is_contiguous() && o.numel() == g.numel() &&
