@@ -189,7 +189,7 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float,
                    out: Optional[Sequence[torch.Tensor]] = None) -> torch.Tensor:
     """Scale ``grads`` (separate tensors, fp32 / bf16 / fp16 mixed freely) to a global L2 norm of at most
     ``max_norm``, in place or into ``out``; returns the norm before clipping (an fp32 scalar tensor; nothing
-    waits for the device).  The factor is the trainer's: ``max_norm / (norm + 1e-6)`` where the norm exceeds
+    waits for the device).  On CUDA the tensors are contiguous, and none overlaps what another one writes.  The factor is the trainer's: ``max_norm / (norm + 1e-6)`` where the norm exceeds
     ``max_norm``, else 1 (also for a NaN norm: non-finite gradients stay visible)."""
     if isinstance(grads, torch.Tensor):
         grads = [grads]

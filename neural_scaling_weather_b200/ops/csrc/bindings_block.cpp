@@ -615,6 +615,51 @@ std::vector<Tensor> norm_gate(const Tensor& y, const Tensor& skip, const Tensor&
 }
 
 // ------------------------------------------------------------------------------ clipping
+// The blocks write all tensors at once, so none may be written that another one is read from or written to; a tensor
+// may be its own result.
+void check_separate(const std::vector<nsw::ClipTensor>& v) {
+  if (v.empty()) return;
+  struct Range {
+    uintptr_t begin, end;
+  };
+  const auto range = [](const void* p, const nsw::ClipTensor& t) {
+    const uintptr_t at = reinterpret_cast<uintptr_t>(p);
+    return Range{at, at + (uintptr_t)t.n * (t.dtype == nsw::kF32 ? 4 : 2)};
+  };
+  // the usual list is settled without sorting: results one after the other in memory, and no input among them
+  const uintptr_t first = range(v.front().out, v.front()).begin, last = range(v.back().out, v.back()).end;
+  uintptr_t at = 0;
+  bool plain = true;
+  for (const auto& t : v) {
+    const Range in = range(t.in, t), out = range(t.out, t);
+    plain = plain && out.begin >= at && (t.in == t.out || in.end <= first || in.begin >= last);
+    at = out.end;
+  }
+  if (plain) return;
+  std::vector<Range> read, written;  // (what is scaled in place: only written)
+  read.reserve(v.size());
+  written.reserve(v.size());
+  for (const auto& t : v) {
+    written.push_back(range(t.out, t));
+    if (t.in != t.out) read.push_back(range(t.in, t));
+  }
+  for (auto* r : {&read, &written})
+    std::sort(r->begin(), r->end(), [](const Range& a, const Range& b) { return a.begin < b.begin; });
+  uintptr_t end = 0, read_end = 0;
+  size_t i = 0;
+  bool apart = true;
+  for (const Range& w : written) {
+    apart = apart && w.begin >= end;
+    for (; i < read.size() && read[i].begin < w.begin; ++i) {
+      apart = apart && read[i].begin >= end;
+      read_end = std::max(read_end, read[i].end);
+    }
+    apart = apart && w.begin >= read_end;
+    end = std::max(end, w.end);
+  }
+  TORCH_CHECK(apart && (i == read.size() || read[i].begin >= end), "clip_grad_norm: tensors overlap");
+}
+
 // out[i] = grads[i] * min(1, max_norm / (norm + 1e-6)) (out empty: in place); returns the norm (fp32 scalar)
 Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, const std::vector<Tensor>& out) {
   TORCH_CHECK(!grads.empty(), "clip_grad_norm: no tensors");
@@ -641,6 +686,7 @@ Tensor clip_grads(const std::vector<Tensor>& grads, double max_norm, const std::
     v.push_back({g.data_ptr(), o.data_ptr(), g.numel(), dt_code(g, "clip_grad_norm")});
     total += g.numel();
   }
+  check_separate(v);
   const c10::cuda::CUDAGuard guard(dev);
   const auto f32 = grads[0].options().dtype(at::kFloat);
   if (v.empty()) return torch::zeros({}, f32);

@@ -750,6 +750,22 @@ def test_second_derivatives_are_refused():
         torch.autograd.grad(s, x, dy, create_graph=True)
 
 
+def test_clip_grad_norm_refuses_tensors_that_overlap():
+    """All tensors are scaled at the same time: one that is given twice, or an output on another's input, would be
+    read and written at once."""
+    flat = torch.ones(3000, device=DEV)
+    a, b = flat[:1000], flat[1000:2000]
+    out = torch.empty_like(flat)
+    for grads, outs in [([a, b, a], None), ([a, flat[999:1500]], None), ([a, b], [out[:1000], out[500:1500]]),
+                        ([a, b], [b, out[:1000]]), ([a], [flat[1:1001]]), ([a, b], [b, a]), ([flat, b], [flat, out[:1000]])]:
+        with pytest.raises(RuntimeError, match="overlap"):
+            ops.clip_grad_norm(grads, 0.5, out=outs)
+    assert torch.equal(flat, torch.ones_like(flat))
+    norm = ops.clip_grad_norm([a, a, b], 1e9, out=[out[:1000], out[1000:2000], b])  # read twice, written once
+    assert abs(norm.item() - 3000 ** 0.5) < 1e-3 and torch.equal(out[:2000], flat[:2000])
+    assert not ops.clip_grad_norm([flat[:0], flat[:0]], 1.0)
+
+
 @pytest.mark.parametrize("frozen", [True, False])
 def test_forward_mode_derivatives_are_refused(frozen):
     """Under no_grad or with frozen parameters the output would have no tangent, which counts as zero."""
