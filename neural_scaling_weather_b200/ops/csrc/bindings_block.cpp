@@ -79,7 +79,7 @@ struct Aligner {
   }
 };
 
-OptTensor packed_vec(const OptTensor& t) { return t ? OptTensor(t->contiguous()) : OptTensor(); }
+OptTensor packed_vec(const OptTensor& t) { return !t || t->is_contiguous() ? t : OptTensor(t->contiguous()); }
 const void* opt_ptr(const OptTensor& t) { return t && t->defined() ? t->data_ptr() : nullptr; }
 
 void check_matrix(const Tensor& t, int64_t rows, int64_t cols, const Tensor& like, const char* name) {
