@@ -256,6 +256,16 @@ def bench_block_ops(a):
     leaves = [t.requires_grad_() for t in [x] + w + b]
     ms = timeit(lambda: torch.autograd.grad(ops.gated_mlp(x, *w, *b, residual=res), leaves, dy), a.iters)
     report(f"gated_mlp forward + backward {M}x{K}x{H}", ms, 3 * flops)
+    params = [torch.nn.Parameter(t.detach().float()) for t in w + b]  # as the trainer keeps them
+    for p in params:
+        p.grad = torch.zeros_like(p)
+
+    def masters():
+        with torch.autocast("cuda", dtype=dt):
+            ops.gated_mlp(x, *params, residual=res).backward(dy)
+
+    ms = timeit(masters, a.iters)
+    report(f"gated_mlp forward + backward {M}x{K}x{H}, fp32 parameters, added to .grad", ms, 3 * flops)
     y, skip = (rand(1, M, K).requires_grad_() for _ in range(2))
     vec = [torch.ones(K, device="cuda", requires_grad=True) for _ in range(3)]
     ds, dn = rand(1, M, K), rand(1, M, K)
@@ -264,6 +274,15 @@ def bench_block_ops(a):
     report(f"norm_gate_residual forward {M}x{K}", ms, None, 4 * 2 * M * K)
     ms = timeit(lambda: torch.autograd.grad(ops.norm_gate_residual(y, skip, *vec), [y, skip, *vec], [ds, dn]), a.iters)
     report(f"norm_gate_residual forward + backward {M}x{K}", ms, None, 10 * 2 * M * K)
+    for samples, rows in ((4096, M // 4096), (M, 1)):  # a gate of its own for each sample
+        if rows < 1 or samples > 65535:
+            continue
+        y, skip, ds, dn = (rand(samples, rows, K) for _ in range(4))
+        leaves = [y.requires_grad_(), skip.requires_grad_(), vec[0], torch.ones(samples, K, device="cuda", requires_grad=True),
+                  vec[2]]
+        ms = timeit(lambda: torch.autograd.grad(ops.norm_gate_residual(*leaves), leaves, [ds, dn]), a.iters)
+        report(f"norm_gate_residual forward + backward {samples} samples x {rows} x {K}", ms, None,
+               10 * 2 * samples * rows * K)
     grads = [torch.randn(H, K, device="cuda") for _ in range(60)]
     out = [torch.empty_like(g) for g in grads]
     ms = timeit(lambda: ops.clip_grad_norm(grads, 1.0, out=out), a.iters)

@@ -26,14 +26,16 @@
 //            (du, Wu), into the same accumulator; the weights are again read MN-major as stored.
 //     kDw    the weight gradients dg^T x, du^T x and dy^T h: both operands token-major as they are, MN-major
 //            for the MMA, the depth is the tokens.  See gated_unit for the schedule.
-//   The wide forms are bound by the tensor cores at the clock that the power limit leaves; kDh, which moves 22
-//   bytes per hidden unit and token for 2 K operations, by memory and its epilogue.
+//   The wide forms are bound by the tensor cores at the clock that the power limit leaves, at fewer tokens by the last
+//   wave of 256-row tiles.  kDh reads and writes 8 bytes per hidden unit and token (g, u, dg, du) for 2 N operations:
+//   neither memory (39 % busy) nor the tensor cores (46 %) are full, its epilogue warps wait for their tiles.
 // * split_kernel: the four products of a few hundred rows, depth split over a cluster.  See there.
 // * skinny_kernel: up to 16 tokens, where the time is that of streaming the weights once.  See there.
 //
 // Sums are fp32 in TMEM / registers.  Rounded to 16 bits: g, u (kept for the backward), h, dg, du,
 // because the following products take 16-bit operands; the forward's h is computed from the unrounded
-// g and u.
+// g and u.  The bias gradients are fp32 sums of the rounded dg and du.  In fp16 those values overflow past 65504, as
+// any 16-bit activation does.
 #include <cuda.h>
 
 #include <algorithm>
@@ -599,7 +601,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
             tma_store_2d(&p.out1, bu, (int)nb, (int)row_base);
           }
           if (p.sums) {
-            // the tiles' column sums: lane l adds columns 2 (l % 16), 2 (l % 16) + 1 of the rows of l / 16's parity
+            // the tiles' column sums, of the rounded values that dx and the weights' gradients are made of too (of the
+            // fp32 ones, by shuffles before they are packed: 466 us against 437 at 64800 x 1024 x 2736): lane l adds columns 2 (l % 16), 2 (l % 16) + 1 of the rows of l / 16's parity
             float a[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int k = 0; k < 16; ++k) {
