@@ -300,6 +300,25 @@ def test_gated_gradients_keep_their_own_types():
             assert torch.equal(a, e if i == mixed else e.to(BF16))
 
 
+@pytest.mark.parametrize("M,K,H,N", [(9001, 1024, 1600, 1024), (4003, 515, 1373, 517)])
+def test_gated_in_place_gradients_of_many_tokens(M, K, H, N):
+    """fp32 parameters with an existing ``.grad``: whole tiles add to it in the product's epilogue, cut ones in the
+    kernel that adds their pieces.  Two backwards onto ones: the fp32 sums twice, exact to their roundings (1e-5)."""
+    x, w, b, _, dy = gated_inputs(M, K, H, N, torch.bfloat16, True, False)
+    params = [torch.nn.Parameter(t.float()) for t in w + b]
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        got = torch.autograd.grad(ops.gated_mlp(x, *params), params, dy)
+        for p in params:
+            p.grad = torch.ones_like(p)
+        at = [p.grad.data_ptr() for p in params]
+        for _ in range(2):
+            ops.gated_mlp(x, *params).backward(dy)
+    _, exact = gated_exact(x, w, b, None, "silu", dy)
+    for p, a, e, q in zip(params, got, exact[1:], at):
+        assert p.grad.data_ptr() == q and rel(p.grad, 1 + 2 * a.double()) < 1e-5
+        assert a.dtype == torch.float32 and rel(a, e) < 4 * U[torch.bfloat16]
+
+
 def test_gated_tied_parameters_and_shared_gradient_buffers():
     """One parameter as both projections and one bias for both: their gradients add up in an existing fp32 ``.grad``
     as in separate ones (two fp32 sums in another order).  Buffers that overlap are refused."""
