@@ -164,6 +164,44 @@ def gated_mlp(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, w_down:
     return reference.gated_mlp(x, w_gate, w_up, w_down, b_gate, b_up, b_down, residual, activation)
 
 
+def route_tokens(logits: torch.Tensor, top_k: int, normalize: bool = True):
+    """The router of a block with routed experts: ``(weights, experts, balance)`` from ``logits`` (..., E).
+
+    ``experts`` (..., top_k, int64) are the indices of each token's largest logits, in falling order, of equal ones the
+    lower index first.  ``weights`` (..., top_k, fp32) are a softmax over the chosen logits, or with ``normalize=False``
+    their values in the softmax over all.  ``balance`` (a scalar) is ``E sum_e f_e P_e``, the share of the choices that
+    fell on an expert times its mean probability: 1 where both are even; its gradient is that of the probabilities.
+    A masked expert has the logit -inf; a token whose logits are all -inf has weights of zero.  On CUDA bf16, fp16 or
+    fp32 logits, at most 512 experts and 16 choices.  First derivatives in reverse mode."""
+    if logits.dim() < 1 or not 1 <= top_k <= logits.shape[-1]:
+        raise ValueError(f"route_tokens: top_k {top_k} of logits {tuple(logits.shape)}")
+    if _use_cuda(logits):
+        return fused.route_tokens_cuda(logits, top_k, normalize)
+    return reference.route_tokens(logits, top_k, normalize)
+
+
+def expert_mlp(x: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor, w_gate: torch.Tensor,
+               w_up: torch.Tensor, w_down: torch.Tensor, residual: Optional[torch.Tensor] = None,
+               activation: str = "silu") -> torch.Tensor:
+    """Routed gated feed-forward networks: ``y_t = sum_j weights[t, j] MLP_experts[t, j](x_t) + residual_t`` with
+    ``MLP_e(x) = (act(x Wg_e^T) * (x Wu_e^T)) Wd_e^T``.
+
+    ``x`` (..., K); ``weights`` and ``experts`` (..., k) as :func:`route_tokens` returns them (any integer and floating
+    types; an index outside ``0 .. E - 1`` leaves its assignment out, an index that is there twice counts twice);
+    ``w_gate`` and ``w_up`` (E, H, K), ``w_down`` (E, N, H); ``residual`` (..., N).  ``activation``: ``"silu"`` or
+    ``"gelu"`` (exact).  Gradients of everything but the indices, each in its tensor's type; first derivatives in
+    reverse mode.  Any sizes and strides on CUDA (weights whose rows are not multiples of 16 bytes are copied once a
+    call), at most 512 experts, 16 a token; the hidden values and the experts' outputs are 16-bit there.  The rows are
+    sorted by expert on the device (nothing waits for it) and the products run grouped by expert; calls without
+    gradients of at most 16 assignments read the chosen experts' weights alone."""
+    if activation not in GATED_ACTIVATIONS:
+        raise ValueError(f"expert_mlp: activation {activation!r} is not one of {GATED_ACTIVATIONS}")
+    if _use_cuda(x):
+        return fused.expert_mlp_cuda(x, weights, experts, w_gate, w_up, w_down, residual, activation)
+    fused.check_expert_shapes(x, weights, experts, w_gate, w_up, w_down, residual)
+    return reference.expert_mlp(x, weights, experts, w_gate, w_up, w_down, residual, activation)
+
+
 def norm_gate_residual(y: torch.Tensor, skip: torch.Tensor, w_post: torch.Tensor,
                        gate: Optional[torch.Tensor] = None, w_next: Optional[torch.Tensor] = None,
                        skip_scale: float = 1.0, eps: Optional[float] = None):
@@ -270,6 +308,7 @@ __all__ = [
     "WindowGeometry",
     "clip_grad_norm",
     "compute_dtype",
+    "expert_mlp",
     "extension_available",
     "gated_mlp",
     "head_unpatchify",
@@ -279,6 +318,7 @@ __all__ = [
     "patch_embed",
     "reference",
     "rms_norm",
+    "route_tokens",
     "weighted_se_per_channel",
     "weighted_sse",
     "window_attention",

@@ -1,0 +1,475 @@
+// Routed experts: y_t = sum_j w_tj MLP_e(t,j)(x_t) + residual_t over the experts that a router chose for each token.
+//
+// The products run grouped by expert (gated_mlp.cu, the GROUPED forms of its pair kernel) on rows sorted by expert.
+// Here is what stands around them:
+//   plan     a stable counting sort of the assignments (token t's j-th expert) by expert, each expert's rows padded to
+//            whole 256-row tiles, so that a tile belongs to one expert and needs no bounds within it;
+//   gather   the sorted rows of x; in the backward those of dy times their weights, and with the same read of dy the
+//            weights' gradients, the dot products with the experts' outputs;
+//   combine  a token's rows of the experts' outputs, weighted, plus the residual; in the backward those of dx;
+//   few      the whole network for a few assignments, which reads the chosen experts' weights and nothing else.
+// Padding rows are zeros: the products make zeros of them, and the weights' gradients add zeros.
+// Rounded to 16 bits: the experts' outputs (before their weighted sum in fp32) and, in the backward, the weighted dy,
+// as operands of the next product and because wider ones would double the traffic here; each adds half a step beside
+// the products' own roundings (gated_mlp.cu).
+#include <algorithm>
+
+#include "gated.cuh"
+
+namespace nsw {
+namespace experts {
+
+// ------------------------------------------------------------------------------------------------------- plan
+// A block sorts a chunk of kChunk assignments, each of its warps kChunk / kWarps of them in order, 32 at once; equal
+// experts among the 32 find one another by match_any.
+constexpr int kWarps = 16, kThreads = 32 * kWarps, kChunk = 4096, kWarpChunk = kChunk / kWarps;
+
+__device__ __forceinline__ int expert_at(const ExpertPlan& p, int64_t i) {
+  if (i >= p.count) return -1;
+  const int64_t e = p.experts[i];
+  return e >= 0 && e < p.num_experts ? (int)e : -1;
+}
+
+// count[warp][e] of this block's chunk
+__device__ __forceinline__ void count_chunk(const ExpertPlan& p, int64_t first, int (*count)[kMaxExperts]) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = lane; e < p.num_experts; e += 32) count[warp][e] = 0;
+  __syncwarp();
+#pragma unroll
+  for (int i = 0; i < kWarpChunk; i += 32) {
+    const int e = expert_at(p, first + warp * kWarpChunk + i + lane);
+    const unsigned same = __match_any_sync(0xffffffffu, e);
+    if (e >= 0 && (same & ((1u << lane) - 1)) == 0) count[warp][e] += __popc(same);
+    __syncwarp();
+  }
+}
+
+// rows, tiles and the padding's sources from every expert's number of assignments; one block, thread e has expert e's
+__device__ __forceinline__ void place_experts(const ExpertPlan& p, int count, int* start) {
+  __shared__ int warp_sum[kWarps];
+  const int e = threadIdx.x, warp = e >> 5, lane = e & 31;
+  const int padded = (count + kExpertTile - 1) / kExpertTile * kExpertTile;
+  int upto = padded;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) warp_sum[warp] = upto;
+  __syncthreads();
+  for (int w = 0; w < warp; ++w) upto += warp_sum[w];
+  const int first = upto - padded;
+  if (e < p.num_experts) {
+    start[e] = first;
+    p.rows[e] = first;
+    for (int t = first / kExpertTile; t < upto / kExpertTile; ++t) p.tiles[1 + t] = e;
+    if (e == p.num_experts - 1) {
+      p.rows[e + 1] = upto;
+      p.tiles[0] = upto / kExpertTile;
+    }
+  }
+  // the padding: a warp writes that of 32 experts, one after the other
+  for (int i = 0; i < 32; ++i) {
+    const int at = __shfl_sync(0xffffffffu, first + count, i), end = __shfl_sync(0xffffffffu, upto, i);
+    for (int r = at + lane; r < end; r += 32) p.src_of[r] = -1;
+  }
+  __syncthreads();
+}
+
+// base[e]: the chunk's first row of expert e; count[warp][e] becomes the warp's
+__device__ __forceinline__ void scatter_chunk(const ExpertPlan& p, int64_t first, int (*count)[kMaxExperts],
+                                              const int* base) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int e = threadIdx.x; e < p.num_experts; e += kThreads) {
+    int at = base[e];
+    for (int w = 0; w < kWarps; ++w) {
+      const int c = count[w][e];
+      count[w][e] = at;
+      at += c;
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kWarpChunk; i += 32) {
+    const int64_t a = first + warp * kWarpChunk + i + lane;
+    const int e = expert_at(p, a);
+    const unsigned same = __match_any_sync(0xffffffffu, e), before = same & ((1u << lane) - 1);
+    int row = -1;
+    if (e >= 0) row = count[warp][e] + __popc(before);
+    __syncwarp();
+    if (e >= 0 && before == 0) count[warp][e] += __popc(same);
+    __syncwarp();
+    if (a < p.count) {
+      p.row_of[a] = row;
+      if (row >= 0) p.src_of[row] = (int)a;
+    }
+  }
+}
+
+// one chunk: all of it in one launch
+__global__ void __launch_bounds__(kThreads) plan_one_kernel(const ExpertPlan p) {
+  __shared__ int count[kWarps][kMaxExperts], start[kMaxExperts];
+  count_chunk(p, 0, count);
+  __syncthreads();
+  int n = 0;
+  if (threadIdx.x < p.num_experts)
+    for (int w = 0; w < kWarps; ++w) n += count[w][threadIdx.x];
+  place_experts(p, n, start);
+  scatter_chunk(p, 0, count, start);
+}
+
+__global__ void __launch_bounds__(kThreads) plan_count_kernel(const ExpertPlan p) {
+  __shared__ int count[kWarps][kMaxExperts];
+  count_chunk(p, (int64_t)blockIdx.x * kChunk, count);
+  __syncthreads();
+  if (threadIdx.x >= p.num_experts) return;
+  int n = 0;
+  for (int w = 0; w < kWarps; ++w) n += count[w][threadIdx.x];
+  p.hist[(int64_t)blockIdx.x * p.num_experts + threadIdx.x] = n;
+}
+// hist becomes every chunk's first row of every expert
+__global__ void __launch_bounds__(kThreads) plan_place_kernel(const ExpertPlan p, int chunks) {
+  __shared__ int start[kMaxExperts];
+  const int e = threadIdx.x;
+  int* hist = p.hist + e;
+  // eight chunks' loads leave together: one behind a store that might alias it waits
+  const auto load8 = [&](int c, int* m) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m[i] = c + i < chunks ? hist[(int64_t)(c + i) * p.num_experts] : 0;
+  };
+  int n = 0, m[8];
+  if (e < p.num_experts)
+    for (int c = 0; c < chunks; c += 8) {
+      load8(c, m);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) n += m[i];
+    }
+  place_experts(p, n, start);
+  if (e >= p.num_experts) return;
+  int at = start[e];
+  for (int c = 0; c < chunks; c += 8) {
+    load8(c, m);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      if (c + i < chunks) hist[(int64_t)(c + i) * p.num_experts] = at;
+      at += m[i];
+    }
+  }
+}
+__global__ void __launch_bounds__(kThreads) plan_scatter_kernel(const ExpertPlan p) {
+  __shared__ int count[kWarps][kMaxExperts];
+  count_chunk(p, (int64_t)blockIdx.x * kChunk, count);
+  __syncthreads();
+  scatter_chunk(p, (int64_t)blockIdx.x * kChunk, count, p.hist + (int64_t)blockIdx.x * p.num_experts);
+}
+
+// ------------------------------------------------------------------------------------------- gather and combine
+__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) { return tc::ld_bias(p, dtype, i); }
+__device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v) {
+  if (dtype == kF32)
+    reinterpret_cast<float*>(p)[i] = v;
+  else if (dtype == kBF16)
+    reinterpret_cast<__nv_bfloat16*>(p)[i] = from_f<__nv_bfloat16>(v);
+  else
+    reinterpret_cast<__half*>(p)[i] = from_f<__half>(v);
+}
+// eight elements at p of which `left` are the row's; NC: by the read-only path, which stores do not hold up
+template <bool VEC, bool NC = true>
+__device__ __forceinline__ uint4 row8(const uint16_t* p, int64_t left) {
+  if (VEC && NC) return __ldg(reinterpret_cast<const uint4*>(p));
+  if (VEC) return *reinterpret_cast<const uint4*>(p);
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < left) w[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// A warp takes a row, 16 bytes a lane and step, four steps' loads in flight.  dst's rows are padded to multiples of
+// eight elements and aligned.
+constexpr int kRowWarps = 8;
+template <typename T, bool WEIGHTED, bool VEC>
+__global__ void __launch_bounds__(32 * kRowWarps) gather_kernel(const ExpertPlan plan, const ExpertGather a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t warp = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5), warps = (int64_t)gridDim.x * kRowWarps;
+  const int64_t rows = (int64_t)__ldg(plan.tiles) * kExpertTile;
+  for (int64_t r = warp; r < rows; r += warps) {
+    const int src = __ldg(plan.src_of + r);
+    uint16_t* d = reinterpret_cast<uint16_t*>(a.dst) + r * a.ld_dst;
+    if (src < 0) {
+      for (int64_t c = 8 * lane; c < a.n; c += 256) *reinterpret_cast<uint4*>(d + c) = make_uint4(0, 0, 0, 0);
+      continue;
+    }
+    const uint16_t* p = reinterpret_cast<const uint16_t*>(a.rows) + (int64_t)(src / (int)a.k) * a.ld_rows;
+    if (!WEIGHTED) {
+#pragma unroll 4
+      for (int64_t c = 8 * lane; c < a.n; c += 256) *reinterpret_cast<uint4*>(d + c) = row8<VEC>(p + c, a.n - c);
+    } else {
+      const uint16_t* o = reinterpret_cast<const uint16_t*>(a.other) + r * a.ld_other;
+      const float w = load_any(a.weights, a.weight_dtype, src);
+      float dot = 0.f;
+#pragma unroll 4
+      for (int64_t c = 8 * lane; c < a.n; c += 256) {
+        float f[8], g[8];
+        unpack8<T>(row8<VEC>(p + c, a.n - c), f);
+        if (a.dweights) {
+          unpack8<T>(row8<true>(o + c, 8), g);
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (VEC || c + j < a.n) dot = fmaf(f[j], g[j], dot);
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] *= w;
+        *reinterpret_cast<uint4*>(d + c) = pack8<T>(f);
+      }
+      if (a.dweights) {
+        dot = warp_sum(dot);
+        if (lane == 0) store_any(a.dweights, a.weight_dtype, src, dot);
+      }
+    }
+  }
+  if (WEIGHTED && a.dweights)
+    for (int64_t i = 32 * warp + lane; i < plan.count; i += 32 * warps)
+      if (plan.row_of[i] < 0) store_any(a.dweights, a.weight_dtype, i, 0.f);
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(32 * kRowWarps) combine_kernel(const ExpertCombine a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t warp = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5), warps = (int64_t)gridDim.x * kRowWarps;
+  const int k = (int)a.k;
+  for (int64_t t = warp; t < a.tokens; t += warps) {
+    const uint16_t* res = reinterpret_cast<const uint16_t*>(a.residual) + t * a.ld_res;
+    T* out = reinterpret_cast<T*>(a.out) + t * a.ld_out;
+    // lane i holds the token's i-th row and weight (kMaxChosen <= 32)
+    const int my_row = lane < k ? __ldg(a.row_of + t * k + lane) : -1;
+    const float my_weight = lane < k && a.weights ? load_any(a.weights, a.weight_dtype, t * k + lane) : 1.f;
+#pragma unroll 2
+    for (int64_t c0 = 0; c0 < a.n; c0 += 256) {
+      const int64_t c = c0 + 8 * lane;
+      const bool live = c < a.n;
+      float f[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+      if (a.residual && live) unpack8<T>(row8<VEC>(res + c, a.n - c), f);
+#pragma unroll 2
+      for (int i = 0; i < k; ++i) {
+        const int row = __shfl_sync(0xffffffffu, my_row, i);
+        const float w = __shfl_sync(0xffffffffu, my_weight, i);
+        if (row < 0 || !live) continue;
+        float g[8];
+        unpack8<T>(row8<true>(reinterpret_cast<const uint16_t*>(a.rows) + row * a.ld_rows + c, 8), g);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) f[j] = fmaf(w, g[j], f[j]);
+      }
+      if (!live) continue;
+      if (VEC) {
+        *reinterpret_cast<uint4*>(out + c) = pack8<T>(f);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (c + j < a.n) out[c + j] = from_f<T>(f[j]);
+      }
+    }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ few assignments
+// Bound by reading the chosen experts' weights once.  A warp takes a row of a matrix (of Wg and of Wu at once), 16
+// bytes a lane and step; there are rows enough that all of them are in flight together.
+//   up    block (8 hidden units, assignment s): if s is the first assignment of its expert, h of the expert's every
+//         assignment, four at a time; other blocks end at once.
+//   down  block (8 outputs, token): the weighted sum over the token's experts in one warp's registers; the weights are
+//         on their way to L2 before the wait for the kernel that writes h.
+constexpr int kFewGroup = 4;
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) few_up_kernel(const ExpertFew a) {
+  __shared__ int list[kExpertFewRows];
+  __shared__ int listed;
+  const int lane = threadIdx.x & 31, total = a.tokens * a.k, s = blockIdx.y;
+  const int64_t unit = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t e = a.experts[s];
+  if (e < 0 || e >= a.num_experts) return;
+  if (threadIdx.x < 32) {  // (kExpertFewRows <= 32)
+    const bool same = lane < total && a.experts[lane] == e;
+    const unsigned m = __ballot_sync(0xffffffffu, same);
+    if (same) list[__popc(m & ((1u << lane) - 1))] = lane;
+    if (lane == 0) listed = (m & ((1u << s) - 1)) ? 0 : __popc(m);
+  }
+  __syncthreads();
+  if (listed == 0 || unit >= a.H) return;
+  const uint16_t* wg = reinterpret_cast<const uint16_t*>(a.wg) + (e * a.H + unit) * a.ldwg;
+  const uint16_t* wu = reinterpret_cast<const uint16_t*>(a.wu) + (e * a.H + unit) * a.ldwu;
+  for (int i0 = 0; i0 < listed; i0 += kFewGroup) {
+    float g[kFewGroup], u[kFewGroup];
+    const uint16_t* x[kFewGroup];
+#pragma unroll
+    for (int i = 0; i < kFewGroup; ++i) {
+      g[i] = u[i] = 0.f;
+      x[i] = reinterpret_cast<const uint16_t*>(a.x) + (int64_t)(list[min(i0 + i, listed - 1)] / a.k) * a.ldx;
+    }
+#pragma unroll 4
+    for (int c = 8 * lane; c < a.K; c += 256) {
+      float fg[8], fu[8];
+      unpack8<T>(row8<VEC>(wg + c, a.K - c), fg);
+      unpack8<T>(row8<VEC>(wu + c, a.K - c), fu);
+#pragma unroll
+      for (int i = 0; i < kFewGroup; ++i) {
+        if (i > 0 && i0 + i >= listed) continue;
+        float f[8];
+        unpack8<T>(row8<VEC>(x[i] + c, a.K - c), f);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          g[i] = fmaf(f[j], fg[j], g[i]);
+          u[i] = fmaf(f[j], fu[j], u[i]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < kFewGroup; ++i) {
+      if (i0 + i >= listed) break;
+      g[i] = warp_sum(g[i]);
+      u[i] = warp_sum(u[i]);
+      if (lane == 0)
+        reinterpret_cast<T*>(a.h)[list[i0 + i] * a.ldh + unit] = from_f<T>(tc::act_parts(g[i], a.act).val * u[i]);
+    }
+  }
+}
+
+template <typename T, bool VEC>
+__global__ void __launch_bounds__(256) few_down_kernel(const ExpertFew a) {
+  const int lane = threadIdx.x & 31, t = blockIdx.y;
+  const int64_t n = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (n < a.N)
+    for (int j = 0; j < a.k; ++j) {
+      const int64_t e = a.experts[t * a.k + j];
+      if (e < 0 || e >= a.num_experts) continue;
+      const uint16_t* w = reinterpret_cast<const uint16_t*>(a.wd) + (e * a.N + n) * a.ldwd;
+      for (int c = 64 * lane; c < a.H; c += 2048) asm volatile("prefetch.global.L2 [%0];" ::"l"(w + c));
+    }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  if (n >= a.N) return;
+  float y = 0.f;
+  for (int j = 0; j < a.k; ++j) {
+    const int64_t e = a.experts[t * a.k + j];
+    if (e < 0 || e >= a.num_experts) continue;
+    const uint16_t* w = reinterpret_cast<const uint16_t*>(a.wd) + (e * a.N + n) * a.ldwd;
+    const uint16_t* h = reinterpret_cast<const uint16_t*>(a.h) + (t * a.k + j) * a.ldh;
+    float dot = 0.f;
+#pragma unroll 4
+    for (int c = 8 * lane; c < a.H; c += 256) {
+      float f[8], g[8];
+      unpack8<T>(row8<VEC>(w + c, a.H - c), f);
+      unpack8<T>(row8<VEC, false>(h + c, a.H - c), g);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dot = fmaf(f[i], g[i], dot);
+    }
+    y = fmaf(load_any(a.weights, a.weight_dtype, t * a.k + j), dot, y);
+  }
+  y = warp_sum(y);
+  if (lane == 0) {
+    if (a.residual) y += to_f(reinterpret_cast<const T*>(a.residual)[t * a.ldres + n]);
+    reinterpret_cast<T*>(a.y)[(int64_t)t * a.N + n] = from_f<T>(y);
+  }
+}
+
+template <typename T, bool VEC>
+static cudaError_t launch_few(const ExpertFew& a, cudaStream_t s) {
+  few_up_kernel<T, VEC><<<dim3((a.H + 7) / 8, a.tokens * a.k), 256, 0, s>>>(a);
+  NSW_CUDA_CHECK(cudaGetLastError());
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((a.N + 7) / 8, a.tokens);
+  cfg.blockDim = dim3(256);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, few_down_kernel<T, VEC>, a);
+}
+
+static bool aligned(const void* p, int64_t ld) { return ld % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace experts
+
+int64_t expert_tiles(int64_t count, int64_t experts) {
+  return (count + (kExpertTile - 1) * std::min(count, experts)) / kExpertTile;
+}
+static int64_t plan_chunks(int64_t count) { return (count + experts::kChunk - 1) / experts::kChunk; }
+int64_t expert_plan_hist(int64_t count, int64_t num_experts) {
+  const int64_t chunks = plan_chunks(count);
+  return chunks > 1 ? chunks * num_experts : 0;
+}
+
+cudaError_t expert_plan(const ExpertPlan& p, cudaStream_t s) {
+  if (p.num_experts < 1 || p.num_experts > kMaxExperts || p.count < 1) return cudaErrorInvalidValue;
+  const int chunks = (int)plan_chunks(p.count);
+  if (chunks == 1) {
+    experts::plan_one_kernel<<<1, experts::kThreads, 0, s>>>(p);
+    return cudaGetLastError();
+  }
+  experts::plan_count_kernel<<<chunks, experts::kThreads, 0, s>>>(p);
+  experts::plan_place_kernel<<<1, experts::kThreads, 0, s>>>(p, chunks);
+  experts::plan_scatter_kernel<<<chunks, experts::kThreads, 0, s>>>(p);
+  return cudaGetLastError();
+}
+
+cudaError_t expert_gather(const ExpertGather& a, cudaStream_t s) {
+  const int64_t rows = kExpertTile * expert_tiles(a.plan->count, a.plan->num_experts);
+  const int blocks = (int)std::min<int64_t>((rows + experts::kRowWarps - 1) / experts::kRowWarps, 8 * tc::sm_count());
+  if (!experts::aligned(a.dst, a.ld_dst) || (a.dweights && !experts::aligned(a.other, a.ld_other)))
+    return cudaErrorInvalidValue;
+  const bool vec = experts::aligned(a.rows, a.ld_rows) && a.n % 8 == 0;
+#define NSW_GATHER(T, W, V) \
+  experts::gather_kernel<T, W, V><<<blocks, 32 * experts::kRowWarps, 0, s>>>(*a.plan, a)
+  if (!a.weights) {  // a copy: either 16-bit type
+    if (vec)
+      NSW_GATHER(__half, false, true);
+    else
+      NSW_GATHER(__half, false, false);
+  } else if (a.dtype == kBF16) {
+    if (vec)
+      NSW_GATHER(__nv_bfloat16, true, true);
+    else
+      NSW_GATHER(__nv_bfloat16, true, false);
+  } else {
+    if (vec)
+      NSW_GATHER(__half, true, true);
+    else
+      NSW_GATHER(__half, true, false);
+  }
+#undef NSW_GATHER
+  return cudaGetLastError();
+}
+
+cudaError_t expert_combine(const ExpertCombine& a, cudaStream_t s) {
+  if (!experts::aligned(a.rows, a.ld_rows)) return cudaErrorInvalidValue;
+  const int blocks = (int)std::min<int64_t>((a.tokens + experts::kRowWarps - 1) / experts::kRowWarps, 8 * tc::sm_count());
+  const bool vec = a.n % 8 == 0 && experts::aligned(a.out, a.ld_out) &&
+                   (!a.residual || experts::aligned(a.residual, a.ld_res));
+#define NSW_COMBINE(T, V) experts::combine_kernel<T, V><<<blocks, 32 * experts::kRowWarps, 0, s>>>(a)
+  if (a.dtype == kBF16) {
+    if (vec)
+      NSW_COMBINE(__nv_bfloat16, true);
+    else
+      NSW_COMBINE(__nv_bfloat16, false);
+  } else {
+    if (vec)
+      NSW_COMBINE(__half, true);
+    else
+      NSW_COMBINE(__half, false);
+  }
+#undef NSW_COMBINE
+  return cudaGetLastError();
+}
+
+cudaError_t expert_few(const ExpertFew& a, cudaStream_t s) {
+  if (a.tokens < 1 || a.k < 1 || a.tokens * a.k > kExpertFewRows) return cudaErrorInvalidValue;
+  const bool vec = a.K % 8 == 0 && a.H % 8 == 0 && experts::aligned(a.x, a.ldx) && experts::aligned(a.wg, a.ldwg) &&
+                   experts::aligned(a.wu, a.ldwu) && experts::aligned(a.wd, a.ldwd) && experts::aligned(a.h, a.ldh);
+  if (a.dtype == kBF16)
+    return vec ? experts::launch_few<__nv_bfloat16, true>(a, s) : experts::launch_few<__nv_bfloat16, false>(a, s);
+  return vec ? experts::launch_few<__half, true>(a, s) : experts::launch_few<__half, false>(a, s);
+}
+
+}  // namespace nsw

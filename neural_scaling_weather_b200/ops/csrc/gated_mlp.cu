@@ -41,7 +41,7 @@
 #include <algorithm>
 #include <cstring>
 
-#include "tcgen05.cuh"
+#include "gated.cuh"
 
 namespace nsw {
 namespace tc {
@@ -63,6 +63,16 @@ struct DwSeg {
   int out_f32, accumulate, tma_out;  // tma_out: 16-bit rows that an output map can address
 };
 constexpr int kDwWeights = 3;
+
+// Grouped form (GROUPED, the routed experts of experts.cu): the rows are sorted by expert, each expert's padded with
+// zero rows to whole 256-row tiles, and the weights are stacked, [experts][rows][cols], behind tensor maps of three
+// dimensions, so that a tile past an expert's last row or column reads zeros and not the next expert's.  How many tiles
+// there are, and whose, is read from device memory: the grid is sized by the most there can be.
+struct GroupParams {
+  const int* tiles;  // [0]: row tiles, then the expert of each
+  const int* rows;   // kDw: [experts + 1] first rows of the experts' groups
+  int64_t experts;
+};
 
 struct GatedParams {
   CUtensorMap a0, a1, a2, b0, b1;  // operands (a1 / b1: Wu in kUp, the second half of the depth in kDx)
@@ -88,19 +98,23 @@ struct GatedParams {
   // kDh: column sums of the rounded dg and du over each CTA's 128 rows, [2 m_tiles][2 sums_half] (null: none)
   float* sums;
   int64_t sums_half;
+  GroupParams group;
 };
 
 // A pair's i-th unit of work: a tile and its range of k-blocks.  Every form but kDw: tiles pair, pair + npairs,
 // ...  kDw has few tiles and a long depth, so whole waves of tiles (`direct` of them, a multiple of the
 // pairs) are worked in full, and the depth of the `rem` tiles that are left is cut into `splits` pieces, in
 // piece-major order, whose fp32 partials go to the workspace and are added in piece order by dw_sum_kernel.
-// Pairs that run at one time read the same tokens' slab of both operands from L2.
+// Pairs that run at one time read the same tokens' slab of both operands from L2.  The grouped kDw has a tile for each
+// weight, expert and part of the expert's matrix, in this order, whose depth is the expert's rows (zero for an expert
+// without tokens: the tile is zeros).
 struct GUnit {
   int64_t tile;
   int kb0, kb1;
   int64_t slot;  // partial's index, or -1
+  int expert;
 };
-template <int MODE>
+template <int MODE, bool GROUPED>
 __device__ __forceinline__ bool gated_unit(const GatedParams& p, int64_t num_tiles, int64_t pair, int64_t npairs,
                                            int64_t i, GUnit& u) {
   const int64_t v = pair + i * npairs;
@@ -108,6 +122,21 @@ __device__ __forceinline__ bool gated_unit(const GatedParams& p, int64_t num_til
   u.kb0 = 0;
   u.kb1 = p.kb;
   u.tile = v;
+  u.expert = 0;
+  if (GROUPED) {
+    if (v >= num_tiles) return false;
+    if (MODE == kDw) {
+      const int seg = v < p.seg[0].end ? 0 : v < p.seg[1].end ? 1 : 2;
+      const int64_t t = v - (seg ? p.seg[seg - 1].end : 0), of = (p.seg[seg].M + BM2 - 1) / BM2 * p.seg[seg].n_tiles;
+      u.expert = (int)(t / of);
+      u.tile = v - u.expert * of;  // as if the weight had this expert's tiles alone
+      u.kb0 = __ldg(p.group.rows + u.expert) / BK;
+      u.kb1 = __ldg(p.group.rows + u.expert + 1) / BK;
+    } else {
+      u.expert = __ldg(p.group.tiles + 1 + v / ((p.N + (MODE == kUp ? 128 : 256) - 1) / (MODE == kUp ? 128 : 256)));
+    }
+    return true;
+  }
   if (MODE != kDw || v < p.direct) return v < num_tiles;
   const int64_t w = v - p.direct;
   if (w >= (int64_t)p.rem * p.splits) return false;
@@ -139,47 +168,6 @@ struct SmemG {
   int abort_flag;
 };
 
-// act(g) and act'(g), whose exponential and reciprocal are the hardware approximations (2 ulp); exp(-g) = inf gives
-// sig = 0.  GELU is g Phi(g) with the tail Phi(-a) = exp(-a^2 / 2) H(a), a = |g|, taken as it is for g < 0: as
-// 1 - (1 - tail) it would keep only what fp32 holds beside 1, nothing of it below -5.5.  H(a) = exp(a^2 / 2) Phi(-a),
-// which falls from 1/2 like 1 / a, is a polynomial in t = 1 / (1 + p a) without constant term, fitted to it over
-// 0 <= a <= 13.5 (where the tail leaves fp32's normal numbers) for the smallest largest relative error, 3.7e-6.  With
-// fp32's roundings, act and act' have relative errors below 1e-5 at any g (act' around its zero at -0.75: 1e-6 of
-// one), a fiftieth of fp16's half spacing.
-struct ActParts {
-  float val, slope;
-};
-__device__ __forceinline__ ActParts act_parts(float g, int act) {
-  ActParts r;
-  float e;
-  if (act == 0) {
-    float sig;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-1.44269504088896340736f * g));
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(sig) : "f"(1.0f + e));
-    r.val = g * sig;
-    r.slope = fmaf(r.val, 1.0f - sig, sig);
-  } else {
-    float t;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(t) : "f"(fmaf(fabsf(g), 0.30764427f, 1.0f)));
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e) : "f"(-g * g * 0.72134752044448170368f));
-    float h = fmaf(t, -0.0758030088f, 0.19158072f);
-    h = fmaf(t, h, 0.00538051427f);
-    h = fmaf(t, h, 0.137291841f);
-    h = fmaf(t, h, 0.118551773f);
-    h = fmaf(t, h, 0.122996339f);
-    const float tail = t * h * e;
-    const float cdf = g < 0.f ? tail : 1.0f - tail;
-    r.val = g * cdf;
-    r.slope = fmaf(g, e * 0.39894228040143267794f, cdf);
-  }
-  return r;
-}
-
-__device__ __forceinline__ float ld_bias(const void* p, int dtype, int64_t i) {
-  if (dtype == kF32) return __ldg(reinterpret_cast<const float*>(p) + i);
-  if (dtype == kBF16) return to_f(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-  return to_f(reinterpret_cast<const __half*>(p)[i]);
-}
 // f[j] += bias[nb + j] for the columns below N
 __device__ __forceinline__ void add_bias32(const void* p, int dtype, int64_t nb, int64_t N, float* f) {
   if (nb + 32 <= N && (((reinterpret_cast<uintptr_t>(p)) & 15) == 0)) {
@@ -214,10 +202,6 @@ __device__ __forceinline__ void add_bias32(const void* p, int dtype, int64_t nb,
 
 __device__ __forceinline__ void bulk_wait_read_3() { asm volatile("cp.async.bulk.wait_group.read 3;" ::: "memory"); }
 
-__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
-}
-
 // named barrier that also ANDs a predicate over its threads
 __device__ __forceinline__ bool bar_and(int id, int threads, bool v) {
   uint32_t out;
@@ -232,7 +216,7 @@ __device__ __forceinline__ bool bar_and(int id, int threads, bool v) {
 // this lane's row of a 32 x 32 tile into the warp's next buffer (ring of BUFS), then one TMA store
 template <typename T, int BUFS>
 __device__ __forceinline__ void ring_store(const CUtensorMap* map, const float* f, T (*buf)[32 * kStageRow], int lane,
-                                           int64_t nb, int64_t row_base, uint32_t& ring) {
+                                           int64_t nb, int64_t row_base, uint32_t& ring, int expert = -1) {
   T* b = buf[ring & (BUFS - 1)];
   if (lane == 0) {  // at most BUFS - 1 later stores pending: this buffer's has been read
     if (BUFS == 4)
@@ -245,7 +229,12 @@ __device__ __forceinline__ void ring_store(const CUtensorMap* map, const float* 
   for (int v = 0; v < 4; ++v) *reinterpret_cast<uint4*>(b + stg_off(lane, v)) = pack8<T>(&f[8 * v]);
   asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   __syncwarp();
-  if (lane == 0) tma_store_2d(map, b, (int)nb, (int)row_base);
+  if (lane == 0) {
+    if (expert >= 0)
+      tma_store_3d(map, b, (int)nb, (int)row_base, expert);
+    else
+      tma_store_2d(map, b, (int)nb, (int)row_base);
+  }
   ++ring;
 }
 
@@ -255,8 +244,8 @@ __device__ __forceinline__ void ring_store(const CUtensorMap* map, const float* 
 // store that might alias it waits.
 template <typename T>
 __device__ __forceinline__ void dw_tile_store(const DwSeg& p, float* t, int64_t row_base, int64_t nb, const float* f,
-                                              int lane) {
-  const int64_t col = nb + lane, at = row_base * p.ldd + col;
+                                              int lane, int expert) {
+  const int64_t col = nb + lane, at = (expert * p.M + row_base) * p.ldd + col;
   const int rows = col < p.N ? (int)(p.M - row_base < 32 ? p.M - row_base : 32) : 0;
   if (lane == 0) bulk_wait_read_0();  // an earlier tile may still leave from these buffers
   __syncwarp();
@@ -347,7 +336,7 @@ __global__ void dw_sum_kernel(const float* __restrict__ ws, const __grid_constan
   }
 }
 
-template <typename T, int MODE>
+template <typename T, int MODE, bool GROUPED>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(MODE), 1)
     gated_kernel(const __grid_constant__ GatedParams p, uint32_t idesc, int* err) {
   constexpr bool kMnA = MODE == kDw;                                // A read as stored, M contiguous
@@ -361,7 +350,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
   const int64_t pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
-  const int64_t m_tiles = (p.M + BM2 - 1) / BM2;
+  const int64_t m_tiles = GROUPED && MODE != kDw ? __ldg(p.group.tiles) : (p.M + BM2 - 1) / BM2;
   const int64_t n_tiles = (p.N + kCols - 1) / kCols;
   const int64_t num_tiles = MODE == kDw ? p.direct : m_tiles * n_tiles;
   volatile int* abort_flag = &S.abort_flag;
@@ -402,7 +391,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
       int stage = 0;
       uint32_t phase = 0;
       GUnit un;
-      for (int64_t i = 0; gated_unit<MODE>(p, num_tiles, pair, npairs, i, un) && !*abort_flag; ++i) {
+      for (int64_t i = 0; gated_unit<MODE, GROUPED>(p, num_tiles, pair, npairs, i, un) && !*abort_flag; ++i) {
         int seg = 0;
         int64_t tile = un.tile, nt = n_tiles;
         if (MODE == kDw) dw_place(p, un.tile, seg, tile, nt);
@@ -414,6 +403,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
           const uint32_t fb = full_leader + 8u * stage;
           const bool second = MODE == kDx && kb >= p.kb0;
           const int k0 = (second ? kb - p.kb0 : kb) * BK;
+          const auto load_b = [&](void* dst, const CUtensorMap* m, int c0, int c1) {
+            if (GROUPED && MODE != kDw)
+              tma_load_3d_pair(dst, m, fb, c0, c1, un.expert);
+            else
+              tma_load_2d_pair(dst, m, fb, c0, c1);
+          };
           if (kMnA) {
             const CUtensorMap* ma = seg == 0 ? &p.a0 : seg == 1 ? &p.a1 : &p.a2;
             tma_load_2d_pair(&S.a[stage][0], ma, fb, m0, k0);
@@ -423,10 +418,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
           }
           if (kMnB) {
             const CUtensorMap* mb = second || seg == 2 ? &p.b1 : &p.b0;
-            tma_load_2d_pair(&S.b[stage][0], mb, fb, nb0, k0);
-            tma_load_2d_pair(&S.b[stage][64 * BK], mb, fb, nb0 + 64, k0);
+            load_b(&S.b[stage][0], mb, nb0, k0);
+            load_b(&S.b[stage][64 * BK], mb, nb0 + 64, k0);
           } else {
-            tma_load_2d_pair(S.b[stage], MODE == kUp && rank ? &p.b1 : &p.b0, fb, k0, nb0);
+            load_b(S.b[stage], MODE == kUp && rank ? &p.b1 : &p.b0, k0, nb0);
           }
           if (++stage == GS) {
             stage = 0;
@@ -443,7 +438,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
       int acc = 0;
       uint32_t acc_phase = 0;
       GUnit un;
-      for (int64_t i = 0; gated_unit<MODE>(p, num_tiles, pair, npairs, i, un) && !*abort_flag; ++i) {
+      for (int64_t i = 0; gated_unit<MODE, GROUPED>(p, num_tiles, pair, npairs, i, un) && !*abort_flag; ++i) {
         if (!mbar_wait(&S.tmem_empty[acc], acc_phase ^ 1, abort_flag, err)) break;
         tc_fence_after();
         const uint32_t d_tmem = tmem_base + (uint32_t)(acc * BN2);
@@ -493,7 +488,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
     bool pending = false;  // input tiles issued and not waited for
     bool ok = true;
     GUnit un;
-    for (int64_t i = 0; ok && gated_unit<MODE>(p, num_tiles, pair, npairs, i, un); ++i) {
+    for (int64_t i = 0; ok && gated_unit<MODE, GROUPED>(p, num_tiles, pair, npairs, i, un); ++i) {
       int seg = 0;
       int64_t tile = un.tile, nt = n_tiles;
       if (MODE == kDw) dw_place(p, un.tile, seg, tile, nt);
@@ -645,8 +640,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(64 + 32 * epi_warps(
               __stcg(reinterpret_cast<float4*>(w) + v, make_float4(f[4 * v], f[4 * v + 1], f[4 * v + 2], f[4 * v + 3]));
             continue;
           }
+          if (GROUPED && MODE == kDw && un.kb0 == un.kb1) {  // no product was made
+#pragma unroll
+            for (int j = 0; j < 32; ++j) f[j] = 0.f;
+          }
           if (MODE == kDw && !p.seg[seg].tma_out) {
-            dw_tile_store<T>(p.seg[seg], reinterpret_cast<float*>(buf[0]), row_base, nb, f, lane);
+            dw_tile_store<T>(p.seg[seg], reinterpret_cast<float*>(buf[0]), row_base, nb, f, lane, un.expert);
+            continue;
+          }
+          if (GROUPED && MODE == kDw) {
+            ring_store<T, epi_bufs(MODE)>(seg == 0 ? &p.out0 : seg == 1 ? &p.out1 : &p.out2, f, buf, lane, nb, row_base,
+                                          ring, un.expert);
             continue;
           }
           if (MODE == kDown && p.bias0) add_bias32(p.bias0, p.bias_dtype, nb, p.N, f);
@@ -741,10 +745,10 @@ static int64_t dw_tiles(const GatedDwArgs::Weight& w) {
 }
 
 // launches gated_kernel for `units` tiles of work; `fill` encodes the operands (false: refused)
-template <typename T, int MODE, typename Fill>
+template <typename T, int MODE, bool GROUPED, typename Fill>
 static cudaError_t launch_pairs(int64_t units, int dtype, cudaStream_t s, GatedParams& p, Fill fill) {
   const size_t smem = sizeof(SmemG<T, MODE>) + 1024;
-  auto k = gated_kernel<T, MODE>;
+  auto k = gated_kernel<T, MODE, GROUPED>;
   // on each call: the attribute belongs to the current device, and a runtime call has to make that device's
   // context current on this thread (an autograd thread may not have one yet) before the maps are encoded
   NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -778,16 +782,23 @@ static cudaError_t launch_pairs(int64_t units, int dtype, cudaStream_t s, GatedP
   return cudaGetLastError();
 }
 
-template <typename T, int MODE>
+template <typename T, int MODE, bool GROUPED = false>
 static cudaError_t launch_gated(const GatedArgs& a, cudaStream_t s) {
   constexpr int cols = MODE == kUp ? 128 : 256;
   const int64_t tiles = ((a.M + BM2 - 1) / BM2) * ((a.N + cols - 1) / cols);
   GatedParams p;
-  return launch_pairs<T, MODE>(tiles, a.dtype, s, p, [&]() {
+  return launch_pairs<T, MODE, GROUPED>(tiles, a.dtype, s, p, [&]() {
     constexpr bool mn = MODE == kDh || MODE == kDx;
     bool ok = make_map(&p.a0, a.a0, a.M, a.K, a.lda, BM, a.dtype);
     if (MODE == kDx) ok = ok && make_map(&p.a1, a.a1, a.M, a.K, a.lda, BM, a.dtype);
-    if (mn) {
+    if (GROUPED) {
+      p.group = {a.groups->tiles, a.groups->rows, a.groups->experts};
+      const int64_t e = a.groups->experts, rows = mn ? a.K : a.N, cols_ = mn ? a.N : a.K;
+      const int bc = 64, br = mn ? BK : 128;  // a K-major box is 64 deep, 128 rows; an MN-major one 64 by 64
+      ok = ok && make_map_3d(&p.b0, a.b0, e, rows, cols_, a.ldb0, bc, br, CU_TENSOR_MAP_SWIZZLE_128B, a.dtype);
+      if (MODE == kUp || MODE == kDx)
+        ok = ok && make_map_3d(&p.b1, a.b1, e, rows, cols_, a.ldb1, bc, br, CU_TENSOR_MAP_SWIZZLE_128B, a.dtype);
+    } else if (mn) {
       ok = ok && make_map_mn(&p.b0, a.b0, a.K, a.N, a.ldb0, a.dtype);
       if (MODE == kDx) ok = ok && make_map_mn(&p.b1, a.b1, a.K, a.N, a.ldb1, a.dtype);
     } else {
@@ -830,7 +841,7 @@ static cudaError_t launch_dw(const GatedDwArgs& a, cudaStream_t s) {
   const DwPlan plan = dw_plan(tiles, a.T);
   if (plan.rem > 0 && !a.ws) return cudaErrorInvalidValue;
   GatedParams p;
-  NSW_CUDA_CHECK((launch_pairs<T, kDw>(
+  NSW_CUDA_CHECK((launch_pairs<T, kDw, false>(
       std::max<int64_t>(plan.direct, (int64_t)plan.rem * plan.splits), a.dtype, s, p, [&]() {
         // a weight without tiles has the maps of one with them: valid, and not read through
         const auto with = [&](int i, int j) -> const GatedDwArgs::Weight& {
@@ -865,6 +876,38 @@ static cudaError_t launch_dw(const GatedDwArgs& a, cudaStream_t s) {
   return cudaGetLastError();
 }
 
+// The grouped weight gradients: every expert's matrices, each a product over its own rows
+template <typename T>
+static cudaError_t launch_dw_grouped(const GatedDwArgs& a, cudaStream_t s) {
+  const int64_t e = a.groups->experts;
+  int64_t tiles = 0;
+  for (const auto& w : a.w) tiles += e * dw_tiles(w);
+  GatedParams p;
+  return launch_pairs<T, kDw, true>(tiles, a.dtype, s, p, [&]() {
+    const auto with = [&](int i, int j) -> const GatedDwArgs::Weight& {  // as in launch_dw
+      return a.w[i].D ? a.w[i] : a.w[j].D ? a.w[j] : a.w[3 - i - j];
+    };
+    const GatedDwArgs::Weight w[kDwWeights] = {with(0, 1), with(1, 0), with(2, 0)};
+    bool ok = make_map_mn(&p.a0, w[0].a, a.T, w[0].M, w[0].lda, a.dtype) &&
+              make_map_mn(&p.a1, w[1].a, a.T, w[1].M, w[1].lda, a.dtype) &&
+              make_map_mn(&p.a2, w[2].a, a.T, w[2].M, w[2].lda, a.dtype) &&
+              make_map_mn(&p.b0, w[0].b, a.T, w[0].N, w[0].ldb, a.dtype) &&
+              make_map_mn(&p.b1, w[2].b, a.T, w[2].N, w[2].ldb, a.dtype);
+    CUtensorMap* out[kDwWeights] = {&p.out0, &p.out1, &p.out2};
+    int64_t end = 0;
+    for (int i = 0; i < kDwWeights; ++i) {
+      end += e * dw_tiles(a.w[i]);
+      const bool tma = a.w[i].D && !w[i].out_f32 && w[i].N % 8 == 0 && (reinterpret_cast<uintptr_t>(w[i].D) & 15) == 0;
+      p.seg[i] = {end, (w[i].N + BN2 - 1) / BN2, w[i].M, w[i].N, w[i].N, w[i].D, w[i].out_f32, w[i].accumulate, tma};
+      if (tma)
+        ok = ok && make_map_3d(out[i], w[i].D, e, w[i].M, w[i].N, w[i].N, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B, a.dtype);
+    }
+    p.group = {a.groups->tiles, a.groups->rows, e};
+    p.direct = end;
+    return ok;
+  });
+}
+
 // ============================================================================ split-depth form
 // The same four products where gated_kernel would have too few tiles to fill the device (a few hundred rows,
 // or few output columns with a long depth).  The weights are the MMA's M operand (128 of their rows, in kUp 64
@@ -877,15 +920,6 @@ static cudaError_t launch_dw(const GatedDwArgs& a, cudaStream_t s) {
 // that writes the tokens.
 constexpr int kSplitThreads = 320;  // a multiple of a tile's quads: a thread's columns stay the same
 constexpr int kMaxSlices = 8;  // the largest portable cluster
-
-__device__ __forceinline__ float4 ld_cluster4(uint32_t at) {
-  float4 o;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w)
-               : "r"(at)
-               : "memory");
-  return o;
-}
 
 struct SplitParams {
   CUtensorMap w0, w1, x0, x1;
@@ -1307,6 +1341,7 @@ static SplitPlan plan_split(const GatedArgs& a) {
 
 template <typename T, int MODE>
 static cudaError_t launch_any(const GatedArgs& a, bool dependent, cudaStream_t s) {
+  if (a.groups) return launch_gated<T, MODE, true>(a, s);
   const SplitPlan plan = plan_split(a);
   if (!plan.use) return launch_gated<T, MODE>(a, s);
   switch (plan.ntok) {
@@ -1359,41 +1394,6 @@ struct SkinnyParams {
   int bias_dtype, act;
   int dependent;  // launched as a programmatic dependent of the kernel that writes x
 };
-
-template <typename T>
-__device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1);
-template <>
-__device__ __forceinline__ void mma16816<__nv_bfloat16>(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                        uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma16816<__half>(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                 uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// eight values at p (those below `left` of them, zeros after); NC: through the read-only path
-template <bool VEC, bool NC>
-__device__ __forceinline__ uint4 load8(const uint16_t* p, int left) {
-  if (left <= 0) return make_uint4(0, 0, 0, 0);
-  if (VEC && left >= 8) {
-    if (NC) return __ldg(reinterpret_cast<const uint4*>(p));
-    return *reinterpret_cast<const uint4*>(p);
-  }
-  uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < left) w[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
 
 // (DUAL: two steps' loads in flight and five blocks an SM, so that a projection's many blocks are resident at once;
 // 16 tokens, 2048 x 5464: 13.2 us against 15.9 with four steps and four blocks.  The down projection has few
@@ -1706,6 +1706,7 @@ cudaError_t gated_dw(const GatedDwArgs& a, cudaStream_t s) {
   if (!a.w[0].D && !a.w[1].D && !a.w[2].D) return cudaErrorInvalidValue;
   for (const auto& w : a.w)
     if (w.D && (!w.a || !w.b || w.M <= 0 || w.N <= 0 || (w.accumulate && !w.out_f32))) return cudaErrorInvalidValue;
+  if (a.groups) return a.dtype == kBF16 ? tc::launch_dw_grouped<__nv_bfloat16>(a, s) : tc::launch_dw_grouped<__half>(a, s);
   return a.dtype == kBF16 ? tc::launch_dw<__nv_bfloat16>(a, s) : tc::launch_dw<__half>(a, s);
 }
 

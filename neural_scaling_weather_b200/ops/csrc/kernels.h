@@ -176,6 +176,13 @@ cudaError_t wgrad_tcgen05(const WgradArgs& a, const WgradPlan& plan, cudaStream_
 //   kGatedDh    d = a0 b0 with b0 [K, N]; out0 = d * in1 * act'(in0), out1 = d * act(in0) (in: g, u, ldin;
 //               out0 in rows of ldout, out1 in rows of ldaux)
 //   kGatedDx    out0 = a0 b0 + a1 b1 with b0, b1 [K, N]; rows of out0 of any alignment
+// Products of stacked weights, one matrix an expert (groups set): the rows are whole 256-row tiles of one expert each,
+// the weights [experts][rows][cols] in rows of ldb, M the most rows there can be; no biases, residual or column sums.
+struct GatedGroups {
+  int64_t experts;
+  const int* tiles;  // device: [0] row tiles, then each one's expert
+  const int* rows;   // device: [experts + 1] first rows of the experts' tiles
+};
 enum GatedMode : int { kGatedUp = 0, kGatedDown = 1, kGatedDh = 2, kGatedDx = 3 };
 struct GatedArgs {
   int mode, dtype, act;  // act: 0 SiLU, 1 GELU
@@ -194,6 +201,7 @@ struct GatedArgs {
   // out1 at [sums_half, sums_half + N) (null: none)
   float* sums;
   int64_t sums_half;
+  const GatedGroups* groups;
 };
 int64_t gated_sum_rows(const GatedArgs& a);
 // The three weight gradients, or those of them with a D, in one launch: w[i].D (+)= w[i].a^T w[i].b over T tokens; a [T, M] in rows of lda,
@@ -209,6 +217,7 @@ struct GatedDwArgs {
     int out_f32, accumulate;
   } w[3];
   float* ws;
+  const GatedGroups* groups;  // each D is [experts][M][N], from the experts' own rows; no workspace
 };
 int64_t gated_dw_workspace(const GatedDwArgs& a);
 cudaError_t gated_dw(const GatedDwArgs& a, cudaStream_t s);
@@ -246,6 +255,73 @@ struct PadCopy {
 };
 constexpr int kPadCopies = 5;
 cudaError_t pad_copy(const PadCopy* v, int count, cudaStream_t s);
+
+// ---- routed experts (experts.cu) ------------------------------------------------------------------------
+constexpr int kMaxExperts = 512, kMaxChosen = 16, kExpertTile = 256;
+// Assignments (token t's j-th expert: index t k + j) sorted by expert, in order within an expert; an index outside
+// [0, experts) is left out.  Rows of an expert start at a multiple of kExpertTile.
+struct ExpertPlan {
+  const int64_t* experts;  // [count]
+  int64_t count;
+  int num_experts;
+  int* tiles;   // [1 + expert_tiles(count, num_experts)]: the number of row tiles, then each one's expert
+  int* rows;    // [num_experts + 1]: first row of each expert
+  int* row_of;  // [count]: an assignment's row, -1: none
+  int* src_of;  // [kExpertTile * expert_tiles(..)]: a row's assignment, -1: padding (rows past the last tile: unset)
+  int* hist;    // expert_plan_hist(count, num_experts) integers
+};
+int64_t expert_tiles(int64_t count, int64_t experts);  // the most row tiles there can be
+int64_t expert_plan_hist(int64_t count, int64_t experts);
+cudaError_t expert_plan(const ExpertPlan& p, cudaStream_t s);
+// dst[r] = rows[src_of[r] / k] (zeros for padding), for the rows of all tiles; with weights, times
+// weights[src_of[r]], and dweights[a] (null: none) = <rows[a / k], other[row_of[a]]>, zero where that is -1
+struct ExpertGather {
+  const ExpertPlan* plan;
+  int64_t k, n, ld_rows, ld_dst, ld_other;
+  const void *rows, *weights, *other;
+  void *dst, *dweights;
+  int dtype, weight_dtype;  // of rows, other and dst; of weights and dweights
+};
+cudaError_t expert_gather(const ExpertGather& a, cudaStream_t s);
+// out[t] = residual[t] (null: 0) + sum over j of weights[t k + j] (null: 1) rows[row_of[t k + j]]
+struct ExpertCombine {
+  const int* row_of;
+  int64_t tokens, k, n, ld_rows, ld_res, ld_out;
+  const void *rows, *weights, *residual;
+  void* out;
+  int dtype, weight_dtype;
+};
+cudaError_t expert_combine(const ExpertCombine& a, cudaStream_t s);
+// The whole network for a few tokens (at most kExpertFewRows assignments): h [tokens k][ldh] is workspace
+constexpr int kExpertFewRows = 16;
+struct ExpertFew {
+  const void *x, *wg, *wu, *wd, *weights, *residual;
+  const int64_t* experts;
+  void *h, *y;
+  int64_t ldx, ldwg, ldwu, ldwd, ldh, ldres;  // y is contiguous; weights [num_experts][rows][ld]
+  int tokens, k, num_experts, K, H, N, act, dtype, weight_dtype;
+};
+cudaError_t expert_few(const ExpertFew& a, cudaStream_t s);
+
+// ---- router (route.cu) -------------------------------------------------------------------------------------
+// The top k of each row's logits with their weights, and the balance; partial: route_blocks(..) rows of `experts`
+// floats (sums of probabilities) and as many of counts, in all 2 route_blocks experts 4-byte words.
+struct RouteArgs {
+  const void* logits;  // [tokens] rows of ld
+  int64_t tokens, ld;
+  int experts, k, normalize, dtype;
+  float* weights;     // [tokens, k]
+  int64_t* chosen;    // [tokens, k]
+  float* balance;     // 1
+  float* share;       // [experts]: experts count_e / (tokens k)
+  void* partial;
+  // backward: dlogits (contiguous, in dtype) from dweights and dbalance (null: zero)
+  const float *dweights, *dbalance;
+  void* dlogits;
+};
+int route_blocks(int64_t tokens, int experts, int sms);
+cudaError_t route_fwd(const RouteArgs& a, int blocks, cudaStream_t s);
+cudaError_t route_bwd(const RouteArgs& a, int sms, cudaStream_t s);
 
 // ---- norms with gate and skip connection (norm_gate.cu) ------------------------------------------------
 // Forward: stream = skip_scale skip + gate * rms(y) * wp; normed = rms(stream) * wn (normed and wn null: only

@@ -442,6 +442,120 @@ def gated_mlp_cuda(x, wg, wu, wd, bg, bu, bd, residual, activation):
                                residual, act)
 
 
+# ---------------------------------------------------------------------------- routed experts
+class _Route(torch.autograd.Function):
+    """The router's choice.  It keeps the logits, from which the backward forms the probabilities again (the bytes of
+    reading them), the choice and its weights."""
+
+    @staticmethod
+    def forward(ctx, logits, k, normalize):
+        w, chosen, balance, share = require().route_fwd(logits, k, normalize)
+        ctx.save_for_backward(logits, w, chosen, share)
+        ctx.normalize = normalize
+        ctx.mark_non_differentiable(chosen)
+        ctx.set_materialize_grads(False)
+        return w, chosen, balance
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dw, _, dbalance):
+        if dw is None and dbalance is None:
+            return None, None, None
+        dw, dbalance = (None if t is None else t.float().contiguous() for t in (dw, dbalance))
+        return require().route_bwd(*ctx.saved_tensors, dw, dbalance, ctx.normalize), None, None
+
+
+def route_tokens_cuda(logits, top_k, normalize):
+    _no_tangents("route_tokens", logits)
+    e = logits.shape[-1]
+    z = logits.reshape(-1, e)
+    if z.dtype not in DT:
+        raise TypeError(f"route_tokens: logits of {z.dtype} on CUDA (bf16, fp16 or fp32)")
+    if z.stride(1) != 1:
+        z = z.contiguous()
+    if torch.is_grad_enabled() and z.requires_grad:
+        w, chosen, balance = _Route.apply(z, top_k, normalize)
+    else:
+        w, chosen, balance, _ = require().route_fwd(z, top_k, normalize)
+    if logits.dim() == 2:
+        return w, chosen, balance
+    shape = (*logits.shape[:-1], top_k)
+    return w.view(shape), chosen.view(shape), balance
+
+
+def check_expert_shapes(x, weights, experts, wg, wu, wd, residual):
+    if (wg.dim() != 3 or wu.shape != wg.shape or wd.dim() != 3 or wd.shape[0] != wg.shape[0]
+            or wd.shape[2] != wg.shape[1] or x.dim() < 1 or x.shape[-1] != wg.shape[2]):
+        raise ValueError(f"expert_mlp: x {tuple(x.shape)}, w_gate {tuple(wg.shape)}, w_up {tuple(wu.shape)} "
+                         f"and w_down {tuple(wd.shape)} do not fit together")
+    if weights.shape != experts.shape or weights.dim() != x.dim() or weights.shape[:-1] != x.shape[:-1]:
+        raise ValueError(f"expert_mlp: weights {tuple(weights.shape)} and experts {tuple(experts.shape)} must be "
+                         f"({', '.join(map(str, (*x.shape[:-1], 'k')))})")
+    if experts.dtype.is_floating_point or experts.dtype.is_complex or experts.dtype == torch.bool:
+        raise TypeError(f"expert_mlp: experts are integers, got {experts.dtype}")
+    if residual is not None and residual.shape != x.shape[:-1] + wd.shape[1:2]:
+        raise ValueError(f"expert_mlp: residual {tuple(residual.shape)} is not the output's shape")
+
+
+class _ExpertMLP(torch.autograd.Function):
+    """The routed gated networks.  The forward keeps the sorted input rows, both pre-activations, their gated product
+    and the experts' outputs (16 bits), and the sorting; the weights' gradients go into the optimizer's buffers where
+    possible (``gradsink``)."""
+
+    @staticmethod
+    def forward(ctx, x, weights, experts, residual, act, wg, wu, wd):
+        ext = require()
+        dt = _cdtype(x)
+        K, k, N = x.shape[-1], weights.shape[-1], wd.shape[1]
+        W = [wcache.get(w, dt) for w in (wg, wu, wd)]
+        w2 = _rows(weights, k).contiguous()
+        res = None if residual is None else _rows(residual, N).to(dt)
+        y, *saved = ext.expert_mlp_fwd(_rows(x, K).to(dt), w2, experts, *W, res, act, True)
+        # (the matrices of parameters in the compute type are the parameters: a change before the backward is noticed)
+        ctx.save_for_backward(w2, *saved)
+        ctx.params, ctx.act = (wg, wu, wd), act
+        ctx.x_shape, ctx.x_dtype, ctx.w_shape = x.shape, x.dtype, weights.shape
+        ctx.res_dtype = None if residual is None else residual.dtype
+        if any(ctx.needs_input_grad[5:]):
+            gradsink.use(ctx.params)
+        return y.view(*x.shape[:-1], N)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        w2, xs, g, u, h, ys, plan, *W = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        given = [id(p) for p in ctx.params]  # a tied parameter's shares are added by autograd, as in _GatedMLP
+        into = [gradsink.target(p) if n and given.count(id(p)) == 1 else None for p, n in zip(ctx.params, need[5:])]
+        dx, dw, *out = require().expert_mlp_bwd(
+            _rows(dy, dy.shape[-1]).to(W[0].dtype), w2, ctx.params[0].shape[0], ctx.x_shape[-1], xs, g, u, h, ys, plan,
+            *W, ctx.act, [need[0], need[1], *need[5:]], into, [p.dtype for p in ctx.params])
+        if any(need[5:]):
+            for p, t in zip(ctx.params, into):
+                gradsink.done(p, t is not None)
+        dx = dx.view(ctx.x_shape).to(ctx.x_dtype) if need[0] else None
+        dw = dw.view(ctx.w_shape) if need[1] else None
+        return (dx, dw, None, dy.to(ctx.res_dtype) if need[3] else None, None, *out)
+
+
+def expert_mlp_cuda(x, weights, experts, wg, wu, wd, residual, activation):
+    act = _GATED_ACT[activation]
+    dt = _cdtype(x)
+    check_expert_shapes(x, weights, experts, wg, wu, wd, residual)
+    _no_tangents("expert_mlp", x, weights, wg, wu, wd, residual)
+    if weights.dtype not in DT:
+        weights = weights.float()
+    k, K, N = experts.shape[-1], x.shape[-1], wd.shape[1]
+    chosen = _rows(experts, k).to(torch.int64).contiguous()
+    given = (x, weights, wg, wu, wd, residual)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
+        return _ExpertMLP.apply(x, weights, chosen, residual, act, wg, wu, wd)
+    y, = require().expert_mlp_fwd(_rows(x, K).to(dt), _rows(weights, k).contiguous(), chosen,
+                                  *(wcache.get(w, dt) for w in (wg, wu, wd)),
+                                  None if residual is None else _rows(residual, N).to(dt), act, False)
+    return y.view(*x.shape[:-1], N)
+
+
 # ---------------------------------------------------------------------------- norms, gate, skip
 def norm_gate_residual_cuda(y, skip, w_post, gate, w_next, skip_scale, eps):
     """One native autograd node.  It keeps the branch's output and the skip connection; the backward recomputes

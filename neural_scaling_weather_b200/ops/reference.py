@@ -15,6 +15,8 @@ The CUDA kernels are tested against these functions, and CPU runs use them direc
 
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn.functional as F
 
@@ -57,6 +59,47 @@ def norm_gate_residual(y, skip, w_post, gate=None, w_next=None, skip_scale=1.0, 
     s = skip_scale * skip.float() + branch
     n = None if w_next is None else rms_norm(s, w_next, eps).to(y.dtype)
     return s.to(y.dtype), n
+
+
+def route_tokens(logits, top_k, normalize=True):
+    """``(weights, experts, balance)`` over the last dimension, in fp32 or wider; see :func:`ops.route_tokens`."""
+    e = logits.shape[-1]
+    z = logits.reshape(-1, e)
+    z = z if z.dtype == torch.float64 else z.float()
+    order = torch.sort(z.detach(), dim=1, descending=True, stable=True)  # equal logits: the lower index first
+    chosen = order.indices[:, :top_k]
+
+    def shifted(v):  # exp(v - max), zeros in a row that is -inf throughout
+        m = order.values[:, :1]
+        return torch.exp(v - m.masked_fill(m == -math.inf, 0.0))
+
+    def over(v, total):
+        return v / total.masked_fill(total == 0, 1.0)
+
+    p = shifted(z)
+    p = over(p, p.sum(1, keepdim=True))
+    if normalize:
+        w = shifted(z.gather(1, chosen))
+        w = over(w, w.sum(1, keepdim=True))
+    else:
+        w = p.gather(1, chosen)
+    share = torch.bincount(chosen.reshape(-1), minlength=e).to(z.dtype) * (e / max(chosen.numel(), 1))
+    balance = (share * p.sum(0)).sum() / max(z.shape[0], 1)
+    shape = (*logits.shape[:-1], top_k)
+    return w.reshape(shape), chosen.reshape(shape), balance
+
+
+def expert_mlp(x, weights, experts, w_gate, w_up, w_down, residual=None, activation="silu"):
+    """The sum over a token's experts of its weight times the expert's gated network; see :func:`ops.expert_mlp`."""
+    k = experts.shape[-1]
+    rows, w, chosen = x.reshape(-1, x.shape[-1]), weights.reshape(-1, k), experts.reshape(-1, k)
+    y = x.new_zeros(rows.shape[0], w_down.shape[1])
+    for e in range(w_gate.shape[0]):
+        tok, slot = torch.nonzero(chosen == e, as_tuple=True)
+        out = gated_mlp(rows[tok], w_gate[e], w_up[e], w_down[e], activation=activation)
+        y = y.index_add(0, tok, out * w[tok, slot].unsqueeze(1).to(out.dtype))
+    y = y.reshape(*x.shape[:-1], y.shape[1])
+    return y if residual is None else y + residual
 
 
 def clip_grad_norm(grads, max_norm, out=None):

@@ -15,11 +15,14 @@ CSRC = os.path.join("neural_scaling_weather_b200", "ops", "csrc")
 SOURCES = [
     os.path.join(CSRC, "bindings.cpp"),
     os.path.join(CSRC, "bindings_block.cpp"),
+    os.path.join(CSRC, "bindings_experts.cpp"),
     os.path.join(CSRC, "elementwise.cu"),
     os.path.join(CSRC, "attention.cu"),
     os.path.join(CSRC, "attention_tc.cu"),
     os.path.join(CSRC, "gemm_tcgen05.cu"),
     os.path.join(CSRC, "gated_mlp.cu"),
+    os.path.join(CSRC, "experts.cu"),
+    os.path.join(CSRC, "route.cu"),
     os.path.join(CSRC, "norm_gate.cu"),
     os.path.join(CSRC, "grad_clip.cu"),
     os.path.join(CSRC, "noalloc_rmsnorm.cu"),
