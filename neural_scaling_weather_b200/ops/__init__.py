@@ -246,13 +246,17 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float,
 
 
 def window_attention(qkv: torch.Tensor, q_norm_w: torch.Tensor, k_norm_w: torch.Tensor,
-                     num_heads: int, head_dim: int, geom: WindowGeometry, scale: float):
-    """Shifted-window attention over (B, T, H, W, 3*nh*hd) -> (B, T, H, W, nh*hd)."""
-    if not _use_cuda(qkv):
-        return reference.window_attention(qkv, q_norm_w, k_norm_w, num_heads, head_dim, geom, scale)
-    from .fused import window_attention_cuda
+                     num_heads: int, head_dim: int, geom: WindowGeometry, scale: float,
+                     rel_bias: Optional[torch.Tensor] = None):
+    """Shifted-window attention over (B, T, H, W, 3*nh*hd) -> (B, T, H, W, nh*hd).
 
-    return window_attention_cuda(qkv, q_norm_w, k_norm_w, num_heads, head_dim, geom, scale)
+    ``rel_bias`` (nh, ``geom.num_buckets(T)``), of any float type and strides: a learned bias that is added to the logits by
+    head and displacement of query and key, entry ``geom.relative_buckets(T)[i, j]``; with its gradient.  Entries of -inf
+    mask displacements; a query that has none left is zero."""
+    if not _use_cuda(qkv):
+        fused.check_rel_bias(rel_bias, num_heads, geom, qkv.shape[1])
+        return reference.window_attention(qkv, q_norm_w, k_norm_w, num_heads, head_dim, geom, scale, rel_bias)
+    return fused.window_attention_cuda(qkv, q_norm_w, k_norm_w, num_heads, head_dim, geom, scale, rel_bias)
 
 
 def patch_embed(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor],

@@ -184,11 +184,29 @@ __device__ __forceinline__ void norm_rows(T* s, const float* w, int L, float* rs
   }
 }
 
+// A row's place in the entries of a relative position bias: the entry of query i and key j is at
+// center + off(i) - off(j) (see attention_bias.cu)
+__device__ __forceinline__ int bias_off(const AttnGeom& g, int pitch, int i) {
+  const int wa = g.wh * g.ww, t = i / wa, r = i - t * wa, y = r / g.ww;
+  return (t * (2 * g.wh - 1) + y) * pitch + (r - y * g.ww);
+}
+__device__ __forceinline__ int bias_center(const AttnGeom& g, int pitch) {
+  return 4 + ((g.T - 1) * (2 * g.wh - 1) + g.wh - 1) * pitch + g.ww - 1;
+}
+__device__ __forceinline__ void load_bias(float* tab, short* off, const AttnBias& b, const AttnGeom& g, int h, int L,
+                                          int rows) {
+  for (int i = threadIdx.x; i < b.stride; i += blockDim.x) tab[i] = b.tab[(int64_t)h * b.stride + i];
+  for (int i = threadIdx.x; i < rows; i += blockDim.x) off[i] = i < L ? (short)bias_off(g, b.pitch, i) : 0;
+}
+static size_t bias_bytes(const AttnBias& b, int rows) {  // of tab and off, rounded up
+  return b.tab ? ((size_t)b.stride * 4 + (size_t)rows * 2 + 15) / 16 * 16 : 0;
+}
+
 // ============================================================================= forward
-template <typename T, int HD>
+template <typename T, int HD, bool BIAS>
 __global__ void __launch_bounds__(256, 2) fwd_kernel(const T* __restrict__ qkv, const float* __restrict__ qw,
                                                   const float* __restrict__ kw, T* __restrict__ out,
-                                                  float* __restrict__ lse, AttnGeom g) {
+                                                  float* __restrict__ lse, AttnGeom g, AttnBias bias) {
   constexpr int RS = HD + 8;  // smem row stride (elements); +16 B breaks bank conflicts
   constexpr int KS = HD / 16;
   constexpr int DT = HD / 8;
@@ -203,10 +221,14 @@ __global__ void __launch_bounds__(256, 2) fwd_kernel(const T* __restrict__ qkv, 
   int* sTok = reinterpret_cast<int*>(sV + lk * RS);
   signed char* sLab = reinterpret_cast<signed char*>(sTok + lk);
 
+  float* sTab = reinterpret_cast<float*>(smem + ((lq + 2 * lk) * RS * sizeof(T) + lk * 5 + 15) / 16 * 16);
+  short* sOff = reinterpret_cast<short*>(sTab + (BIAS ? bias.stride : 0));
+
   const int bw = blockIdx.x, h = blockIdx.y;
   const WinPos p = win_pos(g, bw);
   const int64_t C = (int64_t)g.nh * HD;
   const bool mixed = fill_tokens(sTok, sLab, g, p, L, lk);
+  if (BIAS) load_bias(sTab, sOff, bias, g, h, L, lk);
   load_rows<T, HD>(sQ, qkv, g.qkv_stride, 0 * C + (int64_t)h * HD, sTok, L, lq);
   load_rows<T, HD>(sK, qkv, g.qkv_stride, 1 * C + (int64_t)h * HD, sTok, L, lk);
   load_rows<T, HD>(sV, qkv, g.qkv_stride, 2 * C + (int64_t)h * HD, sTok, L, lk);
@@ -232,6 +254,8 @@ __global__ void __launch_bounds__(256, 2) fwd_kernel(const T* __restrict__ qkv, 
     const int r0 = qt * 16 + gq, r1 = r0 + 8;
     const int lab0 = sLab[r0] < 0 ? 0 : sLab[r0];
     const int lab1 = sLab[r1] < 0 ? 0 : sLab[r1];
+    const float* bias0 = sTab + (BIAS ? bias_center(g, bias.pitch) + sOff[r0] : 0);
+    const float* bias1 = sTab + (BIAS ? bias_center(g, bias.pitch) + sOff[r1] : 0);
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
     float o[DT][4];
 #pragma unroll
@@ -254,7 +278,24 @@ __global__ void __launch_bounds__(256, 2) fwd_kernel(const T* __restrict__ qkv, 
         }
       }
       float mx0 = -INFINITY, mx1 = -INFINITY;
-      if (!mixed && kc + 64 <= L) {
+      if (BIAS) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int col = kc + j * 8 + 2 * tq + e;
+            const int lc = sLab[col], at = sOff[col];
+            float v0 = fmaf(s[j][e], sl2, bias0[-at]), v1 = fmaf(s[j][2 + e], sl2, bias1[-at]);
+            if (lc < 0) v0 = v1 = -INFINITY;
+            if (lc != lab0) v0 += ml2;
+            if (lc != lab1) v1 += ml2;
+            s[j][e] = v0;
+            s[j][2 + e] = v1;
+            mx0 = fmaxf(mx0, v0);
+            mx1 = fmaxf(mx1, v1);
+          }
+        }
+      } else if (!mixed && kc + 64 <= L) {
         // no mask and no padding in this chunk (the common case)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -292,10 +333,15 @@ __global__ void __launch_bounds__(256, 2) fwd_kernel(const T* __restrict__ qkv, 
       mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
       mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
       mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-      const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
-      const float c0 = fast_exp2(m0 - mn0), c1 = fast_exp2(m1 - mn1);
+      float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
+      const float old0 = m0, old1 = m1;
       m0 = mn0;
       m1 = mn1;
+      if (BIAS) {  // a row that the bias has masked so far: P = 0
+        if (mn0 == -INFINITY) mn0 = 0.f;
+        if (mn1 == -INFINITY) mn1 = 0.f;
+      }
+      const float c0 = fast_exp2(old0 - mn0), c1 = fast_exp2(old1 - mn1);
       l0 *= c0;
       l1 *= c1;
 #pragma unroll
@@ -336,7 +382,7 @@ __global__ void __launch_bounds__(256, 2) fwd_kernel(const T* __restrict__ qkv, 
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    const float il0 = 1.f / l0, il1 = 1.f / l1;
+    const float il0 = BIAS && l0 == 0.f ? 0.f : 1.f / l0, il1 = BIAS && l1 == 0.f ? 0.f : 1.f / l1;
     // stage the 16 x HD output tile in this warp's own Q rows, then store 16-byte chunks
     __syncwarp();
 #pragma unroll
@@ -347,8 +393,14 @@ __global__ void __launch_bounds__(256, 2) fwd_kernel(const T* __restrict__ qkv, 
     }
     if (tq == 0) {
       const int64_t base = ((int64_t)bw * g.nh + h) * L;
-      if (r0 < L) lse[base + r0] = m0 + log2f(l0);
-      if (r1 < L) lse[base + r1] = m1 + log2f(l1);
+      if (BIAS) {
+        float2* out2 = reinterpret_cast<float2*>(lse) + base;
+        if (r0 < L) out2[r0] = l0 == 0.f ? make_float2(0.f, 0.f) : make_float2(m0, log2f(l0));
+        if (r1 < L) out2[r1] = l1 == 0.f ? make_float2(0.f, 0.f) : make_float2(m1, log2f(l1));
+      } else {
+        if (r0 < L) lse[base + r0] = m0 + log2f(l0);
+        if (r1 < L) lse[base + r1] = m1 + log2f(l1);
+      }
     }
     __syncwarp();
     for (int idx = lane; idx < 16 * DT; idx += 32) {
@@ -431,12 +483,36 @@ __device__ __forceinline__ void store_rows_c(float (*acc)[4], int row0, int lane
   }
 }
 
-template <typename T, int HD>
+__device__ __forceinline__ void add_bucket(float* sums, int at, int pitch, int nx, float v) {  // `at` in rows of pitch
+  const int row = at / pitch;
+  sums[row * nx + at - row * pitch] += v;
+}
+
+// P of one key and two query rows with a bias; `tab` is the key's center in the entries
+__device__ __forceinline__ void biased_probs(float s0, float s1, float sl2, const float* tab, const short* off, int r0, int r1,
+                                             int key_label, int label0, int label1, float m0, float m1, const float* ll,
+                                             float& p0, float& p1) {
+  const float ml2 = -100.f * kLog2e;
+  p0 = p1 = 0.f;
+  if (key_label < 0) return;
+  const float v0 = fmaf(s0, sl2, tab[off[r0]]) + (key_label != (label0 < 0 ? 0 : label0) ? ml2 : 0.f);
+  const float v1 = fmaf(s1, sl2, tab[off[r1]]) + (key_label != (label1 < 0 ? 0 : label1) ? ml2 : 0.f);
+  p0 = fast_exp2((v0 - m0) - ll[r0]);
+  p1 = fast_exp2((v1 - m1) - ll[r1]);
+}
+
+// With a bias's gradient (dbias_part), a third phase forms dS once more and adds it up by bucket.  A bucket's pairs have one
+// difference i - j, so the 16 x 16 blocks on a diagonal of blocks share no bucket with those on the next but one:
+// every second diagonal at once, a warp each, then the others, all into one array and in a fixed order.  A warp turns a
+// block through its tile of shared memory (in T, as dQ's product takes dS) and its lanes walk the block's diagonals.
+constexpr int kBiasTile = 16 * 18;
+template <typename T, int HD, bool BIAS>
 __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, const float* __restrict__ qw,
                                                   const float* __restrict__ kw, const T* __restrict__ out,
                                                   const T* __restrict__ dout, const float* __restrict__ lse,
                                                   T* __restrict__ dqkv, float* __restrict__ dqw_part,
-                                                  float* __restrict__ dkw_part, AttnGeom g) {
+                                                  float* __restrict__ dkw_part, AttnGeom g, AttnBias bias,
+                                                  float* __restrict__ dbias_part) {
   constexpr int RS = HD + 8;
   constexpr int KS = HD / 16;
   constexpr int DT = HD / 8;
@@ -456,17 +532,31 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
   float* sWk = sWq + HD;  // [HD] partial dkw
   int* sTok = reinterpret_cast<int*>(sWk + HD);
   signed char* sLab = reinterpret_cast<signed char*>(sTok + lp);
+  const int buckets = (2 * g.T - 1) * (2 * g.wh - 1) * (2 * g.ww - 1);
+  float* sTab = reinterpret_cast<float*>(smem + ((size_t)4 * lp * RS * sizeof(T) + lp * 21 + 2 * HD * 4 + 15) / 16 * 16);
+  short* sOff = reinterpret_cast<short*>(sTab + (BIAS ? bias.stride : 0));
+  float* sLl = reinterpret_cast<float*>(sOff + (BIAS ? lp : 0));  // BIAS: log2 of a row's sum; sLse its largest logit
+  float* sSum = sLl + (BIAS ? lp : 0);                           // with dbias_part: the buckets, then the warps' tiles
+  const int center = BIAS ? bias_center(g, bias.pitch) : 0;
 
   const int bw = blockIdx.x, h = blockIdx.y;
   const WinPos p = win_pos(g, bw);
   const int64_t C = (int64_t)g.nh * HD;
   const bool mixed = fill_tokens(sTok, sLab, g, p, L, lp);
+  if (BIAS) {
+    load_bias(sTab, sOff, bias, g, h, L, lp);
+    if (dbias_part)
+      for (int i = threadIdx.x; i < buckets; i += blockDim.x) sSum[i] = 0.f;
+  }
   load_rows<T, HD>(sQ, qkv, g.qkv_stride, 0 * C + (int64_t)h * HD, sTok, L, lp);
   load_rows<T, HD>(sK, qkv, g.qkv_stride, 1 * C + (int64_t)h * HD, sTok, L, lp);
   load_rows<T, HD>(sV, qkv, g.qkv_stride, 2 * C + (int64_t)h * HD, sTok, L, lp);
   load_rows<T, HD>(sG, dout, g.out_stride, (int64_t)h * HD, sTok, L, lp);
   const int64_t lse_base = ((int64_t)bw * g.nh + h) * L;
-  for (int i = threadIdx.x; i < lp; i += blockDim.x) sLse[i] = i < L ? lse[lse_base + i] : INFINITY;
+  for (int i = threadIdx.x; i < lp; i += blockDim.x) {
+    sLse[i] = i >= L ? INFINITY : lse[BIAS ? 2 * (lse_base + i) : lse_base + i];
+    if (BIAS) sLl[i] = i < L ? lse[2 * (lse_base + i) + 1] : 0.f;
+  }
   for (int i = threadIdx.x; i < HD; i += blockDim.x) {
     sWq[i] = 0.f;
     sWk[i] = 0.f;
@@ -547,7 +637,14 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
             const float dq = sD[q];
             float v0 = st[j][e] * sl2, v1 = st[j][2 + e] * sl2;
             float p0, p1;
-            if (plain) {
+            if (BIAS) {  // (rows are keys here)
+              const float* b = sTab + center + sOff[q];
+              const int ql = sLab[q];
+              v0 = fmaf(st[j][e], sl2, b[-sOff[kr0]]) + (ql >= 0 && klab0 != ql ? ml2 : 0.f);
+              v1 = fmaf(st[j][2 + e], sl2, b[-sOff[kr1]]) + (ql >= 0 && klab1 != ql ? ml2 : 0.f);
+              p0 = klab0 < 0 ? 0.f : fast_exp2((v0 - lq) - sLl[q]);
+              p1 = klab1 < 0 ? 0.f : fast_exp2((v1 - lq) - sLl[q]);
+            } else if (plain) {
               p0 = fast_exp2(v0 - lq);
               p1 = fast_exp2(v1 - lq);
             } else {
@@ -637,7 +734,11 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
           for (int e = 0; e < 2; ++e) {
             float v0 = s[j][e] * sl2, v1 = s[j][2 + e] * sl2;
             float p0 = 0.f, p1 = 0.f;
-            if (plain) {
+            if (BIAS) {
+              const int k = kc + j * 8 + 2 * tq + e;
+              biased_probs(s[j][e], s[j][2 + e], sl2, sTab + center - sOff[k], sOff, qr0, qr1, sLab[k], qlab0, qlab1, lq0,
+                           lq1, sLl, p0, p1);
+            } else if (plain) {
               p0 = fast_exp2(v0 - lq0);
               p1 = fast_exp2(v1 - lq1);
             } else {
@@ -677,6 +778,79 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
                                  sRq, sTok, L, dqkv, wq);
     }
   }
+  if (BIAS && dbias_part) {
+    // ---------------- phase C: dS by bucket
+    T* tile = reinterpret_cast<T*>(sSum + buckets) + warp * kBiasTile;
+    for (int odd = 0; odd < 2; ++odd) {
+      __syncthreads();
+      // block diagonals d = query block - key block of this parity
+      const int first = ((nt - 1) & 1) == odd ? 1 - nt : 2 - nt;
+      for (int d = first + 2 * warp; d < nt; d += 2 * nw) {
+        for (int kt = max(0, -d); kt < min(nt, nt - d); ++kt) {
+          const int qt = kt + d;
+          float s[2][4], dpm[2][4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[j][e] = dpm[j][e] = 0.f;
+#pragma unroll
+          for (int ks = 0; ks < KS; ++ks) {
+            uint32_t a[4], b0, b1, b2, b3;
+            const int ra = qt * 16 + (lane & 7) + ((lane >> 3) & 1) * 8, ca = ks * 16 + (lane >> 4) * 8;
+            const int rb = kt * 16 + (lane & 7) + (lane >> 4) * 8, cb = ks * 16 + ((lane >> 3) & 1) * 8;
+            ldsm_x4(smem_u32(sQ + ra * RS + ca), a[0], a[1], a[2], a[3]);
+            ldsm_x4(smem_u32(sK + rb * RS + cb), b0, b1, b2, b3);
+            mma16816<T>(s[0], a, b0, b1);
+            mma16816<T>(s[1], a, b2, b3);
+            ldsm_x4(smem_u32(sG + ra * RS + ca), a[0], a[1], a[2], a[3]);
+            ldsm_x4(smem_u32(sV + rb * RS + cb), b0, b1, b2, b3);
+            mma16816<T>(dpm[0], a, b0, b1);
+            mma16816<T>(dpm[1], a, b2, b3);
+          }
+          const int qr0 = qt * 16 + gq, qr1 = qr0 + 8;
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float ds[4];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int k = kt * 16 + j * 8 + 2 * tq + e;
+              float p0, p1;
+              biased_probs(s[j][e], s[j][2 + e], sl2, sTab + center - sOff[k], sOff, qr0, qr1, sLab[k], sLab[qr0],
+                           sLab[qr1], sLse[qr0], sLse[qr1], sLl, p0, p1);
+              ds[e] = p0 * (dpm[j][e] - sD[qr0]);
+              ds[2 + e] = p1 * (dpm[j][2 + e] - sD[qr1]);
+            }
+            *reinterpret_cast<uint32_t*>(tile + gq * 18 + j * 8 + 2 * tq) = pack2<T>(ds[0], ds[1]);
+            *reinterpret_cast<uint32_t*>(tile + (gq + 8) * 18 + j * 8 + 2 * tq) = pack2<T>(ds[2], ds[3]);
+          }
+          __syncwarp();
+          // lane l: the diagonal i - j = l - 15 of the block (lane 31: none); its bucket changes where a row of the
+          // window ends
+          if (lane < 31) {
+            const int shift = lane - 15;
+            int cur = -1;
+            float sum = 0.f;
+            for (int i = max(0, shift); i < min(16, 16 + shift); ++i) {
+              const int qi = qt * 16 + i, kj = kt * 16 + i - shift;
+              if (qi >= L || kj >= L) break;
+              const int at = center - 4 + sOff[qi] - sOff[kj];
+              if (at != cur) {
+                if (cur >= 0) add_bucket(sSum, cur, bias.pitch, 2 * g.ww - 1, sum);
+                cur = at;
+                sum = 0.f;
+              }
+              sum += to_f(tile[i * 18 + i - shift]);
+            }
+            if (cur >= 0) add_bucket(sSum, cur, bias.pitch, 2 * g.ww - 1, sum);
+          }
+          __syncwarp();
+        }
+      }
+    }
+    __syncthreads();
+    float* part = dbias_part + ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * buckets;
+    for (int i = threadIdx.x; i < buckets; i += blockDim.x) part[i] = sSum[i];
+  }
   // reduce the norm-weight partials: over the 8 row groups of the warp, then the CTA
 #pragma unroll
   for (int i = 0; i < 2 * DT; ++i) {
@@ -706,35 +880,41 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
 
 template <typename T, int HD>
 static cudaError_t launch_fwd(const void* qkv, const float* qw, const float* kw, void* out, float* lse,
-                              const AttnGeom& g, cudaStream_t s) {
+                              const AttnGeom& g, cudaStream_t s, const AttnBias& bias) {
   const int L = g.T * g.wh * g.ww;
   const int nqt = (L + 15) / 16;
   const int lk = ((L + 63) / 64) * 64;
-  const size_t smem = (size_t)(nqt * 16 + 2 * lk) * (HD + 8) * sizeof(T) + (size_t)lk * (sizeof(int) + 1);
+  const size_t smem = (size_t)(nqt * 16 + 2 * lk) * (HD + 8) * sizeof(T) + (size_t)lk * (sizeof(int) + 1) +
+                      (bias.tab ? 16 + bias_bytes(bias, lk) : 0);
   int nw = nqt < 8 ? nqt : 8;
   if (nw < 1) nw = 1;
-  auto k = fwd_kernel<T, HD>;
+  auto k = bias.tab ? fwd_kernel<T, HD, true> : fwd_kernel<T, HD, false>;
   NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   dim3 grid(g.B * (g.H / g.wh) * (g.W / g.ww), g.nh);
-  k<<<grid, nw * 32, smem, s>>>((const T*)qkv, qw, kw, (T*)out, lse, g);
+  k<<<grid, nw * 32, smem, s>>>((const T*)qkv, qw, kw, (T*)out, lse, g, bias);
   return cudaGetLastError();
 }
 
 template <typename T, int HD>
 static cudaError_t launch_bwd(const void* qkv, const float* qw, const float* kw, const void* out,
                               const void* dout, const float* lse, void* dqkv, float* dqw_part,
-                              float* dkw_part, const AttnGeom& g, cudaStream_t s) {
+                              float* dkw_part, const AttnGeom& g, cudaStream_t s, const AttnBias& bias,
+                              float* dbias_part) {
   const int L = g.T * g.wh * g.ww;
   const int nt = (L + 15) / 16;
   const int lp = nt * 16;
   const size_t smem = (size_t)4 * lp * (HD + 8) * sizeof(T) + (size_t)4 * lp * sizeof(float) +
-                      2 * HD * sizeof(float) + (size_t)lp * (sizeof(int) + 1);
+                      2 * HD * sizeof(float) + (size_t)lp * (sizeof(int) + 1) +
+                      (bias.tab ? 16 + bias_bytes(bias, lp) + (size_t)lp * sizeof(float) : 0) +
+                      (dbias_part ? (size_t)(2 * g.T - 1) * (2 * g.wh - 1) * (2 * g.ww - 1) * sizeof(float) +
+                                        6 * kBiasTile * sizeof(T)
+                                  : 0);
   int nw = 2 * nt < 6 ? 2 * nt : 6;
-  auto k = bwd_kernel<T, HD>;
+  auto k = bias.tab ? bwd_kernel<T, HD, true> : bwd_kernel<T, HD, false>;
   NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   dim3 grid(g.B * (g.H / g.wh) * (g.W / g.ww), g.nh);
   k<<<grid, nw * 32, smem, s>>>((const T*)qkv, qw, kw, (const T*)out, (const T*)dout, lse, (T*)dqkv,
-                                dqw_part, dkw_part, g);
+                                dqw_part, dkw_part, g, bias, dbias_part);
   return cudaGetLastError();
 }
 
@@ -757,18 +937,19 @@ static cudaError_t launch_bwd(const void* qkv, const float* qw, const float* kw,
   } while (0)
 
 cudaError_t window_attn_fwd(const void* qkv, const float* qw, const float* kw, void* out, float* lse,
-                            const AttnGeom& g, int dtype, cudaStream_t s) {
+                            const AttnGeom& g, int dtype, cudaStream_t s, const AttnBias& bias) {
   const int L = g.T * g.wh * g.ww;
   if (L > 192 || L <= 0 || g.H % g.wh || g.W % g.ww) return cudaErrorInvalidValue;
-  NSW_ATTN_DISPATCH(launch_fwd, qkv, qw, kw, out, lse, g, s);
+  NSW_ATTN_DISPATCH(launch_fwd, qkv, qw, kw, out, lse, g, s, bias);
 }
 
 cudaError_t window_attn_bwd(const void* qkv, const float* qw, const float* kw, const void* out,
                             const void* dout, const float* lse, void* dqkv, float* dqw_part,
-                            float* dkw_part, const AttnGeom& g, int dtype, cudaStream_t s) {
+                            float* dkw_part, const AttnGeom& g, int dtype, cudaStream_t s, const AttnBias& bias,
+                            float* dbias_part) {
   const int L = g.T * g.wh * g.ww;
   if (L > 192 || L <= 0 || g.H % g.wh || g.W % g.ww) return cudaErrorInvalidValue;
-  NSW_ATTN_DISPATCH(launch_bwd, qkv, qw, kw, out, dout, lse, dqkv, dqw_part, dkw_part, g, s);
+  NSW_ATTN_DISPATCH(launch_bwd, qkv, qw, kw, out, dout, lse, dqkv, dqw_part, dkw_part, g, s, bias, dbias_part);
 }
 
 }  // namespace nsw

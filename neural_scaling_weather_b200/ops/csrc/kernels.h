@@ -72,15 +72,35 @@ struct AttnGeom {
   int64_t qkv_stride;  // elements between consecutive tokens in qkv (3*nh*hd)
   int64_t out_stride;  // elements between tokens in out / dout (nh*hd)
 };
+// Learned bias of the logits by head and displacement of query and key (tab null: none), as attn_bias_prepare leaves it:
+// for each head a row of `stride` floats, the first four a header ([0]: largest less smallest entry), then entry
+// (dt (2 wh - 1) + dy) pitch + dx, in units of log2 and less the head's largest one (a softmax does not see it).
+struct AttnBias {
+  const float* tab;
+  int stride, pitch;
+};
+constexpr int kAttnBiasRow = 1160;  // floats of a row: at most (2 T - 1)(2 wh - 1)(2 ww - 1) = 1155 of 192 tokens
+AttnBias attn_bias_layout(const AttnGeom& g);
+// table (nh, (2 T - 1)(2 wh - 1)(2 ww - 1)) of any strides and type -> b.stride floats a head
+cudaError_t attn_bias_prepare(const void* table, int dtype, int64_t s0, int64_t s1, const AttnGeom& g,
+                              const AttnBias& b, float* tab, cudaStream_t s);
+// With a bias the forward writes two floats a row, (largest logit, log2 of the sum of exponentials less it), and the
+// backward reads them: their sum, the log-sum-exp, would lose the second where a row's logits are far from zero.
+// dbias_part: rows of partial sums of the bias's gradient (null: not wanted), attn_bias_rows(..) of them; sums in
+// units of `unit` (dS is scaled before it is rounded), reduced by attn_bias_grad into out[head, bucket].
+int64_t attn_bias_rows(const AttnGeom& g, bool tc, int sms);
+cudaError_t attn_bias_grad(const float* part, const AttnGeom& g, bool tc, int sms, void* out, int dtype, bool accumulate,
+                           cudaStream_t s);
 cudaError_t window_attn_fwd(const void* qkv, const float* qw, const float* kw, void* out, float* lse,
-                            const AttnGeom& g, int dtype, cudaStream_t s);
+                            const AttnGeom& g, int dtype, cudaStream_t s, const AttnBias& bias = {});
 // tcgen05/TMEM forward (bf16, head_dim 64, T*wh*ww <= 176); same outputs as window_attn_fwd
 bool window_attn_fwd_tc_supported(const AttnGeom& g, int dtype);
 cudaError_t window_attn_fwd_tc(const void* qkv, const float* qw, const float* kw, void* out, float* lse,
                                const AttnGeom& g, cudaStream_t s);
 // warp-specialised tcgen05 forward (same contract and support as window_attn_fwd_tc)
 cudaError_t window_attn_fwd_ws(const void* qkv, const float* qw, const float* kw, void* out, float* lse,
-                               const AttnGeom& g, cudaStream_t s, long long* stamps = nullptr);
+                               const AttnGeom& g, cudaStream_t s, long long* stamps = nullptr,
+                               const AttnBias& bias = {});
 // RMSNorm, one warp per row with the row in registers (n <= 2048); rmsnorm_fwd/bwd use the TMA
 // version below where it applies and these otherwise
 cudaError_t rmsnorm_fwd_rows(const void* x, const float* w, void* y, float* rstd, int64_t rows, int n,
@@ -99,10 +119,12 @@ cudaError_t rmsnorm_bwd_tma(const void* dy, const void* x, const float* w, const
 // dqw_part / dkw_part: one row of head_dim partial sums per CTA, min(items, SM count) rows
 cudaError_t window_attn_bwd_tc(const void* qkv, const float* qw, const float* kw, const void* out,
                                const void* dout, const float* lse, void* dqkv, float* dqw_part, float* dkw_part,
-                               const AttnGeom& g, cudaStream_t s, long long* stamps = nullptr);
+                               const AttnGeom& g, cudaStream_t s, long long* stamps = nullptr,
+                               const AttnBias& bias = {}, float* dbias_part = nullptr);
 cudaError_t window_attn_bwd(const void* qkv, const float* qw, const float* kw, const void* out,
                             const void* dout, const float* lse, void* dqkv, float* dqw_part,
-                            float* dkw_part, const AttnGeom& g, int dtype, cudaStream_t s);
+                            float* dkw_part, const AttnGeom& g, int dtype, cudaStream_t s,
+                            const AttnBias& bias = {}, float* dbias_part = nullptr);
 
 // ---- tcgen05 GEMM ----------------------------------------------------------------
 struct GemmArgs {

@@ -579,41 +579,68 @@ ATTN_FWD_IMPL = int(os.environ.get("NSW_ATTN_FWD_IMPL", "0"))
 
 class _WindowAttn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, qw, kw, gi, scale):
+    def forward(ctx, qkv, qw, kw, gi, scale, rel_bias):
         ext = require()
         qkv2 = qkv.contiguous()
-        out, lse = ext.window_attn_fwd(qkv2, qw.detach().float().contiguous(),
-                                       kw.detach().float().contiguous(), gi, scale, ATTN_FWD_IMPL)
-        ctx.save_for_backward(qkv2, qw, kw, out, lse)
-        ctx.gi, ctx.scale = gi, scale
+        out, lse, *tab = ext.window_attn_fwd(qkv2, qw.detach().float().contiguous(),
+                                             kw.detach().float().contiguous(), gi, scale, ATTN_FWD_IMPL,
+                                             rel_bias=_bias_table(rel_bias))
+        ctx.save_for_backward(qkv2, qw, kw, out, lse, *tab)
+        ctx.gi, ctx.scale, ctx.rel_bias = gi, scale, rel_bias
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             gradsink.use([qw, kw])
+        if ctx.needs_input_grad[5]:
+            gradsink.use([rel_bias])
         return out
 
     @staticmethod
     def backward(ctx, dout):
         ext = require()
-        qkv, qw, kw, out, lse = ctx.saved_tensors
+        qkv, qw, kw, out, lse, *tab = ctx.saved_tensors
         # QK-norm weight gradients straight into the optimizer's gradient buffer where possible
         tq, tk = gradsink.target(qw), gradsink.target(kw)
         inplace = tq is not None and tk is not None
+        # the bias's gradient likewise, or a tensor of its type
+        dbias = tb = None
+        if ctx.needs_input_grad[5]:
+            bias = ctx.rel_bias
+            tb = gradsink.target(bias)
+            dbias = torch.empty(bias.shape, device=bias.device,
+                                dtype=bias.dtype if bias.dtype in DT else torch.float32) if tb is None else tb
         dqkv, dqw, dkw = ext.window_attn_bwd(qkv, qw.detach().float().contiguous(),
                                              kw.detach().float().contiguous(), out,
                                              dout.to(qkv.dtype).contiguous(), lse, ctx.gi, ctx.scale,
-                                             dqw_into=tq if inplace else None, dkw_into=tk if inplace else None)
+                                             dqw_into=tq if inplace else None, dkw_into=tk if inplace else None,
+                                             tab=tab[0] if tab else None, dbias=dbias, dbias_add=tb is not None)
+        if dbias is not None:
+            gradsink.done(ctx.rel_bias, tb is not None)
+            dbias = None if tb is not None else dbias.to(ctx.rel_bias.dtype)
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             gradsink.done(qw, inplace)
             gradsink.done(kw, inplace)
         if inplace:
-            return dqkv, None, None, None, None
-        return dqkv, dqw.to(qw.dtype), dkw.to(kw.dtype), None, None
+            return dqkv, None, None, None, None, dbias
+        return dqkv, dqw.to(qw.dtype), dkw.to(kw.dtype), None, None, dbias
 
 
-def window_attention_cuda(qkv, q_norm_w, k_norm_w, num_heads, head_dim, geom: WindowGeometry, scale):
+def _bias_table(rel_bias):
+    if rel_bias is None:
+        return None
+    return rel_bias.detach() if rel_bias.dtype in DT else rel_bias.detach().float()
+
+
+def check_rel_bias(rel_bias, num_heads, geom: WindowGeometry, steps):
+    if rel_bias is not None and rel_bias.shape != (num_heads, geom.num_buckets(steps)):
+        raise ValueError(f"window_attention: rel_bias {tuple(rel_bias.shape)} is not ({num_heads}, "
+                         f"{geom.num_buckets(steps)}) of {steps} x {geom.window[0]} x {geom.window[1]} tokens")
+
+
+def window_attention_cuda(qkv, q_norm_w, k_norm_w, num_heads, head_dim, geom: WindowGeometry, scale, rel_bias=None):
     B, T, H, W, C3 = qkv.shape
     dt = _cdtype(qkv)
     gi = _geom_ints(B, T, H, W, num_heads, head_dim, geom)
-    out = _WindowAttn.apply(qkv.to(dt), q_norm_w, k_norm_w, gi, float(scale))
+    check_rel_bias(rel_bias, num_heads, geom, T)
+    out = _WindowAttn.apply(qkv.to(dt), q_norm_w, k_norm_w, gi, float(scale), rel_bias)
     return out.view(B, T, H, W, num_heads * head_dim)
 
 

@@ -152,8 +152,8 @@ def window_reverse(x: torch.Tensor, window, B, T, H, W):
 
 
 def window_attention(qkv, q_norm_w, k_norm_w, num_heads, head_dim, geom: WindowGeometry,
-                     scale: float):
-    """qkv: (B, T, H, W, 3*nh*hd) -> (B, T, H, W, nh*hd)."""
+                     scale: float, rel_bias=None):
+    """qkv: (B, T, H, W, 3*nh*hd) -> (B, T, H, W, nh*hd); rel_bias (nh, buckets) is added to the logits."""
     B, T, H, W, _ = qkv.shape
     sh, sw = geom.shift
     x = qkv
@@ -166,12 +166,18 @@ def window_attention(qkv, q_norm_w, k_norm_w, num_heads, head_dim, geom: WindowG
     q = rms_norm(q, q_norm_w)
     k = rms_norm(k, k_norm_w)
     s = torch.matmul(q.float(), k.float().transpose(-1, -2)) * scale
+    if rel_bias is not None:
+        s = s + rel_bias.float()[:, geom.relative_buckets(T).to(rel_bias.device)]
     if geom.mask:
         m = window_mask(geom, H, W, T, qkv.device, torch.float32)  # (nW, L, L)
         nW = m.shape[0]
         s = s.view(Bw // nW, nW, num_heads, L, L) + m.view(1, nW, 1, L, L)
         s = s.view(Bw, num_heads, L, L)
-    p = torch.softmax(s, dim=-1)
+    if rel_bias is not None:  # a row that the bias masks throughout is zero
+        none = (s == -math.inf).all(-1, keepdim=True)
+        p = torch.softmax(s.masked_fill(none, 0.0), dim=-1).masked_fill(none, 0.0)
+    else:
+        p = torch.softmax(s, dim=-1)
     o = torch.matmul(p.to(v.dtype), v)  # Bw, nh, L, hd
     o = o.transpose(1, 2).reshape(Bw, L, num_heads * head_dim)
     o = window_reverse(o, geom.window, B, T, H, W)

@@ -19,6 +19,7 @@ SOURCES = [
     os.path.join(CSRC, "elementwise.cu"),
     os.path.join(CSRC, "attention.cu"),
     os.path.join(CSRC, "attention_tc.cu"),
+    os.path.join(CSRC, "attention_bias.cu"),
     os.path.join(CSRC, "gemm_tcgen05.cu"),
     os.path.join(CSRC, "gated_mlp.cu"),
     os.path.join(CSRC, "experts.cu"),
