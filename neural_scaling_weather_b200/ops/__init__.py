@@ -176,7 +176,9 @@ def route_tokens(logits: torch.Tensor, top_k: int, normalize: bool = True):
     if logits.dim() < 1 or not 1 <= top_k <= logits.shape[-1]:
         raise ValueError(f"route_tokens: top_k {top_k} of logits {tuple(logits.shape)}")
     if _use_cuda(logits):
-        return fused.route_tokens_cuda(logits, top_k, normalize)
+        if logits.dtype not in fused.DT:
+            raise TypeError(f"route_tokens: logits of {logits.dtype} on CUDA (bf16, fp16 or fp32)")
+        return require_extension().route_tokens(logits, top_k, normalize)
     return reference.route_tokens(logits, top_k, normalize)
 
 
@@ -198,6 +200,7 @@ def expert_mlp(x: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor, w_
         raise ValueError(f"expert_mlp: activation {activation!r} is not one of {GATED_ACTIVATIONS}")
     if _use_cuda(x):
         return fused.expert_mlp_cuda(x, weights, experts, w_gate, w_up, w_down, residual, activation)
+    fused.check_expert_ids(experts)
     fused.check_expert_shapes(x, weights, experts, w_gate, w_up, w_down, residual)
     return reference.expert_mlp(x, weights, experts, w_gate, w_up, w_down, residual, activation)
 

@@ -682,46 +682,16 @@ nsw::AttnGeom make_geom(const std::vector<int64_t>& gi, double scale) {
   return g;
 }
 
-// The bias's entries as attn_bias_prepare left them, with the layout of this geometry
-nsw::AttnBias bias_of(const nsw::AttnGeom& g, const c10::optional<Tensor>& tab) {
-  if (!tab) return {};
-  nsw::AttnBias b = nsw::attn_bias_layout(g);
-  TORCH_CHECK(tab->is_cuda() && tab->scalar_type() == at::kFloat && tab->is_contiguous() &&
-                  tab->numel() == (int64_t)g.nh * b.stride,
-              "window_attention: the bias's entries are not this geometry's");
-  b.tab = tab->data_ptr<float>();
-  return b;
-}
-
-// rel_bias (heads, buckets), any strides: {out, lse} or {out, lse, tab}, lse with two values a row and tab what the
-// backward takes
 std::vector<Tensor> window_attn_fwd(Tensor qkv, Tensor qw, Tensor kw, std::vector<int64_t> gi, double scale,
-                                    int64_t impl, c10::optional<Tensor> stamps, c10::optional<Tensor> rel_bias) {
+                                    int64_t impl, c10::optional<Tensor> stamps) {
   need_cuda(qkv, "qkv");
-  const c10::cuda::CUDAGuard guard(qkv.device());
   auto g = make_geom(gi, scale);
   const int64_t tokens = (int64_t)g.B * g.T * g.H * g.W;
   TORCH_CHECK(qkv.numel() == tokens * g.qkv_stride, "qkv size");
   auto out = torch::empty({tokens, (int64_t)g.nh * g.hd}, qkv.options());
   const int L = g.T * g.wh * g.ww;
   const int64_t nwin = (int64_t)g.B * (g.H / g.wh) * (g.W / g.ww);
-  auto lse = torch::empty({nwin * g.nh * L * (rel_bias ? 2 : 1)}, qkv.options().dtype(at::kFloat));
-  nsw::AttnBias bias{};
-  c10::optional<Tensor> tab;
-  if (rel_bias) {
-    const int64_t buckets = (int64_t)(2 * g.T - 1) * (2 * g.wh - 1) * (2 * g.ww - 1);
-    TORCH_CHECK_VALUE(L <= 192, "window_attention: windows of ", L, " tokens (at most 192)");
-    TORCH_CHECK_VALUE(rel_bias->dim() == 2 && rel_bias->size(0) == g.nh && rel_bias->size(1) == buckets,
-                      "window_attention: rel_bias must be [", g.nh, ", ", buckets, "], got ", rel_bias->sizes());
-    TORCH_CHECK(rel_bias->device() == qkv.device(), "window_attention: rel_bias must be on the input's device");
-    TORCH_CHECK(impl != 2, "window_attention: impl 2 takes no bias");
-    bias = nsw::attn_bias_layout(g);
-    tab = torch::empty({g.nh, bias.stride}, qkv.options().dtype(at::kFloat));
-    check(nsw::attn_bias_prepare(rel_bias->data_ptr(), dt_code(*rel_bias), rel_bias->stride(0), rel_bias->stride(1), g,
-                                 bias, tab->data_ptr<float>(), stream()),
-          "attn_bias_prepare");
-    bias.tab = tab->data_ptr<float>();
-  }
+  auto lse = torch::empty({nwin * g.nh * L}, qkv.options().dtype(at::kFloat));
   // impl: 0 = default (the warp-specialised tcgen05 kernel where it applies, else mma.sync),
   // 1 = mma.sync, 2 = persistent tcgen05 (every warp in every phase), 3 = warp-specialised tcgen05.
   // Measured at 64800 tokens x 16 heads: 0.37 / 0.44 / 0.66 ms for impl 3 / 1 / 2.
@@ -731,7 +701,7 @@ std::vector<Tensor> window_attn_fwd(Tensor qkv, Tensor qw, Tensor kw, std::vecto
   if (tc_ok && (impl == 3 || impl == 0))
     check(nsw::window_attn_fwd_ws(qkv.data_ptr(), qw.data_ptr<float>(), kw.data_ptr<float>(), out.data_ptr(),
                                   lse.data_ptr<float>(), g, stream(),
-                                  stamps ? reinterpret_cast<long long*>(stamps->data_ptr<int64_t>()) : nullptr, bias),
+                                  stamps ? reinterpret_cast<long long*>(stamps->data_ptr<int64_t>()) : nullptr),
           "window_attn_fwd_ws");
   else if (tc_ok && impl == 2)
     check(nsw::window_attn_fwd_tc(qkv.data_ptr(), qw.data_ptr<float>(), kw.data_ptr<float>(), out.data_ptr(),
@@ -739,20 +709,17 @@ std::vector<Tensor> window_attn_fwd(Tensor qkv, Tensor qw, Tensor kw, std::vecto
           "window_attn_fwd_tc");
   else
     check(nsw::window_attn_fwd(qkv.data_ptr(), qw.data_ptr<float>(), kw.data_ptr<float>(), out.data_ptr(),
-                               lse.data_ptr<float>(), g, dt_code(qkv), stream(), bias),
+                               lse.data_ptr<float>(), g, dt_code(qkv), stream()),
           "window_attn_fwd");
-  if (tab) return {out, lse, *tab};
   return {out, lse};
 }
 
 std::vector<Tensor> window_attn_bwd(Tensor qkv, Tensor qw, Tensor kw, Tensor out, Tensor dout, Tensor lse,
                                     std::vector<int64_t> gi, double scale, int64_t impl,
                                     c10::optional<Tensor> stamps, c10::optional<Tensor> dqw_into,
-                                    c10::optional<Tensor> dkw_into, c10::optional<Tensor> tab,
-                                    c10::optional<Tensor> dbias, bool dbias_add) {
+                                    c10::optional<Tensor> dkw_into) {
   need_cuda(qkv, "qkv");
   need_cuda(dout, "dout");
-  const c10::cuda::CUDAGuard guard(qkv.device());
   auto g = make_geom(gi, scale);
   auto dqkv = torch::empty_like(qkv);
   const int64_t nwin = (int64_t)g.B * (g.H / g.wh) * (g.W / g.ww);
@@ -768,31 +735,16 @@ std::vector<Tensor> window_attn_bwd(Tensor qkv, Tensor qw, Tensor kw, Tensor out
   auto part = torch::empty({2, rows, (int64_t)g.hd}, qkv.options().dtype(at::kFloat));
   float* qp = part.data_ptr<float>();
   float* kp = qp + rows * g.hd;
-  // the bias's gradient goes to dbias (heads, buckets): a fresh tensor of any type, or an fp32 one that is added to
-  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
-  const nsw::AttnBias bias = bias_of(g, tab);
-  TORCH_CHECK(!tab || lse.numel() == items * g.T * g.wh * g.ww * 2, "window_attn_bwd: lse is not the forward's");
-  const int64_t buckets = (int64_t)(2 * g.T - 1) * (2 * g.wh - 1) * (2 * g.ww - 1);
-  Tensor bpart;
-  float* bp = nullptr;
-  if (dbias) {
-    TORCH_CHECK(tab && dbias->is_cuda() && dbias->is_contiguous() && dbias->numel() == g.nh * buckets,
-                "window_attn_bwd: the bias's gradient is a contiguous CUDA tensor of (heads, buckets)");
-    bpart = torch::empty({nsw::attn_bias_rows(g, tc, sms), buckets}, qkv.options().dtype(at::kFloat));
-    bp = bpart.data_ptr<float>();
-  }
   if (tc)
     check(nsw::window_attn_bwd_tc(qkv.data_ptr(), qw.data_ptr<float>(), kw.data_ptr<float>(), out.data_ptr(),
                                   dout.data_ptr(), lse.data_ptr<float>(), dqkv.data_ptr(), qp, kp, g, stream(),
-                                  stamps ? reinterpret_cast<long long*>(stamps->data_ptr<int64_t>()) : nullptr, bias, bp),
+                                  stamps ? reinterpret_cast<long long*>(stamps->data_ptr<int64_t>()) : nullptr),
           "window_attn_bwd_tc");
   else
     check(nsw::window_attn_bwd(qkv.data_ptr(), qw.data_ptr<float>(), kw.data_ptr<float>(), out.data_ptr(),
                                dout.data_ptr(), lse.data_ptr<float>(), dqkv.data_ptr(), qp, kp, g, dt_code(qkv),
-                               stream(), bias, bp),
+                               stream()),
           "window_attn_bwd");
-  if (bp)
-    check(nsw::attn_bias_grad(bp, g, tc, sms, dbias->data_ptr(), dt_code(*dbias), dbias_add, stream()), "attn_bias_grad");
   // QK-norm weight gradients: added into the given fp32 gradient buffers (both or neither), else fresh
   if (dqw_into || dkw_into) {
     TORCH_CHECK(dqw_into && dkw_into, "window_attn_bwd: dqw_into and dkw_into go together");
@@ -811,13 +763,15 @@ std::vector<Tensor> window_attn_bwd(Tensor qkv, Tensor qw, Tensor kw, Tensor out
 
 }  // namespace
 
-void bind_block(py::module& m);    // bindings_block.cpp
-void bind_experts(py::module& m);  // bindings_experts.cpp
+void bind_block(py::module& m);      // bindings_block.cpp
+void bind_experts(py::module& m);    // bindings_experts.cpp
+void bind_attention(py::module& m);  // bindings_attention.cpp
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.doc() = "sm_100a kernels of neural_scaling_weather_b200";
   bind_block(m);
   bind_experts(m);
+  bind_attention(m);
   m.def("read_error_flag", &read_error_flag, py::arg("clear") = true);
   m.def("wgrad_supported", &wgrad_supported, py::arg("dy"), py::arg("x"));
   m.def("legendre_table", &legendre_table);
@@ -858,9 +812,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("adamw_step", &adamw_step);
   m.def("segment_sumsq", &segment_sumsq);
   m.def("window_attn_fwd", &window_attn_fwd, py::arg("qkv"), py::arg("qw"), py::arg("kw"), py::arg("geom"),
-        py::arg("scale"), py::arg("impl") = 0, py::arg("stamps") = py::none(), py::arg("rel_bias") = py::none());
+        py::arg("scale"), py::arg("impl") = 0, py::arg("stamps") = py::none());
   m.def("window_attn_bwd", &window_attn_bwd, py::arg("qkv"), py::arg("qw"), py::arg("kw"), py::arg("out"),
         py::arg("dout"), py::arg("lse"), py::arg("geom"), py::arg("scale"), py::arg("impl") = 0,
-        py::arg("stamps") = py::none(), py::arg("dqw_into") = py::none(), py::arg("dkw_into") = py::none(),
-        py::arg("tab") = py::none(), py::arg("dbias") = py::none(), py::arg("dbias_add") = false);
+        py::arg("stamps") = py::none(), py::arg("dqw_into") = py::none(), py::arg("dkw_into") = py::none());
 }

@@ -268,16 +268,6 @@ std::vector<Tensor> gated_mlp_bwd(const Tensor& dy, const Tensor& x, const Tenso
   return out;
 }
 
-// (..., n) as a matrix; a matrix y with x's leading dimensions
-Tensor flat(const Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
-OptTensor flat(const OptTensor& t) { return t ? OptTensor(flat(*t)) : OptTensor(); }
-Tensor unflat(const Tensor& y, const Tensor& x) {
-  if (x.dim() == 2) return y;
-  auto sizes = x.sizes().vec();
-  sizes.back() = y.size(1);
-  return y.view(sizes);
-}
-
 // The network of 16-bit parameters as one autograd node (fp32 master parameters, whose gradients may go
 // straight into the optimizer's buffers, go through the Python node on the same two functions).
 struct GatedNode : public torch::autograd::Function<GatedNode> {

@@ -23,21 +23,21 @@ nsw::RouteArgs route_args(const Tensor& logits, int64_t k, bool normalize) {
   return a;
 }
 
-// {weights, experts, balance, share}
+// {weights, experts, balance, share}; share: experts' shares for the backward, in front of the blocks' partial sums
 std::vector<Tensor> route_fwd(const Tensor& logits, int64_t k, bool normalize) {
   nsw::RouteArgs a = route_args(logits, k, normalize);
   const c10::cuda::CUDAGuard guard(logits.device());
   const auto f32 = logits.options().dtype(at::kFloat);
   auto weights = torch::empty({a.tokens, k}, f32);
   auto chosen = torch::empty({a.tokens, k}, logits.options().dtype(at::kLong));
-  auto balance = torch::empty({}, f32), share = torch::empty({a.experts}, f32);
+  auto balance = torch::empty({}, f32);
   const int blocks = nsw::route_blocks(a.tokens, a.experts, sm_count(logits));
-  auto partial = torch::empty({2 * (int64_t)blocks * a.experts}, f32);
+  auto share = torch::empty({(2 * (int64_t)blocks + 1) * a.experts}, f32);
   a.weights = weights.data_ptr<float>();
   a.chosen = chosen.data_ptr<int64_t>();
   a.balance = balance.data_ptr<float>();
   a.share = share.data_ptr<float>();
-  a.partial = partial.data_ptr();
+  a.partial = a.share + a.experts;
   check(nsw::route_fwd(a, blocks, stream()), "route_tokens");
   return {weights, chosen, balance, share};
 }
@@ -63,6 +63,44 @@ Tensor route_bwd(const Tensor& logits, const Tensor& weights, const Tensor& chos
   a.dlogits = d.data_ptr();
   check(nsw::route_bwd(a, sm_count(logits), stream()), "route_tokens backward");
   return d;
+}
+
+struct RouteNode : public torch::autograd::Function<RouteNode> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& logits, int64_t k,
+                                                bool normalize) {
+    const Tensor z = flat(logits), zu = z.stride(1) == 1 || z.size(1) == 1 ? z : z.contiguous();
+    auto r = route_fwd(zu, k, normalize);
+    ctx->save_for_backward({zu, r[0], r[1], r[3]});
+    ctx->saved_data["normalize"] = normalize;
+    ctx->saved_data["shape"] = logits.sizes().vec();
+    ctx->set_materialize_grads(false);
+    const Tensor chosen = unflat(r[1], logits);
+    ctx->mark_non_differentiable({chosen});
+    return {unflat(r[0], logits), chosen, r[2]};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grad) {
+    once_differentiable("route_tokens");
+    const auto v = ctx->get_saved_variables();
+    const auto f32 = [](const Tensor& t) {
+      return t.defined() ? OptTensor(t.to(at::kFloat).contiguous()) : OptTensor();
+    };
+    const Tensor d = route_bwd(v[0], v[1], v[2], v[3], f32(grad[0]), f32(grad[2]), ctx->saved_data["normalize"].toBool());
+    return {d.view(ctx->saved_data["shape"].toIntVector()), Tensor(), Tensor()};
+  }
+};
+
+// logits (..., E) -> (weights (..., k), experts (..., k), balance)
+std::tuple<Tensor, Tensor, Tensor> route_tokens(const Tensor& logits, int64_t k, bool normalize) {
+  TORCH_CHECK_VALUE(logits.dim() >= 1 && logits.size(-1) >= 1, "route_tokens: logits ", logits.sizes());
+  if (tangents()) no_tangent(logits, "route_tokens");
+  if (at::GradMode::is_enabled() && logits.requires_grad()) {
+    auto r = RouteNode::apply(logits, k, normalize);
+    return {r[0], r[1], r[2]};
+  }
+  const Tensor z = flat(logits);
+  auto r = route_fwd(z.stride(1) == 1 || z.size(1) == 1 ? z : z.contiguous(), k, normalize);
+  return {unflat(r[0], logits), unflat(r[1], logits), r[2]};
 }
 
 // ------------------------------------------------------------------------------ experts
@@ -391,11 +429,72 @@ std::vector<Tensor> expert_mlp_bwd(const Tensor& dy, const Tensor& weights, int6
   return out;
 }
 
+// The network of parameters in the compute type as one autograd node (fp32 master parameters, whose gradients may go
+// straight into the optimizer's buffers, go through the Python node on the same two functions).
+struct ExpertNode : public torch::autograd::Function<ExpertNode> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& weights,
+                        const Tensor& experts, const Tensor& wg, const Tensor& wu, const Tensor& wd,
+                        const OptTensor& residual, int64_t act) {
+    const Tensor w2 = flat(weights).contiguous();
+    auto r = expert_mlp_fwd(flat(x), w2, flat(experts).contiguous(), wg, wu, wd, flat(residual), act, true);
+    ctx->save_for_backward({w2, r[1], r[2], r[3], r[4], r[5], r[6], r[7], r[8], r[9]});
+    ctx->saved_data["shape"] = x.sizes().vec();
+    ctx->saved_data["weights"] = weights.sizes().vec();
+    ctx->saved_data["experts"] = wg.size(0);
+    ctx->saved_data["act"] = act;
+    ctx->saved_data["residual"] = residual.has_value();
+    return unflat(r[0], x);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grad) {
+    once_differentiable("expert_mlp");
+    const auto v = ctx->get_saved_variables();
+    const auto shape = ctx->saved_data["shape"].toIntVector();
+    std::vector<bool> need(5);
+    for (int i = 0; i < 5; ++i) need[i] = ctx->needs_input_grad(i < 2 ? i : i + 1);
+    auto g = expert_mlp_bwd(flat(grad[0]), v[0], ctx->saved_data["experts"].toInt(), shape.back(), v[1], v[2], v[3], v[4],
+                            v[5], v[6], v[7], v[8], v[9], ctx->saved_data["act"].toInt(), need, std::vector<OptTensor>(3),
+                            std::vector<at::ScalarType>(3, v[7].scalar_type()));
+    if (need[0]) g[0] = g[0].view(shape);
+    if (need[1]) g[1] = g[1].view(ctx->saved_data["weights"].toIntVector());
+    const bool need_res = ctx->saved_data["residual"].toBool() && ctx->needs_input_grad(6);
+    return {g[0], g[1], Tensor(), g[2], g[3], g[4], need_res ? grad[0] : Tensor(), Tensor()};
+  }
+};
+
+// x (..., K), weights and experts (int64) (..., k), residual (..., N); x, the matrices and residual in one 16-bit type
+Tensor expert_mlp(const Tensor& x, const Tensor& weights, const Tensor& experts, const Tensor& wg, const Tensor& wu,
+                  const Tensor& wd, const OptTensor& residual, int64_t act) {
+  TORCH_CHECK_VALUE(x.dim() >= 1 && wg.dim() == 3 && wd.dim() == 3 && wu.sizes() == wg.sizes() &&
+                        wd.size(0) == wg.size(0) && wd.size(2) == wg.size(1) && x.size(-1) == wg.size(2),
+                    "expert_mlp: x ", x.sizes(), ", w_gate ", wg.sizes(), ", w_up ", wu.sizes(), " and w_down ",
+                    wd.sizes(), " do not fit together");
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  TORCH_CHECK_VALUE(weights.sizes() == experts.sizes() && weights.dim() == x.dim() &&
+                        weights.sizes().slice(0, x.dim() - 1) == lead,
+                    "expert_mlp: weights ", weights.sizes(), " and experts ", experts.sizes(), " are not (", lead, ", k)");
+  TORCH_CHECK_VALUE(!residual || (residual->dim() == x.dim() && residual->size(-1) == wd.size(1) &&
+                                  residual->sizes().slice(0, x.dim() - 1) == lead),
+                    "expert_mlp: residual ", residual->sizes(), " is not the output's shape");
+  if (tangents()) {
+    for (const Tensor* t : {&x, &weights, &wg, &wu, &wd}) no_tangent(*t, "expert_mlp");
+    no_tangent(residual, "expert_mlp");
+  }
+  bool grad = false;
+  if (at::GradMode::is_enabled()) {
+    for (const Tensor* t : {&x, &weights, &wg, &wu, &wd}) grad = grad || t->requires_grad();
+    grad = grad || (residual && residual->requires_grad());
+  }
+  if (grad) return ExpertNode::apply(x, weights, experts, wg, wu, wd, residual, act);
+  return unflat(expert_mlp_fwd(flat(x), flat(weights).contiguous(), flat(experts).contiguous(), wg, wu, wd,
+                               flat(residual), act, false)[0], x);
+}
+
 }  // namespace
 
 void bind_experts(py::module& m) {
-  m.def("route_fwd", &route_fwd);
-  m.def("route_bwd", &route_bwd);
+  m.def("route_tokens", &route_tokens);
+  m.def("expert_mlp", &expert_mlp);
   m.def("expert_mlp_fwd", &expert_mlp_fwd);
   m.def("expert_mlp_bwd", &expert_mlp_bwd);
 }

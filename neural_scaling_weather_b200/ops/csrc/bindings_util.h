@@ -83,6 +83,16 @@ struct Aligner {
 OptTensor packed_vec(const OptTensor& t) { return !t || t->is_contiguous() ? t : OptTensor(t->contiguous()); }
 const void* opt_ptr(const OptTensor& t) { return t && t->defined() ? t->data_ptr() : nullptr; }
 
+// (..., n) as a matrix; a matrix y with x's leading dimensions
+Tensor flat(const Tensor& t) { return t.dim() == 2 ? t : t.reshape({-1, t.size(-1)}); }
+OptTensor flat(const OptTensor& t) { return t ? OptTensor(flat(*t)) : OptTensor(); }
+Tensor unflat(const Tensor& y, const Tensor& x) {
+  if (x.dim() == 2) return y;
+  auto sizes = x.sizes().vec();
+  sizes.back() = y.size(1);
+  return y.view(sizes);
+}
+
 // Where a parameter's gradient goes: added into the given fp32 buffer, or a fresh tensor (16-bit where that is
 // the parameter's type, else fp32 and cast at the end)
 struct GradOut {

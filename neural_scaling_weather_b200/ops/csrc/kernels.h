@@ -81,16 +81,29 @@ struct AttnBias {
 };
 constexpr int kAttnBiasRow = 1160;  // floats of a row: at most (2 T - 1)(2 wh - 1)(2 ww - 1) = 1155 of 192 tokens
 AttnBias attn_bias_layout(const AttnGeom& g);
-// table (nh, (2 T - 1)(2 wh - 1)(2 ww - 1)) of any strides and type -> b.stride floats a head
-cudaError_t attn_bias_prepare(const void* table, int dtype, int64_t s0, int64_t s1, const AttnGeom& g,
+// A vector or matrix of any type and strides
+struct AnyMatrix {
+  const void* p;
+  int dtype;
+  int64_t s0, s1;
+};
+// table (nh, (2 T - 1)(2 wh - 1)(2 ww - 1)) and the norms' weights (hd) -> b.stride floats a head at tab, then the
+// weights of q and of k, hd floats each
+cudaError_t attn_bias_prepare(const AnyMatrix& table, const AnyMatrix& qw, const AnyMatrix& kw, const AttnGeom& g,
                               const AttnBias& b, float* tab, cudaStream_t s);
 // With a bias the forward writes two floats a row, (largest logit, log2 of the sum of exponentials less it), and the
 // backward reads them: their sum, the log-sum-exp, would lose the second where a row's logits are far from zero.
-// dbias_part: rows of partial sums of the bias's gradient (null: not wanted), attn_bias_rows(..) of them; sums in
-// units of `unit` (dS is scaled before it is rounded), reduced by attn_bias_grad into out[head, bucket].
+// dbias_part: rows of partial sums of the bias's gradient (null: not wanted), attn_bias_rows(..) of them.
 int64_t attn_bias_rows(const AttnGeom& g, bool tc, int sms);
-cudaError_t attn_bias_grad(const float* part, const AttnGeom& g, bool tc, int sms, void* out, int dtype, bool accumulate,
-                           cudaStream_t s);
+// The parameters' gradients from their partial sums: out (null: not wanted) in dtype, or fp32 and added to.
+struct AttnGrad {
+  const float* part;
+  void* out;
+  int dtype, add;
+};
+// bias: [nh][buckets]; q, k: [hd], from qk_rows rows of partial sums each
+cudaError_t attn_bias_grads(const AttnGrad& bias, const AttnGrad& q, const AttnGrad& k, int64_t qk_rows, const AttnGeom& g,
+                            bool tc, int sms, cudaStream_t s);
 cudaError_t window_attn_fwd(const void* qkv, const float* qw, const float* kw, void* out, float* lse,
                             const AttnGeom& g, int dtype, cudaStream_t s, const AttnBias& bias = {});
 // tcgen05/TMEM forward (bf16, head_dim 64, T*wh*ww <= 176); same outputs as window_attn_fwd

@@ -62,10 +62,32 @@ __device__ __forceinline__ float group_sum(float v) {
 // exp(z - m), zero for a row without a finite value
 __device__ __forceinline__ float shifted_exp(float z, float m) { return m == -INFINITY ? 0.f : expf(z - m); }
 
+// share and balance of one block's own sums (of all of them: a few tokens take one block and one launch)
+__device__ __forceinline__ void finish_block(const RouteArgs& a, const float* psum, const int* count, int groups,
+                                             float* red) {
+  const int E = a.experts;
+  float term = 0.f;
+  for (int e = threadIdx.x; e < E; e += kThreads) {
+    float p = 0.f;
+    for (int i = 0; i < groups; ++i) p += psum[i * E + e];
+    const float share = a.tokens > 0 ? (float)count[e] * (float)((double)E / ((double)a.tokens * a.k)) : 0.f;
+    a.share[e] = share;
+    term += a.tokens > 0 ? share * p / (float)a.tokens : 0.f;
+  }
+  term = warp_sum(term);
+  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = term;
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int w = 1; w < kThreads / 32; ++w) term += red[w];
+    *a.balance = term;
+  }
+}
+
 // All lanes of a warp run the same number of rounds; groups past the last token take part with nothing.
 template <typename T, int G, int V>
 __global__ void __launch_bounds__(kThreads) fwd_kernel(const RouteArgs a) {
   extern __shared__ float sums[];  // [kThreads / G][experts] probabilities, then [experts] counts
+  __shared__ float red[kThreads / 32];
   constexpr int kGroups = kThreads / G;
   const int E = a.experts, k = a.k, l = threadIdx.x % G, group = threadIdx.x / G;
   int* count = reinterpret_cast<int*>(sums + kGroups * E);
@@ -142,6 +164,7 @@ __global__ void __launch_bounds__(kThreads) fwd_kernel(const RouteArgs a) {
   for (int i = 0; i < V; ++i)
     if (l + G * i < E) sums[group * E + l + G * i] = psum[i];
   __syncthreads();
+  if (gridDim.x == 1) return finish_block(a, sums, count, kGroups, red);
   float* psums = reinterpret_cast<float*>(a.partial);
   int* counts = reinterpret_cast<int*>(psums + (int64_t)gridDim.x * E);
   for (int e = threadIdx.x; e < E; e += kThreads) {
@@ -293,7 +316,7 @@ cudaError_t route_fwd(const RouteArgs& a, int blocks, cudaStream_t s) {
       return cudaGetLastError();
     });
   }));
-  route::balance_kernel<<<1, 1024, 0, s>>>(a, blocks);
+  if (blocks > 1) route::balance_kernel<<<1, 1024, 0, s>>>(a, blocks);
   return cudaGetLastError();
 }
 

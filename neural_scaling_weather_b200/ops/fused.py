@@ -443,46 +443,6 @@ def gated_mlp_cuda(x, wg, wu, wd, bg, bu, bd, residual, activation):
 
 
 # ---------------------------------------------------------------------------- routed experts
-class _Route(torch.autograd.Function):
-    """The router's choice.  It keeps the logits, from which the backward forms the probabilities again (the bytes of
-    reading them), the choice and its weights."""
-
-    @staticmethod
-    def forward(ctx, logits, k, normalize):
-        w, chosen, balance, share = require().route_fwd(logits, k, normalize)
-        ctx.save_for_backward(logits, w, chosen, share)
-        ctx.normalize = normalize
-        ctx.mark_non_differentiable(chosen)
-        ctx.set_materialize_grads(False)
-        return w, chosen, balance
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dw, _, dbalance):
-        if dw is None and dbalance is None:
-            return None, None, None
-        dw, dbalance = (None if t is None else t.float().contiguous() for t in (dw, dbalance))
-        return require().route_bwd(*ctx.saved_tensors, dw, dbalance, ctx.normalize), None, None
-
-
-def route_tokens_cuda(logits, top_k, normalize):
-    _no_tangents("route_tokens", logits)
-    e = logits.shape[-1]
-    z = logits.reshape(-1, e)
-    if z.dtype not in DT:
-        raise TypeError(f"route_tokens: logits of {z.dtype} on CUDA (bf16, fp16 or fp32)")
-    if z.stride(1) != 1:
-        z = z.contiguous()
-    if torch.is_grad_enabled() and z.requires_grad:
-        w, chosen, balance = _Route.apply(z, top_k, normalize)
-    else:
-        w, chosen, balance, _ = require().route_fwd(z, top_k, normalize)
-    if logits.dim() == 2:
-        return w, chosen, balance
-    shape = (*logits.shape[:-1], top_k)
-    return w.view(shape), chosen.view(shape), balance
-
-
 def check_expert_shapes(x, weights, experts, wg, wu, wd, residual):
     if (wg.dim() != 3 or wu.shape != wg.shape or wd.dim() != 3 or wd.shape[0] != wg.shape[0]
             or wd.shape[2] != wg.shape[1] or x.dim() < 1 or x.shape[-1] != wg.shape[2]):
@@ -491,10 +451,13 @@ def check_expert_shapes(x, weights, experts, wg, wu, wd, residual):
     if weights.shape != experts.shape or weights.dim() != x.dim() or weights.shape[:-1] != x.shape[:-1]:
         raise ValueError(f"expert_mlp: weights {tuple(weights.shape)} and experts {tuple(experts.shape)} must be "
                          f"({', '.join(map(str, (*x.shape[:-1], 'k')))})")
-    if experts.dtype.is_floating_point or experts.dtype.is_complex or experts.dtype == torch.bool:
-        raise TypeError(f"expert_mlp: experts are integers, got {experts.dtype}")
     if residual is not None and residual.shape != x.shape[:-1] + wd.shape[1:2]:
         raise ValueError(f"expert_mlp: residual {tuple(residual.shape)} is not the output's shape")
+
+
+def check_expert_ids(experts):
+    if experts.dtype.is_floating_point or experts.dtype.is_complex or experts.dtype == torch.bool:
+        raise TypeError(f"expert_mlp: experts are integers, got {experts.dtype}")
 
 
 class _ExpertMLP(torch.autograd.Function):
@@ -541,19 +504,22 @@ class _ExpertMLP(torch.autograd.Function):
 def expert_mlp_cuda(x, weights, experts, wg, wu, wd, residual, activation):
     act = _GATED_ACT[activation]
     dt = _cdtype(x)
-    check_expert_shapes(x, weights, experts, wg, wu, wd, residual)
-    _no_tangents("expert_mlp", x, weights, wg, wu, wd, residual)
+    if experts.dtype != torch.int64:
+        check_expert_ids(experts)
+        experts = experts.to(torch.int64)
     if weights.dtype not in DT:
         weights = weights.float()
-    k, K, N = experts.shape[-1], x.shape[-1], wd.shape[1]
-    chosen = _rows(experts, k).to(torch.int64).contiguous()
+    if residual is not None and residual.dtype != dt:
+        residual = residual.to(dt)
+    if wg.dtype == wu.dtype == wd.dtype == dt:  # parameters already in the compute type: one native node
+        return require().expert_mlp(x if x.dtype == dt else x.to(dt), weights, experts, wg, wu, wd, residual, act)
+    check_expert_shapes(x, weights, experts, wg, wu, wd, residual)
+    _no_tangents("expert_mlp", x, weights, wg, wu, wd, residual)
     given = (x, weights, wg, wu, wd, residual)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in given):
+        chosen = _rows(experts, experts.shape[-1]).contiguous()
         return _ExpertMLP.apply(x, weights, chosen, residual, act, wg, wu, wd)
-    y, = require().expert_mlp_fwd(_rows(x, K).to(dt), _rows(weights, k).contiguous(), chosen,
-                                  *(wcache.get(w, dt) for w in (wg, wu, wd)),
-                                  None if residual is None else _rows(residual, N).to(dt), act, False)
-    return y.view(*x.shape[:-1], N)
+    return require().expert_mlp(x.to(dt), weights, experts, *(wcache.get(w, dt) for w in (wg, wu, wd)), residual, act)
 
 
 # ---------------------------------------------------------------------------- norms, gate, skip
@@ -579,54 +545,63 @@ ATTN_FWD_IMPL = int(os.environ.get("NSW_ATTN_FWD_IMPL", "0"))
 
 class _WindowAttn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, qkv, qw, kw, gi, scale, rel_bias):
+    def forward(ctx, qkv, qw, kw, gi, scale):
         ext = require()
         qkv2 = qkv.contiguous()
-        out, lse, *tab = ext.window_attn_fwd(qkv2, qw.detach().float().contiguous(),
-                                             kw.detach().float().contiguous(), gi, scale, ATTN_FWD_IMPL,
-                                             rel_bias=_bias_table(rel_bias))
-        ctx.save_for_backward(qkv2, qw, kw, out, lse, *tab)
-        ctx.gi, ctx.scale, ctx.rel_bias = gi, scale, rel_bias
+        out, lse = ext.window_attn_fwd(qkv2, qw.detach().float().contiguous(),
+                                       kw.detach().float().contiguous(), gi, scale, ATTN_FWD_IMPL)
+        ctx.save_for_backward(qkv2, qw, kw, out, lse)
+        ctx.gi, ctx.scale = gi, scale
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             gradsink.use([qw, kw])
-        if ctx.needs_input_grad[5]:
-            gradsink.use([rel_bias])
         return out
 
     @staticmethod
     def backward(ctx, dout):
         ext = require()
-        qkv, qw, kw, out, lse, *tab = ctx.saved_tensors
+        qkv, qw, kw, out, lse = ctx.saved_tensors
         # QK-norm weight gradients straight into the optimizer's gradient buffer where possible
         tq, tk = gradsink.target(qw), gradsink.target(kw)
         inplace = tq is not None and tk is not None
-        # the bias's gradient likewise, or a tensor of its type
-        dbias = tb = None
-        if ctx.needs_input_grad[5]:
-            bias = ctx.rel_bias
-            tb = gradsink.target(bias)
-            dbias = torch.empty(bias.shape, device=bias.device,
-                                dtype=bias.dtype if bias.dtype in DT else torch.float32) if tb is None else tb
         dqkv, dqw, dkw = ext.window_attn_bwd(qkv, qw.detach().float().contiguous(),
                                              kw.detach().float().contiguous(), out,
                                              dout.to(qkv.dtype).contiguous(), lse, ctx.gi, ctx.scale,
-                                             dqw_into=tq if inplace else None, dkw_into=tk if inplace else None,
-                                             tab=tab[0] if tab else None, dbias=dbias, dbias_add=tb is not None)
-        if dbias is not None:
-            gradsink.done(ctx.rel_bias, tb is not None)
-            dbias = None if tb is not None else dbias.to(ctx.rel_bias.dtype)
+                                             dqw_into=tq if inplace else None, dkw_into=tk if inplace else None)
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             gradsink.done(qw, inplace)
             gradsink.done(kw, inplace)
         if inplace:
-            return dqkv, None, None, None, None, dbias
-        return dqkv, dqw.to(qw.dtype), dkw.to(kw.dtype), None, None, dbias
+            return dqkv, None, None, None, None
+        return dqkv, dqw.to(qw.dtype), dkw.to(kw.dtype), None, None
 
 
-def _bias_table(rel_bias):
-    if rel_bias is None:
-        return None
-    return rel_bias.detach() if rel_bias.dtype in DT else rel_bias.detach().float()
+class _BiasedWindowAttn(torch.autograd.Function):
+    """Window attention with a relative position bias and fp32 master parameters, whose gradients are added into the
+    optimizer's buffers where possible (``gradsink``)."""
+
+    @staticmethod
+    def forward(ctx, qkv, qw, kw, rel_bias, gi, scale):
+        qkv = qkv.contiguous()
+        out, lse, tab = require().attn_bias_fwd(qkv, qw, kw, rel_bias, gi, scale)
+        ctx.save_for_backward(qkv, tab, out, lse)
+        ctx.params, ctx.gi, ctx.scale = (qw, kw, rel_bias), gi, scale
+        ctx.used = [p for p, n in zip(ctx.params, ctx.needs_input_grad[1:4]) if n]
+        gradsink.use(ctx.used)
+        return out
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dout):
+        qkv, tab, out, lse = ctx.saved_tensors
+        need = ctx.needs_input_grad[1:4]
+        given = [id(p) for p in ctx.params]  # one that is here twice: its shares meet in autograd
+        into = [gradsink.target(p) if n and given.count(id(p)) == 1 else None for p, n in zip(ctx.params, need)]
+        dqkv, *grads = require().attn_bias_bwd(qkv, tab, out, dout.to(qkv.dtype).contiguous(), lse, ctx.gi, ctx.scale,
+                                               list(need), into, [p.dtype for p in ctx.params])
+        for p, t, n in zip(ctx.params, into, need):
+            if n:
+                gradsink.done(p, t is not None)
+        return (dqkv if ctx.needs_input_grad[0] else None, *grads, None, None)
 
 
 def check_rel_bias(rel_bias, num_heads, geom: WindowGeometry, steps):
@@ -639,8 +614,17 @@ def window_attention_cuda(qkv, q_norm_w, k_norm_w, num_heads, head_dim, geom: Wi
     B, T, H, W, C3 = qkv.shape
     dt = _cdtype(qkv)
     gi = _geom_ints(B, T, H, W, num_heads, head_dim, geom)
-    check_rel_bias(rel_bias, num_heads, geom, T)
-    out = _WindowAttn.apply(qkv.to(dt), q_norm_w, k_norm_w, gi, float(scale), rel_bias)
+    if rel_bias is not None:
+        if qkv.dtype != dt:
+            qkv = qkv.to(dt)
+        params = [p if p.dtype in DT else p.float() for p in (q_norm_w, k_norm_w, rel_bias)]
+        if torch.is_grad_enabled() and any(isinstance(p, torch.nn.Parameter) and p.dtype == torch.float32 and p.requires_grad
+                                           for p in params):
+            _no_tangents("window_attention", qkv, *params)
+            out = _BiasedWindowAttn.apply(qkv, *params, gi, float(scale))
+            return out.view(B, T, H, W, num_heads * head_dim)
+        return require().window_attention_bias(qkv, *params, gi, float(scale))
+    out = _WindowAttn.apply(qkv.to(dt), q_norm_w, k_norm_w, gi, float(scale))
     return out.view(B, T, H, W, num_heads * head_dim)
 
 

@@ -16,6 +16,7 @@ SOURCES = [
     os.path.join(CSRC, "bindings.cpp"),
     os.path.join(CSRC, "bindings_block.cpp"),
     os.path.join(CSRC, "bindings_experts.cpp"),
+    os.path.join(CSRC, "bindings_attention.cpp"),
     os.path.join(CSRC, "elementwise.cu"),
     os.path.join(CSRC, "attention.cu"),
     os.path.join(CSRC, "attention_tc.cu"),
