@@ -21,68 +21,11 @@
 // gradients of the two norm weights are reduced by the caller in a fixed order.
 #include <float.h>
 
-#include "common.cuh"
+#include "attn_mma.cuh"
 #include "kernels.h"
 
 namespace nsw {
 namespace attn {
-
-constexpr float kLog2e = 1.4426950408889634f;
-
-__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2,
-                                        uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
-}
-__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2,
-                                          uint32_t& r3) {
-  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];\n"
-               : "=r"(r0), "=r"(r1), "=r"(r2), "=r"(r3)
-               : "r"(addr));
-}
-
-template <typename T>
-__device__ __forceinline__ void mma16816(float* c, const uint32_t* a, uint32_t b0, uint32_t b1);
-template <>
-__device__ __forceinline__ void mma16816<__nv_bfloat16>(float* c, const uint32_t* a, uint32_t b0,
-                                                        uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};\n"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma16816<__half>(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
-      "{%0,%1,%2,%3};\n"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-
-// Two floats -> one packed pair of 16-bit values in a single conversion instruction.
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float lo, float hi);
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float lo, float hi) {
-  __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float lo, float hi) {
-  __half2 v = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<uint32_t*>(&v);
-}
-
-// Hardware base-2 exponential (ex2.approx.ftz: ~2 ulp), ample for probabilities that are
-// rounded to 16 bits before the P.V product.
-__device__ __forceinline__ float fast_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 struct WinPos {
   int b, wy, wx;
@@ -115,13 +58,6 @@ __device__ __forceinline__ int win_label(const AttnGeom& g, const WinPos& p, int
   const int iy = (i % wa) / g.ww;
   const int row_g = g.row_offset + p.wy * g.wh + iy;
   return row_g >= g.h_global - g.mask_shift ? 1 : 0;
-}
-
-__device__ __forceinline__ void cp_async16(void* dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_wait_all() {
-  asm volatile("cp.async.commit_group;\n cp.async.wait_group 0;" ::: "memory");
 }
 
 // Grid-token index and region label of every window position (the only place with
@@ -203,10 +139,10 @@ static size_t bias_bytes(const AttnBias& b, int rows) {  // of tab and off, roun
 }
 
 // ============================================================================= forward
-template <typename T, int HD, bool BIAS>
+template <typename T, int HD>
 __global__ void __launch_bounds__(256, 2) fwd_kernel(const T* __restrict__ qkv, const float* __restrict__ qw,
                                                   const float* __restrict__ kw, T* __restrict__ out,
-                                                  float* __restrict__ lse, AttnGeom g, AttnBias bias) {
+                                                  float* __restrict__ lse, AttnGeom g) {
   constexpr int RS = HD + 8;  // smem row stride (elements); +16 B breaks bank conflicts
   constexpr int KS = HD / 16;
   constexpr int DT = HD / 8;
@@ -221,14 +157,10 @@ __global__ void __launch_bounds__(256, 2) fwd_kernel(const T* __restrict__ qkv, 
   int* sTok = reinterpret_cast<int*>(sV + lk * RS);
   signed char* sLab = reinterpret_cast<signed char*>(sTok + lk);
 
-  float* sTab = reinterpret_cast<float*>(smem + ((lq + 2 * lk) * RS * sizeof(T) + lk * 5 + 15) / 16 * 16);
-  short* sOff = reinterpret_cast<short*>(sTab + (BIAS ? bias.stride : 0));
-
   const int bw = blockIdx.x, h = blockIdx.y;
   const WinPos p = win_pos(g, bw);
   const int64_t C = (int64_t)g.nh * HD;
   const bool mixed = fill_tokens(sTok, sLab, g, p, L, lk);
-  if (BIAS) load_bias(sTab, sOff, bias, g, h, L, lk);
   load_rows<T, HD>(sQ, qkv, g.qkv_stride, 0 * C + (int64_t)h * HD, sTok, L, lq);
   load_rows<T, HD>(sK, qkv, g.qkv_stride, 1 * C + (int64_t)h * HD, sTok, L, lk);
   load_rows<T, HD>(sV, qkv, g.qkv_stride, 2 * C + (int64_t)h * HD, sTok, L, lk);
@@ -254,8 +186,6 @@ __global__ void __launch_bounds__(256, 2) fwd_kernel(const T* __restrict__ qkv, 
     const int r0 = qt * 16 + gq, r1 = r0 + 8;
     const int lab0 = sLab[r0] < 0 ? 0 : sLab[r0];
     const int lab1 = sLab[r1] < 0 ? 0 : sLab[r1];
-    const float* bias0 = sTab + (BIAS ? bias_center(g, bias.pitch) + sOff[r0] : 0);
-    const float* bias1 = sTab + (BIAS ? bias_center(g, bias.pitch) + sOff[r1] : 0);
     float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
     float o[DT][4];
 #pragma unroll
@@ -278,24 +208,7 @@ __global__ void __launch_bounds__(256, 2) fwd_kernel(const T* __restrict__ qkv, 
         }
       }
       float mx0 = -INFINITY, mx1 = -INFINITY;
-      if (BIAS) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int col = kc + j * 8 + 2 * tq + e;
-            const int lc = sLab[col], at = sOff[col];
-            float v0 = fmaf(s[j][e], sl2, bias0[-at]), v1 = fmaf(s[j][2 + e], sl2, bias1[-at]);
-            if (lc < 0) v0 = v1 = -INFINITY;
-            if (lc != lab0) v0 += ml2;
-            if (lc != lab1) v1 += ml2;
-            s[j][e] = v0;
-            s[j][2 + e] = v1;
-            mx0 = fmaxf(mx0, v0);
-            mx1 = fmaxf(mx1, v1);
-          }
-        }
-      } else if (!mixed && kc + 64 <= L) {
+      if (!mixed && kc + 64 <= L) {
         // no mask and no padding in this chunk (the common case)
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -333,15 +246,10 @@ __global__ void __launch_bounds__(256, 2) fwd_kernel(const T* __restrict__ qkv, 
       mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, 2));
       mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 1));
       mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, 2));
-      float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
-      const float old0 = m0, old1 = m1;
+      const float mn0 = fmaxf(m0, mx0), mn1 = fmaxf(m1, mx1);
+      const float c0 = fast_exp2(m0 - mn0), c1 = fast_exp2(m1 - mn1);
       m0 = mn0;
       m1 = mn1;
-      if (BIAS) {  // a row that the bias has masked so far: P = 0
-        if (mn0 == -INFINITY) mn0 = 0.f;
-        if (mn1 == -INFINITY) mn1 = 0.f;
-      }
-      const float c0 = fast_exp2(old0 - mn0), c1 = fast_exp2(old1 - mn1);
       l0 *= c0;
       l1 *= c1;
 #pragma unroll
@@ -382,7 +290,7 @@ __global__ void __launch_bounds__(256, 2) fwd_kernel(const T* __restrict__ qkv, 
     l0 += __shfl_xor_sync(0xffffffffu, l0, 2);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 1);
     l1 += __shfl_xor_sync(0xffffffffu, l1, 2);
-    const float il0 = BIAS && l0 == 0.f ? 0.f : 1.f / l0, il1 = BIAS && l1 == 0.f ? 0.f : 1.f / l1;
+    const float il0 = 1.f / l0, il1 = 1.f / l1;
     // stage the 16 x HD output tile in this warp's own Q rows, then store 16-byte chunks
     __syncwarp();
 #pragma unroll
@@ -393,14 +301,8 @@ __global__ void __launch_bounds__(256, 2) fwd_kernel(const T* __restrict__ qkv, 
     }
     if (tq == 0) {
       const int64_t base = ((int64_t)bw * g.nh + h) * L;
-      if (BIAS) {
-        float2* out2 = reinterpret_cast<float2*>(lse) + base;
-        if (r0 < L) out2[r0] = l0 == 0.f ? make_float2(0.f, 0.f) : make_float2(m0, log2f(l0));
-        if (r1 < L) out2[r1] = l1 == 0.f ? make_float2(0.f, 0.f) : make_float2(m1, log2f(l1));
-      } else {
-        if (r0 < L) lse[base + r0] = m0 + log2f(l0);
-        if (r1 < L) lse[base + r1] = m1 + log2f(l1);
-      }
+      if (r0 < L) lse[base + r0] = m0 + log2f(l0);
+      if (r1 < L) lse[base + r1] = m1 + log2f(l1);
     }
     __syncwarp();
     for (int idx = lane; idx < 16 * DT; idx += 32) {
@@ -880,18 +782,17 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
 
 template <typename T, int HD>
 static cudaError_t launch_fwd(const void* qkv, const float* qw, const float* kw, void* out, float* lse,
-                              const AttnGeom& g, cudaStream_t s, const AttnBias& bias) {
+                              const AttnGeom& g, cudaStream_t s) {
   const int L = g.T * g.wh * g.ww;
   const int nqt = (L + 15) / 16;
   const int lk = ((L + 63) / 64) * 64;
-  const size_t smem = (size_t)(nqt * 16 + 2 * lk) * (HD + 8) * sizeof(T) + (size_t)lk * (sizeof(int) + 1) +
-                      (bias.tab ? 16 + bias_bytes(bias, lk) : 0);
+  const size_t smem = (size_t)(nqt * 16 + 2 * lk) * (HD + 8) * sizeof(T) + (size_t)lk * (sizeof(int) + 1);
   int nw = nqt < 8 ? nqt : 8;
   if (nw < 1) nw = 1;
-  auto k = bias.tab ? fwd_kernel<T, HD, true> : fwd_kernel<T, HD, false>;
+  auto k = fwd_kernel<T, HD>;
   NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   dim3 grid(g.B * (g.H / g.wh) * (g.W / g.ww), g.nh);
-  k<<<grid, nw * 32, smem, s>>>((const T*)qkv, qw, kw, (T*)out, lse, g, bias);
+  k<<<grid, nw * 32, smem, s>>>((const T*)qkv, qw, kw, (T*)out, lse, g);
   return cudaGetLastError();
 }
 
@@ -910,7 +811,10 @@ static cudaError_t launch_bwd(const void* qkv, const float* qw, const float* kw,
                                         6 * kBiasTile * sizeof(T)
                                   : 0);
   int nw = 2 * nt < 6 ? 2 * nt : 6;
-  auto k = bias.tab ? bwd_kernel<T, HD, true> : bwd_kernel<T, HD, false>;
+  auto k = bwd_kernel<T, HD, false>;
+  if constexpr (HD == 128) {  // (narrower heads with a bias: attention_bias.cu)
+    if (bias.tab) k = bwd_kernel<T, HD, true>;
+  }
   NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   dim3 grid(g.B * (g.H / g.wh) * (g.W / g.ww), g.nh);
   k<<<grid, nw * 32, smem, s>>>((const T*)qkv, qw, kw, (const T*)out, (const T*)dout, lse, (T*)dqkv,
@@ -937,10 +841,10 @@ static cudaError_t launch_bwd(const void* qkv, const float* qw, const float* kw,
   } while (0)
 
 cudaError_t window_attn_fwd(const void* qkv, const float* qw, const float* kw, void* out, float* lse,
-                            const AttnGeom& g, int dtype, cudaStream_t s, const AttnBias& bias) {
+                            const AttnGeom& g, int dtype, cudaStream_t s) {
   const int L = g.T * g.wh * g.ww;
   if (L > 192 || L <= 0 || g.H % g.wh || g.W % g.ww) return cudaErrorInvalidValue;
-  NSW_ATTN_DISPATCH(launch_fwd, qkv, qw, kw, out, lse, g, s, bias);
+  NSW_ATTN_DISPATCH(launch_fwd, qkv, qw, kw, out, lse, g, s);
 }
 
 cudaError_t window_attn_bwd(const void* qkv, const float* qw, const float* kw, const void* out,
@@ -948,7 +852,7 @@ cudaError_t window_attn_bwd(const void* qkv, const float* qw, const float* kw, c
                             float* dkw_part, const AttnGeom& g, int dtype, cudaStream_t s, const AttnBias& bias,
                             float* dbias_part) {
   const int L = g.T * g.wh * g.ww;
-  if (L > 192 || L <= 0 || g.H % g.wh || g.W % g.ww) return cudaErrorInvalidValue;
+  if (L > 192 || L <= 0 || g.H % g.wh || g.W % g.ww || (bias.tab && g.hd != 128)) return cudaErrorInvalidValue;
   NSW_ATTN_DISPATCH(launch_bwd, qkv, qw, kw, out, dout, lse, dqkv, dqw_part, dkw_part, g, s, bias, dbias_part);
 }
 

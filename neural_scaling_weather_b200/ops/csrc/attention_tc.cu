@@ -206,59 +206,6 @@ struct __align__(1024) SmemB {
   uint32_t tmem_base;
 };
 
-// With a bias: the head's entries, each row's offset in them, and the accumulators of the bias's gradient.
-//
-// The bias of query row r and key row j is tab[bias_center + off(r) - off(j)] with off of a token (t, y, x) =
-// (t (2 wh - 1) + y) pitch + x.  Its gradient sums dS over the windows and over the pairs of equal displacement.  One of
-// y and x, `a`, is summed at once and the other, `b`, kept as a pair, acc[dt][da][b_i][b_j], so that neither rows nor
-// keys have to be turned: entry e belongs to one thread, which walks the pairs down a column of dS in shared memory
-// (bf16, as the dK and dQ products read it) while those products run.  Items go through the windows of one head after
-// another, so acc stays for a head's windows and its diagonals b_i - b_j are summed once, in order: no atomics.
-constexpr int kBiasAcc = 4232;  // entries: at most 4225, of 13 x 13 tokens
-struct SmemBB : SmemB {
-  alignas(16) float tab[kAttnBiasRow];
-  float acc[kBiasAcc];
-  float ll[MAXL];                // log2 of the row's sum (lse: its largest logit)
-  alignas(16) short off[2][MAXL];            // of smem row j
-  short row_of[2][MAXL];         // smem row of window token i
-  unsigned short key_at[2][MAXL];  // byte of window token i's column in a row of ps, before the swizzle
-};
-struct BiasShape {
-  bool y;                      // a is the latitude
-  int na, nb, sa, sb, nt, wa;  // extents and window-order strides of a and b; time steps and tokens of one
-  int entries;
-  uint32_t div_nb, div_na;     // ceil(2^32 / divisor); 0 for one
-};
-__host__ __device__ __forceinline__ BiasShape bias_shape(const AttnGeom& g) {
-  BiasShape b;
-  // the axis that leaves fewer entries is summed
-  const bool y = (2 * g.wh - 1) * g.ww * g.ww <= (2 * g.ww - 1) * g.wh * g.wh;
-  b.y = y;
-  b.na = y ? g.wh : g.ww;
-  b.nb = y ? g.ww : g.wh;
-  b.sa = y ? g.ww : 1;
-  b.sb = y ? 1 : g.ww;
-  b.nt = g.T;
-  b.wa = g.wh * g.ww;
-  b.entries = (2 * g.T - 1) * (2 * b.na - 1) * b.nb * b.nb;
-  b.div_nb = b.nb == 1 ? 0u : (uint32_t)(((1ull << 32) + b.nb - 1) / b.nb);
-  b.div_na = b.na == 1 ? 0u : (uint32_t)(((1ull << 32) + 2 * b.na - 2) / (2 * b.na - 1));
-  return b;
-}
-__host__ __device__ __forceinline__ int bias_buckets(const AttnGeom& g) {
-  return (2 * g.T - 1) * (2 * g.wh - 1) * (2 * g.ww - 1);
-}
-// v / d for v < 2^16
-__device__ __forceinline__ int quick_div(int v, uint32_t magic) { return magic ? (int)__umulhi((uint32_t)v, magic) : v; }
-
-__device__ __forceinline__ int bias_off(const AttnGeom& g, int pitch, int i) {
-  const int wa = g.wh * g.ww, t = i / wa, r = i - t * wa, y = r / g.ww;
-  return (t * (2 * g.wh - 1) + y) * pitch + (r - y * g.ww);
-}
-__device__ __forceinline__ int bias_center(const AttnGeom& g, int pitch) {
-  return 4 + ((g.T - 1) * (2 * g.wh - 1) + g.wh - 1) * pitch + g.ww - 1;
-}
-
 __device__ __forceinline__ uint64_t desc_mn(const void* p, uint32_t lbo_bytes) {
   const uint32_t a = smem_u32(p);
   return (uint64_t)((a >> 4) & 0x3FFF) | ((uint64_t)((lbo_bytes >> 4) & 0x3FFF) << 16) |
@@ -376,46 +323,6 @@ __device__ __forceinline__ void ld_cols<3>(uint32_t taddr, float* f) {
   for (int i = 0; i < 48; ++i) f[i] = __uint_as_float(r[i]);
 }
 
-// acc += dS of the tile's rows [lo, hi) (smem rows; the tile's first is qb)
-__device__ __forceinline__ void bias_accumulate(SmemBB& S, const BiasShape& b, int tab, int qb, int lo, int hi) {
-  const short* row_of = S.row_of[tab];
-  const unsigned short* key_at = S.key_at[tab];
-  for (int e = threadIdx.x; e < b.entries; e += BWD_THREADS) {
-    const int e1 = quick_div(e, b.div_nb), bj = e - e1 * b.nb, e2 = quick_div(e1, b.div_nb), bi = e1 - e2 * b.nb;
-    const int e3 = quick_div(e2, b.div_na), da = e2 - e3 * (2 * b.na - 1) - (b.na - 1), dt = e3 - (b.nt - 1);
-    const int n = b.na - abs(da);
-    float sum = 0.f;
-    for (int t = max(dt, 0); t < b.nt + min(dt, 0); ++t) {
-      const short* ri = row_of + t * b.wa + max(da, 0) * b.sa + bi * b.sb;
-      const unsigned short* kj = key_at + (t - dt) * b.wa + max(-da, 0) * b.sa + bj * b.sb;
-#pragma unroll 4
-      for (int k = 0; k < n; ++k) {
-        const int r = ri[k * b.sa];
-        if (r < lo || r >= hi) continue;
-        const uint32_t at = (uint32_t)((r - qb) * ROW_B) + ((uint32_t)kj[k * b.sa] ^ ((uint32_t)(r & 7) << 4));
-        sum += __uint_as_float((uint32_t)*reinterpret_cast<const unsigned short*>(S.ps + at) << 16);
-      }
-    }
-    S.acc[e] += sum;
-  }
-}
-// the head's buckets from the accumulators, which start anew; block barriers
-__device__ __forceinline__ void bias_flush(SmemBB& S, const BiasShape& b, const AttnGeom& g, float* out) {
-  __syncthreads();
-  const int ny = 2 * g.wh - 1, nx = 2 * g.ww - 1;
-  for (int c = threadIdx.x; c < (2 * g.T - 1) * ny * nx; c += BWD_THREADS) {
-    const int dt = c / (ny * nx), dy = c / nx - dt * ny, dx = c % nx;
-    const int da = b.y ? dy : dx, db = (b.y ? dx : dy) - (b.nb - 1);
-    const float* a = S.acc + (dt * (2 * b.na - 1) + da) * b.nb * b.nb + max(db, 0) * b.nb + max(-db, 0);
-    float sum = 0.f;
-    for (int i = 0; i < b.nb - abs(db); ++i) sum += a[i * (b.nb + 1)];
-    out[c] = sum;
-  }
-  __syncthreads();
-  for (int e = threadIdx.x; e < b.entries; e += BWD_THREADS) S.acc[e] = 0.f;
-  __syncthreads();
-}
-
 __device__ __forceinline__ float bf16_lo(uint32_t u) { return __uint_as_float(u << 16); }
 __device__ __forceinline__ float bf16_hi(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
 
@@ -447,43 +354,6 @@ __device__ __forceinline__ void p_chunks(uint32_t trow, SmemB& S, const signed c
           pr[e] = lk >= 0 ? ex2(s) : 0.f;
         }
         pk[i] = pack_bf16(pr[0], pr[1]);
-      }
-    }
-    *reinterpret_cast<uint4*>(S.ps + ps_off(rt, 16 * j)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
-    *reinterpret_cast<uint4*>(S.ps + ps_off(rt, 16 * j + 8)) = make_uint4(pk[4], pk[5], pk[6], pk[7]);
-  }
-}
-// The same with a bias: P = exp2(S * scale * log2e + bias + mask - max - log2 sum); `bias` is the row's center in tab.
-template <int NCH>
-__device__ __forceinline__ void p_chunks_bias(uint32_t trow, SmemBB& S, const signed char* lab, const short* off,
-                                              const float* bias, int rt, int c0, float mx, float ll, int lr, float sl2,
-                                              float ml2, int mixed, int L) {
-  float v[16 * NCH];
-  ld_cols<NCH>(trow + 16 * c0, v);
-#pragma unroll
-  for (int c = 0; c < NCH; ++c) {
-    const int j = c0 + c;
-    uint32_t pk[8];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const uint4 o4 = *reinterpret_cast<const uint4*>(off + 16 * j + 8 * h);
-      const uint32_t o[4] = {o4.x, o4.y, o4.z, o4.w};
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        float pr[2];
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const float b = bias[-(int)(e ? o[i] >> 16 : o[i] & 0xffffu)];
-          pr[e] = fmaf(v[16 * c + 8 * h + 2 * i + e], sl2, b);
-        }
-        if (mixed || 16 * j + 16 > L) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int lk = lab[16 * j + 8 * h + 2 * i + e];
-            pr[e] = lk < 0 ? -INFINITY : pr[e] + (lk != lr ? ml2 : 0.f);
-          }
-        }
-        pk[4 * h + i] = pack_bf16(ex2((pr[0] - mx) - ll), ex2((pr[1] - mx) - ll));
       }
     }
     *reinterpret_cast<uint4*>(S.ps + ps_off(rt, 16 * j)) = make_uint4(pk[0], pk[1], pk[2], pk[3]);
@@ -610,8 +480,7 @@ __device__ __forceinline__ void load_window(unsigned char* buf, const BoxMaps& m
 
 // Token rows and mask labels of window `w`; returns whether the window mixes labels.
 __device__ __forceinline__ int build_table(const AttnGeom& g, int64_t w, int nww, int nwh, int L, int* tok,
-                                           signed char* lab, int tid, short* wr = nullptr, SmemBB* bias = nullptr,
-                                           int pitch = 0, int tab = 0) {
+                                           signed char* lab, int tid, short* wr = nullptr) {
   WinPos p;
   p.wx = (int)(w % nww);
   p.wy = (int)((w / nww) % nwh);
@@ -622,13 +491,6 @@ __device__ __forceinline__ int build_table(const AttnGeom& g, int64_t w, int nww
   for (int j = tid; j < MAXL; j += BWD_THREADS) {
     const int i = j < L ? win_row(g, wl, j) : 0;
     if (wr) wr[j] = (short)i;
-    if (bias) {
-      bias->off[tab][j] = j < L ? (short)bias_off(g, pitch, i) : 0;
-      if (j < L) {
-        bias->row_of[tab][i] = (short)j;
-        bias->key_at[tab][i] = (unsigned short)((j >> 6) * PS_BLOCK + (j & 63) * 2);
-      }
-    }
     tok[j] = j < L ? (int)token(g, p, i) : 0;
     const int lb = j < L ? label(g, p, i) : -1;
     lab[j] = (signed char)lb;
@@ -637,18 +499,14 @@ __device__ __forceinline__ int build_table(const AttnGeom& g, int64_t w, int nww
   return __syncthreads_or(mx);
 }
 
-static_assert(sizeof(SmemBB) + 1024 <= 232448, "shared memory of a block");
-
-template <bool BIAS>
 __global__ void __launch_bounds__(BWD_THREADS, 1)
     bwd_kernel(const __grid_constant__ BoxMaps box_qkv, const __grid_constant__ BoxMaps box_dout,
                const __nv_bfloat16* __restrict__ qkv, const float* __restrict__ qw, const float* __restrict__ kw,
                const __nv_bfloat16* __restrict__ dout, const float* __restrict__ lse,
                __nv_bfloat16* __restrict__ dqkv, float* __restrict__ dqw_part, float* __restrict__ dkw_part,
-               AttnGeom g, int* err, long long* __restrict__ stamps, AttnBias bias, float* __restrict__ dbias_part) {
+               AttnGeom g, int* err, long long* __restrict__ stamps) {
   extern __shared__ unsigned char smem_raw[];
   SmemB& S = *reinterpret_cast<SmemB*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  SmemBB& SB = static_cast<SmemBB&>(S);  // (there with BIAS only)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int lg = warp & 3;   // TMEM lane quarter
   const int cg = warp >> 2;  // column group
@@ -657,14 +515,9 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   const int ntiles = (L + 127) / 128;
   const int nww = g.W / g.ww, nwh = g.H / g.wh;
   const int64_t C = (int64_t)g.nh * HD;
-  const int64_t n_win = (int64_t)g.B * nwh * nww, n_items = n_win * g.nh;
+  const int64_t n_items = (int64_t)g.B * nwh * nww * g.nh;
   const int64_t i_begin = n_items * blockIdx.x / gridDim.x;
   const int64_t i_end = n_items * (blockIdx.x + 1) / gridDim.x;
-  // an item's window and head: heads fastest, with a bias windows fastest (see SmemBB)
-  const auto win_of = [&](int64_t item) { return BIAS ? item % n_win : item / g.nh; };
-  const auto head_of = [&](int64_t item, int64_t w) { return BIAS ? (int)(item / n_win) : (int)(item - w * g.nh); };
-  const BiasShape bs = bias_shape(g);
-  const int center = BIAS ? bias_center(g, bias.pitch) : 0;
   // optional phase timestamps (SM clock) of the third item of the first CTAs; null in production
   long long* st_base = (stamps && blockIdx.x < 64) ? stamps + 32 * blockIdx.x : nullptr;
   long long* st = nullptr;
@@ -704,8 +557,6 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     (&S.wq[0][0])[i] = 0.f;
     (&S.wk[0][0])[i] = 0.f;
   }
-  if (BIAS)
-    for (int e = tid; e < bs.entries; e += BWD_THREADS) SB.acc[e] = 0.f;
   if (tid < HD) {
     S.qwv[tid] = qw[tid];
     S.kwv[tid] = kw[tid];
@@ -728,17 +579,14 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   bool ok = true;
   int raw = 0;   // index of the raw q/k buffers of the current item
   int tcur = 0;  // index of the current window's token table
-  int64_t win = win_of(i_begin);
+  int64_t win = i_begin / g.nh;
   int mixed = 0;
-  int tab_head = -1;        // BIAS: the head whose entries are in shared memory
-  float ll_next = 0.f;      // BIAS: with lse_next, the largest logit, the log2 of the row's sum
   bool ld_pending = false;  // a gather phase was issued and not yet waited for
   float lse_next = 0.f;     // lse of row tid of the next item, loaded a phase ahead
   if (i_begin < i_end) {
     ld_pending = true;
     // first item: its table and all four gathers
-    mixed = BIAS ? build_table(g, win, nww, nwh, L, S.tok[0], S.lab[0], tid, nullptr, &SB, bias.pitch, 0)
-                 : build_table(g, win, nww, nwh, L, S.tok[0], S.lab[0], tid);
+    mixed = build_table(g, win, nww, nwh, L, S.tok[0], S.lab[0], tid);
     const WinLoad wl = win_load(g, win, nww, nwh);
     if (tid == 0)
       asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&S.bar_ld)),
@@ -746,7 +594,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
                    : "memory");
     __syncthreads();
     if (lane == 0 && warp < 4) {
-      const int h0 = head_of(i_begin, win);
+      const int h0 = (int)(i_begin - win * g.nh);
       unsigned char* buf = warp == 0 ? S.qbuf[0] : warp == 1 ? S.kbuf[0] : warp == 2 ? S.v : S.dO;
       load_window(buf, warp < 3 ? box_qkv : box_dout, &S.bar_ld, (warp < 3 ? warp * (int)C : 0) + h0 * HD, wl, g);
     }
@@ -755,33 +603,22 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
   for (int64_t item = i_begin; item < i_end && ok; ++item) {
     st = (st_base && item == i_begin + 2) ? st_base : nullptr;
     NSW_STAMP();
-    const int h = head_of(item, win);
+    const int h = (int)(item - win * g.nh);
     const bool has_next = item + 1 < i_end;
-    const int64_t nwin = win_of(item + 1);
-    const int nh_ = head_of(item + 1, nwin);
+    const int64_t nwin = (item + 1) / g.nh;
+    const int nh_ = (int)(item + 1 - nwin * g.nh);
     const int ntab = nwin == win ? tcur : 1 - tcur;
     int mixed_n = mixed;
     const int* tok = S.tok[tcur];
     const signed char* lab = S.lab[tcur];
-    if (BIAS && h != tab_head) {  // (the last item's readers are behind a barrier)
-      if (tab_head >= 0 && dbias_part) bias_flush(SB, bs, g, dbias_part + (blockIdx.x + tab_head) * (int64_t)bias_buckets(g));
-      for (int i = tid; i < bias.stride; i += BWD_THREADS) SB.tab[i] = bias.tab[(int64_t)h * bias.stride + i];
-      tab_head = h;
-    }
     unsigned char* qx = S.qbuf[raw];       // raw q
     unsigned char* qn = S.qbuf[1 - raw];   // normalized q
     unsigned char* kx = S.kbuf[raw];
     unsigned char* kn = S.kbuf[1 - raw];
     // lse rows of this item (items are (window, head) in the forward's lse order; smem row j
     // holds window token win_row(j)); loaded during the previous item except for the first
-    // (BIAS: two values a row)
-    if (item == i_begin && tid < L) {
-      const int64_t at = (BIAS ? win * g.nh + h : item) * L + win_row(g, win_load(g, win, nww, nwh), tid);
-      lse_next = lse[BIAS ? 2 * at : at];
-      if (BIAS) ll_next = lse[2 * at + 1];
-    }
+    if (item == i_begin && tid < L) lse_next = lse[item * L + win_row(g, win_load(g, win, nww, nwh), tid)];
     if (tid < L) S.lse[tid] = lse_next;
-    if (BIAS && tid < L) SB.ll[tid] = ll_next;
     NSW_STAMP();
     ok = __syncthreads_and(warp == 0 ? wait_bar(&S.bar_ld, ld_parity, err) : true);
     ld_parity ^= 1;
@@ -855,14 +692,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         if (warp_live) {
           const float lse_r = rvalid ? S.lse[r] : INFINITY;
           const int lr = rvalid ? lab[r] : 0;
-          if (BIAS) {
-            const short* off = SB.off[tcur];
-            const float* row_bias = SB.tab + center + (rvalid ? off[r] : 0);
-            const float ll = rvalid ? SB.ll[r] : 0.f;
-            if (nch == 3) p_chunks_bias<3>(trow, SB, lab, off, row_bias, rt, c0, lse_r, ll, lr, sl2, ml2, mixed, L);
-            else if (nch == 2) p_chunks_bias<2>(trow, SB, lab, off, row_bias, rt, c0, lse_r, ll, lr, sl2, ml2, mixed, L);
-            else if (nch == 1) p_chunks_bias<1>(trow, SB, lab, off, row_bias, rt, c0, lse_r, ll, lr, sl2, ml2, mixed, L);
-          } else if (nch == 3) p_chunks<3>(trow, S, lab, rt, c0, lse_r, lr, sl2, ml2, mixed, L);
+          if (nch == 3) p_chunks<3>(trow, S, lab, rt, c0, lse_r, lr, sl2, ml2, mixed, L);
           else if (nch == 2) p_chunks<2>(trow, S, lab, rt, c0, lse_r, lr, sl2, ml2, mixed, L);
           else if (nch == 1) p_chunks<1>(trow, S, lab, rt, c0, lse_r, lr, sl2, ml2, mixed, L);
         } else {
@@ -898,9 +728,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
       fence_after();
       // v and dO are free once the last tile's dP/dV MMAs are done: gather the next item's
       if (t == ntiles - 1 && has_next) {
-        if (nwin != win)
-          mixed_n = BIAS ? build_table(g, nwin, nww, nwh, L, S.tok[ntab], S.lab[ntab], tid, nullptr, &SB, bias.pitch, ntab)
-                         : build_table(g, nwin, nww, nwh, L, S.tok[ntab], S.lab[ntab], tid);
+        if (nwin != win) mixed_n = build_table(g, nwin, nww, nwh, L, S.tok[ntab], S.lab[ntab], tid);
         if (tid == 0)
           asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(&S.bar_ld)),
                        "r"(4 * L * ROW_B)
@@ -910,11 +738,7 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         if (lane == 0 && (warp == 2 || warp == 3))
           load_window(warp == 2 ? S.v : S.dO, warp == 2 ? box_qkv : box_dout, &S.bar_ld,
                       (warp == 2 ? 2 * (int)C : 0) + nh_ * HD, win_load(g, nwin, nww, nwh), g);
-        if (tid < L) {
-          const int64_t at = (BIAS ? nwin * g.nh + nh_ : item + 1) * L + win_row(g, win_load(g, nwin, nww, nwh), tid);
-          lse_next = __ldg(lse + (BIAS ? 2 * at : at));
-          if (BIAS) ll_next = __ldg(lse + 2 * at + 1);
-        }
+        if (tid < L) lse_next = __ldg(lse + (item + 1) * L + win_row(g, win_load(g, nwin, nww, nwh), tid));
       }
       // ---- D = rowsum(P dP) (four column groups combined through smem), then
       // dS = P (dP - D) scale over P (rows of dead warps stay zero)
@@ -952,7 +776,6 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
         commit(&S.bar);
       }
       __syncwarp();
-      if (BIAS && dbias_part) bias_accumulate(SB, bs, tcur, qb, lo, min(qb + 128, L));  // while the products run
       ok = __syncthreads_and(warp == 0 ? wait_bar(&S.bar, parity, err) : true);
       parity ^= 1;
       if (!ok) break;
@@ -1043,8 +866,6 @@ __global__ void __launch_bounds__(BWD_THREADS, 1)
     mixed = mixed_n;
   }
 #undef NSW_STAMP
-  if (BIAS && dbias_part && ok && tab_head >= 0)
-    bias_flush(SB, bs, g, dbias_part + (blockIdx.x + tab_head) * (int64_t)bias_buckets(g));
   // after an error, let gathers still in flight land before the shared memory is released
   // (bounded; a second timeout is not recorded again)
   if (!ok && ld_pending && tid == 0) wait_bar(&S.bar_ld, ld_parity, nullptr);
@@ -1484,14 +1305,6 @@ struct __align__(1024) SmemWS {
   int abort;
 };
 
-// With a bias: the stage's head's entries (a bulk copy beside the rows) and its rows' offsets in them, in bytes
-struct SmemWSB : SmemWS {
-  alignas(16) float tab[WS_STAGES][kAttnBiasRow];
-  alignas(16) unsigned short off[WS_STAGES][MAXL + 16];
-};
-
-static_assert(sizeof(SmemWSB) + 1024 <= 232448, "shared memory of a block");
-
 __device__ __forceinline__ void mb_init(uint64_t* bar, uint32_t count) {
   asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count));
 }
@@ -1569,18 +1382,9 @@ __device__ __forceinline__ void ld_wait32(uint32_t* r) {
                : "memory");
 }
 
-// contiguous bytes (both addresses and the size multiples of 16) onto an mbarrier's transaction count
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
-                   smem_u32(dst)),
-               "l"(src), "r"(bytes), "r"(smem_u32(bar))
-               : "memory");
-}
-
 // Tables of window `w`'s smem rows, by one warp; returns whether the window mixes labels.
 __device__ __forceinline__ int ws_table(const AttnGeom& g, int64_t w, int nww, int nwh, int L, int* tok,
-                                        signed char* lab, short* wr, float (*kbias)[MAXL + 16], int lane,
-                                        unsigned short* off = nullptr, int pitch = 0) {
+                                        signed char* lab, short* wr, float (*kbias)[MAXL + 16], int lane) {
   WinPos p;
   p.wx = (int)(w % nww);
   p.wy = (int)((w / nww) % nwh);
@@ -1597,7 +1401,6 @@ __device__ __forceinline__ int ws_table(const AttnGeom& g, int64_t w, int nww, i
       lab[j] = (signed char)lb;
       tok[j] = j < L ? (int)token(g, p, i) : 0;
     }
-    if (off) off[j] = j < L ? (unsigned short)(4 * bias_off(g, pitch, i)) : 0;
     kbias[0][j] = lb < 0 ? -INFINITY : (lb != 0 ? ml2 : 0.f);
     kbias[1][j] = lb < 0 ? -INFINITY : (lb != 1 ? ml2 : 0.f);
     mx |= (j < L && lb != lab0);
@@ -1634,44 +1437,6 @@ __device__ __forceinline__ void ws_probs(const uint32_t* v, int c, int mixed, in
   st16(trow + (uint32_t)(c >> 1), pk);
 }
 
-// The logits of 32 columns with their bias (log2 units): `bias` points at the row's center in the entries, off holds the
-// keys' offsets in bytes, kb the mask (null: none of these columns is masked or padding)
-__device__ __forceinline__ void ws_biased(uint32_t* v, int c, float sl2, const float* bias, const unsigned short* off,
-                                          const float* kb) {
-#pragma unroll
-  for (int i = 0; i < 32; i += 8) {
-    const uint4 o4 = *reinterpret_cast<const uint4*>(off + c + i);
-    const uint32_t o[4] = {o4.x, o4.y, o4.z, o4.w};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const uint32_t at = j & 1 ? o[j >> 1] >> 16 : o[j >> 1] & 0xffffu;
-      const float b = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(bias) - at);
-      v[i + j] = __float_as_uint(fmaf(__uint_as_float(v[i + j]), sl2, b));
-    }
-  }
-  if (kb) {
-#pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const float4 b4 = *reinterpret_cast<const float4*>(kb + c + i);
-      v[i] = __float_as_uint(__uint_as_float(v[i]) + b4.x);
-      v[i + 1] = __float_as_uint(__uint_as_float(v[i + 1]) + b4.y);
-      v[i + 2] = __float_as_uint(__uint_as_float(v[i + 2]) + b4.z);
-      v[i + 3] = __float_as_uint(__uint_as_float(v[i + 3]) + b4.w);
-    }
-  }
-}
-// P = exp2(s - m) of 32 biased logits, as ws_probs
-__device__ __forceinline__ void ws_probs_biased(const uint32_t* v, int c, float m, uint32_t trow, float& l) {
-  uint32_t pk[16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) {
-    const float p0 = ex2(__uint_as_float(v[2 * i]) - m), p1 = ex2(__uint_as_float(v[2 * i + 1]) - m);
-    l += p0 + p1;
-    pk[i] = pack_bf16(p0, p1);
-  }
-  st16(trow + (uint32_t)(c >> 1), pk);
-}
-
 // The CTAs walk the windows column-major (window row fastest), so that every CTA's contiguous range
 // holds its share of the bottom window row, whose windows mix mask labels and cost more: in row-
 // major order a few CTAs got only such windows and finished last.  Returns the item index
@@ -1686,14 +1451,12 @@ __device__ __forceinline__ int64_t ws_item(const AttnGeom& g, int nww, int nwh, 
   return *win * g.nh + *h;
 }
 
-template <bool BIAS>
 __global__ void __launch_bounds__(WS_THREADS, 1)
     fwd_ws_kernel(const __grid_constant__ BoxMaps box_qkv, const float* __restrict__ qw, const float* __restrict__ kw,
                   __nv_bfloat16* __restrict__ out, float* __restrict__ lse, AttnGeom g, int* err,
-                  long long* __restrict__ stamps, AttnBias bias) {
+                  long long* __restrict__ stamps) {
   extern __shared__ unsigned char smem_raw[];
   SmemWS& S = *reinterpret_cast<SmemWS*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  SmemWSB& SB = static_cast<SmemWSB&>(S);  // (there with BIAS only)
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int L = g.T * g.wh * g.ww;
   const int NK = (L + 15) & ~15;
@@ -1767,16 +1530,14 @@ __global__ void __launch_bounds__(WS_THREADS, 1)
       int h;
       ws_item(g, nww, nwh, i_begin + n, &win, &h);
       if (win != tab_win[s]) {
-        const int mx = BIAS ? ws_table(g, win, nww, nwh, L, S.tok[s], S.lab[s], S.wr[s], S.kbias[s], lane, SB.off[s], bias.pitch)
-                            : ws_table(g, win, nww, nwh, L, S.tok[s], S.lab[s], S.wr[s], S.kbias[s], lane);
+        const int mx = ws_table(g, win, nww, nwh, L, S.tok[s], S.lab[s], S.wr[s], S.kbias[s], lane);
         if (lane == 0) S.mixed[s] = mx;
         tab_win[s] = win;
       }
       __threadfence_block();
       __syncwarp();
       if (lane == 0) {
-        mb_expect_tx(&S.loaded[s], (uint32_t)(3 * L * ROW_B) + (BIAS ? 4u * (uint32_t)bias.stride : 0u));
-        if (BIAS) bulk_load(SB.tab[s], bias.tab + (int64_t)h * bias.stride, 4u * (uint32_t)bias.stride, &S.loaded[s]);
+        mb_expect_tx(&S.loaded[s], (uint32_t)(3 * L * ROW_B));
         const WinLoad wl = win_load(g, win, nww, nwh);
         load_window(S.q[s], box_qkv, &S.loaded[s], h * HD, wl, g);
         load_window(S.k[s], box_qkv, &S.loaded[s], C + h * HD, wl, g);
@@ -1931,22 +1692,8 @@ __global__ void __launch_bounds__(WS_THREADS, 1)
           const int lr = r < L ? S.lab[s][r] : 0;
           const float* kb = S.kbias[s][lr > 0 ? 1 : 0];
           const float bound = sl2 * (r < L ? S.qn[s][r] : 0.f) * kmax;
-          // BIAS: the largest entry is 0, so the bound holds, and P stays normal if it is 48 with half the entries' range
-          const float* row_bias = BIAS ? SB.tab[s] + bias_center(g, bias.pitch) + (SB.off[s][r < L ? r : 0] >> 2) : nullptr;
-          const float spread = BIAS ? 0.5f * SB.tab[s][0] : 0.f;
-          if (__all_sync(0xffffffffu, bound + spread <= WS_MAX_BOUND)) {
+          if (__all_sync(0xffffffffu, bound <= WS_MAX_BOUND)) {
             m = bound;
-          } else if (BIAS) {
-#pragma unroll 1
-            for (int c = 0; c < NK; c += 32) {
-              uint32_t v[32];
-              ld32_async(trow + (uint32_t)c, v);
-              ld_wait32(v);
-              ws_biased(v, c, sl2, row_bias, SB.off[s], !mixed && c + 32 <= L ? nullptr : kb);
-#pragma unroll
-              for (int i = 0; i < 32; ++i) m = fmaxf(m, __uint_as_float(v[i]));
-            }
-            if (m == -INFINITY) m = 0.f;  // a row that the bias masks throughout: P = 0
           } else {
             // exact row max of the scaled, biased logits (scale > 0: the raw maximum of a chunk
             // without bias, scaled once at the end)
@@ -1978,12 +1725,7 @@ __global__ void __launch_bounds__(WS_THREADS, 1)
             uint32_t v[32];
             ld32_async(trow + (uint32_t)c, v);
             ld_wait32(v);
-            if (BIAS) {
-              ws_biased(v, c, sl2, row_bias, SB.off[s], !mixed && c + 32 <= L ? nullptr : kb);
-              ws_probs_biased(v, c, m, trow, l);
-            } else {
-              ws_probs(v, c, mixed, L, sl2, m, kb, trow, l);
-            }
+            ws_probs(v, c, mixed, L, sl2, m, kb, trow, l);
           }
           asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
         }
@@ -1998,7 +1740,7 @@ __global__ void __launch_bounds__(WS_THREADS, 1)
         if (stamper) WS_STAMP(n, 7 + 4 * t);
         fence_after();
         if (warp_live) {
-          const float il = BIAS && l == 0.f ? 0.f : 1.f / l;
+          const float il = 1.f / l;
           uint4* dst = reinterpret_cast<uint4*>(out + (int64_t)S.tok[s][live ? r : 0] * g.out_stride + (int64_t)h * HD);
 #pragma unroll
           for (int hf = 0; hf < 2; ++hf) {
@@ -2014,9 +1756,7 @@ __global__ void __launch_bounds__(WS_THREADS, 1)
               }
             }
           }
-          if (BIAS && live)
-            reinterpret_cast<float2*>(lse)[item * L + S.wr[s][r]] = make_float2(m, l == 0.f ? 0.f : __log2f(l));
-          if (!BIAS && live) lse[item * L + S.wr[s][r]] = m + __log2f(l);
+          if (live) lse[item * L + S.wr[s][r]] = m + __log2f(l);
         }
         fence_before();
         __syncwarp();
@@ -2103,10 +1843,9 @@ bool window_box_maps(attn_tc::BoxMaps* maps, const void* ptr, const AttnGeom& g,
 
 cudaError_t window_attn_bwd_tc(const void* qkv, const float* qw, const float* kw, const void* out,
                                const void* dout, const float* lse, void* dqkv, float* dqw_part, float* dkw_part,
-                               const AttnGeom& g, cudaStream_t s, long long* stamps, const AttnBias& bias,
-                               float* dbias_part) {
-  const size_t smem = (bias.tab ? sizeof(attn_tc::SmemBB) : sizeof(attn_tc::SmemB)) + 1024;
-  auto k = bias.tab ? attn_tc::bwd_kernel<true> : attn_tc::bwd_kernel<false>;
+                               const AttnGeom& g, cudaStream_t s, long long* stamps) {
+  const size_t smem = sizeof(attn_tc::SmemB) + 1024;
+  auto k = attn_tc::bwd_kernel;
   NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   int dev = 0, sms = 0;
   NSW_CUDA_CHECK(cudaGetDevice(&dev));
@@ -2122,15 +1861,15 @@ cudaError_t window_attn_bwd_tc(const void* qkv, const float* qw, const float* kw
   k<<<grid, attn_tc::BWD_THREADS, smem, s>>>(b_qkv, b_dout, (const __nv_bfloat16*)qkv, qw, kw,
                                              (const __nv_bfloat16*)dout, lse,
                                              (__nv_bfloat16*)dqkv, dqw_part, dkw_part, g, device_error_flag(),
-                                             stamps, bias, dbias_part);
+                                             stamps);
   return cudaGetLastError();
 }
 
 cudaError_t window_attn_fwd_ws(const void* qkv, const float* qw, const float* kw, void* out, float* lse,
-                               const AttnGeom& g, cudaStream_t s, long long* stamps, const AttnBias& bias) {
+                               const AttnGeom& g, cudaStream_t s, long long* stamps) {
   if (!(g.scale > 0.f)) return cudaErrorInvalidValue;  // the row max is taken on unscaled logits
-  const size_t smem = (bias.tab ? sizeof(attn_tc::SmemWSB) : sizeof(attn_tc::SmemWS)) + 1024;
-  auto k = bias.tab ? attn_tc::fwd_ws_kernel<true> : attn_tc::fwd_ws_kernel<false>;
+  const size_t smem = sizeof(attn_tc::SmemWS) + 1024;
+  auto k = attn_tc::fwd_ws_kernel;
   NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   int dev = 0, sms = 0;
   NSW_CUDA_CHECK(cudaGetDevice(&dev));
@@ -2142,7 +1881,7 @@ cudaError_t window_attn_fwd_ws(const void* qkv, const float* qw, const float* kw
   const int64_t items = (int64_t)g.B * (g.H / g.wh) * (g.W / g.ww) * g.nh;
   const int grid = (int)std::min<int64_t>(items, sms);
   k<<<grid, attn_tc::WS_THREADS, smem, s>>>(b_qkv, qw, kw, (__nv_bfloat16*)out, lse, g, device_error_flag(),
-                                            stamps, bias);
+                                            stamps);
   return cudaGetLastError();
 }
 

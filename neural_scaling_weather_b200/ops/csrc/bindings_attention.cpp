@@ -28,11 +28,7 @@ nsw::AttnGeom geom_of(const std::vector<int64_t>& gi, double scale, const Tensor
 }
 int64_t buckets_of(const nsw::AttnGeom& g) { return (int64_t)(2 * g.T - 1) * (2 * g.wh - 1) * (2 * g.ww - 1); }
 int64_t windows_of(const nsw::AttnGeom& g) { return (int64_t)g.B * (g.H / g.wh) * (g.W / g.ww); }
-bool tensor_cores(const nsw::AttnGeom& g, const Tensor& qkv) {
-  return nsw::window_attn_fwd_tc_supported(g, dt_code(qkv, "qkv")) && g.scale > 0;
-}
-
-// {out [tokens, heads * head_dim], lse, tab}: lse has two values a row (attention_bias.cu), tab what the kernels take of
+// {out [tokens, heads * head_dim], lse, tab}: lse has two values a row, tab what the kernels take of
 // the parameters
 std::vector<Tensor> attn_bias_fwd(const Tensor& qkv, const Tensor& qw, const Tensor& kw, const Tensor& rel_bias,
                                   const std::vector<int64_t>& gi, double scale) {
@@ -56,14 +52,9 @@ std::vector<Tensor> attn_bias_fwd(const Tensor& qkv, const Tensor& qw, const Ten
   float* norms = tab.data_ptr<float>() + (int64_t)g.nh * bias.stride;
   check(nsw::attn_bias_prepare(table, q, k, g, bias, tab.data_ptr<float>(), stream()), "attn_bias_prepare");
   bias.tab = tab.data_ptr<float>();
-  if (tensor_cores(g, qkv))
-    check(nsw::window_attn_fwd_ws(qkv.data_ptr(), norms, norms + g.hd, out.data_ptr(), lse.data_ptr<float>(), g, stream(),
-                                  nullptr, bias),
-          "window_attn_fwd_ws");
-  else
-    check(nsw::window_attn_fwd(qkv.data_ptr(), norms, norms + g.hd, out.data_ptr(), lse.data_ptr<float>(), g,
-                               dt_code(qkv, "qkv"), stream(), bias),
-          "window_attn_fwd");
+  check(nsw::attn_bias_fwd(qkv.data_ptr(), bias, norms, out.data_ptr(), lse.data_ptr<float>(), g, dt_code(qkv, "qkv"),
+                           stream()),
+        "window_attention");
   return {out, lse, tab};
 }
 
@@ -101,27 +92,20 @@ std::vector<Tensor> attn_bias_bwd(const Tensor& qkv, const Tensor& tab, const Te
     }
   }
   if (qkv.numel() == 0) return res;
-  const bool tc = tensor_cores(g, qkv);
-  const int sms = sm_count(qkv);
-  const int64_t items = windows_of(g) * g.nh, rows = tc ? std::min<int64_t>(items, sms) : items;
-  auto part = torch::empty({2 * rows * g.hd + (need[2] ? nsw::attn_bias_rows(g, tc, sms) * buckets_of(g) : 0)}, f32);
-  float* qp = part.data_ptr<float>();
-  float* kp = qp + rows * g.hd;
-  float* bp = need[2] ? kp + rows * g.hd : nullptr;
-  const float* norms = tab.data_ptr<float>() + (int64_t)g.nh * bias.stride;
   bias.tab = tab.data_ptr<float>();
-  if (tc)
-    check(nsw::window_attn_bwd_tc(qkv.data_ptr(), norms, norms + g.hd, out.data_ptr(), dout.data_ptr(),
-                                  lse.data_ptr<float>(), dqkv.data_ptr(), qp, kp, g, stream(), nullptr, bias, bp),
-          "window_attn_bwd_tc");
-  else
-    check(nsw::window_attn_bwd(qkv.data_ptr(), norms, norms + g.hd, out.data_ptr(), dout.data_ptr(), lse.data_ptr<float>(),
-                               dqkv.data_ptr(), qp, kp, g, dt_code(qkv, "qkv"), stream(), bias, bp),
-          "window_attn_bwd");
+  const int dtype = dt_code(qkv, "qkv");
+  const nsw::AttnBiasPlan plan = nsw::attn_bias_plan(g, bias, dtype, need[2], sm_count(qkv));
+  auto part = torch::empty({2 * plan.norm_rows * g.hd + (need[2] ? plan.bias_rows * buckets_of(g) : 0)}, f32);
+  float* qp = part.data_ptr<float>();
+  float* kp = qp + plan.norm_rows * g.hd;
+  float* bp = need[2] ? kp + plan.norm_rows * g.hd : nullptr;
+  check(nsw::attn_bias_bwd(qkv.data_ptr(), bias, tab.data_ptr<float>() + (int64_t)g.nh * bias.stride, out.data_ptr(),
+                           dout.data_ptr(), lse.data_ptr<float>(), dqkv.data_ptr(), qp, kp, bp, plan, g, dtype, stream()),
+        "window_attention backward");
   grad[0].part = qp;
   grad[1].part = kp;
   grad[2].part = bp;
-  check(nsw::attn_bias_grads(grad[2], grad[0], grad[1], rows, g, tc, sms, stream()), "attn_bias_grads");
+  check(nsw::attn_bias_grads(grad[2], grad[0], grad[1], plan, g, stream()), "window_attention parameter gradients");
   return res;
 }
 

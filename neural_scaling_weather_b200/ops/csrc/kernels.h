@@ -74,12 +74,13 @@ struct AttnGeom {
 };
 // Learned bias of the logits by head and displacement of query and key (tab null: none), as attn_bias_prepare leaves it:
 // for each head a row of `stride` floats, the first four a header ([0]: largest less smallest entry), then entry
-// (dt (2 wh - 1) + dy) pitch + dx, in units of log2 and less the head's largest one (a softmax does not see it).
+// (dt (2 wh - 1) + dy) pitch + dx (y_fast: (dt (2 ww - 1) + dx) pitch + dy), in units of log2 and less the head's largest one
+// (a softmax does not see it).
 struct AttnBias {
   const float* tab;
   int stride, pitch;
+  int y_fast, pair;  // the order of the tokens, and whether the kernels read entries by pairs (attention_bias.cu)
 };
-constexpr int kAttnBiasRow = 1160;  // floats of a row: at most (2 T - 1)(2 wh - 1)(2 ww - 1) = 1155 of 192 tokens
 AttnBias attn_bias_layout(const AttnGeom& g);
 // A vector or matrix of any type and strides
 struct AnyMatrix {
@@ -91,29 +92,37 @@ struct AnyMatrix {
 // weights of q and of k, hd floats each
 cudaError_t attn_bias_prepare(const AnyMatrix& table, const AnyMatrix& qw, const AnyMatrix& kw, const AttnGeom& g,
                               const AttnBias& b, float* tab, cudaStream_t s);
-// With a bias the forward writes two floats a row, (largest logit, log2 of the sum of exponentials less it), and the
-// backward reads them: their sum, the log-sum-exp, would lose the second where a row's logits are far from zero.
-// dbias_part: rows of partial sums of the bias's gradient (null: not wanted), attn_bias_rows(..) of them.
-int64_t attn_bias_rows(const AttnGeom& g, bool tc, int sms);
+// Window attention with a bias (16-bit types; head_dim 16, 32, 64 or 128; at most 192 tokens a window).  lse has two floats
+// a row, (what the exponentials are less, log2 of their sum): added up, they would lose the second where the logits are
+// far from zero.  norms: the weights of q and of k, as prepared.
+cudaError_t attn_bias_fwd(const void* qkv, const AttnBias& bias, const float* norms, void* out, float* lse,
+                          const AttnGeom& g, int dtype, cudaStream_t s);
+// Rows of partial sums that the backward leaves: of the norms' weights (hd floats each) and of the bias (buckets each)
+struct AttnBiasPlan {
+  int blocks, k_bufs;      // 0 blocks: head_dim 128, a block for each window and head
+  int64_t norm_rows, bias_rows;
+};
+AttnBiasPlan attn_bias_plan(const AttnGeom& g, const AttnBias& bias, int dtype, bool dbias, int sms);
+cudaError_t attn_bias_bwd(const void* qkv, const AttnBias& bias, const float* norms, const void* out, const void* dout,
+                          const float* lse, void* dqkv, float* dqw_part, float* dkw_part, float* dbias_part,
+                          const AttnBiasPlan& plan, const AttnGeom& g, int dtype, cudaStream_t s);
 // The parameters' gradients from their partial sums: out (null: not wanted) in dtype, or fp32 and added to.
 struct AttnGrad {
   const float* part;
   void* out;
   int dtype, add;
 };
-// bias: [nh][buckets]; q, k: [hd], from qk_rows rows of partial sums each
-cudaError_t attn_bias_grads(const AttnGrad& bias, const AttnGrad& q, const AttnGrad& k, int64_t qk_rows, const AttnGeom& g,
-                            bool tc, int sms, cudaStream_t s);
+cudaError_t attn_bias_grads(const AttnGrad& bias, const AttnGrad& q, const AttnGrad& k, const AttnBiasPlan& plan,
+                            const AttnGeom& g, cudaStream_t s);
 cudaError_t window_attn_fwd(const void* qkv, const float* qw, const float* kw, void* out, float* lse,
-                            const AttnGeom& g, int dtype, cudaStream_t s, const AttnBias& bias = {});
+                            const AttnGeom& g, int dtype, cudaStream_t s);
 // tcgen05/TMEM forward (bf16, head_dim 64, T*wh*ww <= 176); same outputs as window_attn_fwd
 bool window_attn_fwd_tc_supported(const AttnGeom& g, int dtype);
 cudaError_t window_attn_fwd_tc(const void* qkv, const float* qw, const float* kw, void* out, float* lse,
                                const AttnGeom& g, cudaStream_t s);
 // warp-specialised tcgen05 forward (same contract and support as window_attn_fwd_tc)
 cudaError_t window_attn_fwd_ws(const void* qkv, const float* qw, const float* kw, void* out, float* lse,
-                               const AttnGeom& g, cudaStream_t s, long long* stamps = nullptr,
-                               const AttnBias& bias = {});
+                               const AttnGeom& g, cudaStream_t s, long long* stamps = nullptr);
 // RMSNorm, one warp per row with the row in registers (n <= 2048); rmsnorm_fwd/bwd use the TMA
 // version below where it applies and these otherwise
 cudaError_t rmsnorm_fwd_rows(const void* x, const float* w, void* y, float* rstd, int64_t rows, int n,
@@ -132,8 +141,9 @@ cudaError_t rmsnorm_bwd_tma(const void* dy, const void* x, const float* w, const
 // dqw_part / dkw_part: one row of head_dim partial sums per CTA, min(items, SM count) rows
 cudaError_t window_attn_bwd_tc(const void* qkv, const float* qw, const float* kw, const void* out,
                                const void* dout, const float* lse, void* dqkv, float* dqw_part, float* dkw_part,
-                               const AttnGeom& g, cudaStream_t s, long long* stamps = nullptr,
-                               const AttnBias& bias = {}, float* dbias_part = nullptr);
+                               const AttnGeom& g, cudaStream_t s, long long* stamps = nullptr);
+// bias (head_dim 128 alone): lse as attn_bias_fwd leaves it; dbias_part (null: not wanted): a row of the bias's buckets
+// for each head and window
 cudaError_t window_attn_bwd(const void* qkv, const float* qw, const float* kw, const void* out,
                             const void* dout, const float* lse, void* dqkv, float* dqw_part,
                             float* dkw_part, const AttnGeom& g, int dtype, cudaStream_t s,

@@ -160,7 +160,8 @@ def test_bias_of_any_size(dtype, hd):
 def test_bias_of_zero_is_none_and_types_are_kept():
     qkv, qw, kw, table, geom, dout = inputs(1, 1, 2, 2, 9, 18, 4, 64, BF, True, seed=5)
     plain = ops.window_attention(qkv, qw, kw, 4, 64, geom, 0.125)
-    assert rel(ops.window_attention(qkv, qw, kw, 4, 64, geom, 0.125, rel_bias=torch.zeros_like(table)), plain) < 2 * U[BF]
+    # two kernels that share no rounding, each within 6 u of the definition: 6 + 6
+    assert rel(ops.window_attention(qkv, qw, kw, 4, 64, geom, 0.125, rel_bias=torch.zeros_like(table)), plain) < 12 * U[BF]
     want = ops.window_attention(qkv, qw, kw, 4, 64, geom, 0.125, rel_bias=table)
     turned = table.t().contiguous().t()
     assert torch.equal(ops.window_attention(qkv, qw, kw, 4, 64, geom, 0.125, rel_bias=turned), want)
