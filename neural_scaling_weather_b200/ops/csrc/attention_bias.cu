@@ -8,6 +8,7 @@
 // A window is at most 192 tokens of one head, so its products are short: what counts is how few instructions stand around
 // them, and that several windows are worked on at once on an SM.
 #include <float.h>
+#include <limits.h>
 
 #include <algorithm>
 
@@ -24,6 +25,7 @@ using attn::kLog2e;
 using attn::ldsm_x4;
 using attn::ldsm_x4_t;
 using attn::mma16816;
+using attn::mma16816_from;
 using attn::pack2;
 using attn::stsm_x4;
 using attn::stsm_x4_t;
@@ -52,7 +54,7 @@ constexpr float kAbsorbs = 1099511627776.f;  // 2^40
 // costs no precision, unless that is beyond 2^40: a head of the lowest value throughout, say, absorbs the logits, as it
 // does in 64 bits, and its rows are even.  A finite entry stays finite.
 __global__ void __launch_bounds__(256) prepare_kernel(const AnyMatrix table, const AnyMatrix qw, const AnyMatrix kw, const AttnBias b,
-                                                      int heads, int hd, int nt, int ny, int nx,
+                                                      int heads, int hd, int nt, int ny, int nx, float scale,
                                                       float* __restrict__ tab) {
   __shared__ float hi_w[8], lo_w[8];
   const int h = blockIdx.x, n = nt * ny * nx;
@@ -81,12 +83,17 @@ __global__ void __launch_bounds__(256) prepare_kernel(const AnyMatrix table, con
     const float e = (v - shift) * kLog2e;
     return isinf(e) && !isinf(v) ? copysignf(FLT_MAX, e) : e;
   };
+  float most = 0.f;
+  for (int i = threadIdx.x & 31; i < hd; i += 32)
+    most = fmaxf(most, fabsf(load_any(qw.p, qw.dtype, i * qw.s0) * load_any(kw.p, kw.dtype, i * kw.s0)));
+  // (a margin for the roundings of q and k)
+  most = warp_max(most) * fabsf(scale) * (1.01f * kLog2e * (float)hd);
   const int nf = b.y_fast ? ny : nx, ns = b.y_fast ? nx : ny;
   for (int i = threadIdx.x; i < b.stride; i += 256) {
     const int at = i - 4, row = at / b.pitch, f = at - row * b.pitch, t = row / ns, s = row - t * ns;
     float v = 0.f;
     if (i == 0) {
-      v = shifted ? -entry(lo) : INFINITY;  // (the forward's bound on the logits needs the largest to be 0)
+      v = shifted ? most : INFINITY;  // (the bound needs the largest entry to be 0)
     } else if (at >= 0 && t < nt && f < nf) {
       const int y = b.y_fast ? f : s, x = b.y_fast ? s : f;
       v = entry(load_any(table.p, table.dtype, h * table.s0 + ((t * ny + y) * nx + x) * table.s1));
@@ -148,8 +155,12 @@ struct Order {
   bool y_fast;
   int pitch, entries;             // entry of query i and key j: center + off(i) - off(j)
   int center;
+  int nww, nwh;                   // windows across and down
+  int sh, sw;                     // the shifts, in [0, H) and [0, W)
+  int far;                        // rows of the shifted grid from here on are beyond the wrap
 };
-__host__ __device__ __forceinline__ Order order_of(const AttnGeom& g, const AttnBias& b) {
+static Order order_of(const AttnGeom& g, const AttnBias& b) {
+  const auto wrapped = [](int v, int n) { return (v % n + n) % n; };
   Order o;
   o.y_fast = b.y_fast != 0;
   o.nf = o.y_fast ? g.wh : g.ww;
@@ -160,87 +171,131 @@ __host__ __device__ __forceinline__ Order order_of(const AttnGeom& g, const Attn
   o.pitch = b.pitch;
   o.entries = (2 * g.T - 1) * (2 * o.ns - 1) * b.pitch;
   o.center = ((g.T - 1) * (2 * o.ns - 1) + o.ns - 1) * b.pitch + o.nf - 1;
+  o.nww = g.W / g.ww;
+  o.nwh = g.H / g.wh;
+  o.sh = wrapped(g.sh, g.H);
+  o.sw = wrapped(g.sw, g.W);
+  o.far = g.mask && g.mask_shift > 0 ? g.h_global - g.mask_shift - g.row_offset : INT_MAX;
   return o;
 }
-__device__ __forceinline__ int off_of(const Order& o, int i) {
-  const int s = i / o.nf, t = s / o.ns;
-  return (t * (2 * o.ns - 1) + s - t * o.ns) * o.pitch + i - s * o.nf;
+// A window's corner on the shifted grid (0 <= shift < extent) and on the grid of the wrap's mask
+struct Window {
+  int x, y, image;  // image: b T
+};
+__device__ __forceinline__ Window window_of(const AttnGeom& g, const Order& o, int win) {
+  const int row = win / o.nww, b = row / o.nwh;
+  return {(win - row * o.nww) * g.ww, (row - b * o.nwh) * g.wh, b * g.T};
 }
-// Grid token of window token i, and its side of the latitude wrap
-__device__ __forceinline__ int token_of(const AttnGeom& g, const Order& o, int64_t win, int i, int& side) {
-  const int nww = g.W / g.ww, nwh = g.H / g.wh;
-  const int wx = (int)(win % nww), wy = (int)((win / nww) % nwh), b = (int)(win / ((int64_t)nww * nwh));
-  const int r = i / o.nf, f = i - r * o.nf, t = r / o.ns, s = r - t * o.ns;
-  const int y = wy * g.wh + (o.y_fast ? f : s), x = wx * g.ww + (o.y_fast ? s : f);
-  int gy = (y + g.sh) % g.H, gx = (x + g.sw) % g.W;
-  if (gy < 0) gy += g.H;
-  if (gx < 0) gx += g.W;
-  side = g.mask && g.mask_shift > 0 && g.row_offset + y >= g.h_global - g.mask_shift;
-  return (int)((((int64_t)b * g.T + t) * g.H + gy) * g.W + gx);
+// the next window of the list
+__device__ __forceinline__ void next_window(const AttnGeom& g, Window& w) {
+  w.x += g.ww;
+  if (w.x < g.W) return;
+  w.x = 0;
+  w.y += g.wh;
+  if (w.y < g.H) return;
+  w.y = 0;
+  w.image = w.image + g.T == g.B * g.T ? 0 : w.image + g.T;
 }
-
+// Token i of the order: time, row and column in the window (i < 2^16; a quotient of halves is never close to a whole)
+__device__ __forceinline__ int3 place_of(const Order& o, int i) {
+  const int r = (int)__fdividef(i + 0.5f, (float)o.nf), f = i - r * o.nf;
+  const int t = (int)__fdividef(r + 0.5f, (float)o.ns), s = r - t * o.ns;
+  return make_int3(t, o.y_fast ? f : s, o.y_fast ? s : f);
+}
+__device__ __forceinline__ int off_of(const Order& o, const int3& p) {
+  return (p.x * (2 * o.ns - 1) + (o.y_fast ? p.z : p.y)) * o.pitch + (o.y_fast ? p.y : p.z);
+}
+// Grid token of a window's token
+__device__ __forceinline__ int token_of(const AttnGeom& g, const Order& o, const Window& w, const int3& p) {
+  int y = w.y + p.y + o.sh, x = w.x + p.z + o.sw;
+  if (y >= g.H) y -= g.H;
+  if (x >= g.W) x -= g.W;
+  return ((w.image + p.x) * g.H + y) * g.W + x;
+}
 // The entries of a head in shared memory, twice: a lane of the products has pairs of neighbouring tokens across and one
 // token down, whose entries are two neighbours in either order; if the fast extent and the pitch are even, the pair's
 // place has the parity of the token down, and one of the copies (the second begins one entry later) has it 8-byte
 // aligned, one load for two entries.  Their distance modulo the banks keeps the copies' reads apart.
 __host__ __device__ __forceinline__ int second_copy(int entries) { return (entries + 31) / 32 * 32 + 16; }
 __host__ __device__ __forceinline__ int table_floats(int entries) { return second_copy(entries) + (entries + 1) / 2 * 2; }
-__device__ __forceinline__ void load_table(float* tab, const AttnBias& b, int entries, int head) {
+// REVERSED: last entry first
+template <bool REVERSED>
+__device__ __forceinline__ void load_table(float* tab, const AttnBias& b, int entries, int head, float less) {
   const float* src = b.tab + (int64_t)head * b.stride + 4;
+  const int second = second_copy(entries);
+#pragma unroll 4
   for (int i = threadIdx.x; i < entries; i += blockDim.x) {
-    const float v = src[i];
-    tab[i] = v;
-    if (i > 0) tab[second_copy(entries) + i - 1] = v;
+    const float v = __ldg(src + i) - less;
+    const int at = REVERSED ? entries - 1 - i : i;
+    tab[at] = v;
+    if (at > 0) tab[second + at - 1] = v;
   }
 }
-// where the entry `base` and the next one are a pair
-__device__ __forceinline__ const float* pair_at(const float* tab, int entries, int base) {
-  return tab + (base & 1 ? second_copy(entries) - 1 : 0) + base;
+// shared-memory address of the entry `base`; with pairs, where it and the next one are a pair
+template <bool PAIR>
+__device__ __forceinline__ uint32_t entry_at(const float* tab, int entries, int base) {
+  return smem_u32(tab + (PAIR && (base & 1) ? second_copy(entries) - 1 : 0) + base);
 }
 
-// Eight entries of a 16 x 16 block of logits less `sub` of their row (DOWN: of their column), in the layout of mma's
-// results: c[j][e] for row r0 (e < 2) or r0 + 8 and column 8 j + 2 tq + (e & 1).
-//   rows are queries: entry = center + off(row) - off(column)      (ACROSS = -1)
-//   rows are keys:    entry = center + off(column) - off(row)      (ACROSS = +1)
-// row0 / row1: with pairs, pair_at(center +- off(row) (- 1 for rows of queries)), else tab + center +- off(row).
-// off4: the offsets in bytes.
-template <bool PAIR, int ACROSS>
-__device__ __forceinline__ void load_block(float (&v)[2][4], const float* row0, const float* row1, const int* off4,
-                                           int col, int tq) {
+__device__ __forceinline__ int2 lds_i2(uint32_t at) {
+  int2 v;
+  asm volatile("ld.shared.v2.s32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at));
+  return v;
+}
+__device__ __forceinline__ void lds_f2(uint32_t at, float& a, float& b) {
+  asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(a), "=f"(b) : "r"(at));
+}
+__device__ __forceinline__ void lds_f(uint32_t at, float& a) {
+  asm volatile("ld.shared.f32 %0, [%1];" : "=f"(a) : "r"(at));
+}
+
+// The eight entries of a 16 x 16 block of logits that a lane has, in the layout of mma's results: c[j][e] for row r0 (e < 2)
+// or r0 + 8 and column 8 j + 2 tq + (e & 1).  row0 / row1: addresses of the rows' entries for offset 0; off: address of the
+// offsets (in bytes) of this lane's columns of the block: columns 2 tq and 8 + 2 tq, or without pairs all four.  A row
+// of queries walks its entries backwards, so the forward has them reversed.
+template <bool PAIR>
+__device__ __forceinline__ void load_block(float (&c)[2][4], uint32_t row0, uint32_t row1, uint32_t off) {
+  if (PAIR) {
+    const int2 o = lds_i2(off);
+    lds_f2(row0 + o.x, c[0][0], c[0][1]);
+    lds_f2(row1 + o.x, c[0][2], c[0][3]);
+    lds_f2(row0 + o.y, c[1][0], c[1][1]);
+    lds_f2(row1 + o.y, c[1][2], c[1][3]);
+  } else {
+    const int2 o[2] = {lds_i2(off), lds_i2(off + 8)};
 #pragma unroll
-  for (int j = 0; j < 2; ++j) {
-    if (PAIR) {
-      const int o = ACROSS * off4[col + 8 * j + 2 * tq];
-      const float2 a = *reinterpret_cast<const float2*>(reinterpret_cast<const char*>(row0) + o);
-      const float2 b = *reinterpret_cast<const float2*>(reinterpret_cast<const char*>(row1) + o);
-      v[j][0] = ACROSS < 0 ? a.y : a.x;
-      v[j][1] = ACROSS < 0 ? a.x : a.y;
-      v[j][2] = ACROSS < 0 ? b.y : b.x;
-      v[j][3] = ACROSS < 0 ? b.x : b.y;
-    } else {
-      const int2 o = *reinterpret_cast<const int2*>(off4 + col + 8 * j + 2 * tq);
-      v[j][0] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(row0) + ACROSS * o.x);
-      v[j][1] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(row0) + ACROSS * o.y);
-      v[j][2] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(row1) + ACROSS * o.x);
-      v[j][3] = *reinterpret_cast<const float*>(reinterpret_cast<const char*>(row1) + ACROSS * o.y);
+    for (int j = 0; j < 2; ++j) {
+      lds_f(row0 + o[j].x, c[j][0]);
+      lds_f(row0 + o[j].y, c[j][1]);
+      lds_f(row1 + o[j].x, c[j][2]);
+      lds_f(row1 + o[j].y, c[j][3]);
     }
   }
 }
-// The latitude-wrap mask, and -inf for padding keys: side is 0 / 1, -1 for padding.  Rows are queries or (KEYS) keys.
-template <bool KEYS>
-__device__ __forceinline__ void mask_block(float (&v)[2][4], const signed char* side, int row, int col, int tq) {
-  const int s0 = side[row], s1 = side[row + 8];
+constexpr int kOffRow = 4;  // lanes' columns of a block: four times two (pairs) or four offsets
+template <bool PAIR>
+constexpr int off_bytes() {
+  return PAIR ? 8 : 16;
+}
+// the offset of token i (4 off) to where its block's lanes look for it
+template <bool PAIR>
+__device__ __forceinline__ void put_off(int* offs, int i, int off4) {
+  const int tile = i >> 4, c = i & 15, j = c >> 3, tq = (c & 7) >> 1;
+  if (PAIR) {
+    if (!(c & 1)) offs[(tile * kOffRow + tq) * 2 + j] = off4;
+  } else {
+    offs[(tile * kOffRow + tq) * 4 + 2 * j + (c & 1)] = off4;
+  }
+}
+// The latitude-wrap mask: side is 0 or 1 of each token, s0 / s1 of the rows
+__device__ __forceinline__ void mask_block(float (&c)[2][4], const float* side, float s0, float s1, int col, int tq) {
 #pragma unroll
-  for (int j = 0; j < 2; ++j)
+  for (int j = 0; j < 2; ++j) {
+    const float2 t = *reinterpret_cast<const float2*>(side + col + 8 * j + 2 * tq);
+    const float d[4] = {s0 - t.x, s0 - t.y, s1 - t.x, s1 - t.y};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int sr = e < 2 ? s0 : s1, sc = side[col + 8 * j + 2 * tq + (e & 1)];
-      const int key = KEYS ? sr : sc, query = KEYS ? sc : sr;
-      if (key < 0)
-        v[j][e] = -INFINITY;
-      else if (query >= 0 && key != query)
-        v[j][e] += -100.f * kLog2e;
-    }
+    for (int e = 0; e < 4; ++e) c[j][e] = fmaf(d[e] * d[e], -100.f * kLog2e, c[j][e]);
+  }
 }
 
 __device__ __forceinline__ uint32_t ld32(const void* p) { return __ldg(reinterpret_cast<const uint32_t*>(p)); }
@@ -253,22 +308,62 @@ __device__ __forceinline__ float quad_max(float v) {
   return fmaxf(v, __shfl_xor_sync(0xffffffffu, v, 2));
 }
 
-// a 16 x 16 block of A B^T: A in fragments, B's 16 rows at `rows` in shared memory (row stride RS)
-template <typename T, int HD, int RS>
-__device__ __forceinline__ void block_product(float (&c)[2][4], const uint32_t (&a)[HD / 16][4], const T* rows, int lane) {
-  const uint32_t at = smem_u32(rows + ((lane & 7) + (lane >> 4) * 8) * RS + ((lane >> 3) & 1) * 8);
+// 16 raw rows in the layout of an operand's fragments (element pairs of rows r0 and r0 + 8), zeros past the window
+template <typename T, int HD>
+__device__ __forceinline__ void raw_rows(uint32_t (&raw)[HD / 16][4], const T* base, int64_t stride, const int* tok, int row,
+                                         int length, int lane) {
+  const int r0 = row + (lane >> 2), r1 = r0 + 8;
+  const T* p0 = base + (int64_t)tok[r0] * stride + 2 * (lane & 3);
+  const T* p1 = base + (int64_t)tok[r1] * stride + 2 * (lane & 3);
+#pragma unroll
+  for (int ks = 0; ks < HD / 16; ++ks) {
+    raw[ks][0] = r0 < length ? ld32(p0 + ks * 16) : 0u;
+    raw[ks][1] = r1 < length ? ld32(p1 + ks * 16) : 0u;
+    raw[ks][2] = r0 < length ? ld32(p0 + ks * 16 + 8) : 0u;
+    raw[ks][3] = r1 < length ? ld32(p1 + ks * 16 + 8) : 0u;
+  }
+}
+// Lane's addresses of 16 rows in shared memory (row stride RS) as the second operand: of A B^T (the rows are B's), and of
+// P V (the rows are V's)
+template <typename T, int RS>
+__device__ __forceinline__ uint32_t rows_nt(const T* rows, int lane) {
+  return smem_u32(rows + ((lane & 7) + (lane >> 4) * 8) * RS + ((lane >> 3) & 1) * 8);
+}
+template <typename T, int RS>
+__device__ __forceinline__ uint32_t rows_nn(const T* rows, int lane) {
+  return smem_u32(rows + ((lane & 7) + ((lane >> 3) & 1) * 8) * RS + (lane >> 4) * 8);
+}
+// c (+)= a 16 x 16 block of A B^T, from `from` at first
+template <typename T, int HD>
+__device__ __forceinline__ void block_product(float (&c)[2][4], const float (&from)[2][4], const uint32_t (&a)[HD / 16][4],
+                                              uint32_t at) {
 #pragma unroll
   for (int ks = 0; ks < HD / 16; ++ks) {
     uint32_t b0, b1, b2, b3;
     ldsm_x4(at + ks * 32, b0, b1, b2, b3);
-    mma16816<T>(c[0], a[ks], b0, b1);
-    mma16816<T>(c[1], a[ks], b2, b3);
+    mma16816_from<T>(c[0], ks == 0 ? from[0] : c[0], a[ks], b0, b1);
+    mma16816_from<T>(c[1], ks == 0 ? from[1] : c[1], a[ks], b2, b3);
   }
 }
-// o += P V for 16 rows of P (one fragment) and the 16 rows of V at `rows`
-template <typename T, int HD, int RS>
-__device__ __forceinline__ void block_add(float (&o)[HD / 8][4], const uint32_t (&p)[4], const T* rows, int lane) {
-  const uint32_t at = smem_u32(rows + ((lane & 7) + ((lane >> 3) & 1) * 8) * RS + (lane >> 4) * 8);
+// Two such products side by side: four chains of instructions, of which each waits for the one before it, instead of two
+template <typename T, int HD>
+__device__ __forceinline__ void block_products(float (&c)[2][4], const float (&from)[2][4], const uint32_t (&a)[HD / 16][4],
+                                               uint32_t at, float (&c2)[2][4], const float (&from2)[2][4],
+                                               const uint32_t (&a2)[HD / 16][4], uint32_t at2) {
+#pragma unroll
+  for (int ks = 0; ks < HD / 16; ++ks) {
+    uint32_t b[4], b2[4];
+    ldsm_x4(at + ks * 32, b[0], b[1], b[2], b[3]);
+    ldsm_x4(at2 + ks * 32, b2[0], b2[1], b2[2], b2[3]);
+    mma16816_from<T>(c[0], ks == 0 ? from[0] : c[0], a[ks], b[0], b[1]);
+    mma16816_from<T>(c[1], ks == 0 ? from[1] : c[1], a[ks], b[2], b[3]);
+    mma16816_from<T>(c2[0], ks == 0 ? from2[0] : c2[0], a2[ks], b2[0], b2[1]);
+    mma16816_from<T>(c2[1], ks == 0 ? from2[1] : c2[1], a2[ks], b2[2], b2[3]);
+  }
+}
+// o += P V for 16 rows of P (one fragment) and 16 rows of V
+template <typename T, int HD>
+__device__ __forceinline__ void block_add(float (&o)[HD / 8][4], const uint32_t (&p)[4], uint32_t at) {
 #pragma unroll
   for (int d = 0; d < HD / 16; ++d) {
     uint32_t b0, b1, b2, b3;
@@ -307,59 +402,83 @@ __device__ __forceinline__ void store_rows(const T* rows, T* dst, int64_t stride
   }
 }
 
+// two fp32 numbers in one instruction
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 r;
+  asm("{\n .reg .b64 a, b, c;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mul.rn.f32x2 c, a, b;\n"
+      " mov.b64 {%0, %1}, c;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return r;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 r;
+  asm("{\n .reg .b64 a, b, c;\n mov.b64 a, {%2, %3};\n mov.b64 b, {%4, %5};\n mov.b64 c, {%6, %7};\n"
+      " fma.rn.f32x2 c, a, b, c;\n mov.b64 {%0, %1}, c;\n}"
+      : "=f"(r.x), "=f"(r.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack_pair(uint32_t w) {
+  float f[2];
+  unpack2(w, f, T());
+  return make_float2(f[0], f[1]);
+}
 // RMSNorm of one row by HD / 8 lanes, eight elements each: x * rs * w (w in shared memory); rs of the row
 template <typename T, int HD>
-__device__ __forceinline__ float norm_chunk(const uint4& raw, const float* w, uint4& out, float* norm2) {
-  float f[8], v[8];
-  unpack8<T>(raw, f);
-  float ss = 0.f;
+__device__ __forceinline__ float norm_chunk(const uint4& raw, const float* w, uint4& out) {
+  const float2 f[4] = {unpack_pair<T>(raw.x), unpack_pair<T>(raw.y), unpack_pair<T>(raw.z), unpack_pair<T>(raw.w)};
+  const float4 w0 = *reinterpret_cast<const float4*>(w), w1 = *reinterpret_cast<const float4*>(w + 4);
+  const float2 we[4] = {{w0.x, w0.y}, {w0.z, w0.w}, {w1.x, w1.y}, {w1.z, w1.w}};
+  float2 s2 = mul2(f[0], f[0]);
 #pragma unroll
-  for (int i = 0; i < 8; ++i) ss = fmaf(f[i], f[i], ss);
+  for (int i = 1; i < 4; ++i) s2 = fma2(f[i], f[i], s2);
+  float ss = s2.x + s2.y;
 #pragma unroll
   for (int o = 1; o < HD / 8; o <<= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
   const float rs = rsqrtf(ss * (1.f / HD) + FLT_EPSILON);
-  float n2 = 0.f;
+  uint32_t y[4];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    v[i] = f[i] * (rs * w[i]);
-    n2 = fmaf(v[i], v[i], n2);
+  for (int i = 0; i < 4; ++i) {
+    const float2 v = mul2(mul2(f[i], we[i]), make_float2(rs, rs));
+    y[i] = pack2<T>(v.x, v.y);
   }
-  out = pack8<T>(v);
-  if (norm2) {
-#pragma unroll
-    for (int o = 1; o < HD / 8; o <<= 1) n2 += __shfl_xor_sync(0xffffffffu, n2, o);
-    *norm2 = n2;
-  }
+  out = make_uint4(y[0], y[1], y[2], y[3]);
   return rs;
 }
 
-// A row's exponentials are taken less a bound on its logits where that keeps them normal in T: with the largest entry 0,
-// a logit is at most |q| max |k| and at least its negative less the entries' range.  bf16: results in [2^-96, 1]; fp16: in
-// [2^-14, 2^14].  Otherwise less the row's largest logit, for one more product of q and k.
+// The exponentials are taken less a bound on the window's logits, less `top`: with the largest entry 0, no logit is above
+// head_dim max_i |qw_i kw_i| scale (Cauchy and Schwarz, in the norm that the weights' products give), which the preparation
+// has left in the head's header.  So they are at most 2^top, the bound is in the entries before the products begin, and
+// nothing is looked up or subtracted for a row.  Rows far below the bound lose precision to their type's smallest numbers:
+// those whose sum is below `least` (in fp16, 192 numbers that are each off by at most 2^-25 are off by less than 2^-17 of it) make
+// their tile begin again with every row less its own largest logit, for one more product of q and k.
 template <typename T>
 struct Bound;
 template <>
 struct Bound<__nv_bfloat16> {
-  static constexpr float most = 48.f, top = 0.f;
+  static constexpr float top = 64.f, least = 8.0779357e-28f;  // 2^-90
 };
 template <>
 struct Bound<__half> {
-  static constexpr float most = 14.f, top = 14.f;
+  static constexpr float top = 14.f, least = 1.f;
 };
+constexpr float kMostBound = 1e4f;  // beyond it (or NaN): the second way at once
 
 // ----------------------------------------------------------------------------------------------------- forward
 // A block takes a window and head, a warp 16 queries at a time.  K is normalised into shared memory, V copied there; the
 // queries' fragments come straight from global memory and are normalised in registers, with scale and log2 e, so that
-// the first product, which begins with the entries less the row's bound, ends in the exponents themselves.  P goes from
+// the first product, which begins with the entries less the bound, ends in the exponents themselves.  P goes from
 // registers into the second product.  Nothing waits for a row's maximum, and several blocks share an SM, so that one's
 // loads and norms run beside the others' products.
 constexpr int kFwdWarps = 6;
 template <typename T, int HD>
 struct FwdSmem {
-  float *tab, *qw, *kw, *red;
+  float *tab, *qw, *kw;
   T *k, *v, *stage;
-  int *tok, *off4;
-  signed char* side;
+  int *tok, *off4, *offs;
+  float* side;
   __host__ __device__ size_t carve(unsigned char* base, const Order& o) {
     const int rows = o.tiles * 16, RS = HD + 8;
     Carve c{base, 0};
@@ -369,186 +488,116 @@ struct FwdSmem {
     stage = c.take<T>(16 * kFwdWarps * RS);
     tok = c.take<int>(rows);
     off4 = c.take<int>(rows);
+    offs = c.take<int>(rows);
     qw = c.take<float>(HD);  // with scale and log2 e
     kw = c.take<float>(HD);
-    red = c.take<float>(kFwdWarps);
-    side = c.take<signed char>(rows);
+    side = c.take<float>(rows);
     return c.at;
   }
 };
 template <typename T, int HD, bool PAIR>
 __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
     fwd_kernel(const T* __restrict__ qkv, const AttnBias bias, const float* __restrict__ norms, T* __restrict__ out,
-               float2* __restrict__ lse, const AttnGeom g) {
+               float2* __restrict__ lse, const __grid_constant__ AttnGeom g, const __grid_constant__ Order o) {
   constexpr int RS = HD + 8, KS = HD / 16, CH = HD / 8;
+  constexpr uint32_t kTile = 16 * RS * sizeof(T), kOffTile = kOffRow * off_bytes<PAIR>();
   extern __shared__ __align__(128) unsigned char smem[];
-  const Order o = order_of(g, bias);
   const int L = o.length, rows = o.tiles * 16, nthreads = blockDim.x, nw = nthreads / 32;
   FwdSmem<T, HD> S;
   S.carve(smem, o);
-  float *tab = S.tab, *qw = S.qw, *kw = S.kw, *red = S.red;
-  T *sK = S.k, *sV = S.v, *stage = S.stage;
-  int *tok = S.tok, *off4 = S.off4;
-  signed char* side = S.side;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gq = lane >> 2, tq = lane & 3;
-  const int head = blockIdx.x % g.nh;
-  const int64_t win = blockIdx.x / g.nh;
+  const int win = blockIdx.x / g.nh, head = blockIdx.x - win * g.nh;
   const int64_t C = (int64_t)g.nh * HD;
   const T* base = qkv + (int64_t)head * HD;
 
-  int mixed = 0;
-  {
-    int first;
-    token_of(g, o, win, 0, first);
-    for (int i = threadIdx.x; i < rows; i += nthreads) {
-      int s = -1;
-      tok[i] = i < L ? token_of(g, o, win, i, s) : 0;
-      off4[i] = i < L ? 4 * off_of(o, i) : 0;
-      side[i] = (signed char)s;
-      mixed |= i < L && s != first;
-    }
+  const float bound = bias.tab[(int64_t)head * bias.stride];
+  const bool exact = !(bound <= kMostBound);
+  const float less = exact ? 0.f : bound - Bound<T>::top;  // in the entries
+  const Window window = window_of(g, o, win);
+  const bool mixed = window.y < o.far && window.y + g.wh > o.far;
+  for (int i = threadIdx.x; i < rows; i += nthreads) {
+    const int3 p = place_of(o, i);
+    const int off4 = i < L ? 4 * off_of(o, p) : 0;
+    S.tok[i] = i < L ? token_of(g, o, window, p) : 0;
+    S.off4[i] = off4;
+    put_off<PAIR>(S.offs, i, off4);
+    S.side[i] = window.y + p.y >= o.far ? 1.f : 0.f;
   }
   for (int i = threadIdx.x; i < HD; i += nthreads) {
-    qw[i] = norms[i] * (g.scale * kLog2e);
-    kw[i] = norms[HD + i];
+    S.qw[i] = norms[i] * (g.scale * kLog2e);
+    S.kw[i] = norms[HD + i];
   }
-  mixed = __syncthreads_or(mixed);
-  // the first tile's raw queries, on their way under what follows
+  __syncthreads();
   uint32_t raw[KS][4];
-  const auto load_queries = [&](int qt) {
-    const int r0 = qt * 16 + gq, r1 = r0 + 8;
-    const T* p0 = base + (int64_t)tok[r0] * g.qkv_stride + 2 * tq;
-    const T* p1 = base + (int64_t)tok[r1] * g.qkv_stride + 2 * tq;
-#pragma unroll
-    for (int ks = 0; ks < KS; ++ks) {
-      raw[ks][0] = r0 < L ? ld32(p0 + ks * 16) : 0u;
-      raw[ks][1] = r1 < L ? ld32(p1 + ks * 16) : 0u;
-      raw[ks][2] = r0 < L ? ld32(p0 + ks * 16 + 8) : 0u;
-      raw[ks][3] = r1 < L ? ld32(p1 + ks * 16 + 8) : 0u;
-    }
-  };
-  if (warp < o.tiles) load_queries(warp);
+  if (warp < o.tiles)  // the first tile's raw queries, on their way under what follows
+    raw_rows<T, HD>(raw, base, g.qkv_stride, S.tok, warp * 16, L, lane);
   for (int i = threadIdx.x; i < rows * CH; i += nthreads) {
     const int r = i / CH, c = i % CH;
-    T* dst = sV + r * RS + 8 * c;
+    T* dst = S.v + r * RS + 8 * c;
     if (r < L)
-      cp_async16(dst, base + (int64_t)tok[r] * g.qkv_stride + 2 * C + 8 * c);
+      cp_async16(dst, base + (int64_t)S.tok[r] * g.qkv_stride + 2 * C + 8 * c);
     else
       *reinterpret_cast<uint4*>(dst) = make_uint4(0, 0, 0, 0);
   }
-  load_table(tab, bias, o.entries, head);
   // keys: the lanes of a row are neighbours, and a warp's rows are whole (32 is a multiple of CH)
-  float kmax = 0.f;
-  for (int i0 = 0; i0 < rows * CH; i0 += 4 * nthreads) {
-    uint4 x[4];
+  constexpr int kAhead = 8;
+  for (int i0 = 0; i0 < rows * CH; i0 += kAhead * nthreads) {
+    uint4 x[kAhead];
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kAhead; ++u) {
       const int i = i0 + u * nthreads + threadIdx.x, r = i / CH;
       x[u] = i < rows * CH && r < L
-                 ? __ldg(reinterpret_cast<const uint4*>(base + (int64_t)tok[r] * g.qkv_stride + C + 8 * (i % CH)))
+                 ? __ldg(reinterpret_cast<const uint4*>(base + (int64_t)S.tok[r] * g.qkv_stride + C + 8 * (i % CH)))
                  : make_uint4(0, 0, 0, 0);
     }
+    if (i0 == 0) load_table<true>(S.tab, bias, o.entries, head, less);  // (while the first keys arrive)
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kAhead; ++u) {
       const int i = i0 + u * nthreads + threadIdx.x;
-      float n2;
+      if (i0 + u * nthreads >= rows * CH) break;
       uint4 y;
-      norm_chunk<T, HD>(x[u], kw + 8 * (i % CH), y, &n2);
-      kmax = fmaxf(kmax, n2);
-      if (i < rows * CH) *reinterpret_cast<uint4*>(sK + (i / CH) * RS + 8 * (i % CH)) = y;
+      norm_chunk<T, HD>(x[u], S.kw + 8 * (i % CH), y);
+      if (i < rows * CH) *reinterpret_cast<uint4*>(S.k + (i / CH) * RS + 8 * (i % CH)) = y;
     }
   }
-  kmax = warp_max(kmax);
-  if (lane == 0) red[warp] = kmax;
   cp_async_wait_all();
   __syncthreads();
-  for (int w = 0; w < nw; ++w) kmax = fmaxf(kmax, red[w]);
-  kmax = sqrtf(kmax) * 1.01f;  // (a margin for the roundings of q and k)
-  const float spread = 0.5f * bias.tab[(int64_t)head * bias.stride];
 
+  const uint32_t k_at = rows_nt<T, RS>(S.k, lane), v_at = rows_nn<T, RS>(S.v, lane);
+  const uint32_t off_at = smem_u32(S.offs) + tq * off_bytes<PAIR>();
+  const int whole = mixed ? 0 : L / 16;  // tiles of keys without a mask
   for (int qt = warp; qt < o.tiles; qt += nw) {
-    if (qt != warp) load_queries(qt);
+    if (qt != warp) raw_rows<T, HD>(raw, base, g.qkv_stride, S.tok, qt * 16, L, lane);
     const int r0 = qt * 16 + gq, r1 = r0 + 8;
     uint32_t qa[KS][4];
-    float n0, n1;
     {
-      float s0 = 0.f, s1 = 0.f;
-      float f[2];
+      float2 x[KS][4], s0 = {0.f, 0.f}, s1 = {0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          unpack2(raw[ks][e], f, T());
-          float& s = e & 1 ? s1 : s0;
-          s = fmaf(f[0], f[0], fmaf(f[1], f[1], s));
+          x[ks][e] = unpack_pair<T>(raw[ks][e]);
+          float2& s = e & 1 ? s1 : s0;
+          s = fma2(x[ks][e], x[ks][e], s);
         }
-      const float rs0 = rsqrtf(quad_sum(s0) * (1.f / HD) + FLT_EPSILON);
-      const float rs1 = rsqrtf(quad_sum(s1) * (1.f / HD) + FLT_EPSILON);
-      s0 = s1 = 0.f;
+      const float rs0 = rsqrtf(quad_sum(s0.x + s0.y) * (1.f / HD) + FLT_EPSILON);
+      const float rs1 = rsqrtf(quad_sum(s1.x + s1.y) * (1.f / HD) + FLT_EPSILON);
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          unpack2(raw[ks][e], f, T());
-          const float2 w = *reinterpret_cast<const float2*>(qw + ks * 16 + (e >> 1) * 8 + 2 * tq);
+          const float2 w = *reinterpret_cast<const float2*>(S.qw + ks * 16 + (e >> 1) * 8 + 2 * tq);
           const float rs = e & 1 ? rs1 : rs0;
-          f[0] *= rs * w.x;
-          f[1] *= rs * w.y;
-          float& s = e & 1 ? s1 : s0;
-          s = fmaf(f[0], f[0], fmaf(f[1], f[1], s));
-          qa[ks][e] = pack2<T>(f[0], f[1]);
+          const float2 v = mul2(mul2(x[ks][e], w), make_float2(rs, rs));
+          qa[ks][e] = pack2<T>(v.x, v.y);
         }
-      n0 = sqrtf(quad_sum(s0));
-      n1 = sqrtf(quad_sum(s1));
     }
-    const int at0 = o.center + (off4[r0] >> 2), at1 = o.center + (off4[r1] >> 2);
-    const float* row0 = PAIR ? pair_at(tab, o.entries, at0 - 1) : tab + at0;
-    const float* row1 = PAIR ? pair_at(tab, o.entries, at1 - 1) : tab + at1;
-    const auto logits = [&](float (&c)[2][4], int kb, float m0, float m1) {
-      load_block<PAIR, -1>(c, row0, row1, off4, kb * 16, tq);
-      if (mixed || kb * 16 + 16 > L) mask_block<false>(c, side, r0, kb * 16, tq);
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        c[j][0] -= m0;
-        c[j][1] -= m0;
-        c[j][2] -= m1;
-        c[j][3] -= m1;
-      }
-      block_product<T, HD, RS>(c, qa, sK + kb * 16 * RS, lane);
-    };
-    float m0 = n0 * kmax, m1 = n1 * kmax;
-    bool late = false;  // a row of entries beyond kAbsorbs throughout: they absorb the product before they are subtracted
-    if (__all_sync(0xffffffffu, m0 + spread <= Bound<T>::most && m1 + spread <= Bound<T>::most)) {
-      m0 -= Bound<T>::top;
-      m1 -= Bound<T>::top;
-    } else {
-      m0 = m1 = -INFINITY;
-      for (int kb = 0; kb < o.tiles; ++kb) {
-        float c[2][4];
-        logits(c, kb, 0.f, 0.f);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          m0 = fmaxf(m0, fmaxf(c[j][0], c[j][1]));
-          m1 = fmaxf(m1, fmaxf(c[j][2], c[j][3]));
-        }
-      }
-      m0 = quad_max(m0);
-      m1 = quad_max(m1);
-      if (m0 == -INFINITY) m0 = 0.f;  // a row that the bias masks throughout: P = 0
-      if (m1 == -INFINITY) m1 = 0.f;
-      late = __any_sync(0xffffffffu, fabsf(m0) > kAbsorbs || fabsf(m1) > kAbsorbs);
-    }
-    // the rows' sums are those of the rounded values that are multiplied, by one more product (with ones): so a row's
-    // weights add up to one as they are, and the sum costs an instruction where eight additions would
-    float acc[CH][4], sum[4] = {0.f, 0.f, 0.f, 0.f};
-    const uint32_t ones = pack2<T>(1.f, 1.f);
-#pragma unroll
-    for (int d = 0; d < CH; ++d) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0.f;
-#pragma unroll 1
-    for (int kb = 0; kb < o.tiles; ++kb) {
-      float c[2][4];
-      logits(c, kb, late ? 0.f : m0, late ? 0.f : m1);
-      if (late) {
+    const int last = o.entries - 1 - o.center;
+    const uint32_t row0 = entry_at<PAIR>(S.tab, o.entries, last - (S.off4[r0] >> 2));
+    const uint32_t row1 = entry_at<PAIR>(S.tab, o.entries, last - (S.off4[r1] >> 2));
+    // f(logits less m0 / m1 of their rows, key tile) for all key tiles; late: subtracted after the product
+    const auto each_tile = [&](float m0, float m1, bool late, auto shifted, auto f) {
+      const auto subtract = [&](float (&c)[2][4]) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           c[j][0] -= m0;
@@ -556,7 +605,46 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
           c[j][2] -= m1;
           c[j][3] -= m1;
         }
+      };
+      const auto before = [&](float (&c)[2][4], int kb, auto masked) {
+        load_block<PAIR>(c, row0, row1, off_at + kb * kOffTile);
+        if (masked()) {
+          if (mixed) mask_block(c, S.side, S.side[r0], S.side[r1], kb * 16, tq);
+          if (kb * 16 + 16 > L) {  // padding keys
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (kb * 16 + 8 * j + 2 * tq + (e & 1) >= L) c[j][e] = -INFINITY;
+          }
+        }
+        if (shifted() && !late) subtract(c);
+      };
+      int kb = 0;
+#pragma unroll 1
+      for (; kb + 1 < whole; kb += 2) {
+        float c[2][4], d[2][4];
+        before(c, kb, std::false_type());
+        before(d, kb + 1, std::false_type());
+        block_products<T, HD>(c, c, qa, k_at + kb * kTile, d, d, qa, k_at + (kb + 1) * kTile);
+        if (shifted() && late) subtract(c), subtract(d);
+        f(c, kb);
+        f(d, kb + 1);
       }
+#pragma unroll 1
+      for (; kb < o.tiles; ++kb) {
+        float c[2][4];
+        before(c, kb, std::true_type());
+        block_product<T, HD>(c, c, qa, k_at + kb * kTile);
+        if (shifted() && late) subtract(c);
+        f(c, kb);
+      }
+    };
+    // the rows' sums are those of the rounded values that are multiplied, by one more product (with ones): so a row's
+    // weights add up to one as they are, and the sum costs an instruction where eight additions would
+    float acc[CH][4], sum[4];
+    const uint32_t ones = pack2<T>(1.f, 1.f);
+    const auto weights = [&](float (&c)[2][4], int kb) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
@@ -564,7 +652,34 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
       const uint32_t p[4] = {pack2<T>(c[0][0], c[0][1]), pack2<T>(c[0][2], c[0][3]), pack2<T>(c[1][0], c[1][1]),
                              pack2<T>(c[1][2], c[1][3])};
       mma16816<T>(sum, p, ones, ones);
-      block_add<T, HD, RS>(acc, p, sV + kb * 16 * RS, lane);
+      block_add<T, HD>(acc, p, v_at + kb * kTile);
+    };
+    const auto clear = [&]() {
+      sum[0] = sum[1] = sum[2] = sum[3] = 0.f;
+#pragma unroll
+      for (int d = 0; d < CH; ++d) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0.f;
+    };
+    float m0 = 0.f, m1 = 0.f;  // besides `less`
+    bool again = exact;
+    if (!exact) {
+      clear();
+      each_tile(0.f, 0.f, false, std::false_type(), weights);
+      again = __any_sync(0xffffffffu, sum[0] < Bound<T>::least || sum[2] < Bound<T>::least);
+    }
+    if (again) {
+      m0 = m1 = -INFINITY;
+      each_tile(0.f, 0.f, false, std::false_type(), [&](float (&c)[2][4], int) {
+        m0 = fmaxf(m0, fmaxf(fmaxf(c[0][0], c[0][1]), fmaxf(c[1][0], c[1][1])));
+        m1 = fmaxf(m1, fmaxf(fmaxf(c[0][2], c[0][3]), fmaxf(c[1][2], c[1][3])));
+      });
+      m0 = quad_max(m0);
+      m1 = quad_max(m1);
+      if (m0 == -INFINITY) m0 = 0.f;  // a row that the bias masks throughout: P = 0
+      if (m1 == -INFINITY) m1 = 0.f;
+      // rows of entries beyond kAbsorbs throughout absorb the product before they are subtracted
+      const bool late = __any_sync(0xffffffffu, fabsf(m0) > kAbsorbs || fabsf(m1) > kAbsorbs);
+      clear();
+      each_tile(m0, m1, late, std::true_type(), weights);
     }
     const float l0 = sum[0], l1 = sum[2];
     const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
@@ -576,15 +691,15 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
       acc[d][3] *= i1;
     }
     if (tq == 0) {
-      float2* at = lse + ((int64_t)win * g.nh + head) * L;
-      if (r0 < L) at[r0] = l0 == 0.f ? make_float2(0.f, 0.f) : make_float2(m0, log2f(l0));
-      if (r1 < L) at[r1] = l1 == 0.f ? make_float2(0.f, 0.f) : make_float2(m1, log2f(l1));
+      float2* at = lse + (int64_t)blockIdx.x * L;
+      if (r0 < L) at[r0] = l0 == 0.f ? make_float2(0.f, 0.f) : make_float2(m0 + less, __log2f(l0));
+      if (r1 < L) at[r1] = l1 == 0.f ? make_float2(0.f, 0.f) : make_float2(m1 + less, __log2f(l1));
     }
-    T* st = stage + warp * 16 * RS;
+    T* st = S.stage + warp * 16 * RS;
     __syncwarp();
     stage_rows<T, HD, RS>(st, acc, lane);
     __syncwarp();
-    store_rows<T, HD, RS>(st, out + (int64_t)head * HD, g.out_stride, tok, qt * 16, L, lane);
+    store_rows<T, HD, RS>(st, out + (int64_t)head * HD, g.out_stride, S.tok, qt * 16, L, lane);
   }
 }
 
@@ -601,15 +716,11 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
 // threads; the diagonals b_i - b_j are summed when the head is done, into the block's row for it.
 // The norms' backward takes the raw rows from global memory (L2) again, in the fragments' layout.
 struct BiasSums {
-  bool a_is_s;           // a: the slow extent
-  int na, nb, sa, sb;    // extents and strides in tokens
-  int entries, width;    // width: entries a thread's task has, neighbours in b_j
-  uint32_t div_b, div_b2, div_a;
+  bool a_is_s;         // a: the slow extent
+  int na, nb, sa, sb;  // extents and strides in tokens
+  int entries, width;  // width: entries of a place (b_i, b_j ..) that a thread has, neighbours in b_j
+  int places;          // of one (dt, da)
 };
-__host__ __device__ __forceinline__ uint32_t magic_of(int d) { return d == 1 ? 0u : (uint32_t)(((1ull << 32) + d - 1) / d); }
-__device__ __forceinline__ int quick_div(int v, uint32_t magic) {  // v / d for v < 2^16
-  return magic ? (int)__umulhi((uint32_t)v, magic) : v;
-}
 template <bool PAIR>
 __host__ __device__ __forceinline__ BiasSums sums_of(const Order& o) {
   BiasSums b;
@@ -620,18 +731,16 @@ __host__ __device__ __forceinline__ BiasSums sums_of(const Order& o) {
   b.sb = b.a_is_s ? 1 : o.nf;
   b.width = PAIR ? 2 : 1;
   b.entries = (2 * o.nt - 1) * (2 * b.na - 1) * b.nb * b.nb;
-  b.div_b = magic_of(b.nb / b.width);
-  b.div_b2 = magic_of(b.nb);
-  b.div_a = magic_of(2 * b.na - 1);
+  b.places = b.nb * (b.nb / b.width);
   return b;
 }
 
 template <typename T, int HD>
 struct BwdSmem {
-  float *tab, *acc, *sub, *late, *ll, *negD, *rq, *rk, *qw, *qn, *kw;
+  float *tab, *acc, *sub, *late, *ll, *negD, *rq, *rk, *qw, *qn, *kw, *kn;
   T *q, *v, *g, *k, *s;
-  int *tok, *off4;
-  signed char* side;
+  int *tok, *off4, *offs;
+  float* side;
   // entries: of the bias's sums; k_bufs: buffers for k (two, where there is room: the next item's keys arrive while this
   // one's are read)
   __host__ __device__ size_t carve(unsigned char* base, const Order& o, int entries, int k_bufs) {
@@ -646,6 +755,7 @@ struct BwdSmem {
     s = c.take<T>(rows * (rows + 8));  // dS, [query][key]
     tok = c.take<int>(2 * rows);
     off4 = c.take<int>(rows);
+    offs = c.take<int>(rows);
     sub = c.take<float>(rows);   // what the exponents are less: of each query
     late = c.take<float>(rows);  // wide rows: and after the product, first this, then this
     ll = c.take<float>(rows);
@@ -653,45 +763,32 @@ struct BwdSmem {
     rq = c.take<float>(rows);
     rk = c.take<float>(rows);
     qw = c.take<float>(HD);  // with scale and log2 e
-    qn = c.take<float>(HD);
+    qn = c.take<float>(HD);  // with scale
     kw = c.take<float>(HD);
-    side = c.take<signed char>(2 * rows);
+    kn = c.take<float>(HD);  // with ln 2
+    side = c.take<float>(2 * rows);
     return c.at;
   }
 };
 
-// 16 raw rows in the layout of an operand's fragments (element pairs of rows r0 and r0 + 8), zeros past the window
-template <typename T, int HD>
-__device__ __forceinline__ void raw_rows(uint32_t (&raw)[HD / 16][4], const T* base, int64_t stride, const int* tok, int row,
-                                         int length, int lane) {
-  const int r0 = row + (lane >> 2), r1 = r0 + 8;
-  const T* p0 = base + (int64_t)tok[r0] * stride + 2 * (lane & 3);
-  const T* p1 = base + (int64_t)tok[r1] * stride + 2 * (lane & 3);
-#pragma unroll
-  for (int ks = 0; ks < HD / 16; ++ks) {
-    raw[ks][0] = r0 < length ? ld32(p0 + ks * 16) : 0u;
-    raw[ks][1] = r1 < length ? ld32(p1 + ks * 16) : 0u;
-    raw[ks][2] = r0 < length ? ld32(p0 + ks * 16 + 8) : 0u;
-    raw[ks][3] = r1 < length ? ld32(p1 + ks * 16 + 8) : 0u;
-  }
-}
 // rows past the window become zeros (their places in shared memory hold zeros for good)
 template <typename T, int HD, int RS>
 __device__ __forceinline__ void stage_live(T* rows, float (&o)[HD / 8][4], int row, int length, int lane) {
-  const bool live0 = row + (lane >> 2) < length, live1 = row + (lane >> 2) + 8 < length;
+  if (row + 16 > length) {
+    const bool live0 = row + (lane >> 2) < length, live1 = row + (lane >> 2) + 8 < length;
 #pragma unroll
-  for (int d = 0; d < HD / 8; ++d) {
-    if (!live0) o[d][0] = o[d][1] = 0.f;
-    if (!live1) o[d][2] = o[d][3] = 0.f;
+    for (int d = 0; d < HD / 8; ++d) {
+      if (!live0) o[d][0] = o[d][1] = 0.f;
+      if (!live1) o[d][2] = o[d][3] = 0.f;
+    }
   }
   stage_rows<T, HD, RS>(rows, o, lane);
 }
-// A tile's gradient g (times `scale`) of y = x rs w becomes that of x, dx = rs w g - x rs^3 mean(w g x); sums gets the
-// tile's columns of g x rs: two of them a lane, after a butterfly over the rows that halves what a lane holds.
+// A tile's gradient g (times `scale`, which w holds too) of y = x rs w becomes that of x, dx = rs w g - x rs^3 mean(w g x);
+// sums gets the tile's columns of g x rs: two of them a lane, after a butterfly over the rows that halves what a lane holds.
 template <typename T, int HD>
 __device__ __forceinline__ void norm_backward(float (&g)[HD / 8][4], const uint32_t (&raw)[HD / 16][4], const float* w,
-                                              float scale, float rs0, float rs1, bool live0, bool live1, float (&sums)[2],
-                                              int lane) {
+                                              float scale, float rs0, float rs1, float (&sums)[2], int lane) {
   constexpr int CH = HD / 8;
   const int tq = lane & 3;
   float dot0 = 0.f, dot1 = 0.f, c[2 * CH];
@@ -704,10 +801,9 @@ __device__ __forceinline__ void norm_backward(float (&g)[HD / 8][4], const uint3
     const float we[2] = {wd.x, wd.y};
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
-      const float g0 = live0 ? g[d][e] * scale : 0.f, g1 = live1 ? g[d][2 + e] * scale : 0.f;
-      c[2 * d + e] = fmaf(g0 * x0[e], rs0, g1 * x1[e] * rs1);
-      g[d][e] = g0 * we[e];
-      g[d][2 + e] = g1 * we[e];
+      c[2 * d + e] = fmaf(g[d][e] * x0[e], rs0, g[d][2 + e] * x1[e] * rs1);
+      g[d][e] *= we[e];
+      g[d][2 + e] *= we[e];
       dot0 = fmaf(g[d][e], x0[e], dot0);
       dot1 = fmaf(g[d][2 + e], x1[e], dot1);
     }
@@ -740,8 +836,8 @@ __device__ __forceinline__ void norm_backward(float (&g)[HD / 8][4], const uint3
       c[1] += __shfl_xor_sync(0xffffffffu, c[1], o);
     }
   }
-  sums[0] += c[0];
-  sums[1] += c[1];
+  sums[0] = fmaf(c[0], scale, sums[0]);
+  sums[1] = fmaf(c[1], scale, sums[1]);
 }
 // the columns that norm_backward left with this lane (where lanes hold the same ones, they are equal)
 template <int HD>
@@ -758,30 +854,35 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
     bwd_kernel(const T* __restrict__ qkv, const AttnBias bias, const float* __restrict__ norms, const T* __restrict__ out,
                const T* __restrict__ dout, const float2* __restrict__ lse, T* __restrict__ dqkv,
                float* __restrict__ dqw_part, float* __restrict__ dkw_part, float* __restrict__ dbias_part, int k_bufs,
-               const AttnGeom g) {
+               const __grid_constant__ AttnGeom g, const __grid_constant__ Order o) {
   constexpr int RS = HD + 8, KS = HD / 16, CH = HD / 8;
+  constexpr uint32_t kTile = 16 * RS * sizeof(T), kOffTile = kOffRow * off_bytes<PAIR>();
   extern __shared__ __align__(128) unsigned char smem[];
-  const Order o = order_of(g, bias);
   const BiasSums bs = sums_of<PAIR>(o);
   const int L = o.length, rows = o.tiles * 16, DS = rows + 8, nthreads = blockDim.x;
   const int buckets = (2 * g.T - 1) * (2 * g.wh - 1) * (2 * g.ww - 1);
   BwdSmem<T, HD> S;
   S.carve(smem, o, dbias_part ? bs.entries : 0, k_bufs);
   float *tab = S.tab, *acc = S.acc, *sub = S.sub, *late = S.late, *ll = S.ll, *negD = S.negD, *rq = S.rq, *rk = S.rk, *qw = S.qw,
-        *qn = S.qn, *kw = S.kw;
+        *qn = S.qn, *kw = S.kw, *kn = S.kn;
   T *sQ = S.q, *sV = S.v, *sG = S.g, *sK0 = S.k, *sS = S.s;
   int *tok2 = S.tok, *off4 = S.off4;
-  signed char* side2 = S.side;
+  float* side2 = S.side;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, gq = lane >> 2, tq = lane & 3;
   const int64_t C = (int64_t)g.nh * HD;
   const int64_t n_win = (int64_t)g.B * (g.H / g.wh) * (g.W / g.ww), n_items = n_win * g.nh;
   const int64_t i_begin = n_items * blockIdx.x / gridDim.x, i_end = n_items * (blockIdx.x + 1) / gridDim.x;
 
-  for (int i = threadIdx.x; i < rows; i += nthreads) off4[i] = i < L ? 4 * off_of(o, i) : 0;
+  const int3 place = place_of(o, min((int)threadIdx.x, L - 1));  // of this thread's token
+  if (threadIdx.x < rows) {
+    off4[threadIdx.x] = threadIdx.x < L ? 4 * off_of(o, place) : 0;
+    put_off<PAIR>(S.offs, threadIdx.x, threadIdx.x < L ? 4 * off_of(o, place) : 0);
+  }
   for (int i = threadIdx.x; i < HD; i += nthreads) {
     qw[i] = norms[i] * (g.scale * kLog2e);
-    qn[i] = norms[i];
+    qn[i] = norms[i] * g.scale;
     kw[i] = norms[HD + i];
+    kn[i] = norms[HD + i] * 0.69314718055994530942f;
   }
   // padding rows stay zero: copies and staged rows write the window's rows alone
   for (int i = threadIdx.x; i < (rows - L) * CH * (3 + k_bufs); i += nthreads) {
@@ -790,27 +891,35 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
   }
   if (dbias_part)
     for (int i = threadIdx.x; i < bs.entries; i += nthreads) acc[i] = 0.f;
+  // this thread's part of the bias's sums (groups of threads, if there are several for all places)
+  const int groups = max(1, nthreads / bs.places);
+  const int my_group = groups > 1 ? threadIdx.x / bs.places : 0;
+  const int my_place = my_group >= groups ? bs.places : threadIdx.x - my_group * bs.places;
 
-  // the window's tokens and sides into table `buf`; its mix of sides by the caller's barrier
-  const auto build = [&](int64_t win, int buf) {
-    int first, mix = 0;
-    token_of(g, o, win, 0, first);
-    for (int i = threadIdx.x; i < rows; i += nthreads) {
-      int s = -1;
-      tok2[buf * rows + i] = i < L ? token_of(g, o, win, i, s) : 0;
-      side2[buf * rows + i] = (signed char)s;
-      mix |= i < L && s != first;
-    }
-    return mix;
+  // a window's tokens and sides into table `buf`
+  const auto build = [&](const Window& w, int buf) {
+    if (threadIdx.x >= rows) return;
+    const int at = buf * rows + threadIdx.x;
+    const bool live = threadIdx.x < L;
+    tok2[at] = live ? token_of(g, o, w, place) : 0;
+    side2[at] = w.y + place.y >= o.far ? 1.f : 0.f;
   };
-  // one operand's rows of an item
-  const auto copy = [&](T* dst, const T* src, int64_t stride, const int* tok) {
+  // an item's rows into shared memory: k's (where given a place), and the others'
+  const auto copy = [&](int head, const int* tok, T* k, bool others) {
+    const T* src = qkv + (int64_t)head * HD;
+    const T* src_g = dout + (int64_t)head * HD;
     for (int i = threadIdx.x; i < L * CH; i += nthreads) {
-      const int r = i / CH, c = i % CH;
-      cp_async16(dst + r * RS + 8 * c, src + (int64_t)tok[r] * stride + 8 * c);
+      const int r = i / CH, c = i % CH, at = r * RS + 8 * c;
+      const int64_t t = tok[r];
+      const T* p = src + t * g.qkv_stride + 8 * c;
+      if (k) cp_async16(k + at, p + C);
+      if (others) {
+        cp_async16(sQ + at, p);
+        cp_async16(sV + at, p + 2 * C);
+        cp_async16(sG + at, src_g + t * g.out_stride + 8 * c);
+      }
     }
   };
-  const auto head_of = [&](int64_t item) { return (int)(item / n_win); };
   const auto flush = [&](int head) {  // the head's sums into the block's row for it; between barriers
     float* dst = dbias_part + ((int64_t)blockIdx.x + head) * buckets;
     const int ny = 2 * g.wh - 1, nx = 2 * g.ww - 1;
@@ -827,24 +936,20 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
     for (int i = threadIdx.x; i < bs.entries; i += nthreads) acc[i] = 0.f;
   };
 
-  int mix_next = 0, cur = 0, tab_head = -1;
+  int cur = 0, tab_head = -1;
+  int head = (int)(i_begin / n_win);
+  int64_t win = i_begin - head * n_win;  // of its head's
+  Window window = window_of(g, o, (int)win);
   if (i_begin < i_end) {
-    const int64_t win = i_begin % n_win;
-    mix_next = build(win, 0);
+    build(window, 0);
     __syncthreads();
-    const T* base = qkv + (int64_t)head_of(i_begin) * HD;
-    copy(sQ, base, g.qkv_stride, tok2);
-    copy(sK0, base + C, g.qkv_stride, tok2);
-    copy(sV, base + 2 * C, g.qkv_stride, tok2);
-    copy(sG, dout + (int64_t)head_of(i_begin) * HD, g.out_stride, tok2);
+    copy(head, tok2, sK0, true);
   }
   float wq[2] = {0.f, 0.f}, wk[2] = {0.f, 0.f};  // this lane's columns of the norms' weights' gradients
 
   for (int64_t item = i_begin; item < i_end; ++item) {
-    const int64_t win = item % n_win;
-    const int head = head_of(item);
     const int* tok = tok2 + cur * rows;
-    const signed char* side = side2 + cur * rows;
+    const float* side = side2 + cur * rows;
     T* sK = sK0 + (k_bufs > 1 ? cur * rows * RS : 0);
     const T* base = qkv + (int64_t)head * HD;
     const bool next = item + 1 < i_end;
@@ -859,28 +964,48 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
                             : make_uint4(0, 0, 0, 0);
     }
     float2 st = make_float2(INFINITY, 0.f);
-    if (threadIdx.x < L) st = lse[((int64_t)win * g.nh + head) * L + threadIdx.x];
-    const int mixed = __syncthreads_or(mix_next);  // (and the item before has been worked through)
+    if (threadIdx.x < L) st = lse[(win * g.nh + head) * L + threadIdx.x];
+    const bool mixed = window.y < o.far && window.y + g.wh > o.far;
+    // the item after
+    int head_n = head;
+    Window window_n = window;
+    int64_t win_n = win + 1;
+    next_window(g, window_n);
+    if (win_n == n_win) {
+      win_n = 0;
+      ++head_n;
+    }
+    __syncthreads();  // the item before has been worked through
     if (head != tab_head) {
       if (tab_head >= 0 && dbias_part) flush(tab_head);
-      load_table(tab, bias, o.entries, head);
+      load_table<false>(tab, bias, o.entries, head, 0.f);
       tab_head = head;
     }
     cp_async_wait_all();
     __syncthreads();
     // ---- norms in place, and D
-    for (int i0 = 0; i0 < 2 * rows * CH; i0 += nthreads) {
-      const int i = i0 + threadIdx.x;
-      const bool isk = i >= rows * CH;
-      const int j = isk ? i - rows * CH : i, r = j / CH, c = j % CH;
-      T* at = (isk ? sK : sQ) + r * RS + 8 * c;
-      const bool live = i < 2 * rows * CH;
-      uint4 y;
-      const uint4 x = live ? *reinterpret_cast<const uint4*>(at) : make_uint4(0, 0, 0, 0);
-      const float rs = norm_chunk<T, HD>(x, (isk ? kw : qw) + 8 * c, y, nullptr);
-      if (live) {
-        *reinterpret_cast<uint4*>(at) = y;
-        if (c == 0) (isk ? rk : rq)[r] = rs;
+    constexpr int kChunks = CH < 4 ? CH : 4;  // of a thread at once; it has CH (rows of q, then of k, two threads a token)
+#pragma unroll 1
+    for (int u0 = 0; u0 < CH; u0 += kChunks) {
+      uint4 x[kChunks];
+      T* at[kChunks];
+#pragma unroll
+      for (int u = 0; u < kChunks; ++u) {
+        const int i = (u0 + u) * nthreads + threadIdx.x;
+        const bool isk = i >= rows * CH;
+        const int j = isk ? i - rows * CH : i;
+        at[u] = (isk ? sK : sQ) + (j / CH) * RS + 8 * (j % CH);
+        x[u] = *reinterpret_cast<const uint4*>(at[u]);
+      }
+#pragma unroll
+      for (int u = 0; u < kChunks; ++u) {
+        const int i = (u0 + u) * nthreads + threadIdx.x;
+        const bool isk = i >= rows * CH;
+        const int j = isk ? i - rows * CH : i;
+        uint4 y;
+        const float rs = norm_chunk<T, HD>(x[u], (isk ? kw : qw) + 8 * (j % CH), y);
+        *reinterpret_cast<uint4*>(at[u]) = y;
+        if (j % CH == 0) (isk ? rk : rq)[j / CH] = rs;
       }
     }
 #pragma unroll
@@ -906,7 +1031,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
       ll[threadIdx.x] = st.y;
       if (threadIdx.x >= L) negD[threadIdx.x] = 0.f;
     }
-    if (next) mix_next = build((item + 1) % n_win, 1 - cur);
+    if (next) build(window_n, 1 - cur);
     __syncthreads();
 
     // ---- A
@@ -920,30 +1045,32 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
       for (int d = 0; d < CH; ++d)
 #pragma unroll
         for (int e = 0; e < 4; ++e) dv[d][e] = dk[d][e] = 0.f;
-      const int at0 = o.center - (off4[k0] >> 2), at1 = o.center - (off4[k0 + 8] >> 2);
-      const float* row0 = PAIR ? pair_at(tab, o.entries, at0) : tab + at0;
-      const float* row1 = PAIR ? pair_at(tab, o.entries, at1) : tab + at1;
-      const bool edge = mixed || warp * 16 + 16 > L;
+      const uint32_t row0 = entry_at<PAIR>(tab, o.entries, o.center - (off4[k0] >> 2));
+      const uint32_t row1 = entry_at<PAIR>(tab, o.entries, o.center - (off4[k0 + 8] >> 2));
+      const uint32_t off_at = smem_u32(S.offs) + tq * off_bytes<PAIR>();
+      const uint32_t q_nt = rows_nt<T, RS>(sQ, lane), q_nn = rows_nn<T, RS>(sQ, lane);
+      const uint32_t g_nt = rows_nt<T, RS>(sG, lane), g_nn = rows_nn<T, RS>(sG, lane);
+      const uint32_t sub_at = smem_u32(sub + 2 * tq), d_at = smem_u32(negD + 2 * tq);
       const uint32_t ds_at = smem_u32(sS + ((lane & 7) + (lane >> 4) * 8) * DS + warp * 16 + ((lane >> 3) & 1) * 8);
-#pragma unroll 1
-      for (int qb = 0; qb < o.tiles; ++qb) {
-        float s[2][4], dp[2][4];
-        load_block<PAIR, 1>(s, row0, row1, off4, qb * 16, tq);
-        if (edge) mask_block<true>(s, side, k0, qb * 16, tq);
+      const uint32_t ds_tile = 16 * DS * sizeof(T);
+      const auto tile = [&](int qb, auto masked) {
+        float s[2][4], dp[2][4], nd[2][4];
+        load_block<PAIR>(s, row0, row1, off_at + qb * kOffTile);
+        if (masked() && mixed) mask_block(s, side, side[k0], side[k0 + 8], qb * 16, tq);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float2 m = *reinterpret_cast<const float2*>(sub + qb * 16 + 8 * j + 2 * tq);
-          const float2 d = *reinterpret_cast<const float2*>(negD + qb * 16 + 8 * j + 2 * tq);
-          s[j][0] -= m.x;
-          s[j][1] -= m.y;
-          s[j][2] -= m.x;
-          s[j][3] -= m.y;
-          dp[j][0] = dp[j][2] = d.x;
-          dp[j][1] = dp[j][3] = d.y;
+          float mx, my;
+          lds_f2(sub_at + qb * 64 + j * 32, mx, my);
+          lds_f2(d_at + qb * 64 + j * 32, nd[j][0], nd[j][1]);
+          nd[j][2] = nd[j][0];
+          nd[j][3] = nd[j][1];
+          s[j][0] -= mx;
+          s[j][1] -= my;
+          s[j][2] -= mx;
+          s[j][3] -= my;
         }
-        block_product<T, HD, RS>(s, kf, sQ + qb * 16 * RS, lane);
-        block_product<T, HD, RS>(dp, vf, sG + qb * 16 * RS, lane);
-        if (wide) {
+        block_products<T, HD>(s, s, kf, q_nt + qb * kTile, dp, nd, vf, g_nt + qb * kTile);
+        if (masked() && wide) {
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             const float2 m = *reinterpret_cast<const float2*>(late + qb * 16 + 8 * j + 2 * tq);
@@ -959,16 +1086,29 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             s[j][e] = fast_exp2(s[j][e]);
-            dp[j][e] *= s[j][e];
+            if (masked() && k0 + 8 * (e >> 1) >= L) s[j][e] = 0.f;  // padding keys
           }
         const uint32_t p[4] = {pack2<T>(s[0][0], s[0][1]), pack2<T>(s[0][2], s[0][3]), pack2<T>(s[1][0], s[1][1]),
                                pack2<T>(s[1][2], s[1][3])};
-        const uint32_t ds[4] = {pack2<T>(dp[0][0], dp[0][1]), pack2<T>(dp[0][2], dp[0][3]), pack2<T>(dp[1][0], dp[1][1]),
-                                pack2<T>(dp[1][2], dp[1][3])};
+        uint32_t ds[4];
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 v = mul2(make_float2(s[j][2 * e], s[j][2 * e + 1]), make_float2(dp[j][2 * e], dp[j][2 * e + 1]));
+            ds[2 * j + e] = pack2<T>(v.x, v.y);
+          }
         // ds: (keys, queries) = (0, 0), (8, 0), (0, 8), (8, 8) -> rows of queries
-        stsm_x4_t(ds_at + qb * 16 * DS * (uint32_t)sizeof(T), ds[0], ds[1], ds[2], ds[3]);
-        block_add<T, HD, RS>(dv, p, sG + qb * 16 * RS, lane);
-        block_add<T, HD, RS>(dk, ds, sQ + qb * 16 * RS, lane);
+        stsm_x4_t(ds_at + qb * ds_tile, ds[0], ds[1], ds[2], ds[3]);
+        block_add<T, HD>(dv, p, g_nn + qb * kTile);
+        block_add<T, HD>(dk, ds, q_nn + qb * kTile);
+      };
+      if (mixed || warp * 16 + 16 > L || wide) {
+#pragma unroll 1
+        for (int qb = 0; qb < o.tiles; ++qb) tile(qb, std::true_type());
+      } else {
+#pragma unroll 1
+        for (int qb = 0; qb < o.tiles; ++qb) tile(qb, std::false_type());
       }
       // dV, then dK through the norm, by way of this warp's rows of sV
       T* st_rows = sV + warp * 16 * RS;
@@ -980,7 +1120,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
       __syncwarp();
       store_rows<T, HD, RS>(st_rows, dst + 2 * C, g.qkv_stride, tok, warp * 16, L, lane);
       // dL/dk' = ln 2 dS^T q', q' with log2 e
-      norm_backward<T, HD>(dk, raw, kw, 0.69314718055994530942f, rk[k0], rk[k0 + 8], k0 < L, k0 + 8 < L, wk, lane);
+      norm_backward<T, HD>(dk, raw, kn, 0.69314718055994530942f, rk[k0], rk[k0 + 8], wk, lane);
       __syncwarp();
       stage_live<T, HD, RS>(st_rows, dk, warp * 16, L, lane);
       __syncwarp();
@@ -988,77 +1128,83 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
     }
     __syncthreads();
     // ---- the next item's rows
-    const int64_t after = item + 1;
-    const T* base_n = qkv + (int64_t)head_of(after) * HD;
     const int* tok_n = tok2 + (1 - cur) * rows;
-    if (next) {
-      copy(sQ, base_n, g.qkv_stride, tok_n);
-      if (k_bufs > 1) copy(sK0 + (1 - cur) * rows * RS, base_n + C, g.qkv_stride, tok_n);
-      copy(sV, base_n + 2 * C, g.qkv_stride, tok_n);
-      copy(sG, dout + (int64_t)head_of(after) * HD, g.out_stride, tok_n);
-    }
-    // ---- B
+    if (next) copy(head_n, tok_n, k_bufs > 1 ? sK0 + (1 - cur) * rows * RS : nullptr, true);
+    const auto add_sums = [&]() {
+      // A thread has a place (or several) and every groups-th displacement (dt, da) there
+      const int step = bs.sa * (DS + 1), displacements = (2 * o.nt - 1) * (2 * bs.na - 1);
+      for (int place = my_place; place < bs.places; place += nthreads) {
+        const int bi = place / (bs.nb / bs.width), bj = (place - bi * (bs.nb / bs.width)) * bs.width;
+        const T* at = sS + bi * bs.sb * DS + bj * bs.sb;
+        float* sum = acc + bi * bs.nb + bj + my_group * bs.nb * bs.nb;
+        int dt = 1 - o.nt, da = 1 - bs.na + my_group;
+        for (int d = my_group; d < displacements; d += groups) {
+          while (da >= bs.na) {
+            da -= 2 * bs.na - 1;
+            ++dt;
+          }
+          const int n = bs.na - abs(da);
+          float s0 = 0.f, s1 = 0.f;
+          for (int t = max(dt, 0); t < o.nt + min(dt, 0); ++t) {
+            const T* p = at + (t * o.ns * o.nf + max(da, 0) * bs.sa) * DS + (t - dt) * o.ns * o.nf + max(-da, 0) * bs.sa;
+#pragma unroll 4
+            for (int i = 0; i < n; ++i) {
+              if (PAIR) {
+                float f[2];
+                unpack2(*reinterpret_cast<const uint32_t*>(p), f, T());
+                s0 += f[0];
+                s1 += f[1];
+              } else {
+                s0 += to_f(*p);
+              }
+              p += step;
+            }
+          }
+          if (PAIR) {
+            const float2 old = *reinterpret_cast<const float2*>(sum);
+            *reinterpret_cast<float2*>(sum) = make_float2(old.x + s0, old.y + s1);
+          } else {
+            *sum += s0;
+          }
+          sum += groups * bs.nb * bs.nb;
+          da += groups;
+        }
+      }
+    };
+    // ---- B.  The sums wait for shared memory, the products for one another: half of the warps begin with either.
     float dq[CH][4];
 #pragma unroll
     for (int d = 0; d < CH; ++d) dq[d][0] = dq[d][1] = dq[d][2] = dq[d][3] = 0.f;
     uint32_t raw[KS][4];
     raw_rows<T, HD>(raw, base, g.qkv_stride, tok, warp * 16, L, lane);
+    const uint32_t k_nn = rows_nn<T, RS>(sK, lane);
     const uint32_t a_at = smem_u32(sS + (warp * 16 + (lane & 7) + ((lane >> 3) & 1) * 8) * DS + (lane >> 4) * 8);
-#pragma unroll 1
+    if (dbias_part && (warp & 1)) add_sums();
+#pragma unroll 2
     for (int kb = 0; kb < o.tiles; ++kb) {
       uint32_t a[4];
       ldsm_x4(a_at + kb * 32, a[0], a[1], a[2], a[3]);
-      block_add<T, HD, RS>(dq, a, sK + kb * 16 * RS, lane);
+      block_add<T, HD>(dq, a, k_nn + kb * kTile);
     }
-    if (dbias_part) {
-      // tasks of `width` entries: acc[dt][da][bi][bj ..]
-      const int tasks = bs.entries / bs.width, step = bs.sa * (DS + 1);
-      for (int e = threadIdx.x; e < tasks; e += nthreads) {
-        const int e1 = quick_div(e, bs.div_b), bj = (e - e1 * (bs.nb / bs.width)) * bs.width;
-        const int e2 = quick_div(e1, bs.div_b2), bi = e1 - e2 * bs.nb;
-        const int e3 = quick_div(e2, bs.div_a), da = e2 - e3 * (2 * bs.na - 1) - (bs.na - 1), dt = e3 - (o.nt - 1);
-        const int n = bs.na - abs(da);
-        float s0 = 0.f, s1 = 0.f;
-        for (int t = max(dt, 0); t < o.nt + min(dt, 0); ++t) {
-          const int q = t * o.ns * o.nf + max(da, 0) * bs.sa + bi * bs.sb;
-          const int k = (t - dt) * o.ns * o.nf + max(-da, 0) * bs.sa + bj * bs.sb;
-          const T* p = sS + q * DS + k;
-#pragma unroll 4
-          for (int i = 0; i < n; ++i) {
-            if (PAIR) {
-              float f[2];
-              unpack2(*reinterpret_cast<const uint32_t*>(p + i * step), f, T());
-              s0 += f[0];
-              s1 += f[1];
-            } else {
-              s0 += to_f(p[i * step]);
-            }
-          }
-        }
-        if (PAIR) {
-          float2* at = reinterpret_cast<float2*>(acc + 2 * e);
-          const float2 old = *at;
-          *at = make_float2(old.x + s0, old.y + s1);
-        } else {
-          acc[e] += s0;
-        }
-      }
-    }
+    if (dbias_part && !(warp & 1)) add_sums();
     __syncthreads();  // k's rows have been read: dQ leaves by way of this warp's
     {
       const int q0 = warp * 16 + gq;
       T* st_rows = sK + warp * 16 * RS;
       // dL/dq' = ln 2 dS k', and q' is scale log2 e times the norm's result
-      norm_backward<T, HD>(dq, raw, qn, g.scale, rq[q0], rq[q0 + 8], q0 < L, q0 + 8 < L, wq, lane);
+      norm_backward<T, HD>(dq, raw, qn, g.scale, rq[q0], rq[q0 + 8], wq, lane);
       stage_live<T, HD, RS>(st_rows, dq, warp * 16, L, lane);
       __syncwarp();
       store_rows<T, HD, RS>(st_rows, dqkv + (int64_t)head * HD, g.qkv_stride, tok, warp * 16, L, lane);
     }
     if (next && k_bufs == 1) {
       __syncthreads();
-      copy(sK0, base_n + C, g.qkv_stride, tok_n);
+      copy(head_n, tok_n, sK0, false);
     }
     cur = 1 - cur;
+    head = head_n;
+    win = win_n;
+    window = window_n;
   }
   __syncthreads();
   if (dbias_part && tab_head >= 0) {
@@ -1093,7 +1239,7 @@ cudaError_t launch_fwd(const void* qkv, const AttnBias& bias, const float* norms
   const int64_t items = (int64_t)g.B * (g.H / g.wh) * (g.W / g.ww) * g.nh;
   if (items > INT32_MAX) return cudaErrorInvalidValue;
   k<<<(unsigned)items, 32 * std::min(o.tiles, kFwdWarps), smem, s>>>((const T*)qkv, bias, norms, (T*)out,
-                                                                    reinterpret_cast<float2*>(lse), g);
+                                                                    reinterpret_cast<float2*>(lse), g, o);
   return cudaGetLastError();
 }
 
@@ -1130,7 +1276,7 @@ cudaError_t launch_bwd(const void* qkv, const AttnBias& bias, const float* norms
   NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   k<<<plan.blocks, 32 * o.tiles, smem, s>>>((const T*)qkv, bias, norms, (const T*)out, (const T*)dout,
                                             reinterpret_cast<const float2*>(lse), (T*)dqkv, dqw_part, dkw_part, dbias_part,
-                                            plan.k_bufs, g);
+                                            plan.k_bufs, g, o);
   return cudaGetLastError();
 }
 
@@ -1188,7 +1334,7 @@ AttnBias attn_bias_layout(const AttnGeom& g) {
 cudaError_t attn_bias_prepare(const AnyMatrix& table, const AnyMatrix& qw, const AnyMatrix& kw, const AttnGeom& g,
                               const AttnBias& b, float* tab, cudaStream_t s) {
   attn_bias::prepare_kernel<<<g.nh + 1, 256, 0, s>>>(table, qw, kw, b, g.nh, g.hd, 2 * g.T - 1, 2 * g.wh - 1, 2 * g.ww - 1,
-                                                     tab);
+                                                     g.scale, tab);
   return cudaGetLastError();
 }
 
