@@ -56,7 +56,7 @@ constexpr float kAbsorbs = 1099511627776.f;  // 2^40
 __global__ void __launch_bounds__(256) prepare_kernel(const AnyMatrix table, const AnyMatrix qw, const AnyMatrix kw, const AttnBias b,
                                                       int heads, int hd, int nt, int ny, int nx, float scale,
                                                       float* __restrict__ tab) {
-  __shared__ float hi_w[8], lo_w[8];
+  __shared__ float hi_w[8], held[1160];  // (windows of 192 tokens have at most 1155 displacements)
   const int h = blockIdx.x, n = nt * ny * nx;
   float* out = tab + (int64_t)h * b.stride;
   if (h == heads) {
@@ -66,26 +66,24 @@ __global__ void __launch_bounds__(256) prepare_kernel(const AnyMatrix table, con
     }
     return;
   }
-  float hi = -INFINITY, lo = INFINITY;
+  float hi = -INFINITY, most = 0.f;
+  for (int i = threadIdx.x & 31; i < hd; i += 32)
+    most = fmaxf(most, fabsf(load_any(qw.p, qw.dtype, i * qw.s0) * load_any(kw.p, kw.dtype, i * kw.s0)));
   for (int i = threadIdx.x; i < n; i += 256) {
     const float v = load_any(table.p, table.dtype, h * table.s0 + i * table.s1);
+    held[i] = v;
     hi = fmaxf(hi, v);
-    lo = fminf(lo, v);
   }
   hi = warp_max(hi);
-  lo = -warp_max(-lo);
-  if ((threadIdx.x & 31) == 0) hi_w[threadIdx.x >> 5] = hi, lo_w[threadIdx.x >> 5] = lo;
+  if ((threadIdx.x & 31) == 0) hi_w[threadIdx.x >> 5] = hi;
   __syncthreads();
-  for (int w = 0; w < 8; ++w) hi = fmaxf(hi, hi_w[w]), lo = fminf(lo, lo_w[w]);
+  for (int w = 0; w < 8; ++w) hi = fmaxf(hi, hi_w[w]);
   const bool shifted = fabsf(hi) <= kAbsorbs;
   const float shift = shifted ? hi : 0.f;
   const auto entry = [&](float v) {
     const float e = (v - shift) * kLog2e;
     return isinf(e) && !isinf(v) ? copysignf(FLT_MAX, e) : e;
   };
-  float most = 0.f;
-  for (int i = threadIdx.x & 31; i < hd; i += 32)
-    most = fmaxf(most, fabsf(load_any(qw.p, qw.dtype, i * qw.s0) * load_any(kw.p, kw.dtype, i * kw.s0)));
   // (a margin for the roundings of q and k)
   most = warp_max(most) * fabsf(scale) * (1.01f * kLog2e * (float)hd);
   const int nf = b.y_fast ? ny : nx, ns = b.y_fast ? nx : ny;
@@ -96,7 +94,7 @@ __global__ void __launch_bounds__(256) prepare_kernel(const AnyMatrix table, con
       v = shifted ? most : INFINITY;  // (the bound needs the largest entry to be 0)
     } else if (at >= 0 && t < nt && f < nf) {
       const int y = b.y_fast ? f : s, x = b.y_fast ? s : f;
-      v = entry(load_any(table.p, table.dtype, h * table.s0 + ((t * ny + y) * nx + x) * table.s1));
+      v = entry(held[(t * ny + y) * nx + x]);
     }
     out[i] = v;
   }
@@ -1150,10 +1148,9 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
 #pragma unroll 4
             for (int i = 0; i < n; ++i) {
               if (PAIR) {
-                float f[2];
-                unpack2(*reinterpret_cast<const uint32_t*>(p), f, T());
-                s0 += f[0];
-                s1 += f[1];
+                const float2 f = unpack_pair<T>(*reinterpret_cast<const uint32_t*>(p));
+                s0 += f.x;
+                s1 += f.y;
               } else {
                 s0 += to_f(*p);
               }

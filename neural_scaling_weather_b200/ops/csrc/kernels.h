@@ -73,7 +73,7 @@ struct AttnGeom {
   int64_t out_stride;  // elements between tokens in out / dout (nh*hd)
 };
 // Learned bias of the logits by head and displacement of query and key (tab null: none), as attn_bias_prepare leaves it:
-// for each head a row of `stride` floats, the first four a header ([0]: largest less smallest entry), then entry
+// for each head a row of `stride` floats, the first four a header ([0]: a bound on the logits without the bias), then entry
 // (dt (2 wh - 1) + dy) pitch + dx (y_fast: (dt (2 ww - 1) + dx) pitch + dy), in units of log2 and less the head's largest one
 // (a softmax does not see it).
 struct AttnBias {
