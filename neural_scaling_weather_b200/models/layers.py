@@ -66,6 +66,17 @@ class LinearLayer(nn.Module):
         return torch.nn.functional.linear(x, self.weight)
 
 
+class ExpertLayer(nn.Module):
+    """The weight-only linear layers of ``num_experts`` experts, one weight (E, out, in)."""
+
+    def __init__(self, num_experts: int, in_features: int, out_features: int, comm_metadata=None):
+        super().__init__()
+        self.num_experts, self.in_features, self.out_features = num_experts, in_features, out_features
+        self.weight = nn.Parameter(torch.empty(num_experts, out_features, in_features))
+        self.weight.comm_metadata = comm_metadata or _meta([None, None, None], [], [])
+        trunc_normal_(self.weight, std=0.02)
+
+
 class BiasLayer(nn.Module):
     """Separate bias, so a row-parallel bias is added once after the tp reduction."""
 

@@ -12,11 +12,17 @@ Architecture and parameter layout follow the reference (``models/swin.py:36-323`
   latitude wrap (longitude is periodic and unmasked);
 * a linear head and unpatchify; only the last time step is returned.
 
-Two options that the reference does not have (defaults keep its blocks and parameter names):
-``mlp_type`` "swiglu" or "geglu" replaces the GELU MLP with a gated feed-forward network of hidden width
-``int(dim * mlp_ratio)`` (``mlp_ratio`` 8/3 has about the parameters of the GELU MLP's 4), and
-``block_norm`` "sandwich" also normalises each branch's output and adds it through a learned gate per
-channel: ``x + gate * rms_norm(branch(rms_norm(x)))``.
+Four options that the reference does not have (defaults keep its blocks and parameter names):
+
+* ``mlp_type`` "swiglu" or "geglu" replaces the GELU MLP with a gated feed-forward network of hidden width
+  ``int(dim * mlp_ratio)`` (``mlp_ratio`` 8/3 has about the parameters of the GELU MLP's 4);
+* ``block_norm`` "sandwich" also normalises each branch's output and adds it through a learned gate per
+  channel: ``x + gate * rms_norm(branch(rms_norm(x)))``;
+* ``rel_pos_bias`` adds a learned bias per head and displacement between two tokens of a window to the
+  attention's logits;
+* ``num_experts`` makes each block's gated network that many experts of the same hidden width, of which a
+  router chooses ``experts_per_token`` for every token.  ``forward(x, return_balance=True)`` also returns the
+  mean over blocks of the routers' balance loss (1 for a uniform load), for the training loss.
 
 The B200 design departs from the reference's data flow, not its math:
 
@@ -41,12 +47,17 @@ import torch.nn.functional as F
 from .. import ops
 from ..parallel import comm
 from ..parallel.helpers import offsets
-from ..parallel.mappings import roll_forward_reverseroll_backward
+from ..parallel.mappings import (
+    allreduce_forward_identity_backward,
+    identity_forward_allreduce_backward,
+    roll_forward_reverseroll_backward,
+)
 from ..utils.checkpoint_io import verified_load
 from ..utils.profiler import profile
 from .layers import (
     BiasLayer,
     Conv2DLayer,
+    ExpertLayer,
     LinearLayer,
     NormLayer,
     PatchEmbedLayer,
@@ -56,9 +67,10 @@ from .layers import (
 
 
 class WindowMultiHeadAttention(nn.Module):
-    """Window attention with QK-RMSNorm; q/k/v column-parallel, proj row-parallel over tp."""
+    """Window attention with QK-RMSNorm; q/k/v column-parallel, proj row-parallel over tp.  ``bias_steps``: time
+    steps of a window whose tokens' displacements have a learned bias per head (0: no bias)."""
 
-    def __init__(self, dim: int, num_heads: int, window_size: Tuple[int, int]):
+    def __init__(self, dim: int, num_heads: int, window_size: Tuple[int, int], bias_steps: int = 0):
         super().__init__()
         if dim % num_heads:
             raise AssertionError("embed dim must be divisible by the number of heads")
@@ -83,6 +95,12 @@ class WindowMultiHeadAttention(nn.Module):
         self.biasv = BiasLayer(dl, comm_metadata=colb())
         self.proj = LinearLayer(dl, dim, comm_metadata=_meta([None, "tp"], ["sp1-sp2"], ["sp1-sp2"]))
         self.biasproj = BiasLayer(dim, comm_metadata=_meta([], ["tp-sp1-sp2"], ["sp1-sp2"]))
+        self.rel_bias = None
+        if bias_steps > 0:
+            buckets = ops.WindowGeometry(window=self.window_size).num_buckets(bias_steps)
+            self.rel_bias = nn.Parameter(torch.empty(self.num_heads_local, buckets))
+            self.rel_bias.comm_metadata = col()
+            trunc_normal_(self.rel_bias, std=0.02)
 
     def qkv_params(self):
         """q/k/v weights and biases; the fused GEMM concatenates them along N."""
@@ -165,15 +183,56 @@ class GatedMLP(nn.Module):
         return y if residual is None else y + residual
 
 
+class RoutedMLP(nn.Module):
+    """Gated networks without biases of which a router chooses ``top_k`` for each token; every expert's hidden
+    features are split over tp, so that all ranks route alike.  Logits have the compute type, probabilities fp32."""
+
+    def __init__(self, in_features, hidden_features, num_experts: int, top_k: int, mlp_type: str = "swiglu"):
+        super().__init__()
+        tp = comm.get_size("tp")
+        if hidden_features % tp:
+            raise AssertionError(f"cannot shard MLP hidden {hidden_features} into {tp} shards")
+        if not 1 <= top_k <= num_experts:
+            raise ValueError(f"experts_per_token {top_k} is not in 1 .. num_experts {num_experts}")
+        hl = hidden_features // tp
+        col = lambda: _meta([None, "tp", None], ["sp1-sp2"], ["sp1-sp2"])  # noqa: E731
+        self.router = LinearLayer(in_features, num_experts, comm_metadata=_meta([], ["tp-sp1-sp2"], ["sp1-sp2"]))
+        self.gate = ExpertLayer(num_experts, in_features, hl, comm_metadata=col())
+        self.up = ExpertLayer(num_experts, in_features, hl, comm_metadata=col())
+        self.down = ExpertLayer(num_experts, hl, in_features,
+                                comm_metadata=_meta([None, None, "tp"], ["sp1-sp2"], ["sp1-sp2"]))
+        self.activation = GatedMLP.ACTIVATIONS[mlp_type]
+        self.top_k = top_k
+
+    @profile("mlp")
+    def forward(self, x, residual: Optional[torch.Tensor] = None):
+        """-> (output, balance loss of this call's tokens)"""
+        weights, experts, balance = ops.route_tokens(ops.linear(x, self.router.weight), self.top_k)
+        w = (self.gate.weight, self.up.weight, self.down.weight)
+        if comm.get_size("tp") == 1:
+            return ops.expert_mlp(x, weights, experts, *w, residual=residual, activation=self.activation), balance
+        # each rank has a part of every expert's output: the gradients of x and of the weights are sums over tp
+        x = identity_forward_allreduce_backward(x, "tp")
+        weights = identity_forward_allreduce_backward(weights, "tp")
+        y = ops.expert_mlp(x, weights, experts, *w, activation=self.activation)
+        y = allreduce_forward_identity_backward(y, "tp")
+        return y if residual is None else y + residual, balance
+
+
 class Block(nn.Module):
     def __init__(self, dim, num_heads, feat_size, window_size, temporal_context_window_size,
                  shift_size=(0, 0), mlp_ratio=4.0, drop=0.0, act_layer=nn.GELU,
-                 sp1_shapes=None, sp2_shapes=None, mlp_type: str = "gelu", block_norm: str = "pre"):
+                 sp1_shapes=None, sp2_shapes=None, mlp_type: str = "gelu", block_norm: str = "pre",
+                 rel_pos_bias: bool = False, num_experts: int = 0, experts_per_token: int = 2):
         super().__init__()
         if mlp_type != "gelu" and mlp_type not in GatedMLP.ACTIVATIONS:
             raise ValueError(f"mlp_type {mlp_type!r} is not 'gelu' or one of {sorted(GatedMLP.ACTIVATIONS)}")
         if block_norm not in ("pre", "sandwich"):
             raise ValueError(f"block_norm {block_norm!r} is neither 'pre' nor 'sandwich'")
+        if num_experts < 0 or (num_experts > 0 and mlp_type == "gelu"):
+            raise ValueError(f"num_experts {num_experts}: experts are gated networks (mlp_type 'swiglu' or 'geglu')")
+        if num_experts > 0 and drop > 0:
+            raise ValueError("routed experts have no dropout")
         self.dim = dim
         self.block_norm = block_norm
         self.feat_size = tuple(feat_size)
@@ -190,11 +249,16 @@ class Block(nn.Module):
             )
         norm_meta = lambda: _meta([None], ["tp-sp1-sp2"], ["sp1-sp2"])  # noqa: E731
         self.norm1 = NormLayer(dim, norm_type="rms_norm", comm_metadata=norm_meta())
-        self.attn = WindowMultiHeadAttention(dim, num_heads=num_heads, window_size=window_size)
+        self.attn = WindowMultiHeadAttention(dim, num_heads=num_heads, window_size=window_size,
+                                             bias_steps=temporal_context_window_size if rel_pos_bias else 0)
         self.norm2 = NormLayer(dim, norm_type="rms_norm", comm_metadata=norm_meta())
         hidden = int(dim * mlp_ratio)
-        self.mlp = (MLP(dim, hidden_features=hidden, act_layer=act_layer, drop=drop) if mlp_type == "gelu"
-                    else GatedMLP(dim, hidden, mlp_type, drop))
+        if num_experts > 0:
+            self.mlp = RoutedMLP(dim, hidden, num_experts, experts_per_token, mlp_type)
+        elif mlp_type == "gelu":
+            self.mlp = MLP(dim, hidden_features=hidden, act_layer=act_layer, drop=drop)
+        else:
+            self.mlp = GatedMLP(dim, hidden, mlp_type, drop)
         if block_norm == "sandwich":
             for i in (1, 2):
                 setattr(self, f"post_norm{i}", NormLayer(dim, norm_type="rms_norm", comm_metadata=norm_meta()))
@@ -234,7 +298,7 @@ class Block(nn.Module):
         w_qkv, b_qkv = attn.qkv_params()
         qkv = ops.linear_colparallel(x, w_qkv, b_qkv, group="tp")
         o = ops.window_attention(qkv, attn.q_norm.weight, attn.k_norm.weight,
-                                 attn.num_heads_local, attn.head_dim, geom, attn.scale)
+                                 attn.num_heads_local, attn.head_dim, geom, attn.scale, rel_bias=attn.rel_bias)
         tp = comm.get_size("tp")
         if tp == 1 and not roll:
             return ops.linear(o, attn.proj.weight, attn.biasproj.bias, residual=skip)
@@ -247,27 +311,39 @@ class Block(nn.Module):
             shapes=(self.sp1_shapes, self.sp2_shapes))
         return y if skip is None else y + skip
 
+    def _feed_forward(self, x, skip: Optional[torch.Tensor], balances: Optional[list]):
+        if not isinstance(self.mlp, RoutedMLP):
+            return self.mlp(x, residual=skip)
+        y, balance = self.mlp(x, residual=skip)
+        if balances is not None:
+            balances.append(balance)
+        return y
+
     def forward(self, x: torch.Tensor, condition: Optional[torch.Tensor] = None,
-                normed: Optional[torch.Tensor] = None, next_weight: Optional[torch.Tensor] = None):
+                normed: Optional[torch.Tensor] = None, next_weight: Optional[torch.Tensor] = None,
+                balances: Optional[list] = None):
         """x: (B, T, H, W, C) -> same shape.  A sandwich block that is given ``normed``, the norm of ``x`` by its
-        first weight, returns the pair of :meth:`forward_sandwich`."""
+        first weight, returns the pair of :meth:`forward_sandwich`.  A block with experts appends its router's
+        balance loss to ``balances``."""
         if self.block_norm == "sandwich":
             if normed is not None:
-                return self.forward_sandwich(x, normed, next_weight)
-            return self.forward_sandwich(x, ops.rms_norm(x, self.norm1.weight), None)[0]
+                return self.forward_sandwich(x, normed, next_weight, balances)
+            return self.forward_sandwich(x, ops.rms_norm(x, self.norm1.weight), None, balances)[0]
         # each pre-norm and its skip connection come from one node, so the two gradients of
         # the residual stream are summed inside the RMSNorm backward
         h, skip = self._norm_skip(self.norm1, x)
         x = self._shifted_window_attn(h, skip)
         h, skip = self._norm_skip(self.norm2, x)
-        return self.mlp(h, residual=skip)
+        return self._feed_forward(h, skip, balances)
 
-    def forward_sandwich(self, x: torch.Tensor, normed: torch.Tensor, next_weight: Optional[torch.Tensor]):
+    def forward_sandwich(self, x: torch.Tensor, normed: torch.Tensor, next_weight: Optional[torch.Tensor],
+                         balances: Optional[list] = None):
         """The stream ``x`` and its norm for this block -> the stream after the block and its norm for the next
         one (None without ``next_weight``).  Everything between two branches is one operator."""
         a = self._shifted_window_attn(normed, None)
         x, normed = ops.norm_gate_residual(a, x, self.post_norm1.weight, self.branch_gate1, self.norm2.weight)
-        return ops.norm_gate_residual(self.mlp(normed), x, self.post_norm2.weight, self.branch_gate2, next_weight)
+        return ops.norm_gate_residual(self._feed_forward(normed, None, balances), x, self.post_norm2.weight,
+                                      self.branch_gate2, next_weight)
 
     @staticmethod
     def _norm_skip(norm, x):
@@ -298,6 +374,9 @@ class SwinTransformer(nn.Module):
             coord_pos_embed=getattr(cfg.model, "coord_pos_embed", True),
             mlp_type=getattr(cfg.model, "mlp_type", "gelu"),
             block_norm=getattr(cfg.model, "block_norm", "pre"),
+            rel_pos_bias=getattr(cfg.model, "rel_pos_bias", False),
+            num_experts=getattr(cfg.model, "num_experts", 0),
+            experts_per_token=getattr(cfg.model, "experts_per_token", 2),
             use_transformer_engine=getattr(cfg.parallelism, "use_transformer_engine", True),
             domain_metadata=domain_metadata,
         )
@@ -306,7 +385,7 @@ class SwinTransformer(nn.Module):
                  in_chans=3, out_chans=3, embed_dim=768, depth=12, num_heads=12, mlp_ratio=4.0,
                  drop_rate=0.0, coord_pos_embed=True, domain_metadata=None,
                  use_transformer_engine=True, use_big_skip_conv=False, mlp_type="gelu", block_norm="pre",
-                 **kwargs):
+                 rel_pos_bias=False, num_experts=0, experts_per_token=2, **kwargs):
         super().__init__()
         if domain_metadata is None:
             raise AssertionError("the data loader must provide domain metadata")
@@ -320,6 +399,7 @@ class SwinTransformer(nn.Module):
         self.domain_metadata = domain_metadata
         self.use_big_skip_conv = use_big_skip_conv
         self.block_norm = block_norm
+        self.num_experts = num_experts
         sp1_shapes, sp2_shapes = domain_metadata["sp_shapes"]
         shared = lambda: _meta([], ["tp-sp1-sp2"], ["sp1-sp2"])  # noqa: E731
 
@@ -343,7 +423,8 @@ class SwinTransformer(nn.Module):
                   shift_size=tuple(0 if i % 2 == 0 else w // 2 for w in self.window_size),
                   mlp_ratio=mlp_ratio, drop=drop_rate,
                   sp1_shapes=self.patch_embed.sp1_patch_shapes,
-                  sp2_shapes=self.patch_embed.sp2_patch_shapes, mlp_type=mlp_type, block_norm=block_norm)
+                  sp2_shapes=self.patch_embed.sp2_patch_shapes, mlp_type=mlp_type, block_norm=block_norm,
+                  rel_pos_bias=rel_pos_bias, num_experts=num_experts, experts_per_token=experts_per_token)
             for i in range(depth)
         ])
         self.out_size = out_chans * patch_size * patch_size
@@ -393,23 +474,27 @@ class SwinTransformer(nn.Module):
         return ops.head_unpatchify(x, self.head.weight, self.patch_size, self.out_chans)
 
     @profile("forward")
-    def forward(self, x):
+    def forward(self, x, return_balance: bool = False):
+        if return_balance and not self.num_experts:
+            raise ValueError("return_balance: the model has no experts")
+        balances = [] if return_balance else None
+        collect = {"balances": balances} if return_balance else {}
         b, t, c, h, w = x.shape
         skip = x if self.use_big_skip_conv else None
         x = self.prepare_tokens(x)
         if self.block_norm == "sandwich":
             normed = ops.rms_norm(x, self.blocks[0].norm1.weight)
             for blk, following in zip(self.blocks, [*self.blocks[1:], None]):
-                x, normed = blk(x, normed=normed,
+                x, normed = blk(x, normed=normed, **collect,
                                 next_weight=None if following is None else following.norm1.weight)
         else:
             for blk in self.blocks:
-                x = blk(x)
+                x = blk(x, **collect)
         x = self.forward_head(x)
         if self.use_big_skip_conv:
             s = self.skip_conv(skip.reshape(b * t, c, h, w)).view(b, t, self.out_chans, h, w)
             x = x + s
-        return x[:, -1:]
+        return (x[:, -1:], torch.stack(balances).mean()) if return_balance else x[:, -1:]
 
 
 class TimeStepper(nn.Module):
@@ -421,12 +506,17 @@ class TimeStepper(nn.Module):
         self.num_rollout_steps = int(cfg.train.num_rollout_steps)
         self.num_invariants = len(cfg.data.invariants) if cfg.data.invariants else 0
 
-    def forward(self, inp):
-        preds = []
+    def forward(self, inp, return_balance: bool = False):
+        """With ``return_balance`` also the mean over the steps of the routers' balance loss."""
+        preds, balances = [], []
         x = inp
         c_in = inp.shape[2]
         for step in range(self.num_rollout_steps):
-            pred = self.model(x)
+            if return_balance:
+                pred, balance = self.model(x, return_balance=True)
+                balances.append(balance)
+            else:
+                pred = self.model(x)
             preds.append(pred)
             if step == self.num_rollout_steps - 1:
                 break
@@ -437,7 +527,8 @@ class TimeStepper(nn.Module):
                 x = torch.cat([pred.to(inp.dtype), inp[:, -pred.shape[1]:, -n_inv:]], dim=2)
             else:
                 x = pred.to(inp.dtype)
-        return torch.cat(preds, dim=1)
+        out = torch.cat(preds, dim=1)
+        return (out, torch.stack(balances).mean()) if return_balance else out
 
 
 def get_model(cfg, domain_metadata=None):

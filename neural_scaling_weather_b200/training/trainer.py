@@ -74,6 +74,14 @@ def count_parameters(model) -> float:
     return sum(p.numel() for p in model.parameters() if p.requires_grad) / 1e6
 
 
+# model options that a run's saved configuration may predate; absent, each has this value
+MODEL_OPTIONS = {"rel_pos_bias": False, "num_experts": 0, "experts_per_token": 2, "router_balance_weight": 0.01}
+
+
+def with_model_options(cfg: dict) -> dict:
+    return {**cfg, "model": {**MODEL_OPTIONS, **cfg["model"]}} if isinstance(cfg.get("model"), dict) else cfg
+
+
 class DataParallel(nn.Module):
     """Holds the model under ``.module`` and exposes the reducer's ``no_sync``."""
 
@@ -158,7 +166,7 @@ class Trainer:
         if self.resuming:
             prev = os.path.join(self.exp_dir, "hyperparameters.yaml")
             if os.path.isfile(prev):
-                if C.to_container(C.load(prev)) != C.to_container(self.cfg):
+                if with_model_options(C.to_container(C.load(prev))) != with_model_options(C.to_container(self.cfg)):
                     raise AssertionError(
                         f"Resuming run_name={self.run_name}, run_tag={self.run_tag} failed: config "
                         "saved to hyperparameters.yaml does not match current config")
@@ -239,6 +247,11 @@ class Trainer:
         else:
             self.gscaler = torch.amp.GradScaler("cuda", enabled=fp16)
         self.loss_func = get_loss(cfg, self.metadata).to(self.device)
+        # the routers' balance loss joins the training loss; every rank balances its own tokens, and gradients are
+        # summed over the spatial groups, so a rank's part is its share of their mean
+        self.routed = int(cfg.model.get("num_experts", 0)) > 0
+        self.balance_weight = (float(cfg.model.get("router_balance_weight", 0.01))
+                               / (comm.get_size("sp1") * comm.get_size("sp2")))
         self.weighted_rmse = get_metric("weighted_rmse", self.metadata).to(self.device)
 
         self.iters_per_epoch = self.train_dataset.n_samples_total // int(cfg.data.batch_size)
@@ -260,6 +273,7 @@ class Trainer:
         self.logs = {}
         self.train_loss = torch.zeros(1, dtype=torch.float32, device=self.device)
         self.grad = torch.zeros(1, dtype=torch.float32, device=self.device)
+        self.router_balance = torch.zeros(1, dtype=torch.float32, device=self.device)
         self.train_time = 0.0
         self.flops_consumed = 0.0
         self.iters_last_log = self.iters
@@ -291,6 +305,7 @@ class Trainer:
         self.train_time = time.time()
         self.train_loss.zero_()
         self.grad.zero_()
+        self.router_balance.zero_()
         app = time.time()
         for epoch in range(self.start_epoch, self.end_epoch):
             self.epoch = epoch
@@ -392,9 +407,12 @@ class Trainer:
         """Forward, loss and backward of one micro-batch (gradients accumulate in place)."""
         with profile_range("forward pass"):
             with torch.autocast(self.device.type, dtype=self.amp_dtype, enabled=self.amp_enabled):
-                gen = self.model(inputs)
+                gen, balance = self.model(inputs, return_balance=True) if self.routed else (self.model(inputs), None)
                 loss = self.loss_func(gen, targets)
             self.train_loss += loss.detach()
+            if self.routed:
+                self.router_balance += balance.detach()
+                loss = loss + self.balance_weight * balance
             loss = loss / self.gradient_accum_steps
         with profile_range("backward pass"):
             self.gscaler.scale(loss).backward()
@@ -438,6 +456,7 @@ class Trainer:
                 torch.cuda.synchronize()
                 self.optimizer.zero_grad(set_to_none=False)
                 self.train_loss.zero_()
+                self.router_balance.zero_()
                 return self._micro_batch(inputs, targets)
         self._static[0].copy_(inputs, non_blocking=True)
         self._static[1].copy_(targets, non_blocking=True)
@@ -495,6 +514,7 @@ class Trainer:
                     self.validate_and_checkpoint()
                     self.train_loss.zero_()
                     self.grad.zero_()
+                    self.router_balance.zero_()
                     self.train_time = time.time()
                 o = self.cfg.optimizer
                 if o.scheduler == "cooldown":
@@ -570,9 +590,14 @@ class Trainer:
         n_it = max(1, self.iters - self.iters_last_log)
         train_loss = self.train_loss / n_mbs
         grad = self.grad / n_it
+        balance = self.router_balance / n_mbs
         if dist.is_initialized() and comm.get_size("dp") > 1:
             dist.all_reduce(train_loss, op=dist.ReduceOp.AVG, group=comm.get_group("dp"))
             dist.all_reduce(grad, op=dist.ReduceOp.AVG, group=comm.get_group("dp"))
+            if self.routed:
+                dist.all_reduce(balance, op=dist.ReduceOp.AVG, group=comm.get_group("dp"))
+        if self.routed:
+            self.logs["router_balance"] = float(balance.item())
         self.logs["train_loss"] = float(train_loss.item())
         self.logs["grad"] = float(grad.item())
         samples = n_mbs * int(self.cfg.parallelism.micro_batch_size) * comm.get_size("dp")

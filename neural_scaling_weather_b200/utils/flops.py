@@ -37,6 +37,14 @@ def gated_mlp_flops(batchseq, embed, hidden):
     return (up + 9 * batchseq * hidden + down) * TFLOPS
 
 
+def routed_mlp_flops(batchseq, embed, hidden, experts, per_token):
+    """The router's product and softmax, and per chosen expert three products without biases, the activation, the
+    gate's product and the weighted sum."""
+    router = 2 * batchseq * embed * experts + 5 * batchseq * experts
+    expert = 6 * batchseq * embed * hidden + 9 * batchseq * hidden + 2 * batchseq * embed
+    return (router + per_token * expert) * TFLOPS
+
+
 def patch_embed_flops(batch, h, w, c, patch_size, embed):
     seq = h // patch_size * w // patch_size
     return (2 * batch * h * w * c * embed + batch * seq * embed) * TFLOPS
@@ -69,6 +77,10 @@ class FlopsCalculator:
         # more norms (the gate and skip are counted with them, 3 an element)
         self.gated_hidden = (0 if getattr(m, "mlp_type", "gelu") == "gelu" else int(m.embed_dim * m.mlp_ratio))
         self.extra_norms = 4 if getattr(m, "block_norm", "pre") == "sandwich" else 0
+        # and experts in the gated network's place, and a bias per head and displacement (one addition per logit)
+        self.experts, self.per_token = getattr(m, "num_experts", 0), getattr(m, "experts_per_token", 2)
+        self.bias_buckets = ((2 * self.t - 1) * (2 * self.wh - 1) * (2 * self.ww - 1)
+                             if getattr(m, "rel_pos_bias", False) else 0)
 
     def flops(self, verbose: bool = False) -> float:
         """Forward TFLOPs of one micro-batch."""
@@ -76,9 +88,15 @@ class FlopsCalculator:
         patch = patch_embed_flops(bt, self.h, self.w, self.c_in, self.patch_size, self.embed)
         pos = patch_embed_flops(bt, self.h, self.w, 4, self.patch_size, self.embed)
         attn = attention_flops(self.batch * self.num_windows, self.seq, self.embed, self.heads)
+        if self.bias_buckets:
+            attn += self.batch * self.num_windows * self.heads * self.seq * self.seq * TFLOPS
         ntok = bt * self.h_patch * self.w_patch
-        mlp = (gated_mlp_flops(ntok, self.embed, self.gated_hidden) if self.gated_hidden
-               else mlp_flops(ntok, self.embed, 4 * self.embed))
+        if self.experts:
+            mlp = routed_mlp_flops(ntok, self.embed, self.gated_hidden, self.experts, self.per_token)
+        elif self.gated_hidden:
+            mlp = gated_mlp_flops(ntok, self.embed, self.gated_hidden)
+        else:
+            mlp = mlp_flops(ntok, self.embed, 4 * self.embed)
         norm = rms_norm_flops(ntok * self.embed)
         block = attn + mlp + (4 + self.extra_norms) * norm
         head = head_flops(self.batch, self.h, self.w, self.embed, self.patch_size, self.c_out)
@@ -91,7 +109,9 @@ class FlopsCalculator:
         patch = e * self.c_in * p * p + e
         pos = e * 4 * p * p + e
         ffn = 3 * e * self.gated_hidden if self.gated_hidden else e * 4 * e * 2
-        block = e * e * 3 + e * e + ffn + e * (4 + self.extra_norms)
+        if self.experts:
+            ffn = self.experts * (ffn + e)
+        block = e * e * 3 + e * e + ffn + e * (4 + self.extra_norms) + self.heads * self.bias_buckets
         head = self.c_out * e * p * p
         self.params_backbone = block * self.depth * 1e-6
         return (patch + pos + block * self.depth + head) * 1e-6
