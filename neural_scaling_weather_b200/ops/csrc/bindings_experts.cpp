@@ -106,6 +106,7 @@ std::tuple<Tensor, Tensor, Tensor> route_tokens(const Tensor& logits, int64_t k,
 // ------------------------------------------------------------------------------ experts
 struct ExpertShape {
   int64_t M, k, A, E, K, H, N, Kp, Hp, Np, rows;
+  int tile;
 };
 
 void check_stack(const Tensor& t, at::IntArrayRef sizes, const Tensor& x, const char* name) {
@@ -137,21 +138,23 @@ ExpertShape expert_shape(const Tensor& x, const Tensor& weights, int64_t E, int6
   d.Kp = round8(d.K);
   d.Hp = round8(H);
   d.Np = round8(N);
-  d.rows = nsw::kExpertTile * nsw::expert_tiles(d.A, E);
+  d.tile = nsw::kExpertTile;
+  d.rows = d.tile * nsw::expert_tiles(d.A, E, d.tile);
   return d;
 }
 
 // the plan's arrays, one behind the other
 int64_t plan_size(const ExpertShape& d) {
-  return 1 + d.rows / nsw::kExpertTile + d.E + 1 + d.A + d.rows + nsw::expert_plan_hist(d.A, d.E);
+  return 1 + d.rows / d.tile + d.E + 1 + d.A + d.rows + nsw::expert_plan_hist(d.A, d.E);
 }
 nsw::ExpertPlan plan_of(const ExpertShape& d, const Tensor& t, const int64_t* experts) {
   nsw::ExpertPlan p{};
   p.experts = experts;
   p.count = d.A;
   p.num_experts = (int)d.E;
+  p.tile = d.tile;
   p.tiles = t.data_ptr<int>();
-  p.rows = p.tiles + 1 + d.rows / nsw::kExpertTile;
+  p.rows = p.tiles + 1 + d.rows / d.tile;
   p.row_of = p.rows + d.E + 1;
   p.src_of = p.row_of + d.A;
   p.hist = p.src_of + d.rows;
@@ -165,7 +168,7 @@ std::vector<Tensor> expert_mlp_fwd(const Tensor& x, const Tensor& weights, const
                                    bool save) {
   TORCH_CHECK_VALUE(wg.dim() == 3 && wd.dim() == 3 && weights.dim() == 2 && x.dim() == 2,
                     "expert_mlp: x and weights are matrices, the experts' weights of three dimensions");
-  const ExpertShape d = expert_shape(x, weights, wg.size(0), wg.size(1), wd.size(1));
+  ExpertShape d = expert_shape(x, weights, wg.size(0), wg.size(1), wd.size(1));
   check_stack(wg, {d.E, d.H, d.K}, x, "w_gate");
   check_stack(wu, {d.E, d.H, d.K}, x, "w_up");
   check_stack(wd, {d.E, d.N, d.H}, x, "w_down");
@@ -192,7 +195,7 @@ std::vector<Tensor> expert_mlp_fwd(const Tensor& x, const Tensor& weights, const
   const Tensor xu = unit(x) ? x : x.contiguous();
   const OptTensor res = !residual || unit(*residual) ? residual : OptTensor(residual->contiguous());
   const Tensor g2 = wg.flatten(0, 1), u2 = wu.flatten(0, 1), d2 = wd.flatten(0, 1);
-  if (!save && d.A <= nsw::kExpertFewRows && unit(g2) && unit(u2) && unit(d2)) {
+  if (!save && nsw::expert_few_pays(d.A, d.H, d.K, d.N) && unit(g2) && unit(u2) && unit(d2)) {
     auto h = torch::empty({d.A, d.Hp}, opt);
     nsw::ExpertFew f{};
     f.x = xu.data_ptr();
@@ -222,12 +225,16 @@ std::vector<Tensor> expert_mlp_fwd(const Tensor& x, const Tensor& weights, const
     check(nsw::expert_few(f, stream()), "expert_mlp");
     return {y};
   }
-  auto plan = torch::empty({plan_size(d)}, opt.dtype(at::kInt));
-  const nsw::ExpertPlan p = plan_of(d, plan, experts.data_ptr<int64_t>());
-  check(nsw::expert_plan(p, stream()), "expert_mlp plan");
+  if (!save) {
+    d.tile = nsw::expert_tile(d.A, d.E, d.H, d.N);
+    d.rows = d.tile * nsw::expert_tiles(d.A, d.E, d.tile);
+  }
   Aligner al;
   const Rows ga = al.add(g2), ua = al.add(u2), da = al.add(d2);
   al.run();
+  auto plan = torch::empty({plan_size(d)}, opt.dtype(at::kInt));
+  const nsw::ExpertPlan p = plan_of(d, plan, experts.data_ptr<int64_t>());
+  check(nsw::expert_plan(p, stream()), "expert_mlp plan");
   auto xs = torch::empty({d.rows, d.Kp}, opt);
   nsw::ExpertGather gather{};
   gather.plan = &p;
@@ -238,8 +245,8 @@ std::vector<Tensor> expert_mlp_fwd(const Tensor& x, const Tensor& weights, const
   gather.dst = xs.data_ptr();
   gather.ld_dst = d.Kp;
   gather.dtype = dtype;
-  check(nsw::expert_gather(gather, stream()), "expert_mlp gather");
-  const nsw::GatedGroups groups{d.E, p.tiles, p.rows};
+  check(nsw::expert_gather(gather, true, stream()), "expert_mlp gather");
+  const nsw::GatedGroups groups{d.E, p.tiles, p.rows, p.tile};
   auto h = torch::empty({d.rows, d.Hp}, opt);
   Tensor g, u;
   nsw::GatedArgs up{}, down{};
@@ -266,7 +273,7 @@ std::vector<Tensor> expert_mlp_fwd(const Tensor& x, const Tensor& weights, const
     up.out2 = u.data_ptr();
     up.ldaux = d.Hp;
   }
-  check(nsw::gated_product(up, false, stream()), "expert_mlp up");
+  check(nsw::gated_product(up, d.tile < nsw::kExpertTile, stream()), "expert_mlp up");
   auto ys = torch::empty({d.rows, d.Np}, opt);
   down.N = d.N;
   down.K = d.H;
@@ -276,7 +283,7 @@ std::vector<Tensor> expert_mlp_fwd(const Tensor& x, const Tensor& weights, const
   down.ldb0 = da.ld;
   down.out0 = ys.data_ptr();
   down.ldout = d.Np;
-  check(nsw::gated_product(down, false, stream()), "expert_mlp down");
+  check(nsw::gated_product(down, d.tile < nsw::kExpertTile, stream()), "expert_mlp down");
   nsw::ExpertCombine c{};
   c.row_of = p.row_of;
   c.tokens = d.M;
@@ -291,7 +298,7 @@ std::vector<Tensor> expert_mlp_fwd(const Tensor& x, const Tensor& weights, const
   c.out = y.data_ptr();
   c.ld_out = d.N;
   c.dtype = dtype;
-  check(nsw::expert_combine(c, stream()), "expert_mlp combine");
+  check(nsw::expert_combine(c, true, stream()), "expert_mlp combine");
   if (!save) return {y};
   return {y, xs, g, u, h, ys, plan, ga.t, ua.t, da.t};
 }
@@ -328,7 +335,7 @@ std::vector<Tensor> expert_mlp_bwd(const Tensor& dy, const Tensor& weights, int6
                   h.sizes() == g.sizes() && rows_aligned(wg) && rows_aligned(wu) && rows_aligned(wd),
               "expert_mlp backward: saved tensors must be as the forward returned them");
   const nsw::ExpertPlan p = plan_of(d, plan, nullptr);
-  const nsw::GatedGroups groups{E, p.tiles, p.rows};
+  const nsw::GatedGroups groups{E, p.tiles, p.rows, p.tile};
   const int dtype = dt_code(dy, "dy"), wdt = dt_code(weights, "weights");
   const Tensor dyu = dy.stride(1) == 1 || dy.size(1) == 1 ? dy : dy.contiguous();
   GradOut grad[3];
@@ -352,7 +359,7 @@ std::vector<Tensor> expert_mlp_bwd(const Tensor& dy, const Tensor& weights, int6
     out[1] = torch::empty(weights.sizes(), weights.options());
     gather.dweights = out[1].data_ptr();
   }
-  check(nsw::expert_gather(gather, stream()), "expert_mlp backward gather");
+  check(nsw::expert_gather(gather, false, stream()), "expert_mlp backward gather");
   const auto ld_of = [](const Tensor& t) { return t.size(0) == 1 ? round8(t.size(1)) : t.stride(0); };
   const bool need_hidden = need[0] || need[2] || need[3];
   Tensor dgu;
@@ -410,7 +417,7 @@ std::vector<Tensor> expert_mlp_bwd(const Tensor& dy, const Tensor& weights, int6
     c.out = out[0].data_ptr();
     c.ld_out = d.K;
     c.dtype = dtype;
-    check(nsw::expert_combine(c, stream()), "expert_mlp dx sum");
+    check(nsw::expert_combine(c, true, stream()), "expert_mlp dx sum");
   }
   if (need[2] || need[3] || need[4]) {
     nsw::GatedDwArgs w{};

@@ -50,7 +50,7 @@ __device__ __forceinline__ void place_experts(const ExpertPlan& p, int count, in
   __shared__ int warp_sum[kWarps];
   __shared__ int2 pad[kMaxExperts];
   const int e = threadIdx.x, warp = e >> 5, lane = e & 31;
-  const int padded = (count + kExpertTile - 1) / kExpertTile * kExpertTile;
+  const int padded = (count + p.tile - 1) / p.tile * p.tile;
   int upto = padded;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
@@ -64,10 +64,10 @@ __device__ __forceinline__ void place_experts(const ExpertPlan& p, int count, in
   if (e < p.num_experts) {
     start[e] = first;
     p.rows[e] = first;
-    for (int t = first / kExpertTile; t < upto / kExpertTile; ++t) p.tiles[1 + t] = e;
+    for (int t = first / p.tile; t < upto / p.tile; ++t) p.tiles[1 + t] = e;
     if (e == p.num_experts - 1) {
       p.rows[e + 1] = upto;
-      p.tiles[0] = upto / kExpertTile;
+      p.tiles[0] = upto / p.tile;
     }
   }
   // the padding: a warp takes an expert
@@ -112,6 +112,7 @@ __device__ __forceinline__ void scatter_chunk(const ExpertPlan& p, int64_t first
 // one chunk: all of it in one launch
 __global__ void __launch_bounds__(kThreads) plan_one_kernel(const ExpertPlan p) {
   __shared__ int count[kWarps][kMaxExperts], start[kMaxExperts];
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   count_chunk(p, 0, count);
   __syncthreads();
   int n = 0;
@@ -197,6 +198,9 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4) gather_kernel(const ExpertP
   const int lane = threadIdx.x & 31, k = (int)a.k;
   const int64_t warp = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5), warps = (int64_t)gridDim.x * kRowWarps;
   uint16_t* dst = reinterpret_cast<uint16_t*>(a.dst);
+  // (in this order: what follows this kernel may read the plan before it waits)
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const uint16_t* other = reinterpret_cast<const uint16_t*>(a.other);
   const int64_t tokens = plan.count / k;
   for (int64_t t = warp; t < tokens; t += warps) {
@@ -255,7 +259,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4) gather_kernel(const ExpertP
     if (WEIGHTED && a.dweights && lane < k) store_any(a.dweights, a.weight_dtype, t * k + lane, my_dot);
   }
   // the padding's zeros; lane i looks at the warp's i-th row of 32
-  const int64_t rows = (int64_t)__ldg(plan.tiles) * kExpertTile;
+  const int64_t rows = (int64_t)__ldg(plan.tiles) * plan.tile;
   for (int64_t r0 = warp; r0 < rows; r0 += 32 * warps) {
     const int64_t mine = r0 + lane * warps;
     unsigned empty = __ballot_sync(0xffffffffu, mine < rows && __ldg(plan.src_of + mine) < 0);
@@ -272,6 +276,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4) combine_kernel(const Expert
   const int64_t warp = (int64_t)blockIdx.x * kRowWarps + (threadIdx.x >> 5), warps = (int64_t)gridDim.x * kRowWarps;
   const int k = (int)a.k;
   const uint16_t* rows = reinterpret_cast<const uint16_t*>(a.rows);
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   for (int64_t t = warp; t < a.tokens; t += warps) {
     const uint16_t* res = reinterpret_cast<const uint16_t*>(a.residual) + t * a.ld_res;
     T* out = reinterpret_cast<T*>(a.out) + t * a.ld_out;
@@ -441,12 +446,39 @@ static cudaError_t launch_few(const ExpertFew& a, cudaStream_t s) {
   return cudaLaunchKernelEx(&cfg, few_down_kernel<T, VEC>, a);
 }
 
+// dependent: a programmatic dependent of the kernel before it on the stream
+template <typename... P, typename... A>
+static cudaError_t launch(void (*k)(P...), int blocks, bool dependent, cudaStream_t s, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(32 * kRowWarps);
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = dependent ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, k, args...);
+}
+
 static bool aligned(const void* p, int64_t ld) { return ld % 8 == 0 && (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 
 }  // namespace experts
 
-int64_t expert_tiles(int64_t count, int64_t experts) {
-  return (count + (kExpertTile - 1) * std::min(count, experts)) / kExpertTile;
+int64_t expert_tiles(int64_t count, int64_t experts, int tile) {
+  return (count + (tile - 1) * std::min(count, experts)) / tile;
+}
+// Up to 64 rows an expert on average (in every expert) the split products, whose tiles are 32 or 64 rows, read the
+// weights about as fast as gated_kernel with its 256-row tiles and start and end sooner; so they do while their blocks
+// fit the device at once.  Microseconds of a call without gradients, in a graph, weights not in L2, tiles of 32 / 64 / 256
+// rows: 2 experts of 768 x 1024: 37 rows each 24 / 25 / 37, 128 each 36 / 31 / 41, 512 each 80 / 55 / 43; 8 of 1024 x
+// 2736: 9 each 55 / 59 / 72, 32 each 66 / 64 / 76, 64 each 80 / 70 / 76, 128 each 119 / 94 / 76; 64 of 512 x 680: 4 each
+// 59 / 66 / 76, 64 each 102 / 88 / 82.
+int expert_tile(int64_t count, int64_t experts, int64_t H, int64_t N) {
+  if (experts * std::max(H, N) >= INT32_MAX) return kExpertTile;  // (the split products' rows of all experts' weights)
+  if (count <= 24 * experts) return 32;
+  const int64_t blocks = expert_tiles(count, experts, 64) * ((H + 63) / 64);
+  return count <= 64 * experts || blocks <= 2 * tc::sm_count() ? 64 : kExpertTile;
 }
 static int64_t plan_chunks(int64_t count) { return (count + experts::kChunk - 1) / experts::kChunk; }
 int64_t expert_plan_hist(int64_t count, int64_t num_experts) {
@@ -455,7 +487,7 @@ int64_t expert_plan_hist(int64_t count, int64_t num_experts) {
 }
 
 cudaError_t expert_plan(const ExpertPlan& p, cudaStream_t s) {
-  if (p.num_experts < 1 || p.num_experts > kMaxExperts || p.count < 1) return cudaErrorInvalidValue;
+  if (p.num_experts < 1 || p.num_experts > kMaxExperts || p.count < 1 || p.tile < 1) return cudaErrorInvalidValue;
   const int chunks = (int)plan_chunks(p.count);
   if (chunks == 1) {
     experts::plan_one_kernel<<<1, experts::kThreads, 0, s>>>(p);
@@ -467,14 +499,13 @@ cudaError_t expert_plan(const ExpertPlan& p, cudaStream_t s) {
   return cudaGetLastError();
 }
 
-cudaError_t expert_gather(const ExpertGather& a, cudaStream_t s) {
-  const int64_t rows = kExpertTile * expert_tiles(a.plan->count, a.plan->num_experts);
+cudaError_t expert_gather(const ExpertGather& a, bool dependent, cudaStream_t s) {
+  const int64_t rows = a.plan->tile * expert_tiles(a.plan->count, a.plan->num_experts, a.plan->tile);
   const int blocks = (int)std::min<int64_t>((rows + experts::kRowWarps - 1) / experts::kRowWarps, 4 * tc::sm_count());
   if (!experts::aligned(a.dst, a.ld_dst) || (a.dweights && !experts::aligned(a.other, a.ld_other)))
     return cudaErrorInvalidValue;
   const bool vec = experts::aligned(a.rows, a.ld_rows) && a.n % 8 == 0;
-#define NSW_GATHER(T, W, V) \
-  experts::gather_kernel<T, W, V><<<blocks, 32 * experts::kRowWarps, 0, s>>>(*a.plan, a)
+#define NSW_GATHER(T, W, V) return experts::launch(experts::gather_kernel<T, W, V>, blocks, dependent, s, *a.plan, a)
   if (!a.weights) {  // a copy: either 16-bit type
     if (vec)
       NSW_GATHER(__half, false, true);
@@ -492,15 +523,14 @@ cudaError_t expert_gather(const ExpertGather& a, cudaStream_t s) {
       NSW_GATHER(__half, true, false);
   }
 #undef NSW_GATHER
-  return cudaGetLastError();
 }
 
-cudaError_t expert_combine(const ExpertCombine& a, cudaStream_t s) {
+cudaError_t expert_combine(const ExpertCombine& a, bool dependent, cudaStream_t s) {
   if (!experts::aligned(a.rows, a.ld_rows)) return cudaErrorInvalidValue;
   const int blocks = (int)std::min<int64_t>((a.tokens + experts::kRowWarps - 1) / experts::kRowWarps, 4 * tc::sm_count());
   const bool vec = a.n % 8 == 0 && experts::aligned(a.out, a.ld_out) &&
                    (!a.residual || experts::aligned(a.residual, a.ld_res));
-#define NSW_COMBINE(T, V) experts::combine_kernel<T, V><<<blocks, 32 * experts::kRowWarps, 0, s>>>(a)
+#define NSW_COMBINE(T, V) return experts::launch(experts::combine_kernel<T, V>, blocks, dependent, s, a)
   if (a.dtype == kBF16) {
     if (vec)
       NSW_COMBINE(__nv_bfloat16, true);
@@ -513,7 +543,14 @@ cudaError_t expert_combine(const ExpertCombine& a, cudaStream_t s) {
       NSW_COMBINE(__half, false);
   }
 #undef NSW_COMBINE
-  return cudaGetLastError();
+}
+
+// The kernels for a few assignments read an expert's weights for each of them, the others once; from 64 MB of them on that
+// costs more than sorting.  Microseconds as above, here and by tiles of 32 rows: 2 experts of 768 x 1024 (4.7 MB): 4
+// assignments 14 / 24, 12 21 / 24, 24 33 / 24; 8 of 1024 x 2736 (16.8 MB): 4 39 / 37, 12 53 / 45; 64 of 512 x 680 (2.1 MB):
+// 4 14 / 23, 32 31 / 35; 4 of 128 x 344: 4 10 / 20, 32 14 / 18.
+bool expert_few_pays(int64_t count, int64_t H, int64_t K, int64_t N) {
+  return count <= kExpertFewRows && count * H * (2 * K + N) <= (int64_t)32 << 20;
 }
 
 cudaError_t expert_few(const ExpertFew& a, cudaStream_t s) {

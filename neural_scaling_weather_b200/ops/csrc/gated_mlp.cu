@@ -929,6 +929,7 @@ struct SplitParams {
   void *out0, *out1, *out2;
   int64_t ldin, ldout, ldaux;
   int bias_dtype, act, dependent;
+  const int* tiles;  // grouped: the number of token tiles, then each one's expert
 };
 
 template <typename T, int NTOK, int STAGES>
@@ -990,6 +991,16 @@ __global__ void __launch_bounds__(kSplitThreads, NTOK <= 64 ? 2 : 1) split_kerne
   const int kb_begin = (int)((int64_t)slice * p.kb / slices), kb_end = (int)((int64_t)(slice + 1) * p.kb / slices);
   const int nkb = kb_end - kb_begin;
   volatile int* abort_flag = &S.abort_flag;
+  int w_row = 0;  // the expert's first row of the weights
+  if (MODE == kUp || MODE == kDown)
+    if (p.tiles) {
+      // (written two kernels ago: by way of L2, past what an L1 may hold of its earlier contents)
+      if ((int)blockIdx.z >= __ldcg(p.tiles)) {  // the whole cluster; nobody overtakes the kernel before
+        if (p.dependent) asm volatile("griddepcontrol.wait;" ::: "memory");
+        return;
+      }
+      w_row = __ldcg(p.tiles + 1 + blockIdx.z) * (int)p.N;
+    }
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   if (threadIdx.x == 64) {
     prefetch_map(&p.w0);
@@ -1028,10 +1039,10 @@ __global__ void __launch_bounds__(kSplitThreads, NTOK <= 64 ? 2 : 1) split_kerne
           tma_load_2d(&S.w[st][0], m, &S.full[st], (int)n0, k0);
           tma_load_2d(&S.w[st][64 * BK], m, &S.full[st], (int)n0 + 64, k0);
         } else if (MODE == kUp) {
-          tma_load_2d(&S.w[st][0], &p.w0, &S.full[st], k0, (int)n0);
-          tma_load_2d(&S.w[st][64 * BK], &p.w1, &S.full[st], k0, (int)n0);
+          tma_load_2d(&S.w[st][0], &p.w0, &S.full[st], k0, w_row + (int)n0);
+          tma_load_2d(&S.w[st][64 * BK], &p.w1, &S.full[st], k0, w_row + (int)n0);
         } else {
-          tma_load_2d(&S.w[st][0], m, &S.full[st], k0, (int)n0);
+          tma_load_2d(&S.w[st][0], m, &S.full[st], k0, w_row + (int)n0);
         }
       };
       auto load_x = [&](int i) {
@@ -1228,11 +1239,12 @@ static cudaError_t launch_split(const GatedArgs& a, int slices, bool dependent, 
   SplitParams p;
   memset(&p, 0, sizeof(p));
   const int rows = MODE == kUp ? 64 : 128;
+  const int64_t w_rows = (a.groups ? a.groups->experts : 1) * a.N;
   bool ok = make_map(&p.x0, a.a0, a.M, a.K, a.lda, NTOK, a.dtype);
   if (MODE == kDx) ok = ok && make_map(&p.x1, a.a1, a.M, a.K, a.lda, NTOK, a.dtype);
   ok = ok && (mn ? make_map_mn(&p.w0, a.b0, a.K, a.N, a.ldb0, a.dtype)
-                 : make_map(&p.w0, a.b0, a.N, a.K, a.ldb0, rows, a.dtype));
-  if (MODE == kUp) ok = ok && make_map(&p.w1, a.b1, a.N, a.K, a.ldb1, rows, a.dtype);
+                 : make_map(&p.w0, a.b0, w_rows, a.K, a.ldb0, rows, a.dtype));
+  if (MODE == kUp) ok = ok && make_map(&p.w1, a.b1, w_rows, a.K, a.ldb1, rows, a.dtype);
   if (MODE == kDx) ok = ok && make_map_mn(&p.w1, a.b1, a.K, a.N, a.ldb1, a.dtype);
   if (!ok) return cudaErrorInvalidValue;
   p.M = a.M;
@@ -1252,6 +1264,7 @@ static cudaError_t launch_split(const GatedArgs& a, int slices, bool dependent, 
   p.ldaux = a.ldaux;
   p.act = a.act;
   p.dependent = dependent;
+  if (a.groups) p.tiles = a.groups->tiles;
   const uint32_t fmt = a.dtype == kBF16 ? 1u : 0u;
   const uint32_t idesc = (1u << 4) | (fmt << 7) | (fmt << 10) | (mn ? 1u << 15 : 0u) |
                          ((uint32_t)(NTOK >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
@@ -1339,8 +1352,28 @@ static SplitPlan plan_split(const GatedArgs& a) {
   return best;
 }
 
+// Grouped, a few rows an expert: these products are bound by reading every expert's weights once, so the depth is split
+// until there are about as many CTAs as the device holds, two an SM (8 experts of 2736 x 1024, 74 rows: the down
+// projection's 64 CTAs times four, the call 57 us, with one slice 65; the up projection has 344: with one slice 65 us,
+// with two 66, with four 76).
+static int few_rows_slices(const GatedArgs& a) {
+  const int64_t units = a.mode == kGatedUp ? 64 : 128, kb = (a.K + BK - 1) / BK;
+  const int64_t ctas = a.M / a.groups->tile * ((a.N + units - 1) / units);
+  int slices = 1;
+  while (2 * slices <= std::min<int64_t>(kb, 4) && 2 * slices * ctas <= 2 * sm_count()) slices *= 2;
+  return slices;
+}
+
 template <typename T, int MODE>
 static cudaError_t launch_any(const GatedArgs& a, bool dependent, cudaStream_t s) {
+  if constexpr (MODE == kUp || MODE == kDown) {
+    if (a.groups && a.groups->tile < kExpertTile) {
+      const int slices = few_rows_slices(a);
+      if (a.groups->tile == 32) return launch_split<T, MODE, 32, 5>(a, slices, dependent, s);
+      if (a.groups->tile == 64) return launch_split<T, MODE, 64, 4>(a, slices, dependent, s);
+      return cudaErrorInvalidValue;
+    }
+  }
   if (a.groups) return launch_gated<T, MODE, true>(a, s);
   const SplitPlan plan = plan_split(a);
   if (!plan.use) return launch_gated<T, MODE>(a, s);

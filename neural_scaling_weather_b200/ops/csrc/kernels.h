@@ -221,12 +221,14 @@ cudaError_t wgrad_tcgen05(const WgradArgs& a, const WgradPlan& plan, cudaStream_
 //   kGatedDh    d = a0 b0 with b0 [K, N]; out0 = d * in1 * act'(in0), out1 = d * act(in0) (in: g, u, ldin;
 //               out0 in rows of ldout, out1 in rows of ldaux)
 //   kGatedDx    out0 = a0 b0 + a1 b1 with b0, b1 [K, N]; rows of out0 of any alignment
-// Products of stacked weights, one matrix an expert (groups set): the rows are whole 256-row tiles of one expert each,
+// Products of stacked weights, one matrix an expert (groups set): the rows are whole tiles of one expert each,
 // the weights [experts][rows][cols] in rows of ldb, M the most rows there can be; no biases, residual or column sums.
+// tile is kExpertTile, or for kGatedUp and kGatedDown without out1 32 or 64 (the forms for a few rows an expert).
 struct GatedGroups {
   int64_t experts;
   const int* tiles;  // device: [0] row tiles, then each one's expert
   const int* rows;   // device: [experts + 1] first rows of the experts' tiles
+  int tile;
 };
 enum GatedMode : int { kGatedUp = 0, kGatedDown = 1, kGatedDh = 2, kGatedDx = 3 };
 struct GatedArgs {
@@ -302,20 +304,22 @@ constexpr int kPadCopies = 5;
 cudaError_t pad_copy(const PadCopy* v, int count, cudaStream_t s);
 
 // ---- routed experts (experts.cu) ------------------------------------------------------------------------
-constexpr int kMaxExperts = 512, kMaxChosen = 16, kExpertTile = 256;
+constexpr int kMaxExperts = 512, kMaxChosen = 16, kExpertTile = 256;  // (rows of gated_kernel's tiles)
 // Assignments (token t's j-th expert: index t k + j) sorted by expert, in order within an expert; an index outside
-// [0, experts) is left out.  Rows of an expert start at a multiple of kExpertTile.
+// [0, experts) is left out.  Rows of an expert start at a multiple of tile.
 struct ExpertPlan {
   const int64_t* experts;  // [count]
   int64_t count;
-  int num_experts;
-  int* tiles;   // [1 + expert_tiles(count, num_experts)]: the number of row tiles, then each one's expert
+  int num_experts, tile;
+  int* tiles;   // [1 + expert_tiles(count, num_experts, tile)]: the number of row tiles, then each one's expert
   int* rows;    // [num_experts + 1]: first row of each expert
   int* row_of;  // [count]: an assignment's row, -1: none
-  int* src_of;  // [kExpertTile * expert_tiles(..)]: a row's assignment, -1: padding (rows past the last tile: unset)
+  int* src_of;  // [tile * expert_tiles(..)]: a row's assignment, -1: padding (rows past the last tile: unset)
   int* hist;    // expert_plan_hist(count, num_experts) integers
 };
-int64_t expert_tiles(int64_t count, int64_t experts);  // the most row tiles there can be
+// rows of a tile for calls without gradients: kExpertTile, or what the products' forms for a few rows an expert take
+int expert_tile(int64_t count, int64_t experts, int64_t H, int64_t N);
+int64_t expert_tiles(int64_t count, int64_t experts, int tile);  // the most row tiles there can be
 int64_t expert_plan_hist(int64_t count, int64_t experts);
 cudaError_t expert_plan(const ExpertPlan& p, cudaStream_t s);
 // dst[r] = rows[src_of[r] / k] (zeros for padding), for the rows of all tiles; with weights, times
@@ -327,7 +331,7 @@ struct ExpertGather {
   void *dst, *dweights;
   int dtype, weight_dtype;  // of rows, other and dst; of weights and dweights
 };
-cudaError_t expert_gather(const ExpertGather& a, cudaStream_t s);
+cudaError_t expert_gather(const ExpertGather& a, bool dependent, cudaStream_t s);
 // out[t] = residual[t] (null: 0) + sum over j of weights[t k + j] (null: 1) rows[row_of[t k + j]]
 struct ExpertCombine {
   const int* row_of;
@@ -336,9 +340,9 @@ struct ExpertCombine {
   void* out;
   int dtype, weight_dtype;
 };
-cudaError_t expert_combine(const ExpertCombine& a, cudaStream_t s);
+cudaError_t expert_combine(const ExpertCombine& a, bool dependent, cudaStream_t s);
 // The whole network for a few tokens (at most kExpertFewRows assignments): h [tokens k][ldh] is workspace
-constexpr int kExpertFewRows = 16;
+constexpr int kExpertFewRows = 32;
 struct ExpertFew {
   const void *x, *wg, *wu, *wd, *weights, *residual;
   const int64_t* experts;
@@ -346,6 +350,7 @@ struct ExpertFew {
   int64_t ldx, ldwg, ldwu, ldwd, ldh, ldres;  // y is contiguous; weights [num_experts][rows][ld]
   int tokens, k, num_experts, K, H, N, act, dtype, weight_dtype;
 };
+bool expert_few_pays(int64_t count, int64_t H, int64_t K, int64_t N);  // (false past kExpertFewRows)
 cudaError_t expert_few(const ExpertFew& a, cudaStream_t s);
 
 // ---- router (route.cu) -------------------------------------------------------------------------------------

@@ -245,6 +245,20 @@ def test_experts_uneven_choices():
         assert rel(few, expert_exact(x[:7], wt[:7], c[:7], w, res[:7], "silu")) < 4 * U[BF]
 
 
+@pytest.mark.parametrize("M,E,H", [(3, 4, 64), (30, 2, 64), (300, 5, 136), (3000, 3, 1024)])
+def test_experts_all_left_out(M, E, H):
+    """No assignment inside the experts: the residual, with gradients of zero, whichever kernels run."""
+    x, weights, _, w, res, dy = expert_inputs(M, 2, E, 64, H, 72, BF)
+    chosen = torch.where(torch.rand(M, 2, device=DEV) < 0.5, -1, E)
+    with torch.no_grad():
+        assert torch.equal(ops.expert_mlp(x, weights, chosen, *w, residual=res), res)
+        assert ops.expert_mlp(x, weights, chosen, *w).abs().max() == 0
+    leaves = [t.requires_grad_() for t in (x, weights, *w)]
+    y = ops.expert_mlp(x, weights, chosen, *w, residual=res)
+    assert torch.equal(y, res)
+    assert all(g.abs().max() == 0 for g in torch.autograd.grad(y, leaves, dy))
+
+
 def test_experts_non_finite_tokens_stay_apart():
     x, wt, chosen, w, _, _ = expert_inputs(300, 2, 4, 64, 72, 64, BF, seed=2)
     x[17] = float("nan")
