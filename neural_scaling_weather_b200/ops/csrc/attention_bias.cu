@@ -56,6 +56,7 @@ constexpr float kAbsorbs = 1099511627776.f;  // 2^40
 __global__ void __launch_bounds__(256) prepare_kernel(const AnyMatrix table, const AnyMatrix qw, const AnyMatrix kw, const AttnBias b,
                                                       int heads, int hd, int nt, int ny, int nx, float scale,
                                                       float* __restrict__ tab) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ float hi_w[8], held[1160];  // (windows of 192 tokens have at most 1155 displacements)
   const int h = blockIdx.x, n = nt * ny * nx;
   float* out = tab + (int64_t)h * b.stride;
@@ -223,7 +224,7 @@ __device__ __forceinline__ void load_table(float* tab, const AttnBias& b, int en
   const int second = second_copy(entries);
 #pragma unroll 4
   for (int i = threadIdx.x; i < entries; i += blockDim.x) {
-    const float v = __ldg(src + i) - less;
+    const float v = src[i] - less;  // (no read-only load: the forward may have begun before this was written)
     const int at = REVERSED ? entries - 1 - i : i;
     tab[at] = v;
     if (at > 0) tab[second + at - 1] = v;
@@ -495,7 +496,7 @@ struct FwdSmem {
 };
 template <typename T, int HD, bool PAIR>
 __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
-    fwd_kernel(const T* __restrict__ qkv, const AttnBias bias, const float* __restrict__ norms, T* __restrict__ out,
+    fwd_kernel(const T* __restrict__ qkv, const AttnBias bias, const float* norms, T* __restrict__ out,
                float2* __restrict__ lse, const __grid_constant__ AttnGeom g, const __grid_constant__ Order o) {
   constexpr int RS = HD + 8, KS = HD / 16, CH = HD / 8;
   constexpr uint32_t kTile = 16 * RS * sizeof(T), kOffTile = kOffRow * off_bytes<PAIR>();
@@ -508,6 +509,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
   const int64_t C = (int64_t)g.nh * HD;
   const T* base = qkv + (int64_t)head * HD;
 
+  asm volatile("griddepcontrol.wait;" ::: "memory");  // (for the table and the norms' weights)
   const float bound = bias.tab[(int64_t)head * bias.stride];
   const bool exact = !(bound <= kMostBound);
   const float less = exact ? 0.f : bound - Bound<T>::top;  // in the entries
@@ -527,8 +529,9 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
   }
   __syncthreads();
   uint32_t raw[KS][4];
-  if (warp < o.tiles)  // the first tile's raw queries, on their way under what follows
-    raw_rows<T, HD>(raw, base, g.qkv_stride, S.tok, warp * 16, L, lane);
+  const int first = blockIdx.y * nw + warp;
+  if (first < o.tiles)  // the first tile's raw queries, on their way under what follows
+    raw_rows<T, HD>(raw, base, g.qkv_stride, S.tok, first * 16, L, lane);
   for (int i = threadIdx.x; i < rows * CH; i += nthreads) {
     const int r = i / CH, c = i % CH;
     T* dst = S.v + r * RS + 8 * c;
@@ -564,8 +567,8 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
   const uint32_t k_at = rows_nt<T, RS>(S.k, lane), v_at = rows_nn<T, RS>(S.v, lane);
   const uint32_t off_at = smem_u32(S.offs) + tq * off_bytes<PAIR>();
   const int whole = mixed ? 0 : L / 16;  // tiles of keys without a mask
-  for (int qt = warp; qt < o.tiles; qt += nw) {
-    if (qt != warp) raw_rows<T, HD>(raw, base, g.qkv_stride, S.tok, qt * 16, L, lane);
+  for (int qt = first; qt < o.tiles; qt += nw * gridDim.y) {
+    if (qt != first) raw_rows<T, HD>(raw, base, g.qkv_stride, S.tok, qt * 16, L, lane);
     const int r0 = qt * 16 + gq, r1 = r0 + 8;
     uint32_t qa[KS][4];
     {
@@ -1227,7 +1230,7 @@ constexpr size_t kBlockSmem = 232448, kSmSmem = 233472;
 
 template <typename T, int HD, bool PAIR>
 cudaError_t launch_fwd(const void* qkv, const AttnBias& bias, const float* norms, void* out, float* lse, const AttnGeom& g,
-                       cudaStream_t s) {
+                       int sms, cudaStream_t s) {
   const Order o = order_of(g, bias);
   FwdSmem<T, HD> S;
   const size_t smem = S.carve(nullptr, o);
@@ -1235,9 +1238,21 @@ cudaError_t launch_fwd(const void* qkv, const AttnBias& bias, const float* norms
   NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const int64_t items = (int64_t)g.B * (g.H / g.wh) * (g.W / g.ww) * g.nh;
   if (items > INT32_MAX) return cudaErrorInvalidValue;
-  k<<<(unsigned)items, 32 * std::min(o.tiles, kFwdWarps), smem, s>>>((const T*)qkv, bias, norms, (T*)out,
-                                                                    reinterpret_cast<float2*>(lse), g, o);
-  return cudaGetLastError();
+  const int warps = std::min(o.tiles, kFwdWarps);
+  // Few items: two blocks share one's queries, so that a warp has at most one tile (16 heads of one window of 162 tokens:
+  // with the preparation 16.4 us in a graph, one block 20.5; 128 items 20.5 and 22.6, 224 items 30.5 and 26.6).
+  const int parts = items <= sms && o.tiles > warps ? 2 : 1;
+  cudaLaunchConfig_t cfg = {};
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.gridDim = dim3((unsigned)items, (unsigned)parts);
+  cfg.blockDim = dim3(32 * warps);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, k, (const T*)qkv, bias, norms, (T*)out, reinterpret_cast<float2*>(lse), g, o);
 }
 
 // How many blocks the device holds at once, and whether keys have two buffers: where that costs no block of an SM
@@ -1336,10 +1351,10 @@ cudaError_t attn_bias_prepare(const AnyMatrix& table, const AnyMatrix& qw, const
 }
 
 cudaError_t attn_bias_fwd(const void* qkv, const AttnBias& bias, const float* norms, void* out, float* lse,
-                          const AttnGeom& g, int dtype, cudaStream_t s) {
+                          const AttnGeom& g, int dtype, int sms, cudaStream_t s) {
   if (!attn_bias_ok(g, dtype)) return cudaErrorInvalidValue;
   return attn_bias::dispatch<true>(g, bias, dtype, [&](auto t, auto hd, auto pair) {
-    return attn_bias::launch_fwd<decltype(t), hd(), pair()>(qkv, bias, norms, out, lse, g, s);
+    return attn_bias::launch_fwd<decltype(t), hd(), pair()>(qkv, bias, norms, out, lse, g, sms, s);
   });
 }
 

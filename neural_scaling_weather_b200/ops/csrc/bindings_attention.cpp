@@ -53,7 +53,7 @@ std::vector<Tensor> attn_bias_fwd(const Tensor& qkv, const Tensor& qw, const Ten
   check(nsw::attn_bias_prepare(table, q, k, g, bias, tab.data_ptr<float>(), stream()), "attn_bias_prepare");
   bias.tab = tab.data_ptr<float>();
   check(nsw::attn_bias_fwd(qkv.data_ptr(), bias, norms, out.data_ptr(), lse.data_ptr<float>(), g, dt_code(qkv, "qkv"),
-                           stream()),
+                           sm_count(qkv), stream()),
         "window_attention");
   return {out, lse, tab};
 }

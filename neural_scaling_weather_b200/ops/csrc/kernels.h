@@ -96,7 +96,7 @@ cudaError_t attn_bias_prepare(const AnyMatrix& table, const AnyMatrix& qw, const
 // a row, (what the exponentials are less, log2 of their sum): added up, they would lose the second where the logits are
 // far from zero.  norms: the weights of q and of k, as prepared.
 cudaError_t attn_bias_fwd(const void* qkv, const AttnBias& bias, const float* norms, void* out, float* lse,
-                          const AttnGeom& g, int dtype, cudaStream_t s);
+                          const AttnGeom& g, int dtype, int sms, cudaStream_t s);
 // Rows of partial sums that the backward leaves: of the norms' weights (hd floats each) and of the bias (buckets each)
 struct AttnBiasPlan {
   int blocks, k_bufs;      // 0 blocks: head_dim 128, a block for each window and head
