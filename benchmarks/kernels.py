@@ -239,6 +239,37 @@ def bench_patch(a):
     report("patchify bf16 70x720x1440 p4", ms, None, y2.numel() * 4)
 
 
+def bench_routed(a):
+    """Biased window attention, the router and the routed experts through their public entry points (--H x --W tokens of
+    --heads heads of 64; --M tokens at width 1024, two of eight experts of hidden width 1368)."""
+    from neural_scaling_weather_b200 import ops
+
+    dt, nh, hd, k = torch.bfloat16, a.heads, 64, 2
+    rand = lambda *s, std=1.0: (torch.randn(*s, device="cuda") * std).to(dt).requires_grad_()  # noqa: E731
+
+    def both(name, f, leaves, dy, flops=None, nbytes=None):
+        with torch.no_grad():
+            report(f"{name} forward", timeit(f, a.iters), flops, nbytes)
+        report(f"{name} forward + backward", timeit(lambda: torch.autograd.grad(f(), leaves, dy), a.iters),
+               flops and 3 * flops, nbytes and 3 * nbytes)
+
+    geom = WindowGeometry(window=(9, 18), shift=(4, 9), mask=True, mask_shift=4, h_global=a.H)
+    args = [rand(1, 1, a.H, a.W, 3 * nh * hd), rand(hd), rand(hd), rand(nh, geom.num_buckets(1))]
+    both(f"window_attention with a bias, tokens={a.H * a.W} heads={nh}",
+         lambda: ops.window_attention(*args[:3], nh, hd, geom, hd ** -0.5, rel_bias=args[3]), args,
+         rand(1, 1, a.H, a.W, nh * hd).detach(), 4 * a.H * a.W * 162 * hd * nh)
+    M, K, H, E = a.M, 1024, 1368, 8
+    z = rand(M, 64)
+    both(f"route_tokens {M}x64 top {k}", lambda: ops.route_tokens(z, k)[::2], [z],
+         [torch.randn(M, k, device="cuda"), torch.ones((), device="cuda")], None, M * (2 * 64 + 12 * k))
+    with torch.no_grad():
+        weights, experts, _ = ops.route_tokens(torch.randn(M, E, device="cuda"), k)
+    leaves = [rand(M, K), weights.requires_grad_(), rand(E, H, K, std=K ** -0.5), rand(E, H, K, std=K ** -0.5),
+              rand(E, K, H, std=H ** -0.5)]
+    both(f"expert_mlp {M}x{K}x{H}, {k} of {E}",
+         lambda: ops.expert_mlp(leaves[0], leaves[1], experts, *leaves[2:]), leaves, rand(M, K).detach(), 6 * M * k * K * H)
+
+
 def bench_block_ops(a):
     """The gated feed-forward network, the norms around a residual connection and gradient clipping, through their
     public entry points (--M tokens at width 1024, hidden 2736)."""
@@ -292,7 +323,7 @@ def bench_block_ops(a):
 def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("kernel", choices=["gemm", "block", "attention", "wgrad", "amse", "rmsnorm", "adamw", "sse",
-                                       "patch", "colsum", "blockops", "all"])
+                                       "patch", "colsum", "blockops", "routed", "all"])
     ap.add_argument("--M", type=int, default=64800)
     ap.add_argument("--N", type=int, default=3072)
     ap.add_argument("--K", type=int, default=1024)
@@ -326,6 +357,8 @@ def main():
         bench_patch(a)
     if a.kernel in ("blockops", "all"):
         bench_block_ops(a)
+    if a.kernel in ("routed", "all"):
+        bench_routed(a)
     if a.kernel in ("rmsnorm", "all"):
         a2 = argparse.Namespace(**vars(a))
         if a.kernel == "all":
