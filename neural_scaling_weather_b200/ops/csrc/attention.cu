@@ -122,17 +122,17 @@ __device__ __forceinline__ void norm_rows(T* s, const float* w, int L, float* rs
 
 // A row's place in the entries of a relative position bias: the entry of query i and key j is at
 // center + off(i) - off(j) (see attention_bias.cu)
-__device__ __forceinline__ int bias_off(const AttnGeom& g, int pitch, int i) {
+__device__ __forceinline__ int bias_off(const AttnGeom& g, int i) {
   const int wa = g.wh * g.ww, t = i / wa, r = i - t * wa, y = r / g.ww;
-  return (t * (2 * g.wh - 1) + y) * pitch + (r - y * g.ww);
+  return (t * (2 * g.wh - 1) + y) * (2 * g.ww - 1) + (r - y * g.ww);
 }
-__device__ __forceinline__ int bias_center(const AttnGeom& g, int pitch) {
-  return 4 + ((g.T - 1) * (2 * g.wh - 1) + g.wh - 1) * pitch + g.ww - 1;
+__device__ __forceinline__ int bias_center(const AttnGeom& g) {
+  return 4 + ((g.T - 1) * (2 * g.wh - 1) + g.wh - 1) * (2 * g.ww - 1) + g.ww - 1;
 }
 __device__ __forceinline__ void load_bias(float* tab, short* off, const AttnBias& b, const AttnGeom& g, int h, int L,
                                           int rows) {
   for (int i = threadIdx.x; i < b.stride; i += blockDim.x) tab[i] = b.tab[(int64_t)h * b.stride + i];
-  for (int i = threadIdx.x; i < rows; i += blockDim.x) off[i] = i < L ? (short)bias_off(g, b.pitch, i) : 0;
+  for (int i = threadIdx.x; i < rows; i += blockDim.x) off[i] = i < L ? (short)bias_off(g, i) : 0;
 }
 static size_t bias_bytes(const AttnBias& b, int rows) {  // of tab and off, rounded up
   return b.tab ? ((size_t)b.stride * 4 + (size_t)rows * 2 + 15) / 16 * 16 : 0;
@@ -385,11 +385,6 @@ __device__ __forceinline__ void store_rows_c(float (*acc)[4], int row0, int lane
   }
 }
 
-__device__ __forceinline__ void add_bucket(float* sums, int at, int pitch, int nx, float v) {  // `at` in rows of pitch
-  const int row = at / pitch;
-  sums[row * nx + at - row * pitch] += v;
-}
-
 // P of one key and two query rows with a bias; `tab` is the key's center in the entries
 __device__ __forceinline__ void biased_probs(float s0, float s1, float sl2, const float* tab, const short* off, int r0, int r1,
                                              int key_label, int label0, int label1, float m0, float m1, const float* ll,
@@ -439,7 +434,7 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
   short* sOff = reinterpret_cast<short*>(sTab + (BIAS ? bias.stride : 0));
   float* sLl = reinterpret_cast<float*>(sOff + (BIAS ? lp : 0));  // BIAS: log2 of a row's sum; sLse its largest logit
   float* sSum = sLl + (BIAS ? lp : 0);                           // with dbias_part: the buckets, then the warps' tiles
-  const int center = BIAS ? bias_center(g, bias.pitch) : 0;
+  const int center = BIAS ? bias_center(g) : 0;
 
   const int bw = blockIdx.x, h = blockIdx.y;
   const WinPos p = win_pos(g, bw);
@@ -737,13 +732,13 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
               if (qi >= L || kj >= L) break;
               const int at = center - 4 + sOff[qi] - sOff[kj];
               if (at != cur) {
-                if (cur >= 0) add_bucket(sSum, cur, bias.pitch, 2 * g.ww - 1, sum);
+                if (cur >= 0) sSum[cur] += sum;
                 cur = at;
                 sum = 0.f;
               }
               sum += to_f(tile[i * 18 + i - shift]);
             }
-            if (cur >= 0) add_bucket(sSum, cur, bias.pitch, 2 * g.ww - 1, sum);
+            if (cur >= 0) sSum[cur] += sum;
           }
           __syncwarp();
         }

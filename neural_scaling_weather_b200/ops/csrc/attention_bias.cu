@@ -6,7 +6,10 @@
 //   bucket = ((t_i - t_j + T - 1) (2 wh - 1) + y_i - y_j + wh - 1) (2 ww - 1) + x_i - x_j + ww - 1
 //
 // A window is at most 192 tokens of one head, so its products are short: what counts is how few instructions stand around
-// them, and that several windows are worked on at once on an SM.
+// them, and that several windows are worked on at once on an SM.  64800 tokens of 16 heads of 64 in windows of 9 x 18, bf16:
+// forward 319 us (134 TFLOP/s, 1.7 TB/s), backward 855 (126 TFLOP/s); bound by the instructions of a logit (its entry from
+// shared memory, exponential, rounding) and by shared memory (75 % busy), not by products or memory.  The tcgen05 kernels of
+// the plain attention with the entries added to their logits took 463 and 1335.
 #include <float.h>
 #include <limits.h>
 
@@ -54,11 +57,10 @@ constexpr float kAbsorbs = 1099511627776.f;  // 2^40
 // costs no precision, unless that is beyond 2^40: a head of the lowest value throughout, say, absorbs the logits, as it
 // does in 64 bits, and its rows are even.  A finite entry stays finite.
 __global__ void __launch_bounds__(256) prepare_kernel(const AnyMatrix table, const AnyMatrix qw, const AnyMatrix kw, const AttnBias b,
-                                                      int heads, int hd, int nt, int ny, int nx, float scale,
-                                                      float* __restrict__ tab) {
+                                                      int heads, int hd, int n, float scale, float* __restrict__ tab) {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ float hi_w[8], held[1160];  // (windows of 192 tokens have at most 1155 displacements)
-  const int h = blockIdx.x, n = nt * ny * nx;
+  const int h = blockIdx.x;
   float* out = tab + (int64_t)h * b.stride;
   if (h == heads) {
     for (int i = threadIdx.x; i < hd; i += 256) {
@@ -87,16 +89,12 @@ __global__ void __launch_bounds__(256) prepare_kernel(const AnyMatrix table, con
   };
   // (a margin for the roundings of q and k)
   most = warp_max(most) * fabsf(scale) * (1.01f * kLog2e * (float)hd);
-  const int nf = b.y_fast ? ny : nx, ns = b.y_fast ? nx : ny;
   for (int i = threadIdx.x; i < b.stride; i += 256) {
-    const int at = i - 4, row = at / b.pitch, f = at - row * b.pitch, t = row / ns, s = row - t * ns;
     float v = 0.f;
-    if (i == 0) {
+    if (i == 0)
       v = shifted ? most : INFINITY;  // (the bound needs the largest entry to be 0)
-    } else if (at >= 0 && t < nt && f < nf) {
-      const int y = b.y_fast ? f : s, x = b.y_fast ? s : f;
-      v = entry(held[(t * ny + y) * nx + x]);
-    }
+    else if (i >= 4 && i - 4 < n)
+      v = entry(held[i - 4]);
     out[i] = v;
   }
 }
@@ -147,29 +145,25 @@ __global__ void __launch_bounds__(1024) grad_kernel(const Grads p) {
 }
 
 // ------------------------------------------------------------------------------------------------------ layout
-// Tokens of a window in the order in which the kernels take them: one of latitude and longitude fastest (extent nf), the
-// other (ns) next, time slowest.
+// Tokens of a window: longitude fastest (extent nf), latitude (ns) next, time slowest.
 struct Order {
   int nf, ns, nt, length, tiles;  // tiles of 16 tokens
-  bool y_fast;
-  int pitch, entries;             // entry of query i and key j: center + off(i) - off(j)
+  int entries;                    // entry of query i and key j: center + off(i) - off(j)
   int center;
   int nww, nwh;                   // windows across and down
   int sh, sw;                     // the shifts, in [0, H) and [0, W)
   int far;                        // rows of the shifted grid from here on are beyond the wrap
 };
-static Order order_of(const AttnGeom& g, const AttnBias& b) {
+static Order order_of(const AttnGeom& g) {
   const auto wrapped = [](int v, int n) { return (v % n + n) % n; };
   Order o;
-  o.y_fast = b.y_fast != 0;
-  o.nf = o.y_fast ? g.wh : g.ww;
-  o.ns = o.y_fast ? g.ww : g.wh;
+  o.nf = g.ww;
+  o.ns = g.wh;
   o.nt = g.T;
   o.length = g.T * g.wh * g.ww;
   o.tiles = (o.length + 15) / 16;
-  o.pitch = b.pitch;
-  o.entries = (2 * g.T - 1) * (2 * o.ns - 1) * b.pitch;
-  o.center = ((g.T - 1) * (2 * o.ns - 1) + o.ns - 1) * b.pitch + o.nf - 1;
+  o.entries = (2 * g.T - 1) * (2 * o.ns - 1) * (2 * o.nf - 1);
+  o.center = o.entries / 2;
   o.nww = g.W / g.ww;
   o.nwh = g.H / g.wh;
   o.sh = wrapped(g.sh, g.H);
@@ -199,10 +193,10 @@ __device__ __forceinline__ void next_window(const AttnGeom& g, Window& w) {
 __device__ __forceinline__ int3 place_of(const Order& o, int i) {
   const int r = (int)__fdividef(i + 0.5f, (float)o.nf), f = i - r * o.nf;
   const int t = (int)__fdividef(r + 0.5f, (float)o.ns), s = r - t * o.ns;
-  return make_int3(t, o.y_fast ? f : s, o.y_fast ? s : f);
+  return make_int3(t, s, f);
 }
 __device__ __forceinline__ int off_of(const Order& o, const int3& p) {
-  return (p.x * (2 * o.ns - 1) + (o.y_fast ? p.z : p.y)) * o.pitch + (o.y_fast ? p.y : p.z);
+  return (p.x * (2 * o.ns - 1) + p.y) * (2 * o.nf - 1) + p.z;
 }
 // Grid token of a window's token
 __device__ __forceinline__ int token_of(const AttnGeom& g, const Order& o, const Window& w, const int3& p) {
@@ -211,29 +205,16 @@ __device__ __forceinline__ int token_of(const AttnGeom& g, const Order& o, const
   if (x >= g.W) x -= g.W;
   return ((w.image + p.x) * g.H + y) * g.W + x;
 }
-// The entries of a head in shared memory, twice: a lane of the products has pairs of neighbouring tokens across and one
-// token down, whose entries are two neighbours in either order; if the fast extent and the pitch are even, the pair's
-// place has the parity of the token down, and one of the copies (the second begins one entry later) has it 8-byte
-// aligned, one load for two entries.  Their distance modulo the banks keeps the copies' reads apart.
-__host__ __device__ __forceinline__ int second_copy(int entries) { return (entries + 31) / 32 * 32 + 16; }
-__host__ __device__ __forceinline__ int table_floats(int entries) { return second_copy(entries) + (entries + 1) / 2 * 2; }
-// REVERSED: last entry first
+// The entries of a head into shared memory; REVERSED: last entry first.  They lie in rows of 2 nf - 1.  Measured beside it on
+// 64800 tokens of 16 heads, us of the forward and with the backward: rows padded so that consecutive tokens fall on consecutive
+// banks 294 and 960 for 280 and 929 (windows of 9 x 9); two copies, one shifted by an entry, so that any two neighbours are an
+// aligned pair, 313 and 1202 for 324 and 1182 (9 x 18).
 template <bool REVERSED>
 __device__ __forceinline__ void load_table(float* tab, const AttnBias& b, int entries, int head, float less) {
   const float* src = b.tab + (int64_t)head * b.stride + 4;
-  const int second = second_copy(entries);
 #pragma unroll 4
-  for (int i = threadIdx.x; i < entries; i += blockDim.x) {
-    const float v = src[i] - less;  // (no read-only load: the forward may have begun before this was written)
-    const int at = REVERSED ? entries - 1 - i : i;
-    tab[at] = v;
-    if (at > 0) tab[second + at - 1] = v;
-  }
-}
-// shared-memory address of the entry `base`; with pairs, where it and the next one are a pair
-template <bool PAIR>
-__device__ __forceinline__ uint32_t entry_at(const float* tab, int entries, int base) {
-  return smem_u32(tab + (PAIR && (base & 1) ? second_copy(entries) - 1 : 0) + base);
+  for (int i = threadIdx.x; i < entries; i += blockDim.x)  // (no read-only load: the forward may have begun before it was written)
+    tab[REVERSED ? entries - 1 - i : i] = src[i] - less;
 }
 
 __device__ __forceinline__ int2 lds_i2(uint32_t at) {
@@ -250,41 +231,23 @@ __device__ __forceinline__ void lds_f(uint32_t at, float& a) {
 
 // The eight entries of a 16 x 16 block of logits that a lane has, in the layout of mma's results: c[j][e] for row r0 (e < 2)
 // or r0 + 8 and column 8 j + 2 tq + (e & 1).  row0 / row1: addresses of the rows' entries for offset 0; off: address of the
-// offsets (in bytes) of this lane's columns of the block: columns 2 tq and 8 + 2 tq, or without pairs all four.  A row
-// of queries walks its entries backwards, so the forward has them reversed.
-template <bool PAIR>
+// offsets (in bytes) of this lane's columns of the block.  A row of queries walks its entries backwards, so the forward has
+// them reversed.
 __device__ __forceinline__ void load_block(float (&c)[2][4], uint32_t row0, uint32_t row1, uint32_t off) {
-  if (PAIR) {
-    const int2 o = lds_i2(off);
-    lds_f2(row0 + o.x, c[0][0], c[0][1]);
-    lds_f2(row1 + o.x, c[0][2], c[0][3]);
-    lds_f2(row0 + o.y, c[1][0], c[1][1]);
-    lds_f2(row1 + o.y, c[1][2], c[1][3]);
-  } else {
-    const int2 o[2] = {lds_i2(off), lds_i2(off + 8)};
+  const int2 o[2] = {lds_i2(off), lds_i2(off + 8)};
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      lds_f(row0 + o[j].x, c[j][0]);
-      lds_f(row0 + o[j].y, c[j][1]);
-      lds_f(row1 + o[j].x, c[j][2]);
-      lds_f(row1 + o[j].y, c[j][3]);
-    }
+  for (int j = 0; j < 2; ++j) {
+    lds_f(row0 + o[j].x, c[j][0]);
+    lds_f(row0 + o[j].y, c[j][1]);
+    lds_f(row1 + o[j].x, c[j][2]);
+    lds_f(row1 + o[j].y, c[j][3]);
   }
 }
-constexpr int kOffRow = 4;  // lanes' columns of a block: four times two (pairs) or four offsets
-template <bool PAIR>
-constexpr int off_bytes() {
-  return PAIR ? 8 : 16;
-}
+constexpr uint32_t kOffBytes = 16, kOffTile = 4 * kOffBytes;  // a lane's four offsets of a tile; a tile's
 // the offset of token i (4 off) to where its block's lanes look for it
-template <bool PAIR>
 __device__ __forceinline__ void put_off(int* offs, int i, int off4) {
   const int tile = i >> 4, c = i & 15, j = c >> 3, tq = (c & 7) >> 1;
-  if (PAIR) {
-    if (!(c & 1)) offs[(tile * kOffRow + tq) * 2 + j] = off4;
-  } else {
-    offs[(tile * kOffRow + tq) * 4 + 2 * j + (c & 1)] = off4;
-  }
+  offs[(tile * 4 + tq) * 4 + 2 * j + (c & 1)] = off4;
 }
 // The latitude-wrap mask: side is 0 or 1 of each token, s0 / s1 of the rows
 __device__ __forceinline__ void mask_block(float (&c)[2][4], const float* side, float s0, float s1, int col, int tq) {
@@ -481,7 +444,7 @@ struct FwdSmem {
   __host__ __device__ size_t carve(unsigned char* base, const Order& o) {
     const int rows = o.tiles * 16, RS = HD + 8;
     Carve c{base, 0};
-    tab = c.take<float>(table_floats(o.entries));
+    tab = c.take<float>(o.entries);
     k = c.take<T>(rows * RS);
     v = c.take<T>(rows * RS);
     stage = c.take<T>(16 * kFwdWarps * RS);
@@ -494,12 +457,12 @@ struct FwdSmem {
     return c.at;
   }
 };
-template <typename T, int HD, bool PAIR>
+template <typename T, int HD>
 __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
     fwd_kernel(const T* __restrict__ qkv, const AttnBias bias, const float* norms, T* __restrict__ out,
                float2* __restrict__ lse, const __grid_constant__ AttnGeom g, const __grid_constant__ Order o) {
   constexpr int RS = HD + 8, KS = HD / 16, CH = HD / 8;
-  constexpr uint32_t kTile = 16 * RS * sizeof(T), kOffTile = kOffRow * off_bytes<PAIR>();
+  constexpr uint32_t kTile = 16 * RS * sizeof(T);
   extern __shared__ __align__(128) unsigned char smem[];
   const int L = o.length, rows = o.tiles * 16, nthreads = blockDim.x, nw = nthreads / 32;
   FwdSmem<T, HD> S;
@@ -520,7 +483,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
     const int off4 = i < L ? 4 * off_of(o, p) : 0;
     S.tok[i] = i < L ? token_of(g, o, window, p) : 0;
     S.off4[i] = off4;
-    put_off<PAIR>(S.offs, i, off4);
+    put_off(S.offs, i, off4);
     S.side[i] = window.y + p.y >= o.far ? 1.f : 0.f;
   }
   for (int i = threadIdx.x; i < HD; i += nthreads) {
@@ -565,7 +528,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
   __syncthreads();
 
   const uint32_t k_at = rows_nt<T, RS>(S.k, lane), v_at = rows_nn<T, RS>(S.v, lane);
-  const uint32_t off_at = smem_u32(S.offs) + tq * off_bytes<PAIR>();
+  const uint32_t off_at = smem_u32(S.offs) + tq * kOffBytes;
   const int whole = mixed ? 0 : L / 16;  // tiles of keys without a mask
   for (int qt = first; qt < o.tiles; qt += nw * gridDim.y) {
     if (qt != first) raw_rows<T, HD>(raw, base, g.qkv_stride, S.tok, qt * 16, L, lane);
@@ -594,8 +557,8 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
         }
     }
     const int last = o.entries - 1 - o.center;
-    const uint32_t row0 = entry_at<PAIR>(S.tab, o.entries, last - (S.off4[r0] >> 2));
-    const uint32_t row1 = entry_at<PAIR>(S.tab, o.entries, last - (S.off4[r1] >> 2));
+    const uint32_t row0 = smem_u32(S.tab + last - (S.off4[r0] >> 2));
+    const uint32_t row1 = smem_u32(S.tab + last - (S.off4[r1] >> 2));
     // f(logits less m0 / m1 of their rows, key tile) for all key tiles; late: subtracted after the product
     const auto each_tile = [&](float m0, float m1, bool late, auto shifted, auto f) {
       const auto subtract = [&](float (&c)[2][4]) {
@@ -608,7 +571,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
         }
       };
       const auto before = [&](float (&c)[2][4], int kb, auto masked) {
-        load_block<PAIR>(c, row0, row1, off_at + kb * kOffTile);
+        load_block(c, row0, row1, off_at + kb * kOffTile);
         if (masked()) {
           if (mixed) mask_block(c, S.side, S.side[r0], S.side[r1], kb * 16, tq);
           if (kb * 16 + 16 > L) {  // padding keys
@@ -719,20 +682,18 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
 struct BiasSums {
   bool a_is_s;         // a: the slow extent
   int na, nb, sa, sb;  // extents and strides in tokens
-  int entries, width;  // width: entries of a place (b_i, b_j ..) that a thread has, neighbours in b_j
-  int places;          // of one (dt, da)
+  int entries;         // in all
+  int places;          // (b_i, b_j) of one (dt, da)
 };
-template <bool PAIR>
 __host__ __device__ __forceinline__ BiasSums sums_of(const Order& o) {
   BiasSums b;
-  b.a_is_s = PAIR || (2 * o.ns - 1) * o.nf * o.nf <= (2 * o.nf - 1) * o.ns * o.ns;
+  b.a_is_s = (2 * o.ns - 1) * o.nf * o.nf <= (2 * o.nf - 1) * o.ns * o.ns;
   b.na = b.a_is_s ? o.ns : o.nf;
   b.nb = b.a_is_s ? o.nf : o.ns;
   b.sa = b.a_is_s ? o.nf : 1;
   b.sb = b.a_is_s ? 1 : o.nf;
-  b.width = PAIR ? 2 : 1;
   b.entries = (2 * o.nt - 1) * (2 * b.na - 1) * b.nb * b.nb;
-  b.places = b.nb * (b.nb / b.width);
+  b.places = b.nb * b.nb;
   return b;
 }
 
@@ -747,7 +708,6 @@ struct BwdSmem {
   __host__ __device__ size_t carve(unsigned char* base, const Order& o, int entries, int k_bufs) {
     const int rows = o.tiles * 16, RS = HD + 8;
     Carve c{base, 0};
-    tab = c.take<float>(table_floats(o.entries));
     acc = c.take<float>(entries);
     q = c.take<T>(rows * RS * (3 + k_bufs));
     v = q + rows * RS;
@@ -768,6 +728,7 @@ struct BwdSmem {
     kw = c.take<float>(HD);
     kn = c.take<float>(HD);  // with ln 2
     side = c.take<float>(2 * rows);
+    tab = c.take<float>(o.entries);
     return c.at;
   }
 };
@@ -850,16 +811,16 @@ __device__ __forceinline__ void put_cols(float* dst, const float (&sums)[2], int
 }
 
 constexpr int kBwdWarps = 12;  // 192 tokens
-template <typename T, int HD, bool PAIR>
+template <typename T, int HD>
 __global__ void __launch_bounds__(32 * kBwdWarps, 1)
     bwd_kernel(const T* __restrict__ qkv, const AttnBias bias, const float* __restrict__ norms, const T* __restrict__ out,
                const T* __restrict__ dout, const float2* __restrict__ lse, T* __restrict__ dqkv,
                float* __restrict__ dqw_part, float* __restrict__ dkw_part, float* __restrict__ dbias_part, int k_bufs,
                const __grid_constant__ AttnGeom g, const __grid_constant__ Order o) {
   constexpr int RS = HD + 8, KS = HD / 16, CH = HD / 8;
-  constexpr uint32_t kTile = 16 * RS * sizeof(T), kOffTile = kOffRow * off_bytes<PAIR>();
+  constexpr uint32_t kTile = 16 * RS * sizeof(T);
   extern __shared__ __align__(128) unsigned char smem[];
-  const BiasSums bs = sums_of<PAIR>(o);
+  const BiasSums bs = sums_of(o);
   const int L = o.length, rows = o.tiles * 16, DS = rows + 8, nthreads = blockDim.x;
   const int buckets = (2 * g.T - 1) * (2 * g.wh - 1) * (2 * g.ww - 1);
   BwdSmem<T, HD> S;
@@ -877,7 +838,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
   const int3 place = place_of(o, min((int)threadIdx.x, L - 1));  // of this thread's token
   if (threadIdx.x < rows) {
     off4[threadIdx.x] = threadIdx.x < L ? 4 * off_of(o, place) : 0;
-    put_off<PAIR>(S.offs, threadIdx.x, threadIdx.x < L ? 4 * off_of(o, place) : 0);
+    put_off(S.offs, threadIdx.x, threadIdx.x < L ? 4 * off_of(o, place) : 0);
   }
   for (int i = threadIdx.x; i < HD; i += nthreads) {
     qw[i] = norms[i] * (g.scale * kLog2e);
@@ -926,8 +887,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
     const int ny = 2 * g.wh - 1, nx = 2 * g.ww - 1;
     for (int c = threadIdx.x; c < buckets; c += nthreads) {
       const int dt = c / (ny * nx), dy = c / nx - dt * ny, dx = c % nx;
-      const int df = o.y_fast ? dy : dx, ds = o.y_fast ? dx : dy;
-      const int da = bs.a_is_s ? ds : df, db = (bs.a_is_s ? df : ds) - (bs.nb - 1);
+      const int da = bs.a_is_s ? dy : dx, db = (bs.a_is_s ? dx : dy) - (bs.nb - 1);
       const float* a = acc + (dt * (2 * bs.na - 1) + da) * bs.nb * bs.nb + max(db, 0) * bs.nb + max(-db, 0);
       float s = 0.f;
       for (int i = 0; i < bs.nb - abs(db); ++i) s += a[i * (bs.nb + 1)];
@@ -1046,9 +1006,9 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
       for (int d = 0; d < CH; ++d)
 #pragma unroll
         for (int e = 0; e < 4; ++e) dv[d][e] = dk[d][e] = 0.f;
-      const uint32_t row0 = entry_at<PAIR>(tab, o.entries, o.center - (off4[k0] >> 2));
-      const uint32_t row1 = entry_at<PAIR>(tab, o.entries, o.center - (off4[k0 + 8] >> 2));
-      const uint32_t off_at = smem_u32(S.offs) + tq * off_bytes<PAIR>();
+      const uint32_t row0 = smem_u32(tab + o.center - (off4[k0] >> 2));
+      const uint32_t row1 = smem_u32(tab + o.center - (off4[k0 + 8] >> 2));
+      const uint32_t off_at = smem_u32(S.offs) + tq * kOffBytes;
       const uint32_t q_nt = rows_nt<T, RS>(sQ, lane), q_nn = rows_nn<T, RS>(sQ, lane);
       const uint32_t g_nt = rows_nt<T, RS>(sG, lane), g_nn = rows_nn<T, RS>(sG, lane);
       const uint32_t sub_at = smem_u32(sub + 2 * tq), d_at = smem_u32(negD + 2 * tq);
@@ -1056,7 +1016,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
       const uint32_t ds_tile = 16 * DS * sizeof(T);
       const auto tile = [&](int qb, auto masked) {
         float s[2][4], dp[2][4], nd[2][4];
-        load_block<PAIR>(s, row0, row1, off_at + qb * kOffTile);
+        load_block(s, row0, row1, off_at + qb * kOffTile);
         if (masked() && mixed) mask_block(s, side, side[k0], side[k0 + 8], qb * 16, tq);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -1135,7 +1095,7 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
       // A thread has a place (or several) and every groups-th displacement (dt, da) there
       const int step = bs.sa * (DS + 1), displacements = (2 * o.nt - 1) * (2 * bs.na - 1);
       for (int place = my_place; place < bs.places; place += nthreads) {
-        const int bi = place / (bs.nb / bs.width), bj = (place - bi * (bs.nb / bs.width)) * bs.width;
+        const int bi = place / bs.nb, bj = place - bi * bs.nb;
         const T* at = sS + bi * bs.sb * DS + bj * bs.sb;
         float* sum = acc + bi * bs.nb + bj + my_group * bs.nb * bs.nb;
         int dt = 1 - o.nt, da = 1 - bs.na + my_group;
@@ -1145,27 +1105,16 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
             ++dt;
           }
           const int n = bs.na - abs(da);
-          float s0 = 0.f, s1 = 0.f;
+          float s = 0.f;
           for (int t = max(dt, 0); t < o.nt + min(dt, 0); ++t) {
             const T* p = at + (t * o.ns * o.nf + max(da, 0) * bs.sa) * DS + (t - dt) * o.ns * o.nf + max(-da, 0) * bs.sa;
 #pragma unroll 4
             for (int i = 0; i < n; ++i) {
-              if (PAIR) {
-                const float2 f = unpack_pair<T>(*reinterpret_cast<const uint32_t*>(p));
-                s0 += f.x;
-                s1 += f.y;
-              } else {
-                s0 += to_f(*p);
-              }
+              s += to_f(*p);
               p += step;
             }
           }
-          if (PAIR) {
-            const float2 old = *reinterpret_cast<const float2*>(sum);
-            *reinterpret_cast<float2*>(sum) = make_float2(old.x + s0, old.y + s1);
-          } else {
-            *sum += s0;
-          }
+          *sum += s;
           sum += groups * bs.nb * bs.nb;
           da += groups;
         }
@@ -1228,13 +1177,13 @@ __global__ void __launch_bounds__(32 * kBwdWarps, 1)
 // ------------------------------------------------------------------------------------------------------- launches
 constexpr size_t kBlockSmem = 232448, kSmSmem = 233472;
 
-template <typename T, int HD, bool PAIR>
+template <typename T, int HD>
 cudaError_t launch_fwd(const void* qkv, const AttnBias& bias, const float* norms, void* out, float* lse, const AttnGeom& g,
                        int sms, cudaStream_t s) {
-  const Order o = order_of(g, bias);
+  const Order o = order_of(g);
   FwdSmem<T, HD> S;
   const size_t smem = S.carve(nullptr, o);
-  auto k = fwd_kernel<T, HD, PAIR>;
+  auto k = fwd_kernel<T, HD>;
   NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   const int64_t items = (int64_t)g.B * (g.H / g.wh) * (g.W / g.ww) * g.nh;
   if (items > INT32_MAX) return cudaErrorInvalidValue;
@@ -1256,10 +1205,10 @@ cudaError_t launch_fwd(const void* qkv, const AttnBias& bias, const float* norms
 }
 
 // How many blocks the device holds at once, and whether keys have two buffers: where that costs no block of an SM
-template <typename T, int HD, bool PAIR>
-AttnBiasPlan plan_bwd(const AttnGeom& g, const AttnBias& bias, bool dbias, int sms) {
-  const Order o = order_of(g, bias);
-  const int entries = dbias ? sums_of<PAIR>(o).entries : 0;
+template <typename T, int HD>
+AttnBiasPlan plan_bwd(const AttnGeom& g, bool dbias, int sms) {
+  const Order o = order_of(g);
+  const int entries = dbias ? sums_of(o).entries : 0;
   int blocks[2];
   for (int k = 1; k <= 2; ++k) {
     BwdSmem<T, HD> S;
@@ -1277,14 +1226,14 @@ AttnBiasPlan plan_bwd(const AttnGeom& g, const AttnBias& bias, bool dbias, int s
   return p;
 }
 
-template <typename T, int HD, bool PAIR>
+template <typename T, int HD>
 cudaError_t launch_bwd(const void* qkv, const AttnBias& bias, const float* norms, const void* out, const void* dout,
                        const float* lse, void* dqkv, float* dqw_part, float* dkw_part, float* dbias_part,
                        const AttnBiasPlan& plan, const AttnGeom& g, cudaStream_t s) {
-  const Order o = order_of(g, bias);
+  const Order o = order_of(g);
   BwdSmem<T, HD> S;
-  const size_t smem = S.carve(nullptr, o, dbias_part ? sums_of<PAIR>(o).entries : 0, plan.k_bufs);
-  auto k = bwd_kernel<T, HD, PAIR>;
+  const size_t smem = S.carve(nullptr, o, dbias_part ? sums_of(o).entries : 0, plan.k_bufs);
+  auto k = bwd_kernel<T, HD>;
   NSW_CUDA_CHECK(cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   k<<<plan.blocks, 32 * o.tiles, smem, s>>>((const T*)qkv, bias, norms, (const T*)out, (const T*)dout,
                                             reinterpret_cast<const float2*>(lse), (T*)dqkv, dqw_part, dkw_part, dbias_part,
@@ -1292,19 +1241,18 @@ cudaError_t launch_bwd(const void* qkv, const AttnBias& bias, const float* norms
   return cudaGetLastError();
 }
 
-// f(type, head_dim, pairs) of the call's; WIDE: head_dim 128 too
+// f(type, head_dim) of the call's; WIDE: head_dim 128 too
 template <bool WIDE, typename F>
-auto dispatch(const AttnGeom& g, const AttnBias& b, int dtype, F f) {
-  const auto hd = [&](auto t, auto pair) {
+auto dispatch(const AttnGeom& g, int dtype, F f) {
+  const auto hd = [&](auto t) {
     using I16 = std::integral_constant<int, 16>;
     using I32 = std::integral_constant<int, 32>;
     using I64 = std::integral_constant<int, 64>;
     if constexpr (WIDE)
-      if (g.hd == 128) return f(t, std::integral_constant<int, 128>(), pair);
-    return g.hd == 16 ? f(t, I16(), pair) : g.hd == 32 ? f(t, I32(), pair) : f(t, I64(), pair);
+      if (g.hd == 128) return f(t, std::integral_constant<int, 128>());
+    return g.hd == 16 ? f(t, I16()) : g.hd == 32 ? f(t, I32()) : f(t, I64());
   };
-  const auto type = [&](auto pair) { return dtype == kBF16 ? hd(__nv_bfloat16(), pair) : hd(__half(), pair); };
-  return b.pair ? type(std::true_type()) : type(std::false_type());
+  return dtype == kBF16 ? hd(__nv_bfloat16()) : hd(__half());
 }
 
 }  // namespace attn_bias
@@ -1315,56 +1263,30 @@ static bool attn_bias_ok(const AttnGeom& g, int dtype) {
          (int64_t)g.B * g.T * g.H * g.W < INT32_MAX;
 }
 
-// The fast extent of the tokens' order: one that is even, so that the kernels read entries by pairs (64800 tokens x 16
-// heads: see DESIGN), if the sums of its pairs leave room (at most 6144); of two, the one with fewer of them.  Otherwise
-// longitude, entries one by one, and a pitch that puts a warp's consecutive tokens on consecutive banks where there is room.
-AttnBias attn_bias_layout(const AttnGeom& g) {
-  AttnBias b{};
-  int64_t best = 6145;
-  if (g.hd != 128)
-    for (int y = 0; y < 2; ++y) {
-      const int nf = y ? g.wh : g.ww, ns = y ? g.ww : g.wh;
-      const int64_t sums = (int64_t)(2 * g.T - 1) * (2 * ns - 1) * nf * nf;
-      if (nf % 2 == 0 && sums < best) {
-        best = sums;
-        b.pair = 1;
-        b.y_fast = y;
-      }
-    }
-  const int nf = b.y_fast ? g.wh : g.ww, ns = b.y_fast ? g.ww : g.wh, rows = (2 * g.T - 1) * (2 * ns - 1);
-  b.pitch = 2 * nf - 1;
-  if (b.pair) {
-    b.pitch = 2 * nf;
-  } else {
-    while (b.pitch % 32 != nf % 32) ++b.pitch;
-    if (rows * b.pitch > 1600) b.pitch = 2 * nf - 1;
-  }
-  b.stride = (4 + rows * b.pitch + 3) / 4 * 4;
-  return b;
-}
+static int buckets_of(const AttnGeom& g) { return (2 * g.T - 1) * (2 * g.wh - 1) * (2 * g.ww - 1); }
+AttnBias attn_bias_layout(const AttnGeom& g) { return {nullptr, (4 + buckets_of(g) + 3) / 4 * 4}; }
 
 cudaError_t attn_bias_prepare(const AnyMatrix& table, const AnyMatrix& qw, const AnyMatrix& kw, const AttnGeom& g,
                               const AttnBias& b, float* tab, cudaStream_t s) {
-  attn_bias::prepare_kernel<<<g.nh + 1, 256, 0, s>>>(table, qw, kw, b, g.nh, g.hd, 2 * g.T - 1, 2 * g.wh - 1, 2 * g.ww - 1,
-                                                     g.scale, tab);
+  attn_bias::prepare_kernel<<<g.nh + 1, 256, 0, s>>>(table, qw, kw, b, g.nh, g.hd, buckets_of(g), g.scale, tab);
   return cudaGetLastError();
 }
 
 cudaError_t attn_bias_fwd(const void* qkv, const AttnBias& bias, const float* norms, void* out, float* lse,
                           const AttnGeom& g, int dtype, int sms, cudaStream_t s) {
   if (!attn_bias_ok(g, dtype)) return cudaErrorInvalidValue;
-  return attn_bias::dispatch<true>(g, bias, dtype, [&](auto t, auto hd, auto pair) {
-    return attn_bias::launch_fwd<decltype(t), hd(), pair()>(qkv, bias, norms, out, lse, g, sms, s);
+  return attn_bias::dispatch<true>(g, dtype, [&](auto t, auto hd) {
+    return attn_bias::launch_fwd<decltype(t), hd()>(qkv, bias, norms, out, lse, g, sms, s);
   });
 }
 
-AttnBiasPlan attn_bias_plan(const AttnGeom& g, const AttnBias& bias, int dtype, bool dbias, int sms) {
+AttnBiasPlan attn_bias_plan(const AttnGeom& g, int dtype, bool dbias, int sms) {
   if (g.hd == 128) {
     const int64_t items = (int64_t)g.B * (g.H / g.wh) * (g.W / g.ww) * g.nh;
     return {0, 0, items, items};
   }
-  return attn_bias::dispatch<false>(g, bias, dtype, [&](auto t, auto hd, auto pair) {
-    return attn_bias::plan_bwd<decltype(t), hd(), pair()>(g, bias, dbias, sms);
+  return attn_bias::dispatch<false>(g, dtype, [&](auto t, auto hd) {
+    return attn_bias::plan_bwd<decltype(t), hd()>(g, dbias, sms);
   });
 }
 
@@ -1374,8 +1296,8 @@ cudaError_t attn_bias_bwd(const void* qkv, const AttnBias& bias, const float* no
   if (!attn_bias_ok(g, dtype)) return cudaErrorInvalidValue;
   if (g.hd == 128)
     return window_attn_bwd(qkv, norms, norms + g.hd, out, dout, lse, dqkv, dqw_part, dkw_part, g, dtype, s, bias, dbias_part);
-  return attn_bias::dispatch<false>(g, bias, dtype, [&](auto t, auto hd, auto pair) {
-    return attn_bias::launch_bwd<decltype(t), hd(), pair()>(qkv, bias, norms, out, dout, lse, dqkv, dqw_part, dkw_part,
+  return attn_bias::dispatch<false>(g, dtype, [&](auto t, auto hd) {
+    return attn_bias::launch_bwd<decltype(t), hd()>(qkv, bias, norms, out, dout, lse, dqkv, dqw_part, dkw_part,
                                                             dbias_part, plan, g, s);
   });
 }
@@ -1390,7 +1312,7 @@ cudaError_t attn_bias_grads(const AttnGrad& bias, const AttnGrad& q, const AttnG
   p.qk_rows = plan.norm_rows;
   p.heads = g.nh;
   p.grid = plan.blocks;
-  p.buckets = (2 * g.T - 1) * (2 * g.wh - 1) * (2 * g.ww - 1);
+  p.buckets = buckets_of(g);
   p.hd = g.hd;
   attn_bias::grad_kernel<<<dim3((std::max(p.buckets, g.hd) + 31) / 32, g.nh + 2), 1024, 0, s>>>(p);
   return cudaGetLastError();

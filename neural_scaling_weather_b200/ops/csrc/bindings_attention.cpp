@@ -94,7 +94,7 @@ std::vector<Tensor> attn_bias_bwd(const Tensor& qkv, const Tensor& tab, const Te
   if (qkv.numel() == 0) return res;
   bias.tab = tab.data_ptr<float>();
   const int dtype = dt_code(qkv, "qkv");
-  const nsw::AttnBiasPlan plan = nsw::attn_bias_plan(g, bias, dtype, need[2], sm_count(qkv));
+  const nsw::AttnBiasPlan plan = nsw::attn_bias_plan(g, dtype, need[2], sm_count(qkv));
   auto part = torch::empty({2 * plan.norm_rows * g.hd + (need[2] ? plan.bias_rows * buckets_of(g) : 0)}, f32);
   float* qp = part.data_ptr<float>();
   float* kp = qp + plan.norm_rows * g.hd;

@@ -1,9 +1,10 @@
 // Routed experts: y_t = sum_j w_tj MLP_e(t,j)(x_t) + residual_t over the experts that a router chose for each token.
 //
-// The products run grouped by expert (gated_mlp.cu, the GROUPED forms of its pair kernel) on rows sorted by expert.
+// The products run grouped by expert (gated_mlp.cu, the GROUPED forms of its pair kernel, and its split kernel for few
+// rows an expert) on rows sorted by expert.
 // Here is what stands around them:
 //   plan     a stable counting sort of the assignments (token t's j-th expert) by expert, each expert's rows padded to
-//            whole 256-row tiles, so that a tile belongs to one expert and needs no bounds within it;
+//            whole tiles (256 rows, or fewer: expert_tile), so that a tile belongs to one expert and needs no bounds;
 //   gather   the sorted rows of x; in the backward those of dy times their weights, and with the same read of dy the
 //            weights' gradients, the dot products with the experts' outputs;
 //   combine  a token's rows of the experts' outputs, weighted, plus the residual; in the backward those of dx;

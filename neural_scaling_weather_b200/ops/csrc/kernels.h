@@ -73,13 +73,11 @@ struct AttnGeom {
   int64_t out_stride;  // elements between tokens in out / dout (nh*hd)
 };
 // Learned bias of the logits by head and displacement of query and key (tab null: none), as attn_bias_prepare leaves it:
-// for each head a row of `stride` floats, the first four a header ([0]: a bound on the logits without the bias), then entry
-// (dt (2 wh - 1) + dy) pitch + dx (y_fast: (dt (2 ww - 1) + dx) pitch + dy), in units of log2 and less the head's largest one
-// (a softmax does not see it).
+// for each head a row of `stride` floats, the first four a header ([0]: a bound on the logits without the bias), then the
+// entries, in units of log2 and less the head's largest one (a softmax does not see it).
 struct AttnBias {
   const float* tab;
-  int stride, pitch;
-  int y_fast, pair;  // the order of the tokens, and whether the kernels read entries by pairs (attention_bias.cu)
+  int stride;
 };
 AttnBias attn_bias_layout(const AttnGeom& g);
 // A vector or matrix of any type and strides
@@ -102,7 +100,7 @@ struct AttnBiasPlan {
   int blocks, k_bufs;      // 0 blocks: head_dim 128, a block for each window and head
   int64_t norm_rows, bias_rows;
 };
-AttnBiasPlan attn_bias_plan(const AttnGeom& g, const AttnBias& bias, int dtype, bool dbias, int sms);
+AttnBiasPlan attn_bias_plan(const AttnGeom& g, int dtype, bool dbias, int sms);
 cudaError_t attn_bias_bwd(const void* qkv, const AttnBias& bias, const float* norms, const void* out, const void* dout,
                           const float* lse, void* dqkv, float* dqw_part, float* dkw_part, float* dbias_part,
                           const AttnBiasPlan& plan, const AttnGeom& g, int dtype, cudaStream_t s);
