@@ -69,7 +69,7 @@ ROUTE_TOL = 2.0 ** -19
 @pytest.mark.parametrize("m,e,k,normalize", [
     (1, 1, 1, True), (1, 8, 2, True), (3, 8, 8, False), (33, 9, 1, False), (257, 16, 16, True), (1000, 31, 5, False),
     (4050, 61, 3, False), (2049, 64, 2, True), (515, 65, 4, True), (700, 129, 9, False), (90, 300, 16, True),
-    (19, 512, 7, False), (40000, 8, 2, True)])
+    (19, 512, 7, False), (40000, 8, 2, True), (300, 128, 16, True), (301, 150, 16, False), (67, 256, 9, True)])
 def test_route_matches_definition(dtype, m, e, k, normalize):
     g = torch.Generator(device=DEV).manual_seed(m + e)
     z = (torch.randn(m, e, generator=g, device=DEV) * 2).to(dtype).requires_grad_()
