@@ -195,7 +195,7 @@ def expert_mlp(x: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor, w_
     reverse mode.  Any sizes and strides on CUDA (weights whose rows are not multiples of 16 bytes are copied once a
     call), at most 512 experts, 16 a token; the hidden values and the experts' outputs are 16-bit there.  The rows are
     sorted by expert on the device (nothing waits for it) and the products run grouped by expert; calls without
-    gradients of at most 16 assignments read the chosen experts' weights alone."""
+    gradients have forms of their own for a few assignments and for few rows an expert."""
     if activation not in GATED_ACTIVATIONS:
         raise ValueError(f"expert_mlp: activation {activation!r} is not one of {GATED_ACTIVATIONS}")
     if _use_cuda(x):
