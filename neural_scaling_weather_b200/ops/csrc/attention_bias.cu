@@ -7,9 +7,9 @@
 //
 // A window is at most 192 tokens of one head, so its products are short: what counts is how few instructions stand around
 // them, and that several windows are worked on at once on an SM.  64800 tokens of 16 heads of 64 in windows of 9 x 18, bf16:
-// forward 319 us (134 TFLOP/s, 1.7 TB/s), backward 855 (126 TFLOP/s); bound by the instructions of a logit (its entry from
+// forward 317 us a call (136 TFLOP/s, 1.7 TB/s), with the backward 1173 (backward 126 TFLOP/s); bound by the instructions of a logit (its entry from
 // shared memory, exponential, rounding) and by shared memory (75 % busy), not by products or memory.  The tcgen05 kernels of
-// the plain attention with the entries added to their logits took 463 and 1335.
+// the plain attention with the entries added to their logits took 463 and 1798.
 #include <float.h>
 #include <limits.h>
 
@@ -207,8 +207,8 @@ __device__ __forceinline__ int token_of(const AttnGeom& g, const Order& o, const
 }
 // The entries of a head into shared memory; REVERSED: last entry first.  They lie in rows of 2 nf - 1.  Measured beside it on
 // 64800 tokens of 16 heads, us of the forward and with the backward: rows padded so that consecutive tokens fall on consecutive
-// banks 294 and 960 for 280 and 929 (windows of 9 x 9); two copies, one shifted by an entry, so that any two neighbours are an
-// aligned pair, 313 and 1202 for 324 and 1182 (9 x 18).
+// banks 294 and 960 for 274 and 921 (windows of 9 x 9); two copies, one shifted by an entry, so that any two neighbours are an
+// aligned pair, 313 and 1202 for 317 and 1173 (9 x 18).
 template <bool REVERSED>
 __device__ __forceinline__ void load_table(float* tab, const AttnBias& b, int entries, int head, float less) {
   const float* src = b.tab + (int64_t)head * b.stride + 4;
@@ -444,7 +444,6 @@ struct FwdSmem {
   __host__ __device__ size_t carve(unsigned char* base, const Order& o) {
     const int rows = o.tiles * 16, RS = HD + 8;
     Carve c{base, 0};
-    tab = c.take<float>(o.entries);
     k = c.take<T>(rows * RS);
     v = c.take<T>(rows * RS);
     stage = c.take<T>(16 * kFwdWarps * RS);
@@ -454,6 +453,7 @@ struct FwdSmem {
     qw = c.take<float>(HD);  // with scale and log2 e
     kw = c.take<float>(HD);
     side = c.take<float>(rows);
+    tab = c.take<float>(o.entries);
     return c.at;
   }
 };
