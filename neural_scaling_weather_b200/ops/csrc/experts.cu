@@ -190,8 +190,10 @@ __device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v
   else
     reinterpret_cast<__half*>(p)[i] = from_f<__half>(v);
 }
-// eight elements at p of which `left` are the row's; NC: by the read-only path, which stores do not hold up
-template <bool VEC, bool NC = true>
+// eight elements at p of which `left` are the row's; NC: by the read-only path, which stores do not hold up.  That path
+// is for what was complete before the first of a chain of programmatic dependents began (the caller's tensors): a kernel
+// that is resident while the one before it still writes takes what that one leaves by ordinary loads, behind its wait.
+template <bool VEC, bool NC>
 __device__ __forceinline__ uint4 row8(const uint16_t* p, int64_t left) {
   if (VEC && NC) return __ldg(reinterpret_cast<const uint4*>(p));
   if (VEC) return *reinterpret_cast<const uint4*>(p);
@@ -219,7 +221,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4) gather_kernel(const ExpertP
   for (int64_t t = warp; t < tokens; t += warps) {
     const uint16_t* p = reinterpret_cast<const uint16_t*>(a.rows) + t * a.ld_rows;
     // lane i holds the token's i-th row and weight (kMaxChosen <= 32), and the dot product that is its weight's gradient
-    const int my_row = lane < k ? __ldg(plan.row_of + t * k + lane) : -1;
+    const int my_row = lane < k ? plan.row_of[t * k + lane] : -1;
     const float my_weight = WEIGHTED && lane < k ? load_any(a.weights, a.weight_dtype, t * k + lane) : 1.f;
     float my_dot = 0.f;
     for (int64_t c0 = 8 * lane; c0 - 8 * lane < a.n; c0 += 256 * kSpan) {
@@ -227,7 +229,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4) gather_kernel(const ExpertP
 #pragma unroll
       for (int j = 0; j < kSpan; ++j) {
         const int64_t c = c0 + 256 * j;
-        in[j] = c < a.n ? row8<VEC>(p + c, a.n - c) : make_uint4(0, 0, 0, 0);
+        in[j] = c < a.n ? row8<VEC, true>(p + c, a.n - c) : make_uint4(0, 0, 0, 0);
       }
 #pragma unroll 2
       for (int i = 0; i < k; ++i) {
@@ -238,7 +240,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4) gather_kernel(const ExpertP
 #pragma unroll
           for (int j = 0; j < kSpan; ++j) {
             const int64_t c = c0 + 256 * j;
-            o[j] = c < a.n && row >= 0 ? row8<true>(other + row * a.ld_other + c, 8) : make_uint4(0, 0, 0, 0);
+            o[j] = c < a.n && row >= 0 ? row8<true, true>(other + row * a.ld_other + c, 8) : make_uint4(0, 0, 0, 0);
           }
         }
         float dot = 0.f;
@@ -272,10 +274,10 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4) gather_kernel(const ExpertP
     if (WEIGHTED && a.dweights && lane < k) store_any(a.dweights, a.weight_dtype, t * k + lane, my_dot);
   }
   // the padding's zeros; lane i looks at the warp's i-th row of 32
-  const int64_t rows = (int64_t)__ldg(plan.tiles) * plan.tile;
+  const int64_t rows = (int64_t)*plan.tiles * plan.tile;
   for (int64_t r0 = warp; r0 < rows; r0 += 32 * warps) {
     const int64_t mine = r0 + lane * warps;
-    unsigned empty = __ballot_sync(0xffffffffu, mine < rows && __ldg(plan.src_of + mine) < 0);
+    unsigned empty = __ballot_sync(0xffffffffu, mine < rows && plan.src_of[mine] < 0);
     for (; empty; empty &= empty - 1) {
       uint16_t* d = dst + (r0 + (__ffs(empty) - 1) * warps) * a.ld_dst;
       for (int64_t c = 8 * lane; c < a.n; c += 256) *reinterpret_cast<uint4*>(d + c) = make_uint4(0, 0, 0, 0);
@@ -294,14 +296,14 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4) combine_kernel(const Expert
     const uint16_t* res = reinterpret_cast<const uint16_t*>(a.residual) + t * a.ld_res;
     T* out = reinterpret_cast<T*>(a.out) + t * a.ld_out;
     // lane i holds the token's i-th row and weight (kMaxChosen <= 32)
-    const int my_row = lane < k ? __ldg(a.row_of + t * k + lane) : -1;
+    const int my_row = lane < k ? a.row_of[t * k + lane] : -1;
     const float my_weight = lane < k && a.weights ? load_any(a.weights, a.weight_dtype, t * k + lane) : 1.f;
     for (int64_t c0 = 8 * lane; c0 - 8 * lane < a.n; c0 += 256 * kSpan) {
       float f[kSpan][8];
 #pragma unroll
       for (int j = 0; j < kSpan; ++j) {
         const int64_t c = c0 + 256 * j;
-        unpack8<T>(a.residual && c < a.n ? row8<VEC>(res + c, a.n - c) : make_uint4(0, 0, 0, 0), f[j]);
+        unpack8<T>(a.residual && c < a.n ? row8<VEC, true>(res + c, a.n - c) : make_uint4(0, 0, 0, 0), f[j]);
       }
       for (int i0 = 0; i0 < k; i0 += 2) {
         uint4 in[2][kSpan];
@@ -314,7 +316,7 @@ __global__ void __launch_bounds__(32 * kRowWarps, 4) combine_kernel(const Expert
 #pragma unroll
           for (int j = 0; j < kSpan; ++j) {
             const int64_t c = c0 + 256 * j;
-            in[i][j] = row >= 0 && c < a.n ? row8<true>(rows + row * a.ld_rows + c, 8) : make_uint4(0, 0, 0, 0);
+            in[i][j] = row >= 0 && c < a.n ? row8<true, false>(rows + row * a.ld_rows + c, 8) : make_uint4(0, 0, 0, 0);
           }
         }
 #pragma unroll
@@ -381,13 +383,13 @@ __global__ void __launch_bounds__(256) few_up_kernel(const ExpertFew a) {
 #pragma unroll 4
     for (int c = 8 * lane; c < a.K; c += 256) {
       float fg[8], fu[8];
-      unpack8<T>(row8<VEC>(wg + c, a.K - c), fg);
-      unpack8<T>(row8<VEC>(wu + c, a.K - c), fu);
+      unpack8<T>(row8<VEC, true>(wg + c, a.K - c), fg);
+      unpack8<T>(row8<VEC, true>(wu + c, a.K - c), fu);
 #pragma unroll
       for (int i = 0; i < kFewGroup; ++i) {
         if (i > 0 && i0 + i >= listed) continue;
         float f[8];
-        unpack8<T>(row8<VEC>(x[i] + c, a.K - c), f);
+        unpack8<T>(row8<VEC, true>(x[i] + c, a.K - c), f);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
           g[i] = fmaf(f[j], fg[j], g[i]);
@@ -429,7 +431,7 @@ __global__ void __launch_bounds__(256) few_down_kernel(const ExpertFew a) {
 #pragma unroll 4
     for (int c = 8 * lane; c < a.H; c += 256) {
       float f[8], g[8];
-      unpack8<T>(row8<VEC>(w + c, a.H - c), f);
+      unpack8<T>(row8<VEC, true>(w + c, a.H - c), f);
       unpack8<T>(row8<VEC, false>(h + c, a.H - c), g);
 #pragma unroll
       for (int i = 0; i < 8; ++i) dot = fmaf(f[i], g[i], dot);
