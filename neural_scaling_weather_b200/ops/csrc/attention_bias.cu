@@ -414,17 +414,20 @@ __device__ __forceinline__ float norm_chunk(const uint4& raw, const float* w, ui
 // head_dim max_i |qw_i kw_i| scale (Cauchy and Schwarz, in the norm that the weights' products give), which the preparation
 // has left in the head's header.  So they are at most 2^top, the bound is in the entries before the products begin, and
 // nothing is looked up or subtracted for a row.  Rows far below the bound lose precision to their type's smallest numbers:
-// those whose sum is below `least` (in fp16, 192 numbers that are each off by at most 2^-25 are off by less than 2^-17 of it) make
-// their tile begin again with every row less its own largest logit, for one more product of q and k.
+// those whose sum is below `least` (in fp16, 192 numbers that are each off by at most 2^-25 are off by less than 2^-17 of
+// it; in bf16 what fp32 holds of P V is then no less than with the row's largest logit subtracted) make their tile begin
+// again with every row less its own largest logit, for one more product of q and k.  So does a sum of P V beyond fp32,
+// which bf16 values above 2^30 may reach at weights of 2^top.  The second way's weights are at most 2^-drop, so that 192 of
+// them times any value of the type stay below fp32's largest number.
 template <typename T>
 struct Bound;
 template <>
 struct Bound<__nv_bfloat16> {
-  static constexpr float top = 64.f, least = 8.0779357e-28f;  // 2^-90
+  static constexpr float top = 90.f, least = 1.f, drop = 8.f;
 };
 template <>
 struct Bound<__half> {
-  static constexpr float top = 14.f, least = 1.f;
+  static constexpr float top = 14.f, least = 1.f, drop = 0.f;  // (65504 2^14 192 is far from fp32's limit)
 };
 constexpr float kMostBound = 1e4f;  // beyond it (or NaN): the second way at once
 
@@ -608,11 +611,11 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
     // weights add up to one as they are, and the sum costs an instruction where eight additions would
     float acc[CH][4], sum[4];
     const uint32_t ones = pack2<T>(1.f, 1.f);
-    const auto weights = [&](float (&c)[2][4], int kb) {
+    const auto weights = [&](float (&c)[2][4], int kb, float drop) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) c[j][e] = fast_exp2(c[j][e]);
+        for (int e = 0; e < 4; ++e) c[j][e] = fast_exp2(drop == 0.f ? c[j][e] : c[j][e] - drop);
       const uint32_t p[4] = {pack2<T>(c[0][0], c[0][1]), pack2<T>(c[0][2], c[0][3]), pack2<T>(c[1][0], c[1][1]),
                              pack2<T>(c[1][2], c[1][3])};
       mma16816<T>(sum, p, ones, ones);
@@ -623,12 +626,22 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
 #pragma unroll
       for (int d = 0; d < CH; ++d) acc[d][0] = acc[d][1] = acc[d][2] = acc[d][3] = 0.f;
     };
-    float m0 = 0.f, m1 = 0.f;  // besides `less`
+    float m0 = 0.f, m1 = 0.f, drop = 0.f;  // besides `less`
     bool again = exact;
     if (!exact) {
       clear();
-      each_tile(0.f, 0.f, false, std::false_type(), weights);
-      again = __any_sync(0xffffffffu, sum[0] < Bound<T>::least || sum[2] < Bound<T>::least);
+      each_tile(0.f, 0.f, false, std::false_type(), [&](float (&c)[2][4], int kb) { weights(c, kb, 0.f); });
+      bool redo = sum[0] < Bound<T>::least || sum[2] < Bound<T>::least;
+      if constexpr (Bound<T>::drop > 0.f) {  // zero times what is not finite is not zero
+        float2 finite = {0.f, 0.f};
+#pragma unroll
+        for (int d = 0; d < CH; ++d) {
+          finite = fma2(make_float2(acc[d][0], acc[d][1]), make_float2(0.f, 0.f), finite);
+          finite = fma2(make_float2(acc[d][2], acc[d][3]), make_float2(0.f, 0.f), finite);
+        }
+        redo = redo || !(finite.x + finite.y == 0.f);
+      }
+      again = __any_sync(0xffffffffu, redo);
     }
     if (again) {
       m0 = m1 = -INFINITY;
@@ -643,7 +656,8 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
       // rows of entries beyond kAbsorbs throughout absorb the product before they are subtracted
       const bool late = __any_sync(0xffffffffu, fabsf(m0) > kAbsorbs || fabsf(m1) > kAbsorbs);
       clear();
-      each_tile(m0, m1, late, std::true_type(), weights);
+      drop = Bound<T>::drop;  // (apart from m0 and m1, which may be too large to hold it)
+      each_tile(m0, m1, late, std::true_type(), [&](float (&c)[2][4], int kb) { weights(c, kb, Bound<T>::drop); });
     }
     const float l0 = sum[0], l1 = sum[2];
     const float i0 = l0 == 0.f ? 0.f : 1.f / l0, i1 = l1 == 0.f ? 0.f : 1.f / l1;
@@ -656,8 +670,8 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
     }
     if (tq == 0) {
       float2* at = lse + (int64_t)blockIdx.x * L;
-      if (r0 < L) at[r0] = l0 == 0.f ? make_float2(0.f, 0.f) : make_float2(m0 + less, __log2f(l0));
-      if (r1 < L) at[r1] = l1 == 0.f ? make_float2(0.f, 0.f) : make_float2(m1 + less, __log2f(l1));
+      if (r0 < L) at[r0] = l0 == 0.f ? make_float2(0.f, 0.f) : make_float2(m0 + less, __log2f(l0) + drop);
+      if (r1 < L) at[r1] = l1 == 0.f ? make_float2(0.f, 0.f) : make_float2(m1 + less, __log2f(l1) + drop);
     }
     T* st = S.stage + warp * 16 * RS;
     __syncwarp();

@@ -1,0 +1,110 @@
+"""Window attention with a relative position bias where numbers are large, small, masked or nearly cancel, against its
+definition in 64 bits.
+
+u is 2^-9 for bf16 and 2^-11 for fp16 (the 2-norm of the rounding to 16 bits over the spread of a tensor's significands is
+below that).  As in test_rel_bias_gpu.py 6 u are the output's, 10 u the gradients' of q, k and v, 24 u those of sums
+with changing signs.  dS = P (dP - D) may be what remains of a difference: D_i = <dO_i, O_i> has the rounding of O, u times
+the root sum of squares of its terms, g_i, and P, whose values were rounded before they were divided by their sum, adds up
+to one but for u (sum_j P_ij^2)^1/2.  Both are one number a row, eta_i = u (g_i^2 + D_i^2 sum_j P_ij^2)^1/2, of no sign:
+rows add up like their squares.  Three times that is allowed, `eta` below without its u."""
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():  # pragma: no cover
+    pytest.skip("no CUDA device", allow_module_level=True)
+
+from neural_scaling_weather_b200 import ops  # noqa: E402
+from neural_scaling_weather_b200.ops import _ext  # noqa: E402
+from tests.test_rel_bias_gpu import BF, DEV, EPS, F32, HF, U, inputs, rel  # noqa: E402
+
+INF = float("inf")
+
+
+@pytest.fixture(autouse=True)
+def _no_device_error():
+    ext = _ext.require()
+    yield
+    assert ext.read_error_flag(True) == 0
+
+
+def definition(qkv, qw, kw, table, geom, nh, hd, dout=None):
+    """-> out, or {out, grads of qkv / qw / kw / table, slack: the same gradients of eta P in dS's place, noise: of each head's
+    table (the root sum of squares of eta P)}; fp64, windows gathered token by token."""
+    B, T, H, W, _ = qkv.shape
+    (wh, ww), (sh, sw) = geom.window, geom.shift
+    leaves = [t.detach().double().requires_grad_() for t in (qkv, qw, kw, table)]
+    x, qwd, kwd, tab = leaves
+    at = [(t, y, c) for t in range(T) for y in range(wh) for c in range(ww)]
+    token, far = [], []
+    for b in range(B):
+        for y0 in range(0, H, wh):
+            for x0 in range(0, W, ww):
+                token.append([((b * T + t) * H + (y0 + y + sh) % H) * W + (x0 + c + sw) % W for t, y, c in at])
+                far.append([bool(geom.mask) and y0 + y >= H - geom.mask_shift for _, y, _ in at])
+    token, far = torch.tensor(token, device=DEV), torch.tensor(far, device=DEV)
+    bucket = torch.tensor([[((t - t2 + T - 1) * (2 * wh - 1) + y - y2 + wh - 1) * (2 * ww - 1) + c - c2 + ww - 1
+                            for t2, y2, c2 in at] for t, y, c in at], device=DEV)
+    q, k, v = x.reshape(-1, 3, nh, hd)[token].permute(2, 0, 3, 1, 4)
+    norm = lambda a, w: a * torch.rsqrt(a.square().mean(-1, keepdim=True) + EPS) * w  # noqa: E731
+    s = norm(q, qwd) @ norm(k, kwd).transpose(-1, -2) * hd ** -0.5 + tab[:, bucket]
+    s = s - 100.0 * (far[:, None, :, None] != far[:, None, None, :])
+    none = (s == -INF).all(-1, keepdim=True)
+    p = torch.softmax(s.masked_fill(none, 0.0), -1).masked_fill(none, 0.0)
+    o = p @ v
+    out = torch.zeros(B * T * H * W, nh * hd, dtype=torch.float64, device=DEV)
+    out = out.index_copy(0, token.reshape(-1), o.transpose(1, 2).reshape(-1, nh * hd)).view(B, T, H, W, nh * hd)
+    if dout is None:
+        return out.detach()
+    grads = torch.autograd.grad(out, leaves, dout.double(), retain_graph=True)
+    with torch.no_grad():
+        do = dout.double().reshape(-1, nh, hd)[token].transpose(1, 2)
+        d = (do * o).sum(-1, keepdim=True)
+        eta = ((do * o).square().sum(-1, keepdim=True) + d.square() * p.square().sum(-1, keepdim=True)).sqrt()
+        noise = (p * eta).square().sum((0, 2, 3)).sqrt()
+        weight = p * eta
+    slack = torch.autograd.grad((s.masked_fill(weight == 0, 0.0) * weight).sum(), leaves, allow_unused=True)
+    return {"out": out.detach(), "grads": grads, "slack": slack, "noise": noise}
+
+
+def call(qkv, qw, kw, table, geom, nh, hd, dout):
+    leaves = [t.clone().requires_grad_() for t in (qkv, qw, kw, table)]
+    out = ops.window_attention(*leaves[:3], nh, hd, geom, hd ** -0.5, rel_bias=leaves[3])
+    return out.detach(), torch.autograd.grad(out, leaves, dout)
+
+
+# ------------------------------------------------------------------------------------------------ range of the values
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("size", [1e18, 3e30, 3e38, 1e-30])
+def test_equal_tokens_give_their_value(hd, size):
+    """One window of equal tokens: every weight is 1 / 162, the output is v, whatever its size in bf16."""
+    nh, geom = 2, ops.WindowGeometry(window=(9, 18))
+    qkv = torch.ones(1, 1, 9, 18, 3 * nh * hd, device=DEV, dtype=BF)
+    qkv[..., 2 * nh * hd:] = size
+    one = torch.ones(hd, device=DEV)
+    for bias in (0.0, -3e6):
+        table = torch.full((nh, geom.num_buckets(1)), bias, device=DEV)
+        out = ops.window_attention(qkv, one, one, nh, hd, geom, hd ** -0.5, rel_bias=table)
+        assert rel(out, qkv[..., 2 * nh * hd:]) < 2 * U[BF]  # (it is itself a bf16 number: at most one rounding)
+
+
+@pytest.mark.parametrize("hd", [16, 64, 128])
+@pytest.mark.parametrize("weight", [1.0, 12.0])
+@pytest.mark.parametrize("power", [-100, -40, 40, 100])
+def test_values_of_any_scale(hd, weight, power):
+    """v times a power of two scales the output and all gradients but v's.  weight: of one feature's norms alone, so that most
+    logits are far below what the weights allow."""
+    nh = 2
+    qkv, qw, kw, table, geom, dout = inputs(1, 1, 2, 2, 9, 18, nh, hd, BF, True, seed=hd)
+    qkv[..., 2 * nh * hd:] *= 2.0 ** power
+    qw[3] = kw[3] = weight
+    qkv[..., 3:2 * nh * hd:hd] *= 0.05  # that feature is small in every token
+    out, grads = call(qkv, qw, kw, table, geom, nh, hd, dout)
+    want = definition(qkv, qw, kw, table, geom, nh, hd, dout)
+    c = nh * hd
+    assert rel(out, want["out"]) < 6 * U[BF]
+    for part in (slice(0, c), slice(c, 2 * c), slice(2 * c, 3 * c)):
+        assert rel(grads[0][..., part], want["grads"][0][..., part]) < 10 * U[BF]
+    assert rel(grads[3], want["grads"][3]) < 24 * U[BF]
