@@ -94,9 +94,10 @@ __device__ __forceinline__ void load_rows(T* s, const T* base, int64_t stride, i
   }
 }
 
-// In-place RMSNorm of rows [0, L) of an smem tile; writes rstd per row if requested.
-template <typename T, int HD>
-__device__ __forceinline__ void norm_rows(T* s, const float* w, int L, float* rstd_out) {
+// In-place RMSNorm of rows [0, L) of an smem tile; writes rstd per row if requested.  BIAS: rounds as the forward of
+// attention_bias.cu does, (x (w factor)) rstd.
+template <typename T, int HD, bool BIAS = false>
+__device__ __forceinline__ void norm_rows(T* s, const float* w, int L, float* rstd_out, float factor = 1.f) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
   constexpr int PER = HD / 32 > 0 ? HD / 32 : 1;
   for (int i = warp; i < L; i += nw) {
@@ -115,7 +116,7 @@ __device__ __forceinline__ void norm_rows(T* s, const float* w, int L, float* rs
 #pragma unroll
     for (int k = 0; k < PER; ++k) {
       const int c = lane + 32 * k;
-      if (c < HD) row[c] = from_f<T>(v[k] * rs * w[c]);
+      if (c < HD) row[c] = from_f<T>(BIAS ? v[k] * (w[c] * factor) * rs : v[k] * rs * w[c]);
     }
   }
 }
@@ -385,17 +386,19 @@ __device__ __forceinline__ void store_rows_c(float (*acc)[4], int row0, int lane
   }
 }
 
-// P of one key and two query rows with a bias; `tab` is the key's center in the entries
-__device__ __forceinline__ void biased_probs(float s0, float s1, float sl2, const float* tab, const short* off, int r0, int r1,
-                                             int key_label, int label0, int label1, float m0, float m1, const float* ll,
-                                             float& p0, float& p1) {
-  const float ml2 = -100.f * kLog2e;
-  p0 = p1 = 0.f;
-  if (key_label < 0) return;
-  const float v0 = fmaf(s0, sl2, tab[off[r0]]) + (key_label != (label0 < 0 ? 0 : label0) ? ml2 : 0.f);
-  const float v1 = fmaf(s1, sl2, tab[off[r1]]) + (key_label != (label1 < 0 ? 0 : label1) ? ml2 : 0.f);
-  p0 = fast_exp2((v0 - m0) - ll[r0]);
-  p1 = fast_exp2((v1 - m1) - ll[r1]);
+// With a bias, logits and weights are formed as the forward of attention_bias.cu forms them, whose statistics they meet: q
+// with scale and log2 e before its rounding, so that a row's weights add up to one (from another rounding of q they miss it
+// by 1 to 3 % at norm weights of 2 to 3, and D does not cancel what dP has in common), and the entry less what the row's
+// exponents are less before the product is added, so that entries far from zero do not round it away.
+struct RowStat {
+  float sub, late, ll;  // before the product; after it, this and then this where `wide`
+};
+// what a logit's product begins with; `entry` is the key's center in the entries (tab + center - off(key))
+__device__ __forceinline__ float bias_start(const float* entry, int off, int key_label, int label, float sub) {
+  return entry[off] + (key_label != (label < 0 ? 0 : label) ? -100.f * kLog2e : 0.f) - sub;
+}
+__device__ __forceinline__ float bias_prob(float s, int key_label, bool wide, const RowStat& r) {
+  return key_label < 0 ? 0.f : fast_exp2(wide ? (s - r.late) - r.ll : s);
 }
 
 // With a bias's gradient (dbias_part), a third phase forms dS once more and adds it up by bucket.  A bucket's pairs have one
@@ -432,8 +435,8 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
   const int buckets = (2 * g.T - 1) * (2 * g.wh - 1) * (2 * g.ww - 1);
   float* sTab = reinterpret_cast<float*>(smem + ((size_t)4 * lp * RS * sizeof(T) + lp * 21 + 2 * HD * 4 + 15) / 16 * 16);
   short* sOff = reinterpret_cast<short*>(sTab + (BIAS ? bias.stride : 0));
-  float* sLl = reinterpret_cast<float*>(sOff + (BIAS ? lp : 0));  // BIAS: log2 of a row's sum; sLse its largest logit
-  float* sSum = sLl + (BIAS ? lp : 0);                           // with dbias_part: the buckets, then the warps' tiles
+  RowStat* sStat = reinterpret_cast<RowStat*>(sOff + (BIAS ? lp : 0));
+  float* sSum = reinterpret_cast<float*>(sStat + (BIAS ? lp : 0));  // with dbias_part: the buckets, then the warps' tiles
   const int center = BIAS ? bias_center(g) : 0;
 
   const int bw = blockIdx.x, h = blockIdx.y;
@@ -450,9 +453,17 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
   load_rows<T, HD>(sV, qkv, g.qkv_stride, 2 * C + (int64_t)h * HD, sTok, L, lp);
   load_rows<T, HD>(sG, dout, g.out_stride, (int64_t)h * HD, sTok, L, lp);
   const int64_t lse_base = ((int64_t)bw * g.nh + h) * L;
-  for (int i = threadIdx.x; i < lp; i += blockDim.x) {
-    sLse[i] = i >= L ? INFINITY : lse[BIAS ? 2 * (lse_base + i) : lse_base + i];
-    if (BIAS) sLl[i] = i < L ? lse[2 * (lse_base + i) + 1] : 0.f;
+  bool wide = false;
+  if (BIAS) {  // (largest logit, log2 of the sum): one number, unless the first is so large that the second would be lost beside it
+    for (int i = threadIdx.x; i < L; i += blockDim.x) wide = wide || fabsf(lse[2 * (lse_base + i)]) > 4096.f;
+    wide = __syncthreads_or(wide);
+    for (int i = threadIdx.x; i < lp; i += blockDim.x) {
+      const float m = i < L ? lse[2 * (lse_base + i)] : INFINITY, ll = i < L ? lse[2 * (lse_base + i) + 1] : 0.f;
+      const bool absorbs = i < L && fabsf(m) > kAbsorbs;  // as the forward
+      sStat[i] = {!wide ? m + ll : absorbs ? 0.f : m, absorbs ? m : 0.f, ll};
+    }
+  } else {
+    for (int i = threadIdx.x; i < lp; i += blockDim.x) sLse[i] = i < L ? lse[lse_base + i] : INFINITY;
   }
   for (int i = threadIdx.x; i < HD; i += blockDim.x) {
     sWq[i] = 0.f;
@@ -474,8 +485,8 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
   }
   cp_async_wait_all();
   __syncthreads();
-  norm_rows<T, HD>(sQ, qw, L, sRq);
-  norm_rows<T, HD>(sK, kw, L, sRk);
+  norm_rows<T, HD, BIAS>(sQ, qw, L, sRq, g.scale * kLog2e);
+  norm_rows<T, HD, BIAS>(sK, kw, L, sRk);
   __syncthreads();
 
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
@@ -511,6 +522,16 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) st[j][e] = dpt[j][e] = 0.f;
+        if (BIAS) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {  // (rows are keys here)
+              const int q = qc + j * 8 + 2 * tq + e;
+              st[j][e] = bias_start(sTab + center - sOff[kr0], sOff[q], klab0, sLab[q], sStat[q].sub);
+              st[j][2 + e] = bias_start(sTab + center - sOff[kr1], sOff[q], klab1, sLab[q], sStat[q].sub);
+            }
+        }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           uint32_t b0, b1, b2, b3;
@@ -530,17 +551,13 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int q = qc + j * 8 + 2 * tq + e;
-            const float lq = sLse[q];
+            const float lq = BIAS ? 0.f : sLse[q];
             const float dq = sD[q];
             float v0 = st[j][e] * sl2, v1 = st[j][2 + e] * sl2;
             float p0, p1;
-            if (BIAS) {  // (rows are keys here)
-              const float* b = sTab + center + sOff[q];
-              const int ql = sLab[q];
-              v0 = fmaf(st[j][e], sl2, b[-sOff[kr0]]) + (ql >= 0 && klab0 != ql ? ml2 : 0.f);
-              v1 = fmaf(st[j][2 + e], sl2, b[-sOff[kr1]]) + (ql >= 0 && klab1 != ql ? ml2 : 0.f);
-              p0 = klab0 < 0 ? 0.f : fast_exp2((v0 - lq) - sLl[q]);
-              p1 = klab1 < 0 ? 0.f : fast_exp2((v1 - lq) - sLl[q]);
+            if (BIAS) {
+              p0 = bias_prob(st[j][e], klab0, wide, sStat[q]);
+              p1 = bias_prob(st[j][2 + e], klab1, wide, sStat[q]);
             } else if (plain) {
               p0 = fast_exp2(v0 - lq);
               p1 = fast_exp2(v1 - lq);
@@ -584,7 +601,7 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
 #pragma unroll
       for (int d = 0; d < DT; ++d)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) dk[d][e] *= g.scale;
+        for (int e = 0; e < 4; ++e) dk[d][e] *= BIAS ? 0.69314718055994530942f : g.scale;  // (q with scale and log2 e)
       store_rows_c<T, HD>(dv, kt * 16, lane, g.qkv_stride, 2 * C + (int64_t)h * HD, sTok, L, dqkv);
       norm_backward_store<T, HD>(dk, kt * 16, lane, qkv, g.qkv_stride, 1 * C + (int64_t)h * HD, kw,
                                  sRk, sTok, L, dqkv, wk);
@@ -601,7 +618,7 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
       }
       const int qr0 = qt * 16 + gq, qr1 = qr0 + 8;
       const int qlab0 = sLab[qr0], qlab1 = sLab[qr1];
-      const float lq0 = sLse[qr0], lq1 = sLse[qr1];
+      const float lq0 = BIAS ? 0.f : sLse[qr0], lq1 = BIAS ? 0.f : sLse[qr1];
       const float d0 = sD[qr0], d1 = sD[qr1];
       float dq[DT][4];
 #pragma unroll
@@ -612,6 +629,16 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
         for (int j = 0; j < 2; ++j)
 #pragma unroll
           for (int e = 0; e < 4; ++e) s[j][e] = dpm[j][e] = 0.f;
+        if (BIAS) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int k = kc + j * 8 + 2 * tq + e;
+              s[j][e] = bias_start(sTab + center - sOff[k], sOff[qr0], sLab[k], qlab0, sStat[qr0].sub);
+              s[j][2 + e] = bias_start(sTab + center - sOff[k], sOff[qr1], sLab[k], qlab1, sStat[qr1].sub);
+            }
+        }
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) {
           uint32_t b0, b1, b2, b3;
@@ -633,8 +660,8 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
             float p0 = 0.f, p1 = 0.f;
             if (BIAS) {
               const int k = kc + j * 8 + 2 * tq + e;
-              biased_probs(s[j][e], s[j][2 + e], sl2, sTab + center - sOff[k], sOff, qr0, qr1, sLab[k], qlab0, qlab1, lq0,
-                           lq1, sLl, p0, p1);
+              p0 = bias_prob(s[j][e], sLab[k], wide, sStat[qr0]);
+              p1 = bias_prob(s[j][2 + e], sLab[k], wide, sStat[qr1]);
             } else if (plain) {
               p0 = fast_exp2(v0 - lq0);
               p1 = fast_exp2(v1 - lq1);
@@ -685,11 +712,18 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
       for (int d = first + 2 * warp; d < nt; d += 2 * nw) {
         for (int kt = max(0, -d); kt < min(nt, nt - d); ++kt) {
           const int qt = kt + d;
+          const int qr0 = qt * 16 + gq, qr1 = qr0 + 8;
           float s[2][4], dpm[2][4];
 #pragma unroll
-          for (int j = 0; j < 2; ++j)
+          for (int j = 0; j < 2; ++j) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) s[j][e] = dpm[j][e] = 0.f;
+            for (int e = 0; e < 2; ++e) {
+              const int k = kt * 16 + j * 8 + 2 * tq + e;
+              s[j][e] = bias_start(sTab + center - sOff[k], sOff[qr0], sLab[k], sLab[qr0], sStat[qr0].sub);
+              s[j][2 + e] = bias_start(sTab + center - sOff[k], sOff[qr1], sLab[k], sLab[qr1], sStat[qr1].sub);
+              dpm[j][e] = dpm[j][2 + e] = 0.f;
+            }
+          }
 #pragma unroll
           for (int ks = 0; ks < KS; ++ks) {
             uint32_t a[4], b0, b1, b2, b3;
@@ -704,18 +738,14 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
             mma16816<T>(dpm[0], a, b0, b1);
             mma16816<T>(dpm[1], a, b2, b3);
           }
-          const int qr0 = qt * 16 + gq, qr1 = qr0 + 8;
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
             float ds[4];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const int k = kt * 16 + j * 8 + 2 * tq + e;
-              float p0, p1;
-              biased_probs(s[j][e], s[j][2 + e], sl2, sTab + center - sOff[k], sOff, qr0, qr1, sLab[k], sLab[qr0],
-                           sLab[qr1], sLse[qr0], sLse[qr1], sLl, p0, p1);
-              ds[e] = p0 * (dpm[j][e] - sD[qr0]);
-              ds[2 + e] = p1 * (dpm[j][2 + e] - sD[qr1]);
+              ds[e] = bias_prob(s[j][e], sLab[k], wide, sStat[qr0]) * (dpm[j][e] - sD[qr0]);
+              ds[2 + e] = bias_prob(s[j][2 + e], sLab[k], wide, sStat[qr1]) * (dpm[j][2 + e] - sD[qr1]);
             }
             *reinterpret_cast<uint32_t*>(tile + gq * 18 + j * 8 + 2 * tq) = pack2<T>(ds[0], ds[1]);
             *reinterpret_cast<uint32_t*>(tile + (gq + 8) * 18 + j * 8 + 2 * tq) = pack2<T>(ds[2], ds[3]);
@@ -801,7 +831,7 @@ static cudaError_t launch_bwd(const void* qkv, const float* qw, const float* kw,
   const int lp = nt * 16;
   const size_t smem = (size_t)4 * lp * (HD + 8) * sizeof(T) + (size_t)4 * lp * sizeof(float) +
                       2 * HD * sizeof(float) + (size_t)lp * (sizeof(int) + 1) +
-                      (bias.tab ? 16 + bias_bytes(bias, lp) + (size_t)lp * sizeof(float) : 0) +
+                      (bias.tab ? 16 + bias_bytes(bias, lp) + (size_t)lp * sizeof(RowStat) : 0) +
                       (dbias_part ? (size_t)(2 * g.T - 1) * (2 * g.wh - 1) * (2 * g.ww - 1) * sizeof(float) +
                                         6 * kBiasTile * sizeof(T)
                                   : 0);

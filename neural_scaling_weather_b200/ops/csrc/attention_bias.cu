@@ -24,6 +24,7 @@ namespace attn_bias {
 using attn::cp_async16;
 using attn::cp_async_wait_all;
 using attn::fast_exp2;
+using attn::kAbsorbs;
 using attn::kLog2e;
 using attn::ldsm_x4;
 using attn::ldsm_x4_t;
@@ -50,8 +51,6 @@ __device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
   if (dtype == kBF16) return to_f(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
   return to_f(reinterpret_cast<const __half*>(p)[i]);
 }
-
-constexpr float kAbsorbs = 1099511627776.f;  // 2^40
 
 // One block a head, and one for the norms' weights.  Entries are less the head's largest, so that an offset of all of them
 // costs no precision, unless that is beyond 2^40: a head of the lowest value throughout, say, absorbs the logits, as it

@@ -7,6 +7,7 @@ namespace nsw {
 namespace attn {
 
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kAbsorbs = 1099511627776.f;  // 2^40: entries of a relative position bias beyond it absorb the logits
 
 __device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t& r0, uint32_t& r1, uint32_t& r2,
                                         uint32_t& r3) {

@@ -108,3 +108,49 @@ def test_values_of_any_scale(hd, weight, power):
     for part in (slice(0, c), slice(c, 2 * c), slice(2 * c, 3 * c)):
         assert rel(grads[0][..., part], want["grads"][0][..., part]) < 10 * U[BF]
     assert rel(grads[3], want["grads"][3]) < 24 * U[BF]
+
+
+# ------------------------------------------------------------------------------------------------ rows that add up
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("weight,spread", [(1.0, 1.0), (2.0, 0.3), (3.0, 1.0), (3.0, 0.3)])
+def test_the_backwards_weights_add_up_to_one(hd, dtype, weight, spread):
+    """With dout one for a single query of each window, dv is that query's weights.  Aligned q and k, whose logits are large, at
+    norm weights of one to three.  Rounded on the way: the weights (in the forward, whose sum divides them, and here) and
+    dv, each u of a root sum of squares that is at most one: 3^1/2 u."""
+    nh = 2
+    qkv, qw, kw, table, geom, dout = inputs(1, 1, 8, 8, 9, 18, nh, hd, dtype, True, seed=7)
+    c = nh * hd
+    common = torch.randn(c, generator=torch.Generator(device=DEV).manual_seed(1), device=DEV)
+    qkv = torch.cat([spread * qkv[..., :c] + common, spread * qkv[..., c:2 * c] + common, qkv[..., 2 * c:]], -1).to(dtype)
+    dout = torch.zeros_like(dout)
+    sh, sw = geom.shift
+    dout[:, :, (4 + sh) % 9::9, (7 + sw) % 18::18] = 1.0  # token (4, 7) of every window
+    _, grads = call(qkv, (qw * weight).to(dtype), (kw * weight).to(dtype), table, geom, nh, hd, dout)
+    dv = torch.roll(grads[0][..., 2 * c:].double(), (-sh, -sw), (2, 3))
+    total = dv.view(8, 9, 8, 18, nh, hd).sum((1, 3))
+    assert (total - 1).square().mean().sqrt() < 3 ** 0.5 * U[dtype]
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("weight", [1.0, 2.0, 3.0])
+def test_common_offset_of_dp_cancels(hd, dtype, weight):
+    """Aligned q and k, and dout and v with a common offset: dP is nearly one number in a row, and dS what remains of it less
+    D.  Weights that do not add up to one leave a part of the offset."""
+    nh = 2
+    qkv, qw, kw, table, geom, dout = inputs(1, 1, 2, 2, 9, 18, nh, hd, dtype, True, seed=7)
+    c = nh * hd
+    g = torch.Generator(device=DEV).manual_seed(1)
+    common, of_v = (torch.randn(c, generator=g, device=DEV) for _ in range(2))
+    qkv = torch.cat([0.3 * qkv[..., :c] + common, 0.3 * qkv[..., c:2 * c] + common, 0.25 * qkv[..., 2 * c:] + of_v], -1).to(dtype)
+    qw, kw = (qw * weight).to(dtype), (kw * weight).to(dtype)
+    dout = (0.25 * dout + of_v).to(dtype)
+    out, grads = call(qkv, qw, kw, table, geom, nh, hd, dout)
+    want = definition(qkv, qw, kw, table, geom, nh, hd, dout)
+    u = U[dtype]
+    for name, part in (("dq", slice(0, c)), ("dk", slice(c, 2 * c))):
+        got, g, s = grads[0][..., part].double(), want["grads"][0][..., part], want["slack"][0][..., part]
+        assert (got - g).norm() < 10 * u * g.norm() + 3 * u * s.norm(), name
+    for h in range(nh):
+        assert (grads[3][h].double() - want["grads"][3][h]).norm() < 24 * u * want["grads"][3][h].norm() + 3 * u * want["noise"][h]
