@@ -154,3 +154,41 @@ def test_common_offset_of_dp_cancels(hd, dtype, weight):
         assert (got - g).norm() < 10 * u * g.norm() + 3 * u * s.norm(), name
     for h in range(nh):
         assert (grads[3][h].double() - want["grads"][3][h]).norm() < 24 * u * want["grads"][3][h].norm() + 3 * u * want["noise"][h]
+
+
+@pytest.mark.parametrize("dtype,hd", [(BF, 16), (BF, 32), (BF, 64), (BF, 128), (HF, 32), (HF, 64), (HF, 128)])
+def test_each_heads_gradient(dtype, hd):
+    """The table's gradient head by head, each against its own size, at offsets, wide ranges, the types' lowest values and
+    infinities."""
+    nh, wh, ww = 3, 9, 18
+    qkv, qw, kw, table, geom, dout = inputs(1, 1, 2, 2, wh, ww, nh, hd, dtype, True, seed=4)
+    g = torch.Generator(device=DEV).manual_seed(9)
+    low = torch.finfo(F32).min
+    b = geom.relative_buckets().to(DEV)
+    cases = {"plain": table.float(), "offset": table.float() + 1000.0, "wide": table.float() * 60,
+             "far below": table.float() - 3e6, "all lowest": torch.full_like(table, low, dtype=F32)}
+    cases["masked"] = table.float().masked_fill(torch.rand(table.shape, generator=g, device=DEV) < 0.4, -INF)
+    cases["masked"][:, b[0, 0]] = 1.0
+    apart = table.float().clone()
+    apart[1] = -INF
+    apart[2] = low
+    apart[2, b[0, 1]] = 3.0
+    cases["heads apart"] = apart
+    half = table.float().clone()  # the lowest value of fp16, with one displacement left of the second head
+    half[1:] = torch.finfo(HF).min
+    half[1, b[0, 1]] = 3.0
+    cases["lowest of fp16"] = half
+    u = U[dtype]
+    for name, t in cases.items():
+        out, grads = call(qkv, qw, kw, t, geom, nh, hd, dout)
+        want = definition(qkv, qw, kw, t, geom, nh, hd, dout)
+        assert rel(out, want["out"]) < 6 * u, name
+        c = nh * hd
+        for part in (slice(0, c), slice(c, 2 * c), slice(2 * c, 3 * c)):
+            got, e, s = grads[0][..., part].double(), want["grads"][0][..., part], want["slack"][0][..., part]
+            assert (got - e).norm() < 10 * u * e.norm() + 3 * u * s.norm(), name
+        for h in range(nh):
+            got, e = grads[3][h].double(), want["grads"][3][h]
+            allowed = 24 * u * e.norm() + 3 * u * want["noise"][h]
+            assert (got - e).norm() <= allowed, (name, h)
+            assert allowed < 0.75 * e.norm() or not e.any(), (name, h)  # a gradient of zeros does not pass
