@@ -428,12 +428,10 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
   float* sD = sLse + lp;
   float* sRq = sD + lp;
   float* sRk = sRq + lp;
-  float* sWq = sRk + lp;  // [HD] partial dqw
-  float* sWk = sWq + HD;  // [HD] partial dkw
-  int* sTok = reinterpret_cast<int*>(sWk + HD);
+  int* sTok = reinterpret_cast<int*>(sRk + lp);
   signed char* sLab = reinterpret_cast<signed char*>(sTok + lp);
   const int buckets = (2 * g.T - 1) * (2 * g.wh - 1) * (2 * g.ww - 1);
-  float* sTab = reinterpret_cast<float*>(smem + ((size_t)4 * lp * RS * sizeof(T) + lp * 21 + 2 * HD * 4 + 15) / 16 * 16);
+  float* sTab = reinterpret_cast<float*>(smem + ((size_t)4 * lp * RS * sizeof(T) + lp * 21 + 15) / 16 * 16);
   short* sOff = reinterpret_cast<short*>(sTab + (BIAS ? bias.stride : 0));
   RowStat* sStat = reinterpret_cast<RowStat*>(sOff + (BIAS ? lp : 0));
   float* sSum = reinterpret_cast<float*>(sStat + (BIAS ? lp : 0));  // with dbias_part: the buckets, then the warps' tiles
@@ -464,10 +462,6 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
     }
   } else {
     for (int i = threadIdx.x; i < lp; i += blockDim.x) sLse[i] = i < L ? lse[lse_base + i] : INFINITY;
-  }
-  for (int i = threadIdx.x; i < HD; i += blockDim.x) {
-    sWq[i] = 0.f;
-    sWk[i] = 0.f;
   }
   {  // D_i = sum_d dO_i,d * O_i,d
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
@@ -787,21 +781,25 @@ __global__ void __launch_bounds__(192, 2) bwd_kernel(const T* __restrict__ qkv, 
       wk[i] += __shfl_xor_sync(0xffffffffu, wk[i], o);
     }
   }
+  // the warps' sums in order, so that results repeat; the operands' rows make room for them
+  __syncthreads();
+  float* red = reinterpret_cast<float*>(smem);  // [warps][2][HD]
   if (gq == 0) {
 #pragma unroll
     for (int d = 0; d < DT; ++d) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        atomicAdd(&sWq[d * 8 + 2 * tq + e], wq[2 * d + e]);
-        atomicAdd(&sWk[d * 8 + 2 * tq + e], wk[2 * d + e]);
+        red[2 * warp * HD + d * 8 + 2 * tq + e] = wq[2 * d + e];
+        red[(2 * warp + 1) * HD + d * 8 + 2 * tq + e] = wk[2 * d + e];
       }
     }
   }
   __syncthreads();
   const int64_t cta = (int64_t)blockIdx.y * gridDim.x + blockIdx.x;
-  for (int i = threadIdx.x; i < HD; i += blockDim.x) {
-    dqw_part[cta * HD + i] = sWq[i];
-    dkw_part[cta * HD + i] = sWk[i];
+  for (int i = threadIdx.x; i < 2 * HD; i += blockDim.x) {
+    float sum = 0.f;
+    for (int w = 0; w < nw; ++w) sum += red[2 * w * HD + i];
+    (i < HD ? dqw_part : dkw_part)[cta * HD + i % HD] = sum;
   }
 }
 
@@ -830,7 +828,7 @@ static cudaError_t launch_bwd(const void* qkv, const float* qw, const float* kw,
   const int nt = (L + 15) / 16;
   const int lp = nt * 16;
   const size_t smem = (size_t)4 * lp * (HD + 8) * sizeof(T) + (size_t)4 * lp * sizeof(float) +
-                      2 * HD * sizeof(float) + (size_t)lp * (sizeof(int) + 1) +
+                      (size_t)lp * (sizeof(int) + 1) +
                       (bias.tab ? 16 + bias_bytes(bias, lp) + (size_t)lp * sizeof(RowStat) : 0) +
                       (dbias_part ? (size_t)(2 * g.T - 1) * (2 * g.wh - 1) * (2 * g.ww - 1) * sizeof(float) +
                                         6 * kBiasTile * sizeof(T)

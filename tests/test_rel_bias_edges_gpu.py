@@ -192,3 +192,20 @@ def test_each_heads_gradient(dtype, hd):
             allowed = 24 * u * e.norm() + 3 * u * want["noise"][h]
             assert (got - e).norm() <= allowed, (name, h)
             assert allowed < 0.75 * e.norm() or not e.any(), (name, h)  # a gradient of zeros does not pass
+
+
+# ------------------------------------------------------------------------------------------------ calls
+@pytest.mark.parametrize("bias", [True, False])
+@pytest.mark.parametrize("dtype,hd", [(BF, 16), (BF, 64), (BF, 128), (HF, 32), (HF, 128)])
+def test_results_repeat(dtype, hd, bias):
+    nh = 3
+    qkv, qw, kw, table, geom, dout = inputs(1, 1, 3, 3, 9, 18, nh, hd, dtype, True, seed=2)
+    leaves = [t.clone().requires_grad_() for t in (qkv, qw, kw, table)][:4 if bias else 3]
+
+    def step():
+        out = ops.window_attention(*leaves[:3], nh, hd, geom, hd ** -0.5, rel_bias=leaves[3] if bias else None)
+        return [out.detach(), *torch.autograd.grad(out, leaves, dout)]
+
+    first = step()
+    for _ in range(20):
+        assert all(torch.equal(a, b) for a, b in zip(first, step()))
