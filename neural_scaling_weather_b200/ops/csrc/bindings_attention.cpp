@@ -126,7 +126,7 @@ struct AttnBiasNode : public torch::autograd::Function<AttnBiasNode> {
     const auto v = ctx->get_saved_variables();
     std::vector<at::ScalarType> types;
     for (int64_t t : ctx->saved_data["types"].toIntVector()) types.push_back((at::ScalarType)t);
-    auto r = attn_bias_bwd(v[0], v[1], v[2], grad[0].contiguous(), v[3], ctx->saved_data["geom"].toIntVector(),
+    auto r = attn_bias_bwd(v[0], v[1], v[2], packed(grad[0]), v[3], ctx->saved_data["geom"].toIntVector(),
                            ctx->saved_data["scale"].toDouble(),
                            {ctx->needs_input_grad(1), ctx->needs_input_grad(2), ctx->needs_input_grad(3)},
                            std::vector<OptTensor>(3), types);
@@ -139,7 +139,7 @@ struct AttnBiasNode : public torch::autograd::Function<AttnBiasNode> {
 // qkv (B, T, H, W, 3 heads head_dim) in 16 bits -> (B, T, H, W, heads head_dim); parameters in any of the three types
 Tensor window_attention_bias(const Tensor& qkv_in, const Tensor& qw, const Tensor& kw, const Tensor& rel_bias,
                              const std::vector<int64_t>& gi, double scale) {
-  const Tensor qkv = qkv_in.contiguous();
+  const Tensor qkv = packed(qkv_in);
   if (tangents())
     for (const Tensor* t : {&qkv, &qw, &kw, &rel_bias}) no_tangent(*t, "window_attention");
   bool grad = false;

@@ -62,6 +62,11 @@ bool rows_aligned(const Tensor& t) {
   return t.stride(1) == 1 && (t.size(0) == 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1))) &&
          (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) == 0;
 }
+// contiguous and at a 16-byte boundary, which a view into a packed buffer may miss: t itself or a copy
+Tensor packed(const Tensor& t) {
+  const Tensor c = t.contiguous();
+  return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15) == 0 ? c : c.clone();
+}
 // Operands as the kernels read them: each itself, or a copy with padded rows where its strides or address do not
 // allow 16-byte accesses.  One launch makes all copies of a call.
 struct Aligner {

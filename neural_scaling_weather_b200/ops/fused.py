@@ -543,6 +543,12 @@ def _geom_ints(B, T, H, W, nh, hd, g: WindowGeometry):
 ATTN_FWD_IMPL = int(os.environ.get("NSW_ATTN_FWD_IMPL", "0"))
 
 
+def _packed(t: torch.Tensor) -> torch.Tensor:
+    """Contiguous and at a 16-byte boundary, which a view into a packed buffer may miss: ``t`` itself or a copy."""
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
 class _WindowAttn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, qw, kw, gi, scale):
@@ -581,7 +587,7 @@ class _BiasedWindowAttn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qkv, qw, kw, rel_bias, gi, scale):
-        qkv = qkv.contiguous()
+        qkv = _packed(qkv)
         out, lse, tab = require().attn_bias_fwd(qkv, qw, kw, rel_bias, gi, scale)
         ctx.save_for_backward(qkv, tab, out, lse)
         ctx.params, ctx.gi, ctx.scale = (qw, kw, rel_bias), gi, scale
@@ -596,7 +602,7 @@ class _BiasedWindowAttn(torch.autograd.Function):
         need = ctx.needs_input_grad[1:4]
         given = [id(p) for p in ctx.params]  # one that is here twice: its shares meet in autograd
         into = [gradsink.target(p) if n and given.count(id(p)) == 1 else None for p, n in zip(ctx.params, need)]
-        dqkv, *grads = require().attn_bias_bwd(qkv, tab, out, dout.to(qkv.dtype).contiguous(), lse, ctx.gi, ctx.scale,
+        dqkv, *grads = require().attn_bias_bwd(qkv, tab, out, _packed(dout.to(qkv.dtype)), lse, ctx.gi, ctx.scale,
                                                list(need), into, [p.dtype for p in ctx.params])
         for p, t, n in zip(ctx.params, into, need):
             if n:

@@ -209,3 +209,31 @@ def test_results_repeat(dtype, hd, bias):
     first = step()
     for _ in range(20):
         assert all(torch.equal(a, b) for a, b in zip(first, step()))
+
+
+def shifted(t, by):
+    """The same contiguous tensor, `by` elements into a packed buffer."""
+    flat = torch.zeros(t.numel() + 16, dtype=t.dtype, device=t.device)
+    v = flat[by:by + t.numel()].view(t.shape)
+    v.copy_(t)
+    return v
+
+
+@pytest.mark.parametrize("bias", [True])
+@pytest.mark.parametrize("dtype,hd", [(BF, 64), (HF, 64), (BF, 128), (HF, 32)])
+@pytest.mark.parametrize("master", [False, True])
+def test_inputs_of_any_alignment(dtype, hd, master, bias):
+    nh = 2
+    qkv, qw, kw, table, geom, dout = inputs(1, 1, 2, 2, 9, 18, nh, hd, dtype, True, seed=3)
+    if master:
+        qw, kw, table = (torch.nn.Parameter(t.float()) for t in (qw, kw, table))
+
+    def step(x, d):
+        leaves = [x.detach().requires_grad_(), *(t.detach().requires_grad_() if not master else t for t in (qw, kw, table))]
+        out = ops.window_attention(*leaves[:3], nh, hd, geom, hd ** -0.5, rel_bias=leaves[3] if bias else None)
+        return [out.detach(), *torch.autograd.grad(out, leaves[:4 if bias else 3], d)]
+
+    want = step(qkv, dout)
+    for by in (1, 3, 4):
+        got = step(shifted(qkv, by), shifted(dout, 8 - by))
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
