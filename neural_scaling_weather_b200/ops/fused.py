@@ -553,7 +553,7 @@ class _WindowAttn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, qkv, qw, kw, gi, scale):
         ext = require()
-        qkv2 = qkv.contiguous()
+        qkv2 = _packed(qkv)
         out, lse = ext.window_attn_fwd(qkv2, qw.detach().float().contiguous(),
                                        kw.detach().float().contiguous(), gi, scale, ATTN_FWD_IMPL)
         ctx.save_for_backward(qkv2, qw, kw, out, lse)
@@ -571,7 +571,7 @@ class _WindowAttn(torch.autograd.Function):
         inplace = tq is not None and tk is not None
         dqkv, dqw, dkw = ext.window_attn_bwd(qkv, qw.detach().float().contiguous(),
                                              kw.detach().float().contiguous(), out,
-                                             dout.to(qkv.dtype).contiguous(), lse, ctx.gi, ctx.scale,
+                                             _packed(dout.to(qkv.dtype)), lse, ctx.gi, ctx.scale,
                                              dqw_into=tq if inplace else None, dkw_into=tk if inplace else None)
         if ctx.needs_input_grad[1] or ctx.needs_input_grad[2]:
             gradsink.done(qw, inplace)

@@ -219,7 +219,7 @@ def shifted(t, by):
     return v
 
 
-@pytest.mark.parametrize("bias", [True])
+@pytest.mark.parametrize("bias", [True, False])
 @pytest.mark.parametrize("dtype,hd", [(BF, 64), (HF, 64), (BF, 128), (HF, 32)])
 @pytest.mark.parametrize("master", [False, True])
 def test_inputs_of_any_alignment(dtype, hd, master, bias):
