@@ -93,11 +93,13 @@ def expert_mlp(x, weights, experts, w_gate, w_up, w_down, residual=None, activat
     """The sum over a token's experts of its weight times the expert's gated network; see :func:`ops.expert_mlp`."""
     k = experts.shape[-1]
     rows, w, chosen = x.reshape(-1, x.shape[-1]), weights.reshape(-1, k), experts.reshape(-1, k)
-    y = x.new_zeros(rows.shape[0], w_down.shape[1])
+    y = None
     for e in range(w_gate.shape[0]):
         tok, slot = torch.nonzero(chosen == e, as_tuple=True)
-        out = gated_mlp(rows[tok], w_gate[e], w_up[e], w_down[e], activation=activation)
+        out = gated_mlp(rows[tok], w_gate[e], w_up[e], w_down[e], activation=activation)  # (autocast chooses its type)
+        y = out.new_zeros(rows.shape[0], out.shape[1]) if y is None else y
         y = y.index_add(0, tok, out * w[tok, slot].unsqueeze(1).to(out.dtype))
+    y = x.new_zeros(rows.shape[0], w_down.shape[1]) if y is None else y
     y = y.reshape(*x.shape[:-1], y.shape[1])
     return y if residual is None else y + residual
 

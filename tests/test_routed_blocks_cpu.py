@@ -124,6 +124,26 @@ def test_expert_refusals():
         ok(residual=res[:, 1:])
 
 
+def test_experts_under_autocast():
+    """fp32 parameters under autocast, as the dense gated network takes them: products in bf16, gradients in fp32.  On the
+    way to y about eight roundings (x, a weight, g or u, the activation, h, w_down, the expert's output, its weighted sum),
+    each at most 2^-8 of its value: 2^-5 of the largest.  Gradients pass as many again twice (through y, whose error is in
+    2 y, and back): 2^-3."""
+    x, w, idx, wg, wu, wd, res = (t.float() if t.is_floating_point() else t for t in _experts(m=9, e=4))
+    leaves = [t.requires_grad_() for t in (x, w, wg, wu, wd, res)]
+    want = ops.expert_mlp(x, w, idx, wg, wu, wd, residual=res)
+    exact = torch.autograd.grad(want.square().sum(), leaves)
+    with torch.autocast("cpu", dtype=torch.bfloat16):
+        plain = ops.expert_mlp(x, w, idx, wg, wu, wd)
+        y = ops.expert_mlp(x, w, idx, wg, wu, wd, residual=res)
+        none = ops.expert_mlp(x, w, torch.full_like(idx, -1), wg, wu, wd)
+        assert plain.dtype == none.dtype == ops.gated_mlp(x, wg[0], wu[0], wd[0]).dtype == torch.bfloat16
+        assert none.abs().max() == 0
+    assert (y - want).abs().max() < 2.0 ** -5 * want.abs().max()
+    for a, b in zip(torch.autograd.grad(y.float().square().sum(), leaves), exact):
+        assert a.dtype == torch.float32 and (a - b).abs().max() < 2.0 ** -3 * b.abs().max()
+
+
 # --------------------------------------------------------------------------- relative position bias
 def test_buckets_are_displacements():
     geom = ops.WindowGeometry(window=(3, 2))
