@@ -480,6 +480,7 @@ Tensor expert_mlp(const Tensor& x, const Tensor& weights, const Tensor& experts,
   TORCH_CHECK_VALUE(weights.sizes() == experts.sizes() && weights.dim() == x.dim() &&
                         weights.sizes().slice(0, x.dim() - 1) == lead,
                     "expert_mlp: weights ", weights.sizes(), " and experts ", experts.sizes(), " are not (", lead, ", k)");
+  TORCH_CHECK_VALUE(weights.size(-1) >= 1, "expert_mlp: no experts a token");
   TORCH_CHECK_VALUE(!residual || (residual->dim() == x.dim() && residual->size(-1) == wd.size(1) &&
                                   residual->sizes().slice(0, x.dim() - 1) == lead),
                     "expert_mlp: residual ", residual->sizes(), " is not the output's shape");

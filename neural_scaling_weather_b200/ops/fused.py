@@ -451,6 +451,8 @@ def check_expert_shapes(x, weights, experts, wg, wu, wd, residual):
     if weights.shape != experts.shape or weights.dim() != x.dim() or weights.shape[:-1] != x.shape[:-1]:
         raise ValueError(f"expert_mlp: weights {tuple(weights.shape)} and experts {tuple(experts.shape)} must be "
                          f"({', '.join(map(str, (*x.shape[:-1], 'k')))})")
+    if weights.shape[-1] < 1:
+        raise ValueError("expert_mlp: no experts a token")
     if residual is not None and residual.shape != x.shape[:-1] + wd.shape[1:2]:
         raise ValueError(f"expert_mlp: residual {tuple(residual.shape)} is not the output's shape")
 

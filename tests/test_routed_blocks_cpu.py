@@ -124,6 +124,18 @@ def test_expert_refusals():
         ok(residual=res[:, 1:])
 
 
+@pytest.mark.parametrize("device", ["cpu", pytest.param("cuda", marks=pytest.mark.gpu)])
+@pytest.mark.parametrize("lead", [(7,), (7, 1), (0,)])
+def test_no_experts_a_token_is_refused(device, lead):
+    dt = D if device == "cpu" else torch.bfloat16
+    x = torch.zeros(*lead, 8, device=device, dtype=dt)
+    none = torch.zeros(*lead, 0, device=device, dtype=dt)
+    for master in (dt, torch.float32):
+        w = [torch.zeros(2, 8, 8, device=device, dtype=master) for _ in range(3)]
+        with pytest.raises(ValueError, match="no experts a token"):
+            ops.expert_mlp(x, none, none.long(), *w)
+
+
 def test_experts_under_autocast():
     """fp32 parameters under autocast, as the dense gated network takes them: products in bf16, gradients in fp32.  On the
     way to y about eight roundings (x, a weight, g or u, the activation, h, w_down, the expert's output, its weighted sum),
