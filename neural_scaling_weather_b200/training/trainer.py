@@ -594,9 +594,9 @@ class Trainer:
         if dist.is_initialized() and comm.get_size("dp") > 1:
             dist.all_reduce(train_loss, op=dist.ReduceOp.AVG, group=comm.get_group("dp"))
             dist.all_reduce(grad, op=dist.ReduceOp.AVG, group=comm.get_group("dp"))
-            if self.routed:
-                dist.all_reduce(balance, op=dist.ReduceOp.AVG, group=comm.get_group("dp"))
         if self.routed:
+            if dist.is_initialized() and comm.get_size("dp-sp1-sp2") > 1:  # (spatial ranks route their own tokens)
+                dist.all_reduce(balance, op=dist.ReduceOp.AVG, group=comm.get_group("dp-sp1-sp2"))
             self.logs["router_balance"] = float(balance.item())
         self.logs["train_loss"] = float(train_loss.item())
         self.logs["grad"] = float(grad.item())

@@ -382,3 +382,35 @@ def test_trainer_adds_the_balance_loss_and_resumes_older_runs(tmp_path):
     C.save(cfg, path)
     run(_train, 1, str(tmp_path / "c"), plain, None, None)
     assert with_model_options({"model": {"num_experts": 2}}) != with_model_options({"model": {}})
+
+
+def _logged_balance_worker(rank, world, exp_dir, options, out):
+    """Trains, and keeps of each log what this rank's routers had and what was logged."""
+    from neural_scaling_weather_b200.training.trainer import Trainer
+    from tests.test_trainer_cpu import BASE
+
+    t = Trainer(C.compose("default", BASE + [f"hydra.run.dir={exp_dir}"] + options))
+    log, rows = t.validate_and_checkpoint, []
+
+    def keep():
+        own = (t.router_balance / max(1, t.n_mbs - t.n_mbs_last_log)).item()
+        log()
+        rows.append((own, t.logs["router_balance"]))
+
+    t.validate_and_checkpoint = keep
+    t.launch()
+    torch.save(rows, f"{out}{rank}.pt")
+
+
+@pytest.mark.parametrize("world,split", [(2, ["parallelism.sp2=2"]), (2, ["parallelism.sp1=2"]), (2, []),
+                                         (4, ["parallelism.sp2=2"])])
+def test_the_logged_balance_is_every_ranks(tmp_path, world, split):
+    """The mean over the data-parallel (the ranks that are not split) and the spatial ranks: each routes its own tokens."""
+    run(_logged_balance_worker, world, str(tmp_path / "a"), OPTIONS + split, str(tmp_path / "rank"))
+    ranks = [torch.load(tmp_path / f"rank{r}.pt") for r in range(world)]
+    assert len(ranks[0]) == 2
+    for rows in zip(*ranks):
+        own = [r[0] for r in rows]
+        assert len(set(own)) == world
+        for _, logged in rows:
+            assert abs(logged - sum(own) / world) < 1e-5
