@@ -505,4 +505,5 @@ void bind_experts(py::module& m) {
   m.def("expert_mlp", &expert_mlp);
   m.def("expert_mlp_fwd", &expert_mlp_fwd);
   m.def("expert_mlp_bwd", &expert_mlp_bwd);
+  m.def("expert_tile", &nsw::expert_tile);
 }

@@ -483,17 +483,21 @@ static bool aligned(const void* p, int64_t ld) { return ld % 8 == 0 && (reinterp
 int64_t expert_tiles(int64_t count, int64_t experts, int tile) {
   return (count + (tile - 1) * std::min(count, experts)) / tile;
 }
-// Up to 64 rows an expert on average (in every expert) the split products, whose tiles are 32 or 64 rows, read the
-// weights about as fast as gated_kernel with its 256-row tiles and start and end sooner; so they do while their blocks
-// fit the device at once.  Microseconds of a call without gradients, in a graph, weights not in L2, tiles of 32 / 64 / 256
-// rows: 2 experts of 768 x 1024: 37 rows each 24 / 25 / 37, 128 each 36 / 31 / 41, 512 each 80 / 55 / 43; 8 of 1024 x
-// 2736: 9 each 55 / 59 / 72, 32 each 66 / 64 / 76, 64 each 80 / 70 / 76, 128 each 119 / 94 / 76; 64 of 512 x 680: 4 each
-// 59 / 66 / 76, 64 each 102 / 88 / 82.
+// Up to 48 rows an expert on average (in every expert) the split products, whose tiles are 32 or 64 rows, read the
+// weights about as fast as gated_kernel with its 256-row tiles and start and end sooner; so they do with more rows while
+// their blocks are few, three an SM, or five where most experts have one tile yet.  Microseconds of a call without gradients, in a
+// graph, weights not in L2, tiles of 32 / 64 / 256 rows, and 64-row tiles' blocks of the up projection:
+//   2 experts of 768 x 1024:    512 rows 43 / 35 / 39 (272),  1024 - / 51 / 43 (528)
+//   2 of 1024 x 4096:           128 rows 47 / 41 / 57 (320),  192 59 / 51 / 57 (448),  384 96 / 68 / 66 (832)
+//   8 of 1024 x 2736:           8 rows 55 / 59 / 72,  32 57 / 62 / 70,  64 76 / 66 / 72 (645),  96 84 / 78 / 72 (817)
+//   32 of 768 x 512:            48 rows 57 / 49 / 57,  64 64 / 55 / 58 (504),  96 79 / 68 / 61 (632)
+//   64 of 1024 x 1368:          16 rows 140 / 152 / 162,  48 201 / 162 / 168 (2442),  64 236 / 195 / 172 (2794)
+//   128 of 256 x 344:           8 rows 51 / 53 / 64,  48 82 / 70 / 74 (1332),  64 94 / 82 / 74 (1524)
 int expert_tile(int64_t count, int64_t experts, int64_t H, int64_t N) {
   if (experts * std::max(H, N) >= INT32_MAX) return kExpertTile;  // (the split products' rows of all experts' weights)
   if (count <= 24 * experts) return 32;
   const int64_t blocks = expert_tiles(count, experts, 64) * ((H + 63) / 64);
-  return count <= 64 * experts || blocks <= 2 * tc::sm_count() ? 64 : kExpertTile;
+  return count <= 48 * experts || blocks <= (count <= 64 * experts ? 5 : 3) * tc::sm_count() ? 64 : kExpertTile;
 }
 static int64_t plan_chunks(int64_t count) {
   return count <= experts::kOneChunk ? 1 : (count + experts::kChunk - 1) / experts::kChunk;
