@@ -193,9 +193,11 @@ def expert_mlp(x: torch.Tensor, weights: torch.Tensor, experts: torch.Tensor, w_
     ``w_gate`` and ``w_up`` (E, H, K), ``w_down`` (E, N, H); ``residual`` (..., N).  ``activation``: ``"silu"`` or
     ``"gelu"`` (exact).  Gradients of everything but the indices, each in its tensor's type; first derivatives in
     reverse mode.  Any sizes and strides on CUDA (weights whose rows are not multiples of 16 bytes are copied once a
-    call), at most 512 experts, 16 a token; the hidden values and the experts' outputs are 16-bit there.  The rows are
-    sorted by expert on the device (nothing waits for it) and the products run grouped by expert; calls without
-    gradients have forms of their own for a few assignments and for few rows an expert."""
+    call), at most 512 experts, 16 a token.  The hidden values, the experts' outputs and, in the backward, the weighted
+    gradients of the output and those of the hidden values are 16-bit there (in fp16 they overflow past 65504 and lose
+    bits below 6e-5: scale the loss).  The rows are sorted by expert on the device (nothing waits for it) and the products
+    run grouped by expert; calls without gradients have forms of their own for a few assignments and for few rows an
+    expert."""
     if activation not in GATED_ACTIVATIONS:
         raise ValueError(f"expert_mlp: activation {activation!r} is not one of {GATED_ACTIVATIONS}")
     if _use_cuda(x):

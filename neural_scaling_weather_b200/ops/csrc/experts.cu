@@ -12,7 +12,9 @@
 // Padding rows are zeros: the products make zeros of them, and the weights' gradients add zeros.
 // Rounded to 16 bits: the experts' outputs (before their weighted sum in fp32) and, in the backward, the weighted dy,
 // as operands of the next product and because wider ones would double the traffic here; each adds half a step beside
-// the products' own roundings (gated_mlp.cu).
+// the products' own roundings (gated_mlp.cu).  In fp16 that holds from 6e-5 to 65504: a weight of 1e-3 times a dy of 1e-3
+// keeps four bits, less than 3e-8 is zero, as it is for dg and du, in the dense network too.  A loss scale moves all
+// of them together; bf16 has fp32's range.
 #include <algorithm>
 
 #include "gated.cuh"

@@ -42,3 +42,49 @@ def test_forms_agree_about_the_rule(M, E, K, H):
     for m in (M, 3 * M, 6 * M):
         x, wt, chosen, w, res, _ = expert_inputs(m, 2, E, K, H, K, BF, seed=m)
         assert rel(ops.expert_mlp(x, wt, chosen, *w, residual=res), expert_exact(x, wt, chosen, w, res, "silu")) < 4 * U[BF]
+
+
+def rounded_backward(x, wt, chosen, w, dy, dtype, scale=1.0):
+    """The backward pass of SiLU experts in 64 bits, with what is said to be rounded to `dtype` rounded: g and u, the weighted
+    dy, dg and du, h, an assignment's dx.  dy times `scale` goes in, the gradients come out divided by it."""
+    r = lambda t: t.to(dtype).double()  # noqa: E731
+    xd, wd = x.double(), wt.double()
+    dx, grads = torch.zeros_like(xd), [torch.zeros(t.shape, dtype=torch.float64, device=DEV) for t in w]
+    for e in range(w[0].shape[0]):
+        tok, slot = torch.nonzero(chosen == e, as_tuple=True)
+        wg, wu, wdn = (t[e].double() for t in w)
+        g, u = xd[tok] @ wg.t(), xd[tok] @ wu.t()
+        h, g, u = r(g * torch.sigmoid(g) * u), r(g), r(u)
+        sig = torch.sigmoid(g)
+        dys = r(wd[tok, slot][:, None] * (dy.double() * scale)[tok])
+        dh = dys @ wdn
+        dg, du = r(dh * u * sig * (1 + g * (1 - sig))), r(dh * g * sig)
+        dx = dx.index_add(0, tok, r(dg @ wg + du @ wu))
+        for i, t in enumerate((dg.t() @ xd[tok], du.t() @ xd[tok], dys.t() @ h)):
+            grads[i][e] = t
+    return [t / scale for t in (dx, *grads)]
+
+
+@pytest.mark.parametrize("small", [1.0, 1e-2, 1e-3, 1e-4])
+def test_small_gradients_in_fp16(small):
+    """dy and the weights of the second choice are `small`.  What is rounded to fp16 on the way, no more, limits the gradients:
+    products below 6e-5 lose bits.  A loss scale that keeps them above it gives the definition's gradients again."""
+    M, E, K, H = 800, 4, 64, 72
+    x, wt, chosen, w, _, dy = expert_inputs(M, 2, E, K, H, K, HF, seed=11)
+    wt[:, 1] = (wt[:, 1].float() * small).to(HF)
+    dy = (dy.float() * small).to(HF)
+
+    def run(scale):
+        leaves = [t.clone().requires_grad_() for t in (x, *w)]
+        y = ops.expert_mlp(leaves[0], wt, chosen, *leaves[1:])
+        return [t.double() / scale for t in torch.autograd.grad(y, leaves, (dy.float() * scale).to(HF))]
+
+    # dx has six roundings, the weights' gradients five (see test_expert_ops_gpu.py); both sides have them here
+    for a, b in zip(run(1.0), rounded_backward(x, wt, chosen, w, dy, HF)):
+        # the result's own rounding, below 2^-14 in steps of 2^-24
+        step = 2.0 ** -24 * a.numel() ** 0.5
+        assert (a - b).norm() < 6 * U[HF] * b.norm() + step
+    scale = 2.0 ** round(-torch.tensor(small).log2().item())  # dy near one again
+    want = expert_exact(x, wt, chosen, w, None, "silu", dy)[1]
+    for a, b in zip(run(scale), [want[0], *want[2:]]):
+        assert rel(a, b) < 6 * U[HF]
