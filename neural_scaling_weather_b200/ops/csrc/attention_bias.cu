@@ -46,12 +46,6 @@ struct Carve {
   }
 };
 
-__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
-  if (dtype == kF32) return reinterpret_cast<const float*>(p)[i];
-  if (dtype == kBF16) return to_f(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-  return to_f(reinterpret_cast<const __half*>(p)[i]);
-}
-
 // One block a head, and one for the norms' weights.  Entries are less the head's largest, so that an offset of all of them
 // costs no precision, unless that is beyond 2^40: a head of the lowest value throughout, say, absorbs the logits, as it
 // does in 64 bits, and its rows are even.  A finite entry stays finite.
@@ -135,12 +129,7 @@ __global__ void __launch_bounds__(1024) grad_kernel(const Grads p) {
   for (int i = 1; i < 32; ++i) a += red[i][lane];
   const int64_t at = (head ? (int64_t)h * n : 0) + c;
   if (t.add) a += reinterpret_cast<const float*>(t.out)[at];
-  if (t.dtype == kF32)
-    reinterpret_cast<float*>(t.out)[at] = a;
-  else if (t.dtype == kBF16)
-    reinterpret_cast<__nv_bfloat16*>(t.out)[at] = from_f<__nv_bfloat16>(a);
-  else
-    reinterpret_cast<__half*>(t.out)[at] = from_f<__half>(a);
+  store_any(t.out, t.dtype, at, a);
 }
 
 // ------------------------------------------------------------------------------------------------------ layout

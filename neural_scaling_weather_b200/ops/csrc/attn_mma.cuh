@@ -1,4 +1,5 @@
-// Warp-level matrix products (mma.sync m16n8k16) and what goes with them, shared by the attention kernels on them.
+// Warp-level matrix products (mma.sync m16n8k16) and what goes with them, shared by the attention kernels on them; the
+// gated network's kernel for a few tokens takes the products.
 #pragma once
 
 #include "common.cuh"

@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "kernels.h"
+
 namespace nsw {
 
 // Device-side error word: kernels that give up a bounded wait or see an out-of-range
@@ -37,6 +39,21 @@ template <>
 __device__ __forceinline__ __half from_f<__half>(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ float from_f<float>(float v) { return v; }
+
+// an element of any of the three types
+__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) {
+  if (dtype == kF32) return reinterpret_cast<const float*>(p)[i];
+  if (dtype == kBF16) return to_f(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
+  return to_f(reinterpret_cast<const __half*>(p)[i]);
+}
+__device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v) {
+  if (dtype == kF32)
+    reinterpret_cast<float*>(p)[i] = v;
+  else if (dtype == kBF16)
+    reinterpret_cast<__nv_bfloat16*>(p)[i] = from_f<__nv_bfloat16>(v);
+  else
+    reinterpret_cast<__half*>(p)[i] = from_f<__half>(v);
+}
 
 // unpack/pack 8 16-bit floats from/to a uint4.  The vector is taken by value: a reference to
 // a shared- or global-memory uint4 read through a 16-bit pointer can compile to eight 2-byte

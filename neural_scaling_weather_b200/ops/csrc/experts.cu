@@ -183,15 +183,6 @@ __global__ void __launch_bounds__(kThreads) plan_scatter_kernel(const ExpertPlan
 }
 
 // ------------------------------------------------------------------------------------------- gather and combine
-__device__ __forceinline__ float load_any(const void* p, int dtype, int64_t i) { return tc::ld_bias(p, dtype, i); }
-__device__ __forceinline__ void store_any(void* p, int dtype, int64_t i, float v) {
-  if (dtype == kF32)
-    reinterpret_cast<float*>(p)[i] = v;
-  else if (dtype == kBF16)
-    reinterpret_cast<__nv_bfloat16*>(p)[i] = from_f<__nv_bfloat16>(v);
-  else
-    reinterpret_cast<__half*>(p)[i] = from_f<__half>(v);
-}
 // eight elements at p of which `left` are the row's; NC: by the read-only path, which stores do not hold up.  That path
 // is for what was complete before the first of a chain of programmatic dependents began (the caller's tensors): a kernel
 // that is resident while the one before it still writes takes what that one leaves by ordinary loads, behind its wait.

@@ -1,5 +1,5 @@
-// Device helpers shared by the gated feed-forward networks' kernels, dense and routed: the activations and their
-// slopes, biases of any type, cluster reads, and the warp-level products of a few tokens.
+// Device helpers shared by the gated feed-forward networks' kernels, dense and routed: the activations and their slopes,
+// and biases of any type.
 #pragma once
 
 #include "tcgen05.cuh"
@@ -48,57 +48,6 @@ __device__ __forceinline__ float ld_bias(const void* p, int dtype, int64_t i) {
   if (dtype == kBF16) return to_f(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
   return to_f(reinterpret_cast<const __half*>(p)[i]);
 }
-__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
-  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
-}
-
-__device__ __forceinline__ float4 ld_cluster4(uint32_t at) {
-  float4 o;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
-               : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w)
-               : "r"(at)
-               : "memory");
-  return o;
-}
 
 }  // namespace tc
-
-namespace gated {
-
-template <typename T>
-__device__ __forceinline__ void mma16816(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                         uint32_t b1);
-template <>
-__device__ __forceinline__ void mma16816<__nv_bfloat16>(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                        uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-template <>
-__device__ __forceinline__ void mma16816<__half>(float* c, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
-                                                 uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-
-// eight values at p (those below `left` of them, zeros after); NC: through the read-only path
-template <bool VEC, bool NC>
-__device__ __forceinline__ uint4 load8(const uint16_t* p, int left) {
-  if (left <= 0) return make_uint4(0, 0, 0, 0);
-  if (VEC && left >= 8) {
-    if (NC) return __ldg(reinterpret_cast<const uint4*>(p));
-    return *reinterpret_cast<const uint4*>(p);
-  }
-  uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-  for (int j = 0; j < 8; ++j)
-    if (j < left) w[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
-  return make_uint4(w[0], w[1], w[2], w[3]);
-}
-
-}  // namespace gated
 }  // namespace nsw

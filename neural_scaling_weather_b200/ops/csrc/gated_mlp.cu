@@ -41,6 +41,7 @@
 #include <algorithm>
 #include <cstring>
 
+#include "attn_mma.cuh"
 #include "gated.cuh"
 
 namespace nsw {
@@ -200,6 +201,9 @@ __device__ __forceinline__ void add_bias32(const void* p, int dtype, int64_t nb,
   }
 }
 
+__device__ __forceinline__ void prefetch_map(const CUtensorMap* m) {
+  asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(m)) : "memory");
+}
 __device__ __forceinline__ void bulk_wait_read_3() { asm volatile("cp.async.bulk.wait_group.read 3;" ::: "memory"); }
 
 // named barrier that also ANDs a predicate over its threads
@@ -921,6 +925,15 @@ static cudaError_t launch_dw_grouped(const GatedDwArgs& a, cudaStream_t s) {
 constexpr int kSplitThreads = 320;  // a multiple of a tile's quads: a thread's columns stay the same
 constexpr int kMaxSlices = 8;  // the largest portable cluster
 
+__device__ __forceinline__ float4 ld_cluster4(uint32_t at) {
+  float4 o;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+               : "=f"(o.x), "=f"(o.y), "=f"(o.z), "=f"(o.w)
+               : "r"(at)
+               : "memory");
+  return o;
+}
+
 struct SplitParams {
   CUtensorMap w0, w1, x0, x1;
   int64_t M, N;
@@ -1428,6 +1441,21 @@ struct SkinnyParams {
   int dependent;  // launched as a programmatic dependent of the kernel that writes x
 };
 
+// eight values at p (those below `left` of them, zeros after); NC: through the read-only path
+template <bool VEC, bool NC>
+__device__ __forceinline__ uint4 load8(const uint16_t* p, int left) {
+  if (left <= 0) return make_uint4(0, 0, 0, 0);
+  if (VEC && left >= 8) {
+    if (NC) return __ldg(reinterpret_cast<const uint4*>(p));
+    return *reinterpret_cast<const uint4*>(p);
+  }
+  uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int j = 0; j < 8; ++j)
+    if (j < left) w[j >> 1] |= (uint32_t)p[j] << (16 * (j & 1));
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
 // (DUAL: two steps' loads in flight and five blocks an SM, so that a projection's many blocks are resident at once;
 // 16 tokens, 2048 x 5464: 13.2 us against 15.9 with four steps and four blocks.  The down projection has few
 // blocks, which take four steps: 1 token, 1024 x 2736: 3.9 against 4.1 us)
@@ -1478,8 +1506,9 @@ __global__ void __launch_bounds__(32 * SK_WARPS, DUAL ? 5 : 1) skinny_kernel(con
       }
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
-        mma16816<T>(acc[n], wa[i].x, wb[i].x, wa[i].y, wb[i].y, xv[n].x, xv[n].y);
-        mma16816<T>(acc[n], wa[i].z, wb[i].z, wa[i].w, wb[i].w, xv[n].z, xv[n].w);
+        const uint32_t lo[4] = {wa[i].x, wb[i].x, wa[i].y, wb[i].y}, hi[4] = {wa[i].z, wb[i].z, wa[i].w, wb[i].w};
+        attn::mma16816<T>(acc[n], lo, xv[n].x, xv[n].y);
+        attn::mma16816<T>(acc[n], hi, xv[n].z, xv[n].w);
       }
     }
   }
