@@ -199,7 +199,8 @@ __device__ __forceinline__ uint4 row8(const uint16_t* p, int64_t left) {
 
 // A warp takes a token, 16 bytes a lane and step.  The loads of a step (kSpan column groups of it, two of its rows) leave
 // together and know of no branch: at 1024 columns and two experts a token that alone took the combining sum of 64800
-// tokens from 118 to 81 us (6.5 TB/s), the weighted gather from 140 to 113 and the plain one from 81 to 65.
+// tokens from 118 to 81 us, the weighted gather from 140 to 113 and the plain one from 81 to 65.  With the rows by
+// ordinary loads (see row8) the combining sum takes 91 us (5.8 TB/s), that of dx 69.
 constexpr int kRowWarps = 8, kSpan = 2;
 template <typename T, bool WEIGHTED, bool VEC>
 __global__ void __launch_bounds__(32 * kRowWarps, 4) gather_kernel(const ExpertPlan plan, const ExpertGather a) {
@@ -477,7 +478,7 @@ int64_t expert_tiles(int64_t count, int64_t experts, int tile) {
   return (count + (tile - 1) * std::min(count, experts)) / tile;
 }
 // Up to 48 rows an expert on average (in every expert) the split products, whose tiles are 32 or 64 rows, read the
-// weights about as fast as gated_kernel with its 256-row tiles and start and end sooner; so they do with more rows while
+// weights about as fast as gated_kernel with its 256-row tiles and start and end sooner; so they do up to 512 rows while
 // their blocks are few, three an SM, or five where most experts have one tile yet.  Microseconds of a call without gradients, in a
 // graph, weights not in L2, tiles of 32 / 64 / 256 rows, and 64-row tiles' blocks of the up projection:
 //   2 experts of 768 x 1024:    512 rows 43 / 35 / 39 (272),  1024 - / 51 / 43 (528)
@@ -485,12 +486,14 @@ int64_t expert_tiles(int64_t count, int64_t experts, int tile) {
 //   8 of 1024 x 2736:           8 rows 55 / 59 / 72,  32 57 / 62 / 70,  64 76 / 66 / 72 (645),  96 84 / 78 / 72 (817)
 //   32 of 768 x 512:            48 rows 57 / 49 / 57,  64 64 / 55 / 58 (504),  96 79 / 68 / 61 (632)
 //   64 of 1024 x 1368:          16 rows 140 / 152 / 162,  48 201 / 162 / 168 (2442),  64 236 / 195 / 172 (2794)
+//   4 of 128 x 344:             16 rows 21 / 21 / 31,  512 33 / 30 / 33 (210),  1024 - / 39 / 37 (402)
 //   128 of 256 x 344:           8 rows 51 / 53 / 64,  48 82 / 70 / 74 (1332),  64 94 / 82 / 74 (1524)
 int expert_tile(int64_t count, int64_t experts, int64_t H, int64_t N) {
   if (experts * std::max(H, N) >= INT32_MAX) return kExpertTile;  // (the split products' rows of all experts' weights)
   if (count <= 24 * experts) return 32;
+  if (count <= 48 * experts) return 64;
   const int64_t blocks = expert_tiles(count, experts, 64) * ((H + 63) / 64);
-  return count <= 48 * experts || blocks <= (count <= 64 * experts ? 5 : 3) * tc::sm_count() ? 64 : kExpertTile;
+  return count <= 512 * experts && blocks <= (count <= 64 * experts ? 5 : 3) * tc::sm_count() ? 64 : kExpertTile;
 }
 static int64_t plan_chunks(int64_t count) {
   return count <= experts::kOneChunk ? 1 : (count + experts::kChunk - 1) / experts::kChunk;

@@ -20,13 +20,15 @@ def _no_device_error():
     assert ext.read_error_flag(True) == 0
 
 
-# experts, width, hidden width, rows an expert, rows of a tile: by more than 5 % the fastest of the three where they were
+# experts, width, hidden width, rows an expert, rows of a tile: by 5 % or more the fastest of the three where they were
 # timed (the table beside expert_tile), on 148 SMs
-TILES = [(2, 768, 1024, 512, 64), (2, 768, 1024, 1024, 256), (2, 1024, 4096, 128, 64), (2, 1024, 4096, 512, 256),
-         (1, 1024, 2736, 512, 64), (1, 1024, 2736, 1024, 256), (8, 1024, 2736, 8, 32), (8, 1024, 2736, 64, 64),
-         (8, 1024, 2736, 96, 256), (8, 2048, 2736, 64, 64), (8, 2048, 2736, 96, 256), (32, 768, 512, 48, 64),
-         (32, 768, 512, 96, 256), (64, 512, 680, 48, 64), (64, 512, 680, 64, 256), (64, 1024, 1368, 16, 32),
-         (64, 1024, 1368, 64, 256), (128, 256, 344, 64, 256), (256, 512, 128, 64, 256)]
+TILES = [
+    (2, 768, 1024, 512, 64), (2, 768, 1024, 1024, 256), (2, 1024, 4096, 128, 64), (2, 1024, 4096, 512, 256), (4, 128, 344, 512, 64),
+    (4, 128, 344, 1024, 256), (1, 1024, 2736, 512, 64), (1, 1024, 2736, 1024, 256), (8, 1024, 2736, 8, 32), (8, 1024, 2736, 64, 64),
+    (8, 1024, 2736, 96, 256), (8, 2048, 2736, 64, 64), (8, 2048, 2736, 96, 256), (32, 768, 512, 48, 64), (32, 768, 512, 96, 256),
+    (64, 512, 680, 48, 64), (64, 512, 680, 64, 256), (64, 1024, 1368, 16, 32), (64, 1024, 1368, 64, 256), (128, 256, 344, 64, 256),
+    (256, 512, 128, 64, 256),
+]
 
 
 @pytest.mark.parametrize("E,K,H,rows,tile", TILES)
