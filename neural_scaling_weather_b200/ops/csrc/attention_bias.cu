@@ -7,9 +7,10 @@
 //
 // A window is at most 192 tokens of one head, so its products are short: what counts is how few instructions stand around
 // them, and that several windows are worked on at once on an SM.  64800 tokens of 16 heads of 64 in windows of 9 x 18, bf16:
-// forward 317 us a call (136 TFLOP/s, 1.7 TB/s), with the backward 1173 (backward 126 TFLOP/s); bound by the instructions of a logit (its entry from
-// shared memory, exponential, rounding) and by shared memory (75 % busy), not by products or memory.  The tcgen05 kernels of
-// the plain attention with the entries added to their logits took 463 and 1798.
+// forward 322 us a call (134 TFLOP/s, 1.7 TB/s), with the backward 1195 (backward 126 TFLOP/s); bound by shared memory, whose
+// data path is two thirds busy (a 16 x 16 block of logits takes 32 wavefronts for the fragments of K and V and 25 for its
+// entries and their offsets), and by latencies at four warps a scheduler, not by products or memory.  The tcgen05
+// kernels of the plain attention with the entries added to their logits took 463 and 1798.
 #include <float.h>
 #include <limits.h>
 
@@ -403,19 +404,26 @@ __device__ __forceinline__ float norm_chunk(const uint4& raw, const float* w, ui
 // has left in the head's header.  So they are at most 2^top, the bound is in the entries before the products begin, and
 // nothing is looked up or subtracted for a row.  Rows far below the bound lose precision to their type's smallest numbers:
 // those whose sum is below `least` (in fp16, 192 numbers that are each off by at most 2^-25 are off by less than 2^-17 of
-// it; in bf16 what fp32 holds of P V is then no less than with the row's largest logit subtracted) make their tile begin
-// again with every row less its own largest logit, for one more product of q and k.  So does a sum of P V beyond fp32,
-// which bf16 values above 2^30 may reach at weights of 2^top.  The second way's weights are at most 2^-drop, so that 192 of
-// them times any value of the type stay below fp32's largest number.
+// it) make their tile begin again with every row less its own largest logit, for one more product of q and k.  In bf16 the
+// weights meet V in fp32's range: a tile also begins again where a sum of P V is not finite (|V| above 2^(120 - top) at
+// weights of 2^top), and where a row's weights add up to less than one and one of its sums is below 2^-100, where what
+// 192 products lost below 2^-126 might show.  The second way's weights are at most 2^-drop, so that 192 of them times
+// any value of the type stay below fp32's largest number.
+// top: a product is no further below zero than the bound is above it, so twice the bound, and 24 for a row's entries below
+// the head's largest, leave few tiles to do again; 110 at most, where such weights still meet V of some hundreds.  From
+// there rows may be 154 below the bound, 1.44 head_dim^1/2 times the largest product of two norm weights (16 heads of 64: up
+// to weights of 3 or so a call takes the first way, 323 us, the second 573).
 template <typename T>
 struct Bound;
 template <>
 struct Bound<__nv_bfloat16> {
-  static constexpr float top = 90.f, least = 1.f, drop = 8.f;
+  static constexpr float least = 5.6843419e-14f, drop = 8.f;  // 2^-44
+  static __device__ __forceinline__ float top(float bound) { return fminf(2.f * bound + 24.f, 110.f); }
 };
 template <>
 struct Bound<__half> {
-  static constexpr float top = 14.f, least = 1.f, drop = 0.f;  // (65504 2^14 192 is far from fp32's limit)
+  static constexpr float least = 1.f, drop = 0.f;  // (65504 2^14 192 is far from fp32's limit)
+  static __device__ __forceinline__ float top(float) { return 14.f; }
 };
 constexpr float kMostBound = 1e4f;  // beyond it (or NaN): the second way at once
 
@@ -466,7 +474,7 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
   asm volatile("griddepcontrol.wait;" ::: "memory");  // (for the table and the norms' weights)
   const float bound = bias.tab[(int64_t)head * bias.stride];
   const bool exact = !(bound <= kMostBound);
-  const float less = exact ? 0.f : bound - Bound<T>::top;  // in the entries
+  const float less = exact ? 0.f : bound - Bound<T>::top(bound);  // in the entries
   const Window window = window_of(g, o, win);
   const bool mixed = window.y < o.far && window.y + g.wh > o.far;
   for (int i = threadIdx.x; i < rows; i += nthreads) {
@@ -628,6 +636,15 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
           finite = fma2(make_float2(acc[d][2], acc[d][3]), make_float2(0.f, 0.f), finite);
         }
         redo = redo || !(finite.x + finite.y == 0.f);
+        if (__any_sync(0xffffffffu, sum[0] < 1.f || sum[2] < 1.f)) {
+          float s0 = INFINITY, s1 = INFINITY;
+#pragma unroll
+          for (int d = 0; d < CH; ++d) {
+            s0 = fminf(s0, fminf(fabsf(acc[d][0]), fabsf(acc[d][1])));
+            s1 = fminf(s1, fminf(fabsf(acc[d][2]), fabsf(acc[d][3])));
+          }
+          redo = redo || (sum[0] < 1.f && s0 < 7.8886091e-31f) || (sum[2] < 1.f && s1 < 7.8886091e-31f);  // 2^-100
+        }
       }
       again = __any_sync(0xffffffffu, redo);
     }
@@ -675,7 +692,8 @@ __global__ void __launch_bounds__(32 * kFwdWarps, HD <= 64 ? 3 : 2)
 //           forward took; D_i = <dO_i, O_i>
 //   A       a warp's 16 keys against all queries: S^T begins with the entries less the row's logarithm of the sum, dP^T
 //           with -D, so that P^T is an exponential and dS^T a product away; dV and dK stay in registers; dS goes to shared
-//           memory in T (as the products take it), queries down
+//           memory in T (as the products take it; the bias's sums take it too, each term off by at most half a step of no
+//           sign: an fp32 copy, 103 KB at 162 tokens, does not fit), queries down
 //   B       a warp's 16 queries: dQ = dS K.  The next item's rows are on their way.
 // The bias's gradient sums dS over the windows of a head, without atomics and in a fixed order: of the two extents of the
 // window, one, a, is summed at once and the other, b, kept as a pair, acc[dt][da][b_i][b_j], whose entries belong to

@@ -91,8 +91,8 @@ def test_equal_tokens_give_their_value(hd, size):
 
 
 @pytest.mark.parametrize("hd", [16, 64, 128])
-@pytest.mark.parametrize("weight", [1.0, 12.0])
-@pytest.mark.parametrize("power", [-100, -40, 40, 100])
+@pytest.mark.parametrize("weight", [1.0, 4.0, 6.0, 12.0])
+@pytest.mark.parametrize("power", [-100, -60, -40, 0, 20, 40, 100])
 def test_values_of_any_scale(hd, weight, power):
     """v times a power of two scales the output and all gradients but v's.  weight: of one feature's norms alone, so that most
     logits are far below what the weights allow."""
