@@ -15,7 +15,9 @@
 // groups' sums in order and the blocks' rows are added in order by a second kernel, so results repeat bit for bit
 // (counts are integers, in any order).  A row that is -inf throughout has weights and probabilities of zero.
 //
-// Bound: reading the logits once (64800 x 64 bf16: 8.3 MB), and at a few tokens the launch.
+// Floor: reading the logits once (64800 x 64 bf16: 8.3 MB, 1.3 us).  There the forward takes 16.4 us, the balance's sum 5.8
+// and the backward 12: 2.2 and 2.0 instructions a cycle of 4 with a quarter and under half of the warps, which wait for the
+// results of their own shuffles and comparisons and for their loads.  A few tokens are bound by the launch.
 #include <math.h>
 
 #include "common.cuh"
