@@ -90,3 +90,26 @@ def test_small_gradients_in_fp16(small):
     want = expert_exact(x, wt, chosen, w, None, "silu", dy)[1]
     for a, b in zip(run(scale), [want[0], *want[2:]]):
         assert rel(a, b) < 6 * U[HF]
+
+
+@pytest.mark.parametrize("master", [False, True])
+def test_a_single_token_without_a_batch(master):
+    """x (K,), weights and experts (k,), residual (N,): one token, with its gradients."""
+    x, wt, chosen, w, res, dy = expert_inputs(1, 2, 4, 64, 40, 72, BF, seed=5)
+    logits = torch.randn(4, device=DEV).requires_grad_()
+    weights, experts, balance = ops.route_tokens(logits, 2)
+    rows = ops.route_tokens(logits[None], 2)
+    assert weights.shape == experts.shape == (2,) and torch.equal(weights, rows[0][0]) and torch.equal(experts, rows[1][0])
+    got, want = (torch.autograd.grad([a.sum() + 2 * a.flatten()[0], b], logits, [torch.ones_like(b)] * 2)[0]
+                 for a, b in ((weights, balance), (rows[0], rows[2])))
+    assert torch.equal(got, want)
+    if master:
+        w = [torch.nn.Parameter(t.float()) for t in w]
+    leaves = [x, wt, *w, res]
+    leaves = [t if isinstance(t, torch.nn.Parameter) else t.detach().requires_grad_() for t in leaves]
+    args = [leaves[0], leaves[1], chosen, *leaves[2:5], leaves[5]]
+    y2 = ops.expert_mlp(*args[:6], residual=args[6])
+    y1 = ops.expert_mlp(args[0][0], args[1][0], chosen[0], *args[3:6], residual=args[6][0])
+    assert y1.shape == (72,) and torch.equal(y1, y2[0])
+    for a, b in zip(torch.autograd.grad(y1, leaves, dy[0]), torch.autograd.grad(y2, leaves, dy)):
+        assert a.shape == b.shape and torch.equal(a, b)

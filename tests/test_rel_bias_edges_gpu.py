@@ -194,6 +194,22 @@ def test_each_heads_gradient(dtype, hd):
             assert allowed < 0.75 * e.norm() or not e.any(), (name, h)  # a gradient of zeros does not pass
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("hd", [16, 32, 64, 128])
+@pytest.mark.parametrize("T,wh,ww", [(4, 6, 8), (8, 4, 6), (6, 5, 6), (192, 1, 1)])
+def test_windows_of_three_dimensions(T, wh, ww, hd, dtype):
+    """The most displacements that 192 tokens can have, 7 x 11 x 15, in any order of the dimensions: the largest tables."""
+    nh = 2
+    qkv, qw, kw, table, geom, dout = inputs(1, T, 2, 2, wh, ww, nh, hd, dtype, True, seed=T)
+    out, grads = call(qkv, qw, kw, table, geom, nh, hd, dout)
+    want = definition(qkv, qw, kw, table, geom, nh, hd, dout)
+    u, c = U[dtype], nh * hd
+    assert rel(out, want["out"]) < 6 * u
+    for part in (slice(0, c), slice(c, 2 * c), slice(2 * c, 3 * c)):
+        assert rel(grads[0][..., part], want["grads"][0][..., part]) < 10 * u
+    assert all(rel(a, b) < 24 * u for a, b in zip(grads[1:], want["grads"][1:]))
+
+
 # ------------------------------------------------------------------------------------------------ calls
 @pytest.mark.parametrize("bias", [True, False])
 @pytest.mark.parametrize("dtype,hd", [(BF, 16), (BF, 64), (BF, 128), (HF, 32), (HF, 128)])
